@@ -1,0 +1,180 @@
+"""A paged key/value cache: ``paged_cache``, ``cache_write``, ``cache_read`` and ``cache_attention``.
+
+A cache is a tuple of tensors: keys and values [pages, heads, page, D] in float16 or bfloat16, or in float8_e4m3fn with two more
+tensors of uint8 [pages, heads, page], the exponents of keys and values; a value is then code * 2 ** (exponent - 127).
+
+A call works on packed rows, the new tokens of a batch one sequence behind the other: rows ``starts[b]`` .. ``starts[b + 1] - 1``
+belong to sequence b and sit behind the ``lengths[b]`` keys it has already, so row ``starts[b] + i`` has position ``lengths[b] + i``.
+``table[b, i]`` is the page of positions ``i * page`` .. of sequence b.  The three are int32 tensors on the device, so that a captured
+step can be replayed with other contents.  Their contents are checked by the kernels: what is out of range is left out, and
+``cache_check`` raises.  Rows before ``starts[0]`` and from ``starts[-1]`` on belong to no sequence and are left as they are.
+"""
+import contextlib
+import math
+
+from . import capi
+from .execute import _stream_ptr, _torch, context_for
+
+_CODES = None
+
+
+def _codes():
+    global _CODES
+    if _CODES is None:
+        torch = _torch()
+        _CODES = {torch.float16: capi.F16, torch.bfloat16: capi.BF16, torch.float8_e4m3fn: capi.E4M3}
+    return _CODES
+
+
+def _on_stream(stream, device):
+    """What is allocated in it belongs to the stream the kernels run on."""
+    if stream is None:
+        return contextlib.nullcontext()
+    torch = _torch()
+    return torch.cuda.stream(stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream), device=device))
+
+
+def paged_cache(pages, heads, page, d, dtype, device="cuda"):
+    """A new cache of ``pages`` pages of ``page`` tokens (a power of two from 16 to 1024) with heads of 64 or 128 elements."""
+    torch = _torch()
+    if dtype not in _codes():
+        raise ValueError("frisk-b200-cache: a cache holds float16, bfloat16 or float8_e4m3fn")
+    if pages < 1 or heads < 1 or page < 16 or page > 1024 or page & (page - 1) or d not in (64, 128):
+        raise ValueError("frisk-b200-cache: sizes outside the contract")
+    held = tuple(torch.zeros(pages, heads, page, d, dtype=dtype, device=device) for _ in range(2))
+    if dtype != torch.float8_e4m3fn:
+        return held
+    return held + tuple(torch.zeros(pages, heads, page, dtype=torch.uint8, device=device) for _ in range(2))
+
+
+def _describe(cache, table, starts, lengths, rows):
+    """(descriptor, element code, device index, key heads, D), checked."""
+    torch = _torch()
+    if len(cache) not in (2, 4):
+        raise ValueError("frisk-b200-cache: a cache is (k, v), or (k, v, k exponents, v exponents)")
+    k, v = cache[0], cache[1]
+    code, shape, dev = _codes().get(k.dtype), k.shape, k.get_device()
+    if code is None or (code == capi.E4M3) != (len(cache) == 4):
+        raise ValueError("frisk-b200-cache: a cache holds float16, bfloat16, or float8_e4m3fn with exponents")
+    if len(shape) != 4 or v.shape != shape or v.dtype != k.dtype or not k.is_contiguous() or not v.is_contiguous():
+        raise ValueError("frisk-b200-cache: keys and values must be dense [pages, heads, page, D] of one type")
+    if dev < 0 or v.get_device() != dev:
+        raise ValueError("frisk-b200-cache: tensors must be on one CUDA device (there is no CPU path)")
+    exponents = (None, None)
+    if code == capi.E4M3:
+        for e in cache[2:]:
+            if e.dtype != torch.uint8 or e.shape != shape[:3] or not e.is_contiguous() or e.get_device() != dev:
+                raise ValueError("frisk-b200-cache: exponents must be dense uint8 [pages, heads, page] on the cache's device")
+        exponents = cache[2].data_ptr(), cache[3].data_ptr()
+    batch = lengths.shape[0] if len(lengths.shape) == 1 else -1
+    i32 = torch.int32
+    if batch < 0 or starts.shape != (batch + 1,) or len(table.shape) != 2 or table.shape[0] != batch or \
+            starts.dtype != i32 or lengths.dtype != i32 or table.dtype != i32:
+        raise ValueError("frisk-b200-cache: table, starts and lengths must be int32 [batch, width], [batch + 1] and [batch]")
+    if not starts.is_contiguous() or not lengths.is_contiguous() or (table.stride(1) != 1 and table.shape[1] > 1):
+        raise ValueError("frisk-b200-cache: starts, lengths and the rows of the table must be dense")
+    if starts.get_device() != dev or lengths.get_device() != dev or table.get_device() != dev:
+        raise ValueError("frisk-b200-cache: table, starts and lengths must be on the cache's device")
+    pages, heads, page, d = shape
+    desc = capi.CacheDesc(pages, page, heads, d, code, batch, table.shape[1], table.stride(0), rows, k.data_ptr(), v.data_ptr(),
+                          *exponents, table.data_ptr(), starts.data_ptr(), lengths.data_ptr())
+    return desc, code, dev, heads, d
+
+
+def _packed(t, heads, d, dev, what):
+    shape, s = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != heads or shape[2] != d or s[2] != 1 or t.get_device() != dev:
+        raise ValueError(f"frisk-b200-cache: {what} must be [rows, {heads}, {d}] on the cache's device, the elements of a head neighbours")
+    return capi.Packed(t.data_ptr(), s[0], s[1])
+
+
+def cache_write(cache, k, v, table, starts, lengths, *, stream=None):
+    """Writes the packed rows ``k`` and ``v`` [rows, heads, D] (float16 or bfloat16, each row and head on 16 bytes) to their positions.
+    A 16-bit cache takes its own type.  A float8_e4m3fn cache is quantised as it is written: the scale of a token's head is the least
+    power of two that brings its largest magnitude to 448 or less, codes are rounded to the nearest, ties to even; a row that holds an
+    infinity or a NaN reads back as NaN.  A position must not be that of two rows (a page that two sequences name)."""
+    desc, code, dev, heads, d = _describe(cache, table, starts, lengths, k.shape[0])
+    given = _codes().get(k.dtype)
+    if given is None or given == capi.E4M3 or v.dtype != k.dtype or v.shape != k.shape or (code != capi.E4M3 and code != given):
+        raise ValueError("frisk-b200-cache: keys and values must be float16 or bfloat16 rows of one shape, in the type of a 16-bit cache")
+    pk, pv = _packed(k, heads, d, dev, "keys"), _packed(v, heads, d, dev, "values")
+    context_for(dev).cache_write(desc, given, pk, pv, stream=_stream_ptr(stream, k.device))
+    return cache
+
+
+def cache_read(cache, table, starts, lengths, rows, *, dtype=None, out=None, stream=None):
+    """The packed (keys, values) [rows, heads, D] at the positions of the packed rows, in ``dtype`` (float16 or bfloat16; a 16-bit cache
+    gives its own).  ``lengths`` of zero read sequences from their first key on.  ``out``: a pair of tensors for them; in new ones, rows
+    that belong to no sequence are undefined.  8-bit values beyond the type's range become its largest finite ones."""
+    torch = _torch()
+    desc, code, dev, heads, d = _describe(cache, table, starts, lengths, rows)
+    if dtype is None:
+        dtype = out[0].dtype if out is not None else torch.bfloat16 if code == capi.E4M3 else cache[0].dtype
+    given = _codes().get(dtype)
+    if given is None or given == capi.E4M3 or (code != capi.E4M3 and code != given):
+        raise ValueError("frisk-b200-cache: rows are read as float16 or bfloat16, from a 16-bit cache in its own type")
+    if out is None:
+        device = cache[0].device
+        with _on_stream(stream, device):
+            out = tuple(torch.empty(rows, heads, d, dtype=dtype, device=device) for _ in range(2))
+    elif len(out) != 2 or any(t.dtype != dtype or t.shape[0] != rows for t in out):
+        raise ValueError("frisk-b200-cache: out must be two tensors of the rows' type and count")
+    pk, pv = _packed(out[0], heads, d, dev, "keys"), _packed(out[1], heads, d, dev, "values")
+    context_for(dev).cache_read(desc, given, pk, pv, stream=_stream_ptr(stream, cache[0].device))
+    return tuple(out)
+
+
+def cache_attention(cache, q, table, starts, lengths, *, mask=None, scale=None, max_new=0, out=None, stream=None):
+    """Attention of the packed query rows ``q`` [rows, query heads, D] (float16 or bfloat16; a 16-bit cache has their type) over the
+    cache, which holds their own keys and values already (``cache_write``).  A row sees the ``lengths[b]`` keys before the new tokens
+    of its sequence and, of the new tokens, those up to itself, or those j for which ``mask[row, j]`` is set: ``mask`` is bool
+    [rows, width], j counts within the sequence, and what lies beyond the width is not seen.  A single token is a tree of one.  Query
+    head h reads key head h // (query heads / key heads).  A row that sees no key is zero; what a row does not see does not reach it,
+    whatever it holds.  ``scale`` is 1 / sqrt(D) if not given.  ``max_new``, the largest number of new tokens of a sequence, helps the
+    choice of a kernel and changes no result's meaning.  Rows of a new ``out`` that belong to no sequence are undefined."""
+    torch = _torch()
+    rows = q.shape[0]
+    desc, code, dev, heads, d = _describe(cache, table, starts, lengths, rows)
+    given = _codes().get(q.dtype)
+    if given is None or given == capi.E4M3 or (code != capi.E4M3 and code != given):
+        raise ValueError("frisk-b200-cache: queries must be float16 or bfloat16, in the type of a 16-bit cache")
+    heads_q = q.shape[1] if len(q.shape) == 3 else 0
+    if heads_q < 1 or heads_q % heads:
+        raise ValueError("frisk-b200-cache: queries must be [rows, query heads, D], query heads a multiple of the key heads")
+    device = q.device
+    width = step = 0
+    mask_ptr = None
+    if mask is not None:
+        if mask.dtype != torch.bool or len(mask.shape) != 2 or mask.shape[0] != rows or (mask.stride(1) != 1 and mask.shape[1] > 1) or \
+                mask.get_device() != dev:
+            raise ValueError("frisk-b200-cache: the mask must be bool [rows, width] on the cache's device, its rows dense")
+        width, step = mask.shape[1], mask.stride(0)
+        mask_ptr = mask.data_ptr()
+        if width == 0:  # (an empty tensor has no address; none of the new tokens is seen)
+            mask_ptr = starts.data_ptr()
+    pq = _packed(q, heads_q, d, dev, "queries")
+    adesc = capi.CacheAttnDesc(heads_q, given, max_new, width, step, 1.0 / math.sqrt(d) if scale is None else scale)
+    nbytes = capi.cache_attention_workspace_bytes(desc, adesc)
+    if out is not None and (out.dtype != q.dtype or out.shape != q.shape):
+        raise ValueError("frisk-b200-cache: out must have the type and shape of the queries")
+    if stream is None:
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    else:
+        with _on_stream(stream, device):
+            if out is None:
+                out = torch.empty(q.shape, dtype=q.dtype, device=device)
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    po = _packed(out, heads_q, d, dev, "results")
+    context_for(dev).cache_attention(desc, adesc, pq, po, mask_ptr, workspace.data_ptr(), nbytes, stream=_stream_ptr(stream, device))
+    return out
+
+
+def cache_check(device=None, *, stream=None):
+    """Waits for the stream and raises RuntimeError where a kernel on it met a table entry out of range or gave up a wait."""
+    torch = _torch()
+    device = torch.device("cuda" if device is None else device)
+    index = torch.cuda.current_device() if device.index is None else device.index
+    with torch.cuda.device(index):
+        context_for(index).check(_stream_ptr(stream, torch.device("cuda", index)))

@@ -11,6 +11,7 @@ import os
 import pathlib
 
 F32, F16, BF16 = 0, 1, 2
+E4M3 = 3  # element type of a paged cache only
 ALGO_AUTO, ALGO_SIMT_F32, ALGO_TCGEN05, ALGO_SKINNY, ALGO_TCGEN05_PAIR, ALGO_F32_SPLIT = 0, 1, 2, 3, 4, 5
 ATTN_PAIRS, ATTN_SPLIT_KEYS, ATTN_TWO_HEADS, ATTN_FEW_QUERIES = 0, 1, 2, 3
 DTYPE_CODE = {"fp32": F32, "fp16": F16, "bf16": BF16}
@@ -30,6 +31,8 @@ EXPORTS = (
     "frisk_b200_peer_buffer_create", "frisk_b200_peer_buffer_open", "frisk_b200_peer_buffer_close",
     "frisk_b200_gemm_fused_select", "frisk_b200_gemm_fused_workspace_bytes", "frisk_b200_gemm_fused",
     "frisk_b200_gemm_plan", "frisk_b200_attention_form",
+    "frisk_b200_rotary", "frisk_b200_cache_write", "frisk_b200_cache_read", "frisk_b200_cache_attention",
+    "frisk_b200_cache_attention_workspace_bytes",
 )
 
 
@@ -75,6 +78,30 @@ class AttnDesc(ctypes.Structure):
                 ("dtype_in", ctypes.c_int32), ("dtype_out", ctypes.c_int32), ("normalize_p", ctypes.c_int32)]
 
 
+class Packed(ctypes.Structure):
+    """Packed rows [rows, heads, D]: address and strides in elements."""
+    _fields_ = [("ptr", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("heads_q", ctypes.c_int32), ("heads_k", ctypes.c_int32), ("D", ctypes.c_int32),
+                ("dim", ctypes.c_int32), ("dtype", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("inverse", ctypes.c_int32), ("positions64", ctypes.c_int32), ("amplitude", ctypes.c_float)]
+
+
+class CacheDesc(ctypes.Structure):
+    _fields_ = [("pages", ctypes.c_int64), ("page", ctypes.c_int32), ("heads", ctypes.c_int32), ("D", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("batch", ctypes.c_int32), ("table_width", ctypes.c_int32),
+                ("table_stride", ctypes.c_int64), ("rows", ctypes.c_int64), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_exponent", ctypes.c_void_p), ("v_exponent", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("starts", ctypes.c_void_p), ("lengths", ctypes.c_void_p)]
+
+
+class CacheAttnDesc(ctypes.Structure):
+    _fields_ = [("heads_q", ctypes.c_int32), ("dtype", ctypes.c_int32), ("max_new", ctypes.c_int32),
+                ("mask_width", ctypes.c_int32), ("mask_stride", ctypes.c_int64), ("scale", ctypes.c_float)]
+
+
 _lib = None
 
 
@@ -91,6 +118,7 @@ def load():
     lib = ctypes.CDLL(os.fspath(path))
     vp, sz, i32, i64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int32, ctypes.c_int64
     gd, ad, ge = ctypes.POINTER(GemmDesc), ctypes.POINTER(AttnDesc), ctypes.POINTER(GemmEpilogue)
+    pk, cd, ca = ctypes.POINTER(Packed), ctypes.POINTER(CacheDesc), ctypes.POINTER(CacheAttnDesc)
     sig = {
         "frisk_b200_ctx_create": (ctypes.c_int, [ctypes.POINTER(vp), ctypes.c_int]),
         "frisk_b200_ctx_destroy": (ctypes.c_int, [vp]),
@@ -123,6 +151,11 @@ def load():
         "frisk_b200_gemm_fused_workspace_bytes": (sz, [gd, ge]),
         "frisk_b200_gemm_fused": (ctypes.c_int, [vp, gd, ge, vp, vp, vp, vp, sz, vp]),
         "frisk_b200_gemm_plan": (ctypes.c_int, [vp, gd, vp, ctypes.POINTER(GemmPlanInfo)]),
+        "frisk_b200_rotary": (ctypes.c_int, [vp, ctypes.POINTER(RotaryDesc), vp, vp, pk, pk, pk, pk, vp]),
+        "frisk_b200_cache_write": (ctypes.c_int, [vp, cd, i32, pk, pk, vp]),
+        "frisk_b200_cache_read": (ctypes.c_int, [vp, cd, i32, pk, pk, vp]),
+        "frisk_b200_cache_attention": (ctypes.c_int, [vp, cd, ca, pk, pk, vp, vp, sz, vp]),
+        "frisk_b200_cache_attention_workspace_bytes": (sz, [cd, ca]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -252,6 +285,21 @@ class Context:
     def peer_buffer_close(self, ptr, owned):
         raise_for(load().frisk_b200_peer_buffer_close(self.handle, ptr, int(bool(owned))), self._h)
 
+    def rotary(self, desc, positions, frequencies, q, k, q_out, k_out, stream=None):
+        """``q``, ``k`` and their outputs: ``Packed``; ``k`` and ``k_out`` None where the descriptor has no key heads."""
+        rc = load().frisk_b200_rotary(self.handle, desc, positions, frequencies, q, k, q_out, k_out, stream)
+        raise_for(rc, self._h)
+
+    def cache_write(self, cache, dtype, k, v, stream=None):
+        raise_for(load().frisk_b200_cache_write(self.handle, cache, dtype, k, v, stream), self._h)
+
+    def cache_read(self, cache, dtype, k, v, stream=None):
+        raise_for(load().frisk_b200_cache_read(self.handle, cache, dtype, k, v, stream), self._h)
+
+    def cache_attention(self, cache, desc, q, out, mask, ws_ptr, ws_bytes, stream=None):
+        rc = load().frisk_b200_cache_attention(self.handle, cache, desc, q, out, mask, ws_ptr, ws_bytes, stream)
+        raise_for(rc, self._h)
+
     def check(self, stream=None):
         raise_for(load().frisk_b200_check(self.handle, stream), self._h)
 
@@ -266,6 +314,11 @@ def gemm_fused_select(desc, epi):
 
 def gemm_fused_workspace_bytes(desc, epi):
     return load().frisk_b200_gemm_fused_workspace_bytes(ctypes.byref(desc), ctypes.byref(epi))
+
+
+def cache_attention_workspace_bytes(cache, desc):
+    """Bytes ``Context.cache_attention`` needs; 0 for what it refuses.  Host-only."""
+    return load().frisk_b200_cache_attention_workspace_bytes(cache, desc)
 
 
 _PAIR = ctypes.c_int64 * 2

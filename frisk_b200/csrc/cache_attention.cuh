@@ -1,0 +1,207 @@
+// What the kernels of attention over a paged cache share: parameters, how the work is dealt to CTAs, which keys a row sees, how a
+// row's results leave.
+#pragma once
+#include "attention_common.cuh"
+#include "cache_common.cuh"
+#include "work_split.cuh"
+
+namespace fb {
+
+int cache_validate(const frisk_b200_cache_desc* c);
+int cache_pointers(const frisk_b200_cache_desc* c);
+cache::Tables cache_tables(const frisk_b200_cache_desc* c);
+bool cache_overlaps(const frisk_b200_cache_desc* c, const void* ptr, size_t bytes);
+bool tables_overlap(const frisk_b200_cache_desc* c, const void* ptr, size_t bytes);
+size_t packed_span(const frisk_b200_packed& x, int64_t rows, int heads, int D, size_t es);
+
+namespace cache {
+
+// An item (the rows of a tile, one key head, all keys) that the CTA of this index began and later ones finished; rows = 0: none.
+struct ItemRecord {
+  int rows, parts, first_slot;  // its query rows, the CTAs that hold a part, which of the first one's two slots
+  int first_row, head, row0;    // the sequence's first packed row, the key head, the first row of the tile
+  int pad[2];
+};
+constexpr size_t kRecordBytes = (kNumSMsDefault * sizeof(ItemRecord) + 255) / 256 * 256;
+// a part: O [rows][D], reference maxima [rows], sums [rows]
+__host__ __device__ constexpr size_t partial_floats(int rows, int D) { return (size_t)rows * D + 2 * rows; }
+
+struct CacheAttnParams {
+  Tables t;
+  const void* q;
+  void* out;
+  int64_t q_row, q_head, out_row, out_head;
+  const uint8_t *k_exponent, *v_exponent;
+  const uint8_t* mask;
+  int64_t mask_stride;
+  int mask_width, group;
+  float scale_log2;
+  ItemRecord* records;
+  float* partials;
+  unsigned* status;
+};
+
+constexpr int kTileKeys = 64;
+
+__device__ __forceinline__ int key_tiles(const Seq& s) { return (s.length + s.count + kTileKeys - 1) / kTileKeys; }
+__device__ __forceinline__ int row_tiles(const CacheAttnParams& p, const Seq& s, int tile_rows) {
+  return (s.count * p.group + tile_rows - 1) / tile_rows;
+}
+__device__ __forceinline__ unsigned units_of(const CacheAttnParams& p, const Seq& s, int tile_rows) {
+  return (unsigned)p.t.heads * (unsigned)row_tiles(p, s, tile_rows) * (unsigned)key_tiles(s);
+}
+
+struct PlanShared {
+  unsigned warp_sum[32];
+  unsigned first_b, first_off;
+};
+struct Plan {
+  unsigned begin, end;  // this CTA's units
+  int b;                // the sequence that holds the first of them
+  unsigned off;         // and its index there
+};
+
+// The units of all sequences, summed up by the whole CTA; its range of them; the record of the item it shares with the CTAs behind it.
+template <int THREADS>
+__device__ __forceinline__ Plan make_plan(const CacheAttnParams& p, int tile_rows, PlanShared* sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunk = (p.t.batch + THREADS - 1) / THREADS;
+  const int b_lo = min((int)threadIdx.x * chunk, p.t.batch), b_hi = min(b_lo + chunk, p.t.batch);
+  unsigned mine = 0;
+  for (int b = b_lo; b < b_hi; ++b) mine += units_of(p, load_seq(p.t, b, p.status), tile_rows);
+  unsigned upto = mine;  // of the warp's threads up to this one
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned other = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += other;
+  }
+  if (lane == 31) sh->warp_sum[warp] = upto;
+  __syncthreads();
+  unsigned before = upto - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    const unsigned n = sh->warp_sum[w];
+    before += w < warp ? n : 0;
+    total += n;
+  }
+  const WorkSplit work{total / gridDim.x, total % gridDim.x};
+  Plan plan;
+  plan.begin = work.start(blockIdx.x);
+  plan.end = work.start(blockIdx.x + 1);
+  auto holds = [&](unsigned u) { return before <= u && u - before < mine; };
+  if (plan.begin < plan.end) {
+    if (holds(plan.begin)) {
+      unsigned at = before;
+      for (int b = b_lo; b < b_hi; ++b) {
+        const unsigned n = units_of(p, load_seq(p.t, b, p.status), tile_rows);
+        if (plan.begin - at < n) {
+          sh->first_b = (unsigned)b;
+          sh->first_off = plan.begin - at;
+          break;
+        }
+        at += n;
+      }
+    }
+    if (holds(plan.end - 1)) {
+      unsigned at = before;
+      for (int b = b_lo; b < b_hi; ++b) {
+        const Seq s = load_seq(p.t, b, p.status);
+        const unsigned n = units_of(p, s, tile_rows);
+        if (plan.end - 1 - at < n) {
+          const unsigned kt = (unsigned)key_tiles(s), item = (plan.end - 1 - at) / kt;
+          const unsigned from = at + item * kt, to = from + kt;
+          ItemRecord r{};
+          if (to > plan.end && from >= plan.begin) {
+            const int rt = row_tiles(p, s, tile_rows), h = (int)item / rt;
+            r.row0 = ((int)item - h * rt) * tile_rows;
+            r.rows = min(tile_rows, s.count * p.group - r.row0);
+            r.parts = (int)(work.worker_of(to - 1) - blockIdx.x) + 1;
+            r.first_slot = from == plan.begin ? 0 : 1;
+            r.first_row = s.first;
+            r.head = h;
+          }
+          p.records[blockIdx.x] = r;
+          break;
+        }
+        at += n;
+      }
+    }
+  } else if (threadIdx.x == 0) {
+    p.records[blockIdx.x] = ItemRecord{};
+  }
+  __syncthreads();
+  plan.b = (int)sh->first_b;
+  plan.off = sh->first_off;
+  return plan;
+}
+
+// Walks a CTA's items.
+struct Cursor {
+  int b, h, rt, tile, kt, n_rt;
+  unsigned left;
+  bool first_item;
+  Seq seq;
+  __device__ __forceinline__ void enter(const CacheAttnParams& p, int tile_rows) {
+    seq = load_seq(p.t, b, p.status);
+    kt = key_tiles(seq);
+    n_rt = row_tiles(p, seq, tile_rows);
+  }
+  __device__ __forceinline__ Cursor(const CacheAttnParams& p, const Plan& plan, int tile_rows) : left(plan.end - plan.begin), first_item(true) {
+    if (left == 0) return;
+    b = plan.b;
+    enter(p, tile_rows);
+    const int item = (int)(plan.off / (unsigned)kt);
+    tile = (int)(plan.off - (unsigned)item * (unsigned)kt);
+    h = item / n_rt;
+    rt = item - h * n_rt;
+  }
+  __device__ __forceinline__ int tiles_here() const { return (int)min((unsigned)(kt - tile), left); }
+  __device__ __forceinline__ void next_item(const CacheAttnParams& p, int tile_rows) {
+    left -= (unsigned)tiles_here();
+    first_item = false;
+    tile = 0;
+    if (left == 0 || ++rt < n_rt) return;
+    rt = 0;
+    if (++h < p.t.heads) return;
+    h = 0;
+    do {
+      if (++b >= p.t.batch) {
+        left = 0;
+        return;
+      }
+      enter(p, tile_rows);
+    } while (n_rt == 0);
+  }
+};
+
+// whether new token i of the sequence sees key length + ahead
+__device__ __forceinline__ bool sees(const CacheAttnParams& p, const Seq& s, int i, int ahead) {
+  if (ahead < 0) return true;
+  if (ahead >= s.count) return false;
+  if (!p.mask) return ahead <= i;
+  return ahead < p.mask_width && __ldg(p.mask + (int64_t)(s.first + i) * p.mask_stride + ahead) != 0;
+}
+
+// four results of row r (of the sequence and key head), acc / l; a row that saw nothing is zero
+template <bool QBF16, bool E4M3>
+__device__ __forceinline__ void store_row4(const CacheAttnParams& p, int first, int h, int r, int c4, float4 acc, float l) {
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  float x[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  if (E4M3) {  // values near the end of the type's range may have been rounded beyond it
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = saturated<QBF16>(x[i]);
+  }
+  const int i = r / p.group;
+  uint16_t* out = static_cast<uint16_t*>(p.out) + (int64_t)(first + i) * p.out_row + (int64_t)(h * p.group + r - i * p.group) * p.out_head;
+  *reinterpret_cast<uint2*>(out + c4 * 4) = make_uint2(attn::pack16<QBF16>(x[0], x[1]), attn::pack16<QBF16>(x[2], x[3]));
+}
+
+// `bytes` (a multiple of 16) from global to shared memory
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+}  // namespace cache
+}  // namespace fb

@@ -1,0 +1,285 @@
+// Writing new rows into the paged cache, quantised on the way where it holds 8-bit floats, and reading rows back.
+//
+// A head's row is D elements: 16 bytes of the 16-bit side a lane, D / 8 neighbouring lanes a row, so the largest magnitude of a row
+// takes three or four shuffles and nothing passes through shared memory.  Bound by HBM: each side is read or written once.  A block
+// takes one packed row at a time, its keys and values, and finds the row's place (its sequence by bisection of `starts`, then the
+// page) while the row itself is on its way; few rows are few blocks, and the chain starts -> lengths -> table is what a call costs then.
+#include <algorithm>
+
+#include "cache_common.cuh"
+
+namespace fb {
+namespace {
+using namespace cache;
+
+constexpr int kThreads = 256;
+
+struct Side {  // packed rows outside the cache, 16-bit
+  void* ptr;
+  int64_t row, head;
+};
+struct RowsParams {
+  Tables t;
+  Side k, v;
+  void *ck, *cv;           // pages
+  uint8_t *ek, *ev;        // exponents
+  int64_t rows;
+  unsigned* status;
+};
+
+// The index of packed row r among the cache's token slots of head 0, (page * heads) * P + offset; -1: it has none.
+__device__ __forceinline__ int64_t locate(const Tables& t, int64_t r, unsigned* status) {
+  // the last b with starts[b] <= r; where starts does not ascend, some b that does not hold r
+  int lo = 0, hi = t.batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(t.starts + mid) <= r) lo = mid; else hi = mid;
+  }
+  const Seq s = load_seq(t, lo, status);
+  const int64_t i = r - s.first;
+  if (!s.ok || i < 0 || i >= s.count) return -1;  // (rows before the first sequence and behind the last belong to none)
+  const int64_t pos = s.length + i;
+  const int page = __ldg(t.table + lo * t.stride + (pos >> t.page_log2));
+  if (page < 0 || page >= t.pages) {
+    atomicCAS(status, 0u, ST_CACHE_PAGE);
+    return -1;
+  }
+  return ((int64_t)page * t.heads << t.page_log2) + (pos & (t.page - 1));
+}
+
+template <bool BF16>
+__device__ __forceinline__ float2 unpack16(uint32_t w) {
+  if (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <bool BF16, int D, bool E4M3, bool WRITE>
+__global__ void __launch_bounds__(kThreads) cache_rows_kernel(const RowsParams p) {
+  constexpr int kLanes = D / 8;  // of a row
+  const int sub = threadIdx.x % kLanes;
+  const int units = 2 * p.t.heads;  // K and V rows of a token
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    // (whole groups of kLanes threads take the same unit, and whole warps the same number of rounds: the shuffles below need them)
+    for (int u0 = 0; u0 < units; u0 += kThreads / kLanes) {
+      const int u = u0 + threadIdx.x / kLanes;
+      const bool mine = u < units;
+      const bool values = u >= p.t.heads;
+      const int h = values ? u - p.t.heads : u;
+      const Side& side = values ? p.v : p.k;
+      uint4* packed = reinterpret_cast<uint4*>(static_cast<uint16_t*>(side.ptr) + r * side.row + h * side.head) + sub;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (WRITE && mine) x = __ldg(packed);
+      const int64_t base = locate(p.t, r, p.status);
+      if (base < 0) continue;  // (the same for the whole block)
+      const int64_t token = base + ((int64_t)h << p.t.page_log2);
+      void* pages = values ? p.cv : p.ck;
+      uint8_t* exponents = values ? p.ev : p.ek;
+      if (!E4M3) {
+        uint4* held = reinterpret_cast<uint4*>(static_cast<uint16_t*>(pages) + token * D) + sub;
+        if (mine) {
+          if (WRITE) *held = x; else *packed = __ldg(held);
+        }
+      } else if (WRITE) {
+        float f[8];
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        uint32_t most = 0;  // magnitudes compare as integers; infinities and NaN are the largest
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 two = unpack16<BF16>(w[i]);
+          f[2 * i] = two.x;
+          f[2 * i + 1] = two.y;
+          most = max(most, max(__float_as_uint(two.x) & 0x7fffffffu, __float_as_uint(two.y) & 0x7fffffffu));
+        }
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        // most = 1.m * 2^(E - 127) and 448 = 1.75 * 2^8: the least e with most <= 448 * 2^(e - 127)
+        int e = (int)(most >> 23) - 8 + ((most & 0x7fffffu) > 0x600000u ? 1 : 0);
+        e = most >= 0x7f800000u ? 255 : max(e, 1);
+        if (mine) {
+          uint32_t code[2] = {0, 0};
+          if (e != 255) {
+            const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              code[i >> 1] |= (uint32_t)float2_to_e4m3x2(f[2 * i] * inv, f[2 * i + 1] * inv) << (16 * (i & 1));
+          }
+          reinterpret_cast<uint2*>(static_cast<uint8_t*>(pages) + token * D)[sub] = make_uint2(code[0], code[1]);
+          if (sub == 0) exponents[token] = (uint8_t)e;
+        }
+      } else if (mine) {
+        const uint2 code = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pages) + token * D) + sub);
+        const float scale = scale_of(__ldg(exponents + token));
+        const uint32_t c[2] = {code.x, code.y};
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t h2 = i & 1 ? e4m3x2_to_half2_hi(c[i >> 1]) : e4m3x2_to_half2(c[i >> 1]);
+          float2 two = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+          two.x *= scale;
+          two.y *= scale;
+          // a row near the end of the type's range may have been rounded beyond it
+          two.x = saturated<BF16>(two.x);
+          two.y = saturated<BF16>(two.y);
+          o[i] = pack16<BF16>(two.x, two.y);
+        }
+        *packed = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
+  }
+}
+
+template <bool BF16, int D, bool E4M3, bool WRITE>
+cudaError_t launch(const frisk_b200_ctx* ctx, const RowsParams& p, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel waits (griddepcontrol.wait) itself
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(p.rows, (int64_t)ctx->num_sms * 8));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, cache_rows_kernel<BF16, D, E4M3, WRITE>, p);
+}
+template <bool WRITE>
+cudaError_t launch_any(const frisk_b200_ctx* ctx, const RowsParams& p, bool bf16, int D, bool e4m3, cudaStream_t s) {
+  if (D == 64)
+    return bf16 ? (e4m3 ? launch<true, 64, true, WRITE>(ctx, p, s) : launch<true, 64, false, WRITE>(ctx, p, s))
+                : (e4m3 ? launch<false, 64, true, WRITE>(ctx, p, s) : launch<false, 64, false, WRITE>(ctx, p, s));
+  return bf16 ? (e4m3 ? launch<true, 128, true, WRITE>(ctx, p, s) : launch<true, 128, false, WRITE>(ctx, p, s))
+              : (e4m3 ? launch<false, 128, true, WRITE>(ctx, p, s) : launch<false, 128, false, WRITE>(ctx, p, s));
+}
+
+}  // namespace
+}  // namespace fb
+
+using namespace fb;
+
+namespace fb {
+
+int cache_validate(const frisk_b200_cache_desc* c) {
+  if (!c) return FRISK_B200_E_ARG;
+  if (c->dtype != FRISK_B200_F16 && c->dtype != FRISK_B200_BF16 && c->dtype != FRISK_B200_E4M3) return FRISK_B200_E_CACHE_TYPE;
+  if (c->pages < 1 || c->page < 16 || c->page > 1024 || (c->page & (c->page - 1)) || c->heads < 1 || c->heads > 4096 ||
+      (c->D != 64 && c->D != 128) || c->batch < 0 || c->table_width < 0 || c->rows < 0 || c->rows > INT32_MAX ||
+      (c->batch > 1 && c->table_stride < c->table_width) || c->pages * c->heads > (INT32_MAX / c->page))
+    return FRISK_B200_E_CACHE_SHAPE;
+  return 0;
+}
+
+// pointers of a cache that a call is going to use
+int cache_pointers(const frisk_b200_cache_desc* c) {
+  if (!c->k || !c->v || !c->starts || !c->lengths || (!c->table && c->table_width > 0)) return FRISK_B200_E_ARG;
+  if (c->dtype == FRISK_B200_E4M3 && (!c->k_exponent || !c->v_exponent)) return FRISK_B200_E_ARG;
+  const uintptr_t all = reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) |
+                        (c->dtype == FRISK_B200_E4M3 ? reinterpret_cast<uintptr_t>(c->k_exponent) | reinterpret_cast<uintptr_t>(c->v_exponent) : 0);
+  if (all & 15u) return FRISK_B200_E_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(c->starts) | reinterpret_cast<uintptr_t>(c->lengths) | reinterpret_cast<uintptr_t>(c->table)) & 3u)
+    return FRISK_B200_E_ALIGN;
+  return 0;
+}
+
+cache::Tables cache_tables(const frisk_b200_cache_desc* c) {
+  cache::Tables t{};
+  t.table = c->table;
+  t.starts = c->starts;
+  t.lengths = c->lengths;
+  t.stride = c->table_stride;
+  t.batch = c->batch;
+  t.width = c->table_width;
+  t.rows = c->rows;
+  t.pages = c->pages;
+  t.page = c->page;
+  t.heads = c->heads;
+  while ((1 << t.page_log2) < c->page) ++t.page_log2;
+  return t;
+}
+
+// bytes of the cache's tensors, which outputs must not overlap
+bool cache_overlaps(const frisk_b200_cache_desc* c, const void* ptr, size_t bytes) {
+  const size_t tokens = (size_t)c->pages * c->heads * c->page, held = tokens * c->D * (c->dtype == FRISK_B200_E4M3 ? 1 : 2);
+  return ranges_overlap(ptr, bytes, c->k, held) || ranges_overlap(ptr, bytes, c->v, held) ||
+         (c->dtype == FRISK_B200_E4M3 &&
+          (ranges_overlap(ptr, bytes, c->k_exponent, tokens) || ranges_overlap(ptr, bytes, c->v_exponent, tokens)));
+}
+bool tables_overlap(const frisk_b200_cache_desc* c, const void* ptr, size_t bytes) {
+  return ranges_overlap(ptr, bytes, c->starts, ((size_t)c->batch + 1) * 4) || ranges_overlap(ptr, bytes, c->lengths, (size_t)c->batch * 4) ||
+         (c->batch > 0 && ranges_overlap(ptr, bytes, c->table, (size_t)((c->batch - 1) * c->table_stride + c->table_width) * 4));
+}
+size_t packed_span(const frisk_b200_packed& x, int64_t rows, int heads, int D, size_t es) {
+  return (size_t)((rows - 1) * x.row_stride + (heads - 1) * x.head_stride + D) * es;
+}
+
+}  // namespace fb
+
+static int check_side(const frisk_b200_packed* x, int heads, int D, int64_t rows, bool written) {
+  if (!x || !x->ptr) return FRISK_B200_E_ARG;
+  if (x->row_stride < 0 || x->head_stride < 0) return FRISK_B200_E_CACHE_SHAPE;
+  if (written && ((heads > 1 && x->head_stride < D) || (rows > 1 && x->row_stride < (heads - 1) * x->head_stride + D)))
+    return FRISK_B200_E_CACHE_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(x->ptr) & 15u) || (rows > 1 && x->row_stride % 8) || (heads > 1 && x->head_stride % 8)) return FRISK_B200_E_ALIGN;
+  return 0;
+}
+
+static int cache_rows(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* c, int32_t dtype, const frisk_b200_packed* k,
+                      const frisk_b200_packed* v, bool write, void* stream) {
+  if (!ctx) return FRISK_B200_E_ARG;
+  int rc = cache_validate(c);
+  if (rc) return rc;
+  if (dtype != FRISK_B200_F16 && dtype != FRISK_B200_BF16) return FRISK_B200_E_CACHE_TYPE;
+  if (c->dtype != FRISK_B200_E4M3 && c->dtype != dtype) return FRISK_B200_E_CACHE_TYPE;
+  if (c->rows == 0 || c->batch == 0) return 0;
+  if ((rc = cache_pointers(c))) return rc;
+  if ((rc = check_side(k, c->heads, c->D, c->rows, !write)) || (rc = check_side(v, c->heads, c->D, c->rows, !write))) return rc;
+  const size_t kb = packed_span(*k, c->rows, c->heads, c->D, 2), vb = packed_span(*v, c->rows, c->heads, c->D, 2);
+  if (cache_overlaps(c, k->ptr, kb) || cache_overlaps(c, v->ptr, vb)) return FRISK_B200_E_OVERLAP;
+  if (!write && (ranges_overlap(k->ptr, kb, v->ptr, vb) || tables_overlap(c, k->ptr, kb) || tables_overlap(c, v->ptr, vb)))
+    return FRISK_B200_E_OVERLAP;
+  if (write) {  // the cache's tensors apart from one another and from the tables
+    const size_t tokens = (size_t)c->pages * c->heads * c->page, held = tokens * c->D * (c->dtype == FRISK_B200_E4M3 ? 1 : 2);
+    struct { const void* p; size_t n; } part[4] = {{c->k, held}, {c->v, held}, {c->k_exponent, tokens}, {c->v_exponent, tokens}};
+    const int n = c->dtype == FRISK_B200_E4M3 ? 4 : 2;
+    for (int i = 0; i < n; ++i) {
+      if (tables_overlap(c, part[i].p, part[i].n)) return FRISK_B200_E_OVERLAP;
+      for (int j = i + 1; j < n; ++j)
+        if (ranges_overlap(part[i].p, part[i].n, part[j].p, part[j].n)) return FRISK_B200_E_OVERLAP;
+    }
+  }
+  RowsParams p{};
+  p.t = cache_tables(c);
+  p.k = Side{k->ptr, k->row_stride, k->head_stride};
+  p.v = Side{v->ptr, v->row_stride, v->head_stride};
+  p.ck = c->k;
+  p.cv = c->v;
+  p.ek = c->k_exponent;
+  p.ev = c->v_exponent;
+  p.rows = c->rows;
+  p.status = ctx->d_status;
+  FB_DEVICE(ctx);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool bf16 = dtype == FRISK_B200_BF16, e4m3 = c->dtype == FRISK_B200_E4M3;
+  FB_CUDA(ctx, write ? launch_any<true>(ctx, p, bf16, c->D, e4m3, s) : launch_any<false>(ctx, p, bf16, c->D, e4m3, s));
+  return 0;
+}
+
+extern "C" {
+int frisk_b200_cache_write(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* c, int32_t dtype, const frisk_b200_packed* k,
+                           const frisk_b200_packed* v, void* stream) {
+  return cache_rows(ctx, c, dtype, k, v, true, stream);
+}
+int frisk_b200_cache_read(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* c, int32_t dtype, const frisk_b200_packed* k,
+                          const frisk_b200_packed* v, void* stream) {
+  return cache_rows(ctx, c, dtype, k, v, false, stream);
+}
+}

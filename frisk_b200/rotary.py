@@ -1,0 +1,113 @@
+"""Rotary positions of queries and keys: ``rotary``, its gradients ``rotary_backward``, and ``rotary_frequencies``.
+
+Packed rows [tokens, heads, D], as a projection leaves them: queries and keys may be columns of one buffer.  The first
+``2 * len(frequencies)`` elements of every head are rotated in pairs, the others pass:
+
+    (a, b) -> amplitude * (a cos t - b sin t, b cos t + a sin t),    t = position * frequency
+"""
+import math
+
+from . import capi
+from .execute import _stream_ptr, _torch, context_for
+from .cache import _on_stream
+
+_CODE = None
+
+
+def rotary_frequencies(dim, base=10000.0, *, scaling=None, factor=1.0, trained=None, low=1.0, high=None, device="cuda"):
+    """(frequencies, amplitude) for ``rotary``: radians per position of the ``dim // 2`` pairs, base ** (-2 i / dim), as a
+    float64 tensor, and the factor on the rotated values.
+
+    ``scaling`` stretches them to contexts ``factor`` times as long as the ``trained`` ones:
+
+    * ``"linear"``      every pair turns ``factor`` times slower
+    * ``"ntk"``         a larger base, with which the slowest pair turns ``factor`` times slower and the fastest stays
+    * ``"wavelength"``  pairs with more than ``high`` (4) turns in the trained context stay, those with fewer than ``low`` turn
+      ``factor`` times slower, the others in between by their number of turns
+    * ``"yarn"``        the same with ``high`` 32, and amplitude 0.1 ln(factor) + 1
+    """
+    if dim < 2 or dim % 2:
+        raise ValueError("frisk-b200-rotary: dim must be even and positive")
+    if scaling not in (None, "linear", "ntk", "wavelength", "yarn"):
+        raise ValueError(f"frisk-b200-rotary: unknown scaling {scaling!r}")
+    if not (base > 0 and factor >= 1.0):
+        raise ValueError("frisk-b200-rotary: base must be positive and factor at least 1")
+    if scaling == "ntk" and dim > 2:
+        base *= factor ** (dim / (dim - 2))
+    freq = [base ** (-2.0 * i / dim) for i in range(dim // 2)]
+    if scaling == "linear" or (scaling == "ntk" and dim == 2):
+        freq = [f / factor for f in freq]
+    elif scaling in ("wavelength", "yarn"):
+        if trained is None or trained <= 0:
+            raise ValueError(f"frisk-b200-rotary: scaling {scaling!r} needs the trained context length")
+        if high is None:
+            high = 32.0 if scaling == "yarn" else 4.0
+        if not high > low:
+            raise ValueError("frisk-b200-rotary: high must be above low")
+        stay = [min(1.0, max(0.0, (trained * f / (2 * math.pi) - low) / (high - low))) for f in freq]
+        freq = [f * (s + (1.0 - s) / factor) for f, s in zip(freq, stay)]
+    amplitude = 0.1 * math.log(factor) + 1.0 if scaling == "yarn" else 1.0
+    return _torch().tensor(freq, dtype=_torch().float64, device=device), amplitude
+
+
+def _rotate(q, k, positions, frequencies, amplitude, interleaved, out, stream, inverse):
+    global _CODE
+    torch = _torch()
+    if _CODE is None:
+        _CODE = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
+    code = _CODE.get(q.dtype)
+    if code is None:
+        raise ValueError("frisk-b200-rotary: elements must be float32, float16 or bfloat16")
+    dev, shape = q.get_device(), q.shape
+    if len(shape) != 3:
+        raise ValueError("frisk-b200-rotary: queries and keys must be [tokens, heads, D]")
+    n, heads_q, d = shape
+    heads_k = 0
+    if out is None:
+        with _on_stream(stream, q.device):
+            out = (torch.empty(shape, dtype=q.dtype, device=q.device), None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device))
+    elif not isinstance(out, (tuple, list)) or len(out) != 2:
+        raise ValueError("frisk-b200-rotary: out must be a pair (None for absent keys)")
+    q_out, k_out = out
+    if (k is None) != (k_out is None) or q_out is None:
+        raise ValueError("frisk-b200-rotary: out must be a pair (None for absent keys)")
+    if k is not None:
+        if k.dtype != q.dtype or k_out.dtype != q.dtype or len(k.shape) != 3 or k.shape[0] != n or k.shape[2] != d or k_out.shape != k.shape:
+            raise ValueError("frisk-b200-rotary: keys must have the queries' type, tokens and D")
+        heads_k = k.shape[1]
+    if q_out.dtype != q.dtype or q_out.shape != shape:
+        raise ValueError("frisk-b200-rotary: results must have the type and shape of what is rotated")
+    if len(positions.shape) != 1 or positions.shape[0] != n or positions.dtype not in (torch.int64, torch.int32) or not positions.is_contiguous():
+        raise ValueError("frisk-b200-rotary: positions must be int32 or int64, one for every token")
+    if len(frequencies.shape) != 1 or frequencies.dtype != torch.float64 or not frequencies.is_contiguous():
+        raise ValueError("frisk-b200-rotary: frequencies must be one float64 for every pair")
+    operands = []
+    for t in (q, k, q_out, k_out):
+        if t is None or (n == 0 or heads_q == 0):
+            operands.append(None)
+            continue
+        s = t.stride()
+        if t.get_device() != dev or s[2] != 1 and d > 1:
+            raise ValueError("frisk-b200-rotary: operands must be on one device, the elements of a head neighbours")
+        operands.append(capi.Packed(t.data_ptr(), s[0], s[1]))
+    if dev < 0 or positions.get_device() != dev or frequencies.get_device() != dev:
+        raise ValueError("frisk-b200-rotary: operands must be on one CUDA device (there is no CPU path)")
+    if n == 0:
+        return q_out, k_out
+    desc = capi.RotaryDesc(n, heads_q, heads_k, d, 2 * frequencies.shape[0], code, interleaved, inverse,
+                           positions.dtype == torch.int64, amplitude)
+    context_for(dev).rotary(desc, positions.data_ptr(), frequencies.data_ptr(), *operands, stream=_stream_ptr(stream, q.device))
+    return q_out, k_out
+
+
+def rotary(q, k, positions, frequencies, *, amplitude=1.0, interleaved=False, out=None, stream=None):
+    """The rotated (queries, keys).  ``q`` [tokens, heads, D] and ``k`` [tokens, key heads, D] (or None) in float32, float16 or
+    bfloat16 with any strides of tokens and heads; ``positions`` int32 or int64 [tokens]; ``frequencies`` float64 [pairs].  Pairs are
+    (i, i + pairs), or (2 i, 2 i + 1) if ``interleaved``.  Angles are reduced to one turn in 64 bits.  ``out`` is a pair of tensors
+    for the results; one may be its input (in place)."""
+    return _rotate(q, k, positions, frequencies, amplitude, interleaved, out, stream, False)
+
+
+def rotary_backward(dq, dk, positions, frequencies, *, amplitude=1.0, interleaved=False, out=None, stream=None):
+    """The gradients of ``rotary``'s inputs from those of its results: the transposed rotation, the same arguments."""
+    return _rotate(dq, dk, positions, frequencies, amplitude, interleaved, out, stream, True)

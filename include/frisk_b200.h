@@ -64,8 +64,11 @@ enum {
   FRISK_B200_E_ARG = -7,           /* null pointer, bad enum, bad context                   */
   FRISK_B200_E_ATTN_SHAPE = -8,    /* attention shape outside the launch contract           */
   FRISK_B200_E_TOO_LARGE = -9,     /* exceeds the fixed capacity of a no-allocation entry   */
+  FRISK_B200_E_CACHE_SHAPE = -10,  /* sizes or strides outside the contract of the rotary and cache entries */
+  FRISK_B200_E_CACHE_TYPE = -11,   /* element types outside it                              */
   FRISK_B200_E_DEVICE_TIMEOUT = 1, /* a bounded device-side wait ran out (status word set)  */
-  FRISK_B200_E_CUDA = 2            /* a CUDA runtime/driver call failed (see last_cuda)     */
+  FRISK_B200_E_CUDA = 2,           /* a CUDA runtime/driver call failed (see last_cuda)     */
+  FRISK_B200_E_DEVICE_TABLE = 3    /* a table of the cache named rows, a length or a page out of range (status word 0x301-0x303) */
 };
 
 /*
@@ -283,8 +286,77 @@ int frisk_b200_peer_buffer_create(frisk_b200_ctx* ctx, size_t bytes, void** ptr,
 int frisk_b200_peer_buffer_open(frisk_b200_ctx* ctx, const void* handle64, void** ptr);
 int frisk_b200_peer_buffer_close(frisk_b200_ctx* ctx, void* ptr, int32_t owned);
 
+/* ---- rotary positions and the paged key/value cache ----------------------------------------
+ * No counterpart in the reference, whose attention takes compact BHSD tensors only.  Packed rows: a tensor of
+ * [rows, heads, D] whose elements of a head are neighbours; `ptr` is element 0, strides are in elements. */
+enum { FRISK_B200_E4M3 = 3 }; /* element type of a cache: 8-bit floats, 4 exponent and 3 fraction bits */
+typedef struct frisk_b200_packed {
+  void* ptr;
+  int64_t row_stride, head_stride;
+} frisk_b200_packed;
+
+/* Rotates the first `dim` elements of every head of q (and, heads_k > 0, of k) by the angle position * frequency of
+ * their pair, times `amplitude`: (a, b) -> amplitude * (a cos t - b sin t, b cos t + a sin t).  Pairs are (i, i + dim/2), or
+ * (2i, 2i + 1) where interleaved.  The other elements are copied.  `inverse`: -t, which maps gradients of the results to
+ * gradients of the inputs.  positions: rows of int32 or int64; frequencies: dim/2 doubles, radians per position; both on the
+ * device.  Angles are reduced to one turn in 64 bits.  F32, F16, BF16, any strides; an output may be its input (same
+ * pointer and strides), otherwise outputs overlap nothing.  q and k may be columns of one buffer of rows. */
+typedef struct frisk_b200_rotary_desc {
+  int64_t rows;
+  int32_t heads_q, heads_k, D, dim;
+  int32_t dtype, interleaved, inverse, positions64;
+  float amplitude;
+} frisk_b200_rotary_desc;
+int frisk_b200_rotary(frisk_b200_ctx* ctx, const frisk_b200_rotary_desc* desc, const void* positions,
+                      const double* frequencies, const frisk_b200_packed* q, const frisk_b200_packed* k,
+                      const frisk_b200_packed* q_out, const frisk_b200_packed* k_out, void* stream);
+
+/* A paged cache and the packed rows a call works on.  k, v: [pages, heads, page, D], dense, 16-byte aligned, F16, BF16 or
+ * E4M3; page is a power of two from 16 to 1024, D 64 or 128.  E4M3: k_exponent and v_exponent are [pages, heads, page] bytes, a
+ * value is code * 2^(e - 127), and e = 255 says that the row is NaN.
+ * table[b * table_stride + i] (i < table_width) is the page of keys i * page .. of sequence b.  Packed rows starts[b] ..
+ * starts[b + 1] - 1 belong to sequence b (starts has batch + 1 ascending entries) and row starts[b] + i has position
+ * lengths[b] + i.  Rows before starts[0] and from starts[batch] on belong to no sequence and are left as they are.  table,
+ * starts and lengths are on the device; a call that meets an entry out of range there leaves that row or sequence out (attention
+ * over a page out of range: its results are undefined) and frisk_b200_check returns FRISK_B200_E_DEVICE_TABLE. */
+typedef struct frisk_b200_cache_desc {
+  int64_t pages;
+  int32_t page, heads, D, dtype;
+  int32_t batch, table_width;
+  int64_t table_stride, rows;
+  void *k, *v;
+  uint8_t *k_exponent, *v_exponent;
+  const int32_t *table, *starts, *lengths;
+} frisk_b200_cache_desc;
+/* Writes packed rows of keys and values (dtype F16 or BF16, 16-byte aligned rows and heads) to their positions; a 16-bit cache
+ * takes its own type.  E4M3: the scale of a row is the least power of two that brings its largest magnitude to 448 or less, codes
+ * are rounded to the nearest, ties to even; a row with an infinity or a NaN gets e = 255.  A position must not be that of two rows
+ * (a page that two sequences name): what stays there would be undefined. */
+int frisk_b200_cache_write(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* cache, int32_t dtype,
+                           const frisk_b200_packed* k, const frisk_b200_packed* v, void* stream);
+/* The reverse: the packed rows' keys and values out of the cache, rounded to dtype (values of an E4M3 cache saturate at
+ * its largest finite one). */
+int frisk_b200_cache_read(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* cache, int32_t dtype,
+                          const frisk_b200_packed* k, const frisk_b200_packed* v, void* stream);
+/* Attention of packed query rows [rows, heads_q, D] over the cache, which holds their own keys and values already:
+ * out = softmax(scale * q.k) v over the keys a row sees.  Those are the lengths[b] before the new tokens, and of the
+ * new tokens j of its sequence the ones with mask[row * mask_stride + j] != 0 and j < mask_width (mask == NULL: those up to
+ * itself).  Query head h reads key head h / (heads_q / heads).  A row that sees no key is zero.  What a row does not see
+ * does not reach it, whatever it holds.  dtype: F16 or BF16, of q and out, and of a 16-bit cache.  max_new is a hint: the
+ * largest number of new tokens of a sequence (0: unknown); it bears on speed only.
+ * The workspace (16-byte aligned, contents of no matter before and after) must not be shared by calls that may overlap. */
+typedef struct frisk_b200_cache_attn_desc {
+  int32_t heads_q, dtype, max_new, mask_width;
+  int64_t mask_stride;
+  float scale;
+} frisk_b200_cache_attn_desc;
+size_t frisk_b200_cache_attention_workspace_bytes(const frisk_b200_cache_desc* cache, const frisk_b200_cache_attn_desc* desc);
+int frisk_b200_cache_attention(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* cache, const frisk_b200_cache_attn_desc* desc,
+                               const frisk_b200_packed* q, const frisk_b200_packed* out, const uint8_t* mask,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
 /* Checks the device status word after the stream has drained (synchronises `stream`).
- * Returns 0, FRISK_B200_E_DEVICE_TIMEOUT or FRISK_B200_E_CUDA. */
+ * Returns 0, FRISK_B200_E_DEVICE_TIMEOUT, FRISK_B200_E_DEVICE_TABLE or FRISK_B200_E_CUDA. */
 int frisk_b200_check(frisk_b200_ctx* ctx, void* stream);
 
 #ifdef __cplusplus
