@@ -582,50 +582,52 @@ __global__ void __launch_bounds__(kThreadsRow, 1)
   __syncthreads();
 }
 
-// Joins the parts of the items that several CTAs worked on.  Block (c, y): four rows, a warp each, of the item that CTA c began and
-// others finished.
+// Joins the parts of the items that several CTAs worked on.  Block (c, y): rows 4 y .. of the item that CTA c began and others
+// finished, a warp each, and those gridDim.y blocks on.
 template <bool QBF16, bool E4M3, int D>
 __global__ void __launch_bounds__(128) cache_attention_join_kernel(const CacheAttnParams p, int tile_rows) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const ItemRecord rec = p.records[blockIdx.x];
-  const int row = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= rec.rows) return;  // (0 where the CTA shares no item that it began)
+  const int lane = threadIdx.x & 31;
   const size_t floats = partial_floats(tile_rows, D);
   // the item's first part is the CTA's last item; the others' is their first
   auto slot = [&](int i) { return p.partials + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? rec.first_slot : 0)) * floats; };
-  float m = -INFINITY;
-  for (int i = lane; i < rec.parts; i += 32) m = fmaxf(m, __ldcg(slot(i) + tile_rows * D + row));
+  // (rec.rows is 0 where the CTA shares no item that it began)
+  for (int row = blockIdx.y * 4 + (threadIdx.x >> 5); row < rec.rows; row += gridDim.y * 4) {
+    float m = -INFINITY;
+    for (int i = lane; i < rec.parts; i += 32) m = fmaxf(m, __ldcg(slot(i) + tile_rows * D + row));
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-  constexpr int N = D / 32;  // columns a lane: 4 or 2
-  float acc[N] = {}, l = 0.f;
-  for (int i0 = 0; i0 < rec.parts; i0 += 32) {
-    float f = 0.f, lc = 0.f;
-    if (i0 + lane < rec.parts) {
-      const float* s = slot(i0 + lane) + tile_rows * D + row;
-      const float mc = __ldcg(s);
-      lc = __ldcg(s + tile_rows);
-      f = mc == -INFINITY ? (lc == 0.f ? 0.f : 1.f) : ex2f(mc - m);
-    }
-    const int here = min(32, rec.parts - i0);
+    for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+    constexpr int N = D / 32;  // columns a lane: 4 or 2
+    float acc[N] = {}, l = 0.f;
+    for (int i0 = 0; i0 < rec.parts; i0 += 32) {
+      float f = 0.f, lc = 0.f;
+      if (i0 + lane < rec.parts) {
+        const float* s = slot(i0 + lane) + tile_rows * D + row;
+        const float mc = __ldcg(s);
+        lc = __ldcg(s + tile_rows);
+        f = mc == -INFINITY ? (lc == 0.f ? 0.f : 1.f) : ex2f(mc - m);
+      }
+      const int here = min(32, rec.parts - i0);
 #pragma unroll 4
-    for (int i = 0; i < here; ++i) {
-      const float fi = __shfl_sync(0xffffffffu, f, i), li = __shfl_sync(0xffffffffu, lc, i);
-      const float* from = slot(i0 + i) + row * D + lane * N;
-      float v[N];
-      if (N == 4) *reinterpret_cast<float4*>(v) = __ldcg(reinterpret_cast<const float4*>(from));
-      else *reinterpret_cast<float2*>(v) = __ldcg(reinterpret_cast<const float2*>(from));
-      if (fi == 0.f && li == 0.f) continue;  // saw no key of the row
-      l = fmaf(li, fi, l);
+      for (int i = 0; i < here; ++i) {
+        const float fi = __shfl_sync(0xffffffffu, f, i), li = __shfl_sync(0xffffffffu, lc, i);
+        const float* from = slot(i0 + i) + row * D + lane * N;
+        float v[N];
+        if (N == 4) *reinterpret_cast<float4*>(v) = __ldcg(reinterpret_cast<const float4*>(from));
+        else *reinterpret_cast<float2*>(v) = __ldcg(reinterpret_cast<const float2*>(from));
+        if (fi == 0.f && li == 0.f) continue;  // saw no key of the row
+        l = fmaf(li, fi, l);
 #pragma unroll
-      for (int x = 0; x < N; ++x) acc[x] = fmaf(v[x], fi, acc[x]);
+        for (int x = 0; x < N; ++x) acc[x] = fmaf(v[x], fi, acc[x]);
+      }
     }
-  }
-  if (N == 4) {
-    store_row4<QBF16, E4M3>(p, rec.first_row, rec.head, rec.row0 + row, lane, make_float4(acc[0], acc[1], acc[N - 2], acc[N - 1]), l);
-  } else {
-    const float ox = __shfl_down_sync(0xffffffffu, acc[0], 1), oy = __shfl_down_sync(0xffffffffu, acc[1], 1);
-    if (!(lane & 1)) store_row4<QBF16, E4M3>(p, rec.first_row, rec.head, rec.row0 + row, lane >> 1, make_float4(acc[0], acc[1], ox, oy), l);
+    if (N == 4) {
+      store_row4<QBF16, E4M3>(p, rec.first_row, rec.head, rec.row0 + row, lane, make_float4(acc[0], acc[1], acc[N - 2], acc[N - 1]), l);
+    } else {
+      const float ox = __shfl_down_sync(0xffffffffu, acc[0], 1), oy = __shfl_down_sync(0xffffffffu, acc[1], 1);
+      if (!(lane & 1)) store_row4<QBF16, E4M3>(p, rec.first_row, rec.head, rec.row0 + row, lane >> 1, make_float4(acc[0], acc[1], ox, oy), l);
+    }
   }
 }
 
@@ -649,17 +651,27 @@ int launch_rows(frisk_b200_ctx* ctx, const CacheAttnParams& p, const CUtensorMap
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   FB_CUDA(ctx, cudaLaunchKernelEx(&cfg, kern, tk, tv, p));
-  cfg.gridDim = dim3(grid, L::kRows / 4);
-  cfg.blockDim = dim3(128);
-  cfg.dynamicSmemBytes = 0;
-  FB_CUDA(ctx, cudaLaunchKernelEx(&cfg, cache_attention_join_kernel<QBF16, E4M3, D>, p, (int)L::kRows));
   return 0;
 }
 
 template <bool QBF16, bool E4M3, int D>
-int launch_tile(frisk_b200_ctx* ctx, const CacheAttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, unsigned grid, int tile_rows,
-                cudaStream_t s) {
-  return tile_rows == 16 ? launch_rows<QBF16, E4M3, D, 1>(ctx, p, tk, tv, grid, s) : launch_rows<QBF16, E4M3, D, 2>(ctx, p, tk, tv, grid, s);
+int launch_all(frisk_b200_ctx* ctx, const CacheAttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, unsigned grid, int tile_rows,
+               cudaStream_t s) {
+  const int rc = tile_rows == 16   ? launch_rows<QBF16, E4M3, D, 1>(ctx, p, tk, tv, grid, s)
+                 : tile_rows == 32 ? launch_rows<QBF16, E4M3, D, 2>(ctx, p, tk, tv, grid, s)
+                                   : launch_cache_attention_tiles(ctx, p, tk, tv, grid, QBF16, E4M3, D, tile_rows, s);
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(grid, (unsigned)std::min(tile_rows / 4, 16));
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  FB_CUDA(ctx, cudaLaunchKernelEx(&cfg, cache_attention_join_kernel<QBF16, E4M3, D>, p, tile_rows));
+  return 0;
 }
 
 int check_attention(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_desc* a) {
@@ -679,11 +691,12 @@ int check_attention(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_
   return 0;
 }
 
-// Query rows a tile: 32 where a sequence is said to have more than 16.  (A sequence with more rows than that takes several tiles,
-// so a hint that is too low costs time only.)
+// Query rows a tile, by the rows that a sequence is said to have for a key head.  (A sequence with more than a tile's rows takes several
+// tiles, so a hint that is too low costs time only.)
 int tile_rows_of(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_desc* a) {
   const int64_t per = a->max_new > 0 ? a->max_new : c->batch > 0 ? (c->rows + c->batch - 1) / c->batch : 1;
-  return per * (a->heads_q / c->heads) <= 16 ? 16 : 32;
+  const int64_t rows = per * (a->heads_q / c->heads);
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 128 ? 128 : 256;
 }
 
 }  // namespace
@@ -750,6 +763,7 @@ extern "C" int frisk_b200_cache_attention(frisk_b200_ctx* ctx, const frisk_b200_
   p.out_head = out->head_stride;
   p.k_exponent = c->k_exponent;
   p.v_exponent = c->v_exponent;
+  p.v_pages = c->v;
   p.mask = mask;
   p.mask_stride = a->mask_stride;
   p.mask_width = a->mask_width;
@@ -762,8 +776,8 @@ extern "C" int frisk_b200_cache_attention(frisk_b200_ctx* ctx, const frisk_b200_
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int rows = tile_rows_of(c, a);
   if (c->D == 64)
-    return bf16 ? (e4m3 ? launch_tile<true, true, 64>(ctx, p, tk, tv, grid, rows, s) : launch_tile<true, false, 64>(ctx, p, tk, tv, grid, rows, s))
-                : (e4m3 ? launch_tile<false, true, 64>(ctx, p, tk, tv, grid, rows, s) : launch_tile<false, false, 64>(ctx, p, tk, tv, grid, rows, s));
-  return bf16 ? (e4m3 ? launch_tile<true, true, 128>(ctx, p, tk, tv, grid, rows, s) : launch_tile<true, false, 128>(ctx, p, tk, tv, grid, rows, s))
-              : (e4m3 ? launch_tile<false, true, 128>(ctx, p, tk, tv, grid, rows, s) : launch_tile<false, false, 128>(ctx, p, tk, tv, grid, rows, s));
+    return bf16 ? (e4m3 ? launch_all<true, true, 64>(ctx, p, tk, tv, grid, rows, s) : launch_all<true, false, 64>(ctx, p, tk, tv, grid, rows, s))
+                : (e4m3 ? launch_all<false, true, 64>(ctx, p, tk, tv, grid, rows, s) : launch_all<false, false, 64>(ctx, p, tk, tv, grid, rows, s));
+  return bf16 ? (e4m3 ? launch_all<true, true, 128>(ctx, p, tk, tv, grid, rows, s) : launch_all<true, false, 128>(ctx, p, tk, tv, grid, rows, s))
+              : (e4m3 ? launch_all<false, true, 128>(ctx, p, tk, tv, grid, rows, s) : launch_all<false, false, 128>(ctx, p, tk, tv, grid, rows, s));
 }

@@ -32,6 +32,7 @@ struct CacheAttnParams {
   void* out;
   int64_t q_row, q_head, out_row, out_head;
   const uint8_t *k_exponent, *v_exponent;
+  const void* v_pages;
   const uint8_t* mask;
   int64_t mask_stride;
   int mask_width, group;
@@ -204,4 +205,9 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 
 }  // namespace cache
+
+// tiles of 128 or 256 rows on tcgen05 (cache_attention_tiles.cu); without the join
+int launch_cache_attention_tiles(frisk_b200_ctx* ctx, const cache::CacheAttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv,
+                                 unsigned grid, bool bf16, bool e4m3, int D, int tile_rows, cudaStream_t s);
+
 }  // namespace fb

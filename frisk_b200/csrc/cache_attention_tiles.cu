@@ -1,0 +1,862 @@
+// Attention of drafted tokens over a paged cache for many query rows a key head (cache_attention.cu has the operator, the kernel for few
+// rows and the join of shared items): tcgen05 over tiles of 128 rows.
+//
+// A (sequence, key head) has new tokens times query heads rows; a unit is 64 keys of one tile of 128 rows, or of two tiles
+// that share the K and V (kPair).  Each CTA has two softmax groups of four warps (thread = row) and an MMA-issuing warp for either:
+//   * kPair: group g has row tile g, both take every key tile;
+//   * else one row tile, whose key tiles the groups take in turn, each with scores, O and statistics of its own, put together at the end
+//     of the CTA's part of the item.
+// S = Q.K^T into one of two TMEM buffers a group, P back over its scores as 16-bit pairs, O += P.V from there.  S runs two key tiles ahead of
+// P.V, and a ring stage holds what an MMA warp takes in one step: V of key tile b and K of tile b + 2.
+//
+// 16-bit caches: stages are filled by TMA, page by page.  Key tiles that reach behind lengths[b] are checked by a warp of their own
+// before their values are used: rows behind the last key become zeros, and so do infinities and NaN, because their product with a weight
+// of zero would reach rows that do not see them; if there were any, rows that do see them get them back when O is stored.
+//
+// 8-bit caches: the raw tiles arrive by TMA and four warps turn them into the operands in halves.  Where the scales of a tile's
+// keys (or of its values) lie within 2^8 of each other they are folded into the halves, exactly, relative to the tile's largest; the
+// largest joins the scale of the scores, and that of the values the exponent of the weights, w = 2^(s + v - A), one number a tile.
+// Other tiles are rare: their keys or values stay unscaled and every score or weight takes its own ("wide").  The row sum is
+// kept in units of 2^B of its own, since the values' scales have no part in it.
+//
+// What bounds it: 16-bit, up to 128 rows, HBM; else the softmax groups (some 1700 clk for 64 keys of 256 rows, of which 1024 exponentials)
+// and, with 8-bit caches, the conversion beside them.
+// Every mbarrier wait is bounded (ptx.cuh); no TMA load uses cluster multicast.
+#include <algorithm>
+#include <cfloat>
+
+#include "attention_common.cuh"
+#include "cache_attention.cuh"
+#include "work_split.cuh"
+
+namespace fb {
+namespace {
+using namespace attn;
+using namespace cache;
+
+constexpr int BN = kTileKeys;
+constexpr int kWarpFix = 11;     // 16-bit: checks values; 8-bit: idle
+constexpr int kWarpConvert = 12;  // 8-bit: four warps
+constexpr int kInfos = 8;        // key tiles whose scales are kept, for either group
+constexpr uint32_t kFolded = 8;  // log2: scales of a tile that lie this close are folded
+
+template <bool E4M3> constexpr int threads_of() { return E4M3 ? 512 : 384; }
+template <bool E4M3> constexpr int regs_softmax() { return E4M3 ? 176 : 208; }
+template <bool E4M3> constexpr int regs_other() { return E4M3 ? 80 : 72; }
+
+// the scales of a key tile's keys and values, 8-bit caches
+struct alignas(16) TileInfo {
+  uint8_t k[64], v[64];
+  float k_scale, v_log2;  // of the folded tile: 2^(largest - 127) of the keys, largest - 127 of the values
+  int wide_k, wide_v;         // not folded: the range of the scales is too large
+};
+
+// The scales of a tile's rows (the first `left` of 64), found by a whole warp: the largest, and whether they span too much to be folded.
+// Rows of zeros, and what is no larger than 2^-117, have the least scale: zero beside any other.
+struct Fold {
+  uint32_t top;
+  bool wide;
+};
+__device__ __forceinline__ Fold fold_of(const uint8_t* scales, int left, int lane) {
+  uint32_t top = 0, low = 255;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t e = lane + 32 * i < left ? scales[lane + 32 * i] : 1u;
+    top = max(top, e);
+    low = min(low, e <= 1u ? 255u : e);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  low = __reduce_min_sync(0xffffffffu, low);
+  if (top <= 1u) top = low = 127;
+  return Fold{top, top - low > kFolded || top > 187u || low < 67u};
+}
+
+template <int D, bool E4M3, bool PAIR>
+struct TilesSmem {
+  static constexpr int kQTile = BM * D * 2;
+  static constexpr int kKv = BN * D * 2;                 // a K or V operand tile
+  static constexpr int kStage = 2 * kKv;                 // K, then V
+    static constexpr int kQTiles = PAIR ? 2 : 1;
+  static constexpr int kStages = E4M3 ? (PAIR ? 3 : 4) : (D == 128 ? (PAIR ? 4 : 6) : 8);
+  static constexpr int kRawStages = E4M3 ? (D == 128 ? 3 : 6) : 0;
+  static constexpr int kRing = kQTiles * kQTile;
+  static constexpr int kRawRing = kRing + kStages * kStage;         // 1024-byte aligned tiles
+  static constexpr int kRawTiles = E4M3 ? 2 * BN * D : 0;
+  static constexpr int kRawScales = kRawRing + kRawStages * kRawTiles;  // [raw stages][K's, its values', V's: 64 each]
+  static constexpr int kInfo = kRawScales + kRawStages * 192;
+  static constexpr int kBar = kInfo + (E4M3 ? 2 * kInfos * (int)sizeof(TileInfo) : 0);
+  static constexpr int kTotal = kBar + 1024 + 1024;
+  static_assert(kTotal <= 232448, "rings and tiles must fit");
+};
+
+template <bool QBF16, bool E4M3, int D, bool PAIR>
+__global__ void __launch_bounds__(threads_of<E4M3>(), 1)
+    cache_attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                                 const CacheAttnParams p) {
+  using L = TilesSmem<D, E4M3, PAIR>;
+  constexpr bool MBF16 = QBF16 && !E4M3;  // type of the products' operands
+  constexpr int kRows = PAIR ? 2 * BM : BM;
+  constexpr int kThreadsAll = threads_of<E4M3>();
+  constexpr bool OWN_KV = !PAIR;  // each MMA warp has key tiles, and stages of the ring, of its own
+  constexpr int kBoxes = D / 64, kBoxBytes = BM * 128, kKvBoxBytes = BN * 128;
+  constexpr int kStages = L::kStages, kOwnStages = OWN_KV ? kStages / 2 : kStages;
+  constexpr int kElem = E4M3 ? 1 : 2;
+  extern __shared__ unsigned char smem_unaligned[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  uint64_t* kv_full = bars;            // [8]
+  uint64_t* kv_empty = bars + 8;       // [8]
+  uint64_t* fixed = bars + 16;         // [8] 16-bit: the stage's values are checked; 8-bit: [raw stages] raw tiles are there
+  uint64_t* raw_empty = bars + 24;     // [8]
+  uint64_t* s_full = bars + 32;        // [2 groups][2 buffers] the scores of a key tile are complete
+  uint64_t* p_ready = bars + 36;       // [2 groups][2 buffers] its probabilities are written
+  uint64_t* o_done = bars + 40;        // [2 groups][2] of an item all P.V but the last, all P.V are complete
+  uint64_t* q_full = bars + 44;        // [2]
+  uint64_t* turn = bars + 46;          // [2] the MMA warps issue in turn
+  uint64_t* xchg = bars + 48;          // [1] the two softmax groups meet
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 49);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  volatile uint32_t* bad_values = tmem_slot + 2;  // [8] by item: number + 1 of one in which infinities or NaN were taken out of values
+  PlanShared* plan_shared = reinterpret_cast<PlanShared*>(bars + 56);
+  static_assert(56 * 8 + sizeof(PlanShared) <= 1024, "barriers and plan must fit");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto ring_stage = [](int n, int group) -> int { return (OWN_KV ? group * kOwnStages : 0) + n % kOwnStages; };
+  auto ring_phase = [](int n) -> uint32_t { return (n / kOwnStages) & 1; };
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&kv_full[i], E4M3 ? 4 : 1);                          // the converting warps, or the TMA unit
+      mbar_init(&kv_empty[i], (OWN_KV ? 1 : 2) + (E4M3 ? 0 : 1));  // MMA warps that read the stage, and the checking warp
+      if (!E4M3) mbar_init(&fixed[i], 1);
+    }
+    for (int i = 0; i < L::kRawStages; ++i) {
+      mbar_init(&fixed[i], 1);
+      mbar_init(&raw_empty[i], 4);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_ready[i], 128);
+      mbar_init(&o_done[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], PAIR ? 128 : 256);
+      mbar_init(&turn[i], 1);
+    }
+    mbar_init(xchg, 256);
+    *abort_flag = 0;
+    for (int i = 0; i < 8; ++i) bad_values[i] = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  if (warp == kWarpMma) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Plan plan = make_plan<kThreadsAll>(p, kRows, plan_shared);
+
+  // What the roles agree on about an item: key tiles [tile0, tile0 + n), of which group g takes every one, or every second.
+  struct Work {
+    int tile0, n, keys, rows, nq[2], first_masked;
+  };
+  auto work_of = [&](const Cursor& c) {
+    Work w;
+    w.tile0 = c.tile;
+    w.n = c.tiles_here();
+    w.keys = c.seq.length + c.seq.count;
+    w.rows = min(kRows, c.seq.count * p.group - c.rt * kRows);
+    w.nq[0] = PAIR ? w.n : (w.n + 1) / 2;
+    w.nq[1] = PAIR ? (w.rows > BM ? w.n : 0) : w.n / 2;
+    w.first_masked = c.seq.length / BN;  // key tiles from this one on are not seen whole by every row
+    return w;
+  };
+  // key tile of group g's b-th
+  auto tile_of = [](const Work& w, int b, int g) { return w.tile0 + (PAIR ? b : 2 * b + g); };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(regs_other<E4M3>()));
+    if (warp == kWarpTma) {
+      // ------------------------------------------------------------------ TMA producer: the warp reads the table, lane 0 loads
+      int loaded[2] = {0, 0};  // stages filled so far, over all items; OWN_KV: for either MMA warp
+      int raws = 0;
+      bool ok = true;
+      const int box = min(p.t.page, BN);  // rows a load brings
+      for (Cursor c(p, plan, kRows); c.left > 0 && ok; c.next_item(p, kRows)) {
+        const Work w = work_of(c);
+        const int* row = p.t.table + c.b * p.t.stride;
+        int ids[2] = {0, 0}, from[2] = {-64, -64};  // for K and for V: pages from .. from + 31
+        const int n_keys = w.nq[0];
+        for (int b = -2; b < n_keys && ok; ++b) {
+#pragma unroll
+          for (int g = 0; g < (OWN_KV ? 2 : 1); ++g) {
+            const bool has_k = b + 2 < w.nq[g], has_v = b >= 0 && b < w.nq[g];
+            if (!ok || !(has_k || has_v)) continue;
+            const int st = E4M3 ? raws % (L::kRawStages ? L::kRawStages : 1) : ring_stage(loaded[g], g);
+            uint64_t* const full = E4M3 ? &fixed[st] : &kv_full[st];
+            ok = E4M3 ? mbar_wait_warp(&raw_empty[st], ((raws / (L::kRawStages ? L::kRawStages : 1)) & 1) ^ 1, abort_flag, p.status, ST_CACHE_RAW)
+                      : mbar_wait_warp(&kv_empty[st], ring_phase(loaded[g]) ^ 1, abort_flag, p.status, ST_CACHE_KV);
+            if (!ok) continue;
+            ++loaded[g];
+            ++raws;
+            int boxes[2], tile[2];  // K's, V's
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              tile[x] = tile_of(w, x ? b : b + 2, g);
+              boxes[x] = (x ? has_v : has_k) ? min(BN / box, (w.keys - tile[x] * BN + box - 1) / box) : 0;
+            }
+            if (lane == 0)
+              mbar_expect_tx(full, (uint32_t)box * ((boxes[0] + boxes[1]) * D * kElem + (E4M3 ? 2 * boxes[0] + boxes[1] : 0)));
+            __syncwarp();
+            unsigned char* at = smem + (E4M3 ? L::kRawRing + st * L::kRawTiles : L::kRing + st * L::kStage);
+            unsigned char* scales = smem + L::kRawScales + st * 192;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              for (int i = 0; i < boxes[x]; ++i) {
+                const int key = tile[x] * BN + i * box, n = key >> p.t.page_log2;
+                if (n < from[x] || n >= from[x] + 32) {
+                  from[x] = n;
+                  ids[x] = n + lane < p.t.width ? __ldg(row + n + lane) : 0;
+                }
+                int page = __shfl_sync(0xffffffffu, ids[x], n - from[x]);
+                if (page < 0 || page >= p.t.pages) {  // (page 0 is read in its place)
+                  if (lane == 0) atomicCAS(p.status, 0u, ST_CACHE_PAGE);
+                  page = 0;
+                }
+                if (lane == 0) {
+                  const int token = ((page * p.t.heads + c.h) << p.t.page_log2) + (key & (p.t.page - 1));
+                  if (E4M3) {
+                    // (two rows of 64 bytes make a line of the map)
+                    tma_load_2d(at + x * BN * D + i * box * D, x ? &tmap_v : &tmap_k, full, 0, D == 64 ? token / 2 : token);
+                    if (x == 0) {
+                      bulk_load(scales + i * box, p.k_exponent + token, box, full);
+                      bulk_load(scales + 64 + i * box, p.v_exponent + token, box, full);
+                    } else {
+                      bulk_load(scales + 128 + i * box, p.v_exponent + token, box, full);
+                    }
+                  } else {
+#pragma unroll
+                    for (int d = 0; d < kBoxes; ++d)
+                      tma_load_2d(at + x * L::kKv + d * kKvBoxBytes + i * box * 128, x ? &tmap_v : &tmap_k, full, d * 64, token);
+                  }
+                }
+              }
+          }
+        }
+      }
+    } else if (warp == kWarpMma || warp == kWarpMma + 1) {
+      // ------------------------------------------------------------------ MMA issuers, one warp per softmax group
+      // tcgen05 operations of ONE thread execute in issue order: S(b + 2) overwrites P(b) after P(b).V(b) has read it.  The two warps
+      // issue in turn, so that one's waits lie behind the other's MMAs; one elected lane issues.
+      const int mq = __shfl_sync(0xffffffffu, warp - kWarpMma, 0);
+      constexpr uint32_t idesc_s = umma_idesc_f16(BM, BN, MBF16, false, false);
+      constexpr uint32_t idesc_o = umma_idesc_f16(BM, D, MBF16, false, true);
+      const uint64_t dq = umma_desc_kmajor_sw128(smem_u32(smem) + (PAIR ? mq * L::kQTile : 0));
+      const uint64_t dk = umma_desc_kmajor_sw128(smem_u32(smem + L::kRing));
+      const uint64_t dv = umma_desc_mnmajor_sw128(smem_u32(smem + L::kRing + L::kKv), kKvBoxBytes, 1024);
+      const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+      const uint32_t t_sq = tmem + mq * 128;        // the two buffers of scores, 64 columns each
+      const uint32_t t_oq = tmem + 256 + mq * 128;  // O
+      int turns = 0, taken = 0, begun = 0, finished = 0, items = 0;
+      bool ok = true;
+      for (Cursor c(p, plan, kRows); c.left > 0 && ok; c.next_item(p, kRows)) {
+        const Work w = work_of(c);
+        const int n_mine = w.nq[mq], n_max = OWN_KV ? n_mine : w.n;  // key tiles: used, followed
+        const int n_steps = w.nq[0];                                  // the same for both MMA warps
+        const bool in_turn = w.nq[1] > 0;                             // a lone warp issues as it comes
+        // (a barrier whose item has no key tile for this warp is neither arrived on nor waited for: the warp could be items behind)
+        if (n_mine > 0) {
+          ok = mbar_wait_warp(&q_full[mq], items & 1, abort_flag, p.status, ST_CACHE_Q);
+          ++items;
+        }
+        for (int b = -2; b < n_steps && ok; ++b) {
+          const bool staged = b + 2 < n_max || (b >= 0 && b < n_max);  // a stage of the ring comes with this step
+          const bool use_p = b >= 0 && b < n_mine, use_s = b + 2 < n_mine;
+          const int st = ring_stage(taken, mq), buf = finished & 1;
+          if (use_p && staged)
+            ok = mbar_wait_both(&p_ready[2 * mq + buf], (finished >> 1) & 1, &kv_full[st], ring_phase(taken), abort_flag, p.status,
+                                ST_CACHE_P, ST_CACHE_KV);
+          else if (staged)
+            ok = mbar_wait(&kv_full[st], ring_phase(taken), abort_flag, p.status, ST_CACHE_KV);
+          if (!E4M3 && ok && use_p && tile_of(w, b, mq) >= w.first_masked)
+            ok = mbar_wait(&fixed[st], ring_phase(taken), abort_flag, p.status, ST_CACHE_KV);
+          if (ok && in_turn) ok = mbar_wait(&turn[mq], (turns & 1) ^ (mq ^ 1), abort_flag, p.status, ST_CACHE_S);
+          turns += in_turn;
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint64_t at = static_cast<uint64_t>((st * L::kStage) >> 4);
+          if (use_p) {
+            ++finished;
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < BN / 16; ++kk)
+                umma_f16_ts(t_oq, t_sq + buf * BN + kk * 8, dv + at + static_cast<uint64_t>((kk * 2048) >> 4), idesc_o,
+                            (b > 0 || kk > 0) ? 1u : 0u);
+            }
+          }
+          if (use_s) {
+            const int s_buf = begun & 1;
+            ++begun;
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk)
+                umma_f16_ss(t_sq + s_buf * BN, dq + static_cast<uint64_t>(((kk / 4) * kBoxBytes + (kk % 4) * 32) >> 4),
+                            dk + at + static_cast<uint64_t>(((kk / 4) * kKvBoxBytes + (kk % 4) * 32) >> 4), idesc_s, kk != 0);
+              if (in_turn) mbar_arrive(&turn[mq ^ 1]);
+              umma_commit(&s_full[2 * mq + s_buf]);
+            }
+          } else if (in_turn && elect_one()) {
+            mbar_arrive(&turn[mq ^ 1]);
+          }
+          if (use_p && b >= n_mine - 2 && elect_one()) umma_commit(&o_done[2 * mq + (b == n_mine - 1)]);
+          if (staged) {
+            if (elect_one()) {
+              if (use_p || use_s) umma_commit(&kv_empty[st]); else mbar_arrive(&kv_empty[st]);
+            }
+            ++taken;
+          }
+        }
+      }
+    } else if (!E4M3 && warp == kWarpFix) {
+      // ------------------------------------------------------------------ values that not every row sees (16-bit)
+      // It follows every stage, since the parity of a phase two back reads like its own, and releases it too.
+      int followed[2] = {0, 0}, items = 0;
+      bool ok = true;
+      for (Cursor c(p, plan, kRows); c.left > 0 && ok; c.next_item(p, kRows)) {
+        const Work w = work_of(c);
+        for (int b = -2; b < w.nq[0] && ok; ++b) {
+#pragma unroll
+          for (int g = 0; g < (OWN_KV ? 2 : 1); ++g) {
+            const bool has_k = b + 2 < w.nq[g], has_v = b >= 0 && b < w.nq[g];
+            if (!ok || !(has_k || has_v)) continue;
+            const int st = ring_stage(followed[g], g);
+            ok = mbar_wait_warp(&kv_full[st], ring_phase(followed[g]), abort_flag, p.status, ST_CACHE_KV);
+            if (!ok) continue;
+            ++followed[g];
+            const int tile = tile_of(w, b, g);
+            if (has_v && tile >= w.first_masked) {
+              const int left = w.keys - tile * BN;  // rows of the tile that are keys
+              bool bad = false;
+              unsigned char* v = smem + L::kRing + st * L::kStage + L::kKv;
+#pragma unroll 1
+              for (int e0 = lane; e0 < L::kKv / 16; e0 += 32 * 8) {
+                uint4 x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(v + (e0 + 32 * i) * 16);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const int key = ((e0 + 32 * i) * 16 % kKvBoxBytes) / 128;
+                  uint32_t* y = reinterpret_cast<uint32_t*>(&x[i]);
+                  const uint32_t expo = MBF16 ? 0x7f807f80u : 0x7c007c00u;
+                  uint32_t take = 0;
+#pragma unroll
+                  for (int n = 0; n < 4; ++n) {
+                    const uint32_t m = key < left ? __vcmpeq2(y[n] & expo, expo) : 0xffffffffu;
+                    bad |= key < left && m != 0;
+                    y[n] &= ~m;
+                    take |= m;
+                  }
+                  if (take) *reinterpret_cast<uint4*>(v + (e0 + 32 * i) * 16) = x[i];
+                }
+              }
+              fence_proxy_async_smem();
+              if (bad) bad_values[items & 7] = items + 1;
+              __syncwarp();
+            }
+            if (lane == 0) {
+              mbar_arrive(&fixed[st]);
+              mbar_arrive(&kv_empty[st]);
+            }
+          }
+        }
+        ++items;
+      }
+    } else if (E4M3 && warp >= kWarpConvert) {
+      // ------------------------------------------------------------------ 8-bit tiles into operands
+      const int me = threadIdx.x - kWarpConvert * 32;  // 0 .. 127
+      int made[2] = {0, 0}, raws = 0, items = 0, infos[2] = {0, 0};
+      bool ok = true;
+      constexpr int kRawStages = L::kRawStages ? L::kRawStages : 1;
+      for (Cursor c(p, plan, kRows); c.left > 0 && ok; c.next_item(p, kRows)) {
+        const Work w = work_of(c);
+        for (int b = -2; b < w.nq[0] && ok; ++b) {
+#pragma unroll
+          for (int g = 0; g < (OWN_KV ? 2 : 1); ++g) {
+            const bool has_k = b + 2 < w.nq[g], has_v = b >= 0 && b < w.nq[g];
+            if (!ok || !(has_k || has_v)) continue;
+            const int rs = raws % kRawStages, st = ring_stage(made[g], g);
+            ok = mbar_wait_warp(&fixed[rs], (raws / kRawStages) & 1, abort_flag, p.status, ST_CACHE_RAW) &&
+                 mbar_wait_warp(&kv_empty[st], ring_phase(made[g]) ^ 1, abort_flag, p.status, ST_CACHE_KV);
+            if (!ok) continue;
+            ++raws;
+            ++made[g];
+            const unsigned char* raw = smem + L::kRawRing + rs * L::kRawTiles;
+            unsigned char* op = smem + L::kRing + st * L::kStage;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              if (!(x ? has_v : has_k)) continue;
+              const int left = w.keys - tile_of(w, x ? b : b + 2, g) * BN;
+              const uint8_t* scales = smem + L::kRawScales + rs * 192;
+              // every warp finds the largest scale by itself
+              const Fold fold = fold_of(scales + (x ? 128 : 0), left, lane);
+              if (x == 0 && warp == kWarpConvert) {
+                // what the softmax group has to know about the tile.  (Its place is free: the tile eight before it is long done, since S runs
+                // two tiles ahead of P.V and the ring fewer than that.)
+                TileInfo* info = reinterpret_cast<TileInfo*>(smem + L::kInfo) + g * kInfos + (infos[g] + b + 2) % kInfos;
+                const Fold values = fold_of(scales + 64, left, lane);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  info->k[lane + 32 * i] = scales[lane + 32 * i];
+                  info->v[lane + 32 * i] = scales[64 + lane + 32 * i];
+                }
+                if (lane == 0) {
+                  info->k_scale = __uint_as_float(fold.top << 23);
+                  info->v_log2 = (float)((int)values.top - 127);
+                  info->wide_k = fold.wide;
+                  info->wide_v = values.wide;
+                }
+              }
+              const uint8_t* mine = scales + (x ? 128 : 0);
+              const uint32_t top = fold.top;
+              const bool wide = fold.wide;
+              const unsigned char* from = raw + x * BN * D;
+              unsigned char* to = op + x * L::kKv;
+              bool bad = false;
+              // 16 codes a step: a lane's neighbours have the 16-byte pieces of the same key
+#pragma unroll 4
+              for (int e = me; e < BN * D / 16; e += 128) {
+                const int key = e / (D / 16), piece = e % (D / 16);
+                const uint32_t off = key * D + piece * 16;
+                const uint4 codes = *reinterpret_cast<const uint4*>(from + (off ^ (((off >> 7) & 7) << 4)));
+                // 2^(e - largest), as a half; 0 for what is no key
+                const uint32_t es = mine[key];
+                const int down = wide ? 0 : (int)top - (int)es;
+                const uint16_t f = key >= left || down > 14 ? 0 : (uint16_t)((15 - down) << 10);
+                const uint32_t f2 = f | ((uint32_t)f << 16);
+                const __half2 scale = *reinterpret_cast<const __half2*>(&f2);
+                uint32_t out[8];
+                const uint32_t in[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const uint32_t lo = e4m3x2_to_half2(in[i]), hi = e4m3x2_to_half2_hi(in[i]);
+                  const __half2 a = __hmul2(*reinterpret_cast<const __half2*>(&lo), scale), b2 = __hmul2(*reinterpret_cast<const __half2*>(&hi), scale);
+                  out[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
+                  out[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&b2);
+                }
+                if (x == 1) {
+                  // codes that are NaN (0x7f, 0xff) come back when O is stored
+                  uint32_t nan = 0;
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) nan |= __vcmpeq4(in[i] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                  if (nan || key >= left) {
+                    bad |= nan != 0 && key < left;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) out[i] = key < left ? out[i] & ~__vcmpeq2(out[i] & 0x7c007c00u, 0x7c007c00u) : 0u;
+                  }
+                }
+                const uint32_t line = key * 128, col = (piece & 3) * 2;
+                unsigned char* box = to + (piece >> 2) * kKvBoxBytes;
+                *reinterpret_cast<uint4*>(box + line + ((col ^ (key & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
+                *reinterpret_cast<uint4*>(box + line + (((col + 1) ^ (key & 7)) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
+              }
+              if (bad) bad_values[items & 7] = items + 1;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(&raw_empty[rs]);
+              mbar_arrive(&kv_full[st]);
+            }
+          }
+        }
+        infos[0] += w.nq[0];
+        infos[1] += w.nq[1];
+        ++items;
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(regs_softmax<E4M3>()));
+    // ------------------------------------------------------------------ softmax groups
+    const int q = warp >> 2;    // this group: its row tile, or its share of the key tiles
+    const int quad = warp & 3;  // TMEM lane quadrant this warp may touch
+    const int row = quad * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t t_s = tmem_base + q * 128 + lane_addr;
+    const uint32_t t_o = tmem_base + 256 + q * 128 + lane_addr;
+    int steps = 0;         // key tiles of this group so far, over all items: buffer and phase of s_full
+    int ends[2] = {0, 0};  // items with two key tiles or more, with one or more so far: the phases of o_done
+    int meets = 0, items = 0;
+    int infos = 0;  // key tiles of the items before: the places of their scales
+    bool ok = true;
+    auto meet = [&]() {  // of the two groups
+      tc_fence_before_sync();
+      mbar_arrive(xchg);
+      if (ok) ok = mbar_wait_warp(xchg, meets & 1, abort_flag, p.status, ST_CACHE_O);
+      ++meets;
+      tc_fence_after_sync();
+    };
+    for (Cursor c(p, plan, kRows); c.left > 0 && ok; c.next_item(p, kRows)) {
+      const Work w = work_of(c);
+      const Seq seq = c.seq;
+      const int n_tiles = w.nq[q];
+      const int r = c.rt * kRows + (PAIR ? q * BM : 0) + row;  // row of the (sequence, key head)
+      const bool valid = r < seq.count * p.group;
+      const int i_new = valid ? r / p.group : 0;  // its new token
+
+      // ---- the row's query, to its place in the swizzled tile.  (The products that read the tile before are complete: all of their scores
+      // have been read, by both groups where they share it.)
+      float row_scale = fabsf(p.scale_log2);
+      {
+        const int head = c.h * p.group + (valid ? r - i_new * p.group : 0);
+        const uint16_t* src = static_cast<const uint16_t*>(p.q) + (int64_t)(seq.first + i_new) * p.q_row + (int64_t)head * p.q_head;
+        unsigned char* tile = smem + (PAIR ? q * L::kQTile : 0);
+        const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a negative scale goes into the queries)
+        float down = 1.f;
+        if (E4M3 && QBF16) {
+          uint32_t most = 0;
+          if (valid)
+#pragma unroll 4
+            for (int i = 0; i < D / 8; ++i) {
+              const uint4 x = __ldg(reinterpret_cast<const uint4*>(src) + i);
+              const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+              for (int n = 0; n < 4; ++n) most = max(most, max(y[n] & 0x7fffu, (y[n] >> 16) & 0x7fffu));
+            }
+          const uint32_t e = min(max(most >> 7, 1u), 253u);  // halves with the row's largest magnitude in [1, 2)
+          down = __uint_as_float((254u - e) << 23);
+          row_scale *= __uint_as_float(e << 23);
+        }
+        // where the groups share a tile, each brings half of every row
+        constexpr int kPieces = D / 8 / (PAIR ? 1 : 2);
+        const int first = PAIR ? 0 : q * kPieces;
+#pragma unroll 4
+        for (int i = first; i < first + kPieces; ++i) {
+          uint4 x = valid ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
+          if (E4M3 && QBF16) {
+            auto half = [&](uint32_t b) { return pack16<false>(__uint_as_float(b << 16) * down, __uint_as_float(b & 0xffff0000u) * down); };
+            x = make_uint4(half(x.x), half(x.y), half(x.z), half(x.w));
+          }
+          x = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
+          *reinterpret_cast<uint4*>(tile + (i >> 3) * kBoxBytes + row * 128 + (((i & 7) ^ (row & 7)) << 4)) = x;
+        }
+        fence_proxy_async_smem();
+        if (!PAIR || n_tiles > 0) mbar_arrive(&q_full[PAIR ? q : 0]);
+        if (!PAIR && w.nq[1] > 0) mbar_arrive(&q_full[1]);
+      }
+
+      float a_ref = -FLT_MAX;  // log2: what the stored weights and O are relative to
+      float l_sum = 0.f, b_ref = -FLT_MAX;  // the row sum is l_sum * 2^b_ref (16-bit caches: b_ref stands for a_ref)
+      uint32_t sr[2][32];                   // the scores of a key tile
+      auto load_scores = [&]() {            // of step `steps`
+        tc_fence_after_sync();
+#pragma unroll
+        for (int x = 0; x < 2; ++x) tmem_ld_32x32b_x32(t_s + (steps & 1) * BN + x * 32, sr[x]);
+      };
+      auto wait_scores = [&]() {
+        if (ok) ok = mbar_wait_warp(&s_full[2 * q + (steps & 1)], (steps >> 1) & 1, abort_flag, p.status, ST_CACHE_S);
+        if (ok) load_scores();
+      };
+      if (n_tiles > 0) wait_scores();
+      for (int i = 0; i < n_tiles && ok; ++i) {
+        const int buf = steps & 1, tile = tile_of(w, i, q);
+        const TileInfo* info = reinterpret_cast<const TileInfo*>(smem + L::kInfo) + (PAIR ? 0 : q) * kInfos + (infos + i) % kInfos;
+        ++steps;
+        tmem_ld_wait();
+        const bool more = i + 1 < n_tiles;
+        float scale = row_scale, v_log2 = 0.f;
+        bool wide_k = false, wide_v = false;
+        if (E4M3) {
+          v_log2 = info->v_log2;
+          wide_k = info->wide_k != 0;
+          wide_v = info->wide_v != 0;
+          if (!wide_k) scale *= info->k_scale;
+        }
+        const bool general = wide_k || wide_v || tile >= w.first_masked;
+        // Takes a new reference where it grew by more than the threshold: rare.  O is rescaled in tensor memory.
+        auto settle = [&](float most) {
+          const float a_new = fmaxf(a_ref, most);
+          if (!__any_sync(0xffffffffu, a_new - a_ref > kRescaleThreshold)) return;
+          const float factor = ex2f(a_ref - a_new);
+          a_ref = a_new;
+          if (!E4M3) l_sum *= factor;
+          if (i == 0) return;  // (nothing is there yet)
+          // O must be complete up to the key tile before this one (the scores of the next one come after that product)
+          ok = more ? mbar_wait_warp(&s_full[2 * q + (buf ^ 1)], (steps >> 1) & 1, abort_flag, p.status, ST_CACHE_S)
+                    : mbar_wait_warp(&o_done[2 * q], ends[0] & 1, abort_flag, p.status, ST_CACHE_O);
+          if (!ok) return;
+          tc_fence_after_sync();
+#pragma unroll 1
+          for (int x = 0; x < D / 32; ++x) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(t_o + x * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+            tmem_st_32x32b_x32(t_o + x * 32, o);
+          }
+        };
+        auto add_sum = [&](float sum, float unit) {  // sum * 2^unit to the row sum, 8-bit
+          if (unit > b_ref) {
+            l_sum *= ex2f(b_ref - unit);
+            b_ref = unit;
+          }
+          l_sum = fmaf(sum, ex2f(unit - b_ref), l_sum);
+        };
+        uint32_t pk0[16], pk1[16];
+        if (!general) {
+          float mxc[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains of the row maximum
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              mxc[2 * x + (e & 1)] = max3f(mxc[2 * x + (e & 1)], __uint_as_float(sr[x][2 * e]), __uint_as_float(sr[x][2 * e + 1]));
+          const float mx = max3f(mxc[0], mxc[1], fmaxf(mxc[2], mxc[3])) * scale;
+          settle(E4M3 ? mx + v_log2 : mx);
+          if (!ok) break;
+          const float unit = E4M3 ? a_ref - v_log2 : a_ref;
+          const float2 scale2 = make_float2(scale, scale), neg2 = make_float2(-unit, -unit);
+          float2 sa = make_float2(0.f, 0.f), sb = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float2 xa = fma2(make_float2(__uint_as_float(sr[0][2 * e]), __uint_as_float(sr[0][2 * e + 1])), scale2, neg2);
+            const float2 xb = fma2(make_float2(__uint_as_float(sr[1][2 * e]), __uint_as_float(sr[1][2 * e + 1])), scale2, neg2);
+            const float2 ea = make_float2(ex2f(xa.x), ex2f(xa.y));
+            const float2 eb = make_float2(ex2f(xb.x), ex2f(xb.y));
+            sa = add2(sa, ea);
+            sb = add2(sb, eb);
+            pk0[e] = pack16<MBF16>(ea.x, ea.y);
+            pk1[e] = pack16<MBF16>(eb.x, eb.y);
+          }
+          const float2 tot = add2(sa, sb);
+          if (E4M3) add_sum(tot.x + tot.y, unit); else l_sum += tot.x + tot.y;
+        } else {
+          // What the row sees of the tile's keys, a bit a key.  The warp's rows belong to a few neighbouring tokens: the warp reads each
+          // one's mask side by side.
+          uint32_t see[2] = {0, 0};
+          const int ahead0 = tile * BN - seq.length;
+          const int t0 = __shfl_sync(0xffffffffu, i_new, 0), t1 = __reduce_max_sync(0xffffffffu, i_new);
+          for (int t = min(t0, t1); t <= t1; ++t) {
+            const uint32_t lo = __ballot_sync(0xffffffffu, sees(p, seq, t, ahead0 + lane));
+            const uint32_t hi = __ballot_sync(0xffffffffu, sees(p, seq, t, ahead0 + 32 + lane));
+            if (t == i_new) {
+              see[0] = lo;
+              see[1] = hi;
+            }
+          }
+          float mx = -INFINITY, mw = -INFINITY;  // of scores, of scores and scales
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              float s = __uint_as_float(sr[x][e]) * scale;
+              float v = v_log2;
+              if (E4M3 && wide_k) s = __uint_as_float(sr[x][e]) * scale_of(info->k[x * 32 + e]) * scale;
+              if (E4M3 && wide_v) {
+                const unsigned ev = info->v[x * 32 + e];
+                v = ev == 255u ? __uint_as_float(0x7fc00000u) : (float)((int)ev - 127);
+              }
+              if (!((see[x] >> e) & 1u)) s = -INFINITY;
+              sr[x][e] = __float_as_uint(s);
+              mx = fmaxf(mx, s);
+              if (E4M3) mw = fmaxf(mw, s + v);
+            }
+          settle(E4M3 ? mw : mx);
+          if (!ok) break;
+          if (E4M3 && mx > b_ref) {
+            l_sum *= ex2f(b_ref - mx);
+            b_ref = mx;
+          }
+          float sum = 0.f;
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float wgt[2];
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                const int j = 2 * e + y;
+                const float s = __uint_as_float(sr[x][j]);
+                float v = v_log2;
+                if (E4M3 && wide_v) {
+                  const unsigned ev = info->v[x * 32 + j];
+                  v = ev == 255u ? __uint_as_float(0x7fc00000u) : (float)((int)ev - 127);
+                }
+                const float pr = ex2f(s - (E4M3 ? b_ref : a_ref));
+                sum += pr;
+                wgt[y] = !E4M3 ? pr : s == -INFINITY ? 0.f : ex2f(s + v - a_ref);
+              }
+              (x ? pk1 : pk0)[e] = pack16<MBF16>(wgt[0], wgt[1]);
+            }
+          l_sum += sum;
+        }
+        const bool ahead = __all_sync(0xffffffffu, more && mbar_test(&s_full[2 * q + (steps & 1)], (steps >> 1) & 1));
+        if (ahead) load_scores();
+        // P is written over the first half of the scores it comes from
+        tmem_st_32x32b_x16(t_s + buf * BN, pk0);
+        tmem_st_32x32b_x16(t_s + buf * BN + 16, pk1);
+        tmem_st_wait();
+        tc_fence_before_sync();
+        mbar_arrive(&p_ready[2 * q + buf]);
+        if (more && !ahead) wait_scores();
+      }
+      if (ok && n_tiles > 0) ok = mbar_wait_warp(&o_done[2 * q + 1], ends[1] & 1, abort_flag, p.status, ST_CACHE_O);
+      if (!ok) break;
+      tc_fence_after_sync();
+      ends[0] += n_tiles > 1;
+      ends[1] += n_tiles > 0;
+
+      // ---- O: scaled to the units of the row sum, and out: whole, or as a part for the join
+      const float m_mine = E4M3 ? b_ref : a_ref;
+      float f[2] = {E4M3 ? ex2f(a_ref - b_ref) : 1.f, 0.f}, m = m_mine, l = l_sum;
+      if (!E4M3 || l_sum == 0.f) f[0] = l_sum == 0.f ? 0.f : f[0];
+      if (!PAIR) {
+        meet();  // all scores have been read: the statistics take the queries' place
+        float4* stat = reinterpret_cast<float4*>(smem);
+        stat[q * BM + row] = make_float4(m_mine, l_sum, f[0], 0.f);
+        meet();
+        if (!ok) break;
+        const float4 s0 = stat[row], s1 = stat[BM + row];
+        // a half that saw no key counts for nothing
+        const float m0 = s0.y == 0.f ? -INFINITY : s0.x, m1 = s1.y == 0.f ? -INFINITY : s1.x;
+        m = fmaxf(m0, m1);
+        const float w0 = s0.y == 0.f ? 0.f : ex2f(m0 - m), w1 = s1.y == 0.f ? 0.f : ex2f(m1 - m);
+        l = s0.y * w0 + s1.y * w1;
+        f[0] = s0.z * w0;
+        f[1] = s1.z * w1;
+      } else if (l == 0.f) {
+        m = -INFINITY;
+      }
+      const bool whole = w.tile0 == 0 && w.n == c.kt;
+      float* part = p.partials + ((size_t)blockIdx.x * 2 + (c.first_item ? 0 : 1)) * partial_floats(kRows, D);
+      const int part_row = (PAIR ? q * BM : 0) + row;
+      const bool has_rows = PAIR ? q * BM < w.rows : true;
+      if (has_rows) {
+        const bool bad = bad_values[items & 7] == (uint32_t)items + 1;
+        constexpr int kChunks = D / 32 / (PAIR ? 1 : 2);  // of 32 columns: each group stores half where they share the rows
+        for (int x = PAIR ? 0 : q * kChunks; x < (PAIR ? kChunks : (q + 1) * kChunks); ++x) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_ld_32x32b_x32(tmem_base + 256 + (PAIR ? q * 128 : 0) + lane_addr + x * 32, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = f[0] == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * f[0]);
+          if (!PAIR && w.nq[1] > 0) {
+            uint32_t o1[32];
+            tmem_ld_32x32b_x32(tmem_base + 256 + 128 + lane_addr + x * 32, o1);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              o[e] = f[1] == 0.f ? o[e] : __float_as_uint(fmaf(__uint_as_float(o1[e]), f[1], __uint_as_float(o[e])));
+          }
+          if (bad && valid) {
+            // infinities and NaN that were taken out of the values of partly seen tiles: rows that see them get them
+            for (int key = max(w.tile0, w.first_masked) * BN; key < min(w.keys, (w.tile0 + w.n) * BN); ++key) {
+              if (!sees(p, seq, i_new, key - seq.length)) continue;
+              const int page = __ldg(p.t.table + c.b * p.t.stride + (key >> p.t.page_log2));
+              if (page < 0 || page >= p.t.pages) continue;
+              const int64_t at = ((((int64_t)page * p.t.heads + c.h) << p.t.page_log2) + (key & (p.t.page - 1))) * D + x * 32;
+              for (int e = 0; e < 32; ++e) {
+                float v = 0.f;
+                if (E4M3) {
+                  if ((__ldg(static_cast<const uint8_t*>(p.v_pages) + at + e) & 0x7f) == 0x7f) v = __uint_as_float(0x7fc00000u);
+                } else {
+                  const uint16_t bits = __ldg(static_cast<const uint16_t*>(p.v_pages) + at + e);
+                  const uint16_t expo = MBF16 ? 0x7f80 : 0x7c00;
+                  if ((bits & expo) == expo) v = MBF16 ? __uint_as_float((uint32_t)bits << 16) : __half2float(__ushort_as_half(bits));
+                }
+                if (v != 0.f) {
+#pragma unroll
+                  for (int y = 0; y < 32; ++y)
+                    if (y == e) o[y] = __float_as_uint(__uint_as_float(o[y]) + v);
+                }
+              }
+            }
+          }
+          if (valid) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float4 v = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+              if (whole) store_row4<QBF16, E4M3>(p, seq.first, c.h, r, x * 8 + e, v, l);
+              else __stcg(reinterpret_cast<float4*>(part + (size_t)part_row * D) + x * 8 + e, v);
+            }
+          }
+        }
+        if (!whole && valid && (PAIR || q == 0)) {
+          __stcg(part + (size_t)kRows * D + part_row, m);
+          __stcg(part + (size_t)kRows * D + kRows + part_row, l);
+        }
+      }
+      ++items;
+      infos += PAIR ? w.n : n_tiles;
+      if (!PAIR) meet();  // both groups are done with the statistics, the queries and both O
+    }
+  }
+
+  // ------------------------------------------------------------------ teardown
+  if (*abort_flag) {
+    unsigned long long t0 = globaltimer();
+    while (globaltimer() - t0 < 200000ull) __nanosleep(1000);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == kWarpMma) {
+    __syncwarp();
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+template <bool QBF16, bool E4M3, int D, bool PAIR>
+int launch_tiles(frisk_b200_ctx* ctx, const CacheAttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, unsigned grid, cudaStream_t s) {
+  auto kern = cache_attention_tiles_kernel<QBF16, E4M3, D, PAIR>;
+  using L = TilesSmem<D, E4M3, PAIR>;
+  static PerDeviceOnce opt_in;
+  const int rc = opt_in(ctx->device, [&] {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) != cudaSuccess) return (int)FRISK_B200_E_CUDA;
+    // setmaxnreg.inc waits until the CTA's own registers hold the request: what the launch brings must cover both shares
+    cudaFuncAttributes a;
+    if (cudaFuncGetAttributes(&a, kern) != cudaSuccess) return (int)FRISK_B200_E_CUDA;
+    const int other = threads_of<E4M3>() - 256;
+    return a.numRegs * threads_of<E4M3>() >= 256 * regs_softmax<E4M3>() + other * regs_other<E4M3>() ? 0 : (int)FRISK_B200_E_UNSUPPORTED;
+  });
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel waits (griddepcontrol.wait) itself
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads_of<E4M3>());
+  cfg.dynamicSmemBytes = L::kTotal;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  FB_CUDA(ctx, cudaLaunchKernelEx(&cfg, kern, tk, tv, p));
+  return 0;
+}
+
+template <bool PAIR>
+int launch_any(frisk_b200_ctx* ctx, const CacheAttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, unsigned grid, bool bf16, bool e4m3,
+               int D, cudaStream_t s) {
+  if (D == 64)
+    return bf16 ? (e4m3 ? launch_tiles<true, true, 64, PAIR>(ctx, p, tk, tv, grid, s) : launch_tiles<true, false, 64, PAIR>(ctx, p, tk, tv, grid, s))
+                : (e4m3 ? launch_tiles<false, true, 64, PAIR>(ctx, p, tk, tv, grid, s) : launch_tiles<false, false, 64, PAIR>(ctx, p, tk, tv, grid, s));
+  return bf16 ? (e4m3 ? launch_tiles<true, true, 128, PAIR>(ctx, p, tk, tv, grid, s) : launch_tiles<true, false, 128, PAIR>(ctx, p, tk, tv, grid, s))
+              : (e4m3 ? launch_tiles<false, true, 128, PAIR>(ctx, p, tk, tv, grid, s) : launch_tiles<false, false, 128, PAIR>(ctx, p, tk, tv, grid, s));
+}
+
+}  // namespace
+
+int launch_cache_attention_tiles(frisk_b200_ctx* ctx, const cache::CacheAttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv,
+                                 unsigned grid, bool bf16, bool e4m3, int D, int tile_rows, cudaStream_t s) {
+  return tile_rows == 256 ? launch_any<true>(ctx, p, tk, tv, grid, bf16, e4m3, D, s) : launch_any<false>(ctx, p, tk, tv, grid, bf16, e4m3, D, s);
+}
+
+}  // namespace fb

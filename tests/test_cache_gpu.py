@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 class Batch:
     """Ragged sequences over shuffled pages.  Pages that no sequence has, and page rows behind the keys, hold NaN."""
 
-    def __init__(self, counts, lengths, hkv, group, d, page, dtype, held=None, seed=0, gap=0, fill=True):
+    def __init__(self, counts, lengths, hkv, group, d, page, dtype, held=None, seed=0, gap=0, fill=True, scales=(120, 134)):
         import torch
         g = torch.Generator().manual_seed(seed)
         self.dtype, self.page = dtype, page
@@ -36,7 +36,7 @@ class Batch:
             for i in range(2):
                 where = (table[b].long()[j // page], slice(None), j % page)
                 cache[i][where] = torch.randn(len(j), hkv, d, generator=g)
-                exps[i][where] = torch.randint(120, 134, (len(j), hkv), generator=g, dtype=torch.uint8)
+                exps[i][where] = torch.randint(*scales, (len(j), hkv), generator=g, dtype=torch.uint8)
         if held == torch.float8_e4m3fn:
             cache = [torch.where(torch.isnan(c), c, (c * 100).clamp(-448, 448)).to(held) for c in cache] + exps
             if not fill:
@@ -185,10 +185,11 @@ ATTEND = [  # counts, lengths, key heads, group, d, page
 
 @pytest.mark.parametrize("counts,lengths,hkv,group,d,page", ATTEND)
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
-@pytest.mark.parametrize("e4m3", [False, True])
-def test_attention(counts, lengths, hkv, group, d, page, dtype, e4m3):
+@pytest.mark.parametrize("scales", [None, (120, 134), (116, 122)])  # of an 8-bit cache: far apart, near each other
+def test_attention(counts, lengths, hkv, group, d, page, dtype, scales):
     import torch
-    b = Batch(counts, lengths, hkv, group, d, page, getattr(torch, dtype), torch.float8_e4m3fn if e4m3 else None, 3, gap=1)
+    held = torch.float8_e4m3fn if scales else None
+    b = Batch(counts, lengths, hkv, group, d, page, getattr(torch, dtype), held, 3, gap=1, scales=scales or (0, 1))
     first = attend(b)
     again = attend(b)
     assert torch.equal(bits(first), bits(again))
@@ -200,7 +201,7 @@ def test_attention(counts, lengths, hkv, group, d, page, dtype, e4m3):
 @pytest.mark.parametrize("e4m3", [False, True])
 def test_rows_that_see_nothing_are_zero(e4m3):
     import torch
-    for count in (6, 40):
+    for count in (6, 20, 40):
         b = Batch([count, 3], [0, 0], 2, 4, 64, 16, torch.float16, torch.float8_e4m3fn if e4m3 else None, 5)
         out = attend(b, mask=torch.zeros(b.rows, 4, dtype=torch.bool))
         assert not out.any()
@@ -213,7 +214,7 @@ def test_rows_that_see_nothing_are_zero(e4m3):
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
 @pytest.mark.parametrize("e4m3", [False, True])
-@pytest.mark.parametrize("count", [4, 40])
+@pytest.mark.parametrize("count", [4, 20, 40])
 def test_what_a_row_does_not_see_does_not_reach_it(dtype, e4m3, count):
     """Keys and values of new tokens that are infinite, NaN or large: rows that see them get what the formula gives."""
     import torch
@@ -252,7 +253,7 @@ def test_what_a_row_does_not_see_does_not_reach_it(dtype, e4m3, count):
 @pytest.mark.parametrize("e4m3", [False, True])
 def test_wide_ranges_of_scores_and_values(e4m3):
     import torch
-    for count in (1, 3, 40):
+    for count in (1, 3, 12, 40, 130):
         b = Batch([count], [300], 1, 2, 64, 32, torch.bfloat16, torch.float8_e4m3fn if e4m3 else None, 7)
         cpu = [t.clone() for t in b.cpu]
         g = torch.Generator().manual_seed(1)
