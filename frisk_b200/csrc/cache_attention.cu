@@ -23,6 +23,7 @@
 // K and V tiles arrive by TMA, page by page, in a ring; four warps take 16 keys of a tile each (mma.sync 16x8x16).
 // Every mbarrier wait is bounded (ptx.cuh); no TMA load uses cluster multicast.
 #include <algorithm>
+#include <cfloat>
 
 #include "attention_common.cuh"
 #include "cache_attention.cuh"
@@ -33,24 +34,40 @@ namespace {
 using namespace attn;
 using namespace cache;
 
-constexpr int kKeys = 64;    // of a tile
-constexpr int kWarps = 4;    // consumers
-constexpr int kThreadsRow = 32 * (kWarps + 1);
+constexpr int kKeys = 64;  // of a tile
+constexpr int kRows = 16;  // query rows, padded
 
-template <int D, bool E4M3, int MT>
+// Consumer warps: four share a tile; with 8-bit caches two fours take the tiles in turn, since a tile comes in half the time and has
+// its codes to convert (32 sequences of 8000 keys, 4 rows a head: 240 us with one four).
+template <bool E4M3> constexpr int warps_of() { return E4M3 ? 8 : 4; }
+
+// ones in the elements of `w` (codes, or 16-bit floats) that are infinite or NaN
+template <bool E4M3, bool BF16>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  if (E4M3) return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
+  const uint32_t mask = BF16 ? 0x7f807f80u : 0x7c007c00u;
+  return __vcmpeq2(w & mask, mask);
+}
+template <bool BF16>
+__device__ __forceinline__ float unpack1(uint16_t w) {
+  return BF16 ? __uint_as_float((uint32_t)w << 16) : __half2float(__ushort_as_half(w));
+}
+
+template <int D, bool E4M3>
 struct RowSmem {
-  static constexpr int kRows = 16 * MT;
+  static constexpr int kWarps = warps_of<E4M3>();
   static constexpr int kTile = kKeys * D * (E4M3 ? 1 : 2);
   static constexpr int kStage = 2 * kTile;
-  static constexpr int kFloats = kWarps * kRows * D;            // fp32 O of the four warps, where they meet
-  static constexpr int kRoom = 232448 - 1024 - 2048 - kFloats * 4 - 2 * kWarps * kRows * 4;
-  static constexpr int kStages = (kRoom / (kStage + (E4M3 ? 128 : 0))) > 12 ? 12 : kRoom / (kStage + (E4M3 ? 128 : 0));
+  static constexpr int kFloats = kWarps * kRows * D;            // fp32 O of the warps, where they meet
+  static constexpr int kRoom = 232448 - 1024 - 512 - kFloats * 4 - 2 * kWarps * kRows * 4;
+  static constexpr int kFit = kRoom / (kStage + (E4M3 ? 128 : 0));
+  static constexpr int kStages = kFit > 12 ? 12 : E4M3 ? kFit / 2 * 2 : kFit;  // (8-bit: a stage belongs to one of the two fours)
   static constexpr int kExp = kStages * kStage;                 // [stages][K 64, V 64] exponents
   static constexpr int kO = kExp + (E4M3 ? kStages * 128 : 0);
-  static constexpr int kStat = kO + kFloats * 4;                // [4][rows] maxima, [4][rows] sums
+  static constexpr int kStat = kO + kFloats * 4;                // [warps][rows] maxima, [warps][rows] sums
   static constexpr int kBar = kStat + 2 * kWarps * kRows * 4;
-  static constexpr int kTotal = kBar + 1024 + 1024;
-  static_assert(kTotal <= 232448 && kStages >= 3 && kStages <= 12, "ring and reduction area must fit");
+  static constexpr int kTotal = kBar + 512 + 1024;
+  static_assert(kTotal <= 232448 && kStages >= 4 && kStages <= 12, "ring and reduction area must fit");
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -82,41 +99,30 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// 0xffff in the halves of `w` that are infinite or NaN
-template <bool BF16>
-__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-  const uint32_t mask = BF16 ? 0x7f807f80u : 0x7c007c00u;
-  return __vcmpeq2(w & mask, mask);
-}
-// 1.0 in the halves that `m` selects
-template <bool BF16>
-__device__ __forceinline__ uint32_t ones_of(uint32_t m) {
-  return m & (BF16 ? 0x3f803f80u : 0x3c003c00u);
-}
-
 // QBF16: type of the queries and results.  E4M3: 8-bit cache, products in halves; else the cache has the queries' type.
-template <bool QBF16, bool E4M3, int D, int MT>
-__global__ void __launch_bounds__(kThreadsRow, 1)
+template <bool QBF16, bool E4M3, int D>
+__global__ void __launch_bounds__(32 * (warps_of<E4M3>() + 1), 1)
     cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                            const CacheAttnParams p) {
-  using L = RowSmem<D, E4M3, MT>;
+  using L = RowSmem<D, E4M3>;
   constexpr bool MBF16 = QBF16 && !E4M3;  // type of the products' operands
-  constexpr int kRows = L::kRows;
+  constexpr int kWarps = L::kWarps, kThreads = 32 * (kWarps + 1);
   constexpr int kBoxes = E4M3 ? 1 : D / 64, kBoxBytes = kKeys * 128;
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::kBar);
   uint64_t* empty_bar = full_bar + L::kStages;
-  uint64_t* meet_bar = empty_bar + L::kStages;  // the 128 consumer threads among themselves
+  uint64_t* meet_bar = empty_bar + L::kStages;  // the consumer threads among themselves
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(meet_bar + 1);
   PlanShared* plan_shared = reinterpret_cast<PlanShared*>(meet_bar + 2);
+  static_assert((2 * L::kStages + 3) * 8 + sizeof(PlanShared) <= 512, "barriers and plan must fit");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kStages; ++i) {
-      mbar_init(&full_bar[i], 1);
-      mbar_init(&empty_bar[i], kWarps);
+      mbar_init(&full_bar[i], E4M3 ? 1 + 32 : 1);  // (the lanes that copy exponents arrive, too)
+      mbar_init(&empty_bar[i], 4);
     }
     mbar_init(meet_bar, kWarps * 32);
     *abort_flag = 0;
@@ -127,51 +133,46 @@ __global__ void __launch_bounds__(kThreadsRow, 1)
   // Launched with programmatic stream serialization: the set-up above may overlap the kernel before this one.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Plan plan = make_plan<kThreadsRow>(p, kRows, plan_shared);
+  const Plan plan = make_plan<kThreads>(p, kRows, plan_shared);
 
   if (warp == kWarps) {
-    // ------------------------------------------------------------------ TMA producer: the warp reads the table, lane 0 loads
+    // ------------------------------------------------------------------ TMA producer
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
     const int box = min(p.t.page, kKeys);  // rows a load brings
+    PageWalk walk;
     for (Cursor c(p, plan, kRows); c.left > 0 && ok; c.next_item(p, kRows)) {
-      const int tiles = c.tiles_here();
-      const int keys = c.seq.length + c.seq.count;
-      const int* row = p.t.table + c.b * p.t.stride;
-      int ids = 0, ids_from = -32;  // pages ids_from + lane
-      for (int tile = c.tile; tile < c.tile + tiles; ++tile) {
+      const int end = c.tile + c.tiles_here(), keys = c.seq.length + c.seq.count;
+      walk.enter(p, p.t.table + c.b * p.t.stride, keys, c.h, c.tile, lane);
+      for (int tile = c.tile; tile < end; ++tile) {
+        const int token = walk.token(p, tile, lane);
+        if (tile + 1 < end) walk.look_up(p, tile + 1, lane);
         const int n_boxes = min(kKeys / box, (keys - tile * kKeys + box - 1) / box);
         if (!mbar_wait_warp(&empty_bar[stage], phase ^ 1, abort_flag, p.status, ST_CACHE_KV)) {
           ok = false;
           break;
         }
         unsigned char* sk = smem + stage * L::kStage;
-        unsigned char* se = smem + L::kExp + stage * 128;
-        if (lane == 0) mbar_expect_tx(&full_bar[stage], (uint32_t)n_boxes * box * 2 * (D * (E4M3 ? 1 : 2) + (E4M3 ? 1 : 0)));
-        for (int x = 0; x < n_boxes; ++x) {
-          const int key = tile * kKeys + x * box, at = key >> p.t.page_log2;
-          if (at < ids_from || at >= ids_from + 32) {
-            ids_from = at;
-            ids = at + lane < p.t.width ? __ldg(row + at + lane) : 0;
-          }
-          int page = __shfl_sync(0xffffffffu, ids, at - ids_from);
-          if (page < 0 || page >= p.t.pages) {  // (page 0 is read in its place)
-            if (lane == 0) atomicCAS(p.status, 0u, ST_CACHE_PAGE);
-            page = 0;
-          }
-          if (lane == 0) {
-            const int token = ((page * p.t.heads + c.h) << p.t.page_log2) + (key & (p.t.page - 1));
-            const int at_row = E4M3 && D == 64 ? token / 2 : token;  // (two 64-byte rows make a line of the 8-bit map)
-            const int off = x * box * (E4M3 ? D : 128);
+        if (elect_one()) mbar_expect_tx(&full_bar[stage], (uint32_t)n_boxes * box * 2 * D * (E4M3 ? 1 : 2));
+        __syncwarp();
+        if (E4M3) {
+          unsigned char* se = smem + L::kExp + stage * 128;
+          if (lane < 8 && tile * kKeys + (lane & 3) * 16 < keys)
+            copy16(se + lane * 16, (lane < 4 ? p.k_exponent : p.v_exponent) + token);
+          copies_arrive(&full_bar[stage]);
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if (x >= n_boxes) break;
+          const int at = uniform_of(token, x * (box >> 4), lane);
+          const int row = E4M3 && D == 64 ? at / 2 : at;  // (two 64-byte rows make a line of the 8-bit map)
+          const int off = x * box * (E4M3 ? D : 128);
+          if (elect_one()) {
 #pragma unroll
             for (int b = 0; b < kBoxes; ++b) {
-              tma_load_2d(sk + b * kBoxBytes + off, &tmap_k, &full_bar[stage], b * 64, at_row);
-              tma_load_2d(sk + L::kTile + b * kBoxBytes + off, &tmap_v, &full_bar[stage], b * 64, at_row);
-            }
-            if (E4M3) {
-              bulk_load(se + x * box, p.k_exponent + token, box, &full_bar[stage]);
-              bulk_load(se + 64 + x * box, p.v_exponent + token, box, &full_bar[stage]);
+              tma_load_2d(sk + b * kBoxBytes + off, &tmap_k, &full_bar[stage], b * 64, row);
+              tma_load_2d(sk + L::kTile + b * kBoxBytes + off, &tmap_v, &full_bar[stage], b * 64, row);
             }
           }
         }
@@ -184,6 +185,7 @@ __global__ void __launch_bounds__(kThreadsRow, 1)
   } else {
     // ------------------------------------------------------------------ consumers
     const int g = lane >> 2, tq = lane & 3;  // fragment coordinates: rows g and g + 8, column pair tq
+    const int four = warp >> 2, part_keys = (warp & 3) * 16;  // which tiles, which of their keys
     float* s_o = reinterpret_cast<float*>(smem + L::kO);
     float* s_m = reinterpret_cast<float*>(smem + L::kStat);
     float* s_l = s_m + kWarps * kRows;
@@ -197,10 +199,11 @@ __global__ void __launch_bounds__(kThreadsRow, 1)
     // Which of its 8 keys a column of a score tile is.  8-bit keys of 128 bytes: a quarter-warp reads 16 bytes of two keys, which the
     // 128-byte swizzle keeps in different banks where the keys are 4 apart; keys of 64 bytes lie side by side in a line.
     auto key_of = [](int col) { return E4M3 && D == 128 ? ((col & 1) << 2) | (col >> 1) : col; };
+    // Column of element i of product tile n, first or second of the lane's pair (8-bit: see below)
+    auto column_of = [&](int n, int i) { return E4M3 ? (n >> 1) * 16 + 4 * tq + 2 * (i & 1) + (n & 1) : n * 8 + 2 * tq + (i & 1); };
     const int mat = lane >> 3, mrow = lane & 7;
-    const int k_row = warp * 16 + (mat >> 1) * 8 + mrow, v_row = warp * 16 + (mat & 1) * 8 + mrow;  // 16-bit ldmatrix rows
-    int stage = 0;
-    uint32_t phase = 0;
+    const int k_row = part_keys + (mat >> 1) * 8 + mrow, v_row = part_keys + (mat & 1) * 8 + mrow;  // 16-bit ldmatrix rows
+    unsigned ring = 0;  // stages so far, over all items
 
     for (Cursor c(p, plan, kRows); c.left > 0 && ok; c.next_item(p, kRows)) {
       const int tile0 = c.tile, tile1 = c.tile + c.tiles_here();
@@ -209,285 +212,269 @@ __global__ void __launch_bounds__(kThreadsRow, 1)
       const int rows_here = min(kRows, seq.count * p.group - c.rt * kRows);
       const int row0 = c.rt * kRows;
 
-      uint32_t qf[MT][D / 16][4];
-      float row_scale[MT][2];  // of scores, to log2 units
-      int token[MT][2];        // the row's new token, in its sequence
+      uint32_t qf[D / 16][4];
+      float row_scale[2];  // of scores, to log2 units
+      int token[2];        // the row's new token, in its sequence
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int h = 0; h < 2; ++h) {
+        const int row = h * 8 + g, r = row0 + row;
+        const int i = r / p.group;
+        const bool real = row < rows_here;
+        token[h] = real ? i : 0;
+        const uint16_t* q = static_cast<const uint16_t*>(p.q) + (int64_t)(seq.first + i) * p.q_row +
+                            (int64_t)(c.h * p.group + r - i * p.group) * p.q_head;
+        row_scale[h] = p.scale_log2;
+        if (!E4M3) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = mt * 16 + h * 8 + g, r = row0 + row;
-          const int i = r / p.group;
-          const bool real = row < rows_here;
-          token[mt][h] = real ? i : 0;
-          const uint16_t* q = static_cast<const uint16_t*>(p.q) + (int64_t)(seq.first + i) * p.q_row +
-                              (int64_t)(c.h * p.group + r - i * p.group) * p.q_head;
-          row_scale[mt][h] = p.scale_log2;
-          if (!E4M3) {
+          for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
+            for (int x = 0; x < 2; ++x) qf[kk][h + 2 * x] = real ? __ldg(reinterpret_cast<const uint32_t*>(q) + kk * 8 + x * 4 + tq) : 0u;
+        } else {
+          // this lane's elements of the row: 16 from every 64, so that 16 neighbouring bytes of a key are its part of four products
+          uint32_t w[D / 64][8];
 #pragma unroll
-              for (int x = 0; x < 2; ++x)
-                qf[mt][kk][h + 2 * x] = real ? __ldg(reinterpret_cast<const uint32_t*>(q) + kk * 8 + x * 4 + tq) : 0u;
-          } else {
-            // this lane's elements of the row: 16 from every 64, so that 16 neighbouring bytes of a key are its part of four products
-            uint32_t w[D / 64][8];
-#pragma unroll
-            for (int b = 0; b < D / 64; ++b) {
-              const uint4* from = reinterpret_cast<const uint4*>(q + b * 64 + tq * 16);
-              const uint4 lo = real ? __ldg(from) : make_uint4(0, 0, 0, 0), hi = real ? __ldg(from + 1) : make_uint4(0, 0, 0, 0);
-              w[b][0] = lo.x; w[b][1] = lo.y; w[b][2] = lo.z; w[b][3] = lo.w;
-              w[b][4] = hi.x; w[b][5] = hi.y; w[b][6] = hi.z; w[b][7] = hi.w;
-            }
-            if (QBF16) {
-              // to halves, with the row's largest magnitude in [1, 2): what is 2^14 below it loses bits, at 2^-25 of it
-              uint32_t most = 0;
-#pragma unroll
-              for (int b = 0; b < D / 64; ++b)
-#pragma unroll
-                for (int n = 0; n < 8; ++n) most = max(most, max(w[b][n] & 0x7fffu, (w[b][n] >> 16) & 0x7fffu));
-              most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-              most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-              const uint32_t e = min(max(most >> 7, 1u), 253u);
-              const float down = __uint_as_float((254u - e) << 23);
-              row_scale[mt][h] *= __uint_as_float(e << 23);
-#pragma unroll
-              for (int b = 0; b < D / 64; ++b)
-#pragma unroll
-                for (int n = 0; n < 8; ++n)
-                  w[b][n] = pack16<false>(__uint_as_float(w[b][n] << 16) * down, __uint_as_float(w[b][n] & 0xffff0000u) * down);
-            }
+          for (int b = 0; b < D / 64; ++b) {
+            const uint4* from = reinterpret_cast<const uint4*>(q + b * 64 + tq * 16);
+            const uint4 lo = real ? __ldg(from) : make_uint4(0, 0, 0, 0), hi = real ? __ldg(from + 1) : make_uint4(0, 0, 0, 0);
+            w[b][0] = lo.x; w[b][1] = lo.y; w[b][2] = lo.z; w[b][3] = lo.w;
+            w[b][4] = hi.x; w[b][5] = hi.y; w[b][6] = hi.z; w[b][7] = hi.w;
+          }
+          if (QBF16) {
+            // to halves, with the row's largest magnitude in [1, 2): what is 2^14 below it loses bits, at 2^-25 of it
+            uint32_t most = 0;
 #pragma unroll
             for (int b = 0; b < D / 64; ++b)
 #pragma unroll
-              for (int n = 0; n < 8; ++n) qf[mt][b * 4 + (n >> 1)][h + 2 * (n & 1)] = w[b][n];
+              for (int n = 0; n < 8; ++n) most = max(most, max(w[b][n] & 0x7fffu, (w[b][n] >> 16) & 0x7fffu));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const uint32_t e = min(max(most >> 7, 1u), 253u);
+            const float down = __uint_as_float((254u - e) << 23);
+            row_scale[h] *= __uint_as_float(e << 23);
+#pragma unroll
+            for (int b = 0; b < D / 64; ++b)
+#pragma unroll
+              for (int n = 0; n < 8; ++n)
+                w[b][n] = pack16<false>(__uint_as_float(w[b][n] << 16) * down, __uint_as_float(w[b][n] & 0xffff0000u) * down);
           }
-        }
-      float o[MT][D / 8][4];
-      float m_ref[MT][2], l_sum[MT][2], a_ref[MT][2];  // rows g and g + 8 (l: this lane's columns)
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
+          for (int b = 0; b < D / 64; ++b)
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[mt][n][i] = 0.f;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          m_ref[mt][h] = a_ref[mt][h] = -INFINITY;
-          l_sum[mt][h] = 0.f;
+            for (int n = 0; n < 8; ++n) qf[b * 4 + (n >> 1)][h + 2 * (n & 1)] = w[b][n];
         }
       }
+      float o[D / 8][4];
+      float m_ref[2], l_sum[2], a_ref[2];  // rows g and g + 8 (l: this lane's columns)
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        m_ref[h] = a_ref[h] = -INFINITY;
+        l_sum[h] = 0.f;
+      }
 
-      for (int tile = tile0; tile < tile1; ++tile) {
-        if (!mbar_wait_warp(&full_bar[stage], phase, abort_flag, p.status, ST_CACHE_KV)) {
+      for (int tile = tile0; tile < tile1; ++tile, ++ring) {
+        if (E4M3 && (ring & 1) != (unsigned)four) continue;
+        const int stage = (int)(ring % L::kStages);
+        if (!mbar_wait_warp(&full_bar[stage], (ring / L::kStages) & 1, abort_flag, p.status, ST_CACHE_KV)) {
           ok = false;
           break;
         }
         const uint32_t sk = smem_u32(smem + stage * L::kStage), sv = sk + L::kTile;
-        float s[MT][2][4];
+        float s[2][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[mt][n][i] = 0.f;
+          for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
         float v_exp[2][2];  // 8-bit: log2 of the scale of this lane's values, by n and column
         if (!E4M3) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             uint32_t kf[4];
             ldsm4(kf, sk + (kk >> 2) * kBoxBytes + k_row * 128 + ((((kk & 3) * 2 + (mat & 1)) ^ mrow) << 4));
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              mma16816<MBF16>(s[mt][0], qf[mt][kk], kf[0], kf[1]);
-              mma16816<MBF16>(s[mt][1], qf[mt][kk], kf[2], kf[3]);
-            }
+            mma16816<MBF16>(s[0], qf[kk], kf[0], kf[1]);
+            mma16816<MBF16>(s[1], qf[kk], kf[2], kf[3]);
           }
-        } else {
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const int key = warp * 16 + n * 8 + key_of(g);
-#pragma unroll
-            for (int b = 0; b < D / 64; ++b) {
-              const uint32_t at = key * D + b * 64 + tq * 16;
-              const uint4 raw = lds128(sk + (at ^ (((at >> 7) & 7) << 4)));
-              const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t b0 = e4m3x2_to_half2(w[i]), b1 = e4m3x2_to_half2_hi(w[i]);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) mma16816<false>(s[mt][n], qf[mt][b * 4 + i], b0, b1);
-              }
-            }
-            const unsigned char* se = smem + L::kExp + stage * 128 + warp * 16 + n * 8;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const int at = key_of(2 * tq + x);
-              const float k_scale = scale_of(se[at]);
-              const unsigned e = se[64 + at];
-              v_exp[n][x] = e == 255u ? __uint_as_float(0x7fc00000u) : (float)((int)e - 127);
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                s[mt][n][x] *= k_scale;
-                s[mt][n][2 + x] *= k_scale;
-              }
-            }
-          }
-        }
-        // to log2 units; what a row does not see is -inf, whatever its key holds
-        const bool masked = (tile + 1) * kKeys > seq.length;
-        uint32_t seen = 0xffffffffu;  // bit mt * 8 + n * 4 + i
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[mt][n][i] *= row_scale[mt][i >> 1];
-        if (masked) {
-          seen = 0;
+            for (int i = 0; i < 4; ++i) s[n][i] *= row_scale[i >> 1];
+        } else {
+          uint4 raw[2][D / 64];
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int b = 0; b < D / 64; ++b) {
+              const uint32_t at = (part_keys + n * 8 + key_of(g)) * D + b * 64 + tq * 16;
+              raw[n][b] = lds128(sk + (at ^ (((at >> 7) & 7) << 4)));
+            }
+          float k_scale[2][2];
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const unsigned char* se = smem + L::kExp + stage * 128 + part_keys + n * 8 + key_of(2 * tq + x);
+              k_scale[n][x] = scale_of(se[0]);
+              const unsigned e = se[64];
+              v_exp[n][x] = e == 255u ? __uint_as_float(0x7fc00000u) : (float)((int)e - 127);
+            }
+          float s2[2][4];  // (two chains of products for either n)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s2[n][i] = 0.f;
+#pragma unroll
+          for (int b = 0; b < D / 64; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                const uint32_t w = i == 0 ? raw[n][b].x : i == 1 ? raw[n][b].y : i == 2 ? raw[n][b].z : raw[n][b].w;
+                mma16816<false>(i & 1 ? s2[n] : s[n], qf[b * 4 + i], e4m3x2_to_half2(w), e4m3x2_to_half2_hi(w));
+              }
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][i] = (s[n][i] + s2[n][i]) * k_scale[n][i & 1] * row_scale[i >> 1];
+        }
+        // Scores are in log2 units now.  What a row does not see is -inf, whatever its key holds.  This warp's values are its own: rows
+        // behind the last key become zeros in place, and so do a new token's infinities and NaN, which reach only the rows that see
+        // them: those get them now.  (Their sum is infinite or NaN whatever is added later.)
+        if ((tile + 1) * kKeys > seq.length) {
+          bool see[2][4];
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              see[n][i] = sees(p, seq, token[i >> 1], tile * kKeys + part_keys + n * 8 + key_of(2 * tq + (i & 1)) - seq.length);
+              if (!see[n][i]) s[n][i] = -INFINITY;
+            }
+          unsigned char* v = smem + stage * L::kStage + L::kTile;
+          constexpr int kRowBytes = E4M3 ? D : 2 * D;
+          bool bad = false;
+          for (int e = lane; e < 16 * kRowBytes / 16; e += 32) {
+            const int key = part_keys + e / (kRowBytes / 16), col = e % (kRowBytes / 16) * 16;
+            const uint32_t at = E4M3 ? key * D + col : (col >> 7) * kBoxBytes + key * 128 + (col & 127);
+            uint4* at16 = reinterpret_cast<uint4*>(v + (at ^ (((at >> 7) & 7) << 4)));
+            const uint4 x = *at16;
+            const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+            if (tile * kKeys + key >= keys) {
+              *at16 = make_uint4(0, 0, 0, 0);
+            } else {
+              uint32_t any = 0;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) any |= not_finite<E4M3, MBF16>(y[i]);
+              bad |= any != 0;
+            }
+          }
+          if (__any_sync(0xffffffffu, bad)) {
+            __syncwarp();
+#pragma unroll 1
+            for (int key = part_keys; key < part_keys + 16; ++key) {
+              const int ahead = tile * kKeys + key - seq.length;
+              const bool sees0 = sees(p, seq, token[0], ahead), sees1 = sees(p, seq, token[1], ahead);
+#pragma unroll
+              for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  const int col = column_of(n, i) * (E4M3 ? 1 : 2);
+                  const uint32_t at = E4M3 ? key * D + col : (col >> 7) * kBoxBytes + key * 128 + (col & 127);
+                  const unsigned char* from = v + (at ^ (((at >> 7) & 7) << 4));
+                  float x;
+                  if (E4M3) x = (*from & 0x7f) == 0x7f ? __uint_as_float(0x7fc00000u) : 0.f;
+                  else x = unpack1<MBF16>(*reinterpret_cast<const uint16_t*>(from));
+                  if (!(fabsf(x) <= FLT_MAX)) {
+                    if (sees0) o[n][i] += x;
+                    if (sees1) o[n][2 + i] += x;
+                  }
+                }
+            }
+            __syncwarp();
+            for (int e = lane; e < 16 * kRowBytes / 16; e += 32) {
+              const int key = part_keys + e / (kRowBytes / 16), col = e % (kRowBytes / 16) * 16;
+              const uint32_t at = E4M3 ? key * D + col : (col >> 7) * kBoxBytes + key * 128 + (col & 127);
+              uint4* at16 = reinterpret_cast<uint4*>(v + (at ^ (((at >> 7) & 7) << 4)));
+              const uint4 x = *at16;
+              *at16 = make_uint4(x.x & ~not_finite<E4M3, MBF16>(x.x), x.y & ~not_finite<E4M3, MBF16>(x.y), x.z & ~not_finite<E4M3, MBF16>(x.z),
+                                 x.w & ~not_finite<E4M3, MBF16>(x.w));
+            }
+          }
+          fence_proxy_async_smem();  // (the stage's next load comes after these)
+          __syncwarp();
+        }
+        float m_new[2], a_new[2];
+        bool grow = false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float mx = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+          float mw = -INFINITY;
+          if (E4M3) {
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int ahead = tile * kKeys + warp * 16 + n * 8 + key_of(2 * tq + (i & 1)) - seq.length;
-                const bool see = sees(p, seq, token[mt][i >> 1], ahead);
-                seen |= (see ? 1u : 0u) << (mt * 8 + n * 4 + i);
-                if (!see) s[mt][n][i] = -INFINITY;
-              }
-        }
-        float m_new[MT][2];
-        bool grow = false;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float mx = fmaxf(fmaxf(s[mt][0][2 * h], s[mt][0][2 * h + 1]), fmaxf(s[mt][1][2 * h], s[mt][1][2 * h + 1]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            m_new[mt][h] = fmaxf(m_ref[mt][h], mx);
-            grow |= m_new[mt][h] - m_ref[mt][h] > kRescaleThreshold;  // (false while no key has been seen: -inf - -inf)
+              for (int x = 0; x < 2; ++x) mw = fmaxf(mw, s[n][2 * h + x] + v_exp[n][x]);
           }
-        float a_new[MT][2];
-        if (E4M3) {
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float mx = -INFINITY;
-#pragma unroll
-              for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int x = 0; x < 2; ++x) mx = fmaxf(mx, s[mt][n][2 * h + x] + v_exp[n][x]);
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-              a_new[mt][h] = fmaxf(a_ref[mt][h], mx);
-              grow |= a_new[mt][h] - a_ref[mt][h] > kRescaleThreshold;
-            }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          if (E4M3) mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          m_new[h] = fmaxf(m_ref[h], mx);
+          grow |= m_new[h] - m_ref[h] > kRescaleThreshold;  // (false while no key has been seen: -inf - -inf)
+          if (E4M3) {
+            mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, 2));
+            a_new[h] = fmaxf(a_ref[h], mw);
+            grow |= a_new[h] - a_ref[h] > kRescaleThreshold;
+          }
         }
         if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            float f[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              f[h] = m_ref[mt][h] == -INFINITY ? 0.f : ex2f(m_ref[mt][h] - m_new[mt][h]);
-              m_ref[mt][h] = m_new[mt][h];
-              l_sum[mt][h] *= f[h];
-              if (E4M3) {
-                f[h] = a_ref[mt][h] == -INFINITY ? 0.f : ex2f(a_ref[mt][h] - a_new[mt][h]);
-                a_ref[mt][h] = a_new[mt][h];
-              }
-            }
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n) {
-              o[mt][n][0] *= f[0]; o[mt][n][1] *= f[0];
-              o[mt][n][2] *= f[1]; o[mt][n][3] *= f[1];
-            }
-          }
-        }
-        uint32_t pf[MT][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+          float f[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            // (a row that sees no key yet: keep it finite)
-            const float m0 = m_ref[mt][h] == -INFINITY ? 0.f : m_ref[mt][h], a0 = a_ref[mt][h] == -INFINITY ? 0.f : a_ref[mt][h];
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              float w[2];
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const float sc = s[mt][n][2 * h + x], pr = ex2f(sc - m0);
-                l_sum[mt][h] += pr;
-                // (what is not seen weighs nothing, whatever its value's scale is)
-                w[x] = !E4M3 ? pr : sc == -INFINITY ? 0.f : ex2f(sc + v_exp[n][x] - a0);
-              }
-              pf[mt][n * 2 + h] = pack16<MBF16>(w[0], w[1]);
+            f[h] = m_ref[h] == -INFINITY ? 0.f : ex2f(m_ref[h] - m_new[h]);
+            m_ref[h] = m_new[h];
+            l_sum[h] *= f[h];
+            if (E4M3) {
+              f[h] = a_ref[h] == -INFINITY ? 0.f : ex2f(a_ref[h] - a_new[h]);
+              a_ref[h] = a_new[h];
             }
           }
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            o[n][0] = scaled(o[n][0], f[0]); o[n][1] = scaled(o[n][1], f[0]);
+            o[n][2] = scaled(o[n][2], f[1]); o[n][3] = scaled(o[n][3], f[1]);
+          }
         }
-        // Values behind the last key count as zeros, and a new token's infinities and NaN reach only the rows that see it: they are
-        // taken out of the product, and a product of what each row sees with where they are tells which results they make.
-        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-        if (masked) {
+        uint32_t pf[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          // (a row that sees no key yet: keep it finite)
+          const float m0 = m_ref[h] == -INFINITY ? 0.f : m_ref[h], a0 = a_ref[h] == -INFINITY ? 0.f : a_ref[h];
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
-            const int key = tile * kKeys + warp * 16 + n * 8;
-            keep[n] = (key + key_of(2 * tq) < keys ? 0xffffu : 0u) | (key + key_of(2 * tq + 1) < keys ? 0xffff0000u : 0u);
+            float w[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float sc = s[n][2 * h + x], pr = ex2f(sc - m0);
+              l_sum[h] += pr;
+              // (what is not seen weighs nothing, whatever its value's scale is)
+              w[x] = !E4M3 ? pr : sc == -INFINITY ? 0.f : ex2f(sc + v_exp[n][x] - a0);
+            }
+            pf[n * 2 + h] = pack16<MBF16>(w[0], w[1]);
           }
         }
-        auto times_v = [&](float (&o0)[MT][D / 8][4], int n0, uint32_t b0, uint32_t b1) {
-          if (masked) {
-            b0 &= keep[0];
-            b1 &= keep[1];
-            const uint32_t x0 = not_finite<MBF16>(b0), x1 = not_finite<MBF16>(b1);
-            if (__any_sync(0xffffffffu, (x0 | x1) != 0)) {
-              const uint32_t frac = MBF16 ? 0x007f007fu : 0x03ff03ffu;
-              const uint32_t n_0 = x0 & ~__vcmpeq2(b0 & frac, 0), n_1 = x1 & ~__vcmpeq2(b1 & frac, 0);  // NaN: of both signs
-              const uint32_t s_0 = __vcmpgtu2(b0 & 0x80008000u, 0), s_1 = __vcmpgtu2(b1 & 0x80008000u, 0);
-              const uint32_t pos0 = ones_of<MBF16>(x0 & (~s_0 | n_0)), pos1 = ones_of<MBF16>(x1 & (~s_1 | n_1));
-              const uint32_t neg0 = ones_of<MBF16>(x0 & (s_0 | n_0)), neg1 = ones_of<MBF16>(x1 & (s_1 | n_1));
-              const float inf = __uint_as_float(0x7f800000u);
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                uint32_t sf[4];
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    const uint32_t two = (seen >> (mt * 8 + n * 4 + 2 * h)) & 3u;
-                    sf[n * 2 + h] = ones_of<MBF16>(((two & 1u) ? 0xffffu : 0u) | ((two & 2u) ? 0xffff0000u : 0u));
-                  }
-                float up[4] = {0.f, 0.f, 0.f, 0.f}, down[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16816<MBF16>(up, sf, pos0, pos1);
-                mma16816<MBF16>(down, sf, neg0, neg1);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  if (up[i] > 0.f) o0[mt][n0][i] += inf;
-                  if (down[i] > 0.f) o0[mt][n0][i] -= inf;
-                }
-              }
-              b0 &= ~x0;
-              b1 &= ~x1;
-            }
-          }
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) mma16816<MBF16>(o0[mt][n0], pf[mt], b0, b1);
-        };
         if (!E4M3) {
 #pragma unroll
           for (int j = 0; j < D / 16; ++j) {
             uint32_t vf[4];
             ldsm4_trans(vf, sv + (j >> 2) * kBoxBytes + v_row * 128 + ((((j & 3) * 2 + (mat >> 1)) ^ mrow) << 4));
-            times_v(o, 2 * j, vf[0], vf[1]);
-            times_v(o, 2 * j + 1, vf[2], vf[3]);
+            mma16816<MBF16>(o[2 * j], pf, vf[0], vf[1]);
+            mma16816<MBF16>(o[2 * j + 1], pf, vf[2], vf[3]);
           }
         } else {
           // transposed pairs of codes: a register has the codes of columns 2n, 2n + 1 for two keys.  Even and odd columns go to
           // product tiles of their own: tile 2u has the columns 16u + 2n, tile 2u + 1 the columns 16u + 2n + 1.
-          const int key = warp * 16 + (mat & 1) * 8 + key_of(mrow);
+          const int key = part_keys + (mat & 1) * 8 + key_of(mrow);
 #pragma unroll
           for (int j = 0; j < D / 32; ++j) {
             const uint32_t at = key * D + (2 * j + (mat >> 1)) * 16;
@@ -496,48 +483,41 @@ __global__ void __launch_bounds__(kThreadsRow, 1)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               const uint32_t r0 = __byte_perm(vf[2 * u], 0, 0x3120), r1 = __byte_perm(vf[2 * u + 1], 0, 0x3120);
-              times_v(o, (2 * j + u) * 2, e4m3x2_to_half2(r0), e4m3x2_to_half2(r1));
-              times_v(o, (2 * j + u) * 2 + 1, e4m3x2_to_half2_hi(r0), e4m3x2_to_half2_hi(r1));
+              mma16816<false>(o[(2 * j + u) * 2], pf, e4m3x2_to_half2(r0), e4m3x2_to_half2(r1));
+              mma16816<false>(o[(2 * j + u) * 2 + 1], pf, e4m3x2_to_half2_hi(r0), e4m3x2_to_half2_hi(r1));
             }
           }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty_bar[stage]);
-        if (++stage == L::kStages) {
-          stage = 0;
-          phase ^= 1;
-        }
       }
       if (!ok) break;
 
-      // ---- the four warps' results meet in shared memory
+      // ---- the warps' results meet in shared memory
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float l = l_sum[mt][h];
-          l += __shfl_xor_sync(0xffffffffu, l, 1);
-          l += __shfl_xor_sync(0xffffffffu, l, 2);
-          const int row = mt * 16 + h * 8 + g;
-          if (tq == 0) {
-            s_m[warp * kRows + row] = m_ref[mt][h];
-            s_l[warp * kRows + row] = l;
-          }
-          // columns in blocks of 8, block index xor a function of the row: rows that are stored together fall into different banks
-          float* out = s_o + (warp * kRows + row) * D;
-          if (!E4M3) {
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-              *reinterpret_cast<float2*>(out + ((n ^ (row & 3)) << 3) + 2 * tq) = make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
-          } else {
-            const float f = m_ref[mt][h] == -INFINITY ? 0.f : ex2f(a_ref[mt][h] - m_ref[mt][h]);  // from A's units to m's
-#pragma unroll
-            for (int u = 0; u < D / 16; ++u)
-              *reinterpret_cast<float4*>(out + (((2 * u + (tq >> 1)) ^ (row & 3)) << 3) + (tq & 1) * 4) =
-                  make_float4(o[mt][2 * u][2 * h] * f, o[mt][2 * u + 1][2 * h] * f, o[mt][2 * u][2 * h + 1] * f,
-                              o[mt][2 * u + 1][2 * h + 1] * f);
-          }
+      for (int h = 0; h < 2; ++h) {
+        float l = l_sum[h];
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        const int row = h * 8 + g;
+        if (tq == 0) {
+          s_m[warp * kRows + row] = m_ref[h];
+          s_l[warp * kRows + row] = l;
         }
+        // columns in blocks of 8, block index xor a function of the row: rows that are stored together fall into different banks
+        float* out = s_o + (warp * kRows + row) * D;
+        if (!E4M3) {
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<float2*>(out + ((n ^ (row & 3)) << 3) + 2 * tq) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+        } else {
+          const float f = m_ref[h] == -INFINITY ? 1.f : ex2f(a_ref[h] - m_ref[h]);  // from A's units to m's
+#pragma unroll
+          for (int u = 0; u < D / 16; ++u)
+            *reinterpret_cast<float4*>(out + (((2 * u + (tq >> 1)) ^ (row & 3)) << 3) + (tq & 1) * 4) =
+                make_float4(o[2 * u][2 * h] * f, o[2 * u + 1][2 * h] * f, o[2 * u][2 * h + 1] * f, o[2 * u + 1][2 * h + 1] * f);
+        }
+      }
       meet();
       if (!ok) break;
       const bool whole = tile0 == 0 && tile1 == c.kt;
@@ -557,8 +537,8 @@ __global__ void __launch_bounds__(kThreadsRow, 1)
           const float4 v =
               *reinterpret_cast<const float4*>(s_o + (w * kRows + row) * D + (((c4 >> 1) ^ (row & 3)) << 3) + (c4 & 1) * 4);
           l = fmaf(s_l[w * kRows + row], f, l);
-          acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y);
-          acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+          acc.x += scaled(v.x, f); acc.y += scaled(v.y, f);
+          acc.z += scaled(v.z, f); acc.w += scaled(v.w, f);
         }
         if (whole) {
           store_row4<QBF16, E4M3>(p, seq.first, c.h, row0 + row, c4, acc, l);
@@ -619,7 +599,7 @@ __global__ void __launch_bounds__(128) cache_attention_join_kernel(const CacheAt
         if (fi == 0.f && li == 0.f) continue;  // saw no key of the row
         l = fmaf(li, fi, l);
 #pragma unroll
-        for (int x = 0; x < N; ++x) acc[x] = fmaf(v[x], fi, acc[x]);
+        for (int x = 0; x < N; ++x) acc[x] += scaled(v[x], fi);
       }
     }
     if (N == 4) {
@@ -631,10 +611,10 @@ __global__ void __launch_bounds__(128) cache_attention_join_kernel(const CacheAt
   }
 }
 
-template <bool QBF16, bool E4M3, int D, int MT>
+template <bool QBF16, bool E4M3, int D>
 int launch_rows(frisk_b200_ctx* ctx, const CacheAttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, unsigned grid, cudaStream_t s) {
-  auto kern = cache_attention_kernel<QBF16, E4M3, D, MT>;
-  using L = RowSmem<D, E4M3, MT>;
+  auto kern = cache_attention_kernel<QBF16, E4M3, D>;
+  using L = RowSmem<D, E4M3>;
   static PerDeviceOnce opt_in;
   if (opt_in(ctx->device, [&] {
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) == cudaSuccess ? 0 : 1;
@@ -645,7 +625,7 @@ int launch_rows(frisk_b200_ctx* ctx, const CacheAttnParams& p, const CUtensorMap
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernels wait (griddepcontrol.wait) themselves
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreadsRow);
+  cfg.blockDim = dim3(32 * (L::kWarps + 1));
   cfg.dynamicSmemBytes = L::kTotal;
   cfg.stream = s;
   cfg.attrs = attr;
@@ -657,9 +637,8 @@ int launch_rows(frisk_b200_ctx* ctx, const CacheAttnParams& p, const CUtensorMap
 template <bool QBF16, bool E4M3, int D>
 int launch_all(frisk_b200_ctx* ctx, const CacheAttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, unsigned grid, int tile_rows,
                cudaStream_t s) {
-  const int rc = tile_rows == 16   ? launch_rows<QBF16, E4M3, D, 1>(ctx, p, tk, tv, grid, s)
-                 : tile_rows == 32 ? launch_rows<QBF16, E4M3, D, 2>(ctx, p, tk, tv, grid, s)
-                                   : launch_cache_attention_tiles(ctx, p, tk, tv, grid, QBF16, E4M3, D, tile_rows, s);
+  const int rc = tile_rows == kRows ? launch_rows<QBF16, E4M3, D>(ctx, p, tk, tv, grid, s)
+                                    : launch_cache_attention_tiles(ctx, p, tk, tv, grid, QBF16, E4M3, D, tile_rows, s);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
@@ -696,7 +675,7 @@ int check_attention(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_
 int tile_rows_of(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_desc* a) {
   const int64_t per = a->max_new > 0 ? a->max_new : c->batch > 0 ? (c->rows + c->batch - 1) / c->batch : 1;
   const int64_t rows = per * (a->heads_q / c->heads);
-  return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 128 ? 128 : 256;
+  return rows <= kRows ? kRows : rows <= 128 ? 128 : 256;
 }
 
 }  // namespace

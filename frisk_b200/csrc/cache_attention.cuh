@@ -1,6 +1,8 @@
 // What the kernels of attention over a paged cache share: parameters, how the work is dealt to CTAs, which keys a row sees, how a
 // row's results leave.
 #pragma once
+#include <cfloat>
+
 #include "attention_common.cuh"
 #include "cache_common.cuh"
 #include "work_split.cuh"
@@ -183,6 +185,9 @@ __device__ __forceinline__ bool sees(const CacheAttnParams& p, const Seq& s, int
   return ahead < p.mask_width && __ldg(p.mask + (int64_t)(s.first + i) * p.mask_stride + ahead) != 0;
 }
 
+// x * f, but that what is infinite or NaN stays so where f has vanished
+__device__ __forceinline__ float scaled(float x, float f) { return f == 0.f ? (fabsf(x) <= FLT_MAX ? 0.f : x) : x * f; }
+
 // four results of row r (of the sequence and key head), acc / l; a row that saw nothing is zero
 template <bool QBF16, bool E4M3>
 __device__ __forceinline__ void store_row4(const CacheAttnParams& p, int first, int h, int r, int c4, float4 acc, float l) {
@@ -197,11 +202,44 @@ __device__ __forceinline__ void store_row4(const CacheAttnParams& p, int first, 
   *reinterpret_cast<uint2*>(out + c4 * 4) = make_uint2(attn::pack16<QBF16>(x[0], x[1]), attn::pack16<QBF16>(x[2], x[3]));
 }
 
-// `bytes` (a multiple of 16) from global to shared memory
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
+// 16 bytes from global to shared memory, and this thread's arrival on `bar` (one of its count) when its copies so far are there
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Where a warp that loads key tiles finds their tokens.  A page holds 16 keys at least, so lane l looks up piece l % 4 of 16 keys;
+// the table is read one tile ahead.  What a lane knows becomes an operand of a load by a reduction, whose result the compiler knows
+// to be the same for all lanes (a load costs the issuing warp 60 clk so, 110 with a shuffled operand and one lane's branch).
+struct PageWalk {
+  const int* row;  // of the table
+  int keys, head, id;
+  __device__ __forceinline__ void look_up(const CacheAttnParams& p, int tile, int lane) {
+    const int key = tile * kTileKeys + (lane & 3) * 16;
+    id = key < keys ? __ldg(row + (key >> p.t.page_log2)) : 0;
+  }
+  __device__ __forceinline__ void enter(const CacheAttnParams& p, const int* table_row, int n_keys, int h, int tile, int lane) {
+    row = table_row;
+    keys = n_keys;
+    head = h;
+    look_up(p, tile, lane);
+  }
+  // the token index (page, head, offset) of this lane's piece of the tile
+  __device__ __forceinline__ int token(const CacheAttnParams& p, int tile, int lane) const {
+    const int key = tile * kTileKeys + (lane & 3) * 16;
+    int page = id;
+    if (page < 0 || page >= p.t.pages) {  // (page 0 is read in its place)
+      atomicCAS(p.status, 0u, ST_CACHE_PAGE);
+      page = 0;
+    }
+    return ((page * p.t.heads + head) << p.t.page_log2) + (key & (p.t.page - 1));
+  }
+};
+// lane `from`'s value (not negative), known to be uniform
+__device__ __forceinline__ int uniform_of(int value, int from, int lane) {
+  return (int)__reduce_max_sync(0xffffffffu, lane == from ? (unsigned)value : 0u);
 }
 
 }  // namespace cache

@@ -118,8 +118,9 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 49);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   volatile uint32_t* bad_values = tmem_slot + 2;  // [8] by item: number + 1 of one in which infinities or NaN were taken out of values
-  PlanShared* plan_shared = reinterpret_cast<PlanShared*>(bars + 56);
-  static_assert(56 * 8 + sizeof(PlanShared) <= 1024, "barriers and plan must fit");
+  int* tokens = reinterpret_cast<int*>(bars + 56);  // [8 key tiles][4 pieces of 16 keys] where they are in the cache
+  PlanShared* plan_shared = reinterpret_cast<PlanShared*>(bars + 72);
+  static_assert(72 * 8 + sizeof(PlanShared) <= 1024, "barriers and plan must fit");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto ring_stage = [](int n, int group) -> int { return (OWN_KV ? group * kOwnStages : 0) + n % kOwnStages; };
@@ -132,7 +133,7 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
       if (!E4M3) mbar_init(&fixed[i], 1);
     }
     for (int i = 0; i < L::kRawStages; ++i) {
-      mbar_init(&fixed[i], 1);
+      mbar_init(&fixed[i], 1 + 32);  // (the lanes that copy scales arrive, too)
       mbar_init(&raw_empty[i], 4);
     }
     for (int i = 0; i < 4; ++i) {
@@ -184,63 +185,61 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(regs_other<E4M3>()));
     if (warp == kWarpTma) {
-      // ------------------------------------------------------------------ TMA producer: the warp reads the table, lane 0 loads
+      // ------------------------------------------------------------------ TMA producer
+      // K's tiles come in order, and V's after them: the tokens of the last eight are kept for V.
       int loaded[2] = {0, 0};  // stages filled so far, over all items; OWN_KV: for either MMA warp
       int raws = 0;
       bool ok = true;
+      constexpr int kRawStages = L::kRawStages ? L::kRawStages : 1;
       const int box = min(p.t.page, BN);  // rows a load brings
+      PageWalk walk;
       for (Cursor c(p, plan, kRows); c.left > 0 && ok; c.next_item(p, kRows)) {
         const Work w = work_of(c);
-        const int* row = p.t.table + c.b * p.t.stride;
-        int ids[2] = {0, 0}, from[2] = {-64, -64};  // for K and for V: pages from .. from + 31
-        const int n_keys = w.nq[0];
-        for (int b = -2; b < n_keys && ok; ++b) {
+        walk.enter(p, p.t.table + c.b * p.t.stride, w.keys, c.h, w.tile0, lane);
+        for (int b = -2; b < w.nq[0] && ok; ++b) {
 #pragma unroll
           for (int g = 0; g < (OWN_KV ? 2 : 1); ++g) {
             const bool has_k = b + 2 < w.nq[g], has_v = b >= 0 && b < w.nq[g];
             if (!ok || !(has_k || has_v)) continue;
-            const int st = E4M3 ? raws % (L::kRawStages ? L::kRawStages : 1) : ring_stage(loaded[g], g);
+            const int k_tile = tile_of(w, b + 2, g), v_tile = tile_of(w, b, g);
+            int k_token = 0;
+            if (has_k) {
+              k_token = walk.token(p, k_tile, lane);
+              if (k_tile + 1 < w.tile0 + w.n) walk.look_up(p, k_tile + 1, lane);
+              if (lane < 4) tokens[(k_tile & 7) * 4 + lane] = k_token;
+            }
+            const int v_token = has_v ? tokens[(v_tile & 7) * 4 + (lane & 3)] : 0;
+            const int st = E4M3 ? raws % kRawStages : ring_stage(loaded[g], g);
             uint64_t* const full = E4M3 ? &fixed[st] : &kv_full[st];
-            ok = E4M3 ? mbar_wait_warp(&raw_empty[st], ((raws / (L::kRawStages ? L::kRawStages : 1)) & 1) ^ 1, abort_flag, p.status, ST_CACHE_RAW)
+            ok = E4M3 ? mbar_wait_warp(&raw_empty[st], ((raws / kRawStages) & 1) ^ 1, abort_flag, p.status, ST_CACHE_RAW)
                       : mbar_wait_warp(&kv_empty[st], ring_phase(loaded[g]) ^ 1, abort_flag, p.status, ST_CACHE_KV);
             if (!ok) continue;
             ++loaded[g];
             ++raws;
-            int boxes[2], tile[2];  // K's, V's
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              tile[x] = tile_of(w, x ? b : b + 2, g);
-              boxes[x] = (x ? has_v : has_k) ? min(BN / box, (w.keys - tile[x] * BN + box - 1) / box) : 0;
-            }
-            if (lane == 0)
-              mbar_expect_tx(full, (uint32_t)box * ((boxes[0] + boxes[1]) * D * kElem + (E4M3 ? 2 * boxes[0] + boxes[1] : 0)));
+            const int k_boxes = has_k ? min(BN / box, (w.keys - k_tile * BN + box - 1) / box) : 0;
+            const int v_boxes = has_v ? min(BN / box, (w.keys - v_tile * BN + box - 1) / box) : 0;
+            if (elect_one()) mbar_expect_tx(full, (uint32_t)((k_boxes + v_boxes) * box * D * kElem));
             __syncwarp();
             unsigned char* at = smem + (E4M3 ? L::kRawRing + st * L::kRawTiles : L::kRing + st * L::kStage);
-            unsigned char* scales = smem + L::kRawScales + st * 192;
+            if (E4M3) {
+              // the scales: of the K tile's keys and values, and of the V tile's values
+              unsigned char* scales = smem + L::kRawScales + st * 192;
+              const int piece = (lane & 3) * 16;
+              if (lane < 8 && has_k && k_tile * BN + piece < w.keys)
+                copy16(scales + lane * 16, (lane < 4 ? p.k_exponent : p.v_exponent) + k_token);
+              if (lane < 4 && has_v && v_tile * BN + piece < w.keys) copy16(scales + 128 + lane * 16, p.v_exponent + v_token);
+              copies_arrive(full);
+            }
 #pragma unroll
             for (int x = 0; x < 2; ++x)
-              for (int i = 0; i < boxes[x]; ++i) {
-                const int key = tile[x] * BN + i * box, n = key >> p.t.page_log2;
-                if (n < from[x] || n >= from[x] + 32) {
-                  from[x] = n;
-                  ids[x] = n + lane < p.t.width ? __ldg(row + n + lane) : 0;
-                }
-                int page = __shfl_sync(0xffffffffu, ids[x], n - from[x]);
-                if (page < 0 || page >= p.t.pages) {  // (page 0 is read in its place)
-                  if (lane == 0) atomicCAS(p.status, 0u, ST_CACHE_PAGE);
-                  page = 0;
-                }
-                if (lane == 0) {
-                  const int token = ((page * p.t.heads + c.h) << p.t.page_log2) + (key & (p.t.page - 1));
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (i >= (x ? v_boxes : k_boxes)) break;
+                const int token = uniform_of(x ? v_token : k_token, i * (box >> 4), lane);
+                if (elect_one()) {
                   if (E4M3) {
                     // (two rows of 64 bytes make a line of the map)
                     tma_load_2d(at + x * BN * D + i * box * D, x ? &tmap_v : &tmap_k, full, 0, D == 64 ? token / 2 : token);
-                    if (x == 0) {
-                      bulk_load(scales + i * box, p.k_exponent + token, box, full);
-                      bulk_load(scales + 64 + i * box, p.v_exponent + token, box, full);
-                    } else {
-                      bulk_load(scales + 128 + i * box, p.v_exponent + token, box, full);
-                    }
                   } else {
 #pragma unroll
                     for (int d = 0; d < kBoxes; ++d)
@@ -248,6 +247,7 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
                   }
                 }
               }
+            __syncwarp();
           }
         }
       }
@@ -430,20 +430,25 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
               const unsigned char* from = raw + x * BN * D;
               unsigned char* to = op + x * L::kKv;
               bool bad = false;
-              // 16 codes a step: a lane's neighbours have the 16-byte pieces of the same key
-#pragma unroll 4
-              for (int e = me; e < BN * D / 16; e += 128) {
-                const int key = e / (D / 16), piece = e % (D / 16);
-                const uint32_t off = key * D + piece * 16;
-                const uint4 codes = *reinterpret_cast<const uint4*>(from + (off ^ (((off >> 7) & 7) << 4)));
-                // 2^(e - largest), as a half; 0 for what is no key
-                const uint32_t es = mine[key];
-                const int down = wide ? 0 : (int)top - (int)es;
-                const uint16_t f = key >= left || down > 14 ? 0 : (uint16_t)((15 - down) << 10);
-                const uint32_t f2 = f | ((uint32_t)f << 16);
-                const __half2 scale = *reinterpret_cast<const __half2*>(&f2);
+              // 16 codes a piece; a lane's neighbours have the pieces of the same key.  All loads come before the first store, which the
+              // compiler would not move them across.
+              constexpr int kPieces = BN * D / 16 / 128;
+              uint4 codes[kPieces];
+              uint32_t factor[kPieces];  // 2^(e - largest), a half twice; 0 for what is no key
+#pragma unroll
+              for (int n = 0; n < kPieces; ++n) {
+                const int e = me + n * 128, key = e / (D / 16);
+                const uint32_t off = e * 16;
+                codes[n] = *reinterpret_cast<const uint4*>(from + (off ^ (((off >> 7) & 7) << 4)));
+                const int down = wide ? 0 : (int)top - (int)mine[key];
+                factor[n] = key >= left || down > 14 ? 0u : (uint32_t)(15 - down) * 0x04000400u;
+              }
+#pragma unroll
+              for (int n = 0; n < kPieces; ++n) {
+                const int e = me + n * 128, key = e / (D / 16), piece = e % (D / 16);
+                const __half2 scale = *reinterpret_cast<const __half2*>(&factor[n]);
                 uint32_t out[8];
-                const uint32_t in[4] = {codes.x, codes.y, codes.z, codes.w};
+                const uint32_t in[4] = {codes[n].x, codes[n].y, codes[n].z, codes[n].w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   const uint32_t lo = e4m3x2_to_half2(in[i]), hi = e4m3x2_to_half2_hi(in[i]);
@@ -452,12 +457,12 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
                   out[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&b2);
                 }
                 if (x == 1) {
-                  // codes that are NaN (0x7f, 0xff) come back when O is stored
+                  // codes that are NaN (0x7f, 0xff: adding 1 to the other seven bits carries) come back when O is stored
                   uint32_t nan = 0;
 #pragma unroll
-                  for (int i = 0; i < 4; ++i) nan |= __vcmpeq4(in[i] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                  if (nan || key >= left) {
-                    bad |= nan != 0 && key < left;
+                  for (int i = 0; i < 4; ++i) nan |= (in[i] & 0x7f7f7f7fu) + 0x01010101u;
+                  if ((nan & 0x80808080u) || key >= left) {
+                    bad |= key < left;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) out[i] = key < left ? out[i] & ~__vcmpeq2(out[i] & 0x7c007c00u, 0x7c007c00u) : 0u;
                   }
@@ -599,7 +604,7 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
             tmem_ld_32x32b_x32(t_o + x * 32, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(scaled(__uint_as_float(o[e]), factor));
             tmem_st_32x32b_x32(t_o + x * 32, o);
           }
         };
@@ -643,12 +648,20 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
           uint32_t see[2] = {0, 0};
           const int ahead0 = tile * BN - seq.length;
           const int t0 = __shfl_sync(0xffffffffu, i_new, 0), t1 = __reduce_max_sync(0xffffffffu, i_new);
-          for (int t = min(t0, t1); t <= t1; ++t) {
-            const uint32_t lo = __ballot_sync(0xffffffffu, sees(p, seq, t, ahead0 + lane));
-            const uint32_t hi = __ballot_sync(0xffffffffu, sees(p, seq, t, ahead0 + 32 + lane));
-            if (t == i_new) {
-              see[0] = lo;
-              see[1] = hi;
+          for (int t = min(t0, t1); t <= t1; t += 8) {  // (eight tokens' loads at a time)
+            bool lo[8], hi[8];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+              lo[n] = t + n <= t1 && sees(p, seq, t + n, ahead0 + lane);
+              hi[n] = t + n <= t1 && sees(p, seq, t + n, ahead0 + 32 + lane);
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+              const uint32_t l = __ballot_sync(0xffffffffu, lo[n]), h = __ballot_sync(0xffffffffu, hi[n]);
+              if (t + n == i_new) {
+                see[0] = l;
+                see[1] = h;
+              }
             }
           }
           float mx = -INFINITY, mw = -INFINITY;  // of scores, of scores and scales
