@@ -44,7 +44,8 @@ int encode_tiled(CUtensorMap* out, const TmapKey& k) {
   cuuint32_t box[3] = {k.box[0], k.box[1], k.box[2]};
   cuuint32_t estr[3] = {1, 1, 1};
   return (int)fn(out, tmap_dtype(k.dtype), (cuuint32_t)k.rank, const_cast<void*>(k.base), dims, strides, box, estr,
-                 CU_TENSOR_MAP_INTERLEAVE_NONE, k.swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                 CU_TENSOR_MAP_INTERLEAVE_NONE,
+                 k.swizzle == 1 ? CU_TENSOR_MAP_SWIZZLE_128B : k.swizzle ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE,
                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 // A descriptor depends only on its key (it holds no reference to the memory besides the
@@ -74,6 +75,13 @@ int encode_tmap_2d(frisk_b200_ctx* ctx, CUtensorMap* out, int dtype, const void*
                    uint64_t outer, uint64_t outer_stride_bytes, uint32_t box_inner, uint32_t box_outer,
                    bool swizzle128) {
   TmapKey k{base, {inner, outer, 1}, {outer_stride_bytes, 0}, {box_inner, box_outer, 1}, dtype, 2, swizzle128 ? 1 : 0};
+  return cached_tmap(ctx, out, k);
+}
+
+int encode_tmap_2d(frisk_b200_ctx* ctx, CUtensorMap* out, int dtype, const void* base, uint64_t inner,
+                   uint64_t outer, uint64_t outer_stride_bytes, uint32_t box_inner, uint32_t box_outer,
+                   TmapSwizzle swizzle) {
+  TmapKey k{base, {inner, outer, 1}, {outer_stride_bytes, 0}, {box_inner, box_outer, 1}, dtype, 2, swizzle == TmapSwizzle::k128 ? 1 : 2};
   return cached_tmap(ctx, out, k);
 }
 

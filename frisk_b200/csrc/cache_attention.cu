@@ -719,15 +719,19 @@ extern "C" int frisk_b200_cache_attention(frisk_b200_ctx* ctx, const frisk_b200_
 
   FB_DEVICE(ctx);
   const bool e4m3 = c->dtype == FRISK_B200_E4M3, bf16 = a->dtype == FRISK_B200_BF16;
-  // lines of 128 bytes: one key or half of one at 16 bits, one or two at 8
+  const int tile_rows = tile_rows_of(c, a);
+  // Lines of 128 bytes: one key or half of one at 16 bits, one or two at 8.  (The tensor core wants 8-bit keys of 64 bytes in lines of
+  // their own and the swizzle of that width.)
   const uint64_t tokens = (uint64_t)c->pages * c->heads * c->page;
   const int box_rows = std::min(c->page, kKeys);
   CUtensorMap tk, tv;
   const int map_type = e4m3 ? FRISK_B200_F16 : c->dtype;
-  const uint64_t inner = e4m3 ? 64 : c->D, outer = e4m3 ? tokens * c->D / 128 : tokens;
-  const uint32_t box = e4m3 ? box_rows * c->D / 128 : box_rows;
-  rc = encode_tmap_2d(ctx, &tk, map_type, c->k, inner, outer, inner * 2, 64, box, true);
-  if (!rc) rc = encode_tmap_2d(ctx, &tv, map_type, c->v, inner, outer, inner * 2, 64, box, true);
+  const bool narrow = e4m3 && c->D == 64 && tile_rows > kRows;
+  const uint64_t inner = narrow ? 32 : e4m3 ? 64 : c->D, outer = e4m3 && !narrow ? tokens * c->D / 128 : tokens;
+  const uint32_t box = e4m3 && !narrow ? box_rows * c->D / 128 : box_rows;
+  const TmapSwizzle swizzle = narrow ? TmapSwizzle::k64 : TmapSwizzle::k128;
+  rc = encode_tmap_2d(ctx, &tk, map_type, c->k, inner, outer, inner * 2, narrow ? 32 : 64, box, swizzle);
+  if (!rc) rc = encode_tmap_2d(ctx, &tv, map_type, c->v, inner, outer, inner * 2, narrow ? 32 : 64, box, swizzle);
   if (rc) {
     ctx->last_cuda = rc;
     return FRISK_B200_E_CUDA;
@@ -753,10 +757,9 @@ extern "C" int frisk_b200_cache_attention(frisk_b200_ctx* ctx, const frisk_b200_
   p.status = ctx->d_status;
   const unsigned grid = (unsigned)std::min(ctx->num_sms, kNumSMsDefault);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int rows = tile_rows_of(c, a);
   if (c->D == 64)
-    return bf16 ? (e4m3 ? launch_all<true, true, 64>(ctx, p, tk, tv, grid, rows, s) : launch_all<true, false, 64>(ctx, p, tk, tv, grid, rows, s))
-                : (e4m3 ? launch_all<false, true, 64>(ctx, p, tk, tv, grid, rows, s) : launch_all<false, false, 64>(ctx, p, tk, tv, grid, rows, s));
-  return bf16 ? (e4m3 ? launch_all<true, true, 128>(ctx, p, tk, tv, grid, rows, s) : launch_all<true, false, 128>(ctx, p, tk, tv, grid, rows, s))
-              : (e4m3 ? launch_all<false, true, 128>(ctx, p, tk, tv, grid, rows, s) : launch_all<false, false, 128>(ctx, p, tk, tv, grid, rows, s));
+    return bf16 ? (e4m3 ? launch_all<true, true, 64>(ctx, p, tk, tv, grid, tile_rows, s) : launch_all<true, false, 64>(ctx, p, tk, tv, grid, tile_rows, s))
+                : (e4m3 ? launch_all<false, true, 64>(ctx, p, tk, tv, grid, tile_rows, s) : launch_all<false, false, 64>(ctx, p, tk, tv, grid, tile_rows, s));
+  return bf16 ? (e4m3 ? launch_all<true, true, 128>(ctx, p, tk, tv, grid, tile_rows, s) : launch_all<true, false, 128>(ctx, p, tk, tv, grid, tile_rows, s))
+              : (e4m3 ? launch_all<false, true, 128>(ctx, p, tk, tv, grid, tile_rows, s) : launch_all<false, false, 128>(ctx, p, tk, tv, grid, tile_rows, s));
 }

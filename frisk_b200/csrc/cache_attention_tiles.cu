@@ -9,18 +9,25 @@
 // S = Q.K^T into one of two TMEM buffers a group, P back over its scores as 16-bit pairs, O += P.V from there.  S runs two key tiles ahead of
 // P.V, and a ring stage holds what an MMA warp takes in one step: V of key tile b and K of tile b + 2.
 //
-// 16-bit caches: stages are filled by TMA, page by page.  Key tiles that reach behind lengths[b] are checked by a warp of their own
-// before their values are used: rows behind the last key become zeros, and so do infinities and NaN, because their product with a weight
-// of zero would reach rows that do not see them; if there were any, rows that do see them get them back when O is stored.
+// Stages are filled by TMA, page by page.  Key tiles that reach behind lengths[b] are checked by a warp of their own before their values
+// are used: rows behind the last key become zeros, and so do infinities and NaN, because their product with a weight of zero would reach
+// rows that do not see them; if there were any, rows that do see them get them back when O is stored.
 //
-// 8-bit caches: the raw tiles arrive by TMA and four warps turn them into the operands in halves.  Where the scales of a tile's
-// keys (or of its values) lie within 2^8 of each other they are folded into the halves, exactly, relative to the tile's largest; the
-// largest joins the scale of the scores, and that of the values the exponent of the weights, w = 2^(s + v - A), one number a tile.
-// Other tiles are rare: their keys or values stay unscaled and every score or weight takes its own ("wide").  The row sum is
-// kept in units of 2^B of its own, since the values' scales have no part in it.
+// 8-bit caches: the products take the codes as they are (kind::f8f6f4), and what meets them is written as a sum of e4m3 values, one
+// MMA each.  A query row, scaled by a power of two to at most 256, becomes two terms (bf16) or three (fp16) whose sum is the query but for
+// what lies 2^-19 below the row's largest element.  A weight becomes two: the first has 4 bits, the second 4 of the rest, 2^-8 of the weight
+// in all as with bf16 weights, or 2^-17 of the row's largest: the reference A moves when the maximum grew by more than 2, and the largest
+// weight lies between 2^7 and 2^8.  Converting the codes to halves instead took four warps 1.6 us a tile (2.5 us a tile of 64 rows in all).
+// Keys' scales multiply the scores; values' scales the weights, w = 2^(s + v - A): v is the tile's largest, as one number in the exponent,
+// and a factor for every key relative to it.  The row sum has no part in the values' scales and is kept in units of 2^B of its own.  The
+// checking warp prepares the scales.
 //
-// What bounds it: 16-bit, up to 128 rows, HBM; else the softmax groups (some 1700 clk for 64 keys of 256 rows, of which 1024 exponentials)
-// and, with 8-bit caches, the conversion beside them.
+// Tiles that a row may not see whole, and 8-bit tiles whose values' scales span more than 2^8 ("wide"), take a detour of rolled loops over
+// tensor memory before the common path: hidden scores become -inf there.  (Unrolled, code that runs once an item cost 20 us a tile: it
+// has to be fetched.)
+//
+// What bounds it: up to 128 rows HBM, 0.77 us a 16-bit tile of 64 keys a SM; else the softmax groups (some 1700 clk for 64 keys of 256
+// rows, of which 1024 exponentials).
 // Every mbarrier wait is bounded (ptx.cuh); no TMA load uses cluster multicast.
 #include <algorithm>
 #include <cfloat>
@@ -35,80 +42,77 @@ using namespace attn;
 using namespace cache;
 
 constexpr int BN = kTileKeys;
-constexpr int kWarpFix = 11;     // 16-bit: checks values; 8-bit: idle
-constexpr int kWarpConvert = 12;  // 8-bit: four warps
-constexpr int kInfos = 8;        // key tiles whose scales are kept, for either group
-constexpr uint32_t kFolded = 8;  // log2: scales of a tile that lie this close are folded
+constexpr int kThreadsTiles = 384;  // warps 0-3, 4-7: softmax groups; 8: TMA; 9, 10: MMA; 11: checks values, prepares scales
+constexpr int kWarpFix = 11;
+constexpr int kInfos = 8;            // key tiles whose scales are kept, for either group
+constexpr uint32_t kNarrow = 8;      // log2: scales of a tile's values that lie this close share a reference
+constexpr float kTop8 = 7.f;         // log2 of the 8-bit weight at the reference
+constexpr float kRescale8 = 1.f;     // 8-bit: the reference moves when the maximum grew by more than this
 
-template <bool E4M3> constexpr int threads_of() { return E4M3 ? 512 : 384; }
-template <bool E4M3> constexpr int regs_softmax() { return E4M3 ? 176 : 208; }
-template <bool E4M3> constexpr int regs_other() { return E4M3 ? 80 : 72; }
-
-// the scales of a key tile's keys and values, 8-bit caches
+// the scales of a key tile, 8-bit caches
 struct alignas(16) TileInfo {
-  uint8_t k[64], v[64];
-  float k_scale, v_log2;  // of the folded tile: 2^(largest - 127) of the keys, largest - 127 of the values
-  int wide_k, wide_v;         // not folded: the range of the scales is too large
-};
-
-// The scales of a tile's rows (the first `left` of 64), found by a whole warp: the largest, and whether they span too much to be folded.
-// Rows of zeros, and what is no larger than 2^-117, have the least scale: zero beside any other.
-struct Fold {
-  uint32_t top;
-  bool wide;
-};
-__device__ __forceinline__ Fold fold_of(const uint8_t* scales, int left, int lane) {
-  uint32_t top = 0, low = 255;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t e = lane + 32 * i < left ? scales[lane + 32 * i] : 1u;
-    top = max(top, e);
-    low = min(low, e <= 1u ? 255u : e);
-  }
-  top = __reduce_max_sync(0xffffffffu, top);
-  low = __reduce_min_sync(0xffffffffu, low);
-  if (top <= 1u) top = low = 127;
-  return Fold{top, top - low > kFolded || top > 187u || low < 67u};
-}
-
-template <int D, bool E4M3, bool PAIR>
-struct TilesSmem {
-  static constexpr int kQTile = BM * D * 2;
-  static constexpr int kKv = BN * D * 2;                 // a K or V operand tile
-  static constexpr int kStage = 2 * kKv;                 // K, then V
-    static constexpr int kQTiles = PAIR ? 2 : 1;
-  static constexpr int kStages = E4M3 ? (PAIR ? 3 : 4) : (D == 128 ? (PAIR ? 4 : 6) : 8);
-  static constexpr int kRawStages = E4M3 ? (D == 128 ? 3 : 6) : 0;
-  static constexpr int kRing = kQTiles * kQTile;
-  static constexpr int kRawRing = kRing + kStages * kStage;         // 1024-byte aligned tiles
-  static constexpr int kRawTiles = E4M3 ? 2 * BN * D : 0;
-  static constexpr int kRawScales = kRawRing + kRawStages * kRawTiles;  // [raw stages][K's, its values', V's: 64 each]
-  static constexpr int kInfo = kRawScales + kRawStages * 192;
-  static constexpr int kBar = kInfo + (E4M3 ? 2 * kInfos * (int)sizeof(TileInfo) : 0);
-  static constexpr int kTotal = kBar + 1024 + 1024;
-  static_assert(kTotal <= 232448, "rings and tiles must fit");
+  float k[64];     // of the keys
+  float v[64];     // of the values, relative to 2^v_log2
+  uint8_t raw[64];  // exponents of the values
+  float v_log2;
+  int wide;
+  int pad[2];
 };
 
 template <bool QBF16, bool E4M3, int D, bool PAIR>
-__global__ void __launch_bounds__(threads_of<E4M3>(), 1)
+struct TilesSmem {
+  static constexpr int kElem = E4M3 ? 1 : 2;
+  static constexpr int kTerms = E4M3 ? (QBF16 ? 2 : 3) : 1;  // of a query
+  static constexpr int kQTile = BM * D * kElem;              // a term of a row tile
+  static constexpr int kKv = BN * D * kElem;                 // a K or V tile
+  static constexpr int kStage = 2 * kKv;                     // K, then V
+  static constexpr int kQTiles = PAIR ? 2 : 1;
+  static constexpr int kStages = E4M3 ? (PAIR ? 6 : 8) : (D == 128 ? (PAIR ? 4 : 6) : 8);
+  static constexpr int kRing = kQTiles * kTerms * kQTile;
+  static constexpr int kScales = kRing + kStages * kStage;  // [stages][128] exponents of the K tile's keys and values
+  static constexpr int kInfo = kScales + (E4M3 ? kStages * 128 : 0);
+  static constexpr int kOnes = kInfo + (E4M3 ? 2 * kInfos * (int)sizeof(TileInfo) : 0);  // [64] ones
+  static constexpr int kBar = kOnes + (E4M3 ? 256 : 0);
+  static constexpr int kTotal = kBar + 1024 + 1024;
+  static_assert(kTotal <= 232448, "ring and tiles must fit");
+};
+
+// Shared-memory descriptor of rows of 128 or 64 bytes in the swizzle of that width: K-major, 8 rows apart; MN-major, 8 k apart
+template <int ROW>
+__device__ __forceinline__ uint64_t desc_rows(uint32_t addr) {
+  return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(1) << 16) | (static_cast<uint64_t>(8 * ROW >> 4) << 32) |
+         (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(ROW == 128 ? 2 : 4) << 61);
+}
+// byte `at` of a tile of such rows
+template <int ROW>
+__device__ __forceinline__ uint32_t swizzled(uint32_t at) {
+  return at ^ (ROW == 128 ? ((at >> 7) & 7) << 4 : ((at >> 7) & 3) << 4);
+}
+// two values as e4m3 pairs: the nearest, and the nearest to what is left
+__device__ __forceinline__ uint16_t half2_to_e4m3x2(uint32_t h) {
+  uint16_t c;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(h));
+  return c;
+}
+
+template <bool QBF16, bool E4M3, int D, bool PAIR>
+__global__ void __launch_bounds__(kThreadsTiles, 1)
     cache_attention_tiles_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                                  const CacheAttnParams p) {
-  using L = TilesSmem<D, E4M3, PAIR>;
-  constexpr bool MBF16 = QBF16 && !E4M3;  // type of the products' operands
+  using L = TilesSmem<QBF16, E4M3, D, PAIR>;
   constexpr int kRows = PAIR ? 2 * BM : BM;
-  constexpr int kThreadsAll = threads_of<E4M3>();
   constexpr bool OWN_KV = !PAIR;  // each MMA warp has key tiles, and stages of the ring, of its own
-  constexpr int kBoxes = D / 64, kBoxBytes = BM * 128, kKvBoxBytes = BN * 128;
+  constexpr int kBoxes = E4M3 ? 1 : D / 64, kBoxBytes = BM * 128, kKvBoxBytes = BN * 128;  // (16-bit: column blocks of 128 bytes)
   constexpr int kStages = L::kStages, kOwnStages = OWN_KV ? kStages / 2 : kStages;
-  constexpr int kElem = E4M3 ? 1 : 2;
+  constexpr int kElem = L::kElem;
+  constexpr int kPTerms = E4M3 ? 2 : 1;  // of a weight
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
   uint64_t* kv_full = bars;            // [8]
   uint64_t* kv_empty = bars + 8;       // [8]
-  uint64_t* fixed = bars + 16;         // [8] 16-bit: the stage's values are checked; 8-bit: [raw stages] raw tiles are there
-  uint64_t* raw_empty = bars + 24;     // [8]
+  uint64_t* fixed = bars + 16;         // [8] the stage's values are checked, the scales of its keys prepared
   uint64_t* s_full = bars + 32;        // [2 groups][2 buffers] the scores of a key tile are complete
   uint64_t* p_ready = bars + 36;       // [2 groups][2 buffers] its probabilities are written
   uint64_t* o_done = bars + 40;        // [2 groups][2] of an item all P.V but the last, all P.V are complete
@@ -128,13 +132,9 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&kv_full[i], E4M3 ? 4 : 1);                          // the converting warps, or the TMA unit
-      mbar_init(&kv_empty[i], (OWN_KV ? 1 : 2) + (E4M3 ? 0 : 1));  // MMA warps that read the stage, and the checking warp
-      if (!E4M3) mbar_init(&fixed[i], 1);
-    }
-    for (int i = 0; i < L::kRawStages; ++i) {
-      mbar_init(&fixed[i], 1 + 32);  // (the lanes that copy scales arrive, too)
-      mbar_init(&raw_empty[i], 4);
+      mbar_init(&kv_full[i], E4M3 ? 1 + 32 : 1);         // (the lanes that copy exponents arrive, too)
+      mbar_init(&kv_empty[i], (OWN_KV ? 1 : 2) + 1);  // MMA warps that read the stage, and the checking warp
+      mbar_init(&fixed[i], 1);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
   }
+  if (E4M3 && threadIdx.x < 64) reinterpret_cast<float*>(smem + L::kOnes)[threadIdx.x] = 1.f;
   if (warp == kWarpMma) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -162,7 +163,7 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
   const uint32_t tmem_base = *tmem_slot;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Plan plan = make_plan<kThreadsAll>(p, kRows, plan_shared);
+  const Plan plan = make_plan<kThreadsTiles>(p, kRows, plan_shared);
 
   // What the roles agree on about an item: key tiles [tile0, tile0 + n), of which group g takes every one, or every second.
   struct Work {
@@ -183,14 +184,12 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
   auto tile_of = [](const Work& w, int b, int g) { return w.tile0 + (PAIR ? b : 2 * b + g); };
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(regs_other<E4M3>()));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == kWarpTma) {
       // ------------------------------------------------------------------ TMA producer
       // K's tiles come in order, and V's after them: the tokens of the last eight are kept for V.
       int loaded[2] = {0, 0};  // stages filled so far, over all items; OWN_KV: for either MMA warp
-      int raws = 0;
       bool ok = true;
-      constexpr int kRawStages = L::kRawStages ? L::kRawStages : 1;
       const int box = min(p.t.page, BN);  // rows a load brings
       PageWalk walk;
       for (Cursor c(p, plan, kRows); c.left > 0 && ok; c.next_item(p, kRows)) {
@@ -209,25 +208,19 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
               if (lane < 4) tokens[(k_tile & 7) * 4 + lane] = k_token;
             }
             const int v_token = has_v ? tokens[(v_tile & 7) * 4 + (lane & 3)] : 0;
-            const int st = E4M3 ? raws % kRawStages : ring_stage(loaded[g], g);
-            uint64_t* const full = E4M3 ? &fixed[st] : &kv_full[st];
-            ok = E4M3 ? mbar_wait_warp(&raw_empty[st], ((raws / kRawStages) & 1) ^ 1, abort_flag, p.status, ST_CACHE_RAW)
-                      : mbar_wait_warp(&kv_empty[st], ring_phase(loaded[g]) ^ 1, abort_flag, p.status, ST_CACHE_KV);
+            const int st = ring_stage(loaded[g], g);
+            uint64_t* const full = &kv_full[st];
+            ok = mbar_wait_warp(&kv_empty[st], ring_phase(loaded[g]) ^ 1, abort_flag, p.status, ST_CACHE_KV);
             if (!ok) continue;
             ++loaded[g];
-            ++raws;
             const int k_boxes = has_k ? min(BN / box, (w.keys - k_tile * BN + box - 1) / box) : 0;
             const int v_boxes = has_v ? min(BN / box, (w.keys - v_tile * BN + box - 1) / box) : 0;
             if (elect_one()) mbar_expect_tx(full, (uint32_t)((k_boxes + v_boxes) * box * D * kElem));
             __syncwarp();
-            unsigned char* at = smem + (E4M3 ? L::kRawRing + st * L::kRawTiles : L::kRing + st * L::kStage);
+            unsigned char* at = smem + L::kRing + st * L::kStage;
             if (E4M3) {
-              // the scales: of the K tile's keys and values, and of the V tile's values
-              unsigned char* scales = smem + L::kRawScales + st * 192;
-              const int piece = (lane & 3) * 16;
-              if (lane < 8 && has_k && k_tile * BN + piece < w.keys)
-                copy16(scales + lane * 16, (lane < 4 ? p.k_exponent : p.v_exponent) + k_token);
-              if (lane < 4 && has_v && v_tile * BN + piece < w.keys) copy16(scales + 128 + lane * 16, p.v_exponent + v_token);
+              if (lane < 8 && has_k && k_tile * BN + (lane & 3) * 16 < w.keys)
+                copy16(smem + L::kScales + st * 128 + lane * 16, (lane < 4 ? p.k_exponent : p.v_exponent) + k_token);
               copies_arrive(full);
             }
 #pragma unroll
@@ -237,14 +230,9 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
                 if (i >= (x ? v_boxes : k_boxes)) break;
                 const int token = uniform_of(x ? v_token : k_token, i * (box >> 4), lane);
                 if (elect_one()) {
-                  if (E4M3) {
-                    // (two rows of 64 bytes make a line of the map)
-                    tma_load_2d(at + x * BN * D + i * box * D, x ? &tmap_v : &tmap_k, full, 0, D == 64 ? token / 2 : token);
-                  } else {
 #pragma unroll
-                    for (int d = 0; d < kBoxes; ++d)
-                      tma_load_2d(at + x * L::kKv + d * kKvBoxBytes + i * box * 128, x ? &tmap_v : &tmap_k, full, d * 64, token);
-                  }
+                  for (int d = 0; d < kBoxes; ++d)
+                    tma_load_2d(at + x * L::kKv + d * kKvBoxBytes + i * box * (E4M3 ? D : 128), x ? &tmap_v : &tmap_k, full, d * 64, token);
                 }
               }
             __syncwarp();
@@ -256,11 +244,14 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
       // tcgen05 operations of ONE thread execute in issue order: S(b + 2) overwrites P(b) after P(b).V(b) has read it.  The two warps
       // issue in turn, so that one's waits lie behind the other's MMAs; one elected lane issues.
       const int mq = __shfl_sync(0xffffffffu, warp - kWarpMma, 0);
-      constexpr uint32_t idesc_s = umma_idesc_f16(BM, BN, MBF16, false, false);
-      constexpr uint32_t idesc_o = umma_idesc_f16(BM, D, MBF16, false, true);
-      const uint64_t dq = umma_desc_kmajor_sw128(smem_u32(smem) + (PAIR ? mq * L::kQTile : 0));
-      const uint64_t dk = umma_desc_kmajor_sw128(smem_u32(smem + L::kRing));
-      const uint64_t dv = umma_desc_mnmajor_sw128(smem_u32(smem + L::kRing + L::kKv), kKvBoxBytes, 1024);
+      // (kind::f8f6f4 has the fields of kind::f16; type 0 is e4m3 there)
+      constexpr uint32_t idesc_s = umma_idesc_f16(BM, BN, QBF16 && !E4M3, false, false);
+      constexpr uint32_t idesc_o = umma_idesc_f16(BM, D, QBF16 && !E4M3, false, true);
+      const uint32_t q_tile = smem_u32(smem) + (PAIR ? mq * L::kTerms * L::kQTile : 0);
+      const uint64_t dq = E4M3 ? desc_rows<D>(q_tile) : umma_desc_kmajor_sw128(q_tile);
+      const uint64_t dk = E4M3 ? desc_rows<D>(smem_u32(smem + L::kRing)) : umma_desc_kmajor_sw128(smem_u32(smem + L::kRing));
+      const uint64_t dv = E4M3 ? desc_rows<D>(smem_u32(smem + L::kRing + L::kKv))
+                               : umma_desc_mnmajor_sw128(smem_u32(smem + L::kRing + L::kKv), kKvBoxBytes, 1024);
       const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
       const uint32_t t_sq = tmem + mq * 128;        // the two buffers of scores, 64 columns each
       const uint32_t t_oq = tmem + 256 + mq * 128;  // O
@@ -280,11 +271,13 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
           const bool staged = b + 2 < n_max || (b >= 0 && b < n_max);  // a stage of the ring comes with this step
           const bool use_p = b >= 0 && b < n_mine, use_s = b + 2 < n_mine;
           const int st = ring_stage(taken, mq), buf = finished & 1;
+          // (8-bit: every stage passes the checking warp, which prepares the scales)
+          uint64_t* const stage_bar = E4M3 ? &fixed[st] : &kv_full[st];
           if (use_p && staged)
-            ok = mbar_wait_both(&p_ready[2 * mq + buf], (finished >> 1) & 1, &kv_full[st], ring_phase(taken), abort_flag, p.status,
-                                ST_CACHE_P, ST_CACHE_KV);
+            ok = mbar_wait_both(&p_ready[2 * mq + buf], (finished >> 1) & 1, stage_bar, ring_phase(taken), abort_flag, p.status, ST_CACHE_P,
+                                ST_CACHE_KV);
           else if (staged)
-            ok = mbar_wait(&kv_full[st], ring_phase(taken), abort_flag, p.status, ST_CACHE_KV);
+            ok = mbar_wait(stage_bar, ring_phase(taken), abort_flag, p.status, ST_CACHE_KV);
           if (!E4M3 && ok && use_p && tile_of(w, b, mq) >= w.first_masked)
             ok = mbar_wait(&fixed[st], ring_phase(taken), abort_flag, p.status, ST_CACHE_KV);
           if (ok && in_turn) ok = mbar_wait(&turn[mq], (turns & 1) ^ (mq ^ 1), abort_flag, p.status, ST_CACHE_S);
@@ -296,20 +289,38 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
           if (use_p) {
             ++finished;
             if (elect_one()) {
+              if (E4M3) {
 #pragma unroll
-              for (int kk = 0; kk < BN / 16; ++kk)
-                umma_f16_ts(t_oq, t_sq + buf * BN + kk * 8, dv + at + static_cast<uint64_t>((kk * 2048) >> 4), idesc_o,
-                            (b > 0 || kk > 0) ? 1u : 0u);
+                for (int t = 0; t < kPTerms; ++t)
+#pragma unroll
+                  for (int kk = 0; kk < BN / 32; ++kk)
+                    umma_f8_ts(t_oq, t_sq + buf * BN + t * 16 + kk * 8, dv + at + static_cast<uint64_t>((kk * 32 * D) >> 4), idesc_o,
+                               (b > 0 || t > 0 || kk > 0) ? 1u : 0u);
+              } else {
+#pragma unroll
+                for (int kk = 0; kk < BN / 16; ++kk)
+                  umma_f16_ts(t_oq, t_sq + buf * BN + kk * 8, dv + at + static_cast<uint64_t>((kk * 2048) >> 4), idesc_o,
+                              (b > 0 || kk > 0) ? 1u : 0u);
+              }
             }
           }
           if (use_s) {
             const int s_buf = begun & 1;
             ++begun;
             if (elect_one()) {
+              if (E4M3) {
 #pragma unroll
-              for (int kk = 0; kk < D / 16; ++kk)
-                umma_f16_ss(t_sq + s_buf * BN, dq + static_cast<uint64_t>(((kk / 4) * kBoxBytes + (kk % 4) * 32) >> 4),
-                            dk + at + static_cast<uint64_t>(((kk / 4) * kKvBoxBytes + (kk % 4) * 32) >> 4), idesc_s, kk != 0);
+                for (int t = 0; t < L::kTerms; ++t)
+#pragma unroll
+                  for (int kk = 0; kk < D / 32; ++kk)
+                    umma_f8_ss(t_sq + s_buf * BN, dq + static_cast<uint64_t>((t * L::kQTile + kk * 32) >> 4),
+                               dk + at + static_cast<uint64_t>((kk * 32) >> 4), idesc_s, t > 0 || kk > 0);
+              } else {
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                  umma_f16_ss(t_sq + s_buf * BN, dq + static_cast<uint64_t>(((kk / 4) * kBoxBytes + (kk % 4) * 32) >> 4),
+                              dk + at + static_cast<uint64_t>(((kk / 4) * kKvBoxBytes + (kk % 4) * 32) >> 4), idesc_s, kk != 0);
+              }
               if (in_turn) mbar_arrive(&turn[mq ^ 1]);
               umma_commit(&s_full[2 * mq + s_buf]);
             }
@@ -325,15 +336,15 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
           }
         }
       }
-    } else if (!E4M3 && warp == kWarpFix) {
-      // ------------------------------------------------------------------ values that not every row sees (16-bit)
+    } else if (warp == kWarpFix) {
+      // ------------------------------------------------------------------ values that not every row sees; scales
       // It follows every stage, since the parity of a phase two back reads like its own, and releases it too.
-      int followed[2] = {0, 0}, items = 0;
+      int followed[2] = {0, 0}, infos[2] = {0, 0}, items = 0;
       bool ok = true;
       for (Cursor c(p, plan, kRows); c.left > 0 && ok; c.next_item(p, kRows)) {
         const Work w = work_of(c);
         for (int b = -2; b < w.nq[0] && ok; ++b) {
-#pragma unroll
+#pragma unroll 1
           for (int g = 0; g < (OWN_KV ? 2 : 1); ++g) {
             const bool has_k = b + 2 < w.nq[g], has_v = b >= 0 && b < w.nq[g];
             if (!ok || !(has_k || has_v)) continue;
@@ -341,6 +352,33 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
             ok = mbar_wait_warp(&kv_full[st], ring_phase(followed[g]), abort_flag, p.status, ST_CACHE_KV);
             if (!ok) continue;
             ++followed[g];
+            if (E4M3 && has_k) {
+              // (The place is free: the tile eight before this one is long done, since S runs two tiles ahead of P.V, and the ring's
+              // stages bring few more.)
+              TileInfo* info = reinterpret_cast<TileInfo*>(smem + L::kInfo) + g * kInfos + (infos[g] + b + 2) % kInfos;
+              const uint8_t* scales = smem + L::kScales + st * 128;
+              const int left = w.keys - tile_of(w, b + 2, g) * BN;
+              // Rows of zeros, and what is no larger than 2^-117, have the least scale: it does not make a tile wide.
+              uint32_t e[2], top = 0, low = 255;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const int key = lane + 32 * i;
+                e[i] = key < left ? scales[64 + key] : 1u;
+                top = max(top, e[i]);
+                low = min(low, e[i] <= 1u ? 255u : e[i]);
+                info->k[key] = key < left ? scale_of(scales[key]) : 1.f;
+                info->raw[key] = (uint8_t)e[i];
+              }
+              top = __reduce_max_sync(0xffffffffu, top);
+              low = __reduce_min_sync(0xffffffffu, low);
+              if (top <= 1u) top = low = 127;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) info->v[lane + 32 * i] = __uint_as_float((uint32_t)max((int)e[i] - (int)top + 127, 0) << 23);
+              if (lane == 0) {
+                info->v_log2 = (float)((int)top - 127);
+                info->wide = top - low > kNarrow || top > 187u || low < 67u;
+              }
+            }
             const int tile = tile_of(w, b, g);
             if (has_v && tile >= w.first_masked) {
               const int left = w.keys - tile * BN;  // rows of the tile that are keys
@@ -353,13 +391,16 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
                 for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(v + (e0 + 32 * i) * 16);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                  const int key = ((e0 + 32 * i) * 16 % kKvBoxBytes) / 128;
+                  // (the swizzle moves 16-byte pieces inside lines of 128 bytes; the line tells the key, of 64-byte rows the piece too)
+                  const uint32_t at = swizzled<E4M3 ? D : 128>((e0 + 32 * i) * 16);
+                  const int key = E4M3 ? at / D : at % kKvBoxBytes / 128;
                   uint32_t* y = reinterpret_cast<uint32_t*>(&x[i]);
-                  const uint32_t expo = MBF16 ? 0x7f807f80u : 0x7c007c00u;
                   uint32_t take = 0;
 #pragma unroll
                   for (int n = 0; n < 4; ++n) {
-                    const uint32_t m = key < left ? __vcmpeq2(y[n] & expo, expo) : 0xffffffffu;
+                    const uint32_t m = key < left ? (E4M3 ? __vcmpeq4(y[n] & 0x7f7f7f7fu, 0x7f7f7f7fu)
+                                                          : __vcmpeq2(y[n] & (QBF16 ? 0x7f807f80u : 0x7c007c00u), QBF16 ? 0x7f807f80u : 0x7c007c00u))
+                                                  : 0xffffffffu;
                     bad |= key < left && m != 0;
                     y[n] &= ~m;
                     take |= m;
@@ -369,116 +410,11 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
               }
               fence_proxy_async_smem();
               if (bad) bad_values[items & 7] = items + 1;
-              __syncwarp();
             }
+            __syncwarp();
             if (lane == 0) {
               mbar_arrive(&fixed[st]);
               mbar_arrive(&kv_empty[st]);
-            }
-          }
-        }
-        ++items;
-      }
-    } else if (E4M3 && warp >= kWarpConvert) {
-      // ------------------------------------------------------------------ 8-bit tiles into operands
-      const int me = threadIdx.x - kWarpConvert * 32;  // 0 .. 127
-      int made[2] = {0, 0}, raws = 0, items = 0, infos[2] = {0, 0};
-      bool ok = true;
-      constexpr int kRawStages = L::kRawStages ? L::kRawStages : 1;
-      for (Cursor c(p, plan, kRows); c.left > 0 && ok; c.next_item(p, kRows)) {
-        const Work w = work_of(c);
-        for (int b = -2; b < w.nq[0] && ok; ++b) {
-#pragma unroll
-          for (int g = 0; g < (OWN_KV ? 2 : 1); ++g) {
-            const bool has_k = b + 2 < w.nq[g], has_v = b >= 0 && b < w.nq[g];
-            if (!ok || !(has_k || has_v)) continue;
-            const int rs = raws % kRawStages, st = ring_stage(made[g], g);
-            ok = mbar_wait_warp(&fixed[rs], (raws / kRawStages) & 1, abort_flag, p.status, ST_CACHE_RAW) &&
-                 mbar_wait_warp(&kv_empty[st], ring_phase(made[g]) ^ 1, abort_flag, p.status, ST_CACHE_KV);
-            if (!ok) continue;
-            ++raws;
-            ++made[g];
-            const unsigned char* raw = smem + L::kRawRing + rs * L::kRawTiles;
-            unsigned char* op = smem + L::kRing + st * L::kStage;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              if (!(x ? has_v : has_k)) continue;
-              const int left = w.keys - tile_of(w, x ? b : b + 2, g) * BN;
-              const uint8_t* scales = smem + L::kRawScales + rs * 192;
-              // every warp finds the largest scale by itself
-              const Fold fold = fold_of(scales + (x ? 128 : 0), left, lane);
-              if (x == 0 && warp == kWarpConvert) {
-                // what the softmax group has to know about the tile.  (Its place is free: the tile eight before it is long done, since S runs
-                // two tiles ahead of P.V and the ring fewer than that.)
-                TileInfo* info = reinterpret_cast<TileInfo*>(smem + L::kInfo) + g * kInfos + (infos[g] + b + 2) % kInfos;
-                const Fold values = fold_of(scales + 64, left, lane);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                  info->k[lane + 32 * i] = scales[lane + 32 * i];
-                  info->v[lane + 32 * i] = scales[64 + lane + 32 * i];
-                }
-                if (lane == 0) {
-                  info->k_scale = __uint_as_float(fold.top << 23);
-                  info->v_log2 = (float)((int)values.top - 127);
-                  info->wide_k = fold.wide;
-                  info->wide_v = values.wide;
-                }
-              }
-              const uint8_t* mine = scales + (x ? 128 : 0);
-              const uint32_t top = fold.top;
-              const bool wide = fold.wide;
-              const unsigned char* from = raw + x * BN * D;
-              unsigned char* to = op + x * L::kKv;
-              bool bad = false;
-              // 16 codes a piece; a lane's neighbours have the pieces of the same key.  All loads come before the first store, which the
-              // compiler would not move them across.
-              constexpr int kPieces = BN * D / 16 / 128;
-              uint4 codes[kPieces];
-              uint32_t factor[kPieces];  // 2^(e - largest), a half twice; 0 for what is no key
-#pragma unroll
-              for (int n = 0; n < kPieces; ++n) {
-                const int e = me + n * 128, key = e / (D / 16);
-                const uint32_t off = e * 16;
-                codes[n] = *reinterpret_cast<const uint4*>(from + (off ^ (((off >> 7) & 7) << 4)));
-                const int down = wide ? 0 : (int)top - (int)mine[key];
-                factor[n] = key >= left || down > 14 ? 0u : (uint32_t)(15 - down) * 0x04000400u;
-              }
-#pragma unroll
-              for (int n = 0; n < kPieces; ++n) {
-                const int e = me + n * 128, key = e / (D / 16), piece = e % (D / 16);
-                const __half2 scale = *reinterpret_cast<const __half2*>(&factor[n]);
-                uint32_t out[8];
-                const uint32_t in[4] = {codes[n].x, codes[n].y, codes[n].z, codes[n].w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const uint32_t lo = e4m3x2_to_half2(in[i]), hi = e4m3x2_to_half2_hi(in[i]);
-                  const __half2 a = __hmul2(*reinterpret_cast<const __half2*>(&lo), scale), b2 = __hmul2(*reinterpret_cast<const __half2*>(&hi), scale);
-                  out[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
-                  out[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&b2);
-                }
-                if (x == 1) {
-                  // codes that are NaN (0x7f, 0xff: adding 1 to the other seven bits carries) come back when O is stored
-                  uint32_t nan = 0;
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) nan |= (in[i] & 0x7f7f7f7fu) + 0x01010101u;
-                  if ((nan & 0x80808080u) || key >= left) {
-                    bad |= key < left;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) out[i] = key < left ? out[i] & ~__vcmpeq2(out[i] & 0x7c007c00u, 0x7c007c00u) : 0u;
-                  }
-                }
-                const uint32_t line = key * 128, col = (piece & 3) * 2;
-                unsigned char* box = to + (piece >> 2) * kKvBoxBytes;
-                *reinterpret_cast<uint4*>(box + line + ((col ^ (key & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
-                *reinterpret_cast<uint4*>(box + line + (((col + 1) ^ (key & 7)) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
-              }
-              if (bad) bad_values[items & 7] = items + 1;
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              mbar_arrive(&raw_empty[rs]);
-              mbar_arrive(&kv_full[st]);
             }
           }
         }
@@ -488,7 +424,7 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(regs_softmax<E4M3>()));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     // ------------------------------------------------------------------ softmax groups
     const int q = warp >> 2;    // this group: its row tile, or its share of the key tiles
     const int quad = warp & 3;  // TMEM lane quadrant this warp may touch
@@ -521,36 +457,62 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
       float row_scale = fabsf(p.scale_log2);
       {
         const int head = c.h * p.group + (valid ? r - i_new * p.group : 0);
-        const uint16_t* src = static_cast<const uint16_t*>(p.q) + (int64_t)(seq.first + i_new) * p.q_row + (int64_t)head * p.q_head;
-        unsigned char* tile = smem + (PAIR ? q * L::kQTile : 0);
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + (int64_t)(seq.first + i_new) * p.q_row +
+                                                          (int64_t)head * p.q_head);
+        unsigned char* tile = smem + (PAIR ? q * L::kTerms * L::kQTile : 0);
         const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a negative scale goes into the queries)
-        float down = 1.f;
-        if (E4M3 && QBF16) {
-          uint32_t most = 0;
-          if (valid)
-#pragma unroll 4
-            for (int i = 0; i < D / 8; ++i) {
-              const uint4 x = __ldg(reinterpret_cast<const uint4*>(src) + i);
-              const uint32_t y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-              for (int n = 0; n < 4; ++n) most = max(most, max(y[n] & 0x7fffu, (y[n] >> 16) & 0x7fffu));
-            }
-          const uint32_t e = min(max(most >> 7, 1u), 253u);  // halves with the row's largest magnitude in [1, 2)
-          down = __uint_as_float((254u - e) << 23);
-          row_scale *= __uint_as_float(e << 23);
-        }
         // where the groups share a tile, each brings half of every row
         constexpr int kPieces = D / 8 / (PAIR ? 1 : 2);
         const int first = PAIR ? 0 : q * kPieces;
+        if (!E4M3) {
 #pragma unroll 4
-        for (int i = first; i < first + kPieces; ++i) {
-          uint4 x = valid ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
-          if (E4M3 && QBF16) {
-            auto half = [&](uint32_t b) { return pack16<false>(__uint_as_float(b << 16) * down, __uint_as_float(b & 0xffff0000u) * down); };
-            x = make_uint4(half(x.x), half(x.y), half(x.z), half(x.w));
+          for (int i = first; i < first + kPieces; ++i) {
+            uint4 x = valid ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+            x = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
+            *reinterpret_cast<uint4*>(tile + (i >> 3) * kBoxBytes + row * 128 + (((i & 7) ^ (row & 7)) << 4)) = x;
           }
-          x = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
-          *reinterpret_cast<uint4*>(tile + (i >> 3) * kBoxBytes + row * 128 + (((i & 7) ^ (row & 7)) << 4)) = x;
+        } else {
+          auto pair_of = [&](uint32_t y) {
+            return QBF16 ? make_float2(__uint_as_float(y << 16), __uint_as_float(y & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&y));
+          };
+          float most = 0.f;
+#pragma unroll 4
+          for (int i = 0; i < D / 8; ++i) {
+            const uint4 x = valid ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+            const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int n = 0; n < 4; ++n) most = max3f(most, fabsf(pair_of(y[n]).x), fabsf(pair_of(y[n]).y));
+          }
+          // scaled by a power of two to a largest magnitude in [128, 256)
+          const uint32_t e = min(max(__float_as_uint(most) >> 23, 9u), 253u);
+          const float up = __uint_as_float((254u + 7u - e) << 23);
+          row_scale *= __uint_as_float((e - 7u) << 23);
+#pragma unroll 1
+          for (int i = first / 2; i < (first + kPieces) / 2; ++i) {  // 16 elements: 16 bytes of every term
+            const uint4 x0 = valid ? __ldg(src + 2 * i) : make_uint4(0, 0, 0, 0), x1 = valid ? __ldg(src + 2 * i + 1) : make_uint4(0, 0, 0, 0);
+            const uint32_t y[8] = {x0.x ^ flip, x0.y ^ flip, x0.z ^ flip, x0.w ^ flip, x1.x ^ flip, x1.y ^ flip, x1.z ^ flip, x1.w ^ flip};
+            uint32_t term[3][4] = {};
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+              float2 left = pair_of(y[n]);
+              left = make_float2(left.x * up, left.y * up);
+              // (infinities would saturate: NaN, as their scores are)
+              if (!(fabsf(left.x) <= FLT_MAX)) left.x = __uint_as_float(0x7fc00000u);
+              if (!(fabsf(left.y) <= FLT_MAX)) left.y = __uint_as_float(0x7fc00000u);
+#pragma unroll
+              for (int t = 0; t < L::kTerms; ++t) {
+                const uint32_t codes = float2_to_e4m3x2(left.x, left.y);
+                const uint32_t back = e4m3x2_to_half2(codes);
+                const float2 is = __half22float2(*reinterpret_cast<const __half2*>(&back));
+                left = make_float2(left.x - is.x, left.y - is.y);
+                term[t][n >> 1] |= codes << (16 * (n & 1));
+              }
+            }
+#pragma unroll
+            for (int t = 0; t < L::kTerms; ++t)
+              *reinterpret_cast<uint4*>(tile + t * L::kQTile + swizzled<D>(row * D + i * 16)) =
+                  make_uint4(term[t][0], term[t][1], term[t][2], term[t][3]);
+          }
         }
         fence_proxy_async_smem();
         if (!PAIR || n_tiles > 0) mbar_arrive(&q_full[PAIR ? q : 0]);
@@ -576,19 +538,21 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
         ++steps;
         tmem_ld_wait();
         const bool more = i + 1 < n_tiles;
+        const float* k_mul = nullptr;  // 8-bit: the scales of the keys, and of the values relative to 2^v_log2
+        const float* v_mul = nullptr;
         float scale = row_scale, v_log2 = 0.f;
-        bool wide_k = false, wide_v = false;
+        bool detour = tile >= w.first_masked;
         if (E4M3) {
+          k_mul = info->k;
+          v_mul = info->v;
           v_log2 = info->v_log2;
-          wide_k = info->wide_k != 0;
-          wide_v = info->wide_v != 0;
-          if (!wide_k) scale *= info->k_scale;
+          detour |= info->wide != 0;
         }
-        const bool general = wide_k || wide_v || tile >= w.first_masked;
+        constexpr float kThreshold = E4M3 ? kRescale8 : kRescaleThreshold;
         // Takes a new reference where it grew by more than the threshold: rare.  O is rescaled in tensor memory.
         auto settle = [&](float most) {
           const float a_new = fmaxf(a_ref, most);
-          if (!__any_sync(0xffffffffu, a_new - a_ref > kRescaleThreshold)) return;
+          if (!__any_sync(0xffffffffu, a_new - a_ref > kThreshold)) return;
           const float factor = ex2f(a_ref - a_new);
           a_ref = a_new;
           if (!E4M3) l_sum *= factor;
@@ -615,8 +579,100 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
           }
           l_sum = fmaf(sum, ex2f(unit - b_ref), l_sum);
         };
-        uint32_t pk0[16], pk1[16];
-        if (!general) {
+        float unit = 0.f;  // the exponentials are 2^(score - unit)
+        if (detour) {
+          // What the row sees of the tile's keys, a bit a key.  The warp's rows belong to a few neighbouring tokens: the warp reads each
+          // one's mask side by side, four tokens' at a time.
+          uint32_t see[2] = {0, 0};
+          const int ahead0 = tile * BN - seq.length;
+          const int t0 = __shfl_sync(0xffffffffu, i_new, 0), t1 = __reduce_max_sync(0xffffffffu, i_new);
+#pragma unroll 1
+          for (int t = min(t0, t1); t <= t1; t += 4) {
+            bool lo[4], hi[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              lo[n] = t + n <= t1 && sees(p, seq, t + n, ahead0 + lane);
+              hi[n] = t + n <= t1 && sees(p, seq, t + n, ahead0 + 32 + lane);
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const uint32_t l = __ballot_sync(0xffffffffu, lo[n]), h = __ballot_sync(0xffffffffu, hi[n]);
+              if (t + n == i_new) {
+                see[0] = l;
+                see[1] = h;
+              }
+            }
+          }
+          // The scores, scaled, in tensor memory; -inf for what the row does not see.
+          float mx = -INFINITY, mw = -INFINITY;  // largest score, largest score plus scale of the value
+#pragma unroll 1
+          for (int x = 0; x < BN / 16; ++x) {
+            uint32_t y[16];
+            tmem_ld_32x32b_x16(t_s + buf * BN + x * 16, y);
+            tmem_ld_wait();
+            const uint32_t bits = (x & 2 ? see[1] : see[0]) >> (16 * (x & 1));
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float v = __uint_as_float(y[e]) * (E4M3 ? k_mul[x * 16 + e] * scale : scale);
+              if (!((bits >> e) & 1u)) v = -INFINITY;
+              y[e] = __float_as_uint(v);
+              if (E4M3) {
+                const unsigned ev = info->raw[x * 16 + e];
+                mx = fmaxf(mx, v);
+                mw = fmaxf(mw, v + (ev == 255u ? __uint_as_float(0x7fc00000u) : (float)((int)ev - 127)));
+              }
+            }
+            tmem_st_32x32b_x16(t_s + buf * BN + x * 16, y);
+          }
+          tmem_st_wait();
+          if (E4M3) {
+            // the row sum here; then what the weights' exponents are, in the scores' place
+            settle(mw);
+            if (!ok) break;
+            if (mx > b_ref) {
+              l_sum *= ex2f(b_ref - mx);
+              b_ref = mx;
+            }
+            float sum = 0.f;
+#pragma unroll 1
+            for (int x = 0; x < BN / 16; ++x) {
+              uint32_t y[16];
+              tmem_ld_32x32b_x16(t_s + buf * BN + x * 16, y);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const float v = __uint_as_float(y[e]);
+                const unsigned ev = info->raw[x * 16 + e];
+                sum += ex2f(v - b_ref);
+                const float to = v + (ev == 255u ? __uint_as_float(0x7fc00000u) : (float)((int)ev - 127)) - a_ref + kTop8;
+                y[e] = __float_as_uint(v == -INFINITY ? -INFINITY : to);  // (what is not seen weighs nothing, whatever its value's scale)
+              }
+              tmem_st_32x32b_x16(t_s + buf * BN + x * 16, y);
+            }
+            tmem_st_wait();
+            l_sum += sum;
+            k_mul = v_mul = reinterpret_cast<const float*>(smem + L::kOnes);
+          }
+          scale = 1.f;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) tmem_ld_32x32b_x32(t_s + buf * BN + x * 32, sr[x]);
+          tmem_ld_wait();
+        }
+        if (E4M3) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float4 f = *reinterpret_cast<const float4*>(k_mul + x * 32 + e * 4);
+              float2 lo = make_float2(__uint_as_float(sr[x][4 * e]), __uint_as_float(sr[x][4 * e + 1]));
+              float2 hi = make_float2(__uint_as_float(sr[x][4 * e + 2]), __uint_as_float(sr[x][4 * e + 3]));
+              lo = mul2_rn(lo, make_float2(f.x, f.y));
+              hi = mul2_rn(hi, make_float2(f.z, f.w));
+              sr[x][4 * e] = __float_as_uint(lo.x); sr[x][4 * e + 1] = __float_as_uint(lo.y);
+              sr[x][4 * e + 2] = __float_as_uint(hi.x); sr[x][4 * e + 3] = __float_as_uint(hi.y);
+            }
+        }
+        if (!E4M3 || !detour) {
           float mxc[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains of the row maximum
 #pragma unroll
           for (int e = 0; e < 16; ++e)
@@ -626,9 +682,12 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
           const float mx = max3f(mxc[0], mxc[1], fmaxf(mxc[2], mxc[3])) * scale;
           settle(E4M3 ? mx + v_log2 : mx);
           if (!ok) break;
-          const float unit = E4M3 ? a_ref - v_log2 : a_ref;
-          const float2 scale2 = make_float2(scale, scale), neg2 = make_float2(-unit, -unit);
-          float2 sa = make_float2(0.f, 0.f), sb = make_float2(0.f, 0.f);
+          unit = E4M3 ? a_ref - v_log2 - kTop8 : a_ref;
+        }
+        uint32_t pk0[16], pk1[16];  // the weights' first and second 32 keys (16-bit), or first and second terms
+        const float2 scale2 = make_float2(scale, scale), neg2 = make_float2(-unit, -unit);
+        float2 sa = make_float2(0.f, 0.f), sb = make_float2(0.f, 0.f);
+        if (!E4M3) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const float2 xa = fma2(make_float2(__uint_as_float(sr[0][2 * e]), __uint_as_float(sr[0][2 * e + 1])), scale2, neg2);
@@ -637,79 +696,36 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
             const float2 eb = make_float2(ex2f(xb.x), ex2f(xb.y));
             sa = add2(sa, ea);
             sb = add2(sb, eb);
-            pk0[e] = pack16<MBF16>(ea.x, ea.y);
-            pk1[e] = pack16<MBF16>(eb.x, eb.y);
+            pk0[e] = pack16<QBF16>(ea.x, ea.y);
+            pk1[e] = pack16<QBF16>(eb.x, eb.y);
           }
-          const float2 tot = add2(sa, sb);
-          if (E4M3) add_sum(tot.x + tot.y, unit); else l_sum += tot.x + tot.y;
         } else {
-          // What the row sees of the tile's keys, a bit a key.  The warp's rows belong to a few neighbouring tokens: the warp reads each
-          // one's mask side by side.
-          uint32_t see[2] = {0, 0};
-          const int ahead0 = tile * BN - seq.length;
-          const int t0 = __shfl_sync(0xffffffffu, i_new, 0), t1 = __reduce_max_sync(0xffffffffu, i_new);
-          for (int t = min(t0, t1); t <= t1; t += 8) {  // (eight tokens' loads at a time)
-            bool lo[8], hi[8];
 #pragma unroll
-            for (int n = 0; n < 8; ++n) {
-              lo[n] = t + n <= t1 && sees(p, seq, t + n, ahead0 + lane);
-              hi[n] = t + n <= t1 && sees(p, seq, t + n, ahead0 + 32 + lane);
-            }
-#pragma unroll
-            for (int n = 0; n < 8; ++n) {
-              const uint32_t l = __ballot_sync(0xffffffffu, lo[n]), h = __ballot_sync(0xffffffffu, hi[n]);
-              if (t + n == i_new) {
-                see[0] = l;
-                see[1] = h;
-              }
-            }
+          for (int e = 0; e < 16; ++e) {  // four keys
+            const int x = e >> 3, y = (e & 7) * 4;
+            const float2 xa = fma2(make_float2(__uint_as_float(sr[x][y]), __uint_as_float(sr[x][y + 1])), scale2, neg2);
+            const float2 xb = fma2(make_float2(__uint_as_float(sr[x][y + 2]), __uint_as_float(sr[x][y + 3])), scale2, neg2);
+            float2 ea = make_float2(ex2f(xa.x), ex2f(xa.y));
+            float2 eb = make_float2(ex2f(xb.x), ex2f(xb.y));
+            sa = add2(sa, ea);
+            sb = add2(sb, eb);
+            const float4 f = *reinterpret_cast<const float4*>(v_mul + e * 4);
+            ea = mul2_rn(ea, make_float2(f.x, f.y));
+            eb = mul2_rn(eb, make_float2(f.z, f.w));
+            const uint32_t ha = pack16<false>(ea.x, ea.y), hb = pack16<false>(eb.x, eb.y);
+            const uint32_t c0 = half2_to_e4m3x2(ha), c1 = half2_to_e4m3x2(hb);
+            const uint32_t ba = e4m3x2_to_half2(c0), bb = e4m3x2_to_half2(c1);
+            const __half2 ra = __hsub2(*reinterpret_cast<const __half2*>(&ha), *reinterpret_cast<const __half2*>(&ba));
+            const __half2 rb = __hsub2(*reinterpret_cast<const __half2*>(&hb), *reinterpret_cast<const __half2*>(&bb));
+            pk0[e] = c0 | (c1 << 16);
+            pk1[e] = (uint32_t)half2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&ra)) |
+                     ((uint32_t)half2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&rb)) << 16);
           }
-          float mx = -INFINITY, mw = -INFINITY;  // of scores, of scores and scales
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              float s = __uint_as_float(sr[x][e]) * scale;
-              float v = v_log2;
-              if (E4M3 && wide_k) s = __uint_as_float(sr[x][e]) * scale_of(info->k[x * 32 + e]) * scale;
-              if (E4M3 && wide_v) {
-                const unsigned ev = info->v[x * 32 + e];
-                v = ev == 255u ? __uint_as_float(0x7fc00000u) : (float)((int)ev - 127);
-              }
-              if (!((see[x] >> e) & 1u)) s = -INFINITY;
-              sr[x][e] = __float_as_uint(s);
-              mx = fmaxf(mx, s);
-              if (E4M3) mw = fmaxf(mw, s + v);
-            }
-          settle(E4M3 ? mw : mx);
-          if (!ok) break;
-          if (E4M3 && mx > b_ref) {
-            l_sum *= ex2f(b_ref - mx);
-            b_ref = mx;
-          }
-          float sum = 0.f;
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              float wgt[2];
-#pragma unroll
-              for (int y = 0; y < 2; ++y) {
-                const int j = 2 * e + y;
-                const float s = __uint_as_float(sr[x][j]);
-                float v = v_log2;
-                if (E4M3 && wide_v) {
-                  const unsigned ev = info->v[x * 32 + j];
-                  v = ev == 255u ? __uint_as_float(0x7fc00000u) : (float)((int)ev - 127);
-                }
-                const float pr = ex2f(s - (E4M3 ? b_ref : a_ref));
-                sum += pr;
-                wgt[y] = !E4M3 ? pr : s == -INFINITY ? 0.f : ex2f(s + v - a_ref);
-              }
-              (x ? pk1 : pk0)[e] = pack16<MBF16>(wgt[0], wgt[1]);
-            }
-          l_sum += sum;
         }
+        const float2 tot = add2(sa, sb);
+        if (!E4M3) l_sum += tot.x + tot.y;
+        else if (!detour) add_sum(tot.x + tot.y, unit);
+        // (the scores read ahead take the registers of this tile's)
         const bool ahead = __all_sync(0xffffffffu, more && mbar_test(&s_full[2 * q + (steps & 1)], (steps >> 1) & 1));
         if (ahead) load_scores();
         // P is written over the first half of the scores it comes from
@@ -728,7 +744,7 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
 
       // ---- O: scaled to the units of the row sum, and out: whole, or as a part for the join
       const float m_mine = E4M3 ? b_ref : a_ref;
-      float f[2] = {E4M3 ? ex2f(a_ref - b_ref) : 1.f, 0.f}, m = m_mine, l = l_sum;
+      float f[2] = {E4M3 ? ex2f(a_ref - kTop8 - b_ref) : 1.f, 0.f}, m = m_mine, l = l_sum;
       if (!E4M3 || l_sum == 0.f) f[0] = l_sum == 0.f ? 0.f : f[0];
       if (!PAIR) {
         meet();  // all scores have been read: the statistics take the queries' place
@@ -782,8 +798,8 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
                   if ((__ldg(static_cast<const uint8_t*>(p.v_pages) + at + e) & 0x7f) == 0x7f) v = __uint_as_float(0x7fc00000u);
                 } else {
                   const uint16_t bits = __ldg(static_cast<const uint16_t*>(p.v_pages) + at + e);
-                  const uint16_t expo = MBF16 ? 0x7f80 : 0x7c00;
-                  if ((bits & expo) == expo) v = MBF16 ? __uint_as_float((uint32_t)bits << 16) : __half2float(__ushort_as_half(bits));
+                  const uint16_t expo = QBF16 ? 0x7f80 : 0x7c00;
+                  if ((bits & expo) == expo) v = QBF16 ? __uint_as_float((uint32_t)bits << 16) : __half2float(__ushort_as_half(bits));
                 }
                 if (v != 0.f) {
 #pragma unroll
@@ -830,15 +846,14 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
 template <bool QBF16, bool E4M3, int D, bool PAIR>
 int launch_tiles(frisk_b200_ctx* ctx, const CacheAttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, unsigned grid, cudaStream_t s) {
   auto kern = cache_attention_tiles_kernel<QBF16, E4M3, D, PAIR>;
-  using L = TilesSmem<D, E4M3, PAIR>;
+  using L = TilesSmem<QBF16, E4M3, D, PAIR>;
   static PerDeviceOnce opt_in;
   const int rc = opt_in(ctx->device, [&] {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) != cudaSuccess) return (int)FRISK_B200_E_CUDA;
     // setmaxnreg.inc waits until the CTA's own registers hold the request: what the launch brings must cover both shares
     cudaFuncAttributes a;
     if (cudaFuncGetAttributes(&a, kern) != cudaSuccess) return (int)FRISK_B200_E_CUDA;
-    const int other = threads_of<E4M3>() - 256;
-    return a.numRegs * threads_of<E4M3>() >= 256 * regs_softmax<E4M3>() + other * regs_other<E4M3>() ? 0 : (int)FRISK_B200_E_UNSUPPORTED;
+    return a.numRegs * kThreadsTiles >= 256 * kRegsSoftmax + (kThreadsTiles - 256) * kRegsOther ? 0 : (int)FRISK_B200_E_UNSUPPORTED;
   });
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -846,7 +861,7 @@ int launch_tiles(frisk_b200_ctx* ctx, const CacheAttnParams& p, const CUtensorMa
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel waits (griddepcontrol.wait) itself
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads_of<E4M3>());
+  cfg.blockDim = dim3(kThreadsTiles);
   cfg.dynamicSmemBytes = L::kTotal;
   cfg.stream = s;
   cfg.attrs = attr;

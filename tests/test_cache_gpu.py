@@ -60,6 +60,11 @@ class Batch:
     def refresh(self):
         self.cache = tuple(t.cuda() for t in self.cpu)
 
+    def terms(self, max_new):
+        """Whether the kernel for more than 16 rows a key head runs on an 8-bit cache."""
+        per = max_new if max_new else -(-self.rows // len(self.lengths))
+        return len(self.cpu) == 4 and per * (self.q.shape[1] // self.k.shape[1]) > 16
+
     def inside(self):
         import torch
         i = torch.zeros(self.rows, dtype=torch.bool)
@@ -105,7 +110,7 @@ def attend(batch, mask=None, scale=None, max_new=0, bound_scale=1.0, **more):
     F.cache_check()
     assert got is out
     assert all(torch.equal(a, bits(t)) for a, t in zip(before, batch.cache))
-    ref, bound = co.attention(batch.cpu, batch.q.cpu(), *batch.host, mask=mask, scale=scale)
+    ref, bound = co.attention(batch.cpu, batch.q.cpu(), *batch.host, mask=mask, scale=scale, terms=batch.terms(max_new))
     got, inside = out.cpu().double(), batch.inside()
     assert bool((got[~inside] == 77.0).all())
     finite = torch.isfinite(ref)
