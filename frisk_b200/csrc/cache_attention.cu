@@ -706,7 +706,7 @@ extern "C" int frisk_b200_cache_attention(frisk_b200_ctx* ctx, const frisk_b200_
   if ((a->heads_q > 1 && out->head_stride < c->D) || (c->rows > 1 && out->row_stride < (a->heads_q - 1) * out->head_stride + c->D))
     return FRISK_B200_E_CACHE_SHAPE;
   const size_t need = frisk_b200_cache_attention_workspace_bytes(c, a);
-  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)) return FRISK_B200_E_WORKSPACE;
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 31u)) return FRISK_B200_E_WORKSPACE;
   const size_t ob = packed_span(*out, c->rows, a->heads_q, c->D, 2), qb = packed_span(*q, c->rows, a->heads_q, c->D, 2);
   const size_t mb = mask ? (size_t)((c->rows - 1) * a->mask_stride + a->mask_width) : 0;
   for (int w = 0; w < 2; ++w) {  // what is written: the results and the workspace

@@ -202,6 +202,36 @@ __device__ __forceinline__ void store_row4(const CacheAttnParams& p, int first, 
   *reinterpret_cast<uint2*>(out + c4 * 4) = make_uint2(attn::pack16<QBF16>(x[0], x[1]), attn::pack16<QBF16>(x[2], x[3]));
 }
 
+// 32 bytes in one access: a warp whose lanes write rows of their own takes a cycle for every line it touches, however little of it
+__device__ __forceinline__ void store32(void* at, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+               "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+// columns 32 x .. of a row of results, o * inv
+template <bool QBF16, bool E4M3>
+__device__ __forceinline__ void store_row32(uint16_t* row, int x, const uint32_t (&o)[32], float inv) {
+  uint32_t y[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float a = __uint_as_float(o[2 * i]) * inv, b = __uint_as_float(o[2 * i + 1]) * inv;
+    if (E4M3) {
+      a = saturated<QBF16>(a);
+      b = saturated<QBF16>(b);
+    }
+    y[i] = attn::pack16<QBF16>(a, b);
+  }
+  uint16_t* at = row + x * 32;
+  if ((reinterpret_cast<uintptr_t>(at) & 31u) == 0) {
+    store32(at, y);
+    store32(at + 16, y + 8);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<uint4*>(at + 8 * i) = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+  }
+}
+
 // 16 bytes from global to shared memory, and this thread's arrival on `bar` (one of its count) when its copies so far are there
 __device__ __forceinline__ void copy16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");

@@ -16,15 +16,14 @@
 // 8-bit caches: the products take the codes as they are (kind::f8f6f4), and what meets them is written as a sum of e4m3 values, one
 // MMA each.  A query row, scaled by a power of two to at most 256, becomes two terms (bf16) or three (fp16) whose sum is the query but for
 // what lies 2^-19 below the row's largest element.  A weight becomes two: the first has 4 bits, the second 4 of the rest, 2^-8 of the weight
-// in all as with bf16 weights, or 2^-17 of the row's largest: the reference A moves when the maximum grew by more than 2, and the largest
-// weight lies between 2^7 and 2^8.  Converting the codes to halves instead took four warps 1.6 us a tile (2.5 us a tile of 64 rows in all).
+// in all as with bf16 weights, or 2^-15.75 of the weight at the reference A, which moves when the maximum grew by more than 2^3.  (2^-17 and
+// 2^1 moved it in most of an item's first tiles: 173 us where 157 were due.)  Converting the codes to halves instead took four warps 1.6 us a tile (2.5 us a tile of 64 rows in all).
 // Keys' scales multiply the scores; values' scales the weights, w = 2^(s + v - A): v is the tile's largest, as one number in the exponent,
 // and a factor for every key relative to it.  The row sum has no part in the values' scales and is kept in units of 2^B of its own.  The
 // checking warp prepares the scales.
 //
-// Tiles that a row may not see whole, and 8-bit tiles whose values' scales span more than 2^8 ("wide"), take a detour of rolled loops over
-// tensor memory before the common path: hidden scores become -inf there.  (Unrolled, code that runs once an item cost 20 us a tile: it
-// has to be fetched.)
+// Tiles that a row may not see whole, and 8-bit tiles whose values' scales span more than 2^8 ("wide"), take a path of rolled loops over
+// tensor memory.  (Unrolled, code that runs once an item cost up to 20 us a tile: it has to be fetched.)
 //
 // What bounds it: up to 128 rows HBM, 0.77 us a 16-bit tile of 64 keys a SM; else the softmax groups (some 1700 clk for 64 keys of 256
 // rows, of which 1024 exponentials).
@@ -46,14 +45,14 @@ constexpr int kThreadsTiles = 384;  // warps 0-3, 4-7: softmax groups; 8: TMA; 9
 constexpr int kWarpFix = 11;
 constexpr int kInfos = 8;            // key tiles whose scales are kept, for either group
 constexpr uint32_t kNarrow = 8;      // log2: scales of a tile's values that lie this close share a reference
-constexpr float kTop8 = 7.f;         // log2 of the 8-bit weight at the reference
-constexpr float kRescale8 = 1.f;     // 8-bit: the reference moves when the maximum grew by more than this
+constexpr float kTop8 = 5.75f;       // log2 of the 8-bit weight at the reference
+constexpr float kRescale8 = 3.f;     // 8-bit: the reference moves when the maximum grew by more than this (together 2^8.75, e4m3 ends at 448)
 
 // the scales of a key tile, 8-bit caches
 struct alignas(16) TileInfo {
   float k[64];     // of the keys
   float v[64];     // of the values, relative to 2^v_log2
-  uint8_t raw[64];  // exponents of the values
+  float log2_v[64];  // log2 of the scales of the values
   float v_log2;
   int wide;
   int pad[2];
@@ -71,8 +70,7 @@ struct TilesSmem {
   static constexpr int kRing = kQTiles * kTerms * kQTile;
   static constexpr int kScales = kRing + kStages * kStage;  // [stages][128] exponents of the K tile's keys and values
   static constexpr int kInfo = kScales + (E4M3 ? kStages * 128 : 0);
-  static constexpr int kOnes = kInfo + (E4M3 ? 2 * kInfos * (int)sizeof(TileInfo) : 0);  // [64] ones
-  static constexpr int kBar = kOnes + (E4M3 ? 256 : 0);
+  static constexpr int kBar = kInfo + (E4M3 ? 2 * kInfos * (int)sizeof(TileInfo) : 0);
   static constexpr int kTotal = kBar + 1024 + 1024;
   static_assert(kTotal <= 232448, "ring and tiles must fit");
 };
@@ -88,11 +86,25 @@ template <int ROW>
 __device__ __forceinline__ uint32_t swizzled(uint32_t at) {
   return at ^ (ROW == 128 ? ((at >> 7) & 7) << 4 : ((at >> 7) & 3) << 4);
 }
-// two values as e4m3 pairs: the nearest, and the nearest to what is left
-__device__ __forceinline__ uint16_t half2_to_e4m3x2(uint32_t h) {
-  uint16_t c;
-  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(h));
-  return c;
+// four halves as e4m3 values: the nearest, and the nearest to what is left
+__device__ __forceinline__ void two_terms(uint32_t ha, uint32_t hb, uint32_t& first, uint32_t& second) {
+  uint32_t ba, bb;
+  asm("{\n\t.reg .b16 a, b;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 a, %3;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 b, %4;\n\t"
+      "mov.b32 %0, {a, b};\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, a;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %2, b;\n\t}\n"
+      : "=r"(first), "=r"(ba), "=r"(bb)
+      : "r"(ha), "r"(hb));
+  const __half2 ra = __hsub2(*reinterpret_cast<const __half2*>(&ha), *reinterpret_cast<const __half2*>(&ba));
+  const __half2 rb = __hsub2(*reinterpret_cast<const __half2*>(&hb), *reinterpret_cast<const __half2*>(&bb));
+  asm("{\n\t.reg .b16 a, b;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 a, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 b, %2;\n\t"
+      "mov.b32 %0, {a, b};\n\t}\n"
+      : "=r"(second)
+      : "r"(*reinterpret_cast<const uint32_t*>(&ra)), "r"(*reinterpret_cast<const uint32_t*>(&rb)));
 }
 
 template <bool QBF16, bool E4M3, int D, bool PAIR>
@@ -152,7 +164,6 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
   }
-  if (E4M3 && threadIdx.x < 64) reinterpret_cast<float*>(smem + L::kOnes)[threadIdx.x] = 1.f;
   if (warp == kWarpMma) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -367,7 +378,7 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
                 top = max(top, e[i]);
                 low = min(low, e[i] <= 1u ? 255u : e[i]);
                 info->k[key] = key < left ? scale_of(scales[key]) : 1.f;
-                info->raw[key] = (uint8_t)e[i];
+                info->log2_v[key] = e[i] == 255u ? __uint_as_float(0x7fc00000u) : (float)((int)e[i] - 127);
               }
               top = __reduce_max_sync(0xffffffffu, top);
               low = __reduce_min_sync(0xffffffffu, low);
@@ -465,36 +476,42 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
         constexpr int kPieces = D / 8 / (PAIR ? 1 : 2);
         const int first = PAIR ? 0 : q * kPieces;
         if (!E4M3) {
-#pragma unroll 4
-          for (int i = first; i < first + kPieces; ++i) {
-            uint4 x = valid ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
-            x = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
-            *reinterpret_cast<uint4*>(tile + (i >> 3) * kBoxBytes + row * 128 + (((i & 7) ^ (row & 7)) << 4)) = x;
+          uint4 x[kPieces];
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) x[i] = valid ? __ldg(src + first + i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) {
+            const int at = first + i;
+            *reinterpret_cast<uint4*>(tile + (at >> 3) * kBoxBytes + row * 128 + (((at & 7) ^ (row & 7)) << 4)) =
+                make_uint4(x[i].x ^ flip, x[i].y ^ flip, x[i].z ^ flip, x[i].w ^ flip);
           }
         } else {
           auto pair_of = [&](uint32_t y) {
             return QBF16 ? make_float2(__uint_as_float(y << 16), __uint_as_float(y & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&y));
           };
-          float most = 0.f;
-#pragma unroll 4
-          for (int i = 0; i < D / 8; ++i) {
-            const uint4 x = valid ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
-            const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+          uint4 x[D / 8];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) most = max3f(most, fabsf(pair_of(y[n]).x), fabsf(pair_of(y[n]).y));
+          for (int i = 0; i < D / 8; ++i) x[i] = valid ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+          uint32_t most = 0;  // magnitudes of 16-bit floats compare as integers
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            const uint32_t y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+            for (int n = 0; n < 4; ++n) most = __vmaxu2(most, y[n] & 0x7fff7fffu);
           }
+          most = max(most & 0xffffu, most >> 16);
           // scaled by a power of two to a largest magnitude in [128, 256)
-          const uint32_t e = min(max(__float_as_uint(most) >> 23, 9u), 253u);
+          const uint32_t e = min(max(__float_as_uint(pair_of(most).x) >> 23, 9u), 253u);
           const float up = __uint_as_float((254u + 7u - e) << 23);
           row_scale *= __uint_as_float((e - 7u) << 23);
-#pragma unroll 1
-          for (int i = first / 2; i < (first + kPieces) / 2; ++i) {  // 16 elements: 16 bytes of every term
-            const uint4 x0 = valid ? __ldg(src + 2 * i) : make_uint4(0, 0, 0, 0), x1 = valid ? __ldg(src + 2 * i + 1) : make_uint4(0, 0, 0, 0);
-            const uint32_t y[8] = {x0.x ^ flip, x0.y ^ flip, x0.z ^ flip, x0.w ^ flip, x1.x ^ flip, x1.y ^ flip, x1.z ^ flip, x1.w ^ flip};
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {  // 16 elements: 16 bytes of every term
+            if (!PAIR && i / (D / 32) != q) continue;
+            const uint32_t y[8] = {x[2 * i].x, x[2 * i].y, x[2 * i].z, x[2 * i].w, x[2 * i + 1].x, x[2 * i + 1].y, x[2 * i + 1].z, x[2 * i + 1].w};
             uint32_t term[3][4] = {};
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
-              float2 left = pair_of(y[n]);
+              float2 left = pair_of(y[n] ^ flip);
               left = make_float2(left.x * up, left.y * up);
               // (infinities would saturate: NaN, as their scores are)
               if (!(fabsf(left.x) <= FLT_MAX)) left.x = __uint_as_float(0x7fc00000u);
@@ -538,16 +555,7 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
         ++steps;
         tmem_ld_wait();
         const bool more = i + 1 < n_tiles;
-        const float* k_mul = nullptr;  // 8-bit: the scales of the keys, and of the values relative to 2^v_log2
-        const float* v_mul = nullptr;
-        float scale = row_scale, v_log2 = 0.f;
-        bool detour = tile >= w.first_masked;
-        if (E4M3) {
-          k_mul = info->k;
-          v_mul = info->v;
-          v_log2 = info->v_log2;
-          detour |= info->wide != 0;
-        }
+        const bool detour = tile >= w.first_masked || (E4M3 && info->wide != 0);
         constexpr float kThreshold = E4M3 ? kRescale8 : kRescaleThreshold;
         // Takes a new reference where it grew by more than the threshold: rare.  O is rescaled in tensor memory.
         auto settle = [&](float most) {
@@ -579,31 +587,85 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
           }
           l_sum = fmaf(sum, ex2f(unit - b_ref), l_sum);
         };
-        float unit = 0.f;  // the exponentials are 2^(score - unit)
-        if (detour) {
-          // What the row sees of the tile's keys, a bit a key.  The warp's rows belong to a few neighbouring tokens: the warp reads each
-          // one's mask side by side, four tokens' at a time.
-          uint32_t see[2] = {0, 0};
-          const int ahead0 = tile * BN - seq.length;
-          const int t0 = __shfl_sync(0xffffffffu, i_new, 0), t1 = __reduce_max_sync(0xffffffffu, i_new);
-#pragma unroll 1
-          for (int t = min(t0, t1); t <= t1; t += 4) {
-            bool lo[4], hi[4];
+        uint32_t pk0[16], pk1[16];  // the weights' first and second 32 keys (16-bit), or first and second terms
+        if (!detour) {
+          if (E4M3) {
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              lo[n] = t + n <= t1 && sees(p, seq, t + n, ahead0 + lane);
-              hi[n] = t + n <= t1 && sees(p, seq, t + n, ahead0 + 32 + lane);
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float4 f = *reinterpret_cast<const float4*>(info->k + x * 32 + e * 4);
+                const float2 lo = mul2_rn(make_float2(__uint_as_float(sr[x][4 * e]), __uint_as_float(sr[x][4 * e + 1])), make_float2(f.x, f.y));
+                const float2 hi = mul2_rn(make_float2(__uint_as_float(sr[x][4 * e + 2]), __uint_as_float(sr[x][4 * e + 3])), make_float2(f.z, f.w));
+                sr[x][4 * e] = __float_as_uint(lo.x); sr[x][4 * e + 1] = __float_as_uint(lo.y);
+                sr[x][4 * e + 2] = __float_as_uint(hi.x); sr[x][4 * e + 3] = __float_as_uint(hi.y);
+              }
+          }
+          float mxc[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains of the row maximum
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              mxc[2 * x + (e & 1)] = max3f(mxc[2 * x + (e & 1)], __uint_as_float(sr[x][2 * e]), __uint_as_float(sr[x][2 * e + 1]));
+          const float mx = max3f(mxc[0], mxc[1], fmaxf(mxc[2], mxc[3])) * row_scale;
+          const float v_log2 = E4M3 ? info->v_log2 : 0.f;
+          settle(E4M3 ? mx + v_log2 : mx);
+          if (!ok) break;
+          const float unit = E4M3 ? a_ref - v_log2 - kTop8 : a_ref;  // the exponentials are 2^(score - unit)
+          const float2 scale2 = make_float2(row_scale, row_scale), neg2 = make_float2(-unit, -unit);
+          float2 sa = make_float2(0.f, 0.f), sb = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            // 16-bit: a pair of either half; 8-bit: four neighbouring keys
+            const int xa = E4M3 ? e >> 3 : 0, xb = E4M3 ? e >> 3 : 1, ya = E4M3 ? (e & 7) * 4 : 2 * e, yb = E4M3 ? ya + 2 : 2 * e;
+            const float2 ta = fma2(make_float2(__uint_as_float(sr[xa][ya]), __uint_as_float(sr[xa][ya + 1])), scale2, neg2);
+            const float2 tb = fma2(make_float2(__uint_as_float(sr[xb][yb]), __uint_as_float(sr[xb][yb + 1])), scale2, neg2);
+            float2 ea = make_float2(ex2f(ta.x), ex2f(ta.y));
+            float2 eb = make_float2(ex2f(tb.x), ex2f(tb.y));
+            sa = add2(sa, ea);
+            sb = add2(sb, eb);
+            if (!E4M3) {
+              pk0[e] = pack16<QBF16>(ea.x, ea.y);
+              pk1[e] = pack16<QBF16>(eb.x, eb.y);
+            } else {
+              const float4 f = *reinterpret_cast<const float4*>(info->v + e * 4);
+              ea = mul2_rn(ea, make_float2(f.x, f.y));
+              eb = mul2_rn(eb, make_float2(f.z, f.w));
+              two_terms(pack16<false>(ea.x, ea.y), pack16<false>(eb.x, eb.y), pk0[e], pk1[e]);
             }
+          }
+          const float2 tot = add2(sa, sb);
+          if (E4M3) add_sum(tot.x + tot.y, unit); else l_sum += tot.x + tot.y;
+        } else {
+          // What the row sees of the tile's keys, a bit a key.  The warp's rows belong to a few neighbouring tokens: the warp reads each
+          // one's mask side by side, eight tokens' at a time.
+          uint32_t see[2] = {0, 0};
+          {
+            const int a0 = tile * BN - seq.length + lane, a1 = a0 + 32;  // the lane's two keys, counted from the first new token
+            const int width = p.mask ? min(p.mask_width, seq.count) : seq.count;
+            const bool may0 = a0 >= 0 && a0 < width, may1 = a1 >= 0 && a1 < width;
+            const int t0 = __shfl_sync(0xffffffffu, i_new, 0), t1 = __reduce_max_sync(0xffffffffu, i_new);
+#pragma unroll 1
+            for (int t = min(t0, t1); t <= t1; t += 8) {
+              bool lo[8], hi[8];
+              const uint8_t* m = p.mask + (int64_t)(seq.first + t) * p.mask_stride;
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              const uint32_t l = __ballot_sync(0xffffffffu, lo[n]), h = __ballot_sync(0xffffffffu, hi[n]);
-              if (t + n == i_new) {
-                see[0] = l;
-                see[1] = h;
+              for (int n = 0; n < 8; ++n, m += p.mask_stride) {
+                const bool there = t + n <= t1;
+                lo[n] = a0 < 0 || (there && may0 && (p.mask ? __ldg(m + a0) != 0 : a0 <= t + n));
+                hi[n] = a1 < 0 || (there && may1 && (p.mask ? __ldg(m + a1) != 0 : a1 <= t + n));
+              }
+#pragma unroll
+              for (int n = 0; n < 8; ++n) {
+                const uint32_t l = __ballot_sync(0xffffffffu, lo[n]), h = __ballot_sync(0xffffffffu, hi[n]);
+                if (t + n == i_new) {
+                  see[0] = l;
+                  see[1] = h;
+                }
               }
             }
           }
-          // The scores, scaled, in tensor memory; -inf for what the row does not see.
+          // In rolled loops over 16 keys: the scores, scaled, in tensor memory again, -inf for what the row does not see; their maxima.
           float mx = -INFINITY, mw = -INFINITY;  // largest score, largest score plus scale of the value
 #pragma unroll 1
           for (int x = 0; x < BN / 16; ++x) {
@@ -613,118 +675,60 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
             const uint32_t bits = (x & 2 ? see[1] : see[0]) >> (16 * (x & 1));
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              float v = __uint_as_float(y[e]) * (E4M3 ? k_mul[x * 16 + e] * scale : scale);
+              float v = __uint_as_float(y[e]) * (E4M3 ? info->k[x * 16 + e] * row_scale : row_scale);
               if (!((bits >> e) & 1u)) v = -INFINITY;
               y[e] = __float_as_uint(v);
-              if (E4M3) {
-                const unsigned ev = info->raw[x * 16 + e];
-                mx = fmaxf(mx, v);
-                mw = fmaxf(mw, v + (ev == 255u ? __uint_as_float(0x7fc00000u) : (float)((int)ev - 127)));
-              }
+              mx = fmaxf(mx, v);
+              if (E4M3) mw = fmaxf(mw, v + info->log2_v[x * 16 + e]);
             }
             tmem_st_32x32b_x16(t_s + buf * BN + x * 16, y);
           }
           tmem_st_wait();
-          if (E4M3) {
-            // the row sum here; then what the weights' exponents are, in the scores' place
-            settle(mw);
-            if (!ok) break;
-            if (mx > b_ref) {
-              l_sum *= ex2f(b_ref - mx);
-              b_ref = mx;
-            }
-            float sum = 0.f;
-#pragma unroll 1
-            for (int x = 0; x < BN / 16; ++x) {
-              uint32_t y[16];
-              tmem_ld_32x32b_x16(t_s + buf * BN + x * 16, y);
-              tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const float v = __uint_as_float(y[e]);
-                const unsigned ev = info->raw[x * 16 + e];
-                sum += ex2f(v - b_ref);
-                const float to = v + (ev == 255u ? __uint_as_float(0x7fc00000u) : (float)((int)ev - 127)) - a_ref + kTop8;
-                y[e] = __float_as_uint(v == -INFINITY ? -INFINITY : to);  // (what is not seen weighs nothing, whatever its value's scale)
-              }
-              tmem_st_32x32b_x16(t_s + buf * BN + x * 16, y);
-            }
-            tmem_st_wait();
-            l_sum += sum;
-            k_mul = v_mul = reinterpret_cast<const float*>(smem + L::kOnes);
+          settle(E4M3 ? mw : mx);
+          if (!ok) break;
+          if (E4M3 && mx > b_ref) {
+            l_sum *= ex2f(b_ref - mx);
+            b_ref = mx;
           }
-          scale = 1.f;
+          // the weights; what the loop makes of 16 keys is put into its place by selection, since P is written where scores still are
+          float sum = 0.f;
 #pragma unroll
-          for (int x = 0; x < 2; ++x) tmem_ld_32x32b_x32(t_s + buf * BN + x * 32, sr[x]);
-          tmem_ld_wait();
-        }
-        if (E4M3) {
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
+          for (int e = 0; e < 16; ++e) pk0[e] = pk1[e] = 0;
+#pragma unroll 1
+          for (int x = 0; x < BN / 16; ++x) {
+            uint32_t y[16], a[8], b2[4];
+            tmem_ld_32x32b_x16(t_s + buf * BN + x * 16, y);
+            tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const float4 f = *reinterpret_cast<const float4*>(k_mul + x * 32 + e * 4);
-              float2 lo = make_float2(__uint_as_float(sr[x][4 * e]), __uint_as_float(sr[x][4 * e + 1]));
-              float2 hi = make_float2(__uint_as_float(sr[x][4 * e + 2]), __uint_as_float(sr[x][4 * e + 3]));
-              lo = mul2_rn(lo, make_float2(f.x, f.y));
-              hi = mul2_rn(hi, make_float2(f.z, f.w));
-              sr[x][4 * e] = __float_as_uint(lo.x); sr[x][4 * e + 1] = __float_as_uint(lo.y);
-              sr[x][4 * e + 2] = __float_as_uint(hi.x); sr[x][4 * e + 3] = __float_as_uint(hi.y);
+              float wgt[2];
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                const float v = __uint_as_float(y[2 * e + n]);
+                const float pr = ex2f(v - (E4M3 ? b_ref : a_ref));
+                sum += pr;
+                // (what is not seen weighs nothing, whatever its value's scale is)
+                wgt[n] = !E4M3 ? pr : v == -INFINITY ? 0.f : ex2f(v + info->log2_v[x * 16 + 2 * e + n] - a_ref + kTop8);
+              }
+              a[e] = pack16<QBF16 && !E4M3>(wgt[0], wgt[1]);
             }
-        }
-        if (!E4M3 || !detour) {
-          float mxc[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains of the row maximum
+            if (E4M3) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
+              for (int e = 0; e < 4; ++e) two_terms(a[2 * e], a[2 * e + 1], a[e], b2[e]);
+            }
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-              mxc[2 * x + (e & 1)] = max3f(mxc[2 * x + (e & 1)], __uint_as_float(sr[x][2 * e]), __uint_as_float(sr[x][2 * e + 1]));
-          const float mx = max3f(mxc[0], mxc[1], fmaxf(mxc[2], mxc[3])) * scale;
-          settle(E4M3 ? mx + v_log2 : mx);
-          if (!ok) break;
-          unit = E4M3 ? a_ref - v_log2 - kTop8 : a_ref;
-        }
-        uint32_t pk0[16], pk1[16];  // the weights' first and second 32 keys (16-bit), or first and second terms
-        const float2 scale2 = make_float2(scale, scale), neg2 = make_float2(-unit, -unit);
-        float2 sa = make_float2(0.f, 0.f), sb = make_float2(0.f, 0.f);
-        if (!E4M3) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float2 xa = fma2(make_float2(__uint_as_float(sr[0][2 * e]), __uint_as_float(sr[0][2 * e + 1])), scale2, neg2);
-            const float2 xb = fma2(make_float2(__uint_as_float(sr[1][2 * e]), __uint_as_float(sr[1][2 * e + 1])), scale2, neg2);
-            const float2 ea = make_float2(ex2f(xa.x), ex2f(xa.y));
-            const float2 eb = make_float2(ex2f(xb.x), ex2f(xb.y));
-            sa = add2(sa, ea);
-            sb = add2(sb, eb);
-            pk0[e] = pack16<QBF16>(ea.x, ea.y);
-            pk1[e] = pack16<QBF16>(eb.x, eb.y);
+            for (int e = 0; e < 16; ++e) {
+              if (E4M3) {
+                pk0[e] = e / 4 == x ? a[e % 4] : pk0[e];
+                pk1[e] = e / 4 == x ? b2[e % 4] : pk1[e];
+              } else {
+                pk0[e] = e / 8 == x ? a[e % 8] : pk0[e];
+                pk1[e] = e / 8 + 2 == x ? a[e % 8] : pk1[e];
+              }
+            }
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {  // four keys
-            const int x = e >> 3, y = (e & 7) * 4;
-            const float2 xa = fma2(make_float2(__uint_as_float(sr[x][y]), __uint_as_float(sr[x][y + 1])), scale2, neg2);
-            const float2 xb = fma2(make_float2(__uint_as_float(sr[x][y + 2]), __uint_as_float(sr[x][y + 3])), scale2, neg2);
-            float2 ea = make_float2(ex2f(xa.x), ex2f(xa.y));
-            float2 eb = make_float2(ex2f(xb.x), ex2f(xb.y));
-            sa = add2(sa, ea);
-            sb = add2(sb, eb);
-            const float4 f = *reinterpret_cast<const float4*>(v_mul + e * 4);
-            ea = mul2_rn(ea, make_float2(f.x, f.y));
-            eb = mul2_rn(eb, make_float2(f.z, f.w));
-            const uint32_t ha = pack16<false>(ea.x, ea.y), hb = pack16<false>(eb.x, eb.y);
-            const uint32_t c0 = half2_to_e4m3x2(ha), c1 = half2_to_e4m3x2(hb);
-            const uint32_t ba = e4m3x2_to_half2(c0), bb = e4m3x2_to_half2(c1);
-            const __half2 ra = __hsub2(*reinterpret_cast<const __half2*>(&ha), *reinterpret_cast<const __half2*>(&ba));
-            const __half2 rb = __hsub2(*reinterpret_cast<const __half2*>(&hb), *reinterpret_cast<const __half2*>(&bb));
-            pk0[e] = c0 | (c1 << 16);
-            pk1[e] = (uint32_t)half2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&ra)) |
-                     ((uint32_t)half2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&rb)) << 16);
-          }
+          l_sum += sum;
         }
-        const float2 tot = add2(sa, sb);
-        if (!E4M3) l_sum += tot.x + tot.y;
-        else if (!detour) add_sum(tot.x + tot.y, unit);
         // (the scores read ahead take the registers of this tile's)
         const bool ahead = __all_sync(0xffffffffu, more && mbar_test(&s_full[2 * q + (steps & 1)], (steps >> 1) & 1));
         if (ahead) load_scores();
@@ -768,6 +772,9 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
       const int part_row = (PAIR ? q * BM : 0) + row;
       const bool has_rows = PAIR ? q * BM < w.rows : true;
       if (has_rows) {
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        uint16_t* const out = static_cast<uint16_t*>(p.out) + (int64_t)(seq.first + i_new) * p.out_row +
+                              (int64_t)(c.h * p.group + (valid ? r - i_new * p.group : 0)) * p.out_head;
         const bool bad = bad_values[items & 7] == (uint32_t)items + 1;
         constexpr int kChunks = D / 32 / (PAIR ? 1 : 2);  // of 32 columns: each group stores half where they share the rows
         for (int x = PAIR ? 0 : q * kChunks; x < (PAIR ? kChunks : (q + 1) * kChunks); ++x) {
@@ -810,11 +817,11 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
             }
           }
           if (valid) {
+            if (whole) {
+              store_row32<QBF16, E4M3>(out, x, o, inv);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float4 v = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
-              if (whole) store_row4<QBF16, E4M3>(p, seq.first, c.h, r, x * 8 + e, v, l);
-              else __stcg(reinterpret_cast<float4*>(part + (size_t)part_row * D) + x * 8 + e, v);
+              for (int e = 0; e < 4; ++e) store32(part + (size_t)part_row * D + x * 32 + e * 8, o + e * 8);
             }
           }
         }

@@ -344,7 +344,7 @@ int frisk_b200_cache_read(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* cach
  * itself).  Query head h reads key head h / (heads_q / heads).  A row that sees no key is zero.  What a row does not see
  * does not reach it, whatever it holds.  dtype: F16 or BF16, of q and out, and of a 16-bit cache.  max_new is a hint: the
  * largest number of new tokens of a sequence (0: unknown); it bears on speed only.
- * The workspace (16-byte aligned, contents of no matter before and after) must not be shared by calls that may overlap. */
+ * The workspace (32-byte aligned, contents of no matter before and after) must not be shared by calls that may overlap. */
 typedef struct frisk_b200_cache_attn_desc {
   int32_t heads_q, dtype, max_new, mask_width;
   int64_t mask_stride;

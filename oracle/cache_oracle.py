@@ -103,7 +103,7 @@ def attention(cache, q, table, starts, lengths, mask=None, scale=None, terms=Fal
 
     ``terms``: an 8-bit cache whose products take e4m3 sums.  A weight of two terms, the first off by 2^-4 of it at most and the second by
     2^-4 of the rest, is off by 2^-8, or by half of the smallest e4m3 step, 2^-10, where the largest probability times the largest
-    scale of the values stands at 2^7 or more.  A query's terms leave 2^-10 of a row scaled to 128 or more."""
+    scale of the values stands at 2^5.75 or more.  A query's terms leave 2^-10 of a row scaled to 128 or more."""
     n, heads_q, d = q.shape
     heads, page = cache[0].shape[1], cache[0].shape[2]
     group, scale = heads_q // heads, d ** -0.5 if scale is None else scale
@@ -144,6 +144,6 @@ def attention(cache, q, table, starts, lengths, mask=None, scale=None, terms=Fal
                 e = cache[3][at, h // group, j % page].double()
                 e = torch.where(see.any(0) & (e < 255), e, 0.0)
                 codes = torch.where(torch.isfinite(v), v, 0.0).abs() * torch.exp2(127 - e)[:, None] * (e > 0)[:, None]
-                far = far + 2.0 ** -17 * p.nan_to_num().amax(1, keepdim=True) * 2.0 ** (float(e.max()) - 127) * codes.sum(0)[None]
+                far = far + 2.0 ** -15.75 * p.nan_to_num().amax(1, keepdim=True) * 2.0 ** (float(e.max()) - 127) * codes.sum(0)[None]
             bound[first:first + rows, h] = h_p * a + delta * a + h_out * (o.abs() + (h_p + delta) * a) + far + 1e-30
     return out, bound
