@@ -289,6 +289,17 @@ __global__ void __launch_bounds__(32 * (warps_of<E4M3>() + 1), 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
         float v_exp[2][2];  // 8-bit: log2 of the scale of this lane's values, by n and column
+        // 8-bit values, transposed pairs of codes: a register has the codes of columns 2n, 2n + 1 for two keys.  They are read along with
+        // the keys, since what follows has latency enough.
+        uint32_t vf8[E4M3 ? D / 32 : 1][4];
+        auto load_values = [&]() {
+          const int key = part_keys + (mat & 1) * 8 + key_of(mrow);
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) {
+            const uint32_t at = key * D + (2 * j + (mat >> 1)) * 16;
+            ldsm4_trans(vf8[j], sv + (at ^ (((at >> 7) & 7) << 4)));
+          }
+        };
         if (!E4M3) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
@@ -310,6 +321,7 @@ __global__ void __launch_bounds__(32 * (warps_of<E4M3>() + 1), 1)
               const uint32_t at = (part_keys + n * 8 + key_of(g)) * D + b * 64 + tq * 16;
               raw[n][b] = lds128(sk + (at ^ (((at >> 7) & 7) << 4)));
             }
+          load_values();
           float k_scale[2][2];
 #pragma unroll
           for (int n = 0; n < 2; ++n)
@@ -403,6 +415,7 @@ __global__ void __launch_bounds__(32 * (warps_of<E4M3>() + 1), 1)
           }
           fence_proxy_async_smem();  // (the stage's next load comes after these)
           __syncwarp();
+          if (E4M3) load_values();
         }
         float m_new[2], a_new[2];
         bool grow = false;
@@ -472,21 +485,15 @@ __global__ void __launch_bounds__(32 * (warps_of<E4M3>() + 1), 1)
             mma16816<MBF16>(o[2 * j + 1], pf, vf[2], vf[3]);
           }
         } else {
-          // transposed pairs of codes: a register has the codes of columns 2n, 2n + 1 for two keys.  Even and odd columns go to
-          // product tiles of their own: tile 2u has the columns 16u + 2n, tile 2u + 1 the columns 16u + 2n + 1.
-          const int key = part_keys + (mat & 1) * 8 + key_of(mrow);
+          // Even and odd columns go to product tiles of their own: tile 2u has the columns 16u + 2n, tile 2u + 1 the columns 16u + 2n + 1.
 #pragma unroll
-          for (int j = 0; j < D / 32; ++j) {
-            const uint32_t at = key * D + (2 * j + (mat >> 1)) * 16;
-            uint32_t vf[4];
-            ldsm4_trans(vf, sv + (at ^ (((at >> 7) & 7) << 4)));
+          for (int j = 0; j < D / 32; ++j)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              const uint32_t r0 = __byte_perm(vf[2 * u], 0, 0x3120), r1 = __byte_perm(vf[2 * u + 1], 0, 0x3120);
+              const uint32_t r0 = __byte_perm(vf8[j][2 * u], 0, 0x3120), r1 = __byte_perm(vf8[j][2 * u + 1], 0, 0x3120);
               mma16816<false>(o[(2 * j + u) * 2], pf, e4m3x2_to_half2(r0), e4m3x2_to_half2(r1));
               mma16816<false>(o[(2 * j + u) * 2 + 1], pf, e4m3x2_to_half2_hi(r0), e4m3x2_to_half2_hi(r1));
             }
-          }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty_bar[stage]);

@@ -252,8 +252,10 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
       }
     } else if (warp == kWarpMma || warp == kWarpMma + 1) {
       // ------------------------------------------------------------------ MMA issuers, one warp per softmax group
-      // tcgen05 operations of ONE thread execute in issue order: S(b + 2) overwrites P(b) after P(b).V(b) has read it.  The two warps
-      // issue in turn, so that one's waits lie behind the other's MMAs; one elected lane issues.
+      // tcgen05 operations of ONE thread execute in issue order: S(b + 2) overwrites P(b) after P(b).V(b) has read it.  With 16-bit caches the
+      // two warps issue in turn, so that one's waits lie behind the other's MMAs (64 new tokens over 8 x 32000 keys 462 -> 424 us); with 8-bit
+      // ones the softmax groups are slower than the MMAs, and turns would tie them together (24 over 16 x 6000 keys 115 -> 121).  One
+      // elected lane issues.
       const int mq = __shfl_sync(0xffffffffu, warp - kWarpMma, 0);
       // (kind::f8f6f4 has the fields of kind::f16; type 0 is e4m3 there)
       constexpr uint32_t idesc_s = umma_idesc_f16(BM, BN, QBF16 && !E4M3, false, false);
@@ -272,7 +274,7 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
         const Work w = work_of(c);
         const int n_mine = w.nq[mq], n_max = OWN_KV ? n_mine : w.n;  // key tiles: used, followed
         const int n_steps = w.nq[0];                                  // the same for both MMA warps
-        const bool in_turn = w.nq[1] > 0;                             // a lone warp issues as it comes
+        const bool in_turn = !E4M3 && w.nq[1] > 0;                    // a lone warp issues as it comes
         // (a barrier whose item has no key tile for this warp is neither arrived on nor waited for: the warp could be items behind)
         if (n_mine > 0) {
           ok = mbar_wait_warp(&q_full[mq], items & 1, abort_flag, p.status, ST_CACHE_Q);

@@ -1,9 +1,10 @@
 // Writing new rows into the paged cache, quantised on the way where it holds 8-bit floats, and reading rows back.
 //
 // A head's row is D elements: 16 bytes of the 16-bit side a lane, D / 8 neighbouring lanes a row, so the largest magnitude of a row
-// takes three or four shuffles and nothing passes through shared memory.  Bound by HBM: each side is read or written once.  A block
-// takes one packed row at a time, its keys and values, and finds the row's place (its sequence by bisection of `starts`, then the
-// page) while the row itself is on its way; few rows are few blocks, and the chain starts -> lengths -> table is what a call costs then.
+// takes three or four shuffles and nothing passes through shared memory.  Bound by HBM: each side is read or written once.  A block takes
+// up to 16 packed rows: a thread finds the place of each (its sequence by bisection of `starts`, then the page; a chain of dependent
+// loads), then all threads move the pieces of all of them, four at a time.  (One row at a time, 52 thousand rows of 4 heads of 64 took
+// 102 us.)  Fewer rows a block where that leaves SMs idle: a few rows cost the chain starts -> lengths -> table and little else.
 #include <algorithm>
 
 #include "cache_common.cuh"
@@ -13,6 +14,8 @@ namespace {
 using namespace cache;
 
 constexpr int kThreads = 256;
+constexpr int kMaxRows = 16;  // packed rows a block
+constexpr int kAhead = 4;     // pieces a thread has in flight
 
 struct Side {  // packed rows outside the cache, 16-bit
   void* ptr;
@@ -24,6 +27,7 @@ struct RowsParams {
   void *ck, *cv;           // pages
   uint8_t *ek, *ev;        // exponents
   int64_t rows;
+  int rows_block;
   unsigned* status;
 };
 
@@ -65,34 +69,59 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
 template <bool BF16, int D, bool E4M3, bool WRITE>
 __global__ void __launch_bounds__(kThreads) cache_rows_kernel(const RowsParams p) {
   constexpr int kLanes = D / 8;  // of a row
-  const int sub = threadIdx.x % kLanes;
-  const int units = 2 * p.t.heads;  // K and V rows of a token
+  __shared__ int64_t bases[kMaxRows];
+  const int64_t row0 = (int64_t)blockIdx.x * p.rows_block;
+  const int here = (int)min((int64_t)p.rows_block, p.rows - row0);
+  const int per_row = 2 * p.t.heads * kLanes;  // pieces of a token: keys, then values
+  const int total = here * per_row;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
-    // (whole groups of kLanes threads take the same unit, and whole warps the same number of rounds: the shuffles below need them)
-    for (int u0 = 0; u0 < units; u0 += kThreads / kLanes) {
-      const int u = u0 + threadIdx.x / kLanes;
-      const bool mine = u < units;
-      const bool values = u >= p.t.heads;
-      const int h = values ? u - p.t.heads : u;
-      const Side& side = values ? p.v : p.k;
-      uint4* packed = reinterpret_cast<uint4*>(static_cast<uint16_t*>(side.ptr) + r * side.row + h * side.head) + sub;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (WRITE && mine) x = __ldg(packed);
-      const int64_t base = locate(p.t, r, p.status);
-      if (base < 0) continue;  // (the same for the whole block)
-      const int64_t token = base + ((int64_t)h << p.t.page_log2);
-      void* pages = values ? p.cv : p.ck;
-      uint8_t* exponents = values ? p.ev : p.ek;
+  if ((int)threadIdx.x < here) bases[threadIdx.x] = locate(p.t, row0 + threadIdx.x, p.status);
+  __syncthreads();
+  // (whole groups of kLanes threads have the same head's row, and whole warps the same number of rounds: the shuffles below need them)
+  for (int e0 = 0; e0 < total; e0 += kThreads * kAhead) {
+    uint4 x[kAhead];       // the 16-bit side, or the cache's piece
+    uint32_t e_byte[kAhead];
+    int64_t token[kAhead];  // -1: nothing to do
+    uint4* packed[kAhead];
+    bool values[kAhead];
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) {
+      const int e = e0 + n * kThreads + threadIdx.x;
+      const bool mine = e < total;
+      const int r = mine ? e / per_row : 0, unit = (mine ? e - r * per_row : 0) / kLanes, sub = threadIdx.x % kLanes;
+      values[n] = unit >= p.t.heads;
+      const int h = values[n] ? unit - p.t.heads : unit;
+      const Side& side = values[n] ? p.v : p.k;
+      packed[n] = reinterpret_cast<uint4*>(static_cast<uint16_t*>(side.ptr) + (row0 + r) * side.row + h * side.head) + sub;
+      const int64_t base = bases[r];
+      token[n] = mine && base >= 0 ? base + ((int64_t)h << p.t.page_log2) : -1;
+      x[n] = make_uint4(0, 0, 0, 0);
+      e_byte[n] = 0;
+      if (token[n] < 0) continue;
+      const void* pages = values[n] ? p.cv : p.ck;
+      if (WRITE) {
+        x[n] = __ldcs(packed[n]);
+      } else if (!E4M3) {
+        x[n] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(pages) + token[n] * D) + sub);
+      } else {
+        const uint2 code = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pages) + token[n] * D) + sub);
+        x[n].x = code.x;
+        x[n].y = code.y;
+        e_byte[n] = __ldg((values[n] ? p.ev : p.ek) + token[n]);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) {
+      const int sub = threadIdx.x % kLanes;
+      void* pages = values[n] ? p.cv : p.ck;
       if (!E4M3) {
-        uint4* held = reinterpret_cast<uint4*>(static_cast<uint16_t*>(pages) + token * D) + sub;
-        if (mine) {
-          if (WRITE) *held = x; else *packed = __ldg(held);
-        }
+        if (token[n] < 0) continue;
+        if (WRITE) reinterpret_cast<uint4*>(static_cast<uint16_t*>(pages) + token[n] * D)[sub] = x[n];
+        else __stcs(packed[n], x[n]);
       } else if (WRITE) {
         float f[8];
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        const uint32_t w[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
         uint32_t most = 0;  // magnitudes compare as integers; infinities and NaN are the largest
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -106,46 +135,41 @@ __global__ void __launch_bounds__(kThreads) cache_rows_kernel(const RowsParams p
         // most = 1.m * 2^(E - 127) and 448 = 1.75 * 2^8: the least e with most <= 448 * 2^(e - 127)
         int e = (int)(most >> 23) - 8 + ((most & 0x7fffffu) > 0x600000u ? 1 : 0);
         e = most >= 0x7f800000u ? 255 : max(e, 1);
-        if (mine) {
-          uint32_t code[2] = {0, 0};
-          if (e != 255) {
-            const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+        if (token[n] < 0) continue;
+        uint32_t code[2] = {0, 0};
+        if (e != 255) {
+          const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              code[i >> 1] |= (uint32_t)float2_to_e4m3x2(f[2 * i] * inv, f[2 * i + 1] * inv) << (16 * (i & 1));
-          }
-          reinterpret_cast<uint2*>(static_cast<uint8_t*>(pages) + token * D)[sub] = make_uint2(code[0], code[1]);
-          if (sub == 0) exponents[token] = (uint8_t)e;
+          for (int i = 0; i < 4; ++i)
+            code[i >> 1] |= (uint32_t)float2_to_e4m3x2(f[2 * i] * inv, f[2 * i + 1] * inv) << (16 * (i & 1));
         }
-      } else if (mine) {
-        const uint2 code = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pages) + token * D) + sub);
-        const float scale = scale_of(__ldg(exponents + token));
-        const uint32_t c[2] = {code.x, code.y};
+        reinterpret_cast<uint2*>(static_cast<uint8_t*>(pages) + token[n] * D)[sub] = make_uint2(code[0], code[1]);
+        if (sub == 0) (values[n] ? p.ev : p.ek)[token[n]] = (uint8_t)e;
+      } else {
+        if (token[n] < 0) continue;
+        const float scale = scale_of(e_byte[n]);
+        const uint32_t c[2] = {x[n].x, x[n].y};
         uint32_t o[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t h2 = i & 1 ? e4m3x2_to_half2_hi(c[i >> 1]) : e4m3x2_to_half2(c[i >> 1]);
-          float2 two = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-          two.x *= scale;
-          two.y *= scale;
+          const float2 two = __half22float2(*reinterpret_cast<const __half2*>(&h2));
           // a row near the end of the type's range may have been rounded beyond it
-          two.x = saturated<BF16>(two.x);
-          two.y = saturated<BF16>(two.y);
-          o[i] = pack16<BF16>(two.x, two.y);
+          o[i] = pack16<BF16>(saturated<BF16>(two.x * scale), saturated<BF16>(two.y * scale));
         }
-        *packed = make_uint4(o[0], o[1], o[2], o[3]);
+        __stcs(packed[n], make_uint4(o[0], o[1], o[2], o[3]));
       }
     }
   }
 }
 
 template <bool BF16, int D, bool E4M3, bool WRITE>
-cudaError_t launch(const frisk_b200_ctx* ctx, const RowsParams& p, cudaStream_t s) {
+cudaError_t launch(const RowsParams& p, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel waits (griddepcontrol.wait) itself
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)std::min<int64_t>(p.rows, (int64_t)ctx->num_sms * 8));
+  cfg.gridDim = dim3((unsigned)((p.rows + p.rows_block - 1) / p.rows_block));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = s;
   cfg.attrs = attr;
@@ -153,12 +177,12 @@ cudaError_t launch(const frisk_b200_ctx* ctx, const RowsParams& p, cudaStream_t 
   return cudaLaunchKernelEx(&cfg, cache_rows_kernel<BF16, D, E4M3, WRITE>, p);
 }
 template <bool WRITE>
-cudaError_t launch_any(const frisk_b200_ctx* ctx, const RowsParams& p, bool bf16, int D, bool e4m3, cudaStream_t s) {
+cudaError_t launch_any(const RowsParams& p, bool bf16, int D, bool e4m3, cudaStream_t s) {
   if (D == 64)
-    return bf16 ? (e4m3 ? launch<true, 64, true, WRITE>(ctx, p, s) : launch<true, 64, false, WRITE>(ctx, p, s))
-                : (e4m3 ? launch<false, 64, true, WRITE>(ctx, p, s) : launch<false, 64, false, WRITE>(ctx, p, s));
-  return bf16 ? (e4m3 ? launch<true, 128, true, WRITE>(ctx, p, s) : launch<true, 128, false, WRITE>(ctx, p, s))
-              : (e4m3 ? launch<false, 128, true, WRITE>(ctx, p, s) : launch<false, 128, false, WRITE>(ctx, p, s));
+    return bf16 ? (e4m3 ? launch<true, 64, true, WRITE>(p, s) : launch<true, 64, false, WRITE>(p, s))
+                : (e4m3 ? launch<false, 64, true, WRITE>(p, s) : launch<false, 64, false, WRITE>(p, s));
+  return bf16 ? (e4m3 ? launch<true, 128, true, WRITE>(p, s) : launch<true, 128, false, WRITE>(p, s))
+              : (e4m3 ? launch<false, 128, true, WRITE>(p, s) : launch<false, 128, false, WRITE>(p, s));
 }
 
 }  // namespace
@@ -266,10 +290,12 @@ static int cache_rows(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* c, int32
   p.ev = c->v_exponent;
   p.rows = c->rows;
   p.status = ctx->d_status;
+  p.rows_block = 1;
+  while (p.rows_block < kMaxRows && c->rows / (2 * p.rows_block) >= 4 * ctx->num_sms) p.rows_block *= 2;
   FB_DEVICE(ctx);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = dtype == FRISK_B200_BF16, e4m3 = c->dtype == FRISK_B200_E4M3;
-  FB_CUDA(ctx, write ? launch_any<true>(ctx, p, bf16, c->D, e4m3, s) : launch_any<false>(ctx, p, bf16, c->D, e4m3, s));
+  FB_CUDA(ctx, write ? launch_any<true>(p, bf16, c->D, e4m3, s) : launch_any<false>(p, bf16, c->D, e4m3, s));
   return 0;
 }
 

@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTokens = 8;
+constexpr int kAhead = 4;  // units a thread has in flight
 
 struct Part {  // queries or keys
   const void* in;
@@ -86,42 +87,70 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
     const bool copy = part.in != part.out;  // in place, what passes stays
     const int per_head = n_rot + (copy ? n_pass : 0);
     const int total = here * part.heads * per_head;
-#pragma unroll 2
-    for (int e = threadIdx.x; e < total; e += kThreads) {
-      const int u = e % per_head, th = e / per_head, h = th % part.heads, t = th / part.heads;
-      const T* in = static_cast<const T*>(part.in) + (row0 + t) * part.in_row + h * part.in_head;
-      T* out = static_cast<T*>(part.out) + (row0 + t) * part.out_row + h * part.out_head;
-      const float2* cs = angles + t * p.half;
-      if (u >= n_rot) {
-        const int at = 2 * p.half + (u - n_rot) * V;
-        *reinterpret_cast<Vec<T, V>*>(out + at) = *reinterpret_cast<const Vec<T, V>*>(in + at);
-      } else if (INTERLEAVED) {
-        if (V == 1) {
-          const float a = E::to(in[2 * u]), b = E::to(in[2 * u + 1]);
-          out[2 * u] = E::from(a * cs[u].x - b * cs[u].y);
-          out[2 * u + 1] = E::from(b * cs[u].x + a * cs[u].y);
-        } else {
-          Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(in + u * V);
+    if (total == 0) continue;
+    // this thread's unit, head and token, and what a step of all threads adds to them
+    int u = threadIdx.x % per_head, h = threadIdx.x / per_head % part.heads, t = threadIdx.x / per_head / part.heads;
+    const int du = kThreads % per_head, dh = kThreads / per_head % part.heads, dt = kThreads / per_head / part.heads;
+#pragma unroll 1
+    for (int e0 = threadIdx.x; e0 < total; e0 += kThreads * kAhead) {
+      Vec<T, V> x[kAhead], y[kAhead];
+      int us[kAhead];
+      T* out[kAhead];
+      const float2* cs[kAhead];
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        us[n] = e0 + n * kThreads < total ? u : -1;
+        if (us[n] >= 0) {
+          const T* in = static_cast<const T*>(part.in) + (row0 + t) * part.in_row + h * part.in_head;
+          out[n] = static_cast<T*>(part.out) + (row0 + t) * part.out_row + h * part.out_head;
+          cs[n] = angles + t * p.half;
+          const bool rotated = u < n_rot;
+          if (V == 1 && INTERLEAVED && rotated) {
+            x[n].v[0] = in[2 * u];
+            y[n].v[0] = in[2 * u + 1];
+          } else {
+            x[n] = *reinterpret_cast<const Vec<T, V>*>(in + (rotated ? u * V : 2 * p.half + (u - n_rot) * V));
+            if (!INTERLEAVED && rotated) y[n] = *reinterpret_cast<const Vec<T, V>*>(in + p.half + u * V);
+          }
+        }
+        u += du;
+        h += dh;
+        t += dt;
+        if (u >= per_head) {
+          u -= per_head;
+          ++h;
+        }
+        if (h >= part.heads) {
+          h -= part.heads;
+          ++t;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        const int un = us[n];
+        if (un < 0) continue;
+        if (un >= n_rot) {
+          *reinterpret_cast<Vec<T, V>*>(out[n] + 2 * p.half + (un - n_rot) * V) = x[n];
+        } else if (INTERLEAVED && V > 1) {
 #pragma unroll
           for (int i = 0; i < V / 2; ++i) {
-            const float2 r = cs[u * (V / 2) + i];
-            const float a = E::to(x.v[2 * i]), b = E::to(x.v[2 * i + 1]);
-            x.v[2 * i] = E::from(a * r.x - b * r.y);
-            x.v[2 * i + 1] = E::from(b * r.x + a * r.y);
+            const float2 r = cs[n][un * (V / 2) + i];
+            const float a = E::to(x[n].v[2 * i]), b = E::to(x[n].v[2 * i + 1]);
+            x[n].v[2 * i] = E::from(a * r.x - b * r.y);
+            x[n].v[2 * i + 1] = E::from(b * r.x + a * r.y);
           }
-          *reinterpret_cast<Vec<T, V>*>(out + u * V) = x;
-        }
-      } else {
-        Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(in + u * V), y = *reinterpret_cast<const Vec<T, V>*>(in + p.half + u * V);
+          *reinterpret_cast<Vec<T, V>*>(out[n] + un * V) = x[n];
+        } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float2 r = cs[u * V + i];
-          const float a = E::to(x.v[i]), b = E::to(y.v[i]);
-          x.v[i] = E::from(a * r.x - b * r.y);
-          y.v[i] = E::from(b * r.x + a * r.y);
+          for (int i = 0; i < V; ++i) {
+            const float2 r = cs[n][un * V + i];
+            const float a = E::to(x[n].v[i]), b = E::to(y[n].v[i]);
+            x[n].v[i] = E::from(a * r.x - b * r.y);
+            y[n].v[i] = E::from(b * r.x + a * r.y);
+          }
+          *reinterpret_cast<Vec<T, V>*>(out[n] + (INTERLEAVED ? 2 * un : un * V)) = x[n];
+          *reinterpret_cast<Vec<T, V>*>(out[n] + (INTERLEAVED ? 2 * un + 1 : p.half + un * V)) = y[n];
         }
-        *reinterpret_cast<Vec<T, V>*>(out + u * V) = x;
-        *reinterpret_cast<Vec<T, V>*>(out + p.half + u * V) = y;
       }
     }
   }
