@@ -10,18 +10,18 @@ step can be replayed with other contents.  Their contents are checked by the ker
 ``cache_check`` raises.  Rows before ``starts[0]`` and from ``starts[-1]`` on belong to no sequence and are left as they are.
 """
 import contextlib
-import math
 
 from . import capi
 from .execute import _stream_ptr, _torch, context_for
 
-_CODES = None
+_CODES = _BYTE = _INT = None
 
 
 def _codes():
-    global _CODES
+    global _CODES, _BYTE, _INT
     if _CODES is None:
         torch = _torch()
+        _BYTE, _INT = torch.uint8, torch.int32
         _CODES = {torch.float16: capi.F16, torch.bfloat16: capi.BF16, torch.float8_e4m3fn: capi.E4M3}
     return _CODES
 
@@ -34,13 +34,23 @@ def _on_stream(stream, device):
     return torch.cuda.stream(stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream), device=device))
 
 
+def _new_like(t):
+    """A dense new tensor of the shape, type and device of ``t``."""
+    torch = _torch()
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _refuse(what):
+    raise ValueError("frisk-b200-cache: " + what)
+
+
 def paged_cache(pages, heads, page, d, dtype, device="cuda"):
     """A new cache of ``pages`` pages of ``page`` tokens (a power of two from 16 to 1024) with heads of 64 or 128 elements."""
     torch = _torch()
     if dtype not in _codes():
-        raise ValueError("frisk-b200-cache: a cache holds float16, bfloat16 or float8_e4m3fn")
+        _refuse("a cache holds float16, bfloat16 or float8_e4m3fn")
     if pages < 1 or heads < 1 or page < 16 or page > 1024 or page & (page - 1) or d not in (64, 128):
-        raise ValueError("frisk-b200-cache: sizes outside the contract")
+        _refuse("sizes outside the contract")
     held = tuple(torch.zeros(pages, heads, page, d, dtype=dtype, device=device) for _ in range(2))
     if dtype != torch.float8_e4m3fn:
         return held
@@ -49,42 +59,49 @@ def paged_cache(pages, heads, page, d, dtype, device="cuda"):
 
 def _describe(cache, table, starts, lengths, rows):
     """(descriptor, element code, device index, key heads, D), checked."""
-    torch = _torch()
-    if len(cache) not in (2, 4):
-        raise ValueError("frisk-b200-cache: a cache is (k, v), or (k, v, k exponents, v exponents)")
-    k, v = cache[0], cache[1]
-    code, shape, dev = _codes().get(k.dtype), k.shape, k.get_device()
-    if code is None or (code == capi.E4M3) != (len(cache) == 4):
-        raise ValueError("frisk-b200-cache: a cache holds float16, bfloat16, or float8_e4m3fn with exponents")
-    if len(shape) != 4 or v.shape != shape or v.dtype != k.dtype or not k.is_contiguous() or not v.is_contiguous():
-        raise ValueError("frisk-b200-cache: keys and values must be dense [pages, heads, page, D] of one type")
+    codes = _CODES or _codes()
+    parts = len(cache)
+    if parts == 2:
+        k, v = cache
+        ek = ev = None
+    elif parts == 4:
+        k, v, ek, ev = cache
+    else:
+        _refuse("a cache is (k, v), or (k, v, k exponents, v exponents)")
+    dtype, shape, dev = k.dtype, k.shape, k.get_device()
+    code = codes.get(dtype)
+    if code is None or (code == capi.E4M3) != (parts == 4):
+        _refuse("a cache holds float16, bfloat16, or float8_e4m3fn with exponents")
+    if len(shape) != 4 or v.shape != shape or v.dtype != dtype or not k.is_contiguous() or not v.is_contiguous():
+        _refuse("keys and values must be dense [pages, heads, page, D] of one type")
     if dev < 0 or v.get_device() != dev:
-        raise ValueError("frisk-b200-cache: tensors must be on one CUDA device (there is no CPU path)")
-    exponents = (None, None)
-    if code == capi.E4M3:
-        for e in cache[2:]:
-            if e.dtype != torch.uint8 or e.shape != shape[:3] or not e.is_contiguous() or e.get_device() != dev:
-                raise ValueError("frisk-b200-cache: exponents must be dense uint8 [pages, heads, page] on the cache's device")
-        exponents = cache[2].data_ptr(), cache[3].data_ptr()
-    batch = lengths.shape[0] if len(lengths.shape) == 1 else -1
-    i32 = torch.int32
-    if batch < 0 or starts.shape != (batch + 1,) or len(table.shape) != 2 or table.shape[0] != batch or \
-            starts.dtype != i32 or lengths.dtype != i32 or table.dtype != i32:
-        raise ValueError("frisk-b200-cache: table, starts and lengths must be int32 [batch, width], [batch + 1] and [batch]")
-    if not starts.is_contiguous() or not lengths.is_contiguous() or (table.stride(1) != 1 and table.shape[1] > 1):
-        raise ValueError("frisk-b200-cache: starts, lengths and the rows of the table must be dense")
-    if starts.get_device() != dev or lengths.get_device() != dev or table.get_device() != dev:
-        raise ValueError("frisk-b200-cache: table, starts and lengths must be on the cache's device")
+        _refuse("tensors must be on one CUDA device (there is no CPU path)")
     pages, heads, page, d = shape
-    desc = capi.CacheDesc(pages, page, heads, d, code, batch, table.shape[1], table.stride(0), rows, k.data_ptr(), v.data_ptr(),
-                          *exponents, table.data_ptr(), starts.data_ptr(), lengths.data_ptr())
+    if parts == 4:
+        want = shape[:3]
+        for e in (ek, ev):
+            if e.dtype != _BYTE or e.shape != want or not e.is_contiguous() or e.get_device() != dev:
+                _refuse("exponents must be dense uint8 [pages, heads, page] on the cache's device")
+        ek, ev = ek.data_ptr(), ev.data_ptr()
+    l_shape, t_shape, s_shape = lengths.shape, table.shape, starts.shape
+    if len(l_shape) != 1 or len(t_shape) != 2 or len(s_shape) != 1 or t_shape[0] != l_shape[0] or s_shape[0] != l_shape[0] + 1 or \
+            starts.dtype != _INT or lengths.dtype != _INT or table.dtype != _INT:
+        _refuse("table, starts and lengths must be int32 [batch, width], [batch + 1] and [batch]")
+    batch, width = t_shape
+    step, dense = table.stride()
+    if (dense != 1 and width > 1) or not starts.is_contiguous() or not lengths.is_contiguous():
+        _refuse("starts, lengths and the rows of the table must be dense")
+    if starts.get_device() != dev or lengths.get_device() != dev or table.get_device() != dev:
+        _refuse("table, starts and lengths must be on the cache's device")
+    desc = capi.CacheDesc(pages, page, heads, d, code, batch, width, step, rows, k.data_ptr(), v.data_ptr(), ek, ev,
+                          table.data_ptr(), starts.data_ptr(), lengths.data_ptr())
     return desc, code, dev, heads, d
 
 
 def _packed(t, heads, d, dev, what):
     shape, s = t.shape, t.stride()
     if len(shape) != 3 or shape[1] != heads or shape[2] != d or s[2] != 1 or t.get_device() != dev:
-        raise ValueError(f"frisk-b200-cache: {what} must be [rows, {heads}, {d}] on the cache's device, the elements of a head neighbours")
+        _refuse(f"{what} must be [rows, {heads}, {d}] on the cache's device, the elements of a head neighbours")
     return capi.Packed(t.data_ptr(), s[0], s[1])
 
 
@@ -96,7 +113,7 @@ def cache_write(cache, k, v, table, starts, lengths, *, stream=None):
     desc, code, dev, heads, d = _describe(cache, table, starts, lengths, k.shape[0])
     given = _codes().get(k.dtype)
     if given is None or given == capi.E4M3 or v.dtype != k.dtype or v.shape != k.shape or (code != capi.E4M3 and code != given):
-        raise ValueError("frisk-b200-cache: keys and values must be float16 or bfloat16 rows of one shape, in the type of a 16-bit cache")
+        _refuse("keys and values must be float16 or bfloat16 rows of one shape, in the type of a 16-bit cache")
     pk, pv = _packed(k, heads, d, dev, "keys"), _packed(v, heads, d, dev, "values")
     context_for(dev).cache_write(desc, given, pk, pv, stream=_stream_ptr(stream, k.device))
     return cache
@@ -106,19 +123,18 @@ def cache_read(cache, table, starts, lengths, rows, *, dtype=None, out=None, str
     """The packed (keys, values) [rows, heads, D] at the positions of the packed rows, in ``dtype`` (float16 or bfloat16; a 16-bit cache
     gives its own).  ``lengths`` of zero read sequences from their first key on.  ``out``: a pair of tensors for them; in new ones, rows
     that belong to no sequence are undefined.  8-bit values beyond the type's range become its largest finite ones."""
-    torch = _torch()
     desc, code, dev, heads, d = _describe(cache, table, starts, lengths, rows)
     if dtype is None:
-        dtype = out[0].dtype if out is not None else torch.bfloat16 if code == capi.E4M3 else cache[0].dtype
+        dtype = out[0].dtype if out is not None else _torch().bfloat16 if code == capi.E4M3 else cache[0].dtype
     given = _codes().get(dtype)
     if given is None or given == capi.E4M3 or (code != capi.E4M3 and code != given):
-        raise ValueError("frisk-b200-cache: rows are read as float16 or bfloat16, from a 16-bit cache in its own type")
+        _refuse("rows are read as float16 or bfloat16, from a 16-bit cache in its own type")
     if out is None:
-        device = cache[0].device
-        with _on_stream(stream, device):
-            out = tuple(torch.empty(rows, heads, d, dtype=dtype, device=device) for _ in range(2))
+        like = cache[0]
+        with _on_stream(stream, like.device):
+            out = like.new_empty((rows, heads, d), dtype=dtype), like.new_empty((rows, heads, d), dtype=dtype)
     elif len(out) != 2 or any(t.dtype != dtype or t.shape[0] != rows for t in out):
-        raise ValueError("frisk-b200-cache: out must be two tensors of the rows' type and count")
+        _refuse("out must be two tensors of the rows' type and count")
     pk, pv = _packed(out[0], heads, d, dev, "keys"), _packed(out[1], heads, d, dev, "values")
     context_for(dev).cache_read(desc, given, pk, pv, stream=_stream_ptr(stream, cache[0].device))
     return tuple(out)
@@ -132,42 +148,45 @@ def cache_attention(cache, q, table, starts, lengths, *, mask=None, scale=None, 
     head h reads key head h // (query heads / key heads).  A row that sees no key is zero; what a row does not see does not reach it,
     whatever it holds.  ``scale`` is 1 / sqrt(D) if not given.  ``max_new``, the largest number of new tokens of a sequence, helps the
     choice of a kernel and changes no result's meaning.  Rows of a new ``out`` that belong to no sequence are undefined."""
-    torch = _torch()
-    rows = q.shape[0]
+    shape = q.shape
+    rows = shape[0]
     desc, code, dev, heads, d = _describe(cache, table, starts, lengths, rows)
-    given = _codes().get(q.dtype)
+    dtype = q.dtype
+    given = _CODES.get(dtype)
     if given is None or given == capi.E4M3 or (code != capi.E4M3 and code != given):
-        raise ValueError("frisk-b200-cache: queries must be float16 or bfloat16, in the type of a 16-bit cache")
-    heads_q = q.shape[1] if len(q.shape) == 3 else 0
+        _refuse("queries must be float16 or bfloat16, in the type of a 16-bit cache")
+    heads_q = shape[1] if len(shape) == 3 else 0
     if heads_q < 1 or heads_q % heads:
-        raise ValueError("frisk-b200-cache: queries must be [rows, query heads, D], query heads a multiple of the key heads")
-    device = q.device
+        _refuse("queries must be [rows, query heads, D], query heads a multiple of the key heads")
     width = step = 0
     mask_ptr = None
     if mask is not None:
-        if mask.dtype != torch.bool or len(mask.shape) != 2 or mask.shape[0] != rows or (mask.stride(1) != 1 and mask.shape[1] > 1) or \
-                mask.get_device() != dev:
-            raise ValueError("frisk-b200-cache: the mask must be bool [rows, width] on the cache's device, its rows dense")
-        width, step = mask.shape[1], mask.stride(0)
-        mask_ptr = mask.data_ptr()
-        if width == 0:  # (an empty tensor has no address; none of the new tokens is seen)
-            mask_ptr = starts.data_ptr()
+        m_shape = mask.shape
+        if mask.dtype != _torch().bool or len(m_shape) != 2 or m_shape[0] != rows or mask.get_device() != dev:
+            _refuse("the mask must be bool [rows, width] on the cache's device")
+        width = m_shape[1]
+        step, dense = mask.stride()
+        if dense != 1 and width > 1:
+            _refuse("the rows of the mask must be dense")
+        # (an empty tensor has no address; none of the new tokens is seen)
+        mask_ptr = mask.data_ptr() if width else starts.data_ptr()
     pq = _packed(q, heads_q, d, dev, "queries")
-    adesc = capi.CacheAttnDesc(heads_q, given, max_new, width, step, 1.0 / math.sqrt(d) if scale is None else scale)
+    adesc = capi.CacheAttnDesc(heads_q, given, max_new, width, step, d ** -0.5 if scale is None else scale)
+    if out is not None and (out.dtype != dtype or out.shape != shape):
+        _refuse("out must have the type and shape of the queries")
+    # (a workspace of the call's own: calls on other streams and captured graphs share nothing)
     nbytes = capi.cache_attention_workspace_bytes(desc, adesc)
-    if out is not None and (out.dtype != q.dtype or out.shape != q.shape):
-        raise ValueError("frisk-b200-cache: out must have the type and shape of the queries")
     if stream is None:
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            out = _new_like(q)
+        workspace = starts.new_empty((nbytes // 4,))
     else:
-        with _on_stream(stream, device):
+        with _on_stream(stream, q.device):
             if out is None:
-                out = torch.empty(q.shape, dtype=q.dtype, device=device)
-            workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+                out = _new_like(q)
+            workspace = starts.new_empty((nbytes // 4,))
     po = _packed(out, heads_q, d, dev, "results")
-    context_for(dev).cache_attention(desc, adesc, pq, po, mask_ptr, workspace.data_ptr(), nbytes, stream=_stream_ptr(stream, device))
+    context_for(dev).cache_attention(desc, adesc, pq, po, mask_ptr, workspace.data_ptr(), nbytes, _stream_ptr(stream, q.device))
     return out
 
 

@@ -672,6 +672,7 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
 #pragma unroll 1
           for (int x = 0; x < BN / 16; ++x) {
             uint32_t y[16];
+            __syncwarp();
             tmem_ld_32x32b_x16(t_s + buf * BN + x * 16, y);
             tmem_ld_wait();
             const uint32_t bits = (x & 2 ? see[1] : see[0]) >> (16 * (x & 1));
@@ -685,6 +686,7 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
             }
             tmem_st_32x32b_x16(t_s + buf * BN + x * 16, y);
           }
+          __syncwarp();
           tmem_st_wait();
           settle(E4M3 ? mw : mx);
           if (!ok) break;
@@ -699,6 +701,7 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
 #pragma unroll 1
           for (int x = 0; x < BN / 16; ++x) {
             uint32_t y[16], a[8], b2[4];
+            __syncwarp();
             tmem_ld_32x32b_x16(t_s + buf * BN + x * 16, y);
             tmem_ld_wait();
 #pragma unroll

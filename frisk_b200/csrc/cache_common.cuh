@@ -40,20 +40,22 @@ struct Seq {
   int first, count, length;  // packed rows, keys before them
   bool ok;
 };
-__device__ __forceinline__ Seq load_seq(const Tables& t, int b, unsigned* status) {
+__device__ __forceinline__ Seq check_seq(const Tables& t, int lo, int hi, int length, unsigned* status) {
   Seq s;
-  const int lo = __ldg(t.starts + b), hi = __ldg(t.starts + b + 1);
-  s.length = __ldg(t.lengths + b);
+  s.length = length;
   s.first = lo;
   s.count = hi - lo;
   const bool rows_ok = lo >= 0 && hi >= lo && hi <= t.rows;
-  const bool length_ok = s.length >= 0 && (int64_t)s.length + s.count <= (int64_t)t.width * t.page;
+  const bool length_ok = length >= 0 && (int64_t)length + s.count <= (int64_t)t.width * t.page;
   s.ok = rows_ok && length_ok;
   if (!s.ok) {
     atomicCAS(status, 0u, rows_ok ? ST_CACHE_LENGTH : ST_CACHE_ROWS);
     s.count = 0;
   }
   return s;
+}
+__device__ __forceinline__ Seq load_seq(const Tables& t, int b, unsigned* status) {
+  return check_seq(t, __ldg(t.starts + b), __ldg(t.starts + b + 1), __ldg(t.lengths + b), status);
 }
 
 // 2^(e - 127) of an exponent byte

@@ -1,9 +1,9 @@
 // Writing new rows into the paged cache, quantised on the way where it holds 8-bit floats, and reading rows back.
 //
-// A head's row is D elements: 16 bytes of the 16-bit side a lane, D / 8 neighbouring lanes a row, so the largest magnitude of a row
-// takes three or four shuffles and nothing passes through shared memory.  Bound by HBM: each side is read or written once.  A block takes
+// A head's row is D elements: 16 of them a lane, D / 16 neighbouring lanes a row, so the largest magnitude of a row takes two or three
+// shuffles and nothing passes through shared memory.  Bound by HBM: each side is read or written once.  A block takes
 // up to 16 packed rows: a thread finds the place of each (its sequence by bisection of `starts`, then the page; a chain of dependent
-// loads), then all threads move the pieces of all of them, four at a time.  (One row at a time, 52 thousand rows of 4 heads of 64 took
+// loads), then all threads move the pieces of all of them, two at a time.  (One row at a time, 52 thousand rows of 4 heads of 64 took
 // 102 us.)  Fewer rows a block where that leaves SMs idle: a few rows cost the chain starts -> lengths -> table and little else.
 #include <algorithm>
 
@@ -15,7 +15,8 @@ using namespace cache;
 
 constexpr int kThreads = 256;
 constexpr int kMaxRows = 16;  // packed rows a block
-constexpr int kAhead = 4;     // pieces a thread has in flight
+constexpr int kCopied = 512;  // sequences whose tables fit into shared memory
+constexpr int kAhead = 2;     // pieces a thread has in flight
 
 struct Side {  // packed rows outside the cache, 16-bit
   void* ptr;
@@ -32,14 +33,15 @@ struct RowsParams {
 };
 
 // The index of packed row r among the cache's token slots of head 0, (page * heads) * P + offset; -1: it has none.
-__device__ __forceinline__ int64_t locate(const Tables& t, int64_t r, unsigned* status) {
+// `starts`, `lengths`: the tables, or copies of them in shared memory.
+__device__ __forceinline__ int64_t locate(const Tables& t, const int* starts, const int* lengths, int64_t r, unsigned* status) {
   // the last b with starts[b] <= r; where starts does not ascend, some b that does not hold r
   int lo = 0, hi = t.batch;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (__ldg(t.starts + mid) <= r) lo = mid; else hi = mid;
+    if (starts[mid] <= r) lo = mid; else hi = mid;
   }
-  const Seq s = load_seq(t, lo, status);
+  const Seq s = check_seq(t, starts[lo], starts[lo + 1], lengths[lo], status);
   const int64_t i = r - s.first;
   if (!s.ok || i < 0 || i >= s.count) return -1;  // (rows before the first sequence and behind the last belong to none)
   const int64_t pos = s.length + i;
@@ -68,96 +70,122 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
 
 template <bool BF16, int D, bool E4M3, bool WRITE>
 __global__ void __launch_bounds__(kThreads) cache_rows_kernel(const RowsParams p) {
-  constexpr int kLanes = D / 8;  // of a row
+  constexpr int kLanes = D / 16;  // of a row
   __shared__ int64_t bases[kMaxRows];
+  __shared__ int starts[kCopied + 1], lengths[kCopied];
   const int64_t row0 = (int64_t)blockIdx.x * p.rows_block;
   const int here = (int)min((int64_t)p.rows_block, p.rows - row0);
   const int per_row = 2 * p.t.heads * kLanes;  // pieces of a token: keys, then values
   const int total = here * per_row;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if ((int)threadIdx.x < here) bases[threadIdx.x] = locate(p.t, row0 + threadIdx.x, p.status);
+  if (p.t.batch <= kCopied) {  // (one latency for the tables instead of one a step of the bisection)
+    for (int b = threadIdx.x; b <= p.t.batch; b += kThreads) {
+      starts[b] = __ldg(p.t.starts + b);
+      if (b < p.t.batch) lengths[b] = __ldg(p.t.lengths + b);
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < here) bases[threadIdx.x] = locate(p.t, starts, lengths, row0 + threadIdx.x, p.status);
+  } else if ((int)threadIdx.x < here) {
+    bases[threadIdx.x] = locate(p.t, p.t.starts, p.t.lengths, row0 + threadIdx.x, p.status);
+  }
   __syncthreads();
   // (whole groups of kLanes threads have the same head's row, and whole warps the same number of rounds: the shuffles below need them)
+  const int sub = threadIdx.x % kLanes;
+  int r_next = threadIdx.x / per_row, piece = threadIdx.x - r_next * per_row;  // of the next piece: its row, its place there
+  const int r_step = kThreads / per_row, piece_step = kThreads - r_step * per_row;
   for (int e0 = 0; e0 < total; e0 += kThreads * kAhead) {
-    uint4 x[kAhead];       // the 16-bit side, or the cache's piece
+    uint4 x[kAhead][2];    // the 16-bit side, or the cache's piece
     uint32_t e_byte[kAhead];
     int64_t token[kAhead];  // -1: nothing to do
     uint4* packed[kAhead];
     bool values[kAhead];
 #pragma unroll
     for (int n = 0; n < kAhead; ++n) {
+      if (e0 + n * kThreads >= total) break;
       const int e = e0 + n * kThreads + threadIdx.x;
       const bool mine = e < total;
-      const int r = mine ? e / per_row : 0, unit = (mine ? e - r * per_row : 0) / kLanes, sub = threadIdx.x % kLanes;
+      const int r = mine ? r_next : 0, unit = piece / kLanes;
+      r_next += r_step;
+      piece += piece_step;
+      if (piece >= per_row) {
+        piece -= per_row;
+        ++r_next;
+      }
       values[n] = unit >= p.t.heads;
       const int h = values[n] ? unit - p.t.heads : unit;
       const Side& side = values[n] ? p.v : p.k;
-      packed[n] = reinterpret_cast<uint4*>(static_cast<uint16_t*>(side.ptr) + (row0 + r) * side.row + h * side.head) + sub;
+      packed[n] = reinterpret_cast<uint4*>(static_cast<uint16_t*>(side.ptr) + (row0 + r) * side.row + h * side.head) + 2 * sub;
       const int64_t base = bases[r];
       token[n] = mine && base >= 0 ? base + ((int64_t)h << p.t.page_log2) : -1;
-      x[n] = make_uint4(0, 0, 0, 0);
+      x[n][0] = x[n][1] = make_uint4(0, 0, 0, 0);
       e_byte[n] = 0;
       if (token[n] < 0) continue;
       const void* pages = values[n] ? p.cv : p.ck;
       if (WRITE) {
-        x[n] = __ldcs(packed[n]);
+        x[n][0] = __ldcs(packed[n]);
+        x[n][1] = __ldcs(packed[n] + 1);
       } else if (!E4M3) {
-        x[n] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(pages) + token[n] * D) + sub);
+        const uint4* held = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(pages) + token[n] * D) + 2 * sub;
+        x[n][0] = __ldcs(held);
+        x[n][1] = __ldcs(held + 1);
       } else {
-        const uint2 code = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pages) + token[n] * D) + sub);
-        x[n].x = code.x;
-        x[n].y = code.y;
+        x[n][0] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pages) + token[n] * D) + sub);
         e_byte[n] = __ldg((values[n] ? p.ev : p.ek) + token[n]);
       }
     }
 #pragma unroll
     for (int n = 0; n < kAhead; ++n) {
-      const int sub = threadIdx.x % kLanes;
+      if (e0 + n * kThreads >= total) break;
       void* pages = values[n] ? p.cv : p.ck;
       if (!E4M3) {
         if (token[n] < 0) continue;
-        if (WRITE) reinterpret_cast<uint4*>(static_cast<uint16_t*>(pages) + token[n] * D)[sub] = x[n];
-        else __stcs(packed[n], x[n]);
-      } else if (WRITE) {
-        float f[8];
-        const uint32_t w[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
-        uint32_t most = 0;  // magnitudes compare as integers; infinities and NaN are the largest
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 two = unpack16<BF16>(w[i]);
-          f[2 * i] = two.x;
-          f[2 * i + 1] = two.y;
-          most = max(most, max(__float_as_uint(two.x) & 0x7fffffffu, __float_as_uint(two.y) & 0x7fffffffu));
+        if (WRITE) {
+          uint4* held = reinterpret_cast<uint4*>(static_cast<uint16_t*>(pages) + token[n] * D) + 2 * sub;
+          held[0] = x[n][0];
+          held[1] = x[n][1];
+        } else {
+          __stcs(packed[n], x[n][0]);
+          __stcs(packed[n] + 1, x[n][1]);
         }
+      } else if (WRITE) {
+        const uint32_t w[8] = {x[n][0].x, x[n][0].y, x[n][0].z, x[n][0].w, x[n][1].x, x[n][1].y, x[n][1].z, x[n][1].w};
+        uint32_t most = 0;  // magnitudes of 16-bit floats compare as integers; infinities and NaN are the largest
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = __vmaxu2(most, w[i] & 0x7fff7fffu);
+        most = max(most & 0xffffu, most >> 16);
 #pragma unroll
         for (int o = kLanes / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        most = __float_as_uint(unpack16<BF16>(most).x);
         // most = 1.m * 2^(E - 127) and 448 = 1.75 * 2^8: the least e with most <= 448 * 2^(e - 127)
         int e = (int)(most >> 23) - 8 + ((most & 0x7fffffu) > 0x600000u ? 1 : 0);
         e = most >= 0x7f800000u ? 255 : max(e, 1);
         if (token[n] < 0) continue;
-        uint32_t code[2] = {0, 0};
+        uint32_t code[4] = {0, 0, 0, 0};
         if (e != 255) {
           const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            code[i >> 1] |= (uint32_t)float2_to_e4m3x2(f[2 * i] * inv, f[2 * i + 1] * inv) << (16 * (i & 1));
+          for (int i = 0; i < 8; ++i) {
+            const float2 two = unpack16<BF16>(w[i]);
+            code[i >> 1] |= (uint32_t)float2_to_e4m3x2(two.x * inv, two.y * inv) << (16 * (i & 1));
+          }
         }
-        reinterpret_cast<uint2*>(static_cast<uint8_t*>(pages) + token[n] * D)[sub] = make_uint2(code[0], code[1]);
+        reinterpret_cast<uint4*>(static_cast<uint8_t*>(pages) + token[n] * D)[sub] = make_uint4(code[0], code[1], code[2], code[3]);
         if (sub == 0) (values[n] ? p.ev : p.ek)[token[n]] = (uint8_t)e;
       } else {
         if (token[n] < 0) continue;
         const float scale = scale_of(e_byte[n]);
-        const uint32_t c[2] = {x[n].x, x[n].y};
-        uint32_t o[4];
+        const uint32_t c[4] = {x[n][0].x, x[n][0].y, x[n][0].z, x[n][0].w};
+        uint32_t o[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 8; ++i) {
           const uint32_t h2 = i & 1 ? e4m3x2_to_half2_hi(c[i >> 1]) : e4m3x2_to_half2(c[i >> 1]);
           const float2 two = __half22float2(*reinterpret_cast<const __half2*>(&h2));
           // a row near the end of the type's range may have been rounded beyond it
           o[i] = pack16<BF16>(saturated<BF16>(two.x * scale), saturated<BF16>(two.y * scale));
         }
         __stcs(packed[n], make_uint4(o[0], o[1], o[2], o[3]));
+        __stcs(packed[n] + 1, make_uint4(o[4], o[5], o[6], o[7]));
       }
     }
   }
@@ -291,7 +319,11 @@ static int cache_rows(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* c, int32
   p.rows = c->rows;
   p.status = ctx->d_status;
   p.rows_block = 1;
-  while (p.rows_block < kMaxRows && c->rows / (2 * p.rows_block) >= 4 * ctx->num_sms) p.rows_block *= 2;
+  // up to 1024 pieces a block, four a thread (13 thousand rows of 8 heads of 128, 8 rows a block: write and read 41 us, with 16 rows 48; 52
+  // thousand of 4 heads of 64: 16 rows 21.6, with 8 23.1), and at least four blocks a SM
+  const int pieces = 2 * c->heads * c->D / 16;
+  while (p.rows_block < kMaxRows && 2 * p.rows_block * pieces <= 4 * kThreads && c->rows / (2 * p.rows_block) >= 4 * ctx->num_sms)
+    p.rows_block *= 2;
   FB_DEVICE(ctx);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = dtype == FRISK_B200_BF16, e4m3 = c->dtype == FRISK_B200_E4M3;

@@ -6,11 +6,12 @@
 // so its backward is the transposed rotation: the same with -sin.
 //
 // t grows to 10^6 and more, where 32 bits keep no digit of a turn behind the point that matters: the product and the reduction to one
-// turn are made in 64 bits, then sine and cosine of at most half a turn in 32.  A block does this once for every (token, pair) and
-// uses it for all heads of queries and keys, whose products are rounded once.
+// turn are made in 64 bits, then sine and cosine of at most half a turn in 32.  Each product is rounded once to its type.
 //
-// Bound by HBM: every element is read and written once, 16 bytes a thread and access where addresses and sizes allow, else one
-// element.  A block takes the tokens whose angles make about one a thread, or a single one where that leaves SMs idle.
+// Bound by HBM: every element is read and written once, 16 bytes a lane and access where addresses and sizes allow, else one element.
+// A warp has a token, or some of its heads where there are few tokens: it makes the token's angles once, one a lane, passes them
+// through shared memory and uses them for all its heads of queries and keys; the first heads are on their way meanwhile, and no warp
+// waits for another.
 #include <algorithm>
 
 #include "common.cuh"
@@ -19,9 +20,8 @@
 namespace fb {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxTokens = 8;
-constexpr int kAhead = 4;  // units a thread has in flight
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kAhead = 2;       // heads a lane has in flight
 
 struct Part {  // queries or keys
   const void* in;
@@ -34,123 +34,142 @@ struct RotaryParams {
   const void* positions;
   const double* frequencies;
   int64_t rows;
-  int D, half, tokens;  // half = dim / 2; tokens a block
+  int D, half;      // half = dim / 2
+  int chunk, chunks;  // heads a warp, warps a token
   int positions64;
   float amplitude, sign;
 };
 
-template <typename T> struct Elem;
-template <> struct Elem<float> {
-  static __device__ float to(float x) { return x; }
-  static __device__ float from(float x) { return x; }
-};
-template <> struct Elem<__half> {
-  static __device__ float to(__half x) { return __half2float(x); }
-  static __device__ __half from(float x) { return __float2half_rn(x); }
-};
-template <> struct Elem<__nv_bfloat16> {
-  static __device__ float to(__nv_bfloat16 x) { return __bfloat162float(x); }
-  static __device__ __nv_bfloat16 from(float x) { return __float2bfloat16_rn(x); }
-};
-
+// A unit's group: V elements, as 32-bit words where there are several (two 16-bit elements a word).
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-  T v[V];
+struct Group {
+  static constexpr int kWords = V == 1 ? 1 : V * (int)sizeof(T) / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T* from) {
+    if (V == 1) {
+      w[0] = sizeof(T) == 4 ? *reinterpret_cast<const uint32_t*>(from) : *reinterpret_cast<const uint16_t*>(from);
+    } else {
+      const uint4 x = *reinterpret_cast<const uint4*>(from);
+      w[0] = x.x; w[1 % kWords] = x.y; w[2 % kWords] = x.z; w[3 % kWords] = x.w;
+    }
+  }
+  __device__ __forceinline__ void store(T* to) const {
+    if (V == 1) {
+      if (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(to) = w[0];
+      else *reinterpret_cast<uint16_t*>(to) = (uint16_t)w[0];
+    } else {
+      *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1 % kWords], w[2 % kWords], w[3 % kWords]);
+    }
+  }
 };
+// the two elements of a word (of the first only, where V == 1: the second is zero), and back
+template <typename T> __device__ __forceinline__ float2 unpack(uint32_t w) { return make_float2(__uint_as_float(w), 0.f); }
+template <> __device__ __forceinline__ float2 unpack<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <> __device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack(float2 x) { return __float_as_uint(x.x); }
+template <> __device__ __forceinline__ uint32_t pack<__half>(float2 x) {
+  const __half2 h = __floats2half2_rn(x.x, x.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float2 x) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 turned(float a, float b, float2 cs) { return make_float2(a * cs.x - b * cs.y, b * cs.x + a * cs.y); }
 
 // V elements an access: 16 bytes, or 1 where something is not aligned to that
 template <typename T, int V, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) {
-  extern __shared__ float2 angles[];  // [tokens][half]
-  using E = Elem<T>;
-  const int64_t row0 = (int64_t)blockIdx.x * p.tokens;
-  const int here = (int)min((int64_t)p.tokens, p.rows - row0);
+  extern __shared__ float2 all_angles[];  // [warps][half]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float2* angles = all_angles + warp * p.half;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int e = threadIdx.x; e < here * p.half; e += kThreads) {
-    const int t = e / p.half, i = e - t * p.half;
-    const double pos = p.positions64 ? (double)static_cast<const long long*>(p.positions)[row0 + t]
-                                     : (double)static_cast<const int*>(p.positions)[row0 + t];
-    const double turns = pos * p.frequencies[i] * 0.15915494309189535;  // 1 / (2 pi)
-    float s, c;
-    sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-    angles[e] = make_float2(c * p.amplitude, s * p.amplitude * p.sign);
+  const int64_t task = (int64_t)blockIdx.x * kWarps + warp, row = task / p.chunks;
+  if (row >= p.rows) return;
+  {
+    const double pos = p.positions64 ? (double)static_cast<const long long*>(p.positions)[row]
+                                     : (double)static_cast<const int*>(p.positions)[row];
+    for (int i = lane; i < p.half; i += 32) {
+      const double turns = pos * p.frequencies[i] * 0.15915494309189535;  // 1 / (2 pi)
+      float s, c;
+      sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+      angles[i] = make_float2(c * p.amplitude, s * p.amplitude * p.sign);
+    }
+    __syncwarp();
   }
-  __syncthreads();
-  // units: the V-element groups of a head.  A pair of groups (half layout) or one group (interleaved) is rotated, others are copied.
-  constexpr int kPairs = INTERLEAVED ? V / 2 : V;  // pairs a unit rotates
-  const int n_rot = V == 1 && INTERLEAVED ? p.half : p.half / (kPairs > 0 ? kPairs : 1);
-  const int n_pass = (p.D - 2 * p.half) / V;
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    const Part& part = p.part[which];
-    const bool copy = part.in != part.out;  // in place, what passes stays
-    const int per_head = n_rot + (copy ? n_pass : 0);
-    const int total = here * part.heads * per_head;
-    if (total == 0) continue;
-    // this thread's unit, head and token, and what a step of all threads adds to them
-    int u = threadIdx.x % per_head, h = threadIdx.x / per_head % part.heads, t = threadIdx.x / per_head / part.heads;
-    const int du = kThreads % per_head, dh = kThreads / per_head % part.heads, dt = kThreads / per_head / part.heads;
-#pragma unroll 1
-    for (int e0 = threadIdx.x; e0 < total; e0 += kThreads * kAhead) {
-      Vec<T, V> x[kAhead], y[kAhead];
-      int us[kAhead];
-      T* out[kAhead];
-      const float2* cs[kAhead];
+  // Units: the V-element groups of a head.  A pair of groups (half layout) or one group (interleaved) is rotated, others are copied.  A
+  // lane has one unit of several heads.
+  using G = Group<T, V>;
+  constexpr bool kTwo = !(INTERLEAVED && V > 1);         // a unit has two groups
+  constexpr int kPairs = kTwo ? V : V / 2;               // pairs a unit rotates
+  auto rotate = [](G& x, G& y, const float2 (&cs)[kPairs]) {
+    if (!kTwo) {
 #pragma unroll
-      for (int n = 0; n < kAhead; ++n) {
-        us[n] = e0 + n * kThreads < total ? u : -1;
-        if (us[n] >= 0) {
-          const T* in = static_cast<const T*>(part.in) + (row0 + t) * part.in_row + h * part.in_head;
-          out[n] = static_cast<T*>(part.out) + (row0 + t) * part.out_row + h * part.out_head;
-          cs[n] = angles + t * p.half;
-          const bool rotated = u < n_rot;
-          if (V == 1 && INTERLEAVED && rotated) {
-            x[n].v[0] = in[2 * u];
-            y[n].v[0] = in[2 * u + 1];
-          } else {
-            x[n] = *reinterpret_cast<const Vec<T, V>*>(in + (rotated ? u * V : 2 * p.half + (u - n_rot) * V));
-            if (!INTERLEAVED && rotated) y[n] = *reinterpret_cast<const Vec<T, V>*>(in + p.half + u * V);
-          }
-        }
-        u += du;
-        h += dh;
-        t += dt;
-        if (u >= per_head) {
-          u -= per_head;
-          ++h;
-        }
-        if (h >= part.heads) {
-          h -= part.heads;
-          ++t;
+      for (int i = 0; i < G::kWords; ++i) {
+        if (sizeof(T) == 2) {
+          const float2 ab = unpack<T>(x.w[i]);
+          x.w[i] = pack<T>(turned(ab.x, ab.y, cs[i % kPairs]));
+        } else if (i % 2 == 0) {
+          const float2 r = turned(__uint_as_float(x.w[i]), __uint_as_float(x.w[(i + 1) % G::kWords]), cs[i / 2 % kPairs]);
+          x.w[i] = __float_as_uint(r.x);
+          x.w[(i + 1) % G::kWords] = __float_as_uint(r.y);
         }
       }
+    } else {
 #pragma unroll
-      for (int n = 0; n < kAhead; ++n) {
-        const int un = us[n];
-        if (un < 0) continue;
-        if (un >= n_rot) {
-          *reinterpret_cast<Vec<T, V>*>(out[n] + 2 * p.half + (un - n_rot) * V) = x[n];
-        } else if (INTERLEAVED && V > 1) {
+      for (int i = 0; i < G::kWords; ++i) {
+        constexpr int kEach = sizeof(T) == 2 && V > 1 ? 2 : 1;  // elements a word
+        const float2 a = unpack<T>(x.w[i]), b = unpack<T>(y.w[i]);
+        const float2 r = turned(a.x, b.x, cs[i * kEach]);
+        const float2 q = kEach == 2 ? turned(a.y, b.y, cs[(i * kEach + 1) % kPairs]) : make_float2(0.f, 0.f);
+        x.w[i] = pack<T>(make_float2(r.x, q.x));
+        y.w[i] = pack<T>(make_float2(r.y, q.y));
+      }
+    }
+  };
+  const int n_rot = p.half / kPairs, n_units = n_rot + (p.D - 2 * p.half) / V;
+  const int first = (int)(task - row * p.chunks) * p.chunk, last = first + p.chunk;  // its heads, queries before keys
+  const int width = min(n_units, 32), slots = 32 / width, slot = lane / width;
+  if (slot >= slots) return;
+  for (int u = lane - slot * width; u < n_units; u += width) {
+    const bool rotated = u < n_rot;
+    const int at = !rotated ? 2 * p.half + (u - n_rot) * V : INTERLEAVED && V == 1 ? 2 * u : u * V;  // the unit's first element
+    const int other = INTERLEAVED ? at + 1 : at + p.half;                                             // its second group
+    float2 cs[kPairs];
+    if (rotated) {
 #pragma unroll
-          for (int i = 0; i < V / 2; ++i) {
-            const float2 r = cs[n][un * (V / 2) + i];
-            const float a = E::to(x[n].v[2 * i]), b = E::to(x[n].v[2 * i + 1]);
-            x[n].v[2 * i] = E::from(a * r.x - b * r.y);
-            x[n].v[2 * i + 1] = E::from(b * r.x + a * r.y);
+      for (int i = 0; i < kPairs; ++i) cs[i] = angles[u * kPairs + i];
+    }
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+      const Part& part = p.part[which];
+      if (!rotated && part.in == part.out) continue;  // (in place, what passes stays)
+      const int skip = which ? p.part[0].heads : 0, begin = max(first - skip, 0) + slot, end = min(last - skip, part.heads);
+      const T* in = static_cast<const T*>(part.in) + row * part.in_row + begin * part.in_head + at;
+      T* out = static_cast<T*>(part.out) + row * part.out_row + begin * part.out_head + at;
+      const int64_t in_step = slots * part.in_head, out_step = slots * part.out_head;
+      for (int h = begin; h < end; h += slots * kAhead) {
+        G x[kAhead], y[kAhead];  // (all loads before the first store: the compiler cannot tell that they are apart)
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n)
+          if (h + n * slots < end) {
+            x[n].load(in + n * in_step);
+            if (kTwo && rotated) y[n].load(in + n * in_step + (other - at));
           }
-          *reinterpret_cast<Vec<T, V>*>(out[n] + un * V) = x[n];
-        } else {
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float2 r = cs[n][un * V + i];
-            const float a = E::to(x[n].v[i]), b = E::to(y[n].v[i]);
-            x[n].v[i] = E::from(a * r.x - b * r.y);
-            y[n].v[i] = E::from(b * r.x + a * r.y);
+        for (int n = 0; n < kAhead; ++n) {
+          if (h + n * slots >= end) break;
+          if (rotated) {
+            rotate(x[n], y[n], cs);
+            if (kTwo) y[n].store(out + n * out_step + (other - at));
           }
-          *reinterpret_cast<Vec<T, V>*>(out[n] + (INTERLEAVED ? 2 * un : un * V)) = x[n];
-          *reinterpret_cast<Vec<T, V>*>(out[n] + (INTERLEAVED ? 2 * un + 1 : p.half + un * V)) = y[n];
+          x[n].store(out + n * out_step);
         }
+        in += kAhead * in_step;
+        out += kAhead * out_step;
       }
     }
   }
@@ -162,9 +181,9 @@ cudaError_t launch(const RotaryParams& p, bool interleaved, cudaStream_t s) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel waits (griddepcontrol.wait) itself
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)((p.rows + p.tokens - 1) / p.tokens));
+  cfg.gridDim = dim3((unsigned)((p.rows * p.chunks + kWarps - 1) / kWarps));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)p.tokens * p.half * sizeof(float2);
+  cfg.dynamicSmemBytes = (size_t)kWarps * p.half * sizeof(float2);  // (32 KB at most)
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -252,8 +271,12 @@ extern "C" int frisk_b200_rotary(frisk_b200_ctx* ctx, const frisk_b200_rotary_de
   p.positions64 = d->positions64;
   p.amplitude = d->amplitude;
   p.sign = d->inverse ? -1.f : 1.f;
-  p.tokens = std::max(1, std::min(kMaxTokens, kThreads / p.half));
-  while (p.tokens > 1 && d->rows / p.tokens < 4 * ctx->num_sms) p.tokens /= 2;
+  // all heads of a token to one warp, or fewer where that leaves SMs with less than 16 warps
+  const int all = d->heads_q + d->heads_k;
+  p.chunk = all;
+  while (p.chunk > 2 && d->rows * ((all + p.chunk - 1) / p.chunk) < 16 * ctx->num_sms) p.chunk = (p.chunk + 1) / 2;
+  p.chunks = (all + p.chunk - 1) / p.chunk;
+  if (d->rows * (int64_t)p.chunks > (int64_t)INT32_MAX * kWarps) return FRISK_B200_E_TOO_LARGE;
   FB_DEVICE(ctx);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   FB_CUDA(ctx, d->dtype == FRISK_B200_F32   ? launch_type<float>(p, d->interleaved != 0, s)

@@ -9,7 +9,7 @@ import math
 
 from . import capi
 from .execute import _stream_ptr, _torch, context_for
-from .cache import _on_stream
+from .cache import _new_like, _on_stream
 
 _CODE = None
 
@@ -50,53 +50,61 @@ def rotary_frequencies(dim, base=10000.0, *, scaling=None, factor=1.0, trained=N
     return _torch().tensor(freq, dtype=_torch().float64, device=device), amplitude
 
 
+def _refuse(what):
+    raise ValueError("frisk-b200-rotary: " + what)
+
+
+def _operand(t, dev, d):
+    s = t.stride()
+    if (s[2] != 1 and d > 1) or t.get_device() != dev:
+        _refuse("operands must be on one device, the elements of a head neighbours")
+    return capi.Packed(t.data_ptr(), s[0], s[1])
+
+
 def _rotate(q, k, positions, frequencies, amplitude, interleaved, out, stream, inverse):
     global _CODE
-    torch = _torch()
     if _CODE is None:
-        _CODE = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
-    code = _CODE.get(q.dtype)
+        torch = _torch()
+        _CODE = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}, torch.int64, torch.int32, torch.float64
+    codes, i64, i32, f64 = _CODE
+    dtype, shape, dev = q.dtype, q.shape, q.get_device()
+    code = codes.get(dtype)
     if code is None:
-        raise ValueError("frisk-b200-rotary: elements must be float32, float16 or bfloat16")
-    dev, shape = q.get_device(), q.shape
+        _refuse("elements must be float32, float16 or bfloat16")
     if len(shape) != 3:
-        raise ValueError("frisk-b200-rotary: queries and keys must be [tokens, heads, D]")
+        _refuse("queries and keys must be [tokens, heads, D]")
     n, heads_q, d = shape
     heads_k = 0
-    if out is None:
-        with _on_stream(stream, q.device):
-            out = (torch.empty(shape, dtype=q.dtype, device=q.device), None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device))
-    elif not isinstance(out, (tuple, list)) or len(out) != 2:
-        raise ValueError("frisk-b200-rotary: out must be a pair (None for absent keys)")
-    q_out, k_out = out
-    if (k is None) != (k_out is None) or q_out is None:
-        raise ValueError("frisk-b200-rotary: out must be a pair (None for absent keys)")
     if k is not None:
-        if k.dtype != q.dtype or k_out.dtype != q.dtype or len(k.shape) != 3 or k.shape[0] != n or k.shape[2] != d or k_out.shape != k.shape:
-            raise ValueError("frisk-b200-rotary: keys must have the queries' type, tokens and D")
-        heads_k = k.shape[1]
-    if q_out.dtype != q.dtype or q_out.shape != shape:
-        raise ValueError("frisk-b200-rotary: results must have the type and shape of what is rotated")
-    if len(positions.shape) != 1 or positions.shape[0] != n or positions.dtype not in (torch.int64, torch.int32) or not positions.is_contiguous():
-        raise ValueError("frisk-b200-rotary: positions must be int32 or int64, one for every token")
-    if len(frequencies.shape) != 1 or frequencies.dtype != torch.float64 or not frequencies.is_contiguous():
-        raise ValueError("frisk-b200-rotary: frequencies must be one float64 for every pair")
-    operands = []
-    for t in (q, k, q_out, k_out):
-        if t is None or (n == 0 or heads_q == 0):
-            operands.append(None)
-            continue
-        s = t.stride()
-        if t.get_device() != dev or s[2] != 1 and d > 1:
-            raise ValueError("frisk-b200-rotary: operands must be on one device, the elements of a head neighbours")
-        operands.append(capi.Packed(t.data_ptr(), s[0], s[1]))
+        k_shape = k.shape
+        if k.dtype != dtype or len(k_shape) != 3 or k_shape[0] != n or k_shape[2] != d:
+            _refuse("keys must have the queries' type, tokens and D")
+        heads_k = k_shape[1]
+    if out is None:
+        if stream is None:
+            q_out, k_out = _new_like(q), None if k is None else _new_like(k)
+        else:
+            with _on_stream(stream, q.device):
+                q_out, k_out = _new_like(q), None if k is None else _new_like(k)
+    else:
+        if not isinstance(out, (tuple, list)) or len(out) != 2 or out[0] is None or (k is None) != (out[1] is None):
+            _refuse("out must be a pair (None for absent keys)")
+        q_out, k_out = out
+        if q_out.dtype != dtype or q_out.shape != shape or (k is not None and (k_out.dtype != dtype or k_out.shape != k_shape)):
+            _refuse("results must have the type and shape of what is rotated")
+    p_type, p_shape, f_shape = positions.dtype, positions.shape, frequencies.shape
+    if (p_type != i64 and p_type != i32) or len(p_shape) != 1 or p_shape[0] != n or not positions.is_contiguous():
+        _refuse("positions must be int32 or int64, one for every token")
+    if frequencies.dtype != f64 or len(f_shape) != 1 or not frequencies.is_contiguous():
+        _refuse("frequencies must be one float64 for every pair")
     if dev < 0 or positions.get_device() != dev or frequencies.get_device() != dev:
-        raise ValueError("frisk-b200-rotary: operands must be on one CUDA device (there is no CPU path)")
+        _refuse("operands must be on one CUDA device (there is no CPU path)")
     if n == 0:
         return q_out, k_out
-    desc = capi.RotaryDesc(n, heads_q, heads_k, d, 2 * frequencies.shape[0], code, interleaved, inverse,
-                           positions.dtype == torch.int64, amplitude)
-    context_for(dev).rotary(desc, positions.data_ptr(), frequencies.data_ptr(), *operands, stream=_stream_ptr(stream, q.device))
+    desc = capi.RotaryDesc(n, heads_q, heads_k, d, 2 * f_shape[0], code, interleaved, inverse, p_type == i64, amplitude)
+    absent = heads_k == 0
+    context_for(dev).rotary(desc, positions.data_ptr(), frequencies.data_ptr(), _operand(q, dev, d), None if absent else _operand(k, dev, d),
+                            _operand(q_out, dev, d), None if absent else _operand(k_out, dev, d), _stream_ptr(stream, q.device))
     return q_out, k_out
 
 
