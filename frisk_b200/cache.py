@@ -26,6 +26,14 @@ def _codes():
     return _CODES
 
 
+def _stream_of(stream, dev):
+    torch = _torch()
+    if stream is None:
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        return raw(dev) if raw is not None else torch.cuda.current_stream(dev).cuda_stream
+    return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+
+
 def _on_stream(stream, device):
     """What is allocated in it belongs to the stream the kernels run on."""
     if stream is None:
@@ -38,6 +46,19 @@ def _new_like(t):
     """A dense new tensor of the shape, type and device of ``t``."""
     torch = _torch()
     return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+_shapes = {}
+
+
+def _workspace(nbytes, dev):
+    """New scratch of the call's own, so that calls on other streams and captured graphs share none.  (What is kept is a tensor of that
+    shape over a single byte: an allocation after its like costs half of one by its size.)"""
+    torch = _torch()
+    like = _shapes.get((nbytes, dev))
+    if like is None:
+        like = _shapes[nbytes, dev] = torch.empty(1, dtype=torch.uint8, device=torch.device("cuda", dev)).expand(nbytes)
+    return torch.empty_like(like, memory_format=torch.contiguous_format)
 
 
 def _refuse(what):
@@ -115,7 +136,7 @@ def cache_write(cache, k, v, table, starts, lengths, *, stream=None):
     if given is None or given == capi.E4M3 or v.dtype != k.dtype or v.shape != k.shape or (code != capi.E4M3 and code != given):
         _refuse("keys and values must be float16 or bfloat16 rows of one shape, in the type of a 16-bit cache")
     pk, pv = _packed(k, heads, d, dev, "keys"), _packed(v, heads, d, dev, "values")
-    context_for(dev).cache_write(desc, given, pk, pv, stream=_stream_ptr(stream, k.device))
+    context_for(dev).cache_write(desc, given, pk, pv, _stream_of(stream, dev))
     return cache
 
 
@@ -131,12 +152,15 @@ def cache_read(cache, table, starts, lengths, rows, *, dtype=None, out=None, str
         _refuse("rows are read as float16 or bfloat16, from a 16-bit cache in its own type")
     if out is None:
         like = cache[0]
-        with _on_stream(stream, like.device):
-            out = like.new_empty((rows, heads, d), dtype=dtype), like.new_empty((rows, heads, d), dtype=dtype)
+        if stream is None:
+            out = like.new_empty((2, rows, heads, d), dtype=dtype).unbind()
+        else:
+            with _on_stream(stream, like.device):
+                out = like.new_empty((2, rows, heads, d), dtype=dtype).unbind()
     elif len(out) != 2 or any(t.dtype != dtype or t.shape[0] != rows for t in out):
         _refuse("out must be two tensors of the rows' type and count")
     pk, pv = _packed(out[0], heads, d, dev, "keys"), _packed(out[1], heads, d, dev, "values")
-    context_for(dev).cache_read(desc, given, pk, pv, stream=_stream_ptr(stream, cache[0].device))
+    context_for(dev).cache_read(desc, given, pk, pv, _stream_of(stream, dev))
     return tuple(out)
 
 
@@ -174,19 +198,18 @@ def cache_attention(cache, q, table, starts, lengths, *, mask=None, scale=None, 
     adesc = capi.CacheAttnDesc(heads_q, given, max_new, width, step, d ** -0.5 if scale is None else scale)
     if out is not None and (out.dtype != dtype or out.shape != shape):
         _refuse("out must have the type and shape of the queries")
-    # (a workspace of the call's own: calls on other streams and captured graphs share nothing)
     nbytes = capi.cache_attention_workspace_bytes(desc, adesc)
     if stream is None:
         if out is None:
             out = _new_like(q)
-        workspace = starts.new_empty((nbytes // 4,))
+        workspace = _workspace(nbytes, dev)
     else:
         with _on_stream(stream, q.device):
             if out is None:
                 out = _new_like(q)
-            workspace = starts.new_empty((nbytes // 4,))
+            workspace = _workspace(nbytes, dev)
     po = _packed(out, heads_q, d, dev, "results")
-    context_for(dev).cache_attention(desc, adesc, pq, po, mask_ptr, workspace.data_ptr(), nbytes, _stream_ptr(stream, q.device))
+    context_for(dev).cache_attention(desc, adesc, pq, po, mask_ptr, workspace.data_ptr(), nbytes, _stream_of(stream, dev))
     return out
 
 

@@ -77,7 +77,10 @@ template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float2 x) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float2 turned(float a, float b, float2 cs) { return make_float2(a * cs.x - b * cs.y, b * cs.x + a * cs.y); }
+// (rounded step by step as written, so that the kernels for aligned and other rows agree to the bit)
+__device__ __forceinline__ float2 turned(float a, float b, float2 cs) {
+  return make_float2(__fmaf_rn(a, cs.x, -__fmul_rn(b, cs.y)), __fmaf_rn(b, cs.x, __fmul_rn(a, cs.y)));
+}
 
 // V elements an access: 16 bytes, or 1 where something is not aligned to that
 template <typename T, int V, bool INTERLEAVED>

@@ -8,8 +8,8 @@ Packed rows [tokens, heads, D], as a projection leaves them: queries and keys ma
 import math
 
 from . import capi
-from .execute import _stream_ptr, _torch, context_for
-from .cache import _new_like, _on_stream
+from .cache import _new_like, _on_stream, _stream_of
+from .execute import _torch, context_for
 
 _CODE = None
 
@@ -104,7 +104,7 @@ def _rotate(q, k, positions, frequencies, amplitude, interleaved, out, stream, i
     desc = capi.RotaryDesc(n, heads_q, heads_k, d, 2 * f_shape[0], code, interleaved, inverse, p_type == i64, amplitude)
     absent = heads_k == 0
     context_for(dev).rotary(desc, positions.data_ptr(), frequencies.data_ptr(), _operand(q, dev, d), None if absent else _operand(k, dev, d),
-                            _operand(q_out, dev, d), None if absent else _operand(k_out, dev, d), _stream_ptr(stream, q.device))
+                            _operand(q_out, dev, d), None if absent else _operand(k_out, dev, d), _stream_of(stream, dev))
     return q_out, k_out
 
 
