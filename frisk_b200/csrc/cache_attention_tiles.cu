@@ -22,8 +22,8 @@
 // and a factor for every key relative to it.  The row sum has no part in the values' scales and is kept in units of 2^B of its own.  The
 // checking warp prepares the scales.
 //
-// Tiles that a row may not see whole, and 8-bit tiles whose values' scales span more than 2^8 ("wide"), take a path of rolled loops over
-// tensor memory.  (Unrolled, code that runs once an item cost up to 20 us a tile: it has to be fetched.)
+// 8-bit tiles whose values' scales span more than 2^8 ("wide") take a path of rolled loops over tensor memory.  (Code that runs once an item
+// has to be fetched: unrolled for masked tiles, too, it cost up to 20 us a tile.)
 //
 // What bounds it: up to 128 rows HBM, 0.77 us a 16-bit tile of 64 keys a SM; else the softmax groups (some 1700 clk for 64 keys of 256
 // rows, of which 1024 exponentials).
@@ -457,46 +457,69 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
       ++meets;
       tc_fence_after_sync();
     };
-    for (Cursor c(p, plan, kRows); c.left > 0 && ok; c.next_item(p, kRows)) {
+    // A row's query: 16 bytes a piece.  Where the groups share a tile, each brings half of every row (of an 8-bit cache it reads the whole,
+    // whose largest element sets the scale).  Halves are loaded while the item before ends (32 sequences of 8000 keys, 64 rows a head:
+    // 187 -> 176 us); whole rows would take registers that the epilogue needs.
+    constexpr int kPieces = D / 8 / (PAIR ? 1 : 2), kLoads = E4M3 ? D / 8 : kPieces;
+    constexpr bool kEarly = !E4M3 && !PAIR;
+    const int first = PAIR ? 0 : q * kPieces;
+    struct Place {
+      int r, i_new, head;
+      bool valid;
+    };
+    auto place_of = [&](const Cursor& c) {  // this thread's row of the item
+      Place at;
+      at.r = c.rt * kRows + (PAIR ? q * BM : 0) + row;  // of the (sequence, key head)
+      at.valid = at.r < c.seq.count * p.group;
+      at.i_new = at.valid ? at.r / p.group : 0;  // its new token
+      at.head = c.h * p.group + (at.valid ? at.r - at.i_new * p.group : 0);
+      return at;
+    };
+    auto load_query = [&](uint4 (&x)[kLoads], const Cursor& c) {
+      const Place at = place_of(c);
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + (int64_t)(c.seq.first + at.i_new) * p.q_row +
+                                                        (int64_t)at.head * p.q_head);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) x[i] = at.valid ? __ldg(src + (E4M3 ? 0 : first) + i) : make_uint4(0, 0, 0, 0);
+    };
+    Cursor c(p, plan, kRows);
+    uint4 early[kLoads];
+    if (kEarly && c.left > 0) load_query(early, c);
+    while (c.left > 0 && ok) {
       const Work w = work_of(c);
       const Seq seq = c.seq;
       const int n_tiles = w.nq[q];
-      const int r = c.rt * kRows + (PAIR ? q * BM : 0) + row;  // row of the (sequence, key head)
-      const bool valid = r < seq.count * p.group;
-      const int i_new = valid ? r / p.group : 0;  // its new token
+      const Place at = place_of(c);
+      const bool valid = at.valid;
+      const int i_new = at.i_new;
 
-      // ---- the row's query, to its place in the swizzled tile.  (The products that read the tile before are complete: all of their scores
-      // have been read, by both groups where they share it.)
-      float row_scale = fabsf(p.scale_log2);
+      // ---- the query, to its place in the swizzled tile.  (The products that read the tile before are complete: all of their scores have
+      // been read, by both groups where they share it.)  A scale of zero is one of queries of zeros, so that -inf stays what it is.
+      float row_scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
       {
-        const int head = c.h * p.group + (valid ? r - i_new * p.group : 0);
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + (int64_t)(seq.first + i_new) * p.q_row +
-                                                          (int64_t)head * p.q_head);
         unsigned char* tile = smem + (PAIR ? q * L::kTerms * L::kQTile : 0);
         const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a negative scale goes into the queries)
-        // where the groups share a tile, each brings half of every row
-        constexpr int kPieces = D / 8 / (PAIR ? 1 : 2);
-        const int first = PAIR ? 0 : q * kPieces;
-        if (!E4M3) {
-          uint4 x[kPieces];
+        uint4 x[kLoads];
+        if (!kEarly) load_query(x, c);
 #pragma unroll
-          for (int i = 0; i < kPieces; ++i) x[i] = valid ? __ldg(src + first + i) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < kLoads; ++i) {
+          if (kEarly) x[i] = early[i];
+          if (p.scale_log2 == 0.f) x[i] = make_uint4(0, 0, 0, 0);
+        }
+        if (!E4M3) {
 #pragma unroll
           for (int i = 0; i < kPieces; ++i) {
-            const int at = first + i;
-            *reinterpret_cast<uint4*>(tile + (at >> 3) * kBoxBytes + row * 128 + (((at & 7) ^ (row & 7)) << 4)) =
-                make_uint4(x[i].x ^ flip, x[i].y ^ flip, x[i].z ^ flip, x[i].w ^ flip);
+            const int n = first + i;
+            *reinterpret_cast<uint4*>(tile + (n >> 3) * kBoxBytes + row * 128 + (((n & 7) ^ (row & 7)) << 4)) =
+                make_uint4(x[i % kLoads].x ^ flip, x[i % kLoads].y ^ flip, x[i % kLoads].z ^ flip, x[i % kLoads].w ^ flip);
           }
         } else {
           auto pair_of = [&](uint32_t y) {
             return QBF16 ? make_float2(__uint_as_float(y << 16), __uint_as_float(y & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&y));
           };
-          uint4 x[D / 8];
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) x[i] = valid ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
           uint32_t most = 0;  // magnitudes of 16-bit floats compare as integers
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
+          for (int i = 0; i < kLoads; ++i) {
             const uint32_t y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
             for (int n = 0; n < 4; ++n) most = __vmaxu2(most, y[n] & 0x7fff7fffu);
@@ -509,7 +532,8 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) {  // 16 elements: 16 bytes of every term
             if (!PAIR && i / (D / 32) != q) continue;
-            const uint32_t y[8] = {x[2 * i].x, x[2 * i].y, x[2 * i].z, x[2 * i].w, x[2 * i + 1].x, x[2 * i + 1].y, x[2 * i + 1].z, x[2 * i + 1].w};
+            const uint4 y0 = x[2 * i % kLoads], y1 = x[(2 * i + 1) % kLoads];
+            const uint32_t y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
             uint32_t term[3][4] = {};
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
@@ -557,7 +581,7 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
         ++steps;
         tmem_ld_wait();
         const bool more = i + 1 < n_tiles;
-        const bool detour = tile >= w.first_masked || (E4M3 && info->wide != 0);
+        const bool masked = tile >= w.first_masked;
         constexpr float kThreshold = E4M3 ? kRescale8 : kRescaleThreshold;
         // Takes a new reference where it grew by more than the threshold: rare.  O is rescaled in tensor memory.
         auto settle = [&](float most) {
@@ -590,7 +614,41 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
           l_sum = fmaf(sum, ex2f(unit - b_ref), l_sum);
         };
         uint32_t pk0[16], pk1[16];  // the weights' first and second 32 keys (16-bit), or first and second terms
-        if (!detour) {
+        // What the row sees of the tile's keys, a bit a key.  The warp's rows belong to a few neighbouring tokens: the warp reads each one's
+        // mask side by side, eight tokens' at a time.
+        auto look = [&](uint32_t (&see)[2]) {
+          const int a0 = tile * BN - seq.length + lane, a1 = a0 + 32;  // the lane's two keys, counted from the first new token
+          const int width = p.mask ? min(p.mask_width, seq.count) : seq.count;
+          const bool may0 = a0 >= 0 && a0 < width, may1 = a1 >= 0 && a1 < width;
+          const int t0 = __shfl_sync(0xffffffffu, i_new, 0), t1 = __reduce_max_sync(0xffffffffu, i_new);
+          see[0] = see[1] = 0;
+#pragma unroll 1
+          for (int t = min(t0, t1); t <= t1; t += 8) {
+            bool lo[8], hi[8];
+            const uint8_t* m = p.mask + (int64_t)(seq.first + t) * p.mask_stride;
+#pragma unroll
+            for (int n = 0; n < 8; ++n, m += p.mask_stride) {
+              const bool there = t + n <= t1;
+              lo[n] = a0 < 0 || (there && may0 && (p.mask ? __ldg(m + a0) != 0 : a0 <= t + n));
+              hi[n] = a1 < 0 || (there && may1 && (p.mask ? __ldg(m + a1) != 0 : a1 <= t + n));
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+              const uint32_t l = __ballot_sync(0xffffffffu, lo[n]), h = __ballot_sync(0xffffffffu, hi[n]);
+              if (t + n == i_new) {
+                see[0] = l;
+                see[1] = h;
+              }
+            }
+          }
+          __syncwarp();
+        };
+        // Masked tiles: by selection in the common path where the groups share the rows (32 sequences of 8000 keys, 64 rows a head 187 ->
+        // 174 us), in the rolled path where they do not, whose common path is the slower for it (64 new tokens over 8 x 32000 keys 425 -> 461).
+        const bool inline_mask = !PAIR && masked, rolled = (PAIR && masked) || (E4M3 && info->wide != 0);
+        uint32_t see[2] = {0xffffffffu, 0xffffffffu};
+        if (inline_mask) look(see);
+        if (!rolled) {
           if (E4M3) {
 #pragma unroll
             for (int x = 0; x < 2; ++x)
@@ -602,6 +660,13 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
                 sr[x][4 * e] = __float_as_uint(lo.x); sr[x][4 * e + 1] = __float_as_uint(lo.y);
                 sr[x][4 * e + 2] = __float_as_uint(hi.x); sr[x][4 * e + 3] = __float_as_uint(hi.y);
               }
+          }
+          if (inline_mask) {  // (the row's scale is positive: -inf stays -inf)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+#pragma unroll
+              for (int x = 0; x < 2; ++x)
+                if (!((see[x] >> e) & 1u)) sr[x][e] = 0xff800000u;
           }
           float mxc[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains of the row maximum
 #pragma unroll
@@ -639,34 +704,7 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
           const float2 tot = add2(sa, sb);
           if (E4M3) add_sum(tot.x + tot.y, unit); else l_sum += tot.x + tot.y;
         } else {
-          // What the row sees of the tile's keys, a bit a key.  The warp's rows belong to a few neighbouring tokens: the warp reads each
-          // one's mask side by side, eight tokens' at a time.
-          uint32_t see[2] = {0, 0};
-          {
-            const int a0 = tile * BN - seq.length + lane, a1 = a0 + 32;  // the lane's two keys, counted from the first new token
-            const int width = p.mask ? min(p.mask_width, seq.count) : seq.count;
-            const bool may0 = a0 >= 0 && a0 < width, may1 = a1 >= 0 && a1 < width;
-            const int t0 = __shfl_sync(0xffffffffu, i_new, 0), t1 = __reduce_max_sync(0xffffffffu, i_new);
-#pragma unroll 1
-            for (int t = min(t0, t1); t <= t1; t += 8) {
-              bool lo[8], hi[8];
-              const uint8_t* m = p.mask + (int64_t)(seq.first + t) * p.mask_stride;
-#pragma unroll
-              for (int n = 0; n < 8; ++n, m += p.mask_stride) {
-                const bool there = t + n <= t1;
-                lo[n] = a0 < 0 || (there && may0 && (p.mask ? __ldg(m + a0) != 0 : a0 <= t + n));
-                hi[n] = a1 < 0 || (there && may1 && (p.mask ? __ldg(m + a1) != 0 : a1 <= t + n));
-              }
-#pragma unroll
-              for (int n = 0; n < 8; ++n) {
-                const uint32_t l = __ballot_sync(0xffffffffu, lo[n]), h = __ballot_sync(0xffffffffu, hi[n]);
-                if (t + n == i_new) {
-                  see[0] = l;
-                  see[1] = h;
-                }
-              }
-            }
-          }
+          if (PAIR && masked) look(see);
           // In rolled loops over 16 keys: the scores, scaled, in tensor memory again, -inf for what the row does not see; their maxima.
           float mx = -INFINITY, mw = -INFINITY;  // largest score, largest score plus scale of the value
 #pragma unroll 1
@@ -745,6 +783,9 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
         mbar_arrive(&p_ready[2 * q + buf]);
         if (more && !ahead) wait_scores();
       }
+      Cursor next = c;
+      next.next_item(p, kRows);
+      if (kEarly && next.left > 0) load_query(early, next);
       if (ok && n_tiles > 0) ok = mbar_wait_warp(&o_done[2 * q + 1], ends[1] & 1, abort_flag, p.status, ST_CACHE_O);
       if (!ok) break;
       tc_fence_after_sync();
@@ -779,7 +820,7 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
       if (has_rows) {
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         uint16_t* const out = static_cast<uint16_t*>(p.out) + (int64_t)(seq.first + i_new) * p.out_row +
-                              (int64_t)(c.h * p.group + (valid ? r - i_new * p.group : 0)) * p.out_head;
+                              (int64_t)at.head * p.out_head;
         const bool bad = bad_values[items & 7] == (uint32_t)items + 1;
         constexpr int kChunks = D / 32 / (PAIR ? 1 : 2);  // of 32 columns: each group stores half where they share the rows
         for (int x = PAIR ? 0 : q * kChunks; x < (PAIR ? kChunks : (q + 1) * kChunks); ++x) {
@@ -837,6 +878,7 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
       }
       ++items;
       infos += PAIR ? w.n : n_tiles;
+      c = next;
       if (!PAIR) meet();  // both groups are done with the statistics, the queries and both O
     }
   }
