@@ -164,14 +164,15 @@ def cache_read(cache, table, starts, lengths, rows, *, dtype=None, out=None, str
     return tuple(out)
 
 
-def cache_attention(cache, q, table, starts, lengths, *, mask=None, scale=None, max_new=0, out=None, stream=None):
+def cache_attention(cache, q, table, starts, lengths, *, mask=None, scale=None, max_new=0, tile_rows=0, out=None, stream=None):
     """Attention of the packed query rows ``q`` [rows, query heads, D] (float16 or bfloat16; a 16-bit cache has their type) over the
     cache, which holds their own keys and values already (``cache_write``).  A row sees the ``lengths[b]`` keys before the new tokens
     of its sequence and, of the new tokens, those up to itself, or those j for which ``mask[row, j]`` is set: ``mask`` is bool
     [rows, width], j counts within the sequence, and what lies beyond the width is not seen.  A single token is a tree of one.  Query
     head h reads key head h // (query heads / key heads).  A row that sees no key is zero; what a row does not see does not reach it,
     whatever it holds.  ``scale`` is 1 / sqrt(D) if not given.  ``max_new``, the largest number of new tokens of a sequence, helps the
-    choice of a kernel and changes no result's meaning.  Rows of a new ``out`` that belong to no sequence are undefined."""
+    choice of a kernel and changes no result's meaning; ``tile_rows`` makes it: 16, 128 or 256 query rows (new tokens times query heads
+    of a key head) a tile.  Rows of a new ``out`` that belong to no sequence are undefined."""
     shape = q.shape
     rows = shape[0]
     desc, code, dev, heads, d = _describe(cache, table, starts, lengths, rows)
@@ -195,7 +196,7 @@ def cache_attention(cache, q, table, starts, lengths, *, mask=None, scale=None, 
         # (an empty tensor has no address; none of the new tokens is seen)
         mask_ptr = mask.data_ptr() if width else starts.data_ptr()
     pq = _packed(q, heads_q, d, dev, "queries")
-    adesc = capi.CacheAttnDesc(heads_q, given, max_new, width, step, d ** -0.5 if scale is None else scale)
+    adesc = capi.CacheAttnDesc(heads_q, given, max_new, width, step, d ** -0.5 if scale is None else scale, tile_rows)
     if out is not None and (out.dtype != dtype or out.shape != shape):
         _refuse("out must have the type and shape of the queries")
     nbytes = capi.cache_attention_workspace_bytes(desc, adesc)

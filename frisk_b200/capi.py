@@ -32,7 +32,7 @@ EXPORTS = (
     "frisk_b200_gemm_fused_select", "frisk_b200_gemm_fused_workspace_bytes", "frisk_b200_gemm_fused",
     "frisk_b200_gemm_plan", "frisk_b200_attention_form",
     "frisk_b200_rotary", "frisk_b200_cache_write", "frisk_b200_cache_read", "frisk_b200_cache_attention",
-    "frisk_b200_cache_attention_workspace_bytes",
+    "frisk_b200_cache_attention_workspace_bytes", "frisk_b200_cache_attention_tile_rows",
 )
 
 
@@ -99,7 +99,8 @@ class CacheDesc(ctypes.Structure):
 
 class CacheAttnDesc(ctypes.Structure):
     _fields_ = [("heads_q", ctypes.c_int32), ("dtype", ctypes.c_int32), ("max_new", ctypes.c_int32),
-                ("mask_width", ctypes.c_int32), ("mask_stride", ctypes.c_int64), ("scale", ctypes.c_float)]
+                ("mask_width", ctypes.c_int32), ("mask_stride", ctypes.c_int64), ("scale", ctypes.c_float),
+                ("tile_rows", ctypes.c_int32)]
 
 
 _lib = None
@@ -156,6 +157,7 @@ def load():
         "frisk_b200_cache_read": (ctypes.c_int, [vp, cd, i32, pk, pk, vp]),
         "frisk_b200_cache_attention": (ctypes.c_int, [vp, cd, ca, pk, pk, vp, vp, sz, vp]),
         "frisk_b200_cache_attention_workspace_bytes": (sz, [cd, ca]),
+        "frisk_b200_cache_attention_tile_rows": (ctypes.c_int, [cd, ca]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -319,6 +321,14 @@ def gemm_fused_workspace_bytes(desc, epi):
 def cache_attention_workspace_bytes(cache, desc):
     """Bytes ``Context.cache_attention`` needs; 0 for what it refuses.  Host-only."""
     return load().frisk_b200_cache_attention_workspace_bytes(cache, desc)
+
+
+def cache_attention_tile_rows(cache, desc):
+    """Query rows a tile (16, 128 or 256) of ``Context.cache_attention``.  Host-only."""
+    rows = load().frisk_b200_cache_attention_tile_rows(cache, desc)
+    if rows < 0:
+        raise_for(rows)
+    return rows
 
 
 _PAIR = ctypes.c_int64 * 2

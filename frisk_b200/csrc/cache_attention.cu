@@ -669,6 +669,7 @@ int check_attention(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_
   if (a->heads_q < 1 || a->heads_q > 65536 || a->heads_q % c->heads || a->max_new < 0 || a->mask_width < 0 || a->mask_stride < 0)
     return FRISK_B200_E_CACHE_SHAPE;
   if (!(a->scale == a->scale) || a->scale * 0.f != 0.f) return FRISK_B200_E_ARG;
+  if (a->tile_rows != 0 && a->tile_rows != kRows && a->tile_rows != 128 && a->tile_rows != 256) return FRISK_B200_E_ARG;
   // units are counted in 32 bits (16 rows and 64 keys at least)
   const double tiles = ((double)c->table_width * c->page + kKeys - 1) / kKeys, group = a->heads_q / c->heads;
   if (tiles * c->heads * (c->rows * group / 16 + c->batch) > 2147483647.0 || (double)c->table_width * c->page > 2147483647.0 ||
@@ -678,11 +679,23 @@ int check_attention(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_
 }
 
 // Query rows a tile, by the rows that a sequence is said to have for a key head.  (A sequence with more than a tile's rows takes several
-// tiles, so a hint that is too low costs time only.)
+// tiles, so a hint that is too low costs time only.)  Up to 16 rows this file's kernel; from 129 on tiles of 256.  In between it is
+// weighed: this kernel reads the keys once for every 16 rows, the tiles of 128 once, at a higher cost of beginning and ending an item.  In
+// us, with n key tiles a SM: 16 rows 0.74 n (16-bit, D = 128), 0.40 (D = 64), 0.61 and 0.49 (8-bit); tiles 0.77, 0.71, 1.07 and 1.02 n and 10
+// (8-bit 14) more.  Measured, this kernel and tiles: 8 sequences of 4000 keys at D = 128, 32 rows a head 45.6 and 42.3, 8-bit 53.7 and 60.8; of
+// 1000 keys 21.5 and 27.8, 27.3 and 35.5; 48 rows 29.5 and 28.3, 37.7 and 36.1; 32 sequences of 8000, 32 rows at D = 64 194 and 178, 8-bit 228
+// and 273.  n goes by the table's width, the longest that the sequences can be.
 int tile_rows_of(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_desc* a) {
   const int64_t per = a->max_new > 0 ? a->max_new : c->batch > 0 ? (c->rows + c->batch - 1) / c->batch : 1;
   const int64_t rows = per * (a->heads_q / c->heads);
-  return rows <= kRows ? kRows : rows <= 128 ? 128 : 256;
+  if (a->tile_rows) return a->tile_rows;
+  if (rows <= kRows) return kRows;
+  if (rows > 128) return 256;
+  const bool e4m3 = c->dtype == FRISK_B200_E4M3;
+  const double n = (double)c->batch * c->heads * ((double)c->table_width * c->page / kKeys) / kNumSMsDefault;
+  const double few = e4m3 ? (c->D == 128 ? 0.61 : 0.49) : (c->D == 128 ? 0.74 : 0.40);
+  const double tiles = e4m3 ? (c->D == 128 ? 1.07 : 1.02) : (c->D == 128 ? 0.77 : 0.71);
+  return (rows + kRows - 1) / kRows * few * n < tiles * n + (e4m3 ? 14 : 10) ? kRows : 128;
 }
 
 }  // namespace
@@ -690,6 +703,11 @@ int tile_rows_of(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_des
 
 using namespace fb;
 using namespace fb::cache;
+
+extern "C" int frisk_b200_cache_attention_tile_rows(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_desc* a) {
+  const int rc = check_attention(c, a);
+  return rc ? rc : tile_rows_of(c, a);
+}
 
 extern "C" size_t frisk_b200_cache_attention_workspace_bytes(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_desc* a) {
   if (check_attention(c, a)) return 0;

@@ -795,7 +795,7 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
       // ---- O: scaled to the units of the row sum, and out: whole, or as a part for the join
       const float m_mine = E4M3 ? b_ref : a_ref;
       float f[2] = {E4M3 ? ex2f(a_ref - kTop8 - b_ref) : 1.f, 0.f}, m = m_mine, l = l_sum;
-      if (!E4M3 || l_sum == 0.f) f[0] = l_sum == 0.f ? 0.f : f[0];
+      if (l_sum == 0.f) f[0] = 0.f;
       if (!PAIR) {
         meet();  // all scores have been read: the statistics take the queries' place
         float4* stat = reinterpret_cast<float4*>(smem);
@@ -829,14 +829,14 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
           tmem_ld_32x32b_x32(tmem_base + 256 + (PAIR ? q * 128 : 0) + lane_addr + x * 32, o);
           tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = f[0] == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * f[0]);
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(scaled(__uint_as_float(o[e]), f[0]));  // (NaN stays, however small its weight)
           if (!PAIR && w.nq[1] > 0) {
             uint32_t o1[32];
             tmem_ld_32x32b_x32(tmem_base + 256 + 128 + lane_addr + x * 32, o1);
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              o[e] = f[1] == 0.f ? o[e] : __float_as_uint(fmaf(__uint_as_float(o1[e]), f[1], __uint_as_float(o[e])));
+              o[e] = __float_as_uint(__uint_as_float(o[e]) + scaled(__uint_as_float(o1[e]), f[1]));
           }
           if (bad && valid) {
             // infinities and NaN that were taken out of the values of partly seen tiles: rows that see them get them

@@ -343,13 +343,17 @@ int frisk_b200_cache_read(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* cach
  * new tokens j of its sequence the ones with mask[row * mask_stride + j] != 0 and j < mask_width (mask == NULL: those up to
  * itself).  Query head h reads key head h / (heads_q / heads).  A row that sees no key is zero.  What a row does not see
  * does not reach it, whatever it holds.  dtype: F16 or BF16, of q and out, and of a 16-bit cache.  max_new is a hint: the
- * largest number of new tokens of a sequence (0: unknown); it bears on speed only.
+ * largest number of new tokens of a sequence (0: unknown); it bears on the kernel that is chosen, as the width of the table
+ * does.  tile_rows names one: 16, 128 or 256 query rows a tile (new tokens times query heads of a key head); 0: chosen.
  * The workspace (32-byte aligned, contents of no matter before and after) must not be shared by calls that may overlap. */
 typedef struct frisk_b200_cache_attn_desc {
   int32_t heads_q, dtype, max_new, mask_width;
   int64_t mask_stride;
   float scale;
+  int32_t tile_rows;
 } frisk_b200_cache_attn_desc;
+/* The query rows a tile that a call runs with, or a negative error.  Host-only. */
+int frisk_b200_cache_attention_tile_rows(const frisk_b200_cache_desc* cache, const frisk_b200_cache_attn_desc* desc);
 size_t frisk_b200_cache_attention_workspace_bytes(const frisk_b200_cache_desc* cache, const frisk_b200_cache_attn_desc* desc);
 int frisk_b200_cache_attention(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* cache, const frisk_b200_cache_attn_desc* desc,
                                const frisk_b200_packed* q, const frisk_b200_packed* out, const uint8_t* mask,

@@ -50,7 +50,7 @@ def _cache_desc(**change):
 
 
 def _attn(**change):
-    d = dict(heads_q=4, dtype=capi.BF16, max_new=3, mask_width=0, mask_stride=0, scale=0.125)
+    d = dict(heads_q=4, dtype=capi.BF16, max_new=3, mask_width=0, mask_stride=0, scale=0.125, tile_rows=0)
     d.update(change)
     return capi.CacheAttnDesc(**d)
 
@@ -64,8 +64,22 @@ def test_descriptors_are_checked_on_the_host():
                    dict(table_width=1 << 27, table_stride=1 << 27, heads=4096, rows=1 << 20, pages=1)):
         assert size(_cache_desc(**change), _attn()) == 0, change
     for change in (dict(heads_q=3), dict(heads_q=0), dict(heads_q=1 << 20), dict(dtype=capi.F32), dict(max_new=-1), dict(mask_width=-1),
-                   dict(mask_stride=-1), dict(scale=math.nan), dict(scale=math.inf)):
+                   dict(mask_stride=-1), dict(scale=math.nan), dict(scale=math.inf), dict(tile_rows=32), dict(tile_rows=-1)):
         assert size(_cache_desc(), _attn(**change)) == 0, change
+        with pytest.raises(ValueError):
+            capi.cache_attention_tile_rows(_cache_desc(), _attn(**change))
+
+
+def test_the_choice_of_tiles():
+    rows = capi.cache_attention_tile_rows
+    long = dict(pages=4000, page=64, heads=8, D=128, batch=32, table_width=125, table_stride=125)
+    for heads_q, new, want in ((8, 1, 16), (32, 4, 16), (32, 16, 128), (32, 32, 128), (32, 33, 256), (64, 64, 256)):
+        assert rows(_cache_desc(**long), _attn(heads_q=heads_q, max_new=new)) == want
+    # few key tiles: the cheaper beginning wins
+    assert rows(_cache_desc(**dict(long, batch=1, table_width=8)), _attn(heads_q=32, max_new=16)) == 16
+    assert rows(_cache_desc(**long), _attn(heads_q=32, max_new=16, tile_rows=256)) == 256
+    # no hint: rows over sequences
+    assert rows(_cache_desc(**dict(long, rows=32 * 16)), _attn(heads_q=32, max_new=0)) == 128
 
 
 def test_null_contexts_are_refused():

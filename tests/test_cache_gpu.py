@@ -60,10 +60,13 @@ class Batch:
     def refresh(self):
         self.cache = tuple(t.cuda() for t in self.cpu)
 
-    def terms(self, max_new):
-        """Whether the kernel for more than 16 rows a key head runs on an 8-bit cache."""
-        per = max_new if max_new else -(-self.rows // len(self.lengths))
-        return len(self.cpu) == 4 and per * (self.q.shape[1] // self.k.shape[1]) > 16
+    def tile_rows(self, max_new):
+        from frisk_b200 import capi
+        code = {"float16": capi.F16, "bfloat16": capi.BF16, "float8_e4m3fn": capi.E4M3}
+        (pages, heads, page, d), h = self.cpu[0].shape, self.q.shape[1]
+        cache = capi.CacheDesc(pages, page, heads, d, code[str(self.cpu[0].dtype)[6:]], len(self.lengths), self.plan[0].shape[1],
+                               self.plan[0].stride(0), self.rows)
+        return capi.cache_attention_tile_rows(cache, capi.CacheAttnDesc(h, code[str(self.dtype)[6:]], max_new, 0, 0, 1.0, 0))
 
     def inside(self):
         import torch
@@ -100,23 +103,26 @@ def tree(batch, seed, kind="tree", width=None):
     return mask
 
 
-def attend(batch, mask=None, scale=None, max_new=0, bound_scale=1.0, **more):
-    """Runs the attention, compares every row with 64 bits, and requires that nothing else changed."""
+def attend(batch, mask=None, scale=None, max_new=0, tile_rows=None, **more):
+    """Runs the attention, compares every row with 64 bits, and requires that nothing else changed.  ``tile_rows`` None: every kernel."""
     import torch
     import frisk_b200 as F
+    if tile_rows is None:
+        return [attend(batch, mask, scale, max_new, n, **more) for n in (16, 128, 256, 0)][-1]
     out = torch.full((batch.rows,) + tuple(batch.q.shape[1:]), 77.0, dtype=batch.dtype, device="cuda")
     before = [bits(t) for t in batch.cache]
-    got = F.cache_attention(batch.cache, batch.q, *batch.plan, mask=None if mask is None else mask.cuda(), scale=scale, max_new=max_new, out=out, **more)
+    got = F.cache_attention(batch.cache, batch.q, *batch.plan, mask=None if mask is None else mask.cuda(), scale=scale, max_new=max_new,
+                            tile_rows=tile_rows, out=out, **more)
     F.cache_check()
     assert got is out
     assert all(torch.equal(a, bits(t)) for a, t in zip(before, batch.cache))
-    ref, bound = co.attention(batch.cpu, batch.q.cpu(), *batch.host, mask=mask, scale=scale, terms=batch.terms(max_new))
+    ref, bound = co.attention(batch.cpu, batch.q.cpu(), *batch.host, mask=mask, scale=scale, terms=len(batch.cpu) == 4 and (tile_rows or batch.tile_rows(max_new)) > 16)
     got, inside = out.cpu().double(), batch.inside()
     assert bool((got[~inside] == 77.0).all())
     finite = torch.isfinite(ref)
     assert torch.equal(torch.isfinite(got) | ~inside[:, None, None], finite | ~inside[:, None, None])
     use = finite & inside[:, None, None]
-    off = ((got - ref).abs() - bound_scale * bound)[use]
+    off = ((got - ref).abs() - bound)[use]
     assert off.numel() == 0 or float(off.max()) <= 0, (float(off.max()), float((got - ref)[use].abs().max()))
     return out
 
@@ -195,9 +201,8 @@ def test_attention(counts, lengths, hkv, group, d, page, dtype, scales):
     import torch
     held = torch.float8_e4m3fn if scales else None
     b = Batch(counts, lengths, hkv, group, d, page, getattr(torch, dtype), held, 3, gap=1, scales=scales or (0, 1))
-    first = attend(b)
-    again = attend(b)
-    assert torch.equal(bits(first), bits(again))
+    for n in (16, 128, 256):
+        assert torch.equal(bits(attend(b, tile_rows=n)), bits(attend(b, tile_rows=n)))
     attend(b, mask=tree(b, 1))
     attend(b, mask=tree(b, 2, "random"), max_new=max(counts))
     attend(b, mask=tree(b, 4, width=max(1, max(counts) // 2)), max_new=1, scale=0.31)
