@@ -38,6 +38,7 @@ struct CacheAttnParams {
   const uint8_t* mask;
   int64_t mask_stride;
   int mask_width, group;
+  int whole;  // items are not shared: a unit is an item
   float scale_log2;
   ItemRecord* records;
   float* partials;
@@ -51,7 +52,7 @@ __device__ __forceinline__ int row_tiles(const CacheAttnParams& p, const Seq& s,
   return (s.count * p.group + tile_rows - 1) / tile_rows;
 }
 __device__ __forceinline__ unsigned units_of(const CacheAttnParams& p, const Seq& s, int tile_rows) {
-  return (unsigned)p.t.heads * (unsigned)row_tiles(p, s, tile_rows) * (unsigned)key_tiles(s);
+  return (unsigned)p.t.heads * (unsigned)row_tiles(p, s, tile_rows) * (p.whole ? 1u : (unsigned)key_tiles(s));
 }
 
 struct PlanShared {
@@ -105,7 +106,7 @@ __device__ __forceinline__ Plan make_plan(const CacheAttnParams& p, int tile_row
         at += n;
       }
     }
-    if (holds(plan.end - 1)) {
+    if (!p.whole && holds(plan.end - 1)) {
       unsigned at = before;
       for (int b = b_lo; b < b_hi; ++b) {
         const Seq s = load_seq(p.t, b, p.status);
@@ -129,7 +130,7 @@ __device__ __forceinline__ Plan make_plan(const CacheAttnParams& p, int tile_row
         at += n;
       }
     }
-  } else if (threadIdx.x == 0) {
+  } else if (!p.whole && threadIdx.x == 0) {
     p.records[blockIdx.x] = ItemRecord{};
   }
   __syncthreads();
@@ -141,7 +142,8 @@ __device__ __forceinline__ Plan make_plan(const CacheAttnParams& p, int tile_row
 // Walks a CTA's items.
 struct Cursor {
   int b, h, rt, tile, kt, n_rt;
-  unsigned left;
+  unsigned left;  // units
+  bool whole;
   bool first_item;
   Seq seq;
   __device__ __forceinline__ void enter(const CacheAttnParams& p, int tile_rows) {
@@ -149,18 +151,19 @@ struct Cursor {
     kt = key_tiles(seq);
     n_rt = row_tiles(p, seq, tile_rows);
   }
-  __device__ __forceinline__ Cursor(const CacheAttnParams& p, const Plan& plan, int tile_rows) : left(plan.end - plan.begin), first_item(true) {
+  __device__ __forceinline__ Cursor(const CacheAttnParams& p, const Plan& plan, int tile_rows) : left(plan.end - plan.begin), whole(p.whole != 0), first_item(true) {
     if (left == 0) return;
     b = plan.b;
     enter(p, tile_rows);
-    const int item = (int)(plan.off / (unsigned)kt);
-    tile = (int)(plan.off - (unsigned)item * (unsigned)kt);
+    const unsigned each = whole ? 1u : (unsigned)kt;
+    const int item = (int)(plan.off / each);
+    tile = (int)(plan.off - (unsigned)item * each);
     h = item / n_rt;
     rt = item - h * n_rt;
   }
-  __device__ __forceinline__ int tiles_here() const { return (int)min((unsigned)(kt - tile), left); }
+  __device__ __forceinline__ int tiles_here() const { return whole ? kt : (int)min((unsigned)(kt - tile), left); }
   __device__ __forceinline__ void next_item(const CacheAttnParams& p, int tile_rows) {
-    left -= (unsigned)tiles_here();
+    left -= whole ? 1u : (unsigned)tiles_here();
     first_item = false;
     tile = 0;
     if (left == 0 || ++rt < n_rt) return;
