@@ -683,7 +683,7 @@ int check_attention(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_
   if (a->tile_rows != 0 && a->tile_rows != kRows && a->tile_rows != 128 && a->tile_rows != 256) return FRISK_B200_E_ARG;
   // units are counted in 32 bits (16 rows and 64 keys at least)
   const double tiles = ((double)c->table_width * c->page + kKeys - 1) / kKeys, group = a->heads_q / c->heads;
-  if (tiles * c->heads * (c->rows * group / 16 + c->batch) > 2147483647.0 || (double)c->table_width * c->page > 2147483647.0 ||
+  if (tiles * c->heads * (c->rows * group / 16 + c->batch) > 2147483647.0 || (double)c->table_width * c->page > 2147483647.0 - 4 * kKeys ||
       (double)c->rows * group > 2147483647.0)
     return FRISK_B200_E_TOO_LARGE;
   return 0;
@@ -744,11 +744,11 @@ extern "C" int frisk_b200_cache_attention(frisk_b200_ctx* ctx, const frisk_b200_
   const size_t need = frisk_b200_cache_attention_workspace_bytes(c, a);
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 31u)) return FRISK_B200_E_WORKSPACE;
   const size_t ob = packed_span(*out, c->rows, a->heads_q, c->D, 2), qb = packed_span(*q, c->rows, a->heads_q, c->D, 2);
-  const size_t mb = mask ? (size_t)((c->rows - 1) * a->mask_stride + a->mask_width) : 0;
+  const size_t mb = mask && a->mask_width ? (size_t)((c->rows - 1) * a->mask_stride + a->mask_width) : 0;
   for (int w = 0; w < 2; ++w) {  // what is written: the results and the workspace
     const void* ptr = w ? workspace : out->ptr;
     const size_t n = w ? need : ob;
-    if (ranges_overlap(ptr, n, q->ptr, qb) || (mask && ranges_overlap(ptr, n, mask, mb)) || cache_overlaps(c, ptr, n) || tables_overlap(c, ptr, n))
+    if (ranges_overlap(ptr, n, q->ptr, qb) || (mb && ranges_overlap(ptr, n, mask, mb)) || cache_overlaps(c, ptr, n) || tables_overlap(c, ptr, n))
       return FRISK_B200_E_OVERLAP;
   }
   if (ranges_overlap(workspace, need, out->ptr, ob)) return FRISK_B200_E_OVERLAP;

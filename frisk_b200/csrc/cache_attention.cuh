@@ -65,6 +65,10 @@ struct Plan {
   unsigned off;         // and its index there
 };
 
+// A call has fewer than 2^31 units, unless `starts` descends somewhere and sequences share rows: then sums end here, and nothing is done.
+constexpr unsigned kTooMany = 0xffffffffu;
+__device__ __forceinline__ unsigned add_units(unsigned a, unsigned b) { return a > kTooMany - b ? kTooMany : a + b; }
+
 // The units of all sequences, summed up by the whole CTA; its range of them; the record of the item it shares with the CTAs behind it.
 template <int THREADS>
 __device__ __forceinline__ Plan make_plan(const CacheAttnParams& p, int tile_rows, PlanShared* sh) {
@@ -72,12 +76,12 @@ __device__ __forceinline__ Plan make_plan(const CacheAttnParams& p, int tile_row
   const int chunk = (p.t.batch + THREADS - 1) / THREADS;
   const int b_lo = min((int)threadIdx.x * chunk, p.t.batch), b_hi = min(b_lo + chunk, p.t.batch);
   unsigned mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += units_of(p, load_seq(p.t, b, p.status), tile_rows);
+  for (int b = b_lo; b < b_hi; ++b) mine = add_units(mine, units_of(p, load_seq(p.t, b, p.status), tile_rows));
   unsigned upto = mine;  // of the warp's threads up to this one
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const unsigned other = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += other;
+    if (lane >= o) upto = add_units(upto, other);
   }
   if (lane == 31) sh->warp_sum[warp] = upto;
   __syncthreads();
@@ -86,7 +90,11 @@ __device__ __forceinline__ Plan make_plan(const CacheAttnParams& p, int tile_row
   for (int w = 0; w < THREADS / 32; ++w) {
     const unsigned n = sh->warp_sum[w];
     before += w < warp ? n : 0;
-    total += n;
+    total = add_units(total, n);
+  }
+  if (total == kTooMany) {
+    atomicCAS(p.status, 0u, ST_CACHE_ROWS);
+    total = 0;
   }
   const WorkSplit work{total / gridDim.x, total % gridDim.x};
   Plan plan;

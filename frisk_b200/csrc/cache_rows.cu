@@ -225,7 +225,7 @@ int cache_validate(const frisk_b200_cache_desc* c) {
   if (c->dtype != FRISK_B200_F16 && c->dtype != FRISK_B200_BF16 && c->dtype != FRISK_B200_E4M3) return FRISK_B200_E_CACHE_TYPE;
   if (c->pages < 1 || c->page < 16 || c->page > 1024 || (c->page & (c->page - 1)) || c->heads < 1 || c->heads > 4096 ||
       (c->D != 64 && c->D != 128) || c->batch < 0 || c->table_width < 0 || c->rows < 0 || c->rows > INT32_MAX ||
-      (c->batch > 1 && c->table_stride < c->table_width) || c->pages * c->heads > (INT32_MAX / c->page))
+      (c->batch > 1 && c->table_stride < c->table_width) || c->pages > INT32_MAX || c->pages * c->heads > (INT32_MAX / c->page))
     return FRISK_B200_E_CACHE_SHAPE;
   return 0;
 }
@@ -267,7 +267,7 @@ bool cache_overlaps(const frisk_b200_cache_desc* c, const void* ptr, size_t byte
 }
 bool tables_overlap(const frisk_b200_cache_desc* c, const void* ptr, size_t bytes) {
   return ranges_overlap(ptr, bytes, c->starts, ((size_t)c->batch + 1) * 4) || ranges_overlap(ptr, bytes, c->lengths, (size_t)c->batch * 4) ||
-         (c->batch > 0 && ranges_overlap(ptr, bytes, c->table, (size_t)((c->batch - 1) * c->table_stride + c->table_width) * 4));
+         (c->batch > 0 && c->table_width > 0 && ranges_overlap(ptr, bytes, c->table, (size_t)((c->batch - 1) * c->table_stride + c->table_width) * 4));
 }
 size_t packed_span(const frisk_b200_packed& x, int64_t rows, int heads, int D, size_t es) {
   return (size_t)((rows - 1) * x.row_stride + (heads - 1) * x.head_stride + D) * es;

@@ -242,6 +242,7 @@ extern "C" int frisk_b200_rotary(frisk_b200_ctx* ctx, const frisk_b200_rotary_de
   if (d->rows == 0) return 0;
   if (!positions || !frequencies || !q->ptr || !q_out->ptr) return FRISK_B200_E_ARG;
   if (d->heads_k && (!k || !k_out || !k->ptr || !k_out->ptr)) return FRISK_B200_E_ARG;
+  if (reinterpret_cast<uintptr_t>(positions) % (d->positions64 ? 8 : 4) || reinterpret_cast<uintptr_t>(frequencies) % 8) return FRISK_B200_E_ALIGN;
   const size_t es = dtype_size(d->dtype);
   const frisk_b200_packed *in[2] = {q, k}, *out[2] = {q_out, k_out};
   const int heads[2] = {d->heads_q, d->heads_k}, n = d->heads_k ? 2 : 1;

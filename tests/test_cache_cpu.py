@@ -60,7 +60,8 @@ def test_descriptors_are_checked_on_the_host():
     size = capi.cache_attention_workspace_bytes
     assert size(_cache_desc(), _attn()) > 0 and size(_cache_desc(dtype=capi.E4M3), _attn(dtype=capi.F16)) > 0
     for change in (dict(page=8), dict(page=24), dict(page=2048), dict(D=96), dict(D=256), dict(heads=0), dict(pages=0), dict(rows=-1), dict(batch=-1),
-                   dict(batch=2, table_stride=3), dict(pages=1 << 40), dict(dtype=7), dict(dtype=capi.F32), dict(dtype=capi.F16),
+                   dict(batch=2, table_stride=3), dict(pages=1 << 40), dict(pages=1 << 62, heads=4), dict(table_width=(1 << 27) - 1, table_stride=1 << 27, page=16, heads=1, rows=1, batch=1),
+                   dict(dtype=7), dict(dtype=capi.F32), dict(dtype=capi.F16),
                    dict(table_width=1 << 27, table_stride=1 << 27, heads=4096, rows=1 << 20, pages=1)):
         assert size(_cache_desc(**change), _attn()) == 0, change
     for change in (dict(heads_q=3), dict(heads_q=0), dict(heads_q=1 << 20), dict(dtype=capi.F32), dict(max_new=-1), dict(mask_width=-1),

@@ -358,6 +358,41 @@ def test_tables_out_of_range_are_left_out_and_reported():
     assert run([[0], [1]], [0, 4, 9], [0, 0])[1:] == (good + [5.0] * 4,) * 2
 
 
+def test_sequences_that_share_rows_do_not_overflow_the_plan():
+    """Starts that descend again and again: twenty sequences of all rows, whose work counted in 32 bits would begin anew."""
+    import torch
+    import frisk_b200 as F
+    rows, width, page = 65536, 4096, 1024
+    cache = F.paged_cache(1, 1, page, 64, torch.float16)
+    table = torch.zeros(40, width, dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, rows] * 20 + [0], dtype=torch.int32, device="cuda")
+    lengths = torch.full((40,), 4000000, dtype=torch.int32, device="cuda")
+    q = torch.zeros(rows, 1, 64, dtype=torch.float16, device="cuda")
+    out = torch.full_like(q, 5.0)
+    F.cache_attention(cache, q, table, starts, lengths, tile_rows=16, out=out)
+    with pytest.raises(RuntimeError):
+        F.cache_check()
+    assert bool((out == 5.0).all())
+
+
+def test_a_mask_without_columns_takes_no_memory():
+    """Tables and results in one buffer: the mask's rows have nothing that the results could overlap."""
+    import torch
+    import frisk_b200 as F
+    rows, d = 600, 64
+    buffer = torch.zeros(256 + rows * d * 2, dtype=torch.uint8, device="cuda")
+    starts, lengths, table = (buffer[a:a + 4 * n].view(torch.int32) for a, n in ((0, 2), (8, 1), (16, 40)))
+    starts[1], lengths[0] = rows, 7
+    table.copy_(torch.arange(40))
+    out = buffer[256:].view(torch.float16).view(rows, 1, d)
+    cache = F.paged_cache(40, 1, 16, d, torch.float16)
+    cache[1].fill_(2.0)
+    q = torch.randn(rows, 1, d, generator=torch.Generator().manual_seed(3)).half().cuda()
+    F.cache_attention(cache, q, table.view(1, 40), starts, lengths, mask=torch.empty(rows, 0, dtype=torch.bool, device="cuda"), out=out)
+    F.cache_check()
+    assert bool((out == 2.0).all())
+
+
 def test_captured_step_replayed_with_other_contents():
     """Rotate, write, attend: captured once, replayed as the sequences grow; two graphs at once; and step by step without a graph."""
     import torch
