@@ -2,8 +2,8 @@
 // rows and the join of shared items): tcgen05 over tiles of 128 rows.
 //
 // A (sequence, key head) has new tokens times query heads rows; a unit is 64 keys of one tile of 128 rows, or of two tiles
-// that share the K and V (kPair).  Each CTA has two softmax groups of four warps (thread = row) and an MMA-issuing warp for either:
-//   * kPair: group g has row tile g, both take every key tile;
+// that share the K and V (PAIR).  Each CTA has two softmax groups of four warps (thread = row) and an MMA-issuing warp for either:
+//   * PAIR: group g has row tile g, both take every key tile;
 //   * else one row tile, whose key tiles the groups take in turn, each with scores, O and statistics of its own, put together at the end
 //     of the CTA's part of the item.
 // S = Q.K^T into one of two TMEM buffers a group, P back over its scores as 16-bit pairs, O += P.V from there.  S runs two key tiles ahead of
@@ -15,9 +15,10 @@
 //
 // 8-bit caches: the products take the codes as they are (kind::f8f6f4), and what meets them is written as a sum of e4m3 values, one
 // MMA each.  A query row, scaled by a power of two to at most 256, becomes two terms (bf16) or three (fp16) whose sum is the query but for
-// what lies 2^-19 below the row's largest element.  A weight becomes two: the first has 4 bits, the second 4 of the rest, 2^-8 of the weight
+// what lies 2^-17 below the row's largest element.  A weight becomes two: the first has 4 bits, the second 4 of the rest, 2^-8 of the weight
 // in all as with bf16 weights, or 2^-15.75 of the weight at the reference A, which moves when the maximum grew by more than 2^3.  (2^-17 and
-// 2^1 moved it in most of an item's first tiles: 173 us where 157 were due.)  Converting the codes to halves instead took four warps 1.6 us a tile (2.5 us a tile of 64 rows in all).
+// 2^1 moved it in most of an item's first tiles: 173 us where 157 were due.)  Converting the codes to halves
+// instead took four warps 1.6 us a tile (2.5 us a tile of 64 rows in all).
 // Keys' scales multiply the scores; values' scales the weights, w = 2^(s + v - A): v is the tile's largest, as one number in the exponent,
 // and a factor for every key relative to it.  The row sum has no part in the values' scales and is kept in units of 2^B of its own.  The
 // checking warp prepares the scales.
@@ -25,8 +26,10 @@
 // 8-bit tiles whose values' scales span more than 2^8 ("wide") take a path of rolled loops over tensor memory.  (Code that runs once an item
 // has to be fetched: unrolled for masked tiles, too, it cost up to 20 us a tile.)
 //
-// What bounds it: up to 128 rows HBM, 0.77 us a 16-bit tile of 64 keys a SM; else the softmax groups (some 1700 clk for 64 keys of 256
-// rows, of which 1024 exponentials).
+// What bounds it: up to 128 rows HBM, 0.77 us a 16-bit tile of 64 keys a SM (32 sequences of 8000 keys, 64 rows a head 174 us); else the
+// softmax groups (some 1700 clk for 64 keys of 256 rows, of which 1024 exponentials: 64 new tokens over 8 x 32000 keys 420 us).  At 8 bits
+// the softmax groups throughout, 1.07 us a tile, whose weights take 3900 instructions of a SM's warps where 16 bits take 2200 (16 x 6000
+// keys, 96 rows a head 115 us).
 // Every mbarrier wait is bounded (ptx.cuh); no TMA load uses cluster multicast.
 #include <algorithm>
 #include <cfloat>
