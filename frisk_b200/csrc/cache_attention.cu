@@ -17,7 +17,7 @@
 //
 // Bound by HBM at 16 bits, since every key and value is read once (per row tile): 32 sequences of 8000 keys, 8 heads of 128, 4 rows a head
 // take 146 us, 6.1 TB/s of the 6.5 that a copy reaches.  At 8 bits by the conversion of the codes, several instructions for two of them:
-// 140 us for the same keys, 3.2 TB/s.  (mma.sync on the codes themselves took 1151 instructions for 32 keys of a warp, 182 us.)
+// 123 us for the same keys, 3.6 TB/s.  (mma.sync on the codes themselves took 1151 instructions for 32 keys of a warp, 182 us.)
 // The (sequence, head, row tile, 64-key tile) units are numbered in this order and CTA c takes a contiguous range, whatever the lengths:
 // every SM streams the same number of bytes.  The lengths live on the device, so each CTA sums up the units itself.  What a CTA holds of a
 // shared item goes to the workspace with the record of the item, and a second kernel, launched early and waiting, joins the parts in
@@ -40,8 +40,12 @@ constexpr int kKeys = 64;  // of a tile
 constexpr int kRows = 16;  // query rows, padded
 
 // Consumer warps: four share a tile; with 8-bit caches two fours take the tiles in turn, since a tile comes in half the time and has
-// its codes to convert (32 sequences of 8000 keys, 4 rows a head: 240 us with one four, 140 with two, 204 with three of 152 registers a thread).
+// its codes to convert (32 sequences of 8000 keys, 4 rows a head: 240 us with one four, 123 with two, 159 with three of 152 registers a thread).
 template <bool E4M3> constexpr int warps_of() { return E4M3 ? 8 : 4; }
+// Threads of a CTA.  8-bit: the warp that loads is one of a group of four, which gives its registers to the other two groups: a ninth warp
+// of its own would leave 168 registers a thread to all, and spills (141 us).
+template <bool E4M3> constexpr int threads_of() { return 32 * (warps_of<E4M3>() + (E4M3 ? 4 : 1)); }
+constexpr int kRegsConsumer = 224, kRegsProducer = 56;  // 256 * 224 + 128 * 56 = 384 * 168, what the CTA was launched with
 
 // ones in the elements of `w` (codes, or 16-bit floats) that are infinite or NaN
 template <bool E4M3, bool BF16>
@@ -103,12 +107,12 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 
 // QBF16: type of the queries and results.  E4M3: 8-bit cache, products in halves; else the cache has the queries' type.
 template <bool QBF16, bool E4M3, int D>
-__global__ void __launch_bounds__(32 * (warps_of<E4M3>() + 1), 1)
+__global__ void __launch_bounds__(threads_of<E4M3>(), 1)
     cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                            const CacheAttnParams p) {
   using L = RowSmem<D, E4M3>;
   constexpr bool MBF16 = QBF16 && !E4M3;  // type of the products' operands
-  constexpr int kWarps = L::kWarps, kThreads = 32 * (kWarps + 1);
+  constexpr int kWarps = L::kWarps, kThreads = threads_of<E4M3>();
   constexpr int kBoxes = E4M3 ? 1 : D / 64, kBoxBytes = kKeys * 128;
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
@@ -137,14 +141,15 @@ __global__ void __launch_bounds__(32 * (warps_of<E4M3>() + 1), 1)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Plan plan = make_plan<kThreads>(p, kRows, plan_shared);
 
-  if (warp == kWarps) {
+  if (warp >= kWarps) {
+    if (E4M3) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsProducer));
     // ------------------------------------------------------------------ TMA producer
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
     const int box = min(p.t.page, kKeys);  // rows a load brings
     PageWalk walk;
-    for (Cursor c(p, plan, kRows); c.left > 0 && ok; c.next_item(p, kRows)) {
+    for (Cursor c(p, plan, kRows); warp == kWarps && c.left > 0 && ok; c.next_item(p, kRows)) {
       const int end = c.tile + c.tiles_here(), keys = c.seq.length + c.seq.count;
       walk.enter(p, p.t.table + c.b * p.t.stride, keys, c.h, c.tile, lane);
       for (int tile = c.tile; tile < end; ++tile) {
@@ -185,6 +190,7 @@ __global__ void __launch_bounds__(32 * (warps_of<E4M3>() + 1), 1)
       }
     }
   } else {
+    if (E4M3) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsConsumer));
     // ------------------------------------------------------------------ consumers
     const int g = lane >> 2, tq = lane & 3;  // fragment coordinates: rows g and g + 8, column pair tq
     const int four = warp >> 2, part_keys = (warp & 3) * 16;  // which tiles, which of their keys
@@ -625,16 +631,21 @@ int launch_rows(frisk_b200_ctx* ctx, const CacheAttnParams& p, const CUtensorMap
   auto kern = cache_attention_kernel<QBF16, E4M3, D>;
   using L = RowSmem<D, E4M3>;
   static PerDeviceOnce opt_in;
-  if (opt_in(ctx->device, [&] {
-        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) == cudaSuccess ? 0 : 1;
-      }))
-    return FRISK_B200_E_CUDA;
+  const int rc = opt_in(ctx->device, [&] {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) != cudaSuccess) return (int)FRISK_B200_E_CUDA;
+    if (!E4M3) return 0;
+    // setmaxnreg.inc waits until the CTA's own registers hold the request: what the launch brings must cover both shares
+    cudaFuncAttributes a;
+    if (cudaFuncGetAttributes(&a, kern) != cudaSuccess) return (int)FRISK_B200_E_CUDA;
+    return a.numRegs * threads_of<E4M3>() >= L::kWarps * 32 * kRegsConsumer + 128 * kRegsProducer ? 0 : (int)FRISK_B200_E_UNSUPPORTED;
+  });
+  if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernels wait (griddepcontrol.wait) themselves
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(32 * (L::kWarps + 1));
+  cfg.blockDim = dim3(threads_of<E4M3>());
   cfg.dynamicSmemBytes = L::kTotal;
   cfg.stream = s;
   cfg.attrs = attr;
@@ -694,10 +705,10 @@ int check_attention(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_
 // Query rows a tile, by the rows that a sequence is said to have for a key head.  (A sequence with more than a tile's rows takes several
 // tiles, so a hint that is too low costs time only.)  Up to 16 rows this file's kernel; from 129 on tiles of 256.  In between it is
 // weighed: this kernel reads the keys once for every 16 rows, the tiles of 128 once, at a higher cost of beginning and ending an item.  In
-// us, with n key tiles a SM: 16 rows 0.74 n (16-bit, D = 128), 0.40 (D = 64), 0.61 and 0.49 (8-bit); tiles 0.77, 0.71, 1.07 and 1.02 n and 10
-// (8-bit 14) more.  Measured, this kernel and tiles: 8 sequences of 4000 keys at D = 128, 32 rows a head 45.6 and 42.3, 8-bit 53.7 and 60.8; of
-// 1000 keys 21.5 and 27.8, 27.3 and 35.5; 48 rows 29.5 and 28.3, 37.7 and 36.1; 32 sequences of 8000, 32 rows at D = 64 194 and 178, 8-bit 228
-// and 273.  n goes by the table's width, the longest that the sequences can be.
+// us, with n key tiles a SM: 16 rows 0.74 n (16-bit, D = 128), 0.40 (D = 64), 0.55 and 0.45 (8-bit); tiles 0.77, 0.71, 1.07 and 1.02 n and 10
+// (8-bit 14) more.  Measured, this kernel and tiles: 8 sequences of 4000 keys at D = 128, 32 rows a head 42.8 and 46.3, 8-bit 45.3 and
+// 61.5; of 1000 keys 14.8 and 27.4, 16.6 and 34.6; 48 rows of 1000 keys 27.2 and 28.9, 30.5 and 35.0; 32 sequences of 8000 keys, 32 rows,
+// 8-bit 241 and 259, at D = 64 171 and 154, 8-bit 196 and 237.  n goes by the table's width, the longest that the sequences can be.
 int tile_rows_of(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_desc* a) {
   const int64_t per = a->max_new > 0 ? a->max_new : c->batch > 0 ? (c->rows + c->batch - 1) / c->batch : 1;
   const int64_t rows = per * (a->heads_q / c->heads);
@@ -706,7 +717,7 @@ int tile_rows_of(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_des
   if (rows > 128) return 256;
   const bool e4m3 = c->dtype == FRISK_B200_E4M3;
   const double n = (double)c->batch * c->heads * ((double)c->table_width * c->page / kKeys) / kNumSMsDefault;
-  const double few = e4m3 ? (c->D == 128 ? 0.61 : 0.49) : (c->D == 128 ? 0.74 : 0.40);
+  const double few = e4m3 ? (c->D == 128 ? 0.55 : 0.45) : (c->D == 128 ? 0.74 : 0.40);
   const double tiles = e4m3 ? (c->D == 128 ? 1.07 : 1.02) : (c->D == 128 ? 0.77 : 0.71);
   return (rows + kRows - 1) / kRows * few * n < tiles * n + (e4m3 ? 14 : 10) ? kRows : 128;
 }
