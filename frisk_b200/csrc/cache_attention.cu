@@ -577,53 +577,78 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
   __syncthreads();
 }
 
-// Joins the parts of the items that several CTAs worked on.  Block (c, y): rows 4 y .. of the item that CTA c began and others
-// finished, a warp each, and those gridDim.y blocks on.
+// Joins the parts of the items that several CTAs worked on.  Block (c, y): rows 8 y .. of the item that CTA c began and others
+// finished, a warp each, or several, which take their shares of the parts, where there are fewer rows.  (A warp each for four rows
+// and 125 parts took 20 us of 33.  Blocks of 16 warps: 4 rows of 32000 keys 22 us for 24, but 24 tokens over 16 x 6000 keys 121 for 120.)
+constexpr int kJoinWarps = 8, kJoinAhead = 8;  // parts that a lane has in flight
 template <bool QBF16, bool E4M3, int D>
-__global__ void __launch_bounds__(128) cache_attention_join_kernel(const CacheAttnParams p, int tile_rows) {
+__global__ void __launch_bounds__(32 * kJoinWarps) cache_attention_join_kernel(const CacheAttnParams p, int tile_rows) {
+  __shared__ float4 sums[kJoinWarps][D / 4];
+  __shared__ float sums_l[kJoinWarps];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const ItemRecord rec = p.records[blockIdx.x];
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const size_t floats = partial_floats(tile_rows, D);
   // the item's first part is the CTA's last item; the others' is their first
   auto slot = [&](int i) { return p.partials + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? rec.first_slot : 0)) * floats; };
-  // (rec.rows is 0 where the CTA shares no item that it began)
-  for (int row = blockIdx.y * 4 + (threadIdx.x >> 5); row < rec.rows; row += gridDim.y * 4) {
+  const int rows = min(rec.rows - (int)blockIdx.y * kJoinWarps, kJoinWarps);
+  if (rows <= 0) return;  // (rec.rows is 0 where the CTA shares no item that it began)
+  const int split = kJoinWarps >> (32 - __clz(rows - 1));  // warps a row
+  const int local = warp / split, row = blockIdx.y * kJoinWarps + local;
+  const int share = (rec.parts + split - 1) / split, part0 = warp % split * share, part1 = min(part0 + share, rec.parts);
+  constexpr int N = D / 32;  // columns a lane: 4 or 2
+  float acc[N] = {}, l = 0.f;
+  if (local < rows) {
     float m = -INFINITY;
     for (int i = lane; i < rec.parts; i += 32) m = fmaxf(m, __ldcg(slot(i) + tile_rows * D + row));
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-    constexpr int N = D / 32;  // columns a lane: 4 or 2
-    float acc[N] = {}, l = 0.f;
-    for (int i0 = 0; i0 < rec.parts; i0 += 32) {
+    for (int i0 = part0; i0 < part1; i0 += 32) {
       float f = 0.f, lc = 0.f;
-      if (i0 + lane < rec.parts) {
+      if (i0 + lane < part1) {
         const float* s = slot(i0 + lane) + tile_rows * D + row;
         const float mc = __ldcg(s);
         lc = __ldcg(s + tile_rows);
         f = mc == -INFINITY ? (lc == 0.f ? 0.f : 1.f) : ex2f(mc - m);
       }
-      const int here = min(32, rec.parts - i0);
-#pragma unroll 4
-      for (int i = 0; i < here; ++i) {
-        const float fi = __shfl_sync(0xffffffffu, f, i), li = __shfl_sync(0xffffffffu, lc, i);
-        const float* from = slot(i0 + i) + row * D + lane * N;
-        float v[N];
-        if (N == 4) *reinterpret_cast<float4*>(v) = __ldcg(reinterpret_cast<const float4*>(from));
-        else *reinterpret_cast<float2*>(v) = __ldcg(reinterpret_cast<const float2*>(from));
-        if (fi == 0.f && li == 0.f) continue;  // saw no key of the row
-        l = fmaf(li, fi, l);
+      const int here = min(32, part1 - i0);
+#pragma unroll 1
+      for (int i = 0; i < here; i += kJoinAhead) {
+        float v[kJoinAhead][N];
 #pragma unroll
-        for (int x = 0; x < N; ++x) acc[x] += scaled(v[x], fi);
+        for (int u = 0; u < kJoinAhead; ++u) {
+          if (i + u >= here) break;
+          const float* from = slot(i0 + i + u) + row * D + lane * N;
+          if (N == 4) *reinterpret_cast<float4*>(v[u]) = __ldcg(reinterpret_cast<const float4*>(from));
+          else *reinterpret_cast<float2*>(v[u]) = __ldcg(reinterpret_cast<const float2*>(from));
+        }
+#pragma unroll
+        for (int u = 0; u < kJoinAhead; ++u) {
+          const float fi = __shfl_sync(0xffffffffu, f, i + u), li = __shfl_sync(0xffffffffu, lc, i + u);
+          if (i + u >= here) break;
+          if (fi == 0.f && li == 0.f) continue;  // saw no key of the row
+          l = fmaf(li, fi, l);
+#pragma unroll
+          for (int x = 0; x < N; ++x) acc[x] += scaled(v[u][x], fi);
+        }
       }
     }
-    if (N == 4) {
-      store_row4<QBF16, E4M3>(p, rec.first_row, rec.head, rec.row0 + row, lane, make_float4(acc[0], acc[1], acc[N - 2], acc[N - 1]), l);
-    } else {
-      const float ox = __shfl_down_sync(0xffffffffu, acc[0], 1), oy = __shfl_down_sync(0xffffffffu, acc[1], 1);
-      if (!(lane & 1)) store_row4<QBF16, E4M3>(p, rec.first_row, rec.head, rec.row0 + row, lane >> 1, make_float4(acc[0], acc[1], ox, oy), l);
-    }
+#pragma unroll
+    for (int x = 0; x < N; ++x) reinterpret_cast<float*>(sums[warp])[lane * N + x] = acc[x];
+    if (lane == 0) sums_l[warp] = l;
   }
+  __syncthreads();
+  // a row's shares in order, four columns a lane
+  const int r = warp * (32 / (D / 4)) + lane / (D / 4), c4 = lane % (D / 4);
+  if (r >= rows) return;
+  float4 sum = sums[r * split][c4];
+  l = sums_l[r * split];
+  for (int i = 1; i < split; ++i) {
+    const float4 x = sums[r * split + i][c4];
+    sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
+    l += sums_l[r * split + i];
+  }
+  store_row4<QBF16, E4M3>(p, rec.first_row, rec.head, rec.row0 + blockIdx.y * kJoinWarps + r, c4, sum, l);
 }
 
 template <bool QBF16, bool E4M3, int D>
@@ -664,8 +689,8 @@ int launch_all(frisk_b200_ctx* ctx, const CacheAttnParams& p, const CUtensorMap&
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(grid, (unsigned)std::min(tile_rows / 4, 16));
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(grid, (unsigned)(tile_rows / kJoinWarps));
+  cfg.blockDim = dim3(32 * kJoinWarps);
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;

@@ -56,7 +56,7 @@ __device__ __forceinline__ unsigned units_of(const CacheAttnParams& p, const Seq
 }
 
 struct PlanShared {
-  unsigned warp_sum[32];
+  unsigned warp_sum[16], warp_most[16];
   unsigned first_b, first_off;
 };
 struct Plan {
@@ -75,15 +75,23 @@ __device__ __forceinline__ Plan make_plan(const CacheAttnParams& p, int tile_row
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int chunk = (p.t.batch + THREADS - 1) / THREADS;
   const int b_lo = min((int)threadIdx.x * chunk, p.t.batch), b_hi = min(b_lo + chunk, p.t.batch);
-  unsigned mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine = add_units(mine, units_of(p, load_seq(p.t, b, p.status), tile_rows));
+  unsigned mine = 0, most = 0;  // units; key tiles of the longest sequence
+  for (int b = b_lo; b < b_hi; ++b) {
+    const Seq s = load_seq(p.t, b, p.status);
+    mine = add_units(mine, units_of(p, s, tile_rows));
+    if (s.count > 0) most = max(most, (unsigned)key_tiles(s));
+  }
   unsigned upto = mine;  // of the warp's threads up to this one
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const unsigned other = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto = add_units(upto, other);
   }
-  if (lane == 31) sh->warp_sum[warp] = upto;
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 31) {
+    sh->warp_sum[warp] = upto;
+    sh->warp_most[warp] = most;
+  }
   __syncthreads();
   unsigned before = upto - mine, total = 0;
 #pragma unroll
@@ -91,15 +99,21 @@ __device__ __forceinline__ Plan make_plan(const CacheAttnParams& p, int tile_row
     const unsigned n = sh->warp_sum[w];
     before += w < warp ? n : 0;
     total = add_units(total, n);
+    most = max(most, sh->warp_most[w]);
   }
   if (total == kTooMany) {
     atomicCAS(p.status, 0u, ST_CACHE_ROWS);
     total = 0;
   }
-  const WorkSplit work{total / gridDim.x, total % gridDim.x};
+  // Little work goes to fewer CTAs: the parts of an item of n key tiles cost as much to join as their tiles take where a CTA has some sqrt(n /
+  // 10) tiles.  (One key head, dealt to 148 CTAs and so: 4 rows, 3000 keys 12.4 and 10.8 us, 8000 17.9 and 12.4, 32000 at 8 bits 32.6 and 24.1;
+  // 200 rows, 9500 keys at 8 bits 47.9 and 38.5.)
+  const unsigned least = p.whole ? 1u : max(1u, (unsigned)sqrtf((float)most * 0.1f));
+  const unsigned workers = max(1u, min(gridDim.x, total / least));
+  const WorkSplit work{total / workers, total % workers};
   Plan plan;
-  plan.begin = work.start(blockIdx.x);
-  plan.end = work.start(blockIdx.x + 1);
+  plan.begin = min(work.start(blockIdx.x), total);
+  plan.end = min(work.start(blockIdx.x + 1), total);
   auto holds = [&](unsigned u) { return before <= u && u - before < mine; };
   if (plan.begin < plan.end) {
     if (holds(plan.begin)) {

@@ -208,6 +208,16 @@ def test_attention(counts, lengths, hkv, group, d, page, dtype, scales):
     attend(b, mask=tree(b, 4, width=max(1, max(counts) // 2)), max_new=1, scale=0.31)
 
 
+@pytest.mark.parametrize("dtype,held", [("bfloat16", None), ("float16", "float8_e4m3fn")])
+@pytest.mark.parametrize("count,group,d,length", [(1, 1, 64, 9001), (1, 3, 128, 5000), (5, 1, 128, 4999), (3, 3, 64, 300), (11, 1, 64, 7000), (29, 5, 128, 6007)])
+def test_one_long_sequence(count, group, d, length, dtype, held):
+    """One key head: the parts of many CTAs are joined, shared among the warps where rows are few."""
+    import torch
+    batch = Batch([count], [length], 1, group, d, 16, getattr(torch, dtype), held and getattr(torch, held), 9)
+    attend(batch)
+    attend(batch, mask=tree(batch, 13))
+
+
 @pytest.mark.parametrize("e4m3", [False, True])
 def test_rows_that_see_nothing_are_zero(e4m3):
     import torch
