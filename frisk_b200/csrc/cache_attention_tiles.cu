@@ -26,10 +26,10 @@
 // 8-bit tiles whose values' scales span more than 2^8 ("wide") take a path of rolled loops over tensor memory.  (Code that runs once an item
 // has to be fetched: unrolled for masked tiles, too, it cost up to 20 us a tile.)
 //
-// What bounds it: up to 128 rows HBM, 0.77 us a 16-bit tile of 64 keys a SM (32 sequences of 8000 keys, 64 rows a head 174 us); else the
+// What bounds it: up to 128 rows HBM, 0.77 us a 16-bit tile of 64 keys a SM (32 sequences of 8000 keys, 64 rows a head 182 us); else the
 // softmax groups (some 1700 clk for 64 keys of 256 rows, of which 1024 exponentials: 64 new tokens over 8 x 32000 keys 420 us).  At 8 bits
 // the softmax groups throughout, 1.07 us a tile, whose weights take 3900 instructions of a SM's warps where 16 bits take 2200 (16 x 6000
-// keys, 96 rows a head 115 us).
+// keys, 96 rows a head 120 us).
 // Every mbarrier wait is bounded (ptx.cuh); no TMA load uses cluster multicast.
 #include <algorithm>
 #include <cfloat>

@@ -22,7 +22,7 @@ enum : unsigned {
   ST_CACHE_LENGTH = 0x302,  // a negative length, or more keys than the table's width holds
   ST_CACHE_PAGE = 0x303,    // a page outside the cache
   ST_CACHE_KV = 0x304,      // (a wait) key tiles
-  ST_CACHE_S = 0x305, ST_CACHE_P = 0x306, ST_CACHE_O = 0x307, ST_CACHE_RAW = 0x308, ST_CACHE_Q = 0x309,
+  ST_CACHE_S = 0x305, ST_CACHE_P = 0x306, ST_CACHE_O = 0x307, ST_CACHE_Q = 0x309,
 };
 
 struct Tables {
