@@ -13,12 +13,14 @@
 // are used: rows behind the last key become zeros, and so do infinities and NaN, because their product with a weight of zero would reach
 // rows that do not see them; if there were any, rows that do see them get them back when O is stored.
 //
-// 8-bit caches: the products take the codes as they are (kind::f8f6f4), and what meets them is written as a sum of e4m3 values, one
-// MMA each.  A query row, scaled by a power of two to at most 256, becomes two terms (bf16) or three (fp16) whose sum is the query but for
-// what lies 2^-17 below the row's largest element.  A weight becomes two: the first has 4 bits, the second 4 of the rest, 2^-8 of the weight
-// in all as with bf16 weights, or 2^-15.75 of the weight at the reference A, which moves when the maximum grew by more than 2^3.  (2^-17 and
-// 2^1 moved it in most of an item's first tiles: 173 us where 157 were due.)  Converting the codes to halves
-// instead took four warps 1.6 us a tile (2.5 us a tile of 64 rows in all).
+// 8-bit caches: the products take the codes as they are (kind::f8f6f4), and what meets them is written as a sum of 8-bit values, one
+// MMA each.  A query row, scaled by a power of two to at most 256, becomes two e4m3 terms (bf16) or three (fp16) whose sum is the query but
+// for what lies 2^-17 below the row's largest element.  A weight becomes a half, 2^12.75 at the reference A, and the half three e5m2 terms
+// (bf16; 2^-9 of the weight in all, where bf16 weights have 2^-8) or four (fp16; exact).  e5m2 has the half's exponents: what is lost of a
+// small weight is 2^-17, 2^-29.75 of the weight at A, so that thousands of keys beside a dominant one keep theirs.  (Two e4m3 terms end at
+// 2^-15.75 of it: the rest of 2000 keys, e^-11 each, vanished.  They took 119.6 us where this takes 126, 16 x 6000 keys, 96 rows a head.)
+// A moves when the maximum grew by more than 2^3.  Converting the codes to halves instead took four warps 1.6 us a tile (2.5 us a tile of
+// 64 rows in all).
 // Keys' scales multiply the scores; values' scales the weights, w = 2^(s + v - A): v is the tile's largest, as one number in the exponent,
 // and a factor for every key relative to it.  The row sum has no part in the values' scales and is kept in units of 2^B of its own.  The
 // checking warp prepares the scales.
@@ -28,8 +30,7 @@
 //
 // What bounds it: up to 128 rows HBM, 0.77 us a 16-bit tile of 64 keys a SM (32 sequences of 8000 keys, 64 rows a head 182 us); else the
 // softmax groups (some 1700 clk for 64 keys of 256 rows, of which 1024 exponentials: 64 new tokens over 8 x 32000 keys 420 us).  At 8 bits
-// the softmax groups throughout, 1.07 us a tile, whose weights take 3900 instructions of a SM's warps where 16 bits take 2200 (16 x 6000
-// keys, 96 rows a head 120 us).
+// the softmax groups throughout, 1.12 us a tile, for the terms of their weights (16 x 6000 keys, 96 rows a head 126 us).
 // Every mbarrier wait is bounded (ptx.cuh); no TMA load uses cluster multicast.
 #include <algorithm>
 #include <cfloat>
@@ -48,8 +49,8 @@ constexpr int kThreadsTiles = 384;  // warps 0-3, 4-7: softmax groups; 8: TMA; 9
 constexpr int kWarpFix = 11;
 constexpr int kInfos = 8;            // key tiles whose scales are kept, for either group
 constexpr uint32_t kNarrow = 8;      // log2: scales of a tile's values that lie this close share a reference
-constexpr float kTop8 = 5.75f;       // log2 of the 8-bit weight at the reference
-constexpr float kRescale8 = 3.f;     // 8-bit: the reference moves when the maximum grew by more than this (together 2^8.75, e4m3 ends at 448)
+constexpr float kTop8 = 12.75f;      // log2 of the 8-bit weight at the reference
+constexpr float kRescale8 = 3.f;     // 8-bit: the reference moves when the maximum grew by more than this (together 2^15.75, e5m2 ends at 2^15.8)
 
 // the scales of a key tile, 8-bit caches
 struct alignas(16) TileInfo {
@@ -89,25 +90,30 @@ template <int ROW>
 __device__ __forceinline__ uint32_t swizzled(uint32_t at) {
   return at ^ (ROW == 128 ? ((at >> 7) & 7) << 4 : ((at >> 7) & 3) << 4);
 }
-// four halves as e4m3 values: the nearest, and the nearest to what is left
-__device__ __forceinline__ void two_terms(uint32_t ha, uint32_t hb, uint32_t& first, uint32_t& second) {
-  uint32_t ba, bb;
-  asm("{\n\t.reg .b16 a, b;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f16x2 a, %3;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f16x2 b, %4;\n\t"
-      "mov.b32 %0, {a, b};\n\t"
-      "cvt.rn.f16x2.e4m3x2 %1, a;\n\t"
-      "cvt.rn.f16x2.e4m3x2 %2, b;\n\t}\n"
-      : "=r"(first), "=r"(ba), "=r"(bb)
-      : "r"(ha), "r"(hb));
-  const __half2 ra = __hsub2(*reinterpret_cast<const __half2*>(&ha), *reinterpret_cast<const __half2*>(&ba));
-  const __half2 rb = __hsub2(*reinterpret_cast<const __half2*>(&hb), *reinterpret_cast<const __half2*>(&bb));
-  asm("{\n\t.reg .b16 a, b;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f16x2 a, %1;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f16x2 b, %2;\n\t"
-      "mov.b32 %0, {a, b};\n\t}\n"
-      : "=r"(second)
-      : "r"(*reinterpret_cast<const uint32_t*>(&ra)), "r"(*reinterpret_cast<const uint32_t*>(&rb)));
+// Four halves (not negative) as sums of TERMS e5m2 values.  An e5m2 value is the upper byte of a half, so every term but the last is what
+// three bits hold of the rest, and the rest is exact.  Four terms hold the half's 11 bits, three are off by 2^-9 of it at most, and
+// either by half of the smallest e5m2 step, 2^-17.
+template <int TERMS>
+__device__ __forceinline__ void terms_of(uint32_t ha, uint32_t hb, uint32_t (&term)[TERMS]) {
+#pragma unroll
+  for (int t = 0; t < TERMS - 1; ++t) {
+    term[t] = __byte_perm(ha, hb, 0x7531);
+    const uint32_t ba = ha & 0xff00ff00u, bb = hb & 0xff00ff00u;
+    const __half2 ra = __hsub2(*reinterpret_cast<const __half2*>(&ha), *reinterpret_cast<const __half2*>(&ba));
+    const __half2 rb = __hsub2(*reinterpret_cast<const __half2*>(&hb), *reinterpret_cast<const __half2*>(&bb));
+    ha = *reinterpret_cast<const uint32_t*>(&ra);
+    hb = *reinterpret_cast<const uint32_t*>(&rb);
+  }
+  if (TERMS == 4) {  // (two bits are left, or what lies below the smallest step)
+    term[TERMS - 1] = __byte_perm(ha + 0x00800080u, hb + 0x00800080u, 0x7531);
+  } else {
+    asm("{\n\t.reg .b16 a, b;\n\t"
+        "cvt.rn.satfinite.e5m2x2.f16x2 a, %1;\n\t"
+        "cvt.rn.satfinite.e5m2x2.f16x2 b, %2;\n\t"
+        "mov.b32 %0, {a, b};\n\t}\n"
+        : "=r"(term[TERMS - 1])
+        : "r"(ha), "r"(hb));
+  }
 }
 
 template <bool QBF16, bool E4M3, int D, bool PAIR>
@@ -120,7 +126,8 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
   constexpr int kBoxes = E4M3 ? 1 : D / 64, kBoxBytes = BM * 128, kKvBoxBytes = BN * 128;  // (16-bit: column blocks of 128 bytes)
   constexpr int kStages = L::kStages, kOwnStages = OWN_KV ? kStages / 2 : kStages;
   constexpr int kElem = L::kElem;
-  constexpr int kPTerms = E4M3 ? 2 : 1;  // of a weight
+  constexpr int kPTerms = !E4M3 ? 1 : QBF16 ? 3 : 4;  // of a weight
+  constexpr int kPWords = E4M3 ? kPTerms : 2;         // of four weights, or of two and two
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -260,9 +267,9 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
       // ones the softmax groups are slower than the MMAs, and turns would tie them together (24 over 16 x 6000 keys 115 -> 121).  One
       // elected lane issues.
       const int mq = __shfl_sync(0xffffffffu, warp - kWarpMma, 0);
-      // (kind::f8f6f4 has the fields of kind::f16; type 0 is e4m3 there)
+      // (kind::f8f6f4 has the fields of kind::f16; type 0 is e4m3 there, and 1, of the weights, e5m2)
       constexpr uint32_t idesc_s = umma_idesc_f16(BM, BN, QBF16 && !E4M3, false, false);
-      constexpr uint32_t idesc_o = umma_idesc_f16(BM, D, QBF16 && !E4M3, false, true);
+      constexpr uint32_t idesc_o = umma_idesc_f16(BM, D, QBF16 && !E4M3, false, true) | (E4M3 ? 1u << 7 : 0u);
       const uint32_t q_tile = smem_u32(smem) + (PAIR ? mq * L::kTerms * L::kQTile : 0);
       const uint64_t dq = E4M3 ? desc_rows<D>(q_tile) : umma_desc_kmajor_sw128(q_tile);
       const uint64_t dk = E4M3 ? desc_rows<D>(smem_u32(smem + L::kRing)) : umma_desc_kmajor_sw128(smem_u32(smem + L::kRing));
@@ -616,7 +623,7 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
           }
           l_sum = fmaf(sum, ex2f(unit - b_ref), l_sum);
         };
-        uint32_t pk0[16], pk1[16];  // the weights' first and second 32 keys (16-bit), or first and second terms
+        uint32_t pk[kPWords][16];  // the weights' first and second 32 keys (16-bit), or their terms
         // What the row sees of the tile's keys, a bit a key.  The warp's rows belong to a few neighbouring tokens: the warp reads each one's
         // mask side by side, eight tokens' at a time.
         auto look = [&](uint32_t (&see)[2]) {
@@ -695,13 +702,16 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
             sa = add2(sa, ea);
             sb = add2(sb, eb);
             if (!E4M3) {
-              pk0[e] = pack16<QBF16>(ea.x, ea.y);
-              pk1[e] = pack16<QBF16>(eb.x, eb.y);
+              pk[0][e] = pack16<QBF16>(ea.x, ea.y);
+              pk[1][e] = pack16<QBF16>(eb.x, eb.y);
             } else {
               const float4 f = *reinterpret_cast<const float4*>(info->v + e * 4);
               ea = mul2_rn(ea, make_float2(f.x, f.y));
               eb = mul2_rn(eb, make_float2(f.z, f.w));
-              two_terms(pack16<false>(ea.x, ea.y), pack16<false>(eb.x, eb.y), pk0[e], pk1[e]);
+              uint32_t term[kPWords];
+              terms_of(pack16<false>(ea.x, ea.y), pack16<false>(eb.x, eb.y), term);
+#pragma unroll
+              for (int t = 0; t < kPWords; ++t) pk[t][e] = term[t];
             }
           }
           const float2 tot = add2(sa, sb);
@@ -738,10 +748,12 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
           // the weights; what the loop makes of 16 keys is put into its place by selection, since P is written where scores still are
           float sum = 0.f;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) pk0[e] = pk1[e] = 0;
+          for (int e = 0; e < 16; ++e)
+#pragma unroll
+            for (int t = 0; t < kPWords; ++t) pk[t][e] = 0;
 #pragma unroll 1
           for (int x = 0; x < BN / 16; ++x) {
-            uint32_t y[16], a[8], b2[4];
+            uint32_t y[16], a[8];
             __syncwarp();
             tmem_ld_32x32b_x16(t_s + buf * BN + x * 16, y);
             tmem_ld_wait();
@@ -759,17 +771,18 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
               a[e] = pack16<QBF16 && !E4M3>(wgt[0], wgt[1]);
             }
             if (E4M3) {
+              uint32_t term[4][kPWords];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) two_terms(a[2 * e], a[2 * e + 1], a[e], b2[e]);
-            }
+              for (int e = 0; e < 4; ++e) terms_of(a[2 * e], a[2 * e + 1], term[e]);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              if (E4M3) {
-                pk0[e] = e / 4 == x ? a[e % 4] : pk0[e];
-                pk1[e] = e / 4 == x ? b2[e % 4] : pk1[e];
-              } else {
-                pk0[e] = e / 8 == x ? a[e % 8] : pk0[e];
-                pk1[e] = e / 8 + 2 == x ? a[e % 8] : pk1[e];
+              for (int e = 0; e < 16; ++e)
+#pragma unroll
+                for (int t = 0; t < kPWords; ++t) pk[t][e] = e / 4 == x ? term[e % 4][t] : pk[t][e];
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                pk[0][e] = e / 8 == x ? a[e % 8] : pk[0][e];
+                pk[1][e] = e / 8 + 2 == x ? a[e % 8] : pk[1][e];
               }
             }
           }
@@ -778,9 +791,9 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
         // (the scores read ahead take the registers of this tile's)
         const bool ahead = __all_sync(0xffffffffu, more && mbar_test(&s_full[2 * q + (steps & 1)], (steps >> 1) & 1));
         if (ahead) load_scores();
-        // P is written over the first half of the scores it comes from
-        tmem_st_32x32b_x16(t_s + buf * BN, pk0);
-        tmem_st_32x32b_x16(t_s + buf * BN + 16, pk1);
+        // P is written over the scores it comes from
+#pragma unroll
+        for (int t = 0; t < kPWords; ++t) tmem_st_32x32b_x16(t_s + buf * BN + t * 16, pk[t]);
         tmem_st_wait();
         tc_fence_before_sync();
         mbar_arrive(&p_ready[2 * q + buf]);

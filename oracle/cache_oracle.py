@@ -101,15 +101,16 @@ def attention(cache, q, table, starts, lengths, mask=None, scale=None, terms=Fal
     """(results, bound): float64 [rows, heads, D], and for each how far a kernel may be off that rounds each probability (and scale
     times probability) by half a step of its operands' type, works in 32 bits otherwise and rounds the result once.
 
-    ``terms``: an 8-bit cache whose products take e4m3 sums.  A weight of two terms, the first off by 2^-4 of it at most and the second by
-    2^-4 of the rest, is off by 2^-8, or by half of the smallest e4m3 step, 2^-10, where the largest probability times the largest
-    scale of the values stands at 2^5.75 or more.  A query's terms leave 2^-10 of a row scaled to 128 or more."""
+    ``terms``: an 8-bit cache whose products take sums of 8-bit values.  A weight becomes a half and the half three e5m2 values for bf16 (each
+    keeps 3 bits of the rest, the last is rounded: off by 2^-9) or four for fp16 (exact), and in either case is off by half of the smallest
+    step, 2^-17.  The largest weight times scale stands at 2^12.75 or more, but for the 2^8 that the scales of a tile's values may be apart:
+    2^(8 - 17 - 12.75) of it.  A query's e4m3 terms leave 2^-10 of a row scaled to 128 or more."""
     n, heads_q, d = q.shape
     heads, page = cache[0].shape[1], cache[0].shape[2]
     group, scale = heads_q // heads, d ** -0.5 if scale is None else scale
     k_all, v_all = values(cache, 0), values(cache, 1)
     h_out = H[q.dtype]
-    h_p = 2.0 ** -8 + 2.0 ** -11 if terms else H[torch.float16] if len(cache) == 4 else h_out
+    h_p = (2.0 ** -9 if q.dtype == torch.bfloat16 else 0.0) + 2.0 ** -11 if terms else H[torch.float16] if len(cache) == 4 else h_out
     out, bound = torch.zeros(n, heads_q, d, dtype=torch.float64), torch.zeros(n, heads_q, d, dtype=torch.float64)
     for b in range(len(lengths)):
         first, rows, length = int(starts[b]), int(starts[b + 1]) - int(starts[b]), int(lengths[b])
@@ -142,8 +143,8 @@ def attention(cache, q, table, starts, lengths, mask=None, scale=None, terms=Fal
             far = torch.where(torch.isfinite(weighted), weighted, 0.0).abs().amax(dim=(1, 2))[:, None] * 2.0 ** -22
             if terms:
                 e = cache[3][at, h // group, j % page].double()
-                e = torch.where(see.any(0) & (e < 255), e, 0.0)
-                codes = torch.where(torch.isfinite(v), v, 0.0).abs() * torch.exp2(127 - e)[:, None] * (e > 0)[:, None]
-                far = far + 2.0 ** -15.75 * p.nan_to_num().amax(1, keepdim=True) * 2.0 ** (float(e.max()) - 127) * codes.sum(0)[None]
+                scale_v = torch.where(see.any(0) & (e < 255), torch.exp2(e - 127), 0.0)
+                codes = torch.where(torch.isfinite(v), v, 0.0).abs() * torch.where(scale_v > 0, 1 / scale_v, 0.0)[:, None]
+                far = far + 2.0 ** -21.75 * (p.nan_to_num() * scale_v).amax(1, keepdim=True) * codes.sum(0)[None]
             bound[first:first + rows, h] = h_p * a + delta * a + h_out * (o.abs() + (h_p + delta) * a) + far + 1e-30
     return out, bound

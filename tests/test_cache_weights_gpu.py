@@ -1,0 +1,54 @@
+"""Attention over the cache where weights are far apart: a dominant key and what thousands of others add to it."""
+import pytest
+import torch
+
+from tests.test_cache_gpu import Batch, attend
+
+pytestmark = pytest.mark.gpu
+
+
+def with_a_sink(counts, lengths, hkv, group, d, dtype, held, nats, at=0):
+    """A batch whose key ``at`` of every sequence scores ``nats`` above the others, its value 0.01 beside theirs about 1."""
+    b = Batch(counts, lengths, hkv, group, d, 64, dtype, held, 21)
+    g = torch.Generator().manual_seed(5)
+    b.q[:, :, 0] = 4.0
+    cpu = [t.clone() for t in b.cpu]
+    for n, (count, length) in enumerate(zip(counts, lengths)):
+        j = torch.arange(count + length)
+        where = b.table_cpu[n].long()[j // 64], slice(None), j % 64
+        k, v = 0.05 * torch.randn(len(j), hkv, d, generator=g), 1.0 + 0.1 * torch.randn(len(j), hkv, d, generator=g)
+        k[:, :, 0] = 0.0
+        k[at], v[at] = 0.0, 0.01
+        k[at, :, 0] = nats * d ** 0.5 / 4.0
+        for i, x in enumerate((k, v)):
+            if len(cpu) == 4:  # 2^-6: keys up to 7, 2^-8: values up to 1.75
+                cpu[i][where] = (x * 2.0 ** (6 + 2 * i)).to(torch.float8_e4m3fn)
+                cpu[2 + i][where] = 127 - 6 - 2 * i
+            else:
+                cpu[i][where] = x.to(dtype)
+    if len(cpu) == 4:  # larger keys: another scale
+        for n in range(len(counts)):
+            where = int(b.table_cpu[n, at // 64]), slice(None), at % 64
+            cpu[0][where] = torch.zeros(hkv, d).to(torch.float8_e4m3fn)
+            cpu[0][where[0], :, where[2], 0] = torch.tensor(nats * d ** 0.5 / 4.0 * 8.0).to(torch.float8_e4m3fn)
+            cpu[2][where] = 124
+    b.cpu = tuple(cpu)
+    b.refresh()
+    return b
+
+
+# (one head's parts shared by many CTAs; several whole items a CTA; more rows than a tile)
+SINKS = [([5], [32000], 1, 8, 64), ([3] * 40, [200 + 9 * i for i in range(40)], 8, 2, 128), ([70], [4000], 1, 4, 128)]
+
+
+@pytest.mark.parametrize("nats", [6.0, 8.0, 10.0, 11.0, 14.0])
+@pytest.mark.parametrize("counts,lengths,hkv,group,d", SINKS)
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("held", [None, "float8_e4m3fn"])
+def test_the_others_beside_a_dominant_key(nats, counts, lengths, hkv, group, d, dtype, held):
+    """What the others weigh is in the results of every kernel, however the choice among them falls."""
+    b = with_a_sink(counts, lengths, hkv, group, d, getattr(torch, dtype), held and getattr(torch, held), nats)
+    for rows in (16, 128, 256):
+        attend(b, tile_rows=rows)
+    for hint in (1, 64):
+        attend(b, tile_rows=0, max_new=hint)
