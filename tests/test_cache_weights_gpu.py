@@ -7,11 +7,13 @@ from tests.test_cache_gpu import Batch, attend
 pytestmark = pytest.mark.gpu
 
 
-def with_a_sink(counts, lengths, hkv, group, d, dtype, held, nats, at=0):
-    """A batch whose key ``at`` of every sequence scores ``nats`` above the others, its value 0.01 beside theirs about 1."""
+def with_a_sink(counts, lengths, hkv, group, d, dtype, held, nats, at=0, apart=0):
+    """A batch whose key ``at`` of every sequence scores ``nats`` above the others, its value 0.01 beside theirs about 1.  ``apart``: every
+    64th key scores 280 / sqrt(D) below the others, and its values' scale (8-bit) is 2^apart times theirs."""
     b = Batch(counts, lengths, hkv, group, d, 64, dtype, held, 21)
     g = torch.Generator().manual_seed(5)
-    b.q[:, :, 0] = 4.0
+    size = 40.0 if apart else 4.0
+    b.q[:, :, 0] = size
     cpu = [t.clone() for t in b.cpu]
     for n, (count, length) in enumerate(zip(counts, lengths)):
         j = torch.arange(count + length)
@@ -19,18 +21,23 @@ def with_a_sink(counts, lengths, hkv, group, d, dtype, held, nats, at=0):
         k, v = 0.05 * torch.randn(len(j), hkv, d, generator=g), 1.0 + 0.1 * torch.randn(len(j), hkv, d, generator=g)
         k[:, :, 0] = 0.0
         k[at], v[at] = 0.0, 0.01
-        k[at, :, 0] = nats * d ** 0.5 / 4.0
+        k[at, :, 0] = nats * d ** 0.5 / size
+        if apart:
+            k[5::64] = 0.0
+            k[5::64, :, 0] = -7.0
         for i, x in enumerate((k, v)):
             if len(cpu) == 4:  # 2^-6: keys up to 7, 2^-8: values up to 1.75
                 cpu[i][where] = (x * 2.0 ** (6 + 2 * i)).to(torch.float8_e4m3fn)
                 cpu[2 + i][where] = 127 - 6 - 2 * i
+                if apart and i:
+                    cpu[3][b.table_cpu[n].long()[j[5::64] // 64], :, j[5::64] % 64] += apart
             else:
                 cpu[i][where] = x.to(dtype)
     if len(cpu) == 4:  # larger keys: another scale
         for n in range(len(counts)):
             where = int(b.table_cpu[n, at // 64]), slice(None), at % 64
             cpu[0][where] = torch.zeros(hkv, d).to(torch.float8_e4m3fn)
-            cpu[0][where[0], :, where[2], 0] = torch.tensor(nats * d ** 0.5 / 4.0 * 8.0).to(torch.float8_e4m3fn)
+            cpu[0][where[0], :, where[2], 0] = torch.tensor(nats * d ** 0.5 / size * 8.0).to(torch.float8_e4m3fn)
             cpu[2][where] = 124
     b.cpu = tuple(cpu)
     b.refresh()
@@ -52,3 +59,13 @@ def test_the_others_beside_a_dominant_key(nats, counts, lengths, hkv, group, d, 
         attend(b, tile_rows=rows)
     for hint in (1, 64):
         attend(b, tile_rows=0, max_new=hint)
+
+
+@pytest.mark.parametrize("nats", [6.0, 12.0, 14.0, 15.5])
+@pytest.mark.parametrize("apart", [4, 5, 8])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_scales_that_no_weight_stands_behind(nats, apart, dtype):
+    """Keys that weigh little and have larger values' scales than the others, one in every tile."""
+    b = with_a_sink([6] * 20, [1900 + 17 * i for i in range(20)], 2, 3, 64, getattr(torch, dtype), torch.float8_e4m3fn, nats, apart=apart)
+    for rows in (16, 128, 256):
+        attend(b, tile_rows=rows)
