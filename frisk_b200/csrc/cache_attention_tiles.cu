@@ -26,7 +26,8 @@
 // checking warp prepares the scales.
 //
 // In the common path A goes by the tile's largest score and largest scale, which may be of two keys: what is lost of a weight is then up to
-// 2^-25.75 of the largest.  8-bit tiles whose values' scales span more than 2^4 ("wide") take a path of rolled loops over tensor memory.  (Code that runs once an item
+// 2^-25.75 of the largest.  8-bit tiles whose values' scales span more than 2^4 ("wide"), or lie
+// 2^100 below A, take a path of rolled loops over tensor memory.  (Code that runs once an item
 // has to be fetched: unrolled for masked tiles, too, it cost up to 20 us a tile.)
 //
 // What bounds it: up to 128 rows HBM, 0.77 us a 16-bit tile of 64 keys a SM (32 sequences of 8000 keys, 64 rows a head 182 us); else the
@@ -618,6 +619,7 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
           }
         };
         auto add_sum = [&](float sum, float unit) {  // sum * 2^unit to the row sum, 8-bit
+          if (sum == 0.f) unit = b_ref;  // (the row sees nothing of the tile, whose unit may be far above)
           if (unit > b_ref) {
             l_sum *= ex2f(b_ref - unit);
             b_ref = unit;
@@ -656,9 +658,11 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
         };
         // Masked tiles: by selection in the common path where the groups share the rows (32 sequences of 8000 keys, 64 rows a head 187 ->
         // 174 us), in the rolled path where they do not, whose common path is the slower for it (64 new tokens over 8 x 32000 keys 425 -> 461).
-        const bool inline_mask = !PAIR && masked, rolled = (PAIR && masked) || (E4M3 && info->wide != 0);
+        const bool inline_mask = !PAIR && masked;
+        bool rolled = (PAIR && masked) || (E4M3 && info->wide != 0);
         uint32_t see[2] = {0xffffffffu, 0xffffffffu};
         if (inline_mask) look(see);
+        float mx = -INFINITY;  // the largest score
         if (!rolled) {
           if (E4M3) {
 #pragma unroll
@@ -685,10 +689,21 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
 #pragma unroll
             for (int x = 0; x < 2; ++x)
               mxc[2 * x + (e & 1)] = max3f(mxc[2 * x + (e & 1)], __uint_as_float(sr[x][2 * e]), __uint_as_float(sr[x][2 * e + 1]));
-          const float mx = max3f(mxc[0], mxc[1], fmaxf(mxc[2], mxc[3])) * row_scale;
-          const float v_log2 = E4M3 ? info->v_log2 : 0.f;
-          settle(E4M3 ? mx + v_log2 : mx);
+          mx = max3f(mxc[0], mxc[1], fmaxf(mxc[2], mxc[3])) * row_scale;
+          const float most = E4M3 ? mx + info->v_log2 : mx;
+          // The common path has one exponential for the weight and the row sum.  Where A stands 2^100 above the tile's weights (values of
+          // tiles before were that much larger), the exponentials would leave 32 bits' range, and the sum with them: rolled.
+          constexpr float kFar = 100.f, kMid = (kFar - kThreshold) / 2.f;
+          if (!E4M3) {
+            settle(most);
+          } else if (__any_sync(0xffffffffu, fabsf(most - a_ref + kMid) > kMid + kThreshold)) {  // (one vote for both)
+            rolled = __any_sync(0xffffffffu, mx > -FLT_MAX && a_ref - most > kFar);
+            if (!rolled) settle(most);
+          }
           if (!ok) break;
+        }
+        if (!rolled) {
+          const float v_log2 = E4M3 ? info->v_log2 : 0.f;
           const float unit = E4M3 ? a_ref - v_log2 - kTop8 : a_ref;  // the exponentials are 2^(score - unit)
           const float2 scale2 = make_float2(row_scale, row_scale), neg2 = make_float2(-unit, -unit);
           float2 sa = make_float2(0.f, 0.f), sb = make_float2(0.f, 0.f);
@@ -720,7 +735,8 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
         } else {
           if (PAIR && masked) look(see);
           // In rolled loops over 16 keys: the scores, scaled, in tensor memory again, -inf for what the row does not see; their maxima.
-          float mx = -INFINITY, mw = -INFINITY;  // largest score, largest score plus scale of the value
+          mx = -INFINITY;
+          float mw = -INFINITY;  // largest score plus scale of the value
 #pragma unroll 1
           for (int x = 0; x < BN / 16; ++x) {
             uint32_t y[16];

@@ -69,3 +69,26 @@ def test_scales_that_no_weight_stands_behind(nats, apart, dtype):
     b = with_a_sink([6] * 20, [1900 + 17 * i for i in range(20)], 2, 3, 64, getattr(torch, dtype), torch.float8_e4m3fn, nats, apart=apart)
     for rows in (16, 128, 256):
         attend(b, tile_rows=rows)
+
+
+@pytest.mark.parametrize("first,then", [(243, 80), (67, 187), (243, 107), (230, 66)])
+@pytest.mark.parametrize("count,length", [(40, 700), (130, 128), (70, 64)])
+def test_values_of_tiles_far_apart(first, then, count, length):
+    """Values' scales of the first 64 keys, near the end of the type's range, and of the others: the row sum keeps its range."""
+    counts, lengths = [count] + [3] * 60, [length] + [500 + 7 * i for i in range(60)]  # (a CTA has whole items)
+    b = Batch(counts, lengths, 4, 1, 64, 64, torch.bfloat16, torch.float8_e4m3fn, 22)
+    g = torch.Generator().manual_seed(3)
+    cpu = [t.clone() for t in b.cpu]
+    for n, keys in enumerate(x + y for x, y in zip(counts, lengths)):
+        j = torch.arange(keys)
+        where = b.table_cpu[n].long()[j // 64], slice(None), j % 64
+        cpu[1][where] = (2.0 * torch.randn(keys, 4, 64, generator=g)).clamp(-4, 4).to(torch.float8_e4m3fn)
+        cpu[2][where] = 117
+        cpu[3][where] = torch.where(j < 64, first, then).to(torch.uint8)[:, None]
+    b.cpu = tuple(cpu)
+    b.refresh()
+    alone = torch.eye(count, dtype=torch.bool)  # whole tiles of new tokens that a row does not see
+    alone = torch.cat([alone] + [alone[:3]] * 60)
+    for rows in (16, 128, 256):
+        attend(b, tile_rows=rows)
+        attend(b, tile_rows=rows, mask=alone)
