@@ -112,6 +112,7 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
                            const CacheAttnParams p) {
   using L = RowSmem<D, E4M3>;
   constexpr bool MBF16 = QBF16 && !E4M3;  // type of the products' operands
+  constexpr float kTop = !QBF16 && !E4M3 ? kTopHalf : 0.f;  // log2 of the probabilities (16-bit: weights) at the reference
   constexpr int kWarps = L::kWarps, kThreads = threads_of<E4M3>();
   constexpr int kBoxes = E4M3 ? 1 : D / 64, kBoxBytes = kKeys * 128;
   extern __shared__ unsigned char smem_unaligned[];
@@ -272,7 +273,7 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
         }
       }
       float o[D / 8][4];
-      float m_ref[2], l_sum[2], a_ref[2];  // rows g and g + 8 (l: this lane's columns)
+      float m_ref[2], l_sum[2], a_ref[2];  // rows g and g + 8 (l: this lane's columns; a_ref: what 2^0 of a weight stands for)
 #pragma unroll
       for (int n = 0; n < D / 8; ++n)
 #pragma unroll
@@ -444,7 +445,7 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
           grow |= m_new[h] - m_ref[h] > kRescaleThreshold;  // (false while no key has been seen: -inf - -inf)
           if (E4M3) {
             mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, 2));
-            a_new[h] = fmaxf(a_ref[h], mw);
+            a_new[h] = fmaxf(a_ref[h], mw - kTopHalf);
             grow |= a_new[h] - a_ref[h] > kRescaleThreshold;
           }
         }
@@ -470,7 +471,7 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           // (a row that sees no key yet: keep it finite)
-          const float m0 = m_ref[h] == -INFINITY ? 0.f : m_ref[h], a0 = a_ref[h] == -INFINITY ? 0.f : a_ref[h];
+          const float m0 = (m_ref[h] == -INFINITY ? 0.f : m_ref[h]) - kTop, a0 = a_ref[h] == -INFINITY ? 0.f : a_ref[h];
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
             float w[2];

@@ -47,6 +47,11 @@ struct CacheAttnParams {
 
 constexpr int kTileKeys = 64;
 
+// log2 of a weight held as a half where the score is the reference, which a score passes by 2^8 at most: halves end just below 2^16 and at
+// 2^-25 of nothing is left, so that 2^-32 of the reference is held of every key, however many there are.  (With 2^0 there, 60 thousand keys
+// 17 or 18 below a dominant one in the exponent came out doubled or not at all.)
+constexpr float kTopHalf = 7.f;
+
 __device__ __forceinline__ int key_tiles(const Seq& s) { return (s.length + s.count + kTileKeys - 1) / kTileKeys; }
 __device__ __forceinline__ int row_tiles(const CacheAttnParams& p, const Seq& s, int tile_rows) {
   return (s.count * p.group + tile_rows - 1) / tile_rows;

@@ -595,6 +595,7 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
         const bool more = i + 1 < n_tiles;
         const bool masked = tile >= w.first_masked;
         constexpr float kThreshold = E4M3 ? kRescale8 : kRescaleThreshold;
+        constexpr float kTop = E4M3 ? kTop8 : QBF16 ? 0.f : kTopHalf;  // log2 of the weight at the reference
         // Takes a new reference where it grew by more than the threshold: rare.  O is rescaled in tensor memory.
         auto settle = [&](float most) {
           const float a_new = fmaxf(a_ref, most);
@@ -704,7 +705,7 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
         }
         if (!rolled) {
           const float v_log2 = E4M3 ? info->v_log2 : 0.f;
-          const float unit = E4M3 ? a_ref - v_log2 - kTop8 : a_ref;  // the exponentials are 2^(score - unit)
+          const float unit = a_ref - v_log2 - kTop;  // the exponentials are 2^(score - unit)
           const float2 scale2 = make_float2(row_scale, row_scale), neg2 = make_float2(-unit, -unit);
           float2 sa = make_float2(0.f, 0.f), sb = make_float2(0.f, 0.f);
 #pragma unroll
@@ -780,10 +781,10 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
 #pragma unroll
               for (int n = 0; n < 2; ++n) {
                 const float v = __uint_as_float(y[2 * e + n]);
-                const float pr = ex2f(v - (E4M3 ? b_ref : a_ref));
+                const float pr = ex2f(v - (E4M3 ? b_ref : a_ref - kTop));
                 sum += pr;
                 // (what is not seen weighs nothing, whatever its value's scale is)
-                wgt[n] = !E4M3 ? pr : v == -INFINITY ? 0.f : ex2f(v + info->log2_v[x * 16 + 2 * e + n] - a_ref + kTop8);
+                wgt[n] = !E4M3 ? pr : v == -INFINITY ? 0.f : ex2f(v + info->log2_v[x * 16 + 2 * e + n] - a_ref + kTop);
               }
               a[e] = pack16<QBF16 && !E4M3>(wgt[0], wgt[1]);
             }

@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+import frisk_b200 as F
+from oracle import cache_oracle as co
 from tests.test_cache_gpu import Batch, attend
 
 pytestmark = pytest.mark.gpu
@@ -92,3 +94,18 @@ def test_values_of_tiles_far_apart(first, then, count, length):
     for rows in (16, 128, 256):
         attend(b, tile_rows=rows)
         attend(b, tile_rows=rows, mask=alone)
+
+
+@pytest.mark.parametrize("nats", [17.3, 18.0])
+@pytest.mark.parametrize("dtype,held", [("float16", None), ("bfloat16", None), ("float16", "float8_e4m3fn"), ("bfloat16", "float8_e4m3fn")])
+def test_sixty_thousand_keys_beside_a_dominant_one(nats, dtype, held):
+    """160 sequences over the same pages, so that a CTA holds all keys of one."""
+    many, length = 160, 59_999
+    b = with_a_sink([1], [length], 1, 8, 64, getattr(torch, dtype), held and getattr(torch, held), nats)
+    q, plan = b.q.expand(many, -1, -1).contiguous(), [b.plan[0].expand(many, -1).contiguous()]
+    plan += [torch.tensor(x, dtype=torch.int32, device="cuda") for x in (range(many + 1), [length] * many)]
+    for rows in (16, 128, 256):
+        out = F.cache_attention(b.cache, q, *plan, tile_rows=rows).cpu().double()
+        F.cache_check()
+        ref, bound = co.attention(b.cpu, b.q.cpu(), *b.host, terms=held is not None and rows > 16)
+        assert bool(((out - ref).abs() <= bound).all()), (rows, float((out - ref).abs().max()), float(bound.max()))
