@@ -200,6 +200,40 @@ inline bool ranges_overlap(const void* a, size_t an, const void* b, size_t bn) {
   return a0 < b0 + bn && b0 < a0 + an;
 }
 
+// Packed rows: every element of a tensor has a place of its own, heads inside rows or rows inside heads.
+inline bool packed_distinct(const frisk_b200_packed& x, int64_t rows, int heads, int D) {
+  if (rows <= 1 || heads <= 1) return (rows <= 1 || x.row_stride >= D) && (heads <= 1 || x.head_stride >= D);
+  return (x.head_stride >= D && x.row_stride >= (heads - 1) * x.head_stride + D) ||
+         (x.row_stride >= D && x.head_stride >= (rows - 1) * x.row_stride + D);
+}
+// Two tensors of packed rows have no byte in common.  Ranges that overlap are told apart by their places modulo one of the pitches m:
+// dimensions that step by multiples of m stay in their place, the others widen it; two intervals of a period that do not meet are apart.
+// (Columns of one buffer of rows: m is the row.  Queries and keys side by side in each head: m is the head.)
+inline bool packed_apart(const frisk_b200_packed& a, int a_heads, const frisk_b200_packed& b, int b_heads, int64_t rows, int D, size_t es) {
+  const frisk_b200_packed* x[2] = {&a, &b};
+  const int heads[2] = {a_heads, b_heads};
+  uintptr_t from[2], to[2];
+  for (int i = 0; i < 2; ++i) {
+    from[i] = reinterpret_cast<uintptr_t>(x[i]->ptr);
+    to[i] = from[i] + (size_t)((rows - 1) * x[i]->row_stride + (heads[i] - 1) * x[i]->head_stride + D) * es;
+  }
+  if (to[0] <= from[1] || to[1] <= from[0]) return true;
+  const int64_t size = (int64_t)es, delta = (int64_t)(from[1] - from[0]);
+  for (const int64_t pitch : {a.row_stride, a.head_stride, b.row_stride, b.head_stride}) {
+    const int64_t m = pitch * size;
+    if (m <= 0) continue;
+    int64_t length[2];
+    for (int i = 0; i < 2; ++i) {
+      length[i] = D * size;
+      if (rows > 1 && x[i]->row_stride % pitch) length[i] += (rows - 1) * x[i]->row_stride * size;
+      if (heads[i] > 1 && x[i]->head_stride % pitch) length[i] += (heads[i] - 1) * x[i]->head_stride * size;
+    }
+    const int64_t at = ((delta % m) + m) % m;  // where b's interval begins in a's period
+    if (at >= length[0] && at + length[1] <= m) return true;
+  }
+  return false;
+}
+
 inline size_t operand_bytes(int64_t rows, int64_t cols, int64_t ld, size_t es) {
   if (rows <= 0) return 0;
   return (size_t)((rows - 1) * ld + cols) * es;

@@ -211,17 +211,6 @@ cudaError_t launch_type(const RotaryParams& p, bool interleaved, cudaStream_t s)
 size_t span(const frisk_b200_packed& x, int64_t rows, int heads, int D, size_t es) {
   return (size_t)((rows - 1) * x.row_stride + (heads - 1) * x.head_stride + D) * es;
 }
-// Two tensors that share a buffer of rows, each with its columns of every row: the same row pitch, and the ranges of a row apart.
-bool apart(const frisk_b200_packed& a, int a_heads, const frisk_b200_packed& b, int b_heads, int64_t rows, int D, size_t es) {
-  if (!ranges_overlap(a.ptr, span(a, rows, a_heads, D, es), b.ptr, span(b, rows, b_heads, D, es))) return true;
-  if (a.row_stride != b.row_stride || rows < 2) return false;
-  const int64_t pitch = a.row_stride * (int64_t)es;
-  const int64_t a_len = ((a_heads - 1) * a.head_stride + D) * (int64_t)es, b_len = ((b_heads - 1) * b.head_stride + D) * (int64_t)es;
-  if (pitch <= 0 || a_len > pitch || b_len > pitch) return false;
-  const int64_t delta = (int64_t)(reinterpret_cast<intptr_t>(b.ptr) - reinterpret_cast<intptr_t>(a.ptr));
-  const int64_t at = ((delta % pitch) + pitch) % pitch;  // where b's range begins in a's rows
-  return at >= a_len && at + b_len <= pitch;
-}
 bool same(const frisk_b200_packed& a, const frisk_b200_packed& b) {
   return a.ptr == b.ptr && a.row_stride == b.row_stride && a.head_stride == b.head_stride;
 }
@@ -254,14 +243,13 @@ extern "C" int frisk_b200_rotary(frisk_b200_ctx* ctx, const frisk_b200_rotary_de
   for (int i = 0; i < n; ++i) {
     // what is written: rows and heads apart from one another, from the other tensor's, and from every input but its own
     const frisk_b200_packed& o = *out[i];
-    const int64_t row_len = (heads[i] - 1) * o.head_stride + d->D;
-    if ((heads[i] > 1 && o.head_stride < d->D) || (d->rows > 1 && o.row_stride < row_len)) return FRISK_B200_E_CACHE_SHAPE;
+    if (!packed_distinct(o, d->rows, heads[i], d->D)) return FRISK_B200_E_CACHE_SHAPE;
     if (ranges_overlap(o.ptr, span(o, d->rows, heads[i], d->D, es), positions, (size_t)d->rows * (d->positions64 ? 8 : 4)) ||
         ranges_overlap(o.ptr, span(o, d->rows, heads[i], d->D, es), frequencies, (size_t)d->dim / 2 * 8))
       return FRISK_B200_E_OVERLAP;
     for (int j = 0; j < n; ++j) {
-      if (!(i == j && same(o, *in[i])) && !apart(o, heads[i], *in[j], heads[j], d->rows, d->D, es)) return FRISK_B200_E_OVERLAP;
-      if (i < j && !apart(o, heads[i], *out[j], heads[j], d->rows, d->D, es)) return FRISK_B200_E_OVERLAP;
+      if (!(i == j && same(o, *in[i])) && !packed_apart(o, heads[i], *in[j], heads[j], d->rows, d->D, es)) return FRISK_B200_E_OVERLAP;
+      if (i < j && !packed_apart(o, heads[i], *out[j], heads[j], d->rows, d->D, es)) return FRISK_B200_E_OVERLAP;
     }
   }
   RotaryParams p{};

@@ -1,7 +1,7 @@
 """Rotary positions of queries and keys: ``rotary``, its gradients ``rotary_backward``, and ``rotary_frequencies``.
 
-Packed rows [tokens, heads, D], as a projection leaves them: queries and keys may be columns of one buffer.  The first
-``2 * len(frequencies)`` elements of every head are rotated in pairs, the others pass:
+Packed rows [tokens, heads, D], as a projection leaves them: queries and keys may be columns of one buffer, or lie side by side in each
+head.  The first ``2 * len(frequencies)`` elements of every head are rotated in pairs, the others pass:
 
     (a, b) -> amplitude * (a cos t - b sin t, b cos t + a sin t),    t = position * frequency
 """

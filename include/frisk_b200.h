@@ -299,8 +299,9 @@ typedef struct frisk_b200_packed {
  * their pair, times `amplitude`: (a, b) -> amplitude * (a cos t - b sin t, b cos t + a sin t).  Pairs are (i, i + dim/2), or
  * (2i, 2i + 1) where interleaved.  The other elements are copied.  `inverse`: -t, which maps gradients of the results to
  * gradients of the inputs.  positions: rows of int32 or int64; frequencies: dim/2 doubles, radians per position; both on the
- * device.  Angles are reduced to one turn in 64 bits.  F32, F16, BF16, any strides; an output may be its input (same
- * pointer and strides), otherwise outputs overlap nothing.  q and k may be columns of one buffer of rows. */
+ * device.  Angles are reduced to one turn in 64 bits.  F32, F16, BF16, any strides (of an output: heads inside rows or rows
+ * inside heads); an output may be its input (same pointer and strides), otherwise outputs overlap nothing.  q and k may be columns
+ * of one buffer of rows, or lie side by side in each head. */
 typedef struct frisk_b200_rotary_desc {
   int64_t rows;
   int32_t heads_q, heads_k, D, dim;
