@@ -142,7 +142,7 @@ def cache_write(cache, k, v, table, starts, lengths, *, stream=None):
 
 def cache_read(cache, table, starts, lengths, rows, *, dtype=None, out=None, stream=None):
     """The packed (keys, values) [rows, heads, D] at the positions of the packed rows, in ``dtype`` (float16 or bfloat16; a 16-bit cache
-    gives its own).  ``lengths`` of zero read sequences from their first key on.  ``out``: a pair of tensors for them; in new ones, rows
+    gives its own).  ``lengths`` of zero read sequences from their first key on.  ``out``: a pair of tensors for them, columns of one buffer perhaps; in new ones, rows
     that belong to no sequence are undefined.  8-bit values beyond the type's range become its largest finite ones."""
     desc, code, dev, heads, d = _describe(cache, table, starts, lengths, rows)
     if dtype is None:
@@ -172,7 +172,8 @@ def cache_attention(cache, q, table, starts, lengths, *, mask=None, scale=None, 
     head h reads key head h // (query heads / key heads).  A row that sees no key is zero; what a row does not see does not reach it,
     whatever it holds.  ``scale`` is 1 / sqrt(D) if not given.  ``max_new``, the largest number of new tokens of a sequence, helps the
     choice of a kernel and changes no result's meaning; ``tile_rows`` makes it: 16, 128 or 256 query rows (new tokens times query heads
-    of a key head) a tile.  Rows of a new ``out`` that belong to no sequence are undefined."""
+    of a key head) a tile.  ``out`` may be columns of the queries' buffer.  Rows of a
+    new one that belong to no sequence are undefined."""
     shape = q.shape
     rows = shape[0]
     desc, code, dev, heads, d = _describe(cache, table, starts, lengths, rows)

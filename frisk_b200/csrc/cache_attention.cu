@@ -778,8 +778,7 @@ extern "C" int frisk_b200_cache_attention(frisk_b200_ctx* ctx, const frisk_b200_
     if ((reinterpret_cast<uintptr_t>(x->ptr) & 15u) || (c->rows > 1 && x->row_stride % 8) || (a->heads_q > 1 && x->head_stride % 8))
       return FRISK_B200_E_ALIGN;
   }
-  if ((a->heads_q > 1 && out->head_stride < c->D) || (c->rows > 1 && out->row_stride < (a->heads_q - 1) * out->head_stride + c->D))
-    return FRISK_B200_E_CACHE_SHAPE;
+  if (!packed_distinct(*out, c->rows, a->heads_q, c->D)) return FRISK_B200_E_CACHE_SHAPE;
   const size_t need = frisk_b200_cache_attention_workspace_bytes(c, a);
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 31u)) return FRISK_B200_E_WORKSPACE;
   const size_t ob = packed_span(*out, c->rows, a->heads_q, c->D, 2), qb = packed_span(*q, c->rows, a->heads_q, c->D, 2);
@@ -787,7 +786,8 @@ extern "C" int frisk_b200_cache_attention(frisk_b200_ctx* ctx, const frisk_b200_
   for (int w = 0; w < 2; ++w) {  // what is written: the results and the workspace
     const void* ptr = w ? workspace : out->ptr;
     const size_t n = w ? need : ob;
-    if (ranges_overlap(ptr, n, q->ptr, qb) || (mb && ranges_overlap(ptr, n, mask, mb)) || cache_overlaps(c, ptr, n) || tables_overlap(c, ptr, n))
+    const bool queries = w ? ranges_overlap(ptr, n, q->ptr, qb) : !packed_apart(*out, a->heads_q, *q, a->heads_q, c->rows, c->D, 2);
+    if (queries || (mb && ranges_overlap(ptr, n, mask, mb)) || cache_overlaps(c, ptr, n) || tables_overlap(c, ptr, n))
       return FRISK_B200_E_OVERLAP;
   }
   if (ranges_overlap(workspace, need, out->ptr, ob)) return FRISK_B200_E_OVERLAP;

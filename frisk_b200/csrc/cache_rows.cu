@@ -278,8 +278,7 @@ size_t packed_span(const frisk_b200_packed& x, int64_t rows, int heads, int D, s
 static int check_side(const frisk_b200_packed* x, int heads, int D, int64_t rows, bool written) {
   if (!x || !x->ptr) return FRISK_B200_E_ARG;
   if (x->row_stride < 0 || x->head_stride < 0) return FRISK_B200_E_CACHE_SHAPE;
-  if (written && ((heads > 1 && x->head_stride < D) || (rows > 1 && x->row_stride < (heads - 1) * x->head_stride + D)))
-    return FRISK_B200_E_CACHE_SHAPE;
+  if (written && !packed_distinct(*x, rows, heads, D)) return FRISK_B200_E_CACHE_SHAPE;
   if ((reinterpret_cast<uintptr_t>(x->ptr) & 15u) || (rows > 1 && x->row_stride % 8) || (heads > 1 && x->head_stride % 8)) return FRISK_B200_E_ALIGN;
   return 0;
 }
@@ -296,7 +295,7 @@ static int cache_rows(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* c, int32
   if ((rc = check_side(k, c->heads, c->D, c->rows, !write)) || (rc = check_side(v, c->heads, c->D, c->rows, !write))) return rc;
   const size_t kb = packed_span(*k, c->rows, c->heads, c->D, 2), vb = packed_span(*v, c->rows, c->heads, c->D, 2);
   if (cache_overlaps(c, k->ptr, kb) || cache_overlaps(c, v->ptr, vb)) return FRISK_B200_E_OVERLAP;
-  if (!write && (ranges_overlap(k->ptr, kb, v->ptr, vb) || tables_overlap(c, k->ptr, kb) || tables_overlap(c, v->ptr, vb)))
+  if (!write && (!packed_apart(*k, c->heads, *v, c->heads, c->rows, c->D, 2) || tables_overlap(c, k->ptr, kb) || tables_overlap(c, v->ptr, vb)))
     return FRISK_B200_E_OVERLAP;
   if (write) {  // the cache's tensors apart from one another and from the tables
     const size_t tokens = (size_t)c->pages * c->heads * c->page, held = tokens * c->D * (c->dtype == FRISK_B200_E4M3 ? 1 : 2);

@@ -336,7 +336,7 @@ typedef struct frisk_b200_cache_desc {
 int frisk_b200_cache_write(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* cache, int32_t dtype,
                            const frisk_b200_packed* k, const frisk_b200_packed* v, void* stream);
 /* The reverse: the packed rows' keys and values out of the cache, rounded to dtype (values of an E4M3 cache saturate at
- * its largest finite one). */
+ * its largest finite one).  k and v share no element; they may be columns of one buffer, heads inside rows or rows inside heads. */
 int frisk_b200_cache_read(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* cache, int32_t dtype,
                           const frisk_b200_packed* k, const frisk_b200_packed* v, void* stream);
 /* Attention of packed query rows [rows, heads_q, D] over the cache, which holds their own keys and values already:
@@ -346,6 +346,7 @@ int frisk_b200_cache_read(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* cach
  * does not reach it, whatever it holds.  dtype: F16 or BF16, of q and out, and of a 16-bit cache.  max_new is a hint: the
  * largest number of new tokens of a sequence (0: unknown); it bears on the kernel that is chosen, as the width of the table
  * does.  tile_rows names one: 16, 128 or 256 query rows a tile (new tokens times query heads of a key head); 0: chosen.
+ * out shares no element with q, and may be columns of the same buffer; its heads lie inside rows or its rows inside heads.
  * The workspace (32-byte aligned, contents of no matter before and after) must not be shared by calls that may overlap. */
 typedef struct frisk_b200_cache_attn_desc {
   int32_t heads_q, dtype, max_new, mask_width;
