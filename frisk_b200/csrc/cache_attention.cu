@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
                            const CacheAttnParams p) {
   using L = RowSmem<D, E4M3>;
   constexpr bool MBF16 = QBF16 && !E4M3;  // type of the products' operands
-  constexpr float kTop = !QBF16 && !E4M3 ? kTopHalf : 0.f;  // log2 of the probabilities (16-bit: weights) at the reference
+  constexpr float kTop = E4M3 ? 0.f : QBF16 ? kTopWide : kTopHalf;  // log2 of the probabilities (16-bit: weights) at the reference
   constexpr int kWarps = L::kWarps, kThreads = threads_of<E4M3>();
   constexpr int kBoxes = E4M3 ? 1 : D / 64, kBoxBytes = kKeys * 128;
   extern __shared__ unsigned char smem_unaligned[];
@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
         const int row = h * 8 + g;
         if (tq == 0) {
           s_m[warp * kRows + row] = m_ref[h];
-          s_l[warp * kRows + row] = l;
+          s_l[warp * kRows + row] = E4M3 ? l * kUnitWide : l;
         }
         // columns in blocks of 8, block index xor a function of the row: rows that are stored together fall into different banks
         float* out = s_o + (warp * kRows + row) * D;
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(threads_of<E4M3>(), 1)
           for (int n = 0; n < D / 8; ++n)
             *reinterpret_cast<float2*>(out + ((n ^ (row & 3)) << 3) + 2 * tq) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
         } else {
-          const float f = m_ref[h] == -INFINITY ? 1.f : ex2f(a_ref[h] - m_ref[h]);  // from A's units to m's
+          const float f = m_ref[h] == -INFINITY ? 1.f : ex2f(a_ref[h] - m_ref[h] + kTopWide);  // from A's units to m's
 #pragma unroll
           for (int u = 0; u < D / 16; ++u)
             *reinterpret_cast<float4*>(out + (((2 * u + (tq >> 1)) ^ (row & 3)) << 3) + (tq & 1) * 4) =

@@ -51,6 +51,9 @@ constexpr int kTileKeys = 64;
 // 2^-25 of nothing is left, so that 2^-32 of the reference is held of every key, however many there are.  (With 2^0 there, 60 thousand keys
 // 17 or 18 below a dominant one in the exponent came out doubled or not at all.)
 constexpr float kTopHalf = 7.f;
+// The same for bf16 weights, and for the row sums and results of 8-bit caches: four million values near the end of the type's range, 2^8
+// times weighted, add up to less than 32 bits' end.  (What is lost of values is below 2^-96.)
+constexpr float kTopWide = -30.f, kUnitWide = 1.f / (1 << 30);
 
 __device__ __forceinline__ int key_tiles(const Seq& s) { return (s.length + s.count + kTileKeys - 1) / kTileKeys; }
 __device__ __forceinline__ int row_tiles(const CacheAttnParams& p, const Seq& s, int tile_rows) {

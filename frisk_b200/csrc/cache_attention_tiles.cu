@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
         const bool more = i + 1 < n_tiles;
         const bool masked = tile >= w.first_masked;
         constexpr float kThreshold = E4M3 ? kRescale8 : kRescaleThreshold;
-        constexpr float kTop = E4M3 ? kTop8 : QBF16 ? 0.f : kTopHalf;  // log2 of the weight at the reference
+        constexpr float kTop = E4M3 ? kTop8 : QBF16 ? kTopWide : kTopHalf;  // log2 of the weight at the reference
         // Takes a new reference where it grew by more than the threshold: rare.  O is rescaled in tensor memory.
         auto settle = [&](float most) {
           const float a_new = fmaxf(a_ref, most);
@@ -828,7 +828,9 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
 
       // ---- O: scaled to the units of the row sum, and out: whole, or as a part for the join
       const float m_mine = E4M3 ? b_ref : a_ref;
-      float f[2] = {E4M3 ? ex2f(a_ref - kTop8 - b_ref) : 1.f, 0.f}, m = m_mine, l = l_sum;
+      float f[2] = {E4M3 ? ex2f(a_ref - kTop8 - b_ref + kTopWide) : 1.f, 0.f}, m = m_mine;
+      if (E4M3) l_sum *= kUnitWide;
+      float l = l_sum;
       if (l_sum == 0.f) f[0] = 0.f;
       if (!PAIR) {
         meet();  // all scores have been read: the statistics take the queries' place

@@ -109,3 +109,24 @@ def test_sixty_thousand_keys_beside_a_dominant_one(nats, dtype, held):
         F.cache_check()
         ref, bound = co.attention(b.cpu, b.q.cpu(), *b.host, terms=held is not None and rows > 16)
         assert bool(((out - ref).abs() <= bound).all()), (rows, float((out - ref).abs().max()), float(bound.max()))
+
+
+@pytest.mark.parametrize("held", [None, "float8_e4m3fn"])
+@pytest.mark.parametrize("counts,lengths,hkv", [([5, 1], [700, 64], 2), ([3] * 40, [600 + i for i in range(40)], 4), ([200], [9000], 1)])
+def test_sums_of_values_near_the_end_of_the_range_are_finite(held, counts, lengths, hkv):
+    b = Batch(counts, lengths, hkv, 2, 64, 64, torch.bfloat16, held and getattr(torch, held), 23)
+    cpu = [t.clone() for t in b.cpu]
+    sign = torch.where(torch.arange(64) % 3 == 0, -1.0, 1.0)
+    for n, keys in enumerate(x + y for x, y in zip(counts, lengths)):
+        j = torch.arange(keys)
+        where = b.table_cpu[n].long()[j // 64], slice(None), j % 64
+        if held:  # 240 * 2^120 is 0.94 of the largest bf16 value
+            cpu[1][where] = (240.0 * sign).expand(keys, hkv, 64).to(torch.float8_e4m3fn)
+            cpu[2][where], cpu[3][where] = 117, 247
+        else:
+            cpu[1][where] = (3.2e38 * sign).expand(keys, hkv, 64).to(torch.bfloat16)
+            cpu[0][where] = (0.1 * cpu[0][where].float()).to(torch.bfloat16)
+    b.cpu = tuple(cpu)
+    b.refresh()
+    for rows in (16, 128, 256):
+        assert bool((attend(b, tile_rows=rows)[b.inside()].abs() > 3e38).all())
