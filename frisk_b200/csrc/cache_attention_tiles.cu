@@ -26,9 +26,9 @@
 // checking warp prepares the scales.
 //
 // In the common path A goes by the tile's largest score and largest scale, which may be of two keys: what is lost of a weight is then up to
-// 2^-25.75 of the largest.  8-bit tiles whose values' scales span more than 2^4 ("wide"), or lie
-// 2^100 below A, take a path of rolled loops over tensor memory.  (Code that runs once an item
-// has to be fetched: unrolled for masked tiles, too, it cost up to 20 us a tile.)
+// 2^-24.75 of the largest.  8-bit tiles whose values' scales span more than 2^5 ("wide"), or lie 2^100 below A, take a path of rolled loops
+// over tensor memory, which takes 2.4 times as long (16 x 6000 keys, 96 rows a head, scales all over: 316 us).  (Code that runs once an
+// item has to be fetched: unrolled for masked tiles, too, it cost up to 20 us a tile.)
 //
 // What bounds it: up to 128 rows HBM, 0.77 us a 16-bit tile of 64 keys a SM (32 sequences of 8000 keys, 64 rows a head 182 us); else the
 // softmax groups (some 1700 clk for 64 keys of 256 rows, of which 1024 exponentials: 64 new tokens over 8 x 32000 keys 420 us).  At 8 bits
@@ -50,7 +50,7 @@ constexpr int BN = kTileKeys;
 constexpr int kThreadsTiles = 384;  // warps 0-3, 4-7: softmax groups; 8: TMA; 9, 10: MMA; 11: checks values, prepares scales
 constexpr int kWarpFix = 11;
 constexpr int kInfos = 8;            // key tiles whose scales are kept, for either group
-constexpr uint32_t kNarrow = 4;      // log2: scales of a tile's values that lie this close share a reference, up to that much above any weight
+constexpr uint32_t kNarrow = 5;      // log2: scales of a tile's values that lie this close share a reference, up to that much above any weight
 constexpr float kTop8 = 12.75f;      // log2 of the 8-bit weight at the reference
 constexpr float kRescale8 = 3.f;     // 8-bit: the reference moves when the maximum grew by more than this (together 2^15.75, e5m2 ends at 2^15.8)
 

@@ -103,8 +103,8 @@ def attention(cache, q, table, starts, lengths, mask=None, scale=None, terms=Fal
 
     ``terms``: an 8-bit cache whose products take sums of 8-bit values.  A weight becomes a half and the half three e5m2 values for bf16 (each
     keeps 3 bits of the rest, the last is rounded: off by 2^-9) or four for fp16 (exact), and in either case is off by half of the smallest
-    step, 2^-17.  The largest weight times scale stands at 2^12.75 or more, but for the 2^4 that the scales of a tile's values may be apart:
-    2^(4 - 17 - 12.75) of it.  A query's e4m3 terms leave 2^-10 of a row scaled to 128 or more."""
+    step, 2^-17.  The largest weight times scale stands at 2^12.75 or more, but for the 2^5 that the scales of a tile's values may be apart:
+    2^(5 - 17 - 12.75) of it.  A query's e4m3 terms leave 2^-10 of a row scaled to 128 or more."""
     n, heads_q, d = q.shape
     heads, page = cache[0].shape[1], cache[0].shape[2]
     group, scale = heads_q // heads, d ** -0.5 if scale is None else scale
@@ -145,6 +145,6 @@ def attention(cache, q, table, starts, lengths, mask=None, scale=None, terms=Fal
                 e = cache[3][at, h // group, j % page].double()
                 scale_v = torch.where(see.any(0) & (e < 255), torch.exp2(e - 127), 0.0)
                 codes = torch.where(torch.isfinite(v), v, 0.0).abs() * torch.where(scale_v > 0, 1 / scale_v, 0.0)[:, None]
-                far = far + 2.0 ** -25.75 * (p.nan_to_num() * scale_v).amax(1, keepdim=True) * codes.sum(0)[None]
+                far = far + 2.0 ** -24.75 * (p.nan_to_num() * scale_v).amax(1, keepdim=True) * codes.sum(0)[None]
             bound[first:first + rows, h] = h_p * a + delta * a + h_out * (o.abs() + (h_p + delta) * a) + far + 1e-30
     return out, bound
