@@ -731,10 +731,10 @@ int check_attention(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_
 // Query rows a tile, by the rows that a sequence is said to have for a key head.  (A sequence with more than a tile's rows takes several
 // tiles, so a hint that is too low costs time only.)  Up to 16 rows this file's kernel; from 129 on tiles of 256.  In between it is
 // weighed: this kernel reads the keys once for every 16 rows, the tiles of 128 once, at a higher cost of beginning and ending an item.  In
-// us, with n key tiles a SM: 16 rows 0.74 n (16-bit, D = 128), 0.40 (D = 64), 0.55 and 0.45 (8-bit); tiles 0.77, 0.71, 1.07 and 1.02 n and 10
-// (8-bit 14) more.  Measured, this kernel and tiles: 8 sequences of 4000 keys at D = 128, 32 rows a head 42.8 and 46.3, 8-bit 45.3 and
-// 61.5; of 1000 keys 14.8 and 27.4, 16.6 and 34.6; 48 rows of 1000 keys 27.2 and 28.9, 30.5 and 35.0; 32 sequences of 8000 keys, 32 rows,
-// 8-bit 241 and 259, at D = 64 171 and 154, 8-bit 196 and 237.  n goes by the table's width, the longest that the sequences can be.
+// us, with n key tiles a SM: 16 rows 0.74 n (16-bit, D = 128), 0.40 (D = 64), 0.55 and 0.45 (8-bit); tiles 0.77, 0.71, 1.16 and 1.10 n and 10
+// (8-bit 14) more.  Measured, this kernel and tiles: 8 sequences of 4000 keys at D = 128, 32 rows a head 43.3 and 46.1, 8-bit 46.0 and
+// 65.6, 48 rows 57.3 and 62.6, 64 rows 64.7 and 61.0; of 1000 keys, 32 rows 15.1 and 27.9, 17.2 and 36.0, 48 rows 27.7 and 29.3, 31.4 and
+// 36.4; 32 sequences of 8000 keys, 32 rows, 8-bit 242 and 281, at D = 64 172 and 154, 8-bit 195 and 257.  n goes by the table's width, the longest that the sequences can be.
 int tile_rows_of(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_desc* a) {
   const int64_t per = a->max_new > 0 ? a->max_new : c->batch > 0 ? (c->rows + c->batch - 1) / c->batch : 1;
   const int64_t rows = per * (a->heads_q / c->heads);
@@ -744,7 +744,7 @@ int tile_rows_of(const frisk_b200_cache_desc* c, const frisk_b200_cache_attn_des
   const bool e4m3 = c->dtype == FRISK_B200_E4M3;
   const double n = (double)c->batch * c->heads * ((double)c->table_width * c->page / kKeys) / kNumSMsDefault;
   const double few = e4m3 ? (c->D == 128 ? 0.55 : 0.45) : (c->D == 128 ? 0.74 : 0.40);
-  const double tiles = e4m3 ? (c->D == 128 ? 1.07 : 1.02) : (c->D == 128 ? 0.77 : 0.71);
+  const double tiles = e4m3 ? (c->D == 128 ? 1.16 : 1.10) : (c->D == 128 ? 0.77 : 0.71);
   return (rows + kRows - 1) / kRows * few * n < tiles * n + (e4m3 ? 14 : 10) ? kRows : 128;
 }
 
