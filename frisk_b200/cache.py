@@ -171,9 +171,9 @@ def cache_attention(cache, q, table, starts, lengths, *, mask=None, scale=None, 
     [rows, width], j counts within the sequence, and what lies beyond the width is not seen.  A single token is a tree of one.  Query
     head h reads key head h // (query heads / key heads).  A row that sees no key is zero; what a row does not see does not reach it,
     whatever it holds.  ``scale`` is 1 / sqrt(D) if not given.  ``max_new``, the largest number of new tokens of a sequence, helps the
-    choice of a kernel and changes no result's meaning; ``tile_rows`` makes it: 16, 128 or 256 query rows (new tokens times query heads
-    of a key head) a tile.  ``out`` may be columns of the queries' buffer.  Rows of a
-    new one that belong to no sequence are undefined."""
+    choice of a kernel, as the table's width does; ``tile_rows`` makes it: 16, 128 or 256 query rows (new tokens times query heads of a
+    key head) a tile.  The kernels round weights differently, each to the 8 bits of bfloat16 or better (float16: 11).  ``out`` may be
+    columns of the queries' buffer.  Rows of a new one that belong to no sequence are undefined."""
     shape = q.shape
     rows = shape[0]
     desc, code, dev, heads, d = _describe(cache, table, starts, lengths, rows)

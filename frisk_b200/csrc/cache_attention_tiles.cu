@@ -18,7 +18,7 @@
 // for what lies 2^-17 below the row's largest element.  A weight becomes a half, 2^12.75 at the reference A, and the half three e5m2 terms
 // (bf16; 2^-9 of the weight in all, where bf16 weights have 2^-8) or four (fp16; exact).  e5m2 has the half's exponents: what is lost of a
 // small weight is 2^-17, 2^-29.75 of the weight at A, so that thousands of keys beside a dominant one keep theirs.  (Two e4m3 terms end at
-// 2^-15.75 of it: the rest of 2000 keys, e^-11 each, vanished.  They took 119.6 us where this takes 126, 16 x 6000 keys, 96 rows a head.)
+// 2^-15.75 of it: the rest of 2000 keys, e^-11 each, vanished.  They took 120 us where this takes 129, 16 x 6000 keys, 96 rows a head.)
 // A moves when the maximum grew by more than 2^3.  Converting the codes to halves instead took four warps 1.6 us a tile (2.5 us a tile of
 // 64 rows in all).
 // Keys' scales multiply the scores; values' scales the weights, w = 2^(s + v - A): v is the tile's largest, as one number in the exponent,
@@ -30,9 +30,10 @@
 // over tensor memory, which takes 2.4 times as long (16 x 6000 keys, 96 rows a head, scales all over: 316 us).  (Code that runs once an
 // item has to be fetched: unrolled for masked tiles, too, it cost up to 20 us a tile.)
 //
-// What bounds it: up to 128 rows HBM, 0.77 us a 16-bit tile of 64 keys a SM (32 sequences of 8000 keys, 64 rows a head 182 us); else the
-// softmax groups (some 1700 clk for 64 keys of 256 rows, of which 1024 exponentials: 64 new tokens over 8 x 32000 keys 420 us).  At 8 bits
-// the softmax groups throughout, 1.12 us a tile, for the terms of their weights (16 x 6000 keys, 96 rows a head 126 us).
+// What bounds it: up to 128 rows HBM, 0.77 us a 16-bit tile of 64 keys a SM (32 sequences of 8000 keys, 64 rows a head 180 us); else the
+// softmax groups (some 1700 clk for 64 keys of 256 rows, of which 1024 exponentials: 64 new tokens over 8 x 32000 keys 422 us in short
+// bursts, 502 under load).  At 8 bits the softmax groups throughout, 1.16 us a tile, for the terms of their weights (16 x 6000 keys, 96
+// rows a head 129 us).
 // Every mbarrier wait is bounded (ptx.cuh); no TMA load uses cluster multicast.
 #include <algorithm>
 #include <cfloat>
@@ -470,8 +471,8 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
       tc_fence_after_sync();
     };
     // A row's query: 16 bytes a piece.  Where the groups share a tile, each brings half of every row (of an 8-bit cache it reads the whole,
-    // whose largest element sets the scale).  Halves are loaded while the item before ends (32 sequences of 8000 keys, 64 rows a head:
-    // 187 -> 176 us); whole rows would take registers that the epilogue needs.
+    // whose largest element sets the scale).  Halves are loaded while the item before ends (32 sequences of 8000 keys, 64 rows a head: 11
+    // of 187 us); whole rows would take registers that the epilogue needs.
     constexpr int kPieces = D / 8 / (PAIR ? 1 : 2), kLoads = E4M3 ? D / 8 : kPieces;
     constexpr bool kEarly = !E4M3 && !PAIR;
     const int first = PAIR ? 0 : q * kPieces;
@@ -657,8 +658,8 @@ __global__ void __launch_bounds__(kThreadsTiles, 1)
           }
           __syncwarp();
         };
-        // Masked tiles: by selection in the common path where the groups share the rows (32 sequences of 8000 keys, 64 rows a head 187 ->
-        // 174 us), in the rolled path where they do not, whose common path is the slower for it (64 new tokens over 8 x 32000 keys 425 -> 461).
+        // Masked tiles: by selection in the common path where the groups share the rows (32 sequences of 8000 keys, 64 rows a head: 2 us
+        // less), in the rolled path where they do not, whose common path is the slower for it (64 new tokens over 8 x 32000 keys 425 -> 461).
         const bool inline_mask = !PAIR && masked;
         bool rolled = (PAIR && masked) || (E4M3 && info->wide != 0);
         uint32_t see[2] = {0xffffffffu, 0xffffffffu};

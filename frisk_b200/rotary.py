@@ -24,7 +24,8 @@ def rotary_frequencies(dim, base=10000.0, *, scaling=None, factor=1.0, trained=N
     * ``"ntk"``         a larger base, with which the slowest pair turns ``factor`` times slower and the fastest stays
     * ``"wavelength"``  pairs with more than ``high`` (4) turns in the trained context stay, those with fewer than ``low`` turn
       ``factor`` times slower, the others in between by their number of turns
-    * ``"yarn"``        the same with ``high`` 32, and amplitude 0.1 ln(factor) + 1
+    * ``"yarn"``        the same with ``high`` 32, and amplitude 0.1 ln(factor) + 1.  (As the method was published; a model whose
+      frequencies go over by the index of the pair instead needs its own, which ``rotary`` takes as well.)
     """
     if dim < 2 or dim % 2:
         raise ValueError("frisk-b200-rotary: dim must be even and positive")
@@ -117,5 +118,6 @@ def rotary(q, k, positions, frequencies, *, amplitude=1.0, interleaved=False, ou
 
 
 def rotary_backward(dq, dk, positions, frequencies, *, amplitude=1.0, interleaved=False, out=None, stream=None):
-    """The gradients of ``rotary``'s inputs from those of its results: the transposed rotation, the same arguments."""
+    """The gradients of ``rotary``'s inputs from those of its results: the transposed rotation, the same arguments.  (Neither is bound to
+    autograd: results of ``rotary`` carry no history.)"""
     return _rotate(dq, dk, positions, frequencies, amplitude, interleaved, out, stream, True)

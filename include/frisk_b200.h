@@ -346,6 +346,7 @@ int frisk_b200_cache_read(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* cach
  * does not reach it, whatever it holds.  dtype: F16 or BF16, of q and out, and of a 16-bit cache.  max_new is a hint: the
  * largest number of new tokens of a sequence (0: unknown); it bears on the kernel that is chosen, as the width of the table
  * does.  tile_rows names one: 16, 128 or 256 query rows a tile (new tokens times query heads of a key head); 0: chosen.
+ * The kernels round the weights of the keys differently, each to 8 bits (BF16) or 11 (F16) or better before they meet the values.
  * out shares no element with q, and may be columns of the same buffer; its heads lie inside rows or its rows inside heads.
  * The workspace (32-byte aligned, contents of no matter before and after) must not be shared by calls that may overlap. */
 typedef struct frisk_b200_cache_attn_desc {
