@@ -221,15 +221,20 @@ __device__ __forceinline__ bool sees(const CacheAttnParams& p, const Seq& s, int
 // x * f, but that what is infinite or NaN stays so where f has vanished
 __device__ __forceinline__ float scaled(float x, float f) { return f == 0.f ? (fabsf(x) <= FLT_MAX ? 0.f : x) : x * f; }
 
+// A result that rounded weights brought beyond the type's range is its largest finite value.  Infinities of 16-bit values stay; 8-bit ones
+// have none, but may lie beyond the range themselves.
+template <bool BF16, bool E4M3>
+__device__ __forceinline__ float in_range(float x) {
+  return E4M3 || fabsf(x) <= FLT_MAX ? saturated<BF16>(x) : x;
+}
+
 // four results of row r (of the sequence and key head), acc / l; a row that saw nothing is zero
 template <bool QBF16, bool E4M3>
 __device__ __forceinline__ void store_row4(const CacheAttnParams& p, int first, int h, int r, int c4, float4 acc, float l) {
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   float x[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-  if (E4M3) {  // values near the end of the type's range may have been rounded beyond it
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = saturated<QBF16>(x[i]);
-  }
+  for (int i = 0; i < 4; ++i) x[i] = in_range<QBF16, E4M3>(x[i]);
   const int i = r / p.group;
   uint16_t* out = static_cast<uint16_t*>(p.out) + (int64_t)(first + i) * p.out_row + (int64_t)(h * p.group + r - i * p.group) * p.out_head;
   *reinterpret_cast<uint2*>(out + c4 * 4) = make_uint2(attn::pack16<QBF16>(x[0], x[1]), attn::pack16<QBF16>(x[2], x[3]));
@@ -247,11 +252,7 @@ __device__ __forceinline__ void store_row32(uint16_t* row, int x, const uint32_t
   uint32_t y[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    float a = __uint_as_float(o[2 * i]) * inv, b = __uint_as_float(o[2 * i + 1]) * inv;
-    if (E4M3) {
-      a = saturated<QBF16>(a);
-      b = saturated<QBF16>(b);
-    }
+    const float a = in_range<QBF16, E4M3>(__uint_as_float(o[2 * i]) * inv), b = in_range<QBF16, E4M3>(__uint_as_float(o[2 * i + 1]) * inv);
     y[i] = attn::pack16<QBF16>(a, b);
   }
   uint16_t* at = row + x * 32;

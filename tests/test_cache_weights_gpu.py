@@ -130,3 +130,27 @@ def test_sums_of_values_near_the_end_of_the_range_are_finite(held, counts, lengt
     b.refresh()
     for rows in (16, 128, 256):
         assert bool((attend(b, tile_rows=rows)[b.inside()].abs() > 3e38).all())
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_the_largest_values_stay_finite(dtype):
+    """All values are the largest of the type, and a late key outweighs the others by less than moves the reference: its weight is rounded,
+    in some rows up."""
+    dtype = getattr(torch, dtype)
+    b = Batch([1] * 20, [64 * 3 + i for i in range(20)], 1, 16, 64, 64, dtype, None, 24)
+    cpu = [t.clone() for t in b.cpu]
+    for n, length in enumerate(b.lengths):
+        j = torch.arange(length + 1)
+        where = b.table_cpu[n].long()[j // 64], slice(None), j % 64
+        cpu[1][where] = torch.where(torch.arange(64) % 2 == 0, -1.0, 1.0).to(dtype) * torch.finfo(dtype).max
+        cpu[0][where] = 0.0
+        cpu[0][where[0], :, where[2], 1] = -30.0
+        cpu[0][int(b.table_cpu[n, 0]), :, 0, 1] = 0.0
+        cpu[0][int(b.table_cpu[n, 2]), :, 11, 0] = 1.0
+        cpu[0][int(b.table_cpu[n, 2]), :, 11, 1] = 0.0
+    b.cpu = tuple(cpu)
+    b.refresh()
+    b.q[:, :, 1] = 16.0  # one key at 0, one late key, the others far below
+    b.q[:, :, 0] = 16 + (torch.arange(20 * 16, device="cuda").view(20, 16) / 16).to(dtype)  # 2 to 4.5 above: 2^2.9 to 2^6.5
+    for rows in (16, 128, 256):
+        assert bool((attend(b, tile_rows=rows).abs() > 0.98 * torch.finfo(dtype).max).all())
