@@ -12,6 +12,7 @@ import pathlib
 
 F32, F16, BF16 = 0, 1, 2
 E4M3 = 3  # element type of a paged cache only
+PAGES_FORK, PAGES_GROW, PAGES_COMPACT = 0, 1, 2
 ALGO_AUTO, ALGO_SIMT_F32, ALGO_TCGEN05, ALGO_SKINNY, ALGO_TCGEN05_PAIR, ALGO_F32_SPLIT = 0, 1, 2, 3, 4, 5
 ATTN_PAIRS, ATTN_SPLIT_KEYS, ATTN_TWO_HEADS, ATTN_FEW_QUERIES = 0, 1, 2, 3
 DTYPE_CODE = {"fp32": F32, "fp16": F16, "bf16": BF16}
@@ -33,6 +34,8 @@ EXPORTS = (
     "frisk_b200_gemm_plan", "frisk_b200_attention_form",
     "frisk_b200_rotary", "frisk_b200_cache_write", "frisk_b200_cache_read", "frisk_b200_cache_attention",
     "frisk_b200_cache_attention_workspace_bytes", "frisk_b200_cache_attention_tile_rows",
+    "frisk_b200_cache_pages_workspace_bytes", "frisk_b200_cache_fork", "frisk_b200_cache_grow", "frisk_b200_cache_compact",
+    "frisk_b200_cache_copy", "frisk_b200_cache_keep", "frisk_b200_draft_verify", "frisk_b200_adapter_gemm",
 )
 
 
@@ -103,6 +106,24 @@ class CacheAttnDesc(ctypes.Structure):
                 ("tile_rows", ctypes.c_int32)]
 
 
+class PageTables(ctypes.Structure):
+    _fields_ = [("users", ctypes.c_void_p), ("users_out", ctypes.c_void_p), ("table_out", ctypes.c_void_p),
+                ("lengths_out", ctypes.c_void_p), ("table_out_stride", ctypes.c_int64)]
+
+
+class VerifyDesc(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("target_stride", ctypes.c_int64), ("draft_stride", ctypes.c_int64),
+                ("batch", ctypes.c_int32), ("max_new", ctypes.c_int32), ("vocab", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("tokens64", ctypes.c_int32)]
+
+
+class AdapterDesc(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("K", ctypes.c_int64), ("N", ctypes.c_int64), ("ldx", ctypes.c_int64),
+                ("lda", ctypes.c_int64), ("a_step", ctypes.c_int64), ("ldb", ctypes.c_int64), ("b_step", ctypes.c_int64),
+                ("ldc", ctypes.c_int64), ("ldo", ctypes.c_int64), ("rank", ctypes.c_int32), ("count", ctypes.c_int32),
+                ("batch", ctypes.c_int32), ("dtype", ctypes.c_int32), ("dtype_c", ctypes.c_int32)]
+
+
 _lib = None
 
 
@@ -120,6 +141,7 @@ def load():
     vp, sz, i32, i64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int32, ctypes.c_int64
     gd, ad, ge = ctypes.POINTER(GemmDesc), ctypes.POINTER(AttnDesc), ctypes.POINTER(GemmEpilogue)
     pk, cd, ca = ctypes.POINTER(Packed), ctypes.POINTER(CacheDesc), ctypes.POINTER(CacheAttnDesc)
+    pt, vd, ap = ctypes.POINTER(PageTables), ctypes.POINTER(VerifyDesc), ctypes.POINTER(AdapterDesc)
     sig = {
         "frisk_b200_ctx_create": (ctypes.c_int, [ctypes.POINTER(vp), ctypes.c_int]),
         "frisk_b200_ctx_destroy": (ctypes.c_int, [vp]),
@@ -158,6 +180,14 @@ def load():
         "frisk_b200_cache_attention": (ctypes.c_int, [vp, cd, ca, pk, pk, vp, vp, sz, vp]),
         "frisk_b200_cache_attention_workspace_bytes": (sz, [cd, ca]),
         "frisk_b200_cache_attention_tile_rows": (ctypes.c_int, [cd, ca]),
+        "frisk_b200_cache_pages_workspace_bytes": (sz, [cd, i32]),
+        "frisk_b200_cache_fork": (ctypes.c_int, [vp, cd, pt, vp, vp, sz, vp]),
+        "frisk_b200_cache_grow": (ctypes.c_int, [vp, cd, pt, vp, sz, vp]),
+        "frisk_b200_cache_compact": (ctypes.c_int, [vp, cd, pt, vp, sz, vp]),
+        "frisk_b200_cache_copy": (ctypes.c_int, [vp, cd, cd, vp, vp, i64, vp]),
+        "frisk_b200_cache_keep": (ctypes.c_int, [vp, cd, vp, i64, i32, vp, vp, vp]),
+        "frisk_b200_draft_verify": (ctypes.c_int, [vp, vd, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
+        "frisk_b200_adapter_gemm": (ctypes.c_int, [vp, ap, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -302,6 +332,32 @@ class Context:
         rc = load().frisk_b200_cache_attention(self.handle, cache, desc, q, out, mask, ws_ptr, ws_bytes, stream)
         raise_for(rc, self._h)
 
+    def cache_pages(self, which, cache, tables, parents, ws_ptr, ws_bytes, stream=None):
+        """``which``: ``PAGES_FORK``, ``PAGES_GROW`` or ``PAGES_COMPACT``."""
+        lib = load()
+        if which == PAGES_FORK:
+            rc = lib.frisk_b200_cache_fork(self.handle, cache, tables, parents, ws_ptr, ws_bytes, stream)
+        else:
+            call = lib.frisk_b200_cache_grow if which == PAGES_GROW else lib.frisk_b200_cache_compact
+            rc = call(self.handle, cache, tables, ws_ptr, ws_bytes, stream)
+        raise_for(rc, self._h)
+
+    def cache_copy(self, cache, into, source, target, count, stream=None):
+        raise_for(load().frisk_b200_cache_copy(self.handle, cache, into, source, target, count, stream), self._h)
+
+    def cache_keep(self, cache, kept, kept_stride, kept_width, counts, lengths_out, stream=None):
+        rc = load().frisk_b200_cache_keep(self.handle, cache, kept, kept_stride, kept_width, counts, lengths_out, stream)
+        raise_for(rc, self._h)
+
+    def draft_verify(self, desc, tokens, parents, starts, target, draft, accept, sample, kept, counts, token, stream=None):
+        rc = load().frisk_b200_draft_verify(self.handle, desc, tokens, parents, starts, target, draft, accept, sample, kept,
+                                            counts, token, stream)
+        raise_for(rc, self._h)
+
+    def adapter_gemm(self, desc, x, a, b, c, scales, starts, adapters, out, stream=None):
+        rc = load().frisk_b200_adapter_gemm(self.handle, desc, x, a, b, c, scales, starts, adapters, out, stream)
+        raise_for(rc, self._h)
+
     def check(self, stream=None):
         raise_for(load().frisk_b200_check(self.handle, stream), self._h)
 
@@ -329,6 +385,11 @@ def cache_attention_tile_rows(cache, desc):
     if rows < 0:
         raise_for(rows)
     return rows
+
+
+def cache_pages_workspace_bytes(cache, which):
+    """Bytes ``Context.cache_pages`` needs; 0 for what it refuses.  Host-only."""
+    return load().frisk_b200_cache_pages_workspace_bytes(cache, which)
 
 
 _PAIR = ctypes.c_int64 * 2

@@ -1,0 +1,510 @@
+// Low-rank adapters of many requests, added to a shared projection:
+//
+//   out[r] = c[r] + scale[w] * (x[r] A_w^T) B_w^T,   w: the adapter of row r's sequence, A_w [R, K], B_w [N, R]
+//
+// One launch.  A cluster has up to kRows rows of one sequence.  Its CTAs share K: each makes the products of its part of x and A, and the
+// parts are added up through distributed shared memory, in order, into all of the cluster's CTAs.  Then they share N: each multiplies the R sums of a row by its
+// part of B and adds c.  So nothing between the two products leaves the SMs, and no order of threads changes a result.
+//
+// Bound by memory for the ranks of adapters: an element of x, c or out takes R multiplications (R = 64 at 6.5 TB/s: 0.2 PFLOP/s).  So the products
+// are mma.sync's, operands go from memory to registers without a stop, and no tensor memory is set up.  For a few rows the adapters
+// themselves are what is read, each by a cluster of its own.
+//
+// Order of a product's inner index is free if both sides have the same, so a lane takes 16 bytes of it at once: of 32 neighbouring elements lane q of
+// four has 8 q .. 8 q + 7, which serve two steps of 16.  Columns of a result are permuted the same way: a lane ends up with 8 neighbours.
+//
+// Sums are 32-bit.  Before the second product they become sums of 16-bit terms: two, or three for bf16 whose result is 32-bit, so that less is lost
+// than in the rounding of the result (16 and 24 bits in bf16, 22 in fp16; fp16 terms stand at a power of two that brings a row's
+// largest to 2^14, so that sums beyond fp16's range keep their value).
+#include <algorithm>
+#include <type_traits>
+
+#include "cache_common.cuh"
+
+namespace fb {
+namespace {
+
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kMaxRank = 128;
+
+struct AdapterParams {
+  const void *x, *a, *b, *c;
+  void* out;
+  const float* scales;
+  const int *starts, *adapters;
+  int64_t ldx, lda, a_step, ldb, b_step, ldc, ldo, rows;
+  int K, N, R, count, batch;
+  int cluster;
+  bool wide;  // c and out on 16 bytes, row by row
+  unsigned* status;
+};
+
+template <typename T> struct Terms;  // the 16-bit types
+template <> struct Terms<__half> {
+  static __device__ __forceinline__ float value(uint16_t w) { return __half2float(__ushort_as_half(w)); }
+  static __device__ __forceinline__ uint16_t round(float x) { return __half_as_ushort(__float2half_rn(x)); }
+};
+template <> struct Terms<__nv_bfloat16> {
+  static __device__ __forceinline__ float value(uint16_t w) { return __uint_as_float((uint32_t)w << 16); }
+  static __device__ __forceinline__ uint16_t round(float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); }
+};
+
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// 8 elements from `at` on, of which the first `n` are there (others zero)
+__device__ __forceinline__ uint4 load8(const uint16_t* at, int n) {
+  if (n >= 8) return __ldg(reinterpret_cast<const uint4*>(at));
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) w[i >> 1] |= (uint32_t)__ldg(at + i) << (16 * (i & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint32_t word(const uint4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
+
+// c's 8 neighbours, and the result's
+template <typename C>
+__device__ __forceinline__ void load_c(float (&v)[8], const C* at, int n, bool wide) {
+  if (wide && n >= 8) {
+    uint4 w[sizeof(C) / 2];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(C) / 2; ++i) w[i] = *(reinterpret_cast<const uint4*>(at) + i);
+    if (sizeof(C) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(word(w[i >> 2 & (sizeof(C) / 2 - 1)], i & 3));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint16_t h = (uint16_t)(word(w[0], i >> 1) >> (16 * (i & 1)));
+        v[i] = Terms<typename std::conditional<sizeof(C) == 2, C, __half>::type>::value(h);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)at[i] : 0.f;
+  }
+}
+template <typename C>
+__device__ __forceinline__ void store_out(C* at, const float (&v)[8], int n, bool wide) {
+  if (wide && n >= 8) {
+    if (sizeof(C) == 4) {
+      reinterpret_cast<float4*>(at)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(at)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        using T = typename std::conditional<sizeof(C) == 2, C, __half>::type;
+        w[i] = Terms<T>::round(v[2 * i]) | (uint32_t)Terms<T>::round(v[2 * i + 1]) << 16;
+      }
+      *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) at[i] = (C)v[i];
+  }
+}
+
+// MW: groups of 16 rows a warp has; MWARPS: warps side by side over rows (the others share the inner index, then the columns)
+template <typename T, typename C, int RMAX, int MW, int MWARPS>
+struct Plan {
+  static constexpr int kRows = 16 * MW * MWARPS, kShare = kWarps / MWARPS;
+  static constexpr int kTiles = RMAX / 8, kBlocks = (RMAX + 31) / 32;
+  static constexpr int kTerms = sizeof(C) == 4 && std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
+  static constexpr int kPitch = RMAX + 8;  // of rows of sums, floats (lanes of a fragment meet no bank twice)
+  static constexpr size_t kSumBytes = (size_t)kShare * kRows * kPitch * 4;
+  static constexpr size_t kFullBytes = (size_t)kRows * kPitch * 4;
+  static constexpr size_t kTermBytes = (size_t)MW * MWARPS * kBlocks * 2 * kTerms * 32 * 16;
+  static constexpr size_t kFirstBytes = kSumBytes > kTermBytes ? kSumBytes : kTermBytes;  // (sums are done with where terms begin)
+  static constexpr size_t kBytes = kFirstBytes + kFullBytes + kRows * 4;
+};
+
+template <typename T, typename C, int RMAX, int MW, int MWARPS>
+__global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p) {
+  using P = Plan<T, C, RMAX, MW, MWARPS>;
+  extern __shared__ __align__(16) uint8_t memory[];
+  float* sums = reinterpret_cast<float*>(memory);                                   // [share][row][pitch]
+  uint4* terms = reinterpret_cast<uint4*>(memory);                                  // later: [16 rows][32 of R][half][term][lane]
+  float* full = reinterpret_cast<float*>(memory + P::kFirstBytes);                  // [row][pitch]
+  float* row_scale = reinterpret_cast<float*>(memory + P::kFirstBytes + P::kFullBytes);
+  __shared__ int tiles_of[kWarps], found[3];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+  const int C_ = p.cluster, rank = (int)cluster_ctarank(), tile = blockIdx.x / C_;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // The tile's sequence and rows: tiles are counted over the sequences, a thread each.
+  if (tid == 0) found[0] = -1;
+  int before = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
+    const int b = b0 + tid;
+    int lo = 0, n = 0;
+    if (b < p.batch) {
+      lo = p.starts[b];
+      const int64_t many = (int64_t)p.starts[b + 1] - lo;
+      if (lo < 0 || many < 0 || lo + many > p.rows) atomicCAS(p.status, 0u, cache::ST_CACHE_ROWS);
+      else n = (int)many;
+    }
+    const int mine = (n + P::kRows - 1) / P::kRows;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += other;
+    }
+    __syncthreads();
+    if (lane == 31) tiles_of[warp] = upto;
+    __syncthreads();
+    int at = before + upto - mine;
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) at += tiles_of[i];
+      before += tiles_of[i];
+    }
+    if (tile >= at && tile < at + mine) {
+      found[0] = b;
+      found[1] = lo + (tile - at) * P::kRows;
+      found[2] = min(P::kRows, n - (tile - at) * P::kRows);
+    }
+    if (before > tile) break;  // (the same in all threads)
+  }
+  __syncthreads();
+  if (found[0] < 0) return;  // (the whole cluster: there are fewer tiles than clusters)
+  const int64_t row0 = found[1];
+  const int rows = found[2];
+  int which = p.adapters[found[0]];
+  if (which >= p.count) {
+    if (tid == 0) atomicCAS(p.status, 0u, cache::ST_ADAPTER);
+    which = -1;
+  }
+  const C* c = static_cast<const C*>(p.c) + row0 * p.ldc;
+  C* out = static_cast<C*>(p.out) + row0 * p.ldo;
+  const int blocks_n = (p.N + 31) / 32, n0 = (int)((int64_t)blocks_n * rank / C_), n1 = (int)((int64_t)blocks_n * (rank + 1) / C_);
+  if (which < 0) {  // no adapter (the whole cluster)
+    if (p.out != p.c) {
+      const int pieces = (n1 - n0) * 4;
+      for (int i = tid; i < rows * pieces; i += kThreads) {
+        const int r = i / pieces, col = n0 * 32 + (i - r * pieces) * 8;
+        if (col >= p.N) continue;
+        float v[8];
+        load_c<C>(v, c + r * p.ldc + col, p.N - col, p.wide);
+        store_out<C>(out + r * p.ldo + col, v, p.N - col, p.wide);
+      }
+    }
+    return;
+  }
+  const uint16_t* x = static_cast<const uint16_t*>(p.x) + row0 * p.ldx;
+  const uint16_t* a = static_cast<const uint16_t*>(p.a) + which * p.a_step;
+  const uint16_t* bw = static_cast<const uint16_t*>(p.b) + which * p.b_step;
+  const int mw = warp % MWARPS, share = warp / MWARPS;  // the warp's rows; its part of the inner index, then of the columns
+  const int my_row = mw * 16 * MW;
+
+  // ---- x A^T over this CTA's part of K, shared by kShare warps in turns of 32
+  float acc[MW][P::kTiles][4];
+#pragma unroll
+  for (int m = 0; m < MW; ++m)
+#pragma unroll
+    for (int t = 0; t < P::kTiles; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[m][t][i] = 0.f;
+  const int blocks_k = (p.K + 31) / 32, k0 = (int)((int64_t)blocks_k * rank / C_), k1 = (int)((int64_t)blocks_k * (rank + 1) / C_);
+  if (my_row < rows) {
+#pragma unroll 2
+    for (int kb = k0 + share; kb < k1; kb += P::kShare) {
+      const int k = kb * 32 + q * 8, left = p.K - k;
+      uint4 xa[MW][2], w[P::kTiles];
+#pragma unroll
+      for (int m = 0; m < MW; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = my_row + 16 * m + 8 * h + g;
+          xa[m][h] = load8(x + r * p.ldx + k, r < rows ? left : 0);
+        }
+#pragma unroll
+      for (int t = 0; t < P::kTiles; ++t) w[t] = load8(a + (8 * t + g) * p.lda + k, 8 * t < p.R ? left : 0);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int m = 0; m < MW; ++m) {
+          const uint32_t fa[4] = {word(xa[m][0], 2 * s), word(xa[m][1], 2 * s), word(xa[m][0], 2 * s + 1), word(xa[m][1], 2 * s + 1)};
+#pragma unroll
+          for (int t = 0; t < P::kTiles; ++t) mma<T>(acc[m][t], fa, word(w[t], 2 * s), word(w[t], 2 * s + 1));
+        }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MW; ++m)
+#pragma unroll
+    for (int t = 0; t < P::kTiles; ++t) {
+      float* to = sums + (share * P::kRows + my_row + 16 * m + g) * P::kPitch + 8 * t + 2 * q;
+      *reinterpret_cast<float2*>(to) = make_float2(acc[m][t][0], acc[m][t][1]);
+      *reinterpret_cast<float2*>(to + 8 * P::kPitch) = make_float2(acc[m][t][2], acc[m][t][3]);
+    }
+  __syncthreads();
+  // ---- parts added up: the CTA's warps, then the CTAs, each in their order
+  const int quads = RMAX / 4, n_quads = rows * quads;
+  for (int i = tid; i < n_quads; i += kThreads) {
+    float* at = sums + i / quads * P::kPitch + i % quads * 4;
+    float4 s = *reinterpret_cast<const float4*>(at);
+#pragma unroll
+    for (int j = 1; j < P::kShare; ++j) {
+      const float4 o = *reinterpret_cast<const float4*>(at + j * P::kRows * P::kPitch);
+      s.x += o.x; s.y += o.y; s.z += o.z; s.w += o.w;
+    }
+    *reinterpret_cast<float4*>(at) = s;
+  }
+  cluster_sync_all();
+  for (int i = rank * kThreads + tid; i < n_quads; i += C_ * kThreads) {
+    const int offset = i / quads * P::kPitch + i % quads * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r = 0; r < C_; ++r) {
+      const float4 o = ld_cluster_f4(mapa_addr(smem_u32(sums + offset), r));
+      s.x += o.x; s.y += o.y; s.z += o.z; s.w += o.w;
+    }
+    for (int r = 0; r < C_; ++r) st_cluster_f4(mapa_addr(smem_u32(full + offset), r), s);
+  }
+  cluster_sync_all();  // (from here on no CTA reads or writes another's memory)
+  // ---- as terms, in the order in which the second product takes them
+  if (std::is_same<T, __half>::value) {
+    for (int r = warp; r < rows; r += kWarps) {
+      float most = 0.f;
+      for (int i = lane; i < RMAX; i += 32) most = fmaxf(most, fabsf(full[r * P::kPitch + i]));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      // most = 1.m * 2^(e - 127): times 2^(14 - (e - 127)).  (Infinities stay; a row of zeros or subnormals stands at 2^126.)
+      const int e = (int)(__float_as_uint(most) >> 23);
+      if (lane == 0) row_scale[r] = e == 255 ? 1.f : __uint_as_float((uint32_t)min(254, 268 - max(e, 15)) << 23);
+    }
+    __syncthreads();
+  }
+  for (int i = warp; i < MW * MWARPS * P::kBlocks * 2; i += kWarps) {
+    const int s = i & 1, kb = (i >> 1) % P::kBlocks, m = (i >> 1) / P::kBlocks;
+    if (16 * m >= rows) continue;
+    uint32_t f[P::kTerms][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = 16 * m + g + 8 * (j & 1), k = 32 * kb + 8 * q + 4 * s + 2 * (j >> 1);
+      float v[2] = {0.f, 0.f};
+      if (r < rows && k < p.R) {
+        const float2 two = *reinterpret_cast<const float2*>(full + r * P::kPitch + k);
+        const float up = std::is_same<T, __half>::value ? row_scale[r] : 1.f;
+        v[0] = two.x * up;
+        v[1] = two.y * up;
+      }
+#pragma unroll
+      for (int t = 0; t < P::kTerms; ++t) {
+        uint32_t both = 0;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const uint16_t h = Terms<T>::round(v[n]);
+          const float back = Terms<T>::value(h);
+          both |= (uint32_t)h << (16 * n);
+          v[n] = isfinite(back) ? v[n] - back : 0.f;  // (exact)
+        }
+        f[t][j] = both;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < P::kTerms; ++t) terms[(i * P::kTerms + t) * 32 + lane] = make_uint4(f[t][0], f[t][1], f[t][2], f[t][3]);
+  }
+  __syncthreads();
+  // ---- times B^T, 32 columns a step
+  if (my_row >= rows) return;
+  const float alpha = p.scales ? p.scales[which] : 1.f;
+  float up[MW][2];
+#pragma unroll
+  for (int m = 0; m < MW; ++m)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = my_row + 16 * m + 8 * h + g;
+      up[m][h] = std::is_same<T, __half>::value && r < rows ? 1.f / row_scale[r] : 1.f;  // (of a power of two: exact)
+    }
+  const int first = 8 * (g >> 1) + (g & 1);  // of the rows of B that this lane's columns of the four tiles are: first + 2 j
+  for (int nb = n0 + share; nb < n1; nb += P::kShare) {
+    const int col = nb * 32 + 8 * q, left = p.N - col;
+    float y[MW][2][8];
+#pragma unroll
+    for (int m = 0; m < MW; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = my_row + 16 * m + 8 * h + g;
+        load_c<C>(y[m][h], c + r * p.ldc + col, r < rows ? left : 0, p.wide);
+      }
+    float d[MW][4][4];
+#pragma unroll
+    for (int m = 0; m < MW; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[m][j][i] = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < P::kBlocks; ++kb) {
+      uint4 w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = nb * 32 + first + 2 * j, k = 32 * kb + 8 * q;
+        w[j] = load8(bw + (int64_t)n * p.ldb + k, n < p.N ? p.R - k : 0);
+      }
+#pragma unroll
+      for (int m = 0; m < MW; ++m)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int t = 0; t < P::kTerms; ++t) {
+            const uint4 f = terms[((((my_row / 16 + m) * P::kBlocks + kb) * 2 + s) * P::kTerms + t) * 32 + lane];
+            const uint32_t fa[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma<T>(d[m][j], fa, word(w[j], 2 * s), word(w[j], 2 * s + 1));
+          }
+    }
+#pragma unroll
+    for (int m = 0; m < MW; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = my_row + 16 * m + 8 * h + g;
+        if (r >= rows) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          y[m][h][2 * j] = fmaf(alpha, d[m][j][2 * h] * up[m][h], y[m][h][2 * j]);
+          y[m][h][2 * j + 1] = fmaf(alpha, d[m][j][2 * h + 1] * up[m][h], y[m][h][2 * j + 1]);
+        }
+        store_out<C>(out + r * p.ldo + col, y[m][h], left, p.wide);
+      }
+  }
+}
+
+template <typename T, typename C, int RMAX, int MW, int MWARPS>
+cudaError_t launch(frisk_b200_ctx* ctx, AdapterParams p, cudaStream_t s) {
+  using P = Plan<T, C, RMAX, MW, MWARPS>;
+  auto kernel = adapter_kernel<T, C, RMAX, MW, MWARPS>;
+  static PerDeviceOnce once;
+  cudaError_t e = cudaSuccess;
+  once(ctx->device, [&] {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kBytes);
+    return e == cudaSuccess ? 0 : 1;
+  });
+  if (e != cudaSuccess) return e;
+  // (at most: every sequence may end with a tile that is not full)
+  const int64_t tiles = std::min<int64_t>(p.rows, p.rows / P::kRows + p.batch);
+  p.cluster = kMaxCluster;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel waits (griddepcontrol.wait) itself
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(tiles * p.cluster));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = P::kBytes;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <typename T, typename C, int RMAX>
+cudaError_t launch_rows(frisk_b200_ctx* ctx, const AdapterParams& p, cudaStream_t s) {
+  const int64_t mean = (p.rows + p.batch - 1) / p.batch;  // rows of a sequence
+  if (mean <= 16) return launch<T, C, RMAX, 1, 1>(ctx, p, s);
+  if (mean <= 48) return launch<T, C, RMAX, 2, 1>(ctx, p, s);
+  return launch<T, C, RMAX, 2, RMAX <= 64 ? 4 : 2>(ctx, p, s);
+}
+template <typename T, typename C>
+cudaError_t launch_rank(frisk_b200_ctx* ctx, const AdapterParams& p, cudaStream_t s) {
+  if (p.R <= 16) return launch_rows<T, C, 16>(ctx, p, s);
+  if (p.R <= 32) return launch_rows<T, C, 32>(ctx, p, s);
+  if (p.R <= 64) return launch_rows<T, C, 64>(ctx, p, s);
+  return launch_rows<T, C, 128>(ctx, p, s);
+}
+
+}  // namespace
+}  // namespace fb
+
+using namespace fb;
+
+extern "C" int frisk_b200_adapter_gemm(frisk_b200_ctx* ctx, const frisk_b200_adapter_desc* d, const void* x, const void* a, const void* b, const void* c,
+                                       const float* scales, const int32_t* starts, const int32_t* adapters, void* out, void* stream) {
+  if (!ctx || !d) return FRISK_B200_E_ARG;
+  if (d->dtype != FRISK_B200_F16 && d->dtype != FRISK_B200_BF16) return FRISK_B200_E_CACHE_TYPE;
+  if (d->dtype_c != d->dtype && d->dtype_c != FRISK_B200_F32) return FRISK_B200_E_CACHE_TYPE;
+  if (d->rows < 0 || d->rows > INT32_MAX || d->batch < 0 || d->count < 0 || d->K < 1 || d->N < 1 || d->K > INT32_MAX - 64 || d->N > INT32_MAX - 64 || d->rank < 8 ||
+      d->rank > kMaxRank || d->rank % 8)
+    return FRISK_B200_E_CACHE_SHAPE;
+  if (d->rows == 0 || d->batch == 0) return 0;
+  if ((std::min<int64_t>(d->rows, d->rows / 16 + d->batch)) * kMaxCluster > INT32_MAX) return FRISK_B200_E_TOO_LARGE;
+  if (!x || !c || !out || !starts || !adapters || (d->count > 0 && (!a || !b))) return FRISK_B200_E_ARG;
+  const int64_t rows = d->rows;
+  if ((rows > 1 && (d->ldx < d->K || d->ldc < d->N || d->ldo < d->N)) || d->lda < d->K || d->ldb < d->rank || (d->count > 1 && (d->a_step < 0 || d->b_step < 0)))
+    return FRISK_B200_E_CACHE_SHAPE;
+  const size_t es = 2, cs = dtype_size(d->dtype_c);
+  if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15u) || (rows > 1 && d->ldx % 8) || d->lda % 8 || d->ldb % 8 ||
+      (d->count > 1 && (d->a_step % 8 || d->b_step % 8)))
+    return FRISK_B200_E_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(c) | reinterpret_cast<uintptr_t>(out)) % cs ||
+      ((reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(starts) | reinterpret_cast<uintptr_t>(adapters)) & 3u))
+    return FRISK_B200_E_ALIGN;
+  // out apart from everything but a c in its own place; x, c and out may be columns of one buffer
+  auto bytes = [](const void* p, int64_t ld, size_t e) { return frisk_b200_packed{const_cast<void*>(p), ld * (int64_t)e, 0}; };
+  const frisk_b200_packed po = bytes(out, d->ldo, cs);
+  auto apart = [&](const frisk_b200_packed& y, int64_t width) {
+    // (as rows of bytes of one width: the wider of the two would do, but ends apart are told by their own)
+    const uintptr_t o0 = reinterpret_cast<uintptr_t>(po.ptr), o1 = o0 + (rows - 1) * po.row_stride + d->N * cs, y0 = reinterpret_cast<uintptr_t>(y.ptr),
+                    y1 = y0 + (rows - 1) * y.row_stride + width;
+    if (o1 <= y0 || y1 <= o0) return true;
+    if (rows == 1 || po.row_stride != y.row_stride) return false;
+    const int64_t m = po.row_stride, at = ((int64_t)(y0 - o0) % m + m) % m;  // where y's columns begin in out's rows
+    return at >= (int64_t)(d->N * cs) && at + width <= m;
+  };
+  const bool in_place = out == c && (rows == 1 || d->ldo == d->ldc);
+  if (!in_place && !apart(bytes(c, d->ldc, cs), d->N * cs)) return FRISK_B200_E_OVERLAP;
+  if (!apart(bytes(x, d->ldx, es), d->K * es)) return FRISK_B200_E_OVERLAP;
+  const size_t out_bytes = (size_t)((rows - 1) * d->ldo + d->N) * cs;
+  auto weights = [&](int64_t step, int64_t ld, int64_t n, int64_t width) { return d->count ? (size_t)((d->count - 1) * step + (n - 1) * ld + width) * es : 0; };
+  const size_t a_bytes = weights(d->a_step, d->lda, d->rank, d->K), b_bytes = weights(d->b_step, d->ldb, d->N, d->rank);
+  if ((a_bytes && ranges_overlap(out, out_bytes, a, a_bytes)) || (b_bytes && ranges_overlap(out, out_bytes, b, b_bytes)) ||
+      (scales && d->count && ranges_overlap(out, out_bytes, scales, (size_t)d->count * 4)) || ranges_overlap(out, out_bytes, starts, ((size_t)d->batch + 1) * 4) ||
+      ranges_overlap(out, out_bytes, adapters, (size_t)d->batch * 4))
+    return FRISK_B200_E_OVERLAP;
+  AdapterParams p{};
+  p.x = x;
+  p.a = a;
+  p.b = b;
+  p.c = c;
+  p.out = out;
+  p.scales = scales;
+  p.starts = starts;
+  p.adapters = adapters;
+  p.ldx = d->ldx;
+  p.lda = d->lda;
+  p.a_step = d->a_step;
+  p.ldb = d->ldb;
+  p.b_step = d->b_step;
+  p.ldc = d->ldc;
+  p.ldo = d->ldo;
+  p.rows = rows;
+  p.K = (int)d->K;
+  p.N = (int)d->N;
+  p.R = d->rank;
+  p.count = d->count;
+  p.batch = d->batch;
+  p.wide = ((reinterpret_cast<uintptr_t>(c) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0 && (rows == 1 || (d->ldc | d->ldo) * (int64_t)cs % 16 == 0);
+  p.status = ctx->d_status;
+  FB_DEVICE(ctx);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool f32 = d->dtype_c == FRISK_B200_F32;
+  FB_CUDA(ctx, d->dtype == FRISK_B200_F16 ? (f32 ? launch_rank<__half, float>(ctx, p, s) : launch_rank<__half, __half>(ctx, p, s))
+                                          : (f32 ? launch_rank<__nv_bfloat16, float>(ctx, p, s) : launch_rank<__nv_bfloat16, __nv_bfloat16>(ctx, p, s)));
+  return 0;
+}

@@ -280,9 +280,9 @@ const char* frisk_b200_strerror(int code) {
     case FRISK_B200_E_UNSUPPORTED: return "no kernel for this element type / layout / algorithm";
     case FRISK_B200_E_ARG: return "invalid argument";
     case FRISK_B200_E_ATTN_SHAPE: return "shape outside the attention launch contract";
-    case FRISK_B200_E_CACHE_SHAPE: return "sizes or strides outside the contract of the rotary and cache operators";
-    case FRISK_B200_E_CACHE_TYPE: return "element types outside the contract of the rotary and cache operators";
-    case FRISK_B200_E_DEVICE_TABLE: return "a table of the cache named rows, a length or a page out of range";
+    case FRISK_B200_E_CACHE_SHAPE: return "sizes or strides outside the contract of the rotary, cache, draft and adapter operators";
+    case FRISK_B200_E_CACHE_TYPE: return "element types outside the contract of the rotary, cache, draft and adapter operators";
+    case FRISK_B200_E_DEVICE_TABLE: return "a table on the device named rows, a length, a page or an adapter out of range";
     case FRISK_B200_E_TOO_LARGE: return "problem exceeds the fixed capacity of this entry point";
     case FRISK_B200_E_DEVICE_TIMEOUT: return "a bounded device-side wait ran out";
     case FRISK_B200_E_CUDA: return "CUDA call failed";
@@ -367,8 +367,9 @@ int frisk_b200_check(frisk_b200_ctx* ctx, void* stream) {
   if (ctx->last_status != 0) {
     cudaMemsetAsync(ctx->d_status, 0, sizeof(unsigned), s);
     cudaStreamSynchronize(s);
-    // (0x301-0x303: cache_common.cuh)
-    return ctx->last_status >= 0x301 && ctx->last_status <= 0x303 ? FRISK_B200_E_DEVICE_TABLE : FRISK_B200_E_DEVICE_TIMEOUT;
+    // (0x301-0x303, 0x310: cache_common.cuh)
+    const bool table = (ctx->last_status >= 0x301 && ctx->last_status <= 0x303) || ctx->last_status == 0x310;
+    return table ? FRISK_B200_E_DEVICE_TABLE : FRISK_B200_E_DEVICE_TIMEOUT;
   }
   return 0;
 }

@@ -23,6 +23,7 @@ enum : unsigned {
   ST_CACHE_PAGE = 0x303,    // a page outside the cache
   ST_CACHE_KV = 0x304,      // (a wait) key tiles
   ST_CACHE_S = 0x305, ST_CACHE_P = 0x306, ST_CACHE_O = 0x307, ST_CACHE_Q = 0x309,
+  ST_ADAPTER = 0x310,  // an adapter out of range
 };
 
 struct Tables {

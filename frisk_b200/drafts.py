@@ -1,0 +1,65 @@
+"""Verification of drafted tokens: ``draft_verify``."""
+from . import capi
+from .cache import _on_stream, _stream_of
+from .execute import _torch, context_for
+
+
+def _refuse(what):
+    raise ValueError("frisk-b200-draft: " + what)
+
+
+def _list(t, n, kinds, dev, what):
+    if t.dtype not in kinds or t.shape != (n,) or t.get_device() != dev or not t.is_contiguous():
+        _refuse(f"{what} must be dense, {' or '.join(str(k)[6:] for k in kinds)} [{n}], on the probabilities' device")
+    return t.data_ptr()
+
+
+def draft_verify(tokens, parents, starts, target, draft, accept, sample, *, max_new, stream=None):
+    """Which drafted tokens stand, and the token behind them: (kept int32 [batch, max_new], counts int32 [batch], next [batch] in the
+    tokens' type).
+
+    Sequence b's rows ``starts[b]`` .. ``starts[b + 1] - 1`` are the nodes of a tree, as ``cache_attention`` scores them with a mask: node 0 the
+    token sampled last, node i > 0 a drafted token behind node ``parents[row]`` < i (``parents`` None: behind node i - 1).  ``target`` [rows, vocabulary]
+    holds the target's probabilities of the token behind each row, ``draft`` those that the children of each row were drawn from independently, or None
+    where they were picked otherwise (looked up, or the most likely ones): float32, float16 or bfloat16, rows of any pitch.
+
+    From node 0 on, the children of a node are tried in their order: a child stands if its random number ``accept[row]`` (float32, in [0, 1)) is
+    below the target's probability of it over the draft's; otherwise the draft's distribution is taken off the target's for the next child.
+    Where none is left, the next token is drawn with ``sample[b]`` from what is left: the first whose running sum passes it.  So tokens are
+    distributed as the target's, whatever the draft.  Sums have 64 bits.  A distribution that is 1 at one token verifies greedily.
+
+    ``kept[b, :counts[b]]`` are the nodes that stand, node 0 first, -1 behind them: what ``cache_keep`` takes.  A sequence without rows has count 0
+    and next -1, as one with more than ``max_new`` (1 to 1024) rows or rows out of range, for which ``cache_check`` raises.  Probabilities that are NaN or
+    negative count as 0."""
+    torch = _torch()
+    code = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}.get(target.dtype)
+    shape, dev = target.shape, target.get_device()
+    if code is None or len(shape) != 2 or (target.stride(1) != 1 and shape[1] > 1):
+        _refuse("target must be float32, float16 or bfloat16 [rows, vocabulary] with dense rows")
+    if dev < 0:
+        _refuse("tensors must be on one CUDA device (there is no CPU path)")
+    if draft is not None and (draft.dtype != target.dtype or draft.shape != shape or draft.get_device() != dev or (draft.stride(1) != 1 and shape[1] > 1)):
+        _refuse("draft must have the type, shape and device of target, and dense rows")
+    rows, vocab = shape
+    batch = starts.shape[0] - 1 if starts.dim() == 1 else -1
+    if batch < 0:
+        _refuse("starts must be int32 [batch + 1]")
+    p_tokens = _list(tokens, rows, (torch.int64, torch.int32), dev, "tokens")
+    p_parents = None if parents is None else _list(parents, rows, (torch.int32,), dev, "parents")
+    p_starts = _list(starts, batch + 1, (torch.int32,), dev, "starts")
+    p_accept, p_sample = _list(accept, rows, (torch.float32,), dev, "accept"), _list(sample, batch, (torch.float32,), dev, "sample")
+    if not 1 <= max_new <= 1024:
+        _refuse("max_new must be between 1 and 1024")
+
+    def new():
+        return starts.new_empty((batch, max_new)), starts.new_empty(batch), tokens.new_empty(batch)
+
+    if stream is None:
+        kept, counts, token = new()
+    else:
+        with _on_stream(stream, target.device):
+            kept, counts, token = new()
+    desc = capi.VerifyDesc(rows, target.stride(0), 0 if draft is None else draft.stride(0), batch, max_new, vocab, code, tokens.dtype == torch.int64)
+    context_for(dev).draft_verify(desc, p_tokens, p_parents, p_starts, target.data_ptr(), None if draft is None else draft.data_ptr(), p_accept, p_sample,
+                                  kept.data_ptr(), counts.data_ptr(), token.data_ptr(), _stream_of(stream, dev))
+    return kept, counts, token

@@ -64,11 +64,11 @@ enum {
   FRISK_B200_E_ARG = -7,           /* null pointer, bad enum, bad context                   */
   FRISK_B200_E_ATTN_SHAPE = -8,    /* attention shape outside the launch contract           */
   FRISK_B200_E_TOO_LARGE = -9,     /* exceeds the fixed capacity of a no-allocation entry   */
-  FRISK_B200_E_CACHE_SHAPE = -10,  /* sizes or strides outside the contract of the rotary and cache entries */
+  FRISK_B200_E_CACHE_SHAPE = -10,  /* sizes or strides outside the contract of the rotary, cache, draft and adapter entries */
   FRISK_B200_E_CACHE_TYPE = -11,   /* element types outside it                              */
   FRISK_B200_E_DEVICE_TIMEOUT = 1, /* a bounded device-side wait ran out (status word set)  */
   FRISK_B200_E_CUDA = 2,           /* a CUDA runtime/driver call failed (see last_cuda)     */
-  FRISK_B200_E_DEVICE_TABLE = 3    /* a table of the cache named rows, a length or a page out of range (status word 0x301-0x303) */
+  FRISK_B200_E_DEVICE_TABLE = 3    /* a table named rows, a length, a page (status word 0x301-0x303) or an adapter (0x310) out of range */
 };
 
 /*
@@ -361,6 +361,81 @@ size_t frisk_b200_cache_attention_workspace_bytes(const frisk_b200_cache_desc* c
 int frisk_b200_cache_attention(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* cache, const frisk_b200_cache_attn_desc* desc,
                                const frisk_b200_packed* q, const frisk_b200_packed* out, const uint8_t* mask,
                                void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- pages of a cache that sequences share ---------------------------------------------------
+ * users[p] is the number of table entries that name page p of the cache, 0 where it is free (a caller that holds a page
+ * otherwise adds to it).  A table entry below 0 names no page.  Results go to users_out, table_out and lengths_out, which may be
+ * users, the cache's table (with its stride) and lengths themselves; else they overlap nothing.  Everything is on the device, and
+ * results follow from the tables' contents alone.  What is out of range there is left out, and frisk_b200_check returns
+ * FRISK_B200_E_DEVICE_TABLE.  The workspace (4-byte aligned, contents of no matter) must not be shared by calls that may overlap.
+ * fork: row b of the table becomes what row parents[b] was (b itself: stays; -1: no pages, length 0), without entries behind
+ *   the last key; users follow.  Uses batch, table and lengths of the cache descriptor; lengths_out: the new lengths.
+ * grow: gives sequence b pages for the starts[b + 1] - starts[b] keys behind its lengths[b].  Pages are taken lowest first, by
+ *   sequences in their order.  A page that would be written and that others have too is replaced by one of its own, into which the
+ *   keys that are in it are copied; of several sequences of the call that have it, the last one keeps it if no one else does.
+ *   A sequence gets all or nothing, and from the first that lacks pages on only those that need none get theirs.
+ *   lengths_out: the new keys that have a place now, [batch] (0 where there was none).
+ * compact: moves the used pages to the lowest indices: the k-th used page behind the first n, n their number, becomes the k-th
+ *   free one among them.  lengths_out: n, [1].  starts and lengths are not used. */
+enum { FRISK_B200_PAGES_FORK = 0, FRISK_B200_PAGES_GROW = 1, FRISK_B200_PAGES_COMPACT = 2 };
+typedef struct frisk_b200_page_tables {
+  const int32_t* users;
+  int32_t *users_out, *table_out, *lengths_out;
+  int64_t table_out_stride;
+} frisk_b200_page_tables;
+/* Bytes of workspace for one of the three (FRISK_B200_PAGES_*); 0 for what it refuses.  Host-only. */
+size_t frisk_b200_cache_pages_workspace_bytes(const frisk_b200_cache_desc* cache, int32_t which);
+int frisk_b200_cache_fork(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* cache, const frisk_b200_page_tables* tables,
+                          const int32_t* parents, void* workspace, size_t workspace_bytes, void* stream);
+int frisk_b200_cache_grow(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* cache, const frisk_b200_page_tables* tables,
+                          void* workspace, size_t workspace_bytes, void* stream);
+int frisk_b200_cache_compact(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* cache, const frisk_b200_page_tables* tables,
+                             void* workspace, size_t workspace_bytes, void* stream);
+/* Copies page source[i] of `from` to page target[i] of `into` (the same cache or another of the same heads, page, D and type),
+ * i < count; both lists are on the device.  A page must not be target twice, nor, in one cache, source and target. */
+int frisk_b200_cache_copy(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* from, const frisk_b200_cache_desc* into,
+                          const int32_t* source, const int32_t* target, int64_t count, void* stream);
+/* Of the new keys of sequence b (packed rows, in the cache behind its lengths[b] keys) keeps counts[b]: the key at
+ * lengths[b] + kept[b * kept_stride + i] moves to lengths[b] + i.  kept ascends within a sequence.  lengths_out (it may be
+ * lengths): lengths[b] + counts[b].  A sequence whose kept or counts are out of range stays as it is. */
+int frisk_b200_cache_keep(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* cache, const int32_t* kept, int64_t kept_stride,
+                          int32_t kept_width, const int32_t* counts, int32_t* lengths_out, void* stream);
+
+/* ---- verification of drafted tokens ----------------------------------------------------------
+ * A sequence's packed rows starts[b] .. starts[b + 1] - 1 are the nodes of a tree: node 0 the token sampled last, node i > 0 a drafted
+ * token that follows node parents[starts[b] + i] < i (parents == NULL: i - 1).  target: [rows, vocab] probabilities of the token
+ * behind each row; draft: those that the children of each row were drawn from independently, or NULL where they were not drawn (picked by rank, or
+ * looked up).  From node 0 on, a node's children x are tried in their order, with weights w = target[node] and a mass S = 1: x stands
+ * where w(x) > 0 and accept[x's row] * S * draft[node](x) < w(x) (draft NULL: its probability is 1), and the walk goes on from there;
+ * else w <- max(w - S * draft[node], 0) and S <- sum of w (draft NULL: w(x) <- 0 and S <- max(S - w(x), 0)).  Where no child is left,
+ * next[b] is the first token whose running sum of w passes sample[b] times the sum of w; if nothing is left of w, of target[node];
+ * -1 if that is empty too.  kept[b * max_new ..]: the nodes that stand, node 0 first, -1 behind them; counts[b]: how many.  64-bit sums.
+ * F32, F16 or BF16 rows of any alignment; probabilities that are NaN or negative count as 0.  tokens and next are int32 or
+ * int64; a token outside the vocabulary does not stand.  A sequence without rows has count 0 and next -1; so has one with more
+ * than max_new (1 to 1024) or rows out of range, and frisk_b200_check returns FRISK_B200_E_DEVICE_TABLE. */
+typedef struct frisk_b200_verify_desc {
+  int64_t rows, target_stride, draft_stride;
+  int32_t batch, max_new, vocab, dtype, tokens64;
+} frisk_b200_verify_desc;
+int frisk_b200_draft_verify(frisk_b200_ctx* ctx, const frisk_b200_verify_desc* desc, const void* tokens, const int32_t* parents,
+                            const int32_t* starts, const void* target, const void* draft, const float* accept,
+                            const float* sample, int32_t* kept, int32_t* counts, void* next, void* stream);
+
+/* ---- low-rank adapters of many requests ------------------------------------------------------
+ * out[r] = c[r] + scales[w] * (x[r] . a[w]^T) . b[w]^T for the packed rows r of sequence s, w = adapters[s] (below 0: none, out[r] = c[r]).
+ * x [rows, K], a [count, rank, K], b [count, N, rank] of dtype (F16 or BF16), rows on 16 bytes; rank a multiple of 8 up to 128.
+ * c and out [rows, N] of dtype_c (dtype or F32), any row pitch and alignment; out may be c, else overlaps nothing (x, c and out
+ * may be columns of one buffer of rows).  scales: [count] floats or NULL (1).  32-bit sums, one rounding.  starts, adapters and scales are on
+ * the device.  Rows of no sequence are left as they are; an adapter out of range counts as none, and frisk_b200_check returns
+ * FRISK_B200_E_DEVICE_TABLE. */
+typedef struct frisk_b200_adapter_desc {
+  int64_t rows, K, N;
+  int64_t ldx, lda, a_step, ldb, b_step, ldc, ldo; /* row pitches and steps from one adapter to the next, in elements */
+  int32_t rank, count, batch, dtype, dtype_c;
+} frisk_b200_adapter_desc;
+int frisk_b200_adapter_gemm(frisk_b200_ctx* ctx, const frisk_b200_adapter_desc* desc, const void* x, const void* a, const void* b,
+                            const void* c, const float* scales, const int32_t* starts, const int32_t* adapters, void* out,
+                            void* stream);
 
 /* Checks the device status word after the stream has drained (synchronises `stream`).
  * Returns 0, FRISK_B200_E_DEVICE_TIMEOUT, FRISK_B200_E_DEVICE_TABLE or FRISK_B200_E_CUDA. */
