@@ -13,10 +13,10 @@
 //
 // All in 64 bits: in 32 the sums over 10^5 tokens would move borders between tokens by more than many tokens have.
 //
-// A cluster of eight CTAs has a sequence, its CTAs neighbouring parts of the vocabulary, their warps neighbouring parts of those.  A tested child
-// costs two single values, fetched for all nodes at once; whole rows are read only for a rejection (with a draft) and for the last sum.
-// The sums of a part stay in shared memory, so the token is found by descending: CTA, warp, 256 values, lane.  Bound by
-// HBM where there are many sequences, else by the chain starts -> tokens -> values -> row -> exchange of sums.
+// A cluster of up to eight CTAs has a sequence, its warps neighbouring parts of the vocabulary.  A tested child costs two single values, fetched for
+// all nodes at once; whole rows are read only for a rejection (with a draft) and for the last sum, and come out of the L2 when the node's next child is
+// rejected.  The parts' sums go to all CTAs, so that each decides by itself, and the token is found by descending: the warp's part, an eighth of it,
+// 256 values, a lane.  Bound by HBM where there are many sequences, else by the chain starts -> tokens -> values -> row -> sums -> row.
 #include <cfloat>
 
 #include "cache_common.cuh"
@@ -24,8 +24,9 @@
 namespace fb {
 namespace {
 
-constexpr int kCluster = 8;
-constexpr int kWarps = 16, kThreads = 32 * kWarps;
+constexpr int kMostCtas = 8;  // of a cluster
+constexpr int kWarps = 8, kThreads = 32 * kWarps, kMostParts = kMostCtas * kWarps;
+constexpr int kAhead = 4;  // steps a warp has in flight
 constexpr int kLane = 8, kStep = 32 * kLane;  // values a lane and a warp look at in a step
 constexpr int kMaxNodes = 1024;
 
@@ -38,7 +39,7 @@ struct VerifyParams {
   int *kept, *counts;
   void* next;
   int64_t rows;
-  int tokens64, max_new, vocab;
+  int tokens64, max_new, vocab, ctas;
   unsigned* status;
 };
 
@@ -50,20 +51,30 @@ template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat
 // what a probability weighs: NaN and what is below zero nothing, an infinity the largest finite value
 __device__ __forceinline__ float weight(float x) { return fminf(fmaxf(x, 0.f), FLT_MAX); }
 
-// kLane values from `at` on, of which the first `n` are there
+// kLane values of a row, as they are
 template <typename T>
-__device__ __forceinline__ void load_lane(float (&x)[kLane], const T* at, int n) {
-  if (n >= kLane && (reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
-    uint4 w[sizeof(T) / 2];
+struct Values {
+  uint4 w[sizeof(T) / 2];
+  // from an address on 16 bytes
+  __device__ __forceinline__ void load(const T* at) {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
-    const T* v = reinterpret_cast<const T*>(w);
-#pragma unroll
-    for (int i = 0; i < kLane; ++i) x[i] = weight(to_float<T>(v[i]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < kLane; ++i) x[i] = i < n ? weight(to_float<T>(at[i])) : 0.f;
   }
+  // from index `at` of a row of n on: those before and behind the row are zero
+  __device__ __forceinline__ void load_any(const T* row, int at, int n) {
+    T v[kLane];
+#pragma unroll
+    for (int i = 0; i < kLane; ++i) v[i] = at + i >= 0 && at + i < n ? row[at + i] : T(0.f);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(v)[i];
+  }
+  __device__ __forceinline__ float operator[](int i) const { return weight(to_float<T>(reinterpret_cast<const T*>(w)[i])); }
+};
+
+// what is left of a weight w
+__device__ __forceinline__ double less(double w, double mass, double q) {
+  const double x = __dsub_rn(w, __dmul_rn(mass, q));
+  return x > 0.0 ? x : 0.0;
 }
 
 __device__ __forceinline__ void st_cluster_f64(uint32_t addr, double x) { asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(x) : "memory"); }
@@ -75,18 +86,18 @@ __device__ __forceinline__ double warp_sum(double x) {
 }
 
 template <typename T, bool DRAFT>
-__global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster, 1, 1) verify_kernel(const VerifyParams p) {
-  extern __shared__ int nodes[];  // of every node: token, parent, weight there, the draft's, random number; masses or tokens taken off
-  __shared__ double warp_sums[kWarps], cta_sums[2][kCluster];
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams p) {
+  extern __shared__ int nodes[];  // of every node: token, parent, weight there, the draft's, random number; then masses or tokens taken off
+  __shared__ double part_sums[2][kMostParts], eighths[kWarps];
   __shared__ int n_off;
   int *token = nodes, *parent = token + p.max_new;
   float *at_target = reinterpret_cast<float*>(parent + p.max_new), *at_draft = at_target + p.max_new, *random = at_draft + p.max_new;
   // (doubles: behind five arrays of 32 bits, rounded up)
-  double* masses = reinterpret_cast<double*>(nodes + (5 * p.max_new + 1) / 2 * 2);
+  double* masses = reinterpret_cast<double*>(nodes + (5 * p.max_new + 1) / 2 * 2);  // two sets, of one node with rejections and the next
   int* off = reinterpret_cast<int*>(masses);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.x / kCluster;
-  const uint32_t rank = cluster_ctarank();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.x / p.ctas;
+  const int rank = (int)cluster_ctarank();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int first = p.starts[b], last = p.starts[b + 1];
@@ -120,66 +131,96 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster, 1, 1) ver
   }
   cluster_sync_all();  // (and no CTA is written to before it runs)
 
-  // this warp's part of the vocabulary: steps [step0, step1)
-  const int steps = (p.vocab + kStep - 1) / kStep, each = (steps + kCluster * kWarps - 1) / (kCluster * kWarps);
-  const int step0 = min(steps, ((int)rank * kWarps + warp) * each), step1 = min(steps, step0 + each);
-
+  // Steps are cut where the row's addresses are multiples of 16, so a row may begin up to kLane - 1 values into the first.
+  const int steps = (p.vocab + kLane - 1 + kStep - 1) / kStep, parts = p.ctas * kWarps, each = (steps + parts - 1) / parts;
   int node = 0, taken_off = 0;  // distributions taken off, at this node
-  // the kLane weights of step s that are this lane's
-  auto weights = [&](double (&w)[kLane], int s) {
-    const int at = s * kStep + lane * kLane;
-    float x[kLane];
-    load_lane<T>(x, target + node * p.target_stride + at, p.vocab - at);
+  double* mine_off = masses;
+  // the weights of a step, of the values x and q
+  auto weights = [&](double (&w)[kLane], const Values<T>& x, const Values<T>& q, int at) {
+#pragma unroll
+    for (int i = 0; i < kLane; ++i) w[i] = x[i];
     if (DRAFT) {
-      float q[kLane];
-      if (taken_off) load_lane<T>(q, draft + node * p.draft_stride + at, p.vocab - at);
+      if (taken_off == 0) return;
+      double d[kLane];
 #pragma unroll
-      for (int i = 0; i < kLane; ++i) w[i] = x[i];
+      for (int i = 0; i < kLane; ++i) d[i] = q[i];
+#pragma unroll 1
       for (int j = 0; j < taken_off; ++j) {
-        const double mass = masses[j];
+        const double mass = mine_off[j];
 #pragma unroll
-        for (int i = 0; i < kLane; ++i) w[i] = fmax(__dsub_rn(w[i], __dmul_rn(mass, (double)q[i])), 0.0);
+        for (int i = 0; i < kLane; ++i) w[i] = less(w[i], mass, d[i]);
       }
     } else {
+#pragma unroll 1
       for (int j = 0; j < taken_off; ++j) {
         const int d = off[j] - at;
+        if (d >= 0 && d < kLane) {
 #pragma unroll
-        for (int i = 0; i < kLane; ++i)
-          if (d == i) x[i] = 0.f;
+          for (int i = 0; i < kLane; ++i)
+            if (d == i) w[i] = 0.0;
+        }
       }
-#pragma unroll
-      for (int i = 0; i < kLane; ++i) w[i] = x[i];
     }
   };
-  int turn = 0;
-  // The sum of the weights; those of the warps and CTAs stay in warp_sums and cta_sums[turn ^ 1].  The whole cluster calls it.
-  auto sum = [&]() {
-    double mine = 0.0;
-#pragma unroll 2
-    for (int s = step0; s < step1; ++s) {
-      double w[kLane];
-      weights(w, s);
+  auto total_of = [](const double (&w)[kLane]) { return ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])); };
+  auto shift_of = [&]() { return (int)((reinterpret_cast<uintptr_t>(target + node * p.target_stride) & 15u) / sizeof(T)); };
+  // the sum of a lane's weights in step s, and the weights
+  auto one_step = [&](double (&w)[kLane], int s) {
+    const int at = s * kStep + lane * kLane - shift_of();
+    Values<T> x, q;
+    x.load_any(target + node * p.target_stride, at, p.vocab);
+    if (DRAFT && taken_off) q.load_any(draft + node * p.draft_stride, at, p.vocab);
+    weights(w, x, q, at);
+    return total_of(w);
+  };
+  // the sum of a lane's weights in steps [from, to)
+  auto lane_sum = [&](int from, int to) {
+    const T *row = target + node * p.target_stride, *others = DRAFT ? draft + node * p.draft_stride : row;
+    const int shift = shift_of();
+    // steps that lie in the row and begin on 16 bytes: kAhead at a time
+    const bool even = !DRAFT || ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(others)) & 15u) == 0;
+    const int whole0 = even ? max(from, shift ? 1 : 0) : to, whole1 = even ? min(to, (p.vocab + shift) / kStep) : to;
+    double total = 0.0, w[kLane];
+#pragma unroll 1
+    for (int s0 = whole0; s0 < whole1; s0 += kAhead) {
+      Values<T> x[kAhead], q[kAhead];
 #pragma unroll
-      for (int i = 0; i < kLane; ++i) mine += w[i];
+      for (int u = 0; u < kAhead; ++u) {
+        if (s0 + u >= whole1) break;
+        const int at = (s0 + u) * kStep + lane * kLane - shift;
+        x[u].load(row + at);
+        if (DRAFT && taken_off) q[u].load(others + at);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (s0 + u >= whole1) break;
+        weights(w, x[u], q[u], (s0 + u) * kStep + lane * kLane - shift);
+        total += total_of(w);
+      }
     }
-    mine = warp_sum(mine);
-    __syncthreads();  // (the sums of the call before have been read)
-    if (lane == 0) warp_sums[warp] = mine;
-    __syncthreads();
-    if (warp == 0) {
-      double cta = warp_sum(lane < kWarps ? warp_sums[lane] : 0.0);
-      if (lane < kCluster) st_cluster_f64(mapa_addr(smem_u32(&cta_sums[turn][rank]), lane), cta);
+#pragma unroll 1
+    for (int s = from; s < to; ++s) {
+      if (s == whole0 && whole0 < whole1) s = whole1 - 1;  // (done)
+      else total += one_step(w, s);
     }
+    return total;
+  };
+  const int step0 = min(steps, (rank * kWarps + warp) * each), step1 = min(steps, step0 + each);
+  int turn = 0;
+  // The sum of the weights; the parts' stay in part_sums[turn ^ 1].  The whole cluster calls it.
+  auto sum = [&]() {
+    const double part = warp_sum(lane_sum(step0, step1));
+    if (lane < p.ctas) st_cluster_f64(mapa_addr(smem_u32(&part_sums[turn][rank * kWarps + warp]), lane), part);
     cluster_sync_all();
     double all = 0.0;
-#pragma unroll
-    for (int r = 0; r < kCluster; ++r) all += cta_sums[turn][r];
+    for (int i = lane; i < parts; i += 32) all += part_sums[turn][i];
+    all = warp_sum(all);
     turn ^= 1;  // (two sets: a CTA may be one call ahead)
     return all;
   };
 
   // The walk: every warp takes the same steps.
-  int length = 1, at = 0;
+  int length = 1, at = 0, set = 0;
   double mass = 1.0, whole = -1.0;  // whole: the sum of the weights as they are, if it is known
   if (rank == 0 && tid == 0) kept[0] = 0;
   while (true) {
@@ -196,7 +237,7 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster, 1, 1) ver
     const double q = at_draft[child];
     double w = at_target[child];
     if (DRAFT) {
-      for (int j = 0; j < taken_off; ++j) w = fmax(__dsub_rn(w, __dmul_rn(masses[j], q)), 0.0);
+      for (int j = 0; j < taken_off; ++j) w = less(w, mine_off[j], q);
     } else {  // the same token again: nothing is left of it
       for (int i = node + 1; i < child; i += 32)
         if (__any_sync(0xffffffffu, i + lane < child && parent[i + lane] == node && token[i + lane] == token[child])) w = 0.0;
@@ -209,9 +250,15 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster, 1, 1) ver
       whole = -1.0;
       taken_off = 0;
     } else if (DRAFT) {
-      __syncthreads();  // (all have read the masses that are there; those of another node are overwritten)
-      if (tid == 0) masses[taken_off] = mass;
-      __syncthreads();
+      // All warps write the same.  A warp may be ahead of others by less than one sum, so with a node's first rejection it may overwrite what
+      // they still read of the node before, if there were not two sets.
+      if (taken_off == 0) {
+        mine_off = masses + set * p.max_new;
+        set ^= 1;
+      }
+      __syncwarp();
+      if (lane == 0) mine_off[taken_off] = mass;
+      __syncwarp();
       ++taken_off;
       mass = whole = sum();
     } else {
@@ -219,7 +266,6 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster, 1, 1) ver
     }
   }
   if (!DRAFT) {  // all children of the node are off
-    __syncthreads();
     if (warp == 0) {
       int count = 0;
       for (int i = node + 1; i < n; i += 32) {
@@ -248,90 +294,101 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster, 1, 1) ver
   };
   if (whole == 0.0) {
     if (rank == 0 && tid == 0) answer(-1);
-  } else {
-    // The first part whose running sum passes the border; where rounding leaves none, the last one that weighs anything.
-    const double border = (double)p.sample[b] * whole;
-    const double* ctas = cta_sums[turn ^ 1];
-    double before = 0.0, start = 0.0;
-    int part = -1;
-    bool passed = false;
-    for (int r = 0; r < kCluster && !passed; ++r) {
-      const double x = ctas[r];
-      passed = before + x > border;
-      if (passed || x > 0.0) {
-        part = r;
-        start = before;
-      }
-      before += x;
-    }
-    if (part == (int)rank) {
-      int chosen = -1;
-      double from = start;
-      before = start;
-      passed = false;
-      for (int r = 0; r < kWarps && !passed; ++r) {
-        const double x = warp_sums[r];
-        passed = before + x > border;
-        if (passed || x > 0.0) {
-          chosen = r;
-          from = before;
-        }
-        before += x;
-      }
-      if (chosen == warp) {
-        int best = -1;
-        bool done = false;
-        for (int s = step0; s < step1 && !done; ++s) {
-          double w[kLane], lane_sum = 0.0;
-          weights(w, s);
-#pragma unroll
-          for (int i = 0; i < kLane; ++i) lane_sum += w[i];
-          double upto = lane_sum;  // of the lanes up to this one
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double other = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += other;
-          }
-          double run = from + (upto - lane_sum);
-          int here = -1, latest = -1;  // the first that passes; the last that weighs anything
-#pragma unroll
-          for (int i = 0; i < kLane; ++i) {
-            run += w[i];
-            if (w[i] > 0.0) {
-              latest = i;
-              if (here < 0 && run > border) here = i;
-            }
-          }
-          const unsigned hits = __ballot_sync(0xffffffffu, here >= 0), some = __ballot_sync(0xffffffffu, latest >= 0);
-          if (hits) {
-            const int who = __ffs(hits) - 1;
-            best = s * kStep + who * kLane + __shfl_sync(0xffffffffu, here, who);
-            done = true;
-          } else if (some) {
-            const int who = 31 - __clz(some);
-            best = s * kStep + who * kLane + __shfl_sync(0xffffffffu, latest, who);
-          }
-          from += __shfl_sync(0xffffffffu, upto, 31);
-        }
-        if (lane == 0) answer(best);
-      }
-    }
+    return;
   }
-  // (the last exchange of sums was behind a barrier of the cluster: nobody writes into a CTA that has gone)
+  // The first part whose running sum passes the border; where rounding leaves none, the last one that weighs anything.
+  const double border = (double)p.sample[b] * whole;
+  double start = 0.0;  // the weights before the part
+  auto pick = [&](const double* sums, int count) {  // (kMostParts / 32 a lane)
+    constexpr int kEach = kMostParts / 32;
+    double x[kEach], own = 0.0;
+    int mine = -1;  // the lane's first that passes, or its last that weighs anything
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      x[i] = kEach * lane + i < count ? sums[kEach * lane + i] : 0.0;
+      own += x[i];
+    }
+    double upto = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += other;
+    }
+    double run = start + (upto - own), before = run;
+    bool passed = false;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (!passed && x[i] > 0.0) {
+        passed = run + x[i] > border;
+        mine = i;
+        before = run;
+      }
+      run += x[i];
+    }
+    const unsigned hits = __ballot_sync(0xffffffffu, passed), some = __ballot_sync(0xffffffffu, mine >= 0);
+    const int who = hits ? __ffs(hits) - 1 : 31 - __clz(some);
+    start = __shfl_sync(0xffffffffu, before, who);
+    return kEach * who + __shfl_sync(0xffffffffu, mine, who);
+  };
+  const int part = pick(part_sums[turn ^ 1], parts);
+  if (part / kWarps != rank) return;  // (nobody writes into a CTA that has gone: all sums were behind a barrier of the cluster)
+  // its eighths, a warp each
+  const int from = min(steps, part * each), to = min(steps, from + each), piece = (to - from + kWarps - 1) / kWarps;
+  const int mine0 = min(to, from + warp * piece), mine1 = min(to, mine0 + piece);
+  const double eighth = warp_sum(lane_sum(mine0, mine1));
+  if (lane == 0) eighths[warp] = eighth;
+  __syncthreads();
+  if (pick(eighths, kWarps) != warp) return;
+  int best = -1;
+  for (int s = mine0; s < mine1; ++s) {
+    double w[kLane];
+    const double own = one_step(w, s);
+    double upto = own;  // of the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += other;
+    }
+    double run = start + (upto - own);
+    int here = -1, latest = -1;  // the first that passes; the last that weighs anything
+#pragma unroll
+    for (int i = 0; i < kLane; ++i) {
+      run += w[i];
+      if (w[i] > 0.0) {
+        latest = i;
+        if (here < 0 && run > border) here = i;
+      }
+    }
+    const unsigned hits = __ballot_sync(0xffffffffu, here >= 0), some = __ballot_sync(0xffffffffu, latest >= 0);
+    if (hits || some) {
+      const int who = hits ? __ffs(hits) - 1 : 31 - __clz(some);
+      best = s * kStep + who * kLane - shift_of() + __shfl_sync(0xffffffffu, hits ? here : latest, who);
+    }
+    if (hits) break;
+    start += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  if (lane == 0) answer(best);
 }
 
 template <typename T>
-cudaError_t launch(const VerifyParams& p, int batch, cudaStream_t s) {
+cudaError_t launch(VerifyParams p, int batch, cudaStream_t s) {
+  // As many CTAs a sequence as run at once, two a SM (64 sequences, 128000 tokens: with four 23 us, with eight of half the registers
+  // and one step in flight 30).  Sixteen warps a CTA where one runs a SM gave nothing (16 trees of 24 over 50001 tokens 23.7 us, with eight 23.1).
+  p.ctas = kMostCtas;
+  while (p.ctas > 1 && (int64_t)batch * p.ctas > 2 * kNumSMsDefault) p.ctas /= 2;
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel waits (griddepcontrol.wait) itself
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)batch * kCluster);
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)batch * p.ctas);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)((5 * p.max_new + 1) / 2 * 2) * 4 + (size_t)p.max_new * 8;  // (28 KB at most)
+  cfg.dynamicSmemBytes = (size_t)((5 * p.max_new + 1) / 2 * 2) * 4 + (size_t)p.max_new * 16;  // (36 KB at most)
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return p.draft ? cudaLaunchKernelEx(&cfg, verify_kernel<T, true>, p) : cudaLaunchKernelEx(&cfg, verify_kernel<T, false>, p);
 }
 
@@ -345,7 +402,7 @@ extern "C" int frisk_b200_draft_verify(frisk_b200_ctx* ctx, const frisk_b200_ver
                                        void* next, void* stream) {
   if (!ctx || !d) return FRISK_B200_E_ARG;
   if (!dtype_ok(d->dtype)) return FRISK_B200_E_CACHE_TYPE;
-  if (d->rows < 0 || d->rows > INT32_MAX || d->batch < 0 || d->batch > INT32_MAX / kCluster || d->max_new < 1 || d->max_new > kMaxNodes || d->vocab < 1 ||
+  if (d->rows < 0 || d->rows > INT32_MAX || d->batch < 0 || d->batch > INT32_MAX / kMostCtas || d->max_new < 1 || d->max_new > kMaxNodes || d->vocab < 1 ||
       d->vocab > INT32_MAX - 2 * kStep || (d->rows > 1 && (d->target_stride < 0 || d->draft_stride < 0)))
     return FRISK_B200_E_CACHE_SHAPE;
   if (d->batch == 0) return 0;
