@@ -1,6 +1,8 @@
 """Low-rank adapters of many requests, added to a shared projection: ``adapter_gemm``."""
+import contextlib
+
 from . import capi
-from .cache import _new_like, _on_stream, _stream_of
+from .cache import _new_like, _on_stream, _stream_of, _workspace
 from .execute import _torch, context_for
 
 
@@ -39,16 +41,15 @@ def adapter_gemm(x, a, b, c, starts, adapters, *, scales=None, out=None, stream=
         _refuse("starts and adapters must be dense int32 [batch + 1] and [batch]")
     if scales is not None and (scales.dtype != torch.float32 or scales.shape != (count,) or not scales.is_contiguous()):
         _refuse("scales must be dense float32, one for each adapter")
-    if out is None:
-        if stream is None:
-            out = _new_like(c)
-        else:
-            with _on_stream(stream, c.device):
-                out = _new_like(c)
-    elif out.dtype != c.dtype or out.shape != c.shape or out.get_device() != dev or (n > 1 and out.stride(1) != 1):
+    if out is not None and (out.dtype != c.dtype or out.shape != c.shape or out.get_device() != dev or (n > 1 and out.stride(1) != 1)):
         _refuse("out must have the type, shape and device of c, and dense rows")
-    desc = capi.AdapterDesc(rows, k, n, x.stride(0), a.stride(1), a.stride(0), b.stride(1), b.stride(0), c.stride(0), out.stride(0), rank, count, batch, code,
-                            code if c.dtype == x.dtype else capi.F32)
+    with contextlib.nullcontext() if stream is None else _on_stream(stream, c.device):
+        if out is None:
+            out = _new_like(c)
+        desc = capi.AdapterDesc(rows, k, n, x.stride(0), a.stride(1), a.stride(0), b.stride(1), b.stride(0), c.stride(0), out.stride(0), rank, count, batch, code,
+                                code if c.dtype == x.dtype else capi.F32)
+        nbytes = capi.adapter_workspace_bytes(desc)
+        workspace = _workspace(nbytes, dev) if nbytes else None
     context_for(dev).adapter_gemm(desc, x.data_ptr(), a.data_ptr(), b.data_ptr(), c.data_ptr(), None if scales is None else scales.data_ptr(), starts.data_ptr(),
-                                  adapters.data_ptr(), out.data_ptr(), _stream_of(stream, dev))
+                                  adapters.data_ptr(), out.data_ptr(), None if workspace is None else workspace.data_ptr(), nbytes, _stream_of(stream, dev))
     return out

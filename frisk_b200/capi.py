@@ -36,6 +36,7 @@ EXPORTS = (
     "frisk_b200_cache_attention_workspace_bytes", "frisk_b200_cache_attention_tile_rows",
     "frisk_b200_cache_pages_workspace_bytes", "frisk_b200_cache_fork", "frisk_b200_cache_grow", "frisk_b200_cache_compact",
     "frisk_b200_cache_copy", "frisk_b200_cache_keep", "frisk_b200_draft_verify", "frisk_b200_adapter_gemm",
+    "frisk_b200_adapter_workspace_bytes",
 )
 
 
@@ -187,7 +188,8 @@ def load():
         "frisk_b200_cache_copy": (ctypes.c_int, [vp, cd, cd, vp, vp, i64, vp]),
         "frisk_b200_cache_keep": (ctypes.c_int, [vp, cd, vp, i64, i32, vp, vp, vp]),
         "frisk_b200_draft_verify": (ctypes.c_int, [vp, vd, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
-        "frisk_b200_adapter_gemm": (ctypes.c_int, [vp, ap, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
+        "frisk_b200_adapter_gemm": (ctypes.c_int, [vp, ap, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+        "frisk_b200_adapter_workspace_bytes": (sz, [ap]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -354,8 +356,8 @@ class Context:
                                             counts, token, stream)
         raise_for(rc, self._h)
 
-    def adapter_gemm(self, desc, x, a, b, c, scales, starts, adapters, out, stream=None):
-        rc = load().frisk_b200_adapter_gemm(self.handle, desc, x, a, b, c, scales, starts, adapters, out, stream)
+    def adapter_gemm(self, desc, x, a, b, c, scales, starts, adapters, out, ws_ptr, ws_bytes, stream=None):
+        rc = load().frisk_b200_adapter_gemm(self.handle, desc, x, a, b, c, scales, starts, adapters, out, ws_ptr, ws_bytes, stream)
         raise_for(rc, self._h)
 
     def check(self, stream=None):
@@ -385,6 +387,11 @@ def cache_attention_tile_rows(cache, desc):
     if rows < 0:
         raise_for(rows)
     return rows
+
+
+def adapter_workspace_bytes(desc):
+    """Bytes ``Context.adapter_gemm`` needs.  Host-only."""
+    return load().frisk_b200_adapter_workspace_bytes(desc)
 
 
 def cache_pages_workspace_bytes(cache, which):

@@ -17,38 +17,14 @@
 // than in the rounding of the result (16 and 24 bits in bf16, 22 in fp16; fp16 terms stand at a power of two that brings a row's
 // largest to 2^14, so that sums beyond fp16's range keep their value).
 #include <algorithm>
-#include <type_traits>
 
-#include "cache_common.cuh"
+#include "adapters.cuh"
 
 namespace fb {
 namespace {
+using namespace adapter;
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kMaxRank = 128;
-
-struct AdapterParams {
-  const void *x, *a, *b, *c;
-  void* out;
-  const float* scales;
-  const int *starts, *adapters;
-  int64_t ldx, lda, a_step, ldb, b_step, ldc, ldo, rows;
-  int K, N, R, count, batch;
-  int cluster;
-  bool wide;  // c and out on 16 bytes, row by row
-  unsigned* status;
-};
-
-template <typename T> struct Terms;  // the 16-bit types
-template <> struct Terms<__half> {
-  static __device__ __forceinline__ float value(uint16_t w) { return __half2float(__ushort_as_half(w)); }
-  static __device__ __forceinline__ uint16_t round(float x) { return __half_as_ushort(__float2half_rn(x)); }
-};
-template <> struct Terms<__nv_bfloat16> {
-  static __device__ __forceinline__ float value(uint16_t w) { return __uint_as_float((uint32_t)w << 16); }
-  static __device__ __forceinline__ uint16_t round(float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); }
-};
-
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if (std::is_same<T, __half>::value)
@@ -70,58 +46,13 @@ __device__ __forceinline__ uint4 load8(const uint16_t* at, int n) {
     if (i < n) w[i >> 1] |= (uint32_t)__ldg(at + i) << (16 * (i & 1));
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ uint32_t word(const uint4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
-
-// c's 8 neighbours, and the result's
-template <typename C>
-__device__ __forceinline__ void load_c(float (&v)[8], const C* at, int n, bool wide) {
-  if (wide && n >= 8) {
-    uint4 w[sizeof(C) / 2];
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(C) / 2; ++i) w[i] = *(reinterpret_cast<const uint4*>(at) + i);
-    if (sizeof(C) == 4) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(word(w[i >> 2 & (sizeof(C) / 2 - 1)], i & 3));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint16_t h = (uint16_t)(word(w[0], i >> 1) >> (16 * (i & 1)));
-        v[i] = Terms<typename std::conditional<sizeof(C) == 2, C, __half>::type>::value(h);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)at[i] : 0.f;
-  }
-}
-template <typename C>
-__device__ __forceinline__ void store_out(C* at, const float (&v)[8], int n, bool wide) {
-  if (wide && n >= 8) {
-    if (sizeof(C) == 4) {
-      reinterpret_cast<float4*>(at)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(at)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        using T = typename std::conditional<sizeof(C) == 2, C, __half>::type;
-        w[i] = Terms<T>::round(v[2 * i]) | (uint32_t)Terms<T>::round(v[2 * i + 1]) << 16;
-      }
-      *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) at[i] = (C)v[i];
-  }
-}
 
 // MW: groups of 16 rows a warp has; MWARPS: warps side by side over rows (the others share the inner index, then the columns)
 template <typename T, typename C, int RMAX, int MW, int MWARPS>
 struct Plan {
   static constexpr int kRows = 16 * MW * MWARPS, kShare = kWarps / MWARPS;
   static constexpr int kTiles = RMAX / 8, kBlocks = (RMAX + 31) / 32;
-  static constexpr int kTerms = sizeof(C) == 4 && std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
+  static constexpr int kTerms = kTermsOf<T, C>;
   static constexpr int kPitch = RMAX + 8;  // of rows of sums, floats (lanes of a fragment meet no bank twice)
   static constexpr size_t kSumBytes = (size_t)kShare * kRows * kPitch * 4;
   static constexpr size_t kFullBytes = (size_t)kRows * kPitch * 4;
@@ -138,56 +69,16 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
   uint4* terms = reinterpret_cast<uint4*>(memory);                                  // later: [16 rows][32 of R][half][term][lane]
   float* full = reinterpret_cast<float*>(memory + P::kFirstBytes);                  // [row][pitch]
   float* row_scale = reinterpret_cast<float*>(memory + P::kFirstBytes + P::kFullBytes);
-  __shared__ int tiles_of[kWarps], found[3];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int C_ = p.cluster, rank = (int)cluster_ctarank(), tile = blockIdx.x / C_;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  // The tile's sequence and rows: tiles are counted over the sequences, a thread each.
-  if (tid == 0) found[0] = -1;
-  int before = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
-    const int b = b0 + tid;
-    int lo = 0, n = 0;
-    if (b < p.batch) {
-      lo = p.starts[b];
-      const int64_t many = (int64_t)p.starts[b + 1] - lo;
-      if (lo < 0 || many < 0 || lo + many > p.rows) atomicCAS(p.status, 0u, cache::ST_CACHE_ROWS);
-      else n = (int)many;
-    }
-    const int mine = (n + P::kRows - 1) / P::kRows;
-    int upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int other = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += other;
-    }
-    __syncthreads();
-    if (lane == 31) tiles_of[warp] = upto;
-    __syncthreads();
-    int at = before + upto - mine;
-    for (int i = 0; i < kWarps; ++i) {
-      if (i < warp) at += tiles_of[i];
-      before += tiles_of[i];
-    }
-    if (tile >= at && tile < at + mine) {
-      found[0] = b;
-      found[1] = lo + (tile - at) * P::kRows;
-      found[2] = min(P::kRows, n - (tile - at) * P::kRows);
-    }
-    if (before > tile) break;  // (the same in all threads)
-  }
-  __syncthreads();
-  if (found[0] < 0) return;  // (the whole cluster: there are fewer tiles than clusters)
-  const int64_t row0 = found[1];
-  const int rows = found[2];
-  int which = p.adapters[found[0]];
-  if (which >= p.count) {
-    if (tid == 0) atomicCAS(p.status, 0u, cache::ST_ADAPTER);
-    which = -1;
-  }
+  const Tile found = find_tile<kThreads>(p, tile, P::kRows, false);
+  if (found.seq < 0) return;  // (the whole cluster: there are fewer tiles than clusters)
+  const int64_t row0 = found.row;
+  const int rows = found.rows, which = adapter_of(p, found.seq);
   const C* c = static_cast<const C*>(p.c) + row0 * p.ldc;
   C* out = static_cast<C*>(p.out) + row0 * p.ldo;
   const int blocks_n = (p.N + 31) / 32, n0 = (int)((int64_t)blocks_n * rank / C_), n1 = (int)((int64_t)blocks_n * (rank + 1) / C_);
@@ -197,9 +88,12 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
       for (int i = tid; i < rows * pieces; i += kThreads) {
         const int r = i / pieces, col = n0 * 32 + (i - r * pieces) * 8;
         if (col >= p.N) continue;
+        Eight<C> old;
+        old.load(c + r * p.ldc + col, p.N - col, p.wide);
         float v[8];
-        load_c<C>(v, c + r * p.ldc + col, p.N - col, p.wide);
-        store_out<C>(out + r * p.ldo + col, v, p.N - col, p.wide);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = old[j];
+        store_eight<C>(out + r * p.ldo + col, v, p.N - col, p.wide);
       }
     }
     return;
@@ -282,9 +176,7 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
       for (int i = lane; i < RMAX; i += 32) most = fmaxf(most, fabsf(full[r * P::kPitch + i]));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      // most = 1.m * 2^(e - 127): times 2^(14 - (e - 127)).  (Infinities stay; a row of zeros or subnormals stands at 2^126.)
-      const int e = (int)(__float_as_uint(most) >> 23);
-      if (lane == 0) row_scale[r] = e == 255 ? 1.f : __uint_as_float((uint32_t)min(254, 268 - max(e, 15)) << 23);
+      if (lane == 0) row_scale[r] = row_power(most);
     }
     __syncthreads();
   }
@@ -302,18 +194,10 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
         v[0] = two.x * up;
         v[1] = two.y * up;
       }
+      uint32_t both[P::kTerms];
+      split<T>(v[0], v[1], both);
 #pragma unroll
-      for (int t = 0; t < P::kTerms; ++t) {
-        uint32_t both = 0;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const uint16_t h = Terms<T>::round(v[n]);
-          const float back = Terms<T>::value(h);
-          both |= (uint32_t)h << (16 * n);
-          v[n] = isfinite(back) ? v[n] - back : 0.f;  // (exact)
-        }
-        f[t][j] = both;
-      }
+      for (int t = 0; t < P::kTerms; ++t) f[t][j] = both[t];
     }
 #pragma unroll
     for (int t = 0; t < P::kTerms; ++t) terms[(i * P::kTerms + t) * 32 + lane] = make_uint4(f[t][0], f[t][1], f[t][2], f[t][3]);
@@ -333,13 +217,13 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
   const int first = 8 * (g >> 1) + (g & 1);  // of the rows of B that this lane's columns of the four tiles are: first + 2 j
   for (int nb = n0 + share; nb < n1; nb += P::kShare) {
     const int col = nb * 32 + 8 * q, left = p.N - col;
-    float y[MW][2][8];
+    Eight<C> old[MW][2];
 #pragma unroll
     for (int m = 0; m < MW; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r = my_row + 16 * m + 8 * h + g;
-        load_c<C>(y[m][h], c + r * p.ldc + col, r < rows ? left : 0, p.wide);
+        old[m][h].load(c + r * p.ldc + col, r < rows ? left : 0, p.wide);
       }
     float d[MW][4][4];
 #pragma unroll
@@ -374,12 +258,10 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
       for (int h = 0; h < 2; ++h) {
         const int r = my_row + 16 * m + 8 * h + g;
         if (r >= rows) continue;
+        float y[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          y[m][h][2 * j] = fmaf(alpha, d[m][j][2 * h] * up[m][h], y[m][h][2 * j]);
-          y[m][h][2 * j + 1] = fmaf(alpha, d[m][j][2 * h + 1] * up[m][h], y[m][h][2 * j + 1]);
-        }
-        store_out<C>(out + r * p.ldo + col, y[m][h], left, p.wide);
+        for (int j = 0; j < 8; ++j) y[j] = fmaf(alpha, d[m][j / 2][2 * h + j % 2] * up[m][h], old[m][h][j]);
+        store_eight<C>(out + r * p.ldo + col, y, left, p.wide);
       }
   }
 }
@@ -434,16 +316,27 @@ cudaError_t launch_rank(frisk_b200_ctx* ctx, const AdapterParams& p, cudaStream_
 
 using namespace fb;
 
-extern "C" int frisk_b200_adapter_gemm(frisk_b200_ctx* ctx, const frisk_b200_adapter_desc* d, const void* x, const void* a, const void* b, const void* c,
-                                       const float* scales, const int32_t* starts, const int32_t* adapters, void* out, void* stream) {
-  if (!ctx || !d) return FRISK_B200_E_ARG;
+static int check_sizes(const frisk_b200_adapter_desc* d) {
   if (d->dtype != FRISK_B200_F16 && d->dtype != FRISK_B200_BF16) return FRISK_B200_E_CACHE_TYPE;
   if (d->dtype_c != d->dtype && d->dtype_c != FRISK_B200_F32) return FRISK_B200_E_CACHE_TYPE;
   if (d->rows < 0 || d->rows > INT32_MAX || d->batch < 0 || d->count < 0 || d->K < 1 || d->N < 1 || d->K > INT32_MAX - 64 || d->N > INT32_MAX - 64 || d->rank < 8 ||
       d->rank > kMaxRank || d->rank % 8)
     return FRISK_B200_E_CACHE_SHAPE;
-  if (d->rows == 0 || d->batch == 0) return 0;
   if ((std::min<int64_t>(d->rows, d->rows / 16 + d->batch)) * kMaxCluster > INT32_MAX) return FRISK_B200_E_TOO_LARGE;
+  return 0;
+}
+
+extern "C" size_t frisk_b200_adapter_workspace_bytes(const frisk_b200_adapter_desc* d) {
+  return !d || check_sizes(d) || d->rows == 0 || d->batch == 0 ? 0 : adapter_tiles_workspace_bytes(*d);
+}
+
+extern "C" int frisk_b200_adapter_gemm(frisk_b200_ctx* ctx, const frisk_b200_adapter_desc* d, const void* x, const void* a, const void* b, const void* c,
+                                       const float* scales, const int32_t* starts, const int32_t* adapters, void* out, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+  if (!ctx || !d) return FRISK_B200_E_ARG;
+  const int rc = check_sizes(d);
+  if (rc) return rc;
+  if (d->rows == 0 || d->batch == 0) return 0;
   if (!x || !c || !out || !starts || !adapters || (d->count > 0 && (!a || !b))) return FRISK_B200_E_ARG;
   const int64_t rows = d->rows;
   if ((rows > 1 && (d->ldx < d->K || d->ldc < d->N || d->ldo < d->N)) || d->lda < d->K || d->ldb < d->rank || (d->count > 1 && (d->a_step < 0 || d->b_step < 0)))
@@ -477,6 +370,17 @@ extern "C" int frisk_b200_adapter_gemm(frisk_b200_ctx* ctx, const frisk_b200_ada
       (scales && d->count && ranges_overlap(out, out_bytes, scales, (size_t)d->count * 4)) || ranges_overlap(out, out_bytes, starts, ((size_t)d->batch + 1) * 4) ||
       ranges_overlap(out, out_bytes, adapters, (size_t)d->batch * 4))
     return FRISK_B200_E_OVERLAP;
+  const size_t need = adapter_tiles_workspace_bytes(*d);
+  if (need) {
+    if (!workspace || workspace_bytes < need) return FRISK_B200_E_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(workspace) & 15u) return FRISK_B200_E_ALIGN;
+    const size_t x_bytes = (size_t)((rows - 1) * d->ldx + d->K) * es, c_bytes = (size_t)((rows - 1) * d->ldc + d->N) * cs;
+    if (ranges_overlap(workspace, need, out, out_bytes) || ranges_overlap(workspace, need, x, x_bytes) || ranges_overlap(workspace, need, c, c_bytes) ||
+        (a_bytes && ranges_overlap(workspace, need, a, a_bytes)) || (b_bytes && ranges_overlap(workspace, need, b, b_bytes)) ||
+        (scales && d->count && ranges_overlap(workspace, need, scales, (size_t)d->count * 4)) ||
+        ranges_overlap(workspace, need, starts, ((size_t)d->batch + 1) * 4) || ranges_overlap(workspace, need, adapters, (size_t)d->batch * 4))
+      return FRISK_B200_E_OVERLAP;
+  }
   AdapterParams p{};
   p.x = x;
   p.a = a;
@@ -503,6 +407,7 @@ extern "C" int frisk_b200_adapter_gemm(frisk_b200_ctx* ctx, const frisk_b200_ada
   p.status = ctx->d_status;
   FB_DEVICE(ctx);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (need) return launch_adapter_tiles(ctx, *d, p, workspace, s);
   const bool f32 = d->dtype_c == FRISK_B200_F32;
   FB_CUDA(ctx, d->dtype == FRISK_B200_F16 ? (f32 ? launch_rank<__half, float>(ctx, p, s) : launch_rank<__half, __half>(ctx, p, s))
                                           : (f32 ? launch_rank<__nv_bfloat16, float>(ctx, p, s) : launch_rank<__nv_bfloat16, __nv_bfloat16>(ctx, p, s)));

@@ -1,0 +1,165 @@
+// Pieces shared by the kernels of low-rank adapters: parameters, the 16-bit types, eight neighbours of c and the result.
+#pragma once
+#include <type_traits>
+
+#include "cache_common.cuh"
+
+namespace fb {
+namespace adapter {
+
+constexpr int kMaxRank = 128;
+
+struct AdapterParams {
+  const void *x, *a, *b, *c;
+  void* out;
+  const float* scales;
+  const int *starts, *adapters;
+  int64_t ldx, lda, a_step, ldb, b_step, ldc, ldo, rows;
+  int K, N, R, count, batch;
+  int cluster;
+  bool wide;  // c and out on 16 bytes, row by row
+  unsigned* status;
+};
+
+template <typename T> struct Terms;  // the 16-bit types
+template <> struct Terms<__half> {
+  static __device__ __forceinline__ float value(uint16_t w) { return __half2float(__ushort_as_half(w)); }
+  static __device__ __forceinline__ uint16_t round(float x) { return __half_as_ushort(__float2half_rn(x)); }
+};
+template <> struct Terms<__nv_bfloat16> {
+  static __device__ __forceinline__ float value(uint16_t w) { return __uint_as_float((uint32_t)w << 16); }
+  static __device__ __forceinline__ uint16_t round(float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); }
+};
+
+// The 16-bit terms that a sum between the products becomes: two, or three for bf16 whose result is 32-bit
+template <typename T, typename C>
+constexpr int kTermsOf = sizeof(C) == 4 && std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
+
+// fp16: the power of two that brings a row's largest sum, most = 1.m * 2^(e - 127), to 2^14.  (Infinities stay; a row of zeros or subnormals
+// stands at 2^126.)
+__device__ __forceinline__ float row_power(float most) {
+  const int e = (int)(__float_as_uint(most) >> 23);
+  return e == 255 ? 1.f : __uint_as_float((uint32_t)min(254, 268 - max(e, 15)) << 23);
+}
+// two neighbours as kTerms words of 16-bit terms: each term is what those before it leave (exact, but for the last)
+template <typename T, int kTerms>
+__device__ __forceinline__ void split(float a, float b, uint32_t (&words)[kTerms]) {
+  float v[2] = {a, b};
+#pragma unroll
+  for (int t = 0; t < kTerms; ++t) {
+    words[t] = 0;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const uint16_t h = Terms<T>::round(v[n]);
+      const float back = Terms<T>::value(h);
+      words[t] |= (uint32_t)h << (16 * n);
+      v[n] = isfinite(back) ? v[n] - back : 0.f;
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t word(const uint4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
+
+// Eight neighbours of c, as they are in memory, of which the first n are there
+template <typename C>
+struct Eight {
+  uint4 w[sizeof(C) / 2];
+  __device__ __forceinline__ void load(const C* at, int n, bool wide) {
+    if (wide && n >= 8) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(C) / 2; ++i) w[i] = *(reinterpret_cast<const uint4*>(at) + i);
+    } else {
+      C v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i < n ? at[i] : C(0.f);
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(C) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(v)[i];
+    }
+  }
+  __device__ __forceinline__ float operator[](int i) const {
+    if (sizeof(C) == 4) return __uint_as_float(word(w[i / 4 % (sizeof(C) / 2)], i % 4));
+    using T = typename std::conditional<sizeof(C) == 2, C, __half>::type;
+    return Terms<T>::value((uint16_t)(word(w[0], i / 2) >> (16 * (i & 1))));
+  }
+};
+template <typename C>
+__device__ __forceinline__ void store_eight(C* at, const float (&v)[8], int n, bool wide) {
+  if (wide && n >= 8) {
+    if (sizeof(C) == 4) {
+      reinterpret_cast<float4*>(at)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(at)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      using T = typename std::conditional<sizeof(C) == 2, C, __half>::type;
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = Terms<T>::round(v[2 * i]) | (uint32_t)Terms<T>::round(v[2 * i + 1]) << 16;
+      *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) at[i] = (C)v[i];
+  }
+}
+
+// The tile of `tile_rows` packed rows that is number `tile` over all sequences.  Counted by a block of kThreads threads, a sequence each; the answer
+// is the same in all of them.  `everything`: all tiles are counted.
+struct Tile {
+  int seq, row, rows;  // seq < 0: there are fewer
+  int counted;         // tiles up to here; all, where `everything` is asked for
+};
+template <int kThreads>
+__device__ __forceinline__ Tile find_tile(const AdapterParams& p, int tile, int tile_rows, bool everything) {
+  __shared__ int sums[kThreads / 32], found[3];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) found[0] = -1;
+  int before = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
+    const int b = b0 + tid;
+    int lo = 0, n = 0;
+    if (b < p.batch) {
+      lo = p.starts[b];
+      const int64_t many = (int64_t)p.starts[b + 1] - lo;
+      if (lo < 0 || many < 0 || lo + many > p.rows) atomicCAS(p.status, 0u, cache::ST_CACHE_ROWS);
+      else n = (int)many;
+    }
+    const int mine = (n + tile_rows - 1) / tile_rows;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += other;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    int at = before + upto - mine;
+    for (int i = 0; i < kThreads / 32; ++i) {
+      if (i < warp) at += sums[i];
+      before += sums[i];
+    }
+    if (tile >= at && tile < at + mine) {
+      found[0] = b;
+      found[1] = lo + (tile - at) * tile_rows;
+      found[2] = min(tile_rows, n - (tile - at) * tile_rows);
+    }
+    if (before > tile && !everything) break;  // (the same in all threads)
+  }
+  __syncthreads();
+  return Tile{found[0], found[1], found[2], before};
+}
+// a sequence's adapter; -1: none
+__device__ __forceinline__ int adapter_of(const AdapterParams& p, int seq) {
+  const int which = p.adapters[seq];
+  if (which < p.count) return max(which, -1);
+  if (threadIdx.x == 0) atomicCAS(p.status, 0u, cache::ST_ADAPTER);
+  return -1;
+}
+
+}  // namespace adapter
+
+// long sequences (adapters_tiles.cu)
+size_t adapter_tiles_workspace_bytes(const frisk_b200_adapter_desc& d);  // 0: adapters.cu takes it
+int launch_adapter_tiles(frisk_b200_ctx* ctx, const frisk_b200_adapter_desc& d, const adapter::AdapterParams& p, void* workspace, cudaStream_t s);
+
+}  // namespace fb

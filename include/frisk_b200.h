@@ -427,15 +427,17 @@ int frisk_b200_draft_verify(frisk_b200_ctx* ctx, const frisk_b200_verify_desc* d
  * c and out [rows, N] of dtype_c (dtype or F32), any row pitch and alignment; out may be c, else overlaps nothing (x, c and out
  * may be columns of one buffer of rows).  scales: [count] floats or NULL (1).  32-bit sums, one rounding.  starts, adapters and scales are on
  * the device.  Rows of no sequence are left as they are; an adapter out of range counts as none, and frisk_b200_check returns
- * FRISK_B200_E_DEVICE_TABLE. */
+ * FRISK_B200_E_DEVICE_TABLE.  The workspace (16-byte aligned, contents of no matter) must not be shared by calls that may overlap. */
 typedef struct frisk_b200_adapter_desc {
   int64_t rows, K, N;
   int64_t ldx, lda, a_step, ldb, b_step, ldc, ldo; /* row pitches and steps from one adapter to the next, in elements */
   int32_t rank, count, batch, dtype, dtype_c;
 } frisk_b200_adapter_desc;
+/* Bytes of workspace the call needs (0: none, or refused).  Host-only. */
+size_t frisk_b200_adapter_workspace_bytes(const frisk_b200_adapter_desc* desc);
 int frisk_b200_adapter_gemm(frisk_b200_ctx* ctx, const frisk_b200_adapter_desc* desc, const void* x, const void* a, const void* b,
                             const void* c, const float* scales, const int32_t* starts, const int32_t* adapters, void* out,
-                            void* stream);
+                            void* workspace, size_t workspace_bytes, void* stream);
 
 /* Checks the device status word after the stream has drained (synchronises `stream`).
  * Returns 0, FRISK_B200_E_DEVICE_TIMEOUT, FRISK_B200_E_DEVICE_TABLE or FRISK_B200_E_CUDA. */

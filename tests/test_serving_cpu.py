@@ -36,7 +36,7 @@ def test_null_contexts_are_refused():
     assert lib.frisk_b200_cache_copy(None, _cache(), _cache(), 1 << 20, 1 << 21, 1, None) == -7
     assert lib.frisk_b200_cache_keep(None, _cache(), 1 << 20, 4, 4, 1 << 21, 1 << 22, None) == -7
     assert lib.frisk_b200_draft_verify(None, capi.VerifyDesc(1, 8, 0, 1, 1, 8, 0, 0), *[1 << 20] * 10, None) == -7
-    assert lib.frisk_b200_adapter_gemm(None, capi.AdapterDesc(), *[1 << 20] * 8, None) == -7
+    assert lib.frisk_b200_adapter_gemm(None, capi.AdapterDesc(), *[1 << 20] * 9, 1 << 20, None) == -7
     assert ctypes.sizeof(capi.PageTables) == 40 and ctypes.sizeof(capi.VerifyDesc) == 48 and ctypes.sizeof(capi.AdapterDesc) == 104
 
 
