@@ -11,6 +11,8 @@
 #include <algorithm>
 
 #include "adapters.cuh"
+#include "box_rows.cuh"
+#include "gemm_common.cuh"
 
 namespace fb {
 namespace {
@@ -20,7 +22,7 @@ enum : unsigned { ST_SUMS_EMPTY = 0x311, ST_SUMS_FULL = 0x312, ST_SUMS_DONE = 0x
 
 constexpr int kRows = 128;          // of a tile
 constexpr int kBoxBytes = kRows * 128;  // 128 rows of 64 16-bit elements
-constexpr int kCtas = 8;            // share the K of a tile
+constexpr int kMostCtas = 8;        // share the K of a tile
 
 // The workspace: terms [terms][rows][R], what undoes the rows' powers of two [rows], tiles [most], their number
 struct Work {
@@ -59,7 +61,7 @@ struct SumsLayout {  // of `width` columns, R rounded up to a multiple of 16
 };
 
 template <typename T, int kTerms>
-__global__ void __launch_bounds__(kSumThreads) __cluster_dims__(kCtas, 1, 1)
+__global__ void __launch_bounds__(kSumThreads)
     adapter_sums_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ AdapterParams p,
                         const __grid_constant__ Work work) {
   extern __shared__ unsigned char smem_unaligned[];
@@ -68,7 +70,7 @@ __global__ void __launch_bounds__(kSumThreads) __cluster_dims__(kCtas, 1, 1)
   __shared__ uint32_t tmem_slot, abort_word;
   volatile uint32_t* abort_flag = &abort_word;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = (int)cluster_ctarank(), tile = blockIdx.x / kCtas;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, ctas = p.cluster, rank = (int)cluster_ctarank(), tile = blockIdx.x / ctas;
   const int width = (p.R + 15) / 16 * 16, columns = width <= 32 ? 32 : width <= 64 ? 64 : 128, stage_bytes = SumsLayout::stage_bytes(width);
   if (tid == 0) {
     for (int i = 0; i < kSumStages; ++i) {
@@ -97,7 +99,7 @@ __global__ void __launch_bounds__(kSumThreads) __cluster_dims__(kCtas, 1, 1)
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
-  const int blocks = (p.K + 63) / 64, k0 = (int)((int64_t)blocks * rank / kCtas), n_k = (int)((int64_t)blocks * (rank + 1) / kCtas) - k0;
+  const int blocks = (p.K + 63) / 64, k0 = (int)((int64_t)blocks * rank / ctas), n_k = (int)((int64_t)blocks * (rank + 1) / ctas) - k0;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -151,43 +153,46 @@ __global__ void __launch_bounds__(kSumThreads) __cluster_dims__(kCtas, 1, 1)
   __syncwarp();
   cluster_sync_all();  // every part is there (all roles of all CTAs end: their waits are bounded)
   if (warp >= 2) {
-    // eight threads a row, four neighbours each in turns of 32; the parts in the order of the CTAs
-    const int t = tid - 64, row = rank * (kRows / kCtas) + (t >> 3), quads = width / 4, pitch = SumsLayout::pitch(width);
-    const bool valid = row < found.rows;
-    float4 v[kMaxRank / 32];
-    float most = 0.f;
+    // Eight threads a row, four neighbours each in turns of 32; the parts in the order of the CTAs.
+    const int t = tid - 64, quads = width / 4, pitch = SumsLayout::pitch(width), each = kRows / ctas;
+#pragma unroll 1
+    for (int row = rank * each + (t >> 3); row < (rank + 1) * each; row += 16) {
+      const bool valid = row < found.rows;
+      float4 v[kMaxRank / 32];
+      float most = 0.f;
 #pragma unroll
-    for (int j = 0; j < kMaxRank / 32; ++j) {
-      const int quad = (t & 7) + 8 * j;
-      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (valid && quad < quads) {
-        const uint32_t at = smem_u32(smem) + (row * pitch + quad * 4) * 4;
-        float4 part[kCtas];
+      for (int j = 0; j < kMaxRank / 32; ++j) {
+        const int quad = (t & 7) + 8 * j;
+        v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (valid && quad < quads) {
+          const uint32_t at = smem_u32(smem) + (row * pitch + quad * 4) * 4;
+          float4 part[kMostCtas];
 #pragma unroll
-        for (int r = 0; r < kCtas; ++r) part[r] = ld_cluster_f4(mapa_addr(at, r));
+          for (int r = 0; r < kMostCtas; ++r) part[r] = r < ctas ? ld_cluster_f4(mapa_addr(at, r)) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int r = 0; r < kCtas; ++r) {
-          v[j].x += part[r].x; v[j].y += part[r].y; v[j].z += part[r].z; v[j].w += part[r].w;
+          for (int r = 0; r < kMostCtas; ++r) {
+            v[j].x += part[r].x; v[j].y += part[r].y; v[j].z += part[r].z; v[j].w += part[r].w;
+          }
+          most = fmaxf(fmaxf(fmaxf(most, fabsf(v[j].x)), fabsf(v[j].y)), fmaxf(fabsf(v[j].z), fabsf(v[j].w)));
         }
-        most = fmaxf(fmaxf(fmaxf(most, fabsf(v[j].x)), fabsf(v[j].y)), fmaxf(fabsf(v[j].z), fabsf(v[j].w)));
       }
-    }
-    float up = 1.f;
-    if (!kBf16) {
+      float up = 1.f;
+      if (!kBf16) {
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      up = row_power(most);
-    }
-    if (valid && (t & 7) == 0) work.down[found.row + row] = 1.f / up;  // (of a power of two: exact)
+        for (int o = 4; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        up = row_power(most);
+      }
+      if (valid && (t & 7) == 0) work.down[found.row + row] = 1.f / up;  // (of a power of two: exact)
 #pragma unroll
-    for (int j = 0; j < kMaxRank / 32; ++j) {
-      const int k = ((t & 7) + 8 * j) * 4;
-      if (!valid || k >= p.R) continue;
-      uint32_t lo[kTerms], hi[kTerms];
-      split<T>(v[j].x * up, v[j].y * up, lo);
-      split<T>(v[j].z * up, v[j].w * up, hi);
+      for (int j = 0; j < kMaxRank / 32; ++j) {
+        const int k = ((t & 7) + 8 * j) * 4;
+        if (!valid || k >= p.R) continue;
+        uint32_t lo[kTerms], hi[kTerms];
+        split<T>(v[j].x * up, v[j].y * up, lo);
+        split<T>(v[j].z * up, v[j].w * up, hi);
 #pragma unroll
-      for (int n = 0; n < kTerms; ++n) *reinterpret_cast<uint2*>(work.terms + ((int64_t)n * p.rows + found.row + row) * p.R + k) = make_uint2(lo[n], hi[n]);
+        for (int n = 0; n < kTerms; ++n) *reinterpret_cast<uint2*>(work.terms + ((int64_t)n * p.rows + found.row + row) * p.R + k) = make_uint2(lo[n], hi[n]);
+      }
     }
   }
   __syncwarp();
@@ -206,27 +211,77 @@ __global__ void __launch_bounds__(kSumThreads) __cluster_dims__(kCtas, 1, 1)
 constexpr int kColumns = 128;   // of an item
 constexpr int kWriters = 8;     // warps that add c and store
 constexpr int kColThreads = 64 + 32 * kWriters;
-constexpr int kPitch = 36;      // floats of a row of 32 results on their way from lane = row to rows of lanes
+constexpr int kBox = 32 * 128;   // bytes of a writer's box of c and results: 32 rows of 128 bytes
 
 template <int kTerms, int kHalves>  // halves: 64 of R each
 struct ColumnsLayout {
   static constexpr int kTermBytes = kTerms * kHalves * kBoxBytes;
   static constexpr int kStages = 2;
   static constexpr int kStageBytes = kHalves * kBoxBytes;
-  static constexpr int kTurnOffset = kTermBytes + kStages * kStageBytes;
-  static constexpr int kBytes = kTurnOffset + kWriters * 32 * kPitch * 4 + 1024;
+  static constexpr int kBoxes = kHalves == 1 ? 4 : 2;  // of a writer
+  static constexpr int kBoxOffset = kTermBytes + kStages * kStageBytes;
+  static constexpr int kBytes = kBoxOffset + kWriters * kBoxes * kBox + 1024;
+  static_assert(kBytes <= 232448 - 1024, "shared memory of a CTA");
+};
+
+// A writer's way through its CTA's items: 32 rows and 64 columns of each, in boxes of kWide columns.  Boxes that hold nothing are left out.
+struct Way {
+  const AdapterParams& p;
+  const int4* tiles;
+  int across, quarter, half, wide, n_items;
+  bool in_place;
+  int item, tile, column, box, held;
+  int4 t;       // the tile: first row, rows, adapter
+  int left, rows, col, cols;  // of the box: the tile's rows from its first on; rows and columns that are there
+  __device__ __forceinline__ Way(const AdapterParams& p, const int4* tiles, int across, int quarter, int half, int wide, int n_items, int tile, int column)
+      : p(p), tiles(tiles), across(across), quarter(quarter), half(half), wide(wide), n_items(n_items), in_place(p.c == p.out), item(0), tile(tile), column(column), box(-1),
+        held(-1), t(make_int4(0, 0, -1, 0)) {}
+  __device__ __forceinline__ bool item_read() {  // the item's tile
+    if (item >= n_items) return false;
+    if (held != tile) {
+      held = tile;
+      t = tiles[tile];
+      left = t.y - quarter * 32;
+      rows = left <= 0 ? 0 : left >= 32 ? 32 : left;
+    }
+    return true;
+  }
+  __device__ __forceinline__ void next_item() {
+    ++item;
+    box = -1;
+    if (++column == across) {
+      column = 0;
+      ++tile;
+    }
+  }
+  // the next box of the item, if it has one
+  __device__ __forceinline__ bool next_box() {
+    if (rows == 0 || (t.z < 0 && in_place) || ++box == 64 / wide) return false;
+    col = column * kColumns + half * 64 + box * wide;
+    cols = min(wide, p.N - col);
+    return cols > 0;
+  }
+  // the next box of all
+  __device__ __forceinline__ bool next() {
+    while (item_read()) {
+      if (next_box()) return true;
+      next_item();
+    }
+    return false;
+  }
 };
 
 template <typename T, typename C, int kHalves>
-__global__ void __launch_bounds__(kColThreads, sizeof(C) == 2 && kHalves == 1 ? 2 : 1)
-    adapter_columns_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ AdapterParams p,
-                           const __grid_constant__ Work work) {
+__global__ void __launch_bounds__(kColThreads, 1)
+    adapter_columns_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c,
+                           const __grid_constant__ CUtensorMap map_out, const __grid_constant__ AdapterParams p, const __grid_constant__ Work work, const bool c_by_tma,
+                           const bool out_by_tma) {
   constexpr int kTerms = kTermsOf<T, C>;
   using L = ColumnsLayout<kTerms, kHalves>;
   constexpr int kStages = L::kStages;
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~static_cast<uintptr_t>(1023));
-  __shared__ uint64_t terms_full, terms_empty, b_full[kStages], b_empty[kStages], acc_full[2], acc_empty[2];
+  __shared__ uint64_t terms_full, terms_empty, b_full[kStages], b_empty[kStages], acc_full[2], acc_empty[2], box_full[kWriters * L::kBoxes];
   __shared__ uint32_t tmem_slot, abort_word;
   volatile uint32_t* abort_flag = &abort_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -241,10 +296,13 @@ __global__ void __launch_bounds__(kColThreads, sizeof(C) == 2 && kHalves == 1 ? 
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], kWriters);
     }
+    for (int i = 0; i < kWriters * L::kBoxes; ++i) mbar_init(&box_full[i], 1);
     abort_word = 0;
     mbar_fence_init();
     tma_prefetch_desc(&map_t);
     tma_prefetch_desc(&map_b);
+    if (c_by_tma) tma_prefetch_desc(&map_c);
+    if (out_by_tma) tma_prefetch_desc(&map_out);
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -347,88 +405,119 @@ __global__ void __launch_bounds__(kColThreads, sizeof(C) == 2 && kHalves == 1 ? 
       }
     }
   } else {
-    // A warp has 32 rows (its quarter of tensor memory) and 64 columns of an item, in two turns of 32.  In a turn a lane has a row's results out of tensor
-    // memory, then, through shared memory, 8 neighbours of rows lane / 4, lane / 4 + 8, ...: 64 bytes of a row are 4 lanes' accesses.
+    // A warp has 32 rows (its quarter of tensor memory) and 64 columns of an item.  Boxes of c come by TMA, kBoxes - 1 of them ahead; a lane adds the results of
+    // its row where c stands, and the box leaves by TMA, or row by row where the tile ends inside it.
     const int quarter = warp & 3, half = (warp - 2) >> 2;
-    float* turn = reinterpret_cast<float*>(smem + L::kTurnOffset) + (warp - 2) * 32 * kPitch;
+    constexpr int U = 128 / (int)sizeof(C), kBoxes = L::kBoxes;
+    unsigned char* boxes = smem + L::kBoxOffset + (warp - 2) * kBoxes * kBox;
+    uint64_t* bars = box_full + (warp - 2) * kBoxes;
     const C* const c = static_cast<const C*>(p.c);
     C* const out = static_cast<C*>(p.out);
-    const bool in_place = p.c == p.out;
-    int tile = tile0, column = col0, held = -1, acc = 0;
-    uint32_t acc_phase = 0;
-    int4 t = make_int4(0, 0, -1, 0);
-    float scale = 1.f, down[4] = {1.f, 1.f, 1.f, 1.f};  // (one after the other: their product may leave fp32's range)
-    for (int i = 0; i < n_items; ++i) {
-      if (held != tile) {
-        held = tile;
-        t = work.tiles[tile];
-        scale = t.z >= 0 && p.scales ? p.scales[t.z] : 1.f;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const int r = quarter * 32 + 8 * n + (lane >> 2);
-          if (std::is_same<T, __half>::value && t.z >= 0 && r < t.y) down[n] = work.down[t.x + r];
-        }
+    Way now(p, work.tiles, across, quarter, half, U, n_items, tile0, col0), ahead(p, work.tiles, across, quarter, half, U, n_items, tile0, col0);
+    int slot = 0, ahead_slot = 0, acc = 0;
+    uint32_t phases = 0, acc_phase = 0;
+    bool ok = true, more = c_by_tma;
+    auto fetch = [&]() {  // the next box ahead, into a slot that has been read and stored from
+      if (!more || !(more = ahead.next())) return;
+      if (lane == 0) {
+        mbar_expect_tx(&bars[ahead_slot], kBox);
+        tma_load_2d(boxes + ahead_slot * kBox, &map_c, &bars[ahead_slot], ahead.col, ahead.t.x + quarter * 32);
       }
-      const int first_col = column * kColumns + half * 64 + (lane & 3) * 8;
-      Eight<C> old[2][4];
-      if (t.z >= 0 || !in_place) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const int r = quarter * 32 + 8 * n + (lane >> 2), col = first_col + 32 * u;
-            old[u][n].load(c + (t.x + r) * p.ldc + col, r < t.y ? p.N - col : 0, p.wide);
-          }
+      ahead_slot = ahead_slot + 1 == kBoxes ? 0 : ahead_slot + 1;
+    };
+#pragma unroll 1
+    for (int i = 0; i + 1 < kBoxes; ++i) fetch();
+    int held = -1;
+    float scale = 1.f, down = 1.f;  // (one after the other: their product may leave fp32's range)
+    for (; ok && now.item_read(); now.next_item()) {
+      const bool product = now.t.z >= 0;
+      if (held != now.tile) {
+        held = now.tile;
+        scale = product && p.scales ? p.scales[now.t.z] : 1.f;
+        down = std::is_same<T, __half>::value && product && lane < now.rows ? work.down[now.t.x + quarter * 32 + lane] : 1.f;
       }
-      if (t.z >= 0) {
+      if (product) {
         if (!mbar_wait_warp(&acc_full[acc], acc_phase, abort_flag, p.status, ST_COLUMNS)) break;
         tc_fence_after_sync();
       }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (t.z >= 0) {
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(tmem + acc * kColumns + half * 64 + 32 * u + ((uint32_t)(quarter * 32) << 16), v);
-          tmem_ld_wait();
-          if (u == 1) {
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[acc]);
-          }
+      const uint32_t results = tmem + acc * kColumns + half * 64 + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+      while (now.next_box()) {
+        unsigned char* box = boxes + slot * kBox;
+        uint4* const mine = reinterpret_cast<uint4*>(box + lane * 128);
+        const int64_t row0 = now.t.x + quarter * 32;
+        if (c_by_tma) {
+          ok = mbar_wait_warp(&bars[slot], (phases >> slot) & 1, abort_flag, p.status, ST_COLUMNS);
+          if (!ok) break;
+          phases ^= 1u << slot;
+        } else {
+          if (lane == 0) tma_store_wait_read<0>();
           __syncwarp();
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<float4*>(turn + lane * kPitch + 4 * j) =
-                make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
+          load_box_rows(c + row0 * p.ldc + now.col, p.ldc, now.rows, now.cols, lane, [&](int r, uint32_t w) {
+            *reinterpret_cast<uint32_t*>(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = w;
+          });
           __syncwarp();
         }
+        if (product) {
+          constexpr int kEach = 16 / (int)sizeof(C);  // columns of 16 bytes
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const int r = quarter * 32 + 8 * n + (lane >> 2), col = first_col + 32 * u;
-          if (r >= t.y || col >= p.N || (t.z < 0 && in_place)) continue;
-          float y[8];
-          if (t.z >= 0) {
-            const float4* from = reinterpret_cast<const float4*>(turn + (8 * n + (lane >> 2)) * kPitch + (lane & 3) * 8);
-            const float4 a = from[0], b = from[1];
-            const float d[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+          for (int h = 0; h < U / 32; ++h) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(results + now.box * U + h * 32, v);
+            tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = fmaf(scale, std::is_same<T, __half>::value ? d[j] * down[n] : d[j], old[u][n][j]);
-          } else {
+            for (int j = 0; j < 32 / kEach; ++j) {
+              uint4& at = mine[(h * (32 / kEach) + j) ^ (lane & 7)];
+              const uint4 old = at;
+              uint32_t w[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = old[u][n][j];
+              for (int e = 0; e < 4; ++e) {
+                float2 f = gemm_detail::unpack_out<C>(word(old, e));
+                constexpr int kIn = kEach / 4;  // columns of a word
+                const float d0 = __uint_as_float(v[j * kEach + e * kIn]), d1 = __uint_as_float(v[j * kEach + e * kIn + kIn - 1]);
+                f.x = fmaf(scale, std::is_same<T, __half>::value ? d0 * down : d0, f.x);
+                f.y = fmaf(scale, std::is_same<T, __half>::value ? d1 * down : d1, f.y);
+                w[e] = gemm_detail::pack_out<C>(f.x, f.y);
+              }
+              at = make_uint4(w[0], w[1], w[2], w[3]);
+            }
           }
-          store_eight<C>(out + (t.x + r) * p.ldo + col, y, p.N - col, p.wide);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        // (not `rows == 32`: where rows is max(0, min(32, left)), nvcc 12.9 makes left <= 32 of it)
+        const bool whole = out_by_tma && now.left >= 32;
+        if (whole) {
+          if (lane == 0) {
+            tma_store_2d(&map_out, box, now.col, (int)row0);
+            tma_store_commit();
+          }
+        } else {
+          store_box_rows(out + row0 * p.ldo + now.col, p.ldo, now.rows, now.cols, lane,
+                         [&](int r) { return *reinterpret_cast<const uint32_t*>(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4); });
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        slot = slot + 1 == kBoxes ? 0 : slot + 1;
+        if (c_by_tma) {
+          // the box before this one has left: its slot is next
+          if (lane == 0 && whole) tma_store_wait_read<1>();
+          if (lane == 0 && !whole) tma_store_wait_read<0>();
+          __syncwarp();
+          fetch();
         }
       }
-      if (t.z >= 0 && ++acc == 2) {
-        acc = 0;
-        acc_phase ^= 1;
-      }
-      if (++column == across) {
-        column = 0;
-        ++tile;
+      if (product) {
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[acc]);
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
       }
     }
+    if (lane == 0) tma_store_wait<0>();  // the boxes are read and written out before the CTA leaves
   }
   __syncwarp();
   land(abort_flag);
@@ -443,17 +532,20 @@ __global__ void __launch_bounds__(kColThreads, sizeof(C) == 2 && kHalves == 1 ? 
 
 // ------------------------------------------------------------------------------------------------ launches
 template <typename... A>
-cudaError_t launch(void (*kernel)(A...), int64_t blocks, int threads, int smem, cudaStream_t s, const typename std::common_type<A>::type&... args) {
+cudaError_t launch(void (*kernel)(A...), int64_t blocks, int threads, int cluster, int smem, cudaStream_t s, const typename std::common_type<A>::type&... args) {
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernels wait (griddepcontrol.wait) themselves
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 template <typename K>
@@ -467,16 +559,22 @@ cudaError_t allow(PerDeviceOnce& once, int device, K kernel, int smem) {
 }
 
 template <typename T, typename C, int kHalves>
-int launch_both(frisk_b200_ctx* ctx, const AdapterParams& p, const Work& work, cudaStream_t s) {
+int launch_both(frisk_b200_ctx* ctx, AdapterParams p, const Work& work, cudaStream_t s) {
   constexpr int kTerms = kTermsOf<T, C>, dtype = std::is_same<T, __half>::value ? FRISK_B200_F16 : FRISK_B200_BF16;
   using L = ColumnsLayout<kTerms, kHalves>;
   const int width = (p.R + 15) / 16 * 16;
-  CUtensorMap map_x, map_a, map_t, map_b;
+  CUtensorMap map_x, map_a, map_t, map_b, map_c{}, map_out{};
   const int64_t a_step = p.count > 1 ? p.a_step : p.lda * p.R, b_step = p.count > 1 ? p.b_step : p.ldb * p.N;
   int bad = encode_tmap_2d(ctx, &map_x, dtype, p.x, p.K, p.rows, p.ldx * 2, 64, kRows, true);
   bad |= encode_tmap_3d(ctx, &map_a, dtype, p.a, p.K, p.R, p.count, p.lda * 2, a_step * 2, 64, width, 1, true);
   bad |= encode_tmap_3d(ctx, &map_t, dtype, work.terms, p.R, p.rows, kTerms, p.R * 2, p.rows * p.R * 2, 64, kRows, 1, true);
   bad |= encode_tmap_3d(ctx, &map_b, dtype, p.b, p.R, p.N, p.count, p.ldb * 2, b_step * 2, 64, kColumns, 1, true);
+  // c comes by TMA, and results leave by it, where rows begin on 16 bytes; a store clips at 16 bytes too
+  constexpr int dtype_c = sizeof(C) == 4 ? FRISK_B200_F32 : dtype, U = 128 / (int)sizeof(C);
+  const bool c_by_tma = (reinterpret_cast<uintptr_t>(p.c) & 15u) == 0 && p.ldc * (int64_t)sizeof(C) % 16 == 0;
+  const bool out_by_tma = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.ldo * (int64_t)sizeof(C) % 16 == 0 && p.N * (int64_t)sizeof(C) % 16 == 0;
+  if (c_by_tma) bad |= encode_tmap_2d(ctx, &map_c, dtype_c, p.c, p.N, p.rows, p.ldc * sizeof(C), U, 32, true);
+  if (out_by_tma) bad |= encode_tmap_2d(ctx, &map_out, dtype_c, p.out, p.N, p.rows, p.ldo * sizeof(C), U, 32, true);
   if (bad) return FRISK_B200_E_CUDA;
   static PerDeviceOnce once_sums, once_columns;
   auto sums = adapter_sums_kernel<T, kTerms>;
@@ -484,9 +582,10 @@ int launch_both(frisk_b200_ctx* ctx, const AdapterParams& p, const Work& work, c
   FB_CUDA(ctx, allow(once_sums, ctx->device, sums, SumsLayout::bytes(kMaxRank)));
   FB_CUDA(ctx, allow(once_columns, ctx->device, columns, L::kBytes));
   const int64_t tiles = most_tiles(p.rows, p.batch), items = tiles * ((p.N + kColumns - 1) / kColumns);
-  FB_CUDA(ctx, launch(sums, tiles * kCtas, kSumThreads, SumsLayout::bytes(width), s, map_x, map_a, p, work));
-  FB_CUDA(ctx, launch(columns, std::min<int64_t>(items, (int64_t)ctx->num_sms * (L::kBytes <= 113 * 1024 && sizeof(C) == 2 ? 2 : 1)), kColThreads, L::kBytes, s, map_t, map_b,
-                      p, work));
+  p.cluster = kMostCtas;
+  while (p.cluster > 2 && tiles * p.cluster > 2 * ctx->num_sms) p.cluster /= 2;
+  FB_CUDA(ctx, launch(sums, tiles * p.cluster, kSumThreads, p.cluster, SumsLayout::bytes(width), s, map_x, map_a, p, work));
+  FB_CUDA(ctx, launch(columns, std::min<int64_t>(items, ctx->num_sms), kColThreads, 1, L::kBytes, s, map_t, map_b, map_c, map_out, p, work, c_by_tma, out_by_tma));
   return 0;
 }
 
