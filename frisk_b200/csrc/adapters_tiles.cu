@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(kSumThreads)
 
 // ------------------------------------------------------------------------------------------------ columns
 constexpr int kColumns = 128;   // of an item
-constexpr int kWriters = 8;     // warps that add c and store
+constexpr int kWriters = 16;    // warps that add c and store, eight an item in turn
 constexpr int kColThreads = 64 + 32 * kWriters;
 constexpr int kBox = 32 * 128;   // bytes of a writer's box of c and results: 32 rows of 128 bytes
 
@@ -218,13 +218,13 @@ struct ColumnsLayout {
   static constexpr int kTermBytes = kTerms * kHalves * kBoxBytes;
   static constexpr int kStages = 2;
   static constexpr int kStageBytes = kHalves * kBoxBytes;
-  static constexpr int kBoxes = kHalves == 1 ? 4 : 2;  // of a writer
+  static constexpr int kBoxes = kHalves == 1 ? 2 : 1;  // of a writer, in flight or at work
   static constexpr int kBoxOffset = kTermBytes + kStages * kStageBytes;
   static constexpr int kBytes = kBoxOffset + kWriters * kBoxes * kBox + 1024;
   static_assert(kBytes <= 232448 - 1024, "shared memory of a CTA");
 };
 
-// A writer's way through its CTA's items: 32 rows and 64 columns of each, in boxes of kWide columns.  Boxes that hold nothing are left out.
+// A writer's way through its CTA's items, every other one: 32 rows and 64 columns of each, in boxes of `wide` columns.  Boxes that hold nothing are left out.
 struct Way {
   const AdapterParams& p;
   const int4* tiles;
@@ -233,9 +233,17 @@ struct Way {
   int item, tile, column, box, held;
   int4 t;       // the tile: first row, rows, adapter
   int left, rows, col, cols;  // of the box: the tile's rows from its first on; rows and columns that are there
-  __device__ __forceinline__ Way(const AdapterParams& p, const int4* tiles, int across, int quarter, int half, int wide, int n_items, int tile, int column)
-      : p(p), tiles(tiles), across(across), quarter(quarter), half(half), wide(wide), n_items(n_items), in_place(p.c == p.out), item(0), tile(tile), column(column), box(-1),
-        held(-1), t(make_int4(0, 0, -1, 0)) {}
+  __device__ __forceinline__ Way(const AdapterParams& p, const int4* tiles, int across, int quarter, int half, int wide, int n_items, int tile, int column, int turn)
+      : p(p), tiles(tiles), across(across), quarter(quarter), half(half), wide(wide), n_items(n_items), in_place(p.c == p.out), item(turn), tile(tile), column(column + turn), box(-1),
+        held(-1), t(make_int4(0, 0, -1, 0)) {
+    wrap();
+  }
+  __device__ __forceinline__ void wrap() {
+    while (column >= across) {
+      column -= across;
+      ++tile;
+    }
+  }
   __device__ __forceinline__ bool item_read() {  // the item's tile
     if (item >= n_items) return false;
     if (held != tile) {
@@ -247,12 +255,10 @@ struct Way {
     return true;
   }
   __device__ __forceinline__ void next_item() {
-    ++item;
+    item += 2;
+    column += 2;
     box = -1;
-    if (++column == across) {
-      column = 0;
-      ++tile;
-    }
+    wrap();
   }
   // the next box of the item, if it has one
   __device__ __forceinline__ bool next_box() {
@@ -294,7 +300,7 @@ __global__ void __launch_bounds__(kColThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], kWriters);
+      mbar_init(&acc_empty[i], kWriters / 2);
     }
     for (int i = 0; i < kWriters * L::kBoxes; ++i) mbar_init(&box_full[i], 1);
     abort_word = 0;
@@ -362,8 +368,8 @@ __global__ void __launch_bounds__(kColThreads, 1)
     constexpr uint32_t idesc = umma_idesc_f16(kRows, kColumns, std::is_same<T, __nv_bfloat16>::value, false, false);
     const uint32_t d = __shfl_sync(0xffffffffu, tmem, 0);
     const int steps = (p.R + 15) / 16;
-    int tile = tile0, column = col0, held = -1, which = -1, stage = 0, acc = 0;
-    uint32_t phase = 0, terms_phase = 0, acc_phase = 0;
+    int tile = tile0, column = col0, held = -1, which = -1, stage = 0;
+    uint32_t phase = 0, terms_phase = 0, acc_phases = 0;
     for (int i = 0; i < n_items; ++i) {
       if (held != tile) {
         held = tile;
@@ -374,7 +380,9 @@ __global__ void __launch_bounds__(kColThreads, 1)
         }
       }
       if (which >= 0) {
-        if (!mbar_wait_warp(&acc_empty[acc], acc_phase ^ 1, abort_flag, p.status, ST_COLUMNS)) break;
+        const int acc = i & 1;  // (whose writers take the item)
+        if (!mbar_wait_warp(&acc_empty[acc], (acc_phases >> acc & 1) ^ 1, abort_flag, p.status, ST_COLUMNS)) break;
+        acc_phases ^= 1u << acc;
         if (!mbar_wait_warp(&b_full[stage], phase, abort_flag, p.status, ST_COLUMNS)) break;
         tc_fence_after_sync();
         const uint32_t at = smem_u32(smem), b = at + L::kTermBytes + stage * L::kStageBytes;
@@ -394,10 +402,6 @@ __global__ void __launch_bounds__(kColThreads, 1)
           stage = 0;
           phase ^= 1;
         }
-        if (++acc == 2) {
-          acc = 0;
-          acc_phase ^= 1;
-        }
       }
       if (++column == across) {
         column = 0;
@@ -405,16 +409,17 @@ __global__ void __launch_bounds__(kColThreads, 1)
       }
     }
   } else {
-    // A warp has 32 rows (its quarter of tensor memory) and 64 columns of an item.  Boxes of c come by TMA, kBoxes - 1 of them ahead; a lane adds the results of
-    // its row where c stands, and the box leaves by TMA, or row by row where the tile ends inside it.
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    // Eight warps have the even items, eight the odd ones (one after the other they would take the time of each box's chain of waits, 1.9 us, for each item).  A warp
+    // has 32 rows (its quarter of tensor memory) and 64 columns.  Boxes of c come by TMA, the next while one is at work; a lane adds the results of its row
+    // where c stands; eight rows leave at a time, by TMA, and those of a tile that ends among eight one by one.
+    const int quarter = warp & 3, half = (warp - 2) >> 2 & 1, acc = (warp - 2) >> 3;
     constexpr int U = 128 / (int)sizeof(C), kBoxes = L::kBoxes;
     unsigned char* boxes = smem + L::kBoxOffset + (warp - 2) * kBoxes * kBox;
     uint64_t* bars = box_full + (warp - 2) * kBoxes;
     const C* const c = static_cast<const C*>(p.c);
     C* const out = static_cast<C*>(p.out);
-    Way now(p, work.tiles, across, quarter, half, U, n_items, tile0, col0), ahead(p, work.tiles, across, quarter, half, U, n_items, tile0, col0);
-    int slot = 0, ahead_slot = 0, acc = 0;
+    Way now(p, work.tiles, across, quarter, half, U, n_items, tile0, col0, acc), ahead(p, work.tiles, across, quarter, half, U, n_items, tile0, col0, acc);
+    int slot = 0, ahead_slot = 0;
     uint32_t phases = 0, acc_phase = 0;
     bool ok = true, more = c_by_tma;
     auto fetch = [&]() {  // the next box ahead, into a slot that has been read and stored from
@@ -426,7 +431,7 @@ __global__ void __launch_bounds__(kColThreads, 1)
       ahead_slot = ahead_slot + 1 == kBoxes ? 0 : ahead_slot + 1;
     };
 #pragma unroll 1
-    for (int i = 0; i + 1 < kBoxes; ++i) fetch();
+    for (int i = 0; i < kBoxes; ++i) fetch();
     int held = -1;
     float scale = 1.f, down = 1.f;  // (one after the other: their product may leave fp32's range)
     for (; ok && now.item_read(); now.next_item()) {
@@ -451,8 +456,6 @@ __global__ void __launch_bounds__(kColThreads, 1)
           if (!ok) break;
           phases ^= 1u << slot;
         } else {
-          if (lane == 0) tma_store_wait_read<0>();
-          __syncwarp();
           load_box_rows(c + row0 * p.ldc + now.col, p.ldc, now.rows, now.cols, lane, [&](int r, uint32_t w) {
             *reinterpret_cast<uint32_t*>(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = w;
           });
@@ -485,39 +488,31 @@ __global__ void __launch_bounds__(kColThreads, 1)
         }
         fence_proxy_async_smem();
         __syncwarp();
-        // (not `rows == 32`: where rows is max(0, min(32, left)), nvcc 12.9 makes left <= 32 of it)
-        const bool whole = out_by_tma && now.left >= 32;
-        if (whole) {
-          if (lane == 0) {
-            tma_store_2d(&map_out, box, now.col, (int)row0);
-            tma_store_commit();
-          }
-        } else {
-          store_box_rows(out + row0 * p.ldo + now.col, p.ldo, now.rows, now.cols, lane,
-                         [&](int r) { return *reinterpret_cast<const uint32_t*>(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4); });
+        // (`rows` is not clamped by max(0, min(32, left)): nvcc 12.9 made left <= 32 of a comparison of that with 32)
+        const int by_tma = out_by_tma ? now.rows & ~7 : 0;
+        if (lane < 4 && 8 * lane < by_tma) {
+          tma_store_2d(&map_out, box + lane * 1024, now.col, (int)row0 + 8 * lane);
+          tma_store_commit();
+        }
+        if (by_tma < now.rows) {
+          store_box_rows(out + (row0 + by_tma) * p.ldo + now.col, p.ldo, now.rows - by_tma, now.cols, lane, [&](int r) {
+            return *reinterpret_cast<const uint32_t*>(box + (by_tma + r) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+          });
           fence_proxy_async_smem();
-          __syncwarp();
         }
+        if (lane < 4) tma_store_wait_read<0>();
+        __syncwarp();
         slot = slot + 1 == kBoxes ? 0 : slot + 1;
-        if (c_by_tma) {
-          // the box before this one has left: its slot is next
-          if (lane == 0 && whole) tma_store_wait_read<1>();
-          if (lane == 0 && !whole) tma_store_wait_read<0>();
-          __syncwarp();
-          fetch();
-        }
+        fetch();
       }
       if (product) {
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&acc_empty[acc]);
-        if (++acc == 2) {
-          acc = 0;
-          acc_phase ^= 1;
-        }
+        acc_phase ^= 1;
       }
     }
-    if (lane == 0) tma_store_wait<0>();  // the boxes are read and written out before the CTA leaves
+    if (lane < 4) tma_store_wait<0>();  // the boxes are read and written out before the CTA leaves
   }
   __syncwarp();
   land(abort_flag);
@@ -574,7 +569,7 @@ int launch_both(frisk_b200_ctx* ctx, AdapterParams p, const Work& work, cudaStre
   const bool c_by_tma = (reinterpret_cast<uintptr_t>(p.c) & 15u) == 0 && p.ldc * (int64_t)sizeof(C) % 16 == 0;
   const bool out_by_tma = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.ldo * (int64_t)sizeof(C) % 16 == 0 && p.N * (int64_t)sizeof(C) % 16 == 0;
   if (c_by_tma) bad |= encode_tmap_2d(ctx, &map_c, dtype_c, p.c, p.N, p.rows, p.ldc * sizeof(C), U, 32, true);
-  if (out_by_tma) bad |= encode_tmap_2d(ctx, &map_out, dtype_c, p.out, p.N, p.rows, p.ldo * sizeof(C), U, 32, true);
+  if (out_by_tma) bad |= encode_tmap_2d(ctx, &map_out, dtype_c, p.out, p.N, p.rows, p.ldo * sizeof(C), U, 8, true);
   if (bad) return FRISK_B200_E_CUDA;
   static PerDeviceOnce once_sums, once_columns;
   auto sums = adapter_sums_kernel<T, kTerms>;
