@@ -395,7 +395,7 @@ def adapter_workspace_bytes(desc):
 
 
 def cache_pages_workspace_bytes(cache, which):
-    """Bytes ``Context.cache_pages`` needs; 0 for what it refuses.  Host-only."""
+    """Bytes ``Context.cache_pages`` needs; 0: none, or refused.  Host-only."""
     return load().frisk_b200_cache_pages_workspace_bytes(cache, which)
 
 

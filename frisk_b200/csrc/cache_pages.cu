@@ -4,7 +4,8 @@
 // device, so that a captured step is replayed with other contents, and every result follows from them alone: pages are taken lowest
 // first, by sequences in their order, whatever the order of threads.
 //
-// fork     row b of the table becomes the old row parents[b], its entries behind the last key -1; users follow by integer atomics
+// fork     row b of the table becomes the old row parents[b], its entries behind the last key -1; users follow by integer atomics.  A cluster reads all
+//          and then writes all, or (larger tables) two launches and a workspace do
 // grow     one CTA plans: the slots that new tokens touch, in order of (sequence, slot), take the free pages in order (block scans); then
 //          a second kernel copies the keys of last pages that were shared
 // compact  one CTA pairs the k-th used page behind the first n (n: used pages) with the k-th free one among them; then all copy
@@ -72,43 +73,55 @@ __device__ __forceinline__ int block_scan(int x, int* sums, int* total) {
   return incl - x + (warp ? before : 0);
 }
 
-// ------------------------------------------------------------------------------------------------ fork
-// The new table into the workspace: [batch][width], then the lengths [batch].  (The old one is still read, by other rows too.)
-__global__ void __launch_bounds__(kMove) fork_stage_kernel(const PageTables t) {
-  pdl_begin();
-  const int64_t i = (int64_t)blockIdx.x * kMove + threadIdx.x, slots = (int64_t)t.batch * t.width;
-  if (t.users_out != t.users)
-    for (int64_t p = i; p < t.pages; p += (int64_t)gridDim.x * kMove) t.users_out[p] = t.users[p];
-  if (i < t.batch) {
-    const int parent = t.parents[i];
-    const bool known = parent >= -1 && parent < t.batch;
-    const int length = t.lengths[known && parent >= 0 ? parent : i];
-    const bool ok = known && (parent < 0 || (length >= 0 && length <= (int64_t)t.width * t.page));
-    if (!ok) flag(t.status, known ? ST_CACHE_LENGTH : ST_CACHE_ROWS);
-    t.ws[slots + i] = ok ? (parent < 0 ? 0 : length) : t.lengths[i];
+// What is not done in place, eight entries in flight: the compiler cannot tell that a store does not change what is still to be read.
+constexpr int kDeep = 8;
+__device__ __forceinline__ void copy_users(const PageTables& t, int64_t first, int64_t step) {
+  if (t.users_out == t.users) return;
+  for (int64_t p0 = first; p0 < t.pages; p0 += kDeep * step) {
+    int x[kDeep];
+#pragma unroll
+    for (int j = 0; j < kDeep; ++j)
+      if (p0 + j * step < t.pages) x[j] = t.users[p0 + j * step];
+#pragma unroll
+    for (int j = 0; j < kDeep; ++j)
+      if (p0 + j * step < t.pages) t.users_out[p0 + j * step] = x[j];
   }
-  if (i >= slots) return;
-  const int b = (int)(i / t.width), slot = (int)(i - (int64_t)b * t.width);
-  const int parent = t.parents[b];
-  int entry;
-  if (parent < -1 || parent >= t.batch) {
-    entry = t.table[b * t.stride + slot];
-  } else if (parent < 0) {
-    entry = -1;
-  } else {
-    const int length = t.lengths[parent];
-    if (length < 0 || length > (int64_t)t.width * t.page) entry = t.table[b * t.stride + slot];
-    else entry = (int64_t)slot << t.page_log2 < length ? t.table[parent * t.stride + slot] : -1;
-  }
-  t.ws[i] = entry < 0 ? -1 : entry;
 }
-__global__ void __launch_bounds__(kMove) fork_apply_kernel(const PageTables t) {
-  pdl_begin();
-  const int64_t i = (int64_t)blockIdx.x * kMove + threadIdx.x, slots = (int64_t)t.batch * t.width;
-  if (i < t.batch) t.lengths_out[i] = t.ws[slots + i];
-  if (i >= slots) return;
-  const int b = (int)(i / t.width), slot = (int)(i - (int64_t)b * t.width);
-  const int old = t.table[b * t.stride + slot], entry = t.ws[i];
+__device__ __forceinline__ void copy_table(const PageTables& t, int64_t first, int64_t step) {
+  if (t.table_out == t.table) return;
+  const uint32_t slots = (uint32_t)t.batch * t.width, width = max(t.width, 1);
+  for (uint32_t i0 = (uint32_t)first; i0 < slots; i0 += kDeep * (uint32_t)step) {
+    int x[kDeep];
+#pragma unroll
+    for (int j = 0; j < kDeep; ++j) {
+      const uint32_t i = i0 + j * (uint32_t)step, b = i / width;
+      if (i < slots) x[j] = t.table[b * t.stride + i - b * width];
+    }
+#pragma unroll
+    for (int j = 0; j < kDeep; ++j) {
+      const uint32_t i = i0 + j * (uint32_t)step, b = i / width;
+      if (i < slots) t.table_out[b * t.out_stride + i - b * width] = x[j];
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ fork
+// The row that slot `slot` of row b comes from, of its parent and the parent's length; -1: from none
+__device__ __forceinline__ int forked_from(const PageTables& t, int b, int slot, int parent, int length) {
+  if (parent < -1 || parent >= t.batch) return b;  // (said where the lengths are made)
+  if (parent < 0) return -1;
+  if (length < 0 || length > (int64_t)t.width * t.page) return b;
+  return (int64_t)slot << t.page_log2 >= length ? -1 : parent;
+}
+__device__ __forceinline__ int forked_length(const PageTables& t, int b) {
+  const int parent = t.parents[b];
+  const bool known = parent >= -1 && parent < t.batch;
+  const int length = t.lengths[known && parent >= 0 ? parent : b];
+  const bool ok = known && (parent < 0 || (length >= 0 && length <= (int64_t)t.width * t.page));
+  if (!ok) flag(t.status, known ? ST_CACHE_LENGTH : ST_CACHE_ROWS);
+  return !ok ? t.lengths[b] : parent < 0 ? 0 : length;
+}
+__device__ __forceinline__ void apply_fork(const PageTables& t, int b, int slot, int old, int entry) {
   if (old != entry) {
     if (old >= t.pages || entry >= t.pages) flag(t.status, ST_CACHE_PAGE);
     if (old >= 0 && old < t.pages) atomicSub(t.users_out + old, 1);
@@ -117,17 +130,76 @@ __global__ void __launch_bounds__(kMove) fork_apply_kernel(const PageTables t) {
   t.table_out[b * t.out_stride + slot] = entry;
 }
 
+// Tables that one cluster's threads can hold: all is read, then all is written.  (16 rows of 34 pages 5.7 us, in two launches 6.4 and more of the host; 192 rows of
+// 378 pages 13.9, in two launches 7.8: eight SMs have too many instructions to do.)
+constexpr int kTogether = 8, kHeldSlots = 4;
+constexpr int64_t kForkTogether = (int64_t)kTogether * kPlan * kHeldSlots;
+__global__ void __launch_bounds__(kPlan) fork_kernel(const PageTables t) {
+  pdl_begin();
+  constexpr int kStep = kTogether * kPlan;
+  const int first = blockIdx.x * kPlan + threadIdx.x, slots = t.batch * t.width;
+  copy_users(t, first, kStep);
+  // (in steps of their own, so that the loads of all slots are on their way at once)
+  int old[kHeldSlots], entry[kHeldSlots], parent[kHeldSlots];
+#pragma unroll
+  for (int j = 0; j < kHeldSlots; ++j) {
+    const int i = first + j * kStep, b = i / max(t.width, 1);
+    if (i < slots) parent[j] = t.parents[b];
+  }
+#pragma unroll
+  for (int j = 0; j < kHeldSlots; ++j) {
+    const int i = first + j * kStep, b = i / max(t.width, 1);
+    if (i < slots) {
+      old[j] = t.table[b * t.stride + i - b * t.width];
+      entry[j] = t.lengths[parent[j] >= 0 && parent[j] < t.batch ? parent[j] : b];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kHeldSlots; ++j) {
+    const int i = first + j * kStep, b = i / max(t.width, 1);
+    if (i < slots) {
+      const int slot = i - b * t.width, from = forked_from(t, b, slot, parent[j], entry[j]);
+      entry[j] = from < 0 ? -1 : max(t.table[from * t.stride + slot], -1);
+    }
+  }
+  const int length = first < t.batch ? forked_length(t, first) : 0;
+  cluster_sync_all();
+  if (first < t.batch) t.lengths_out[first] = length;
+#pragma unroll
+  for (int j = 0; j < kHeldSlots; ++j) {
+    const int i = first + j * kStep;
+    if (i >= slots) break;
+    const int b = i / t.width;
+    apply_fork(t, b, i - b * t.width, old[j], entry[j]);
+  }
+}
+
+// Larger ones.  The new table into the workspace: [batch][width], then the lengths [batch].  (The old one is still read, by other rows too.)
+__global__ void __launch_bounds__(kMove) fork_stage_kernel(const PageTables t) {
+  pdl_begin();
+  const int64_t i = (int64_t)blockIdx.x * kMove + threadIdx.x, slots = (int64_t)t.batch * t.width;
+  if (t.users_out != t.users)
+    for (int64_t p = i; p < t.pages; p += (int64_t)gridDim.x * kMove) t.users_out[p] = t.users[p];
+  if (i < t.batch) t.ws[slots + i] = forked_length(t, (int)i);
+  if (i >= slots) return;
+  const int b = (int)(i / t.width), slot = (int)(i - (int64_t)b * t.width), parent = t.parents[b];
+  const int from = forked_from(t, b, slot, parent, t.lengths[parent >= 0 && parent < t.batch ? parent : b]);
+  t.ws[i] = from < 0 ? -1 : max(t.table[from * t.stride + slot], -1);
+}
+__global__ void __launch_bounds__(kMove) fork_apply_kernel(const PageTables t) {
+  pdl_begin();
+  const int64_t i = (int64_t)blockIdx.x * kMove + threadIdx.x, slots = (int64_t)t.batch * t.width;
+  if (i < t.batch) t.lengths_out[i] = t.ws[slots + i];
+  if (i >= slots) return;
+  const int b = (int)(i / t.width), slot = (int)(i - (int64_t)b * t.width);
+  apply_fork(t, b, slot, t.table[b * t.stride + slot], t.ws[i]);
+}
+
 // ------------------------------------------------------------------------------------------------ grow
 __global__ void __launch_bounds__(kMove) copy_tables_kernel(const PageTables t) {
   pdl_begin();
-  const int64_t first = (int64_t)blockIdx.x * kMove + threadIdx.x, step = (int64_t)gridDim.x * kMove, slots = (int64_t)t.batch * t.width;
-  if (t.users_out != t.users)
-    for (int64_t p = first; p < t.pages; p += step) t.users_out[p] = t.users[p];
-  if (t.table_out != t.table)
-    for (int64_t i = first; i < slots; i += step) {
-      const int64_t b = i / t.width;
-      t.table_out[b * t.out_stride + i - b * t.width] = t.table[b * t.stride + i - b * t.width];
-    }
+  copy_users(t, (int64_t)blockIdx.x * kMove + threadIdx.x, (int64_t)gridDim.x * kMove);
+  copy_table(t, (int64_t)blockIdx.x * kMove + threadIdx.x, (int64_t)gridDim.x * kMove);
 }
 
 // What becomes of a touched slot
@@ -141,6 +213,7 @@ struct GrowWork {
   int *kind, *before;  // [T], [T + 1]: what becomes of the slot; pages taken by those before it
   int *shared, *page;  // [T]: touched slots whose page others have too, and the page
   int *free;           // [T]
+  static constexpr int kSmall = 1536;  // touched slots whose lists are in shared memory
   __host__ __device__ static int64_t ints(int64_t batch, int64_t width) { return 5 * batch + 1 + 5 * batch * width + 1; }
   __device__ GrowWork(int* ws, int64_t batch, int64_t width) {
     const int64_t slots = batch * width;
@@ -155,12 +228,21 @@ struct GrowWork {
   }
 };
 
+// COPIES: a cluster copies the tables that are not changed in place, then its first CTA plans
+template <bool COPIES>
 __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
   __shared__ int sums[32];
   __shared__ int near[kSearched + 1];  // offsets, where they fit
-  const GrowWork w(t.ws, t.batch, t.width);
+  extern __shared__ int lists[];       // five of kSmall, and one place
+  GrowWork w(t.ws, t.batch, t.width);
   const int tid = threadIdx.x, lane = tid & 31;
   pdl_begin();
+  if (COPIES) {
+    copy_users(t, (int64_t)blockIdx.x * kPlan + tid, (int64_t)gridDim.x * kPlan);
+    copy_table(t, (int64_t)blockIdx.x * kPlan + tid, (int64_t)gridDim.x * kPlan);
+    cluster_sync_all();
+    if (blockIdx.x > 0) return;
+  }
   // 1. the slots that each sequence's new tokens touch
   int all = 0;
   for (int b0 = 0; b0 < t.batch; b0 += kPlan) {
@@ -190,6 +272,13 @@ __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
   }
   __syncthreads();
   const int* offset = t.batch <= kSearched ? near : w.offset;
+  if (all <= GrowWork::kSmall) {
+    w.kind = lists;
+    w.before = w.kind + GrowWork::kSmall;
+    w.shared = w.before + GrowWork::kSmall + 1;
+    w.page = w.shared + GrowWork::kSmall;
+    w.free = w.page + GrowWork::kSmall;
+  }
   auto owner = [&](int i) {  // the last b with offset[b] <= i: the one whose slot it is
     int lo = 0, hi = t.batch;
     while (hi - lo > 1) {
@@ -225,6 +314,7 @@ __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
   for (int k = tid; k < n_shared; k += kPlan) {
     const int page = w.page[k];
     int earlier = 0;
+#pragma unroll 8
     for (int j = 0; j < k; ++j) earlier += w.page[j] == page;
     const int i = w.shared[k];
     if (t.users_out[page] - earlier > 1) w.kind[i] = SWAP;
@@ -513,17 +603,25 @@ __global__ void __launch_bounds__(kMove) keep_kernel(const KeepParams p) {
 
 // ------------------------------------------------------------------------------------------------ launches
 template <typename... A>
-cudaError_t launch(void (*kernel)(A...), int64_t blocks, int threads, cudaStream_t s, typename std::common_type<A>::type... args) {
+cudaError_t launch_with(void (*kernel)(A...), int64_t blocks, int threads, int smem, cudaStream_t s, typename std::common_type<A>::type... args) {
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernels wait (griddepcontrol.wait) themselves
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;  // planning CTAs, where there are several
+  attr[1].val.clusterDim.x = kTogether;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3((unsigned)threads);
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = threads == kPlan && blocks == kTogether ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+template <typename... A>
+cudaError_t launch(void (*kernel)(A...), int64_t blocks, int threads, cudaStream_t s, typename std::common_type<A>::type... args) {
+  return launch_with(kernel, blocks, threads, 0, s, args...);
 }
 
 size_t element(const frisk_b200_cache_desc* c) { return c->dtype == FRISK_B200_E4M3 ? 1 : 2; }
@@ -581,8 +679,10 @@ int check_ranges(const Range* r, int n) {
 size_t table_bytes(int64_t batch, int64_t width, int64_t stride) { return batch > 0 && width > 0 ? (size_t)((batch - 1) * stride + width) * 4 : 0; }
 
 enum Which { FORK, GROW, COMPACT };
+constexpr int64_t kCopiedTogether = 1 << 17;  // entries that a cluster copies in a few microseconds
 int64_t workspace_ints(const frisk_b200_cache_desc* c, int which) {
   const int64_t batch = c->batch, width = c->table_width;
+  if (which == FORK && batch * width <= kForkTogether && batch <= kTogether * kPlan && c->pages <= kCopiedTogether) return 0;
   return which == FORK ? batch * width + batch : which == GROW ? GrowWork::ints(batch, width) : 1 + 3 * c->pages;
 }
 int check_sizes(const frisk_b200_cache_desc* c, int which) {
@@ -600,9 +700,9 @@ int prepare(const frisk_b200_ctx* ctx, const frisk_b200_cache_desc* c, const fri
   int rc = check_sizes(c, which);
   if (rc) return rc;
   if (c->batch > 1 && t->table_out_stride < c->table_width) return FRISK_B200_E_CACHE_SHAPE;
-  if (t->table_out == c->table && c->batch > 1 && t->table_out_stride != c->table_stride) return FRISK_B200_E_OVERLAP;
+  if (t->table_out == c->table && c->batch > 1 && c->table_width > 0 && t->table_out_stride != c->table_stride) return FRISK_B200_E_OVERLAP;
   const size_t need = (size_t)workspace_ints(c, which) * 4, batch = (size_t)c->batch * 4, pages = (size_t)c->pages * 4;
-  if (!ws || ws_bytes < need) return FRISK_B200_E_WORKSPACE;
+  if (need && (!ws || ws_bytes < need)) return FRISK_B200_E_WORKSPACE;
   const Range all[] = {
       {t->users, pages, false, nullptr},
       {c->table, table_bytes(c->batch, c->table_width, c->table_stride), false, nullptr},
@@ -666,6 +766,10 @@ int frisk_b200_cache_fork(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* c, c
   FB_DEVICE(ctx);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t slots = (int64_t)t.batch * t.width, work = std::max<int64_t>(slots, t.batch);
+  if (workspace_ints(c, FORK) == 0) {
+    FB_CUDA(ctx, launch(fork_kernel, kTogether, kPlan, s, t));
+    return 0;
+  }
   FB_CUDA(ctx, launch(fork_stage_kernel, std::max<int64_t>(blocks_for(work), blocks_up_to(ctx, t.users_out != t.users ? blocks_for(t.pages) : 1)), kMove, s, t));
   FB_CUDA(ctx, launch(fork_apply_kernel, std::max<int64_t>(1, blocks_for(work)), kMove, s, t));
   return 0;
@@ -678,9 +782,12 @@ int frisk_b200_cache_grow(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* c, c
   FB_DEVICE(ctx);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t slots = (int64_t)t.batch * t.width;
-  if (t.users_out != t.users || t.table_out != t.table)
-    FB_CUDA(ctx, launch(copy_tables_kernel, blocks_up_to(ctx, blocks_for(std::max<int64_t>(t.pages, slots))), kMove, s, t));
-  FB_CUDA(ctx, launch(grow_plan_kernel, 1, kPlan, s, t));
+  const bool copies = t.users_out != t.users || t.table_out != t.table, together = copies && t.pages + slots <= kCopiedTogether;
+  if (copies && !together) FB_CUDA(ctx, launch(copy_tables_kernel, blocks_up_to(ctx, blocks_for(std::max<int64_t>(t.pages, slots))), kMove, s, t));
+  constexpr int kLists = (5 * GrowWork::kSmall + 1) * 4;
+  static_assert(kLists + (kSearched + 1) * 4 + 256 <= 48 * 1024, "what any kernel may have");
+  if (together) FB_CUDA(ctx, launch_with(grow_plan_kernel<true>, kTogether, kPlan, kLists, s, t));
+  else FB_CUDA(ctx, launch_with(grow_plan_kernel<false>, 1, kPlan, kLists, s, t));
   const Held h = held_of(c);
   if (t.batch > 0 && t.width > 0)
     FB_CUDA(ctx, launch(grow_copy_kernel, (int64_t)t.batch * c->heads, kMove, s, t.ws, reinterpret_cast<uint4*>(h.part[0]), reinterpret_cast<uint4*>(h.part[1]), h.part[2],

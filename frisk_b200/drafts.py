@@ -1,4 +1,6 @@
 """Verification of drafted tokens: ``draft_verify``."""
+import contextlib
+
 from . import capi
 from .cache import _on_stream, _stream_of
 from .execute import _torch, context_for
@@ -8,9 +10,14 @@ def _refuse(what):
     raise ValueError("frisk-b200-draft: " + what)
 
 
-def _list(t, n, kinds, dev, what):
-    if t.dtype not in kinds or t.shape != (n,) or t.get_device() != dev or not t.is_contiguous():
-        _refuse(f"{what} must be dense, {' or '.join(str(k)[6:] for k in kinds)} [{n}], on the probabilities' device")
+_KINDS = None
+_NOTHING = contextlib.nullcontext()
+
+
+def _list(t, n, kind, dev, what):
+    shape = t.shape
+    if t.dtype != kind or len(shape) != 1 or shape[0] != n or t.get_device() != dev or not t.is_contiguous():
+        _refuse(f"{what} must be dense {str(kind)[6:]} [{n}] on the probabilities' device")
     return t.data_ptr()
 
 
@@ -31,35 +38,43 @@ def draft_verify(tokens, parents, starts, target, draft, accept, sample, *, max_
     ``kept[b, :counts[b]]`` are the nodes that stand, node 0 first, -1 behind them: what ``cache_keep`` takes.  A sequence without rows has count 0
     and next -1, as one with more than ``max_new`` (1 to 1024) rows or rows out of range, for which ``cache_check`` raises.  Probabilities that are NaN or
     negative count as 0."""
-    torch = _torch()
-    code = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}.get(target.dtype)
-    shape, dev = target.shape, target.get_device()
-    if code is None or len(shape) != 2 or (target.stride(1) != 1 and shape[1] > 1):
-        _refuse("target must be float32, float16 or bfloat16 [rows, vocabulary] with dense rows")
+    global _KINDS
+    if _KINDS is None:
+        torch = _torch()
+        _KINDS = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}, torch.int32, torch.int64, torch.float32
+    codes, i32, i64, f32 = _KINDS
+    dtype, shape, dev = target.dtype, target.shape, target.get_device()
+    code = codes.get(dtype)
+    if code is None or len(shape) != 2:
+        _refuse("target must be float32, float16 or bfloat16 [rows, vocabulary]")
+    rows, vocab = shape
+    step, dense = target.stride()
+    if dense != 1 and vocab > 1:
+        _refuse("the rows of target must be dense")
     if dev < 0:
         _refuse("tensors must be on one CUDA device (there is no CPU path)")
-    if draft is not None and (draft.dtype != target.dtype or draft.shape != shape or draft.get_device() != dev or (draft.stride(1) != 1 and shape[1] > 1)):
-        _refuse("draft must have the type, shape and device of target, and dense rows")
-    rows, vocab = shape
-    batch = starts.shape[0] - 1 if starts.dim() == 1 else -1
-    if batch < 0:
+    p_draft, draft_step = None, 0
+    if draft is not None:
+        if draft.dtype != dtype or draft.shape != shape or draft.get_device() != dev:
+            _refuse("draft must have the type, shape and device of target")
+        draft_step, dense = draft.stride()
+        if dense != 1 and vocab > 1:
+            _refuse("the rows of draft must be dense")
+        p_draft = draft.data_ptr()
+    if starts.dim() != 1 or starts.shape[0] < 1:
         _refuse("starts must be int32 [batch + 1]")
-    p_tokens = _list(tokens, rows, (torch.int64, torch.int32), dev, "tokens")
-    p_parents = None if parents is None else _list(parents, rows, (torch.int32,), dev, "parents")
-    p_starts = _list(starts, batch + 1, (torch.int32,), dev, "starts")
-    p_accept, p_sample = _list(accept, rows, (torch.float32,), dev, "accept"), _list(sample, batch, (torch.float32,), dev, "sample")
+    batch, kind = starts.shape[0] - 1, tokens.dtype
+    if kind != i64 and kind != i32:
+        _refuse("tokens must be int32 or int64")
+    p_tokens = _list(tokens, rows, kind, dev, "tokens")
+    p_parents = None if parents is None else _list(parents, rows, i32, dev, "parents")
+    p_starts = _list(starts, batch + 1, i32, dev, "starts")
+    p_accept, p_sample = _list(accept, rows, f32, dev, "accept"), _list(sample, batch, f32, dev, "sample")
     if not 1 <= max_new <= 1024:
         _refuse("max_new must be between 1 and 1024")
-
-    def new():
-        return starts.new_empty((batch, max_new)), starts.new_empty(batch), tokens.new_empty(batch)
-
-    if stream is None:
-        kept, counts, token = new()
-    else:
-        with _on_stream(stream, target.device):
-            kept, counts, token = new()
-    desc = capi.VerifyDesc(rows, target.stride(0), 0 if draft is None else draft.stride(0), batch, max_new, vocab, code, tokens.dtype == torch.int64)
-    context_for(dev).draft_verify(desc, p_tokens, p_parents, p_starts, target.data_ptr(), None if draft is None else draft.data_ptr(), p_accept, p_sample,
-                                  kept.data_ptr(), counts.data_ptr(), token.data_ptr(), _stream_of(stream, dev))
+    with _NOTHING if stream is None else _on_stream(stream, target.device):
+        kept, counts, token = starts.new_empty((batch, max_new)), starts.new_empty(batch), tokens.new_empty(batch)
+    desc = capi.VerifyDesc(rows, step, draft_step, batch, max_new, vocab, code, kind == i64)
+    context_for(dev).draft_verify(desc, p_tokens, p_parents, p_starts, target.data_ptr(), p_draft, p_accept, p_sample, kept.data_ptr(), counts.data_ptr(),
+                                  token.data_ptr(), _stream_of(stream, dev))
     return kept, counts, token

@@ -13,9 +13,13 @@ Tables live on the device and results follow from their contents alone, whatever
 takes tensors for them, which may be the inputs (in place), so that a captured step can be replayed.  Contents are checked by the
 kernels: what is out of range is left out, and ``cache_check`` raises.
 """
+import contextlib
+
 from . import capi
 from .cache import _codes, _on_stream, _refuse, _stream_of, _workspace
 from .execute import _torch, context_for
+
+_NOTHING = contextlib.nullcontext()
 
 
 def page_tables(cache, batch, width):
@@ -27,39 +31,56 @@ def page_tables(cache, batch, width):
     return torch.zeros(cache[0].shape[0], **made), torch.full((batch, width), -1, **made), torch.zeros(batch, **made)
 
 
+_INT = _BYTE = None
+
+
 def _held(cache):
     """(element code, device index, [pages, heads, page, D], pointers of the four tensors), checked."""
+    global _INT, _BYTE
+    if _INT is None:
+        _INT, _BYTE = _torch().int32, _torch().uint8
     parts = len(cache)
-    if parts not in (2, 4):
+    if parts == 2:
+        k, v = cache
+        p_ek = p_ev = None
+    elif parts == 4:
+        k, v, ek, ev = cache
+    else:
         _refuse("a cache is (k, v), or (k, v, k exponents, v exponents)")
-    k, v = cache[0], cache[1]
-    code, shape, dev = _codes().get(k.dtype), k.shape, k.get_device()
+    dtype, shape, dev = k.dtype, k.shape, k.get_device()
+    code = _codes().get(dtype)
     if code is None or (code == capi.E4M3) != (parts == 4):
         _refuse("a cache holds float16, bfloat16, or float8_e4m3fn with exponents")
-    if len(shape) != 4 or v.shape != shape or v.dtype != k.dtype or not k.is_contiguous() or not v.is_contiguous():
+    if len(shape) != 4 or v.shape != shape or v.dtype != dtype or not k.is_contiguous() or not v.is_contiguous():
         _refuse("keys and values must be dense [pages, heads, page, D] of one type")
     if dev < 0 or v.get_device() != dev:
         _refuse("tensors must be on one CUDA device (there is no CPU path)")
-    byte = _torch().uint8
-    for e in cache[2:]:
-        if e.dtype != byte or e.shape != shape[:3] or not e.is_contiguous() or e.get_device() != dev:
-            _refuse("exponents must be dense uint8 [pages, heads, page] on the cache's device")
-    return code, dev, shape, [t.data_ptr() for t in cache] + [None] * (4 - parts)
+    if parts == 4:
+        want = shape[:3]
+        for e in (ek, ev):
+            if e.dtype != _BYTE or e.shape != want or not e.is_contiguous() or e.get_device() != dev:
+                _refuse("exponents must be dense uint8 [pages, heads, page] on the cache's device")
+        p_ek, p_ev = ek.data_ptr(), ev.data_ptr()
+    return code, dev, shape, (k.data_ptr(), v.data_ptr(), p_ek, p_ev)
 
 
-def _ints(t, shape, dev, what):
-    """The address of a dense int32 tensor of that shape."""
-    if t.dtype != _torch().int32 or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
-        _refuse(f"{what} must be dense int32 {list(shape)} on the cache's device")
+def _ints(t, n, dev, what):
+    """The address of a dense int32 tensor [n]."""
+    shape = t.shape
+    if t.dtype != _INT or len(shape) != 1 or shape[0] != n or t.get_device() != dev or not t.is_contiguous():
+        _refuse(f"{what} must be dense int32 [{n}] on the cache's device")
     return t.data_ptr()
 
 
 def _rows(t, dev, what):
     """(address, rows, width, pitch) of an int32 table."""
     shape = t.shape
-    if t.dtype != _torch().int32 or len(shape) != 2 or t.get_device() != dev or (t.stride(1) != 1 and shape[1] > 1):
-        _refuse(f"{what} must be int32 [batch, width] with dense rows on the cache's device")
-    return t.data_ptr(), shape[0], shape[1], t.stride(0)
+    if t.dtype != _INT or len(shape) != 2 or t.get_device() != dev:
+        _refuse(f"{what} must be int32 [batch, width] on the cache's device")
+    step, dense = t.stride()
+    if dense != 1 and shape[1] > 1:
+        _refuse(f"the rows of {what} must be dense")
+    return t.data_ptr(), shape[0], shape[1], step
 
 
 _EVERY_ROW = 2 ** 31 - 1  # (calls that see no packed rows, only their counts)
@@ -74,34 +95,31 @@ def _cache_desc(held, table, starts, lengths):
 def _change(which, cache, users, table, starts, lengths, parents, out, stream):
     """fork, grow and compact: new (users, table, third), or those in ``out``."""
     held = _held(cache)
-    _, dev, (pages, _, _, _), _ = held
+    dev, pages = held[1], held[2][0]
     rows = _rows(table, dev, "the table")
     batch, width = rows[1], rows[2]
-    p_users = _ints(users, (pages,), dev, "users")
-    p_lengths = None if lengths is None else _ints(lengths, (batch,), dev, "lengths")
-    p_starts = None if starts is None else _ints(starts, (batch + 1,), dev, "starts")
-    p_parents = None if parents is None else _ints(parents, (batch,), dev, "parents")
+    p_users = _ints(users, pages, dev, "users")
+    p_lengths = None if lengths is None else _ints(lengths, batch, dev, "lengths")
+    p_starts = None if starts is None else _ints(starts, batch + 1, dev, "starts")
+    p_parents = None if parents is None else _ints(parents, batch, dev, "parents")
     n_third = 1 if which == capi.PAGES_COMPACT else batch
     desc = _cache_desc(held, rows, p_starts, p_lengths)
     nbytes = capi.cache_pages_workspace_bytes(desc, which)
-
-    def new():
-        return users.new_empty(pages), users.new_empty((batch, width)), users.new_empty(n_third)
-
-    if stream is None:
-        out = new() if out is None else out
-        workspace = _workspace(max(nbytes, 16), dev)
-    else:
-        with _on_stream(stream, users.device):
-            out = new() if out is None else out
-            workspace = _workspace(max(nbytes, 16), dev)
-    if not isinstance(out, (tuple, list)) or len(out) != 3:
-        _refuse("out must be three tensors")
-    to = _rows(out[1], dev, "the new table")
-    if to[1:3] != (batch, width):
-        _refuse("the new table must have the shape of the old one")
-    tables = capi.PageTables(p_users, _ints(out[0], (pages,), dev, "the new users"), to[0], _ints(out[2], (n_third,), dev, "the third result"), to[3])
-    context_for(dev).cache_pages(which, desc, tables, p_parents, workspace.data_ptr(), max(nbytes, 16), _stream_of(stream, dev))
+    workspace = None
+    with _NOTHING if stream is None else _on_stream(stream, users.device):
+        if nbytes:
+            workspace = _workspace(nbytes, dev)
+        if out is None:
+            out = new_users, new_table, third = users.new_empty(pages), table.new_empty((batch, width)), users.new_empty(n_third)
+            tables = capi.PageTables(p_users, new_users.data_ptr(), new_table.data_ptr(), third.data_ptr(), width)
+        else:
+            if not isinstance(out, (tuple, list)) or len(out) != 3:
+                _refuse("out must be three tensors")
+            to = _rows(out[1], dev, "the new table")
+            if to[1] != batch or to[2] != width:
+                _refuse("the new table must have the shape of the old one")
+            tables = capi.PageTables(p_users, _ints(out[0], pages, dev, "the new users"), to[0], _ints(out[2], n_third, dev, "the third result"), to[3])
+    context_for(dev).cache_pages(which, desc, tables, p_parents, None if workspace is None else workspace.data_ptr(), nbytes, _stream_of(stream, dev))
     return tuple(out)
 
 
@@ -131,10 +149,11 @@ def cache_copy(cache, source, target, *, into=None, stream=None):
     page): both int32 [n] on the device.  A page must not be target twice nor, in one cache, source and target.  Returns ``into``."""
     held = _held(cache)
     other = held if into is None else _held(into)
-    dev, n = held[1], source.shape[0] if source.dim() == 1 else -1
-    if n < 0 or other[1] != dev:
+    dev, shape = held[1], source.shape
+    if len(shape) != 1 or other[1] != dev:
         _refuse("source and target must be lists of pages, and both caches on one device")
-    a, b = _ints(source, (n,), dev, "source"), _ints(target, (n,), dev, "target")
+    n = shape[0]
+    a, b = _ints(source, n, dev, "source"), _ints(target, n, dev, "target")
     no_table = (None, 0, 0, 0)
     context_for(dev).cache_copy(_cache_desc(held, no_table, None, None), _cache_desc(other, no_table, None, None), a, b, n, _stream_of(stream, dev))
     return cache if into is None else into
@@ -150,13 +169,10 @@ def cache_keep(cache, table, starts, lengths, kept, counts, *, out=None, stream=
     batch = rows[1]
     if path[1] != batch:
         _refuse("kept must have a row for each sequence")
-    p_starts, p_lengths, p_counts = _ints(starts, (batch + 1,), dev, "starts"), _ints(lengths, (batch,), dev, "lengths"), _ints(counts, (batch,), dev, "counts")
+    p_starts, p_lengths, p_counts = _ints(starts, batch + 1, dev, "starts"), _ints(lengths, batch, dev, "lengths"), _ints(counts, batch, dev, "counts")
     if out is None:
-        if stream is None:
+        with _NOTHING if stream is None else _on_stream(stream, lengths.device):
             out = lengths.new_empty(batch)
-        else:
-            with _on_stream(stream, lengths.device):
-                out = lengths.new_empty(batch)
-    p_out = _ints(out, (batch,), dev, "the new lengths")
+    p_out = _ints(out, batch, dev, "the new lengths")
     context_for(dev).cache_keep(_cache_desc(held, rows, p_starts, p_lengths), path[0], path[3], path[2], p_counts, p_out, _stream_of(stream, dev))
     return out

@@ -383,7 +383,7 @@ typedef struct frisk_b200_page_tables {
   int32_t *users_out, *table_out, *lengths_out;
   int64_t table_out_stride;
 } frisk_b200_page_tables;
-/* Bytes of workspace for one of the three (FRISK_B200_PAGES_*); 0 for what it refuses.  Host-only. */
+/* Bytes of workspace for one of the three (FRISK_B200_PAGES_*); 0 where it needs none (fork, of small tables) or refuses.  Host-only. */
 size_t frisk_b200_cache_pages_workspace_bytes(const frisk_b200_cache_desc* cache, int32_t which);
 int frisk_b200_cache_fork(frisk_b200_ctx* ctx, const frisk_b200_cache_desc* cache, const frisk_b200_page_tables* tables,
                           const int32_t* parents, void* workspace, size_t workspace_bytes, void* stream);

@@ -19,7 +19,8 @@ def _cache(**change):
 def test_workspace_sizes_say_what_is_refused():
     size = capi.cache_pages_workspace_bytes
     for which in (capi.PAGES_FORK, capi.PAGES_GROW, capi.PAGES_COMPACT):
-        assert size(_cache(), which) > 0
+        assert size(_cache(batch=4000, table_width=100, table_stride=100), which) > 0
+        assert (size(_cache(), which) > 0) == (which != capi.PAGES_FORK)  # (small tables are forked without)
         for change in (dict(page=8), dict(page=24), dict(D=96), dict(heads=0), dict(pages=0), dict(batch=-1), dict(table_width=-1), dict(table_stride=3),
                        dict(dtype=capi.F32), dict(pages=1 << 40), dict(batch=1 << 20, table_width=1 << 12, table_stride=1 << 12),
                        dict(table_width=1 << 28, table_stride=1 << 28)):
