@@ -279,7 +279,10 @@ cudaError_t launch(frisk_b200_ctx* ctx, AdapterParams p, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   // (at most: every sequence may end with a tile that is not full)
   const int64_t tiles = std::min<int64_t>(p.rows, p.rows / P::kRows + p.batch);
+  // The most CTAs a tile with which all tiles run at once (64 requests of a token, rank 128: clusters of eight 57 us, of four 33).
+  static ClusterCapacity capacity;
   p.cluster = kMaxCluster;
+  while (p.cluster > 2 && capacity(ctx->device, kernel, kThreads, (int)P::kBytes, p.cluster) < tiles) p.cluster /= 2;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel waits (griddepcontrol.wait) itself
@@ -300,8 +303,7 @@ template <typename T, typename C, int RMAX>
 cudaError_t launch_rows(frisk_b200_ctx* ctx, const AdapterParams& p, cudaStream_t s) {
   const int64_t mean = (p.rows + p.batch - 1) / p.batch;  // rows of a sequence
   if (mean <= 16) return launch<T, C, RMAX, 1, 1>(ctx, p, s);
-  if (mean <= 48) return launch<T, C, RMAX, 2, 1>(ctx, p, s);
-  return launch<T, C, RMAX, 2, RMAX <= 64 ? 4 : 2>(ctx, p, s);
+  return launch<T, C, RMAX, 2, 1>(ctx, p, s);
 }
 template <typename T, typename C>
 cudaError_t launch_rank(frisk_b200_ctx* ctx, const AdapterParams& p, cudaStream_t s) {

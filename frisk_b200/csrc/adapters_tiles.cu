@@ -53,7 +53,7 @@ __device__ __forceinline__ void land(volatile uint32_t* abort_flag) {
 }
 
 // ------------------------------------------------------------------------------------------------ sums
-constexpr int kSumStages = 4, kSumThreads = 192;
+constexpr int kSumStages = 4, kAdders = 8, kSumThreads = 64 + 32 * kAdders;
 struct SumsLayout {  // of `width` columns, R rounded up to a multiple of 16
   static __host__ __device__ int stage_bytes(int width) { return kBoxBytes + width * 128; }
   static __host__ __device__ int pitch(int width) { return width + 4; }  // of rows of sums, floats
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kSumThreads)
       }
       __syncwarp();
     }
-  } else {
+  } else if (warp < 6) {
     // this CTA's part into the ring, all of which has been read: lane = row
     const int row = (warp & 3) * 32 + lane, pitch = SumsLayout::pitch(width);
     float* mine = reinterpret_cast<float*>(smem) + row * pitch;
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kSumThreads)
     // Eight threads a row, four neighbours each in turns of 32; the parts in the order of the CTAs.
     const int t = tid - 64, quads = width / 4, pitch = SumsLayout::pitch(width), each = kRows / ctas;
 #pragma unroll 1
-    for (int row = rank * each + (t >> 3); row < (rank + 1) * each; row += 16) {
+    for (int row = rank * each + (t >> 3); row < (rank + 1) * each; row += 4 * kAdders) {
       const bool valid = row < found.rows;
       float4 v[kMaxRank / 32];
       float most = 0.f;
@@ -586,9 +586,10 @@ int launch_both(frisk_b200_ctx* ctx, AdapterParams p, const Work& work, cudaStre
 
 }  // namespace
 
-// Sequences of more than 48 rows in the mean, if adapters lie one behind the other (no tensor map has a step of 0)
+// Long sequences, if adapters lie one behind the other (no tensor map has a step of 0).  K = N = 4096, here and in adapters.cu, us: rank 16, 64 sequences of 64 rows
+// 38 and 33, of 128 rows 50 and 62; rank 64, 16 of 32 rows 17.5 and 16.9, of 40 rows 18 and 31, 64 of 64 rows 42 and 66; 2 of 64 rows 12.8 and 11.7.
 size_t adapter_tiles_workspace_bytes(const frisk_b200_adapter_desc& d) {
-  if (d.batch < 1 || d.rows <= 48 * (int64_t)d.batch || d.count < 1) return 0;
+  if (d.batch < 1 || d.rows < 512 || d.rows <= (d.rank <= 32 ? 64 : 32) * (int64_t)d.batch || d.count < 1) return 0;
   if (d.count > 1 && (d.a_step < d.lda || d.b_step < d.ldb)) return 0;
   if (most_tiles(d.rows, d.batch) * ((d.N + kColumns - 1) / kColumns) > INT32_MAX || d.rows * (int64_t)d.rank > INT32_MAX) return 0;
   const int terms = d.dtype_c == FRISK_B200_F32 && d.dtype == FRISK_B200_BF16 ? 3 : 2;

@@ -67,7 +67,7 @@ class Requests:
         assert off.numel() == 0 or float(off.max()) <= 0, (float(off.max()), float((got - want)[inside].abs().max()))
 
 
-@pytest.mark.parametrize("counts", [[1], [1] * 9, [0, 3, 16, 0, 17, 1], [40, 5, 33], [64], [128, 1], [129, 300], [3] * 300, [200, 0, 1, 130, 77, 128]])
+@pytest.mark.parametrize("counts", [[1], [1] * 9, [0, 3, 16, 0, 17, 1], [40, 5, 33], [64], [128, 1], [129, 300], [3] * 300, [200, 0, 1, 130, 77, 128], [300, 129, 200], [640]])
 @pytest.mark.parametrize("k,n,rank", [(64, 32, 8), (72, 100, 16), (8, 8, 24), (1, 1, 8), (250, 333, 32), (1000, 96, 40), (513, 520, 64), (300, 70, 128), (33, 31, 72)])
 @pytest.mark.parametrize("dtype,wide", [("bfloat16", False), ("bfloat16", True), ("float16", False), ("float16", True)])
 def test_adapters(counts, k, n, rank, dtype, wide):
