@@ -1,9 +1,10 @@
 """Low-rank adapters of many requests, added to a shared projection: ``adapter_gemm``."""
 import contextlib
 
-from . import capi
+from . import calls, capi
 from .cache import _new_like, _on_stream, _stream_of, _workspace
-from .execute import _torch, context_for
+from .calls import context_for
+from .execute import _torch
 
 _KINDS = None
 _NOTHING = contextlib.nullcontext()
@@ -23,6 +24,10 @@ def adapter_gemm(x, a, b, c, starts, adapters, *, scales=None, out=None, stream=
     captured step can be replayed for other requests; an adapter out of range counts as none, and ``cache_check`` raises.  Sums have 32
     bits, and the result is rounded once."""
     global _KINDS
+    if out is None and stream is None:
+        r = calls.adapters(x, a, b, c, starts, adapters, scales)
+        if r is not None:
+            return calls.result(r, x.get_device())
     if _KINDS is None:
         torch = _torch()
         _KINDS = {torch.float16: capi.F16, torch.bfloat16: capi.BF16}, torch.float32, torch.int32

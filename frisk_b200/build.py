@@ -6,9 +6,12 @@ Each ``csrc/*.cu`` is compiled to an object (in parallel, only when it or a head
 is newer than the object) and linked into ``frisk_b200/lib/libfrisk_b200.so``.
 nvcc cross-compiles without a GPU.  ``csrc/recognise.cpp``, a host-only CPython module, is compiled by g++ into
 ``frisk_b200/lib/_recognise`` + the interpreter's extension suffix; where g++ or Python's headers are missing the package does without.
+So is ``csrc/calls.cpp``, which also needs torch's headers, into ``frisk_b200/lib/_calls_`` + torch's version + that suffix.
 """
 import concurrent.futures
 import importlib.machinery
+import importlib.metadata
+import importlib.util
 import os
 import pathlib
 import shutil
@@ -62,6 +65,30 @@ def build_recognise(force=False):
     return target
 
 
+def build_calls(force=False):
+    """The native form of the serving operators' calls, or None where it cannot be built here: they are then made in Python, more slowly."""
+    from .calls import path
+    spec, gxx, headers = importlib.util.find_spec("torch"), shutil.which("g++"), sysconfig.get_paths()["include"]
+    cuda = pathlib.Path(_nvcc()).resolve().parent.parent / "include"
+    torch = None if spec is None else pathlib.Path(spec.submodule_search_locations[0])
+    source = CSRC / "calls.cpp"
+    if torch is None or gxx is None or not all(p.exists() for p in (torch / "include/ATen/cuda/EmptyTensor.h", pathlib.Path(headers, "Python.h"), cuda / "cuda_runtime_api.h")):
+        sys.stderr.write("frisk_b200: no g++, or no headers of Python, torch or CUDA: built without native calls\n")
+        return None
+    target = path(importlib.metadata.version("torch"))
+    if not force and not _stale(target, [source, INCLUDE / "frisk_b200.h"]):
+        return target
+    target.parent.mkdir(exist_ok=True)
+    flags = ["-O2", "-std=c++17", "-shared", "-fPIC", "-I", headers, "-I", str(torch / "include"), "-I", str(torch / "include/torch/csrc/api/include"), "-I", str(cuda)]
+    libs = ["-L", str(torch / "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    res = subprocess.run([gxx, *flags, str(source), "-o", str(target), *libs], capture_output=True, text=True)
+    if res.returncode:
+        sys.stderr.write("frisk_b200: built without native calls, g++ failed on calls.cpp\n" + res.stderr[-2000:])
+        target.unlink(missing_ok=True)  # (one of an older source)
+        return None
+    return target
+
+
 def build(force=False, verbose=False):
     nvcc = _nvcc()
     OBJ.mkdir(exist_ok=True)
@@ -95,6 +122,7 @@ def build(force=False, verbose=False):
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError("link of libfrisk_b200.so failed")
     build_recognise(force)
+    build_calls(force)
     return LIB
 
 

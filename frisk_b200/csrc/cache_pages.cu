@@ -414,43 +414,42 @@ __global__ void __launch_bounds__(kPlan) compact_plan_kernel(const PageTables t)
   int *from = t.ws + 1, *to = from + t.pages, *goes = to + t.pages;
   pdl_begin();
   int mine = 0, used;
-  for (int p = tid; p < t.pages; p += kPlan) mine += t.users[p] != 0;
+  for (int p0 = tid; p0 < t.pages; p0 += kPlan * kEach) {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) mine += p0 + j * kPlan < t.pages && t.users[p0 + j * kPlan] != 0;
+  }
   block_scan(mine, sums, &used);
   int holes = 0, moves = 0;
   for (int p0 = 0; p0 < t.pages; p0 += kPlan * kEach) {
     const int first = p0 + (tid >> 5) * 32 * kEach + lane;
-    unsigned masks[kEach];
-    int users[kEach], n_hole = 0, n_move = 0;
+    unsigned empty[kEach], moving[kEach];  // of 32 neighbours: free pages among the first `used`, used ones behind them
+    int users[kEach], both = 0;            // (a round's moves, and its holes, are at most kPlan * kEach: two counts in one sum)
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) users[j] = first + 32 * j < t.pages ? t.users[first + 32 * j] : 0;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
       const int p = first + 32 * j;
-      users[j] = p < t.pages ? t.users[p] : 0;
-      const bool is_used = users[j] != 0;
-      // (a free page among the first `used`, or a used one behind them: 32 neighbours may hold both)
-      const bool hole = p < used && !is_used, move = p >= used && is_used;
-      masks[j] = __ballot_sync(0xffffffffu, hole || move);
-      const unsigned moving = __ballot_sync(0xffffffffu, move);
-      n_move += __popc(moving);
-      n_hole += __popc(masks[j] & ~moving);
-      if (p < t.pages && p < used && is_used && t.users_out != t.users) t.users_out[p] = users[j];
+      empty[j] = __ballot_sync(0xffffffffu, p < used && users[j] == 0);
+      moving[j] = __ballot_sync(0xffffffffu, p >= used && users[j] != 0);
+      both += __popc(empty[j]) + (__popc(moving[j]) << 16);
     }
-    int all_holes, all_moves;
-    int at_hole = holes + __shfl_sync(0xffffffffu, block_scan(lane == 0 ? n_hole : 0, sums, &all_holes), 0);
-    int at_move = moves + __shfl_sync(0xffffffffu, block_scan(lane == 0 ? n_move : 0, sums, &all_moves), 0);
+    static_assert(kPlan * kEach < 1 << 15, "two counts in one sum");
+    int all;
+    const int at = __shfl_sync(0xffffffffu, block_scan(lane == 0 ? both : 0, sums, &all), 0);
+    int at_hole = holes + (at & 0xffff), at_move = moves + (at >> 16);
     const unsigned below = (1u << lane) - 1u;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
       const int p = first + 32 * j;
-      const bool move = p < t.pages && p >= used && users[j] != 0;
-      const unsigned moving = __ballot_sync(0xffffffffu, move), empty = masks[j] & ~moving;
-      if (move) from[at_move + __popc(moving & below)] = p;
-      else if (empty >> lane & 1u) to[at_hole + __popc(empty & below)] = p;
-      else if (p < t.pages && p >= used) goes[p] = -1;
-      at_move += __popc(moving);
-      at_hole += __popc(empty);
+      if (moving[j] >> lane & 1u) from[at_move + __popc(moving[j] & below)] = p;
+      else if (empty[j] >> lane & 1u) to[at_hole + __popc(empty[j] & below)] = p;
+      else if (p >= used && p < t.pages) goes[p] = -1;
+      if (p < used && users[j] != 0 && t.users_out != t.users) t.users_out[p] = users[j];
+      at_move += __popc(moving[j]);
+      at_hole += __popc(empty[j]);
     }
-    holes += all_holes;
-    moves += all_moves;
+    holes += all & 0xffff;
+    moves += all >> 16;
   }
   __syncthreads();
   for (int k = tid; k < moves; k += kPlan) {  // (as many holes as moves)

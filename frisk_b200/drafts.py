@@ -1,9 +1,10 @@
 """Verification of drafted tokens: ``draft_verify``."""
 import contextlib
 
-from . import capi
+from . import calls, capi
 from .cache import _on_stream, _stream_of
-from .execute import _torch, context_for
+from .calls import context_for
+from .execute import _torch
 
 
 def _refuse(what):
@@ -39,6 +40,10 @@ def draft_verify(tokens, parents, starts, target, draft, accept, sample, *, max_
     and next -1, as one with more than ``max_new`` (1 to 1024) rows or rows out of range, for which ``cache_check`` raises.  Probabilities that are NaN or
     negative count as 0."""
     global _KINDS
+    if stream is None:
+        r = calls.verify(tokens, parents, starts, target, draft, accept, sample, max_new)
+        if r is not None:
+            return calls.result(r, target.get_device())
     if _KINDS is None:
         torch = _torch()
         _KINDS = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}, torch.int32, torch.int64, torch.float32

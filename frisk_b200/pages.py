@@ -15,9 +15,10 @@ kernels: what is out of range is left out, and ``cache_check`` raises.
 """
 import contextlib
 
-from . import capi
+from . import calls, capi
 from .cache import _codes, _on_stream, _refuse, _stream_of, _workspace
-from .execute import _torch, context_for
+from .calls import context_for
+from .execute import _torch
 
 _NOTHING = contextlib.nullcontext()
 
@@ -94,6 +95,10 @@ def _cache_desc(held, table, starts, lengths):
 
 def _change(which, cache, users, table, starts, lengths, parents, out, stream):
     """fork, grow and compact: new (users, table, third), or those in ``out``."""
+    if out is None and stream is None:
+        r = calls.change(which, cache, users, table, starts, lengths, parents)
+        if r is not None:
+            return calls.result(r, users.get_device())
     held = _held(cache)
     dev, pages = held[1], held[2][0]
     rows = _rows(table, dev, "the table")
@@ -147,6 +152,11 @@ def cache_compact(cache, users, table, *, out=None, stream=None):
 def cache_copy(cache, source, target, *, into=None, stream=None):
     """Copies page ``source[i]`` of ``cache`` to page ``target[i]`` of ``into`` (the cache itself if not given, or another of the same type and
     page): both int32 [n] on the device.  A page must not be target twice nor, in one cache, source and target.  Returns ``into``."""
+    if stream is None:
+        r = calls.copy(cache, source, target, cache if into is None else into)
+        if r is not None:
+            calls.result(r, source.get_device())
+            return cache if into is None else into
     held = _held(cache)
     other = held if into is None else _held(into)
     dev, shape = held[1], source.shape
@@ -163,6 +173,10 @@ def cache_keep(cache, table, starts, lengths, kept, counts, *, out=None, stream=
     """The new lengths after ``counts[b]`` of the new tokens of each sequence were accepted: the key and value at position
     ``lengths[b] + kept[b, i]`` move to ``lengths[b] + i``.  ``kept`` int32 [batch, width] ascends within a sequence (``draft_verify`` gives
     both); what is behind the counts does not matter.  Pages stay where they are.  ``out`` may be ``lengths``."""
+    if out is None and stream is None:
+        r = calls.keep(cache, table, starts, lengths, kept, counts)
+        if r is not None:
+            return calls.result(r, lengths.get_device())
     held = _held(cache)
     dev = held[1]
     rows, path = _rows(table, dev, "the table"), _rows(kept, dev, "kept")
