@@ -158,6 +158,7 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
     }
     *reinterpret_cast<float4*>(at) = s;
   }
+  __syncwarp();
   cluster_sync_all();
   for (int i = rank * kThreads + tid; i < n_quads; i += C_ * kThreads) {
     const int offset = i / quads * P::kPitch + i % quads * 4;
@@ -168,6 +169,7 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
     }
     for (int r = 0; r < C_; ++r) st_cluster_f4(mapa_addr(smem_u32(full + offset), r), s);
   }
+  __syncwarp();
   cluster_sync_all();  // (from here on no CTA reads or writes another's memory)
   // ---- as terms, in the order in which the second product takes them
   if (std::is_same<T, __half>::value) {

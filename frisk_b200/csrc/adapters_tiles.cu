@@ -459,8 +459,8 @@ __global__ void __launch_bounds__(kColThreads, 1)
           load_box_rows(c + row0 * p.ldc + now.col, p.ldc, now.rows, now.cols, lane, [&](int r, uint32_t w) {
             *reinterpret_cast<uint32_t*>(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = w;
           });
-          __syncwarp();
         }
+        __syncwarp();
         if (product) {
           constexpr int kEach = 16 / (int)sizeof(C);  // columns of 16 bytes
 #pragma unroll

@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(kPlan) fork_kernel(const PageTables t) {
     }
   }
   const int length = first < t.batch ? forked_length(t, first) : 0;
+  __syncwarp();
   cluster_sync_all();
   if (first < t.batch) t.lengths_out[first] = length;
 #pragma unroll
@@ -240,6 +241,7 @@ __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
   if (COPIES) {
     copy_users(t, (int64_t)blockIdx.x * kPlan + tid, (int64_t)gridDim.x * kPlan);
     copy_table(t, (int64_t)blockIdx.x * kPlan + tid, (int64_t)gridDim.x * kPlan);
+    __syncwarp();
     cluster_sync_all();
     if (blockIdx.x > 0) return;
   }

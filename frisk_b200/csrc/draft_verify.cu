@@ -129,6 +129,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams 
     at_draft[i] = DRAFT && there ? weight(to_float<T>(draft[up * p.draft_stride + x])) : 1.f;
     random[i] = p.accept[first + i];
   }
+  __syncwarp();
   cluster_sync_all();  // (and no CTA is written to before it runs)
 
   // Steps are cut where the row's addresses are multiples of 16, so a row may begin up to kLane - 1 values into the first.
@@ -211,6 +212,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams 
   auto sum = [&]() {
     const double part = warp_sum(lane_sum(step0, step1));
     if (lane < p.ctas) st_cluster_f64(mapa_addr(smem_u32(&part_sums[turn][rank * kWarps + warp]), lane), part);
+    __syncwarp();
     cluster_sync_all();
     double all = 0.0;
     for (int i = lane; i < parts; i += 32) all += part_sums[turn][i];

@@ -55,7 +55,7 @@ class Requests:
 
     def check(self, scales=True, in_place=False, **more):
         import torch
-        got = self.run(scales, in_place, **more).cpu().double()
+        got = self.run(scales, in_place, **more).cpu().double()  # (``out`` of another's holds 55 where nothing is written)
         want, bound = so.adapters(*self.cpu, self.starts, self.which, self.scales if scales else None)
         inside = torch.zeros(self.rows, dtype=torch.bool)
         inside[self.starts[0]:self.starts[-1]] = True
@@ -74,6 +74,19 @@ def test_adapters(counts, k, n, rank, dtype, wide):
     r = Requests(counts, k, n, rank, 5, dtype, wide, seed=k + len(counts), gap=len(counts) % 3, pitch=8 * (n % 2), odd=n % 4)
     r.check()
     r.check(scales=False, in_place=True)
+
+
+@pytest.mark.parametrize("counts", [[3, 0, 17], [300, 129, 200]])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("c_at,out_at,n", [(0, 1, 64), (1, 0, 64), (0, 8, 136), (3, 5, 37), (8, 0, 130), (0, 2, 2), (1, 1, 1)])
+def test_results_elsewhere(counts, wide, c_at, out_at, n):
+    """c and the result begin at other places of 16 bytes; what is beside the result, and behind the last row, stays."""
+    import torch
+    r = Requests(counts, 72, n, 16, 3, "bfloat16", wide, seed=n, gap=1, odd=c_at)
+    buf = torch.full((r.rows, n + out_at + 7), 55.0, dtype=r.whole[3].dtype, device="cuda")
+    r.check(out=buf[:, out_at:out_at + n])
+    buf[:, out_at:out_at + n] = 55.0
+    assert bool((buf == 55.0).all())
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])

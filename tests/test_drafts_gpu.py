@@ -72,6 +72,25 @@ def test_verify(counts, vocab, dtype, draft, tree):
     F.cache_check()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("vocab", [100, 4099])
+def test_the_draft_in_rows_of_another_pitch(dtype, vocab):
+    """Rows of the two begin at other places of 16 bytes."""
+    import torch
+    d = Drafts([9, 6, 12], vocab, dtype, seed=7, pitch=1)
+    for more in (0, 2, 5):
+        whole = torch.full((len(d.draft), vocab + more), math.nan, dtype=d.draft.dtype)
+        whole[:, more // 2:more // 2 + vocab] = d.draft
+        target, d.draft = d.draft, whole[:, more // 2:more // 2 + vocab]
+        import frisk_b200 as F
+        wide = whole.cuda()
+        got = F.draft_verify(d.tokens.cuda(), torch.tensor(d.parents, dtype=torch.int32).cuda(), torch.tensor(d.starts, dtype=torch.int32).cuda(),
+                             d.target._base.cuda()[:, :vocab], wide[:, more // 2:more // 2 + vocab], d.accept.cuda(), d.sample.cuda(), max_new=12)
+        assert [t.tolist() for t in got] == d.want()
+        d.draft = target
+    F.cache_check()
+
+
 def test_many_seeds_and_types_of_tokens():
     """Every kind of walk: all stand, none does, several children of a node fall, the same child twice."""
     import torch

@@ -54,7 +54,7 @@ def sequences(rng, pages, batch, width, page, share=0.5):
     return users, table, lengths
 
 
-SIZES = [(40, 1, 3, 16), (64, 7, 9, 16), (200, 33, 5, 64), (3000, 300, 11, 16), (9000, 2500, 3, 32), (17, 5, 1, 128)]
+SIZES = [(40, 1, 3, 16), (64, 7, 9, 16), (200, 33, 5, 64), (3000, 300, 11, 16), (9000, 2500, 3, 32), (17, 5, 1, 128), (5000, 700, 60, 16)]
 
 
 @pytest.mark.parametrize("pages,batch,width,page", SIZES)
@@ -107,6 +107,36 @@ def test_grow(pages, batch, width, page, held, in_place):
             for t in cpu:
                 t.view(cpu[-1].dtype if held != "bfloat16" else t.dtype)[go, :, :keys] = t.view(cpu[-1].dtype if held != "bfloat16" else t.dtype)[come, :, :keys]
         assert same(cpu, cache), kind
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_many_pages(in_place):
+    """More than a cluster copies, and free pages far behind the first."""
+    import torch
+    import frisk_b200 as F
+    pages, batch, width, page = 300000, 500, 300, 16
+    rng = random.Random(8)
+    cache = F.paged_cache(pages, 1, page, 64, torch.float8_e4m3fn)
+    users, table, lengths = sequences(rng, pages - 2000, batch, width - 1, page, 0.9)
+    table = [r + [-1] for r in table]
+    users = [max(n, 1) for n in users[:pages - 3000]] + users[pages - 3000:] + [0] * 2000  # (others have the first)
+    parents = [rng.randint(-1, batch - 1) for _ in range(batch)]
+    given = ints(users), ints(table), ints(lengths)
+    got = F.cache_fork(cache, *given, ints(parents), out=given if in_place else None)
+    want = so.fork(users, table, lengths, parents, page)
+    assert [t.tolist() for t in got] == list(want)
+    counts = [rng.randint(0, 20) for _ in range(batch)]
+    counts = [min(n, width * page - m) for n, m in zip(counts, want[2])]
+    starts = [0]
+    for n in counts:
+        starts.append(starts[-1] + n)
+    got = F.cache_grow(cache, got[0], got[1], ints(starts), got[2], out=(got[0], got[1], ints([0] * batch)) if in_place else None)
+    want = so.grow(*want[:2], starts, want[2], page)
+    assert [t.tolist() for t in got] == list(want[:3])
+    got = F.cache_compact(cache, got[0], got[1])
+    want = so.compact(*want[:2])
+    F.cache_check()
+    assert got[0].tolist() == want[0] and got[1].tolist() == want[1] and got[2].tolist() == [want[2]]
 
 
 def test_grow_is_granted_in_order():
