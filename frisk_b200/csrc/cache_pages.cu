@@ -229,7 +229,8 @@ struct GrowWork {
   }
 };
 
-// COPIES: a cluster copies the tables that are not changed in place, then its first CTA plans
+// COPIES: beside the planning CTA, the others of its cluster copy the tables that are not changed in place.  (The plan is made from the old ones; only what
+// it changes waits for the copies.)
 template <bool COPIES>
 __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
   __shared__ int sums[32];
@@ -238,13 +239,19 @@ __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
   GrowWork w(t.ws, t.batch, t.width);
   const int tid = threadIdx.x, lane = tid & 31;
   pdl_begin();
-  if (COPIES) {
-    copy_users(t, (int64_t)blockIdx.x * kPlan + tid, (int64_t)gridDim.x * kPlan);
-    copy_table(t, (int64_t)blockIdx.x * kPlan + tid, (int64_t)gridDim.x * kPlan);
+  if (COPIES && blockIdx.x > 0) {
+    copy_users(t, (int64_t)(blockIdx.x - 1) * kPlan + tid, (int64_t)(gridDim.x - 1) * kPlan);
+    copy_table(t, (int64_t)(blockIdx.x - 1) * kPlan + tid, (int64_t)(gridDim.x - 1) * kPlan);
     __syncwarp();
     cluster_sync_all();
-    if (blockIdx.x > 0) return;
+    return;
   }
+  // (the first pages that may be free are looked at meanwhile)
+  constexpr int kEach = 8;
+  const int own = (tid >> 5) * 32 * kEach + lane;  // of a round of kPlan * kEach pages, the first that this thread looks at
+  int ahead[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) ahead[j] = own + 32 * j < t.pages ? t.users[own + 32 * j] : 1;
   // 1. the slots that each sequence's new tokens touch
   int all = 0;
   for (int b0 = 0; b0 < t.batch; b0 += kPlan) {
@@ -297,9 +304,9 @@ __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
     bool shared = false;
     if (i < all) {
       const int b = owner(i), slot = (t.lengths[b] >> t.page_log2) + i - offset[b];
-      entry = t.table_out[b * t.out_stride + slot];
+      entry = t.table[b * t.stride + slot];
       if (entry >= t.pages) flag(t.status, ST_CACHE_PAGE);
-      const int users = entry >= 0 && entry < t.pages ? t.users_out[entry] : 0;
+      const int users = entry >= 0 && entry < t.pages ? t.users[entry] : 0;
       shared = users > 1;
       w.kind[i] = entry < 0 ? TAKE : KEEP;
     }
@@ -319,7 +326,7 @@ __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
 #pragma unroll 8
     for (int j = 0; j < k; ++j) earlier += w.page[j] == page;
     const int i = w.shared[k];
-    if (t.users_out[page] - earlier > 1) w.kind[i] = SWAP;
+    if (t.users[page] - earlier > 1) w.kind[i] = SWAP;
     else if (earlier) w.kind[i] = KEEP_AS_LAST;
   }
   __syncthreads();
@@ -336,15 +343,17 @@ __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
   if (tid == 0) w.before[all] = taken;
   // 5. that many free pages, lowest first: a warp looks at 256 pages a round, 32 at a time
   int found = 0;
-  constexpr int kEach = 8;
   for (int p0 = 0; p0 < t.pages && found < taken; p0 += kPlan * kEach) {
-    const int first = p0 + (tid >> 5) * 32 * kEach + lane;
+    const int first = p0 + own;
+    if (p0 > 0) {
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) ahead[j] = first + 32 * j < t.pages ? t.users[first + 32 * j] : 1;
+    }
     unsigned masks[kEach];
     int mine = 0;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      const int p = first + 32 * j;
-      masks[j] = __ballot_sync(0xffffffffu, p < t.pages && t.users_out[p] == 0);
+      masks[j] = __ballot_sync(0xffffffffu, ahead[j] == 0);
       mine += __popc(masks[j]);
     }
     int total;
@@ -366,15 +375,19 @@ __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
     w.depends[b] = granted;
   }
   __syncthreads();
+  if (COPIES) {
+    __syncwarp();
+    cluster_sync_all();
+  }
   for (int i = tid; i < all; i += kPlan) {
     const int kind = w.kind[i];
     if (kind < TAKE) continue;
     const int b = owner(i);
     if (!w.depends[b]) continue;
     const int length = t.lengths[b], nth = i - offset[b], page = w.free[w.before[i]];
-    int* entry = t.table_out + b * t.out_stride + (length >> t.page_log2) + nth;
+    const int64_t slot = (length >> t.page_log2) + nth;
     if (kind == SWAP) {
-      const int old = *entry;
+      const int old = t.table[b * t.stride + slot];
       atomicSub(t.users_out + old, 1);
       if (nth == 0 && (length & (t.page - 1))) {  // its keys come along
         w.copies[3 * b] = old;
@@ -382,7 +395,7 @@ __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
         w.copies[3 * b + 2] = length & (t.page - 1);
       }
     }
-    *entry = page;
+    t.table_out[b * t.out_stride + slot] = page;
     t.users_out[page] = 1;
   }
 }
