@@ -8,7 +8,8 @@
 //
 // Bound by memory for the ranks of adapters: an element of x, c or out takes R multiplications (R = 64 at 6.5 TB/s: 0.2 PFLOP/s).  So the products
 // are mma.sync's, operands go from memory to registers without a stop, and no tensor memory is set up.  For a few rows the adapters
-// themselves are what is read, each by a cluster of its own.
+// themselves are what is read, each by a cluster of its own; then the time is a chain: tables, x and A, two meetings of the cluster, B and c (one token, rank 16,
+// K = N = 4096: 7.2 us with the launch; 64 tokens over 40 adapters of rank 32: 12.7, 25 MB).  Long sequences have kernels of their own (adapters_tiles.cu).
 //
 // Order of a product's inner index is free if both sides have the same, so a lane takes 16 bytes of it at once: of 32 neighbouring elements lane q of
 // four has 8 q .. 8 q + 7, which serve two steps of 16.  Columns of a result are permuted the same way: a lane ends up with 8 neighbours.
@@ -320,13 +321,15 @@ cudaError_t launch_rank(frisk_b200_ctx* ctx, const AdapterParams& p, cudaStream_
 
 using namespace fb;
 
+constexpr int64_t kMostRows = 1 << 26, kMostColumns = 1 << 28;
 static int check_sizes(const frisk_b200_adapter_desc* d) {
   if (d->dtype != FRISK_B200_F16 && d->dtype != FRISK_B200_BF16) return FRISK_B200_E_CACHE_TYPE;
   if (d->dtype_c != d->dtype && d->dtype_c != FRISK_B200_F32) return FRISK_B200_E_CACHE_TYPE;
   if (d->rows < 0 || d->rows > INT32_MAX || d->batch < 0 || d->count < 0 || d->K < 1 || d->N < 1 || d->K > INT32_MAX - 64 || d->N > INT32_MAX - 64 || d->rank < 8 ||
       d->rank > kMaxRank || d->rank % 8)
     return FRISK_B200_E_CACHE_SHAPE;
-  if ((std::min<int64_t>(d->rows, d->rows / 16 + d->batch)) * kMaxCluster > INT32_MAX) return FRISK_B200_E_TOO_LARGE;
+  // (tiles over all sequences, and a tile's 16-byte pieces, are counted in 32 bits)
+  if (d->rows > kMostRows || d->N > kMostColumns || (std::min<int64_t>(d->rows, d->rows / 16 + d->batch)) * kMaxCluster > INT32_MAX) return FRISK_B200_E_TOO_LARGE;
   return 0;
 }
 

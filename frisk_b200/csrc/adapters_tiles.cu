@@ -6,8 +6,11 @@
 // columns   c + terms B^T: items of 128 rows x 128 columns, dealt out in order, so a CTA keeps the terms of its rows in shared memory while it
 //           goes along the columns.  One warp brings B, one issues, eight add c, which they load while the product is made, and store.
 //
-// Bound by HBM (x, c, out once): mma.sync would need the whole time for the products at R = 64 (7000 rows, K 4096, N 8192: 43 us at its rate, which is the
-// floor too; a kernel of adapters.cu's kind took 330).
+// Why not in one: the columns need all of K, and a CTA that made the sums for itself would read x as often as there are CTAs along the columns.  Why not mma.sync:
+// at R = 64 its rate is the whole time (7000 rows, K 4096, N 8192: 43 us, the floor at HBM's rate too; the kernel of adapters.cu took 330, with loads that nothing hid).
+//
+// Bound by HBM (x, c and the result once) and by a chain of barriers, MMAs and adding warps beside it: 67 us for these rows, 17 the sums (3.3 TB/s: 220 CTAs on 148 SMs, and 5
+// us of tables, meeting and terms), 45 the columns (5 TB/s; 30 without their loads and stores).
 #include <algorithm>
 
 #include "adapters.cuh"
@@ -86,7 +89,8 @@ __global__ void __launch_bounds__(kSumThreads)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Tile found = find_tile<kSumThreads>(p, tile, kRows, tile == 0);
-  if (tile == 0 && rank == 0 && tid == 0) *work.count = found.counted;
+  // (no more than there are places: sequences behind one whose rows are out of range may name rows again)
+  if (tile == 0 && rank == 0 && tid == 0) *work.count = min(found.counted, (int)gridDim.x / ctas);
   if (found.seq < 0) return;  // (the whole cluster, here and below)
   const int which = adapter_of(p, found.seq);
   if (rank == 0 && tid == 0) work.tiles[tile] = make_int4(found.row, found.rows, which, 0);

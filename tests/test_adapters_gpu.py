@@ -161,6 +161,13 @@ def test_tables_out_of_range():
             lo, hi = starts[s], starts[s + 1]
             if 0 <= lo <= hi <= 9 and starts[s:s + 2] == [0, 3, 7, 9][s:s + 2]:
                 assert not torch.equal(out[lo:hi], c[lo:hi])
+    # long sequences: behind one out of range all rows come again, more tiles than there are places for
+    r = Requests([1024, 0, 0], 64, 40, 8, 2, seed=5)
+    x, a, b, c = (t.cuda()[..., s] for t, s in zip(r.whole, r.cut))
+    starts, which = torch.tensor([0, 1024, 1024, 1024], dtype=torch.int32).cuda(), torch.tensor([1, 1, 1], dtype=torch.int32).cuda()
+    want = F.adapter_gemm(x, a, b, c, starts, which)
+    F.cache_check()
+    assert torch.equal(says([0, 1024, 0, 1024], [1, 1, 1]), want)
 
 
 def test_refusals():

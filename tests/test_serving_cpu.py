@@ -28,6 +28,14 @@ def test_workspace_sizes_say_what_is_refused():
     assert size(_cache(), 3) == 0 and size(_cache(), -1) == 0
 
 
+def test_adapters_beyond_the_limits_need_no_workspace():
+    def size(rows, n, rank=8):
+        return capi.adapter_workspace_bytes(capi.AdapterDesc(rows, 64, n, 64, 64, 64 * rank, rank, rank * n, n, n, rank, 1, 1, capi.BF16, capi.BF16))
+
+    assert size(1 << 26, 64) >= (1 << 26) * 8 * 2 * 2 and size((1 << 26) + 1, 64) == 0
+    assert size(512, 1 << 28) > 0 and size(512, (1 << 28) + 8) == 0 and size(512, 64, 12) == 0 and size(512, 64, 136) == 0
+
+
 def test_null_contexts_are_refused():
     lib = capi.load()
     t = capi.PageTables(1 << 20, 1 << 21, 1 << 22, 1 << 23, 4)
