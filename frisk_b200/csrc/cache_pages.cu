@@ -12,7 +12,8 @@
 // keep     a block a sequence; a thread has one 16-byte column of the rows and moves it row by row: row kept[i] >= i comes to row i, so
 //          no store meets a row that is still to be read
 //
-// Bound by HBM where pages are copied (copy of 1400 pages of 256 KB: 6.2 TB/s read and written), else by launches and a few dependent loads.
+// Bound by HBM where pages are copied (1400 pages of 256 KB: 126 us, 5.8 TB/s read and written; 2000 of 9000 pages of 33 KB moved together: 33 us, 22 of them
+// the copy at 6.1 TB/s, 10 the plan), else by launches and chains of dependent loads (fork of 16 rows 4.5 us, plan of grow for 16 sequences 8.7, for 192 10.9).
 #include <algorithm>
 
 #include "cache_common.cuh"
@@ -214,9 +215,10 @@ struct GrowWork {
   int *kind, *before;  // [T], [T + 1]: what becomes of the slot; pages taken by those before it
   int *shared, *page;  // [T]: touched slots whose page others have too, and the page
   int *free;           // [T]
+  int *holders, *last; // [pages]: of the touched slots whose page others have too, those with that page, and the last
   static constexpr int kSmall = 1536;  // touched slots whose lists are in shared memory
-  __host__ __device__ static int64_t ints(int64_t batch, int64_t width) { return 5 * batch + 1 + 5 * batch * width + 1; }
-  __device__ GrowWork(int* ws, int64_t batch, int64_t width) {
+  __host__ __device__ static int64_t ints(int64_t batch, int64_t width, int64_t pages) { return 5 * batch + 1 + 5 * batch * width + 1 + 2 * pages; }
+  __device__ GrowWork(int* ws, int64_t batch, int64_t width, int64_t pages) {
     const int64_t slots = batch * width;
     copies = ws;
     offset = copies + 3 * batch;
@@ -226,6 +228,8 @@ struct GrowWork {
     shared = before + slots + 1;
     page = shared + slots;
     free = page + slots;
+    holders = free + slots;
+    last = holders + pages;
   }
 };
 
@@ -236,7 +240,7 @@ __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
   __shared__ int sums[32];
   __shared__ int near[kSearched + 1];  // offsets, where they fit
   extern __shared__ int lists[];       // five of kSmall, and one place
-  GrowWork w(t.ws, t.batch, t.width);
+  GrowWork w(t.ws, t.batch, t.width, t.pages);
   const int tid = threadIdx.x, lane = tid & 31;
   pdl_begin();
   if (COPIES && blockIdx.x > 0) {
@@ -319,15 +323,40 @@ __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
     n_shared += total;
   }
   __syncthreads();
-  // 3. of the sequences that are going to write into a page, all take one of their own but the last that has it
-  for (int k = tid; k < n_shared; k += kPlan) {
-    const int page = w.page[k];
-    int earlier = 0;
+  // 3. of the sequences that are going to write into a page, all take one of their own but the last that has it, if no one else does
+  auto decide = [&](int k, int page, int holders, bool last) {  // of the touched slots with that page: how many, and whether k is the last
+    const int users = t.users[page];
+    if (users < holders) flag(t.status, ST_CACHE_PAGE);  // (it has more users than are said: left)
+    else if (users > holders || !last) w.kind[w.shared[k]] = SWAP;
+    else w.kind[w.shared[k]] = KEEP_AS_LAST;
+  };
+  if (all <= GrowWork::kSmall) {
+    for (int k = tid; k < n_shared; k += kPlan) {
+      const int page = w.page[k];
+      int holders = 0, later = 0;
 #pragma unroll 8
-    for (int j = 0; j < k; ++j) earlier += w.page[j] == page;
-    const int i = w.shared[k];
-    if (t.users[page] - earlier > 1) w.kind[i] = SWAP;
-    else if (earlier) w.kind[i] = KEEP_AS_LAST;
+      for (int j = 0; j < n_shared; ++j) {
+        const int same = w.page[j] == page;
+        holders += same;
+        later += same & (int)(j > k);
+      }
+      decide(k, page, holders, later == 0);
+    }
+  } else {  // (pair by pair, 10^5 of them would take seconds)
+    for (int k = tid; k < n_shared; k += kPlan) {
+      w.holders[w.page[k]] = 0;
+      w.last[w.page[k]] = -1;
+    }
+    __syncthreads();
+    for (int k = tid; k < n_shared; k += kPlan) {
+      atomicAdd(w.holders + w.page[k], 1);
+      atomicMax(w.last + w.page[k], k);
+    }
+    __syncthreads();
+    for (int k = tid; k < n_shared; k += kPlan) {
+      const int page = w.page[k];
+      decide(k, page, __ldcg(w.holders + page), __ldcg(w.last + page) == k);
+    }
   }
   __syncthreads();
   // 4. how many pages are taken before each slot
@@ -697,7 +726,7 @@ constexpr int64_t kCopiedTogether = 1 << 17;  // entries that a cluster copies i
 int64_t workspace_ints(const frisk_b200_cache_desc* c, int which) {
   const int64_t batch = c->batch, width = c->table_width;
   if (which == FORK && batch * width <= kForkTogether && batch <= kTogether * kPlan && c->pages <= kCopiedTogether) return 0;
-  return which == FORK ? batch * width + batch : which == GROW ? GrowWork::ints(batch, width) : 1 + 3 * c->pages;
+  return which == FORK ? batch * width + batch : which == GROW ? GrowWork::ints(batch, width, c->pages) : 1 + 3 * c->pages;
 }
 int check_sizes(const frisk_b200_cache_desc* c, int which) {
   const int rc = cache_validate(c);

@@ -161,6 +161,32 @@ def test_grow_is_granted_in_order():
         assert [t.tolist() for t in got] == list(so.grow(users, table, [0, 1, 2, 3], [4, 4, 4], 16)[:3])
 
 
+@pytest.mark.parametrize("batch,slots", [(3, 200), (4, 500), (40, 2500)])
+def test_grow_over_many_shared_pages(batch, slots):
+    """Rows that name the pages their new keys go to, all of them shared: the last row keeps what no one else has."""
+    import torch
+    import frisk_b200 as F
+    others = [p % 7 == 0 for p in range(slots)]
+    users, table, lengths = [batch + o for o in others] + [0] * batch * slots, [list(range(slots)) for _ in range(batch)], [3 + b % 12 for b in range(batch)]
+    starts = [0]
+    for n in lengths:
+        starts.append(starts[-1] + slots * 16 - n)
+    cache = F.paged_cache(len(users), 1, 16, 64, torch.float8_e4m3fn)
+    got = F.cache_grow(cache, ints(users), ints(table), ints(starts), ints(lengths))
+    F.cache_check()
+    want = so.grow(users, table, starts, lengths, 16)
+    assert [t.tolist() for t in got] == list(want[:3])
+    # tables that name a page more often than is said: such pages are left
+    few = [2 if p % 5 == 0 else n for p, n in enumerate(users[:slots])] + users[slots:]
+    got = F.cache_grow(cache, ints(few), ints(table), ints(starts), ints(lengths))
+    with pytest.raises(RuntimeError, match="table"):
+        F.cache_check()
+    left = torch.arange(0, slots, 5, device="cuda", dtype=torch.int32)
+    assert torch.equal(got[1][:, ::5], left.expand(batch, -1)) and bool((got[0][left.long()] == 2).all())
+    rest = torch.tensor([p for p in range(slots) if p % 5 and not others[p]], device="cuda")
+    assert torch.equal(got[1][-1, rest], rest.int()) and bool((got[0][rest] == 1).all()) and bool((got[1][:-1, rest] >= slots).all())
+
+
 @pytest.mark.parametrize("pages,page,held", [(1, 16, "bfloat16"), (33, 16, "float8_e4m3fn"), (700, 64, "float16"), (9001, 16, "float8_e4m3fn"), (257, 1024, "bfloat16")])
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("full", [0.0, 0.3, 0.9, 1.0])
