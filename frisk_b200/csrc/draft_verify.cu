@@ -33,6 +33,7 @@ constexpr int kWarps = 8, kThreads = 32 * kWarps, kMostParts = kMostCtas * kWarp
 constexpr int kAhead = 4;  // steps a warp has in flight
 constexpr int kLane = 8, kStep = 32 * kLane;  // values a lane and a warp look at in a step
 constexpr int kMaxNodes = 1024;
+enum : unsigned { ST_VERIFY = 0x315 };  // a wait
 
 struct VerifyParams {
   const void* tokens;
@@ -81,7 +82,40 @@ __device__ __forceinline__ double less(double w, double mass, double q) {
   return x > 0.0 ? x : 0.0;
 }
 
-__device__ __forceinline__ void st_cluster_f64(uint32_t addr, double x) { asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(x) : "memory"); }
+// x to a CTA of the cluster, and its 8 bytes to a barrier there
+__device__ __forceinline__ void send(uint32_t addr, double x, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(addr), "l"(__double_as_longlong(x)), "r"(bar) : "memory");
+}
+// A bounded wait of a whole warp for what the cluster sends.
+__device__ __forceinline__ bool received(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return __all_sync(0xffffffffu, ok != 0);
+}
+__device__ __forceinline__ void wait_for(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, unsigned* status) {
+  if (received(bar, parity)) return;
+  const unsigned long long t0 = globaltimer();
+  for (uint32_t spins = 1; !received(bar, parity); ++spins) {
+    if (spins & 63u) continue;
+    bool stop = *abort_flag != 0;
+    if (!stop && globaltimer() - t0 > kWaitBudgetNs) {
+      *abort_flag = 1;
+      atomicCAS(status, 0u, ST_VERIFY);
+      stop = true;
+    }
+    if (__any_sync(0xffffffffu, stop)) {
+      const unsigned long long t1 = globaltimer();  // what is still in flight has time to land
+      while (globaltimer() - t1 < 200000ull) __nanosleep(1000);
+      return;
+    }
+  }
+}
 
 __device__ __forceinline__ double warp_sum(double x) {
 #pragma unroll
@@ -93,6 +127,8 @@ template <typename T, bool DRAFT>
 __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams p) {
   extern __shared__ int nodes[];  // of every node: token, parent, weight there, the draft's, random number; then masses or tokens taken off
   __shared__ double part_sums[2][kMostParts], eighths[kWarps];
+  __shared__ uint64_t arrived[2];  // all parts of a sum
+  __shared__ uint32_t abort_word;
   __shared__ int n_off;
   int *token = nodes, *parent = token + p.max_new;
   float *at_target = reinterpret_cast<float*>(parent + p.max_new), *at_draft = at_target + p.max_new, *random = at_draft + p.max_new;
@@ -102,6 +138,12 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams 
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.x / p.ctas;
   const int rank = (int)cluster_ctarank();
+  if (tid == 0) {
+    mbar_init(&arrived[0], 1);
+    mbar_init(&arrived[1], 1);
+    abort_word = 0;
+    mbar_fence_init();
+  }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int first = p.starts[b], last = p.starts[b + 1];
@@ -212,16 +254,19 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams 
   };
   const int step0 = min(steps, (rank * kWarps + warp) * each), step1 = min(steps, step0 + each);
   int turn = 0;
+  uint32_t phases = 0;
   // The sum of the weights; the parts' stay in part_sums[turn ^ 1].  The whole cluster calls it.
   auto sum = [&]() {
     const double part = warp_sum(lane_sum(step0, step1));
-    if (lane < p.ctas) st_cluster_f64(mapa_addr(smem_u32(&part_sums[turn][rank * kWarps + warp]), lane), part);
+    if (tid == 0) mbar_expect_tx(&arrived[turn], parts * 8);
+    if (lane < p.ctas) send(mapa_addr(smem_u32(&part_sums[turn][rank * kWarps + warp]), lane), part, mapa_addr(smem_u32(&arrived[turn]), lane));
     __syncwarp();
-    cluster_sync_all();
+    wait_for(&arrived[turn], phases >> turn & 1, &abort_word, p.status);
+    phases ^= 1u << turn;
     double all = 0.0;
     for (int i = lane; i < parts; i += 32) all += part_sums[turn][i];
     all = warp_sum(all);
-    turn ^= 1;  // (two sets: a CTA may be one call ahead)
+    turn ^= 1;  // (two sets: a warp may be one call ahead)
     return all;
   };
 
@@ -337,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams 
     return kEach * who + __shfl_sync(0xffffffffu, mine, who);
   };
   const int part = pick(part_sums[turn ^ 1], parts);
-  if (part / kWarps != rank) return;  // (nobody writes into a CTA that has gone: all sums were behind a barrier of the cluster)
+  if (part / kWarps != rank) return;  // (nobody writes into a CTA that has gone: it has received all parts of the last sum)
   // its eighths, a warp each
   const int from = min(steps, part * each), to = min(steps, from + each), piece = (to - from + kWarps - 1) / kWarps;
   const int mine0 = min(to, from + warp * piece), mine1 = min(to, mine0 + piece);
