@@ -26,6 +26,7 @@ namespace {
 using namespace adapter;
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kChain = 4;  // blocks of 32 of the inner index that an accumulator takes
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if (std::is_same<T, __half>::value)
@@ -106,17 +107,23 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
   const int my_row = mw * 16 * MW;
 
   // ---- x A^T over this CTA's part of K, shared by kShare warps in turns of 32
-  float acc[MW][P::kTiles][4];
-#pragma unroll
-  for (int m = 0; m < MW; ++m)
-#pragma unroll
-    for (int t = 0; t < P::kTiles; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[m][t][i] = 0.f;
+  // (The tensor cores cut what an addition leaves below 24 bits, always towards zero, some 2e-8 of the result each time.  Where the result has 32 bits an accumulator
+  // takes kChain blocks, and the parts are summed up rounding to nearest, in shared memory.)
   const int blocks_k = (p.K + 31) / 32, k0 = (int)((int64_t)blocks_k * rank / C_), k1 = (int)((int64_t)blocks_k * (rank + 1) / C_);
-  if (my_row < rows) {
+  constexpr bool kExact = sizeof(C) == 4;
+  int kb = my_row < rows ? k0 + share : k1;
+  bool begun = false;
+  do {
+    float acc[MW][P::kTiles][4];
+#pragma unroll
+    for (int m = 0; m < MW; ++m)
+#pragma unroll
+      for (int t = 0; t < P::kTiles; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][t][i] = 0.f;
+    const int end = kExact ? min(k1, kb + kChain * P::kShare) : k1;
 #pragma unroll 2
-    for (int kb = k0 + share; kb < k1; kb += P::kShare) {
+    for (; kb < end; kb += P::kShare) {
       const int k = kb * 32 + q * 8, left = p.K - k;
       uint4 xa[MW][2], w[P::kTiles];
 #pragma unroll
@@ -137,15 +144,18 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
           for (int t = 0; t < P::kTiles; ++t) mma<T>(acc[m][t], fa, word(w[t], 2 * s), word(w[t], 2 * s + 1));
         }
     }
-  }
 #pragma unroll
-  for (int m = 0; m < MW; ++m)
+    for (int m = 0; m < MW; ++m)
 #pragma unroll
-    for (int t = 0; t < P::kTiles; ++t) {
-      float* to = sums + (share * P::kRows + my_row + 16 * m + g) * P::kPitch + 8 * t + 2 * q;
-      *reinterpret_cast<float2*>(to) = make_float2(acc[m][t][0], acc[m][t][1]);
-      *reinterpret_cast<float2*>(to + 8 * P::kPitch) = make_float2(acc[m][t][2], acc[m][t][3]);
-    }
+      for (int t = 0; t < P::kTiles; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float2* to = reinterpret_cast<float2*>(sums + (share * P::kRows + my_row + 16 * m + 8 * h + g) * P::kPitch + 8 * t + 2 * q);
+          const float2 old = kExact && begun ? *to : make_float2(0.f, 0.f);
+          *to = make_float2(old.x + acc[m][t][2 * h], old.y + acc[m][t][2 * h + 1]);
+        }
+    begun = true;
+  } while (kExact && kb < k1);
   __syncthreads();
   // ---- parts added up: the CTA's warps, then the CTAs, each in their order
   const int quads = RMAX / 4, n_quads = rows * quads;
@@ -228,13 +238,17 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
         const int r = my_row + 16 * m + 8 * h + g;
         old[m][h].load(c + r * p.ldc + col, r < rows ? left : 0, p.wide);
       }
-    float d[MW][4][4];
+    // (the smaller terms apart, so that chains of cut additions are half as long)
+    float d[MW][4][4], low[kExact ? MW : 1][4][4];
 #pragma unroll
     for (int m = 0; m < MW; ++m)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[m][j][i] = 0.f;
+        for (int i = 0; i < 4; ++i) {
+          d[m][j][i] = 0.f;
+          if (kExact) low[m][j][i] = 0.f;
+        }
 #pragma unroll
     for (int kb = 0; kb < P::kBlocks; ++kb) {
       uint4 w[4];
@@ -252,7 +266,7 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
             const uint4 f = terms[((((my_row / 16 + m) * P::kBlocks + kb) * 2 + s) * P::kTerms + t) * 32 + lane];
             const uint32_t fa[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mma<T>(d[m][j], fa, word(w[j], 2 * s), word(w[j], 2 * s + 1));
+            for (int j = 0; j < 4; ++j) mma<T>(kExact && t > 0 ? low[m][j] : d[m][j], fa, word(w[j], 2 * s), word(w[j], 2 * s + 1));
           }
     }
 #pragma unroll
@@ -263,7 +277,10 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
         if (r >= rows) continue;
         float y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = fmaf(alpha, d[m][j / 2][2 * h + j % 2] * up[m][h], old[m][h][j]);
+        for (int j = 0; j < 8; ++j) {
+          const float sum = d[m][j / 2][2 * h + j % 2] + (kExact ? low[m][j / 2][2 * h + j % 2] : 0.f);
+          y[j] = fmaf(alpha, sum * up[m][h], old[m][h][j]);
+        }
         store_eight<C>(out + r * p.ldo + col, y, left, p.wide);
       }
   }

@@ -21,7 +21,7 @@ namespace fb {
 namespace {
 using namespace adapter;
 
-enum : unsigned { ST_SUMS_EMPTY = 0x311, ST_SUMS_FULL = 0x312, ST_SUMS_DONE = 0x313, ST_COLUMNS = 0x314 };  // waits
+enum : unsigned { ST_SUMS_EMPTY = 0x311, ST_SUMS_FULL = 0x312, ST_SUMS_PART = 0x313, ST_COLUMNS = 0x314 };  // waits
 
 constexpr int kRows = 128;          // of a tile
 constexpr int kBoxBytes = kRows * 128;  // 128 rows of 64 16-bit elements
@@ -57,30 +57,36 @@ __device__ __forceinline__ void land(volatile uint32_t* abort_flag) {
 
 // ------------------------------------------------------------------------------------------------ sums
 constexpr int kSumStages = 4, kAdders = 8, kSumThreads = 64 + 32 * kAdders;
+// The tensor cores cut what an addition leaves below 24 bits, always towards zero, so a chain of n additions is off by some 2e-8 n of its result (K = 8192 in
+// two CTAs: 5e-6).  So no accumulator takes more than 8 steps of 16, and the adders sum up what they leave, rounding to nearest (3e-7).
+constexpr int kChain = 2;  // stages that an accumulator takes
 struct SumsLayout {  // of `width` columns, R rounded up to a multiple of 16
   static __host__ __device__ int stage_bytes(int width) { return kBoxBytes + width * 128; }
   static __host__ __device__ int pitch(int width) { return width + 4; }  // of rows of sums, floats
   static __host__ __device__ int bytes(int width) { return kSumStages * stage_bytes(width) + 1024; }
 };
 
-template <typename T, int kTerms>
+template <typename T, int kTerms, int kMost>  // kMost: the rank at most, 64 or 128
 __global__ void __launch_bounds__(kSumThreads)
     adapter_sums_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ AdapterParams p,
                         const __grid_constant__ Work work) {
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~static_cast<uintptr_t>(1023));
-  __shared__ uint64_t full_bar[kSumStages], empty_bar[kSumStages], done_bar;
+  __shared__ uint64_t full_bar[kSumStages], empty_bar[kSumStages], part_full[2], part_empty[2];
   __shared__ uint32_t tmem_slot, abort_word;
   volatile uint32_t* abort_flag = &abort_word;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, ctas = p.cluster, rank = (int)cluster_ctarank(), tile = blockIdx.x / ctas;
-  const int width = (p.R + 15) / 16 * 16, columns = width <= 32 ? 32 : width <= 64 ? 64 : 128, stage_bytes = SumsLayout::stage_bytes(width);
+  const int width = (p.R + 15) / 16 * 16, columns = width <= 16 ? 32 : width <= 32 ? 64 : width <= 64 ? 128 : 256, stage_bytes = SumsLayout::stage_bytes(width);
   if (tid == 0) {
     for (int i = 0; i < kSumStages; ++i) {
       mbar_init(&full_bar[i], 1);
       mbar_init(&empty_bar[i], 1);
     }
-    mbar_init(&done_bar, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&part_full[i], 1);
+      mbar_init(&part_empty[i], kAdders);
+    }
     abort_word = 0;
     mbar_fence_init();
     tma_prefetch_desc(&map_x);
@@ -119,40 +125,57 @@ __global__ void __launch_bounds__(kSumThreads)
   } else if (warp == 1) {
     const uint32_t idesc = umma_idesc_f16(kRows, width, kBf16, false, false), d = __shfl_sync(0xffffffffu, tmem, 0);
     for (int i = 0; i < n_k; ++i) {
-      const int stage = i % kSumStages;
+      const int stage = i % kSumStages, chain = i / kChain, acc = chain & 1;
+      if (i % kChain == 0 && chain >= 2 && !mbar_wait_warp(&part_empty[acc], (chain / 2 - 1) & 1, abort_flag, p.status, ST_SUMS_PART)) break;
       if (!mbar_wait_warp(&full_bar[stage], (i / kSumStages) & 1, abort_flag, p.status, ST_SUMS_FULL)) break;
       tc_fence_after_sync();
       const uint32_t at = smem_u32(smem + stage * stage_bytes);
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          umma_f16_ss(d, umma_desc_kmajor_sw128(at + k * 32), umma_desc_kmajor_sw128(at + kBoxBytes + k * 32), idesc, i > 0 || k > 0 ? 1u : 0u);
+          umma_f16_ss(d + acc * (columns / 2), umma_desc_kmajor_sw128(at + k * 32), umma_desc_kmajor_sw128(at + kBoxBytes + k * 32), idesc, i % kChain > 0 || k > 0 ? 1u : 0u);
         umma_commit(&empty_bar[stage]);
-        if (i + 1 == n_k) umma_commit(&done_bar);
+        if (i % kChain == kChain - 1 || i + 1 == n_k) umma_commit(&part_full[acc]);
       }
       __syncwarp();
     }
-  } else if (warp < 6) {
-    // this CTA's part into the ring, all of which has been read: lane = row
-    const int row = (warp & 3) * 32 + lane, pitch = SumsLayout::pitch(width);
-    float* mine = reinterpret_cast<float*>(smem) + row * pitch;
-    const bool there = n_k > 0 && mbar_wait_warp(&done_bar, 0, abort_flag, p.status, ST_SUMS_DONE);
-    tc_fence_after_sync();
-    for (int c = 0; c < width; c += 16) {
-      uint32_t v[16];
-      if (there) {
-        tmem_ld_32x32b_x16(tmem + c + ((uint32_t)((warp & 3) * 32) << 16), v);
+  } else {
+    // lane = row; a warp has every other 16 columns
+    constexpr int kGroups = kMost / 32;
+    const int row = (warp & 3) * 32 + lane, half = (warp - 2) >> 2, pitch = SumsLayout::pitch(width);
+    float sum[kGroups][16];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum[g][i] = 0.f;
+    const int chains = (n_k + kChain - 1) / kChain;
+    for (int chain = 0; chain < chains; ++chain) {
+      const int acc = chain & 1;
+      if (!mbar_wait_warp(&part_full[acc], (chain >> 1) & 1, abort_flag, p.status, ST_SUMS_PART)) break;
+      tc_fence_after_sync();
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const int c = (2 * g + half) * 16;
+        if (c >= width) break;
+        uint32_t v[16];
+        tmem_ld_32x32b_x16(tmem + acc * (columns / 2) + c + ((uint32_t)((warp & 3) * 32) << 16), v);
         tmem_ld_wait();
-      } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = 0;
+        for (int i = 0; i < 16; ++i) sum[g][i] += __uint_as_float(v[i]);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<float4*>(mine + c + 4 * i) =
-            make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&part_empty[acc]);
     }
-    tc_fence_before_sync();
+    // this CTA's part into the ring, all of which has been read
+    float* mine = reinterpret_cast<float*>(smem) + row * pitch;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const int c = (2 * g + half) * 16;
+      if (c >= width) break;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(mine + c + 4 * i) = make_float4(sum[g][4 * i], sum[g][4 * i + 1], sum[g][4 * i + 2], sum[g][4 * i + 3]);
+    }
   }
   __syncwarp();
   cluster_sync_all();  // every part is there (all roles of all CTAs end: their waits are bounded)
@@ -392,10 +415,10 @@ __global__ void __launch_bounds__(kColThreads, 1)
         const uint32_t at = smem_u32(smem), b = at + L::kTermBytes + stage * L::kStageBytes;
         if (elect_one()) {
 #pragma unroll
-          for (int n = 0; n < kTerms; ++n)
+          for (int n = kTerms - 1; n >= 0; --n)  // (the smallest first: what the additions cut off them is the less)
             for (int k = 0; k < steps; ++k) {
               const uint32_t in = (k >> 2) * kBoxBytes + (k & 3) * 32;
-              umma_f16_ss(d + acc * kColumns, umma_desc_kmajor_sw128(at + n * kHalves * kBoxBytes + in), umma_desc_kmajor_sw128(b + in), idesc, n > 0 || k > 0 ? 1u : 0u);
+              umma_f16_ss(d + acc * kColumns, umma_desc_kmajor_sw128(at + n * kHalves * kBoxBytes + in), umma_desc_kmajor_sw128(b + in), idesc, n < kTerms - 1 || k > 0 ? 1u : 0u);
             }
           umma_commit(&b_empty[stage]);
           umma_commit(&acc_full[acc]);
@@ -576,9 +599,9 @@ int launch_both(frisk_b200_ctx* ctx, AdapterParams p, const Work& work, cudaStre
   if (out_by_tma) bad |= encode_tmap_2d(ctx, &map_out, dtype_c, p.out, p.N, p.rows, p.ldo * sizeof(C), U, 8, true);
   if (bad) return FRISK_B200_E_CUDA;
   static PerDeviceOnce once_sums, once_columns;
-  auto sums = adapter_sums_kernel<T, kTerms>;
+  auto sums = adapter_sums_kernel<T, kTerms, 64 * kHalves>;
   auto columns = adapter_columns_kernel<T, C, kHalves>;
-  FB_CUDA(ctx, allow(once_sums, ctx->device, sums, SumsLayout::bytes(kMaxRank)));
+  FB_CUDA(ctx, allow(once_sums, ctx->device, sums, SumsLayout::bytes(64 * kHalves)));
   FB_CUDA(ctx, allow(once_columns, ctx->device, columns, L::kBytes));
   const int64_t tiles = most_tiles(p.rows, p.batch), items = tiles * ((p.N + kColumns - 1) / kColumns);
   p.cluster = kMostCtas;

@@ -129,6 +129,27 @@ def test_what_is_not_finite_stays_in_its_row():
         assert torch.equal(r.run().cpu(), plain)
 
 
+@pytest.mark.parametrize("batch,new", [(80, 128), (2, 300), (64, 1), (130, 20)])
+@pytest.mark.parametrize("rank", [16, 128])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_long_sums(dtype, rank, batch, new):
+    """32-bit results of an inner index of 8192.  Tensor cores cut what an addition leaves below 24 bits: less than 2 u of the accumulator, u = 2^-24.  In the norm
+    over all results, where a sum's beginning is no larger than the sum, chains of 8 additions are off by at most 16 u, in two products 32 u; the terms that a
+    sum becomes leave 4 u, and adding up 64 parts, each time rounded by u, in random directions, 8 u.  (One chain over half of the index would be off by 256 u and more.)"""
+    import torch
+    import frisk_b200 as F
+    k, n, t = 8192, 256, getattr(torch, dtype)
+    torch.manual_seed(rank + batch)
+    x, a, b = torch.randn(batch * new, k, device="cuda").to(t), torch.randn(2, rank, k, device="cuda").to(t), torch.randn(2, n, rank, device="cuda").to(t)
+    starts, which = torch.arange(batch + 1, dtype=torch.int32, device="cuda") * new, torch.arange(batch, dtype=torch.int32, device="cuda") % 2
+    got = F.adapter_gemm(x, a, b, torch.zeros(batch * new, n, device="cuda"), starts, which).double()
+    F.cache_check()
+    for w in range(2):
+        rows = (which == w).repeat_interleave(new)
+        want = x[rows].double() @ a[w].double().t() @ b[w].double().t()
+        assert float((got[rows] - want).norm() / want.norm()) <= 44 * 2.0 ** -24
+
+
 def test_the_same_result_every_time():
     import torch
     r = Requests([1, 5, 70, 200, 0, 3], 1500, 700, 32, 4, seed=8)
