@@ -9,7 +9,7 @@
 // Why not in one: the columns need all of K, and a CTA that made the sums for itself would read x as often as there are CTAs along the columns.  Why not mma.sync:
 // at R = 64 its rate is the whole time (7000 rows, K 4096, N 8192: 43 us, the floor at HBM's rate too; the kernel of adapters.cu took 330, with loads that nothing hid).
 //
-// Bound by HBM (x, c and the result once) and by a chain of barriers, MMAs and adding warps beside it: 67 us for these rows, 17 the sums (3.3 TB/s: 220 CTAs on 148 SMs, and 5
+// Bound by HBM (x, c and the result once) and by a chain of barriers, MMAs and adding warps beside it: 67 us for these rows, 17 the sums (3.3 TB/s: 236 CTAs on 148 SMs, and 5
 // us of tables, meeting and terms), 45 the columns (5 TB/s; 30 without their loads and stores).
 #include <algorithm>
 

@@ -12,8 +12,8 @@
 // keep     a block a sequence; a thread has one 16-byte column of the rows and moves it row by row: row kept[i] >= i comes to row i, so
 //          no store meets a row that is still to be read
 //
-// Bound by HBM where pages are copied (1400 pages of 256 KB: 126 us, 5.8 TB/s read and written; 2000 of 9000 pages of 33 KB moved together: 33 us, 22 of them
-// the copy at 6.1 TB/s, 10 the plan), else by launches and chains of dependent loads (fork of 16 rows 4.5 us, plan of grow for 16 sequences 8.7, for 192 10.9).
+// Bound by HBM where pages are copied (1400 pages of 256 KB: 128 us, 5.7 TB/s read and written; 2000 of 9000 pages of 33 KB moved together: 31 us, 22 of them
+// the copy at 6.1 TB/s, the rest the plan), else by launches and chains of dependent loads (fork of 16 rows 4.5 us, plan of grow for 16 sequences 8.7, for 192 10.9).
 #include <algorithm>
 
 #include "cache_common.cuh"
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(kMove) grow_copy_kernel(const int* copies, uin
 // ------------------------------------------------------------------------------------------------ whole pages
 // The workspace of compact: moves, then from [pages], to [pages], goes [pages].  With n used pages, u(p) of them before page p, a free page p < n is hole
 // p - u(p), and a used one p >= n is move u(p) - u(n): one scan gives both.  A warp has neighbouring pages, 32 at a time, the first kHold of these
-// words in registers (up to 16384 pages are read once).  9000 pages: 6 us; in two scans, with lists in memory, 10.
+// words in registers (up to 16384 pages are read once).  2000 of 9000 pages of 33 KB: 31.4 us with the move; in two scans, with lists in memory, 33.5.
 constexpr int kHold = 16;
 constexpr int kNear = 2560;  // moves whose lists are in shared memory too
 __global__ void __launch_bounds__(kPlan) compact_plan_kernel(const PageTables t) {
