@@ -158,6 +158,33 @@ def test_the_same_result_every_time():
         assert torch.equal(r.run(), first)
 
 
+@pytest.mark.parametrize("new", [35, 7000])
+def test_offsets_beyond_32_bits(new):
+    """Rows of c and the result behind the first 2^31 elements, and adapters behind them: as those by themselves."""
+    import torch
+    import frisk_b200 as F
+    rows, k, n, t = 70000, 64, 32768, torch.bfloat16
+    torch.manual_seed(new)
+    x, a, b = torch.randn(rows, k, device="cuda").to(t), torch.randn(2, 16, k, device="cuda").to(t), torch.randn(2, n, 16, device="cuda").to(t)
+    c = torch.zeros(rows, n, dtype=t, device="cuda")
+    c[-new:] = torch.randn(new, n, device="cuda").to(t)
+    starts = torch.arange(rows // new + 1, dtype=torch.int32, device="cuda") * new
+    which = torch.arange(rows // new, dtype=torch.int32, device="cuda") % 2
+    got = F.adapter_gemm(x, a, b, c, starts, which)
+    few = F.adapter_gemm(x[-new:].clone(), a, b, c[-new:].clone(), starts[:2], which[-1:])
+    assert torch.equal(got[-new:], few)
+    del c, got
+    a = torch.zeros(20000, 16, 8192, dtype=t, device="cuda")
+    a[-1] = torch.randn(16, 8192, device="cuda").to(t)
+    x = torch.randn(new, 8192, device="cuda").to(t)
+    b = torch.randn(20000, 8, 16, device="cuda").to(t)
+    c = torch.zeros(new, 8, device="cuda")
+    got = F.adapter_gemm(x, a, b, c, starts[:2], which[:1] * 0 + 19999)
+    few = F.adapter_gemm(x, a[-1:].clone(), b[-1:].clone(), c, starts[:2], which[:1] * 0)
+    F.cache_check()
+    assert torch.equal(got, few) and bool(got.any())
+
+
 def test_tables_out_of_range():
     import torch
     import frisk_b200 as F

@@ -164,6 +164,24 @@ def test_trees_as_they_come():
     assert d.run() == d.want()
 
 
+def test_offsets_beyond_32_bits():
+    """Rows behind the first 2^31 values: as those rows by themselves."""
+    import torch
+    import frisk_b200 as F
+    rows, vocab, n = 12000, 200000, 9
+    both = [torch.zeros(rows, vocab, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    torch.manual_seed(3)
+    for t in both:
+        t[-n:] = torch.rand(n, vocab, device="cuda").bfloat16()
+    tokens, accept, sample = torch.randint(0, vocab, (rows,), device="cuda"), torch.rand(rows, device="cuda"), torch.rand(2, device="cuda")
+    starts = torch.tensor([rows - n, rows - 4, rows], dtype=torch.int32, device="cuda")
+    for draft in (False, True):
+        got = F.draft_verify(tokens, None, starts, both[0], both[1] if draft else None, accept, sample, max_new=6)
+        few = F.draft_verify(tokens[-n:].clone(), None, starts - (rows - n), both[0][-n:].clone(), both[1][-n:].clone() if draft else None, accept[-n:].clone(), sample, max_new=6)
+        F.cache_check()
+        assert all(torch.equal(a, b) for a, b in zip(got, few)) and bool((got[2] >= 0).all())
+
+
 def test_rows_out_of_range_are_left_out():
     import frisk_b200 as F
     d = Drafts([3, 5, 2], 40)

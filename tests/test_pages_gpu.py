@@ -322,6 +322,43 @@ def test_what_tables_hold_out_of_range_is_left_out():
     assert same(cpu, cache)
 
 
+def test_offsets_beyond_32_bits():
+    """Pages behind the first 2^32 bytes and 2^31 elements of keys."""
+    import torch
+    import frisk_b200 as F
+    n, heads, page, d = 70000, 4, 64, 128
+    cache = F.paged_cache(n, heads, page, d, torch.bfloat16)
+    marks = torch.randn(2, 6, heads, page, d, device="cuda").bfloat16()
+    at = [n - 1, n - 2, n - 3, 5, n - 4, n - 5]
+    for t, m in zip(cache, marks):
+        t.zero_()
+        for i, p in enumerate(at[:4]):
+            t[p] = m[i]
+    # copied: the first backwards and the last forwards
+    F.cache_copy(cache, ints([5, n - 1]), ints([n - 4, 6]))
+    assert all(torch.equal(t[n - 4], m[3]) and torch.equal(t[6], m[0]) for t, m in zip(cache, marks))
+    # a shared last page is written: its keys go to the only free page
+    users = torch.ones(n, dtype=torch.int32, device="cuda")
+    users[n - 2], users[n - 5] = 2, 0
+    table = ints([[n - 2, -1], [n - 2, -1]])
+    users, table, granted = F.cache_grow(cache, users, table, ints([0, 1, 1]), ints([50, 50]))
+    assert table.tolist() == [[n - 5, -1], [n - 2, -1]] and granted.tolist() == [1, 0] and int(users[n - 5]) == 1
+    assert all(torch.equal(t[n - 5, :, :50], m[1, :, :50]) for t, m in zip(cache, marks))
+    # accepted rows move within the page, and over its end
+    got = F.cache_keep(cache, ints([[n - 3, n - 1]]), ints([0, 8]), ints([62]), ints([[0, 3, 7]]), ints([3]))
+    assert got.tolist() == [65]
+    for t, m in zip(cache, marks):
+        assert torch.equal(t[n - 3, :, :63], m[2, :, :63]) and torch.equal(t[n - 3, :, 63], m[0, :, 1])
+        assert torch.equal(t[n - 1, :, 0], m[0, :, 5]) and torch.equal(t[n - 1, :, 1:], m[0, :, 1:])
+    # the last page comes to the front
+    users = torch.zeros(n, dtype=torch.int32, device="cuda")
+    users[n - 2] = 3
+    users, table, used = F.cache_compact(cache, users, ints([[n - 2, -1]]))
+    F.cache_check()
+    assert table.tolist() == [[0, -1]] and used.tolist() == [1] and int(users[0]) == 3 and int(users.sum()) == 3
+    assert all(torch.equal(t[0], m[1]) for t, m in zip(cache, marks))
+
+
 def test_refusals():
     import torch
     import frisk_b200 as F
