@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
   const Tile found = find_tile<kThreads>(p, tile, P::kRows, false);
   if (found.seq < 0) return;  // (the whole cluster: there are fewer tiles than clusters)
   const int64_t row0 = found.row;
-  const int rows = found.rows, which = adapter_of(p, found.seq);
+  const int rows = found.rows, which = found.which;
   const C* c = static_cast<const C*>(p.c) + row0 * p.ldc;
   C* out = static_cast<C*>(p.out) + row0 * p.ldo;
   const int blocks_n = (p.N + 31) / 32, n0 = (int)((int64_t)blocks_n * rank / C_), n1 = (int)((int64_t)blocks_n * (rank + 1) / C_);

@@ -106,19 +106,21 @@ __device__ __forceinline__ void store_eight(C* at, const float (&v)[8], int n, b
 // is the same in all of them.  `everything`: all tiles are counted.
 struct Tile {
   int seq, row, rows;  // seq < 0: there are fewer
+  int which;           // the sequence's adapter; -1: none
   int counted;         // tiles up to here; all, where `everything` is asked for
 };
 template <int kThreads>
 __device__ __forceinline__ Tile find_tile(const AdapterParams& p, int tile, int tile_rows, bool everything) {
-  __shared__ int sums[kThreads / 32], found[3];
+  __shared__ int sums[kThreads / 32], found[4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) found[0] = -1;
   int before = 0;
   for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
     const int b = b0 + tid;
-    int lo = 0, n = 0;
+    int lo = 0, n = 0, which = -1;
     if (b < p.batch) {
       lo = p.starts[b];
+      which = p.adapters[b];  // (on its way at the same time)
       const int64_t many = (int64_t)p.starts[b + 1] - lo;
       if (lo < 0 || many < 0 || lo + many > p.rows) atomicCAS(p.status, 0u, cache::ST_CACHE_ROWS);
       else n = (int)many;
@@ -143,18 +145,13 @@ __device__ __forceinline__ Tile find_tile(const AdapterParams& p, int tile, int 
       found[0] = b;
       found[1] = lo + (tile - at) * tile_rows;
       found[2] = min(tile_rows, n - (tile - at) * tile_rows);
+      found[3] = which < p.count ? max(which, -1) : -1;
+      if (which >= p.count) atomicCAS(p.status, 0u, cache::ST_ADAPTER);
     }
     if (before > tile && !everything) break;  // (the same in all threads)
   }
   __syncthreads();
-  return Tile{found[0], found[1], found[2], before};
-}
-// a sequence's adapter; -1: none
-__device__ __forceinline__ int adapter_of(const AdapterParams& p, int seq) {
-  const int which = p.adapters[seq];
-  if (which < p.count) return max(which, -1);
-  if (threadIdx.x == 0) atomicCAS(p.status, 0u, cache::ST_ADAPTER);
-  return -1;
+  return Tile{found[0], found[1], found[2], found[3], before};
 }
 
 }  // namespace adapter

@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kSumThreads)
   // (no more than there are places: sequences behind one whose rows are out of range may name rows again)
   if (tile == 0 && rank == 0 && tid == 0) *work.count = min(found.counted, (int)gridDim.x / ctas);
   if (found.seq < 0) return;  // (the whole cluster, here and below)
-  const int which = adapter_of(p, found.seq);
+  const int which = found.which;
   if (rank == 0 && tid == 0) work.tiles[tile] = make_int4(found.row, found.rows, which, 0);
   if (which < 0) return;
   if (warp == 1) {
