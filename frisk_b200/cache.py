@@ -11,8 +11,9 @@ step can be replayed with other contents.  Their contents are checked by the ker
 """
 import contextlib
 
-from . import capi
-from .execute import _stream_ptr, _torch, context_for
+from . import calls, capi
+from .calls import context_for
+from .execute import _stream_ptr, _torch
 
 _CODES = _BYTE = _INT = None
 
@@ -131,6 +132,11 @@ def cache_write(cache, k, v, table, starts, lengths, *, stream=None):
     A 16-bit cache takes its own type.  A float8_e4m3fn cache is quantised as it is written: the scale of a token's head is the least
     power of two that brings its largest magnitude to 448 or less, codes are rounded to the nearest, ties to even; a row that holds an
     infinity or a NaN reads back as NaN.  A position must not be that of two rows (a page that two sequences name)."""
+    if stream is None:
+        r = calls.write(cache, k, v, table, starts, lengths)
+        if r is not None:
+            calls.result(r, k.get_device())
+            return cache
     desc, code, dev, heads, d = _describe(cache, table, starts, lengths, k.shape[0])
     given = _codes().get(k.dtype)
     if given is None or given == capi.E4M3 or v.dtype != k.dtype or v.shape != k.shape or (code != capi.E4M3 and code != given):

@@ -1,6 +1,6 @@
 """Loads ``_calls`` (``csrc/calls.cpp``): the usual calls of the serving operators, made natively.
 
-``verify``, ``change``, ``keep``, ``copy`` and ``adapters`` give an operator's results, an error number of the C ABI, or None where the Python functions
+``verify``, ``change``, ``keep``, ``copy``, ``adapters`` and ``write`` give an operator's results, an error number of the C ABI, or None where the Python functions
 have to look for themselves (and report what is wrong, if anything is): always where the extension is not built for this interpreter
 and this torch, which costs time and nothing else.
 """
@@ -13,7 +13,7 @@ import pathlib
 from . import capi, execute
 
 _FUNCTIONS = ("draft_verify", "cache_fork", "cache_grow", "cache_compact", "cache_pages_workspace_bytes", "cache_copy", "cache_keep", "adapter_gemm",
-              "adapter_workspace_bytes")
+              "adapter_workspace_bytes", "cache_write")
 
 
 def path(torch_version):
@@ -26,7 +26,7 @@ def _unknown(*_):
     return None
 
 
-verify = change = keep = copy = adapters = _unknown
+verify = change = keep = copy = adapters = write = _unknown
 _register, _known = None, set()
 
 
@@ -40,7 +40,7 @@ def context_for(device):
 
 
 def _know(device, context):
-    global verify, change, keep, copy, adapters, _register
+    global verify, change, keep, copy, adapters, write, _register
     if _register is None:
         import torch
         file = path(torch.__version__)
@@ -52,7 +52,7 @@ def _know(device, context):
         loader.exec_module(module)
         lib = capi.load()
         module.library(*(ctypes.cast(getattr(lib, "frisk_b200_" + name), ctypes.c_void_p).value for name in _FUNCTIONS))
-        verify, change, keep, copy, adapters, _register = module.verify, module.change, module.keep, module.copy, module.adapters, module.context
+        verify, change, keep, copy, adapters, write, _register = module.verify, module.change, module.keep, module.copy, module.adapters, module.write, module.context
     _register(device, context.handle.value)
 
 

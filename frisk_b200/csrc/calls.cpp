@@ -1,9 +1,9 @@
-// The usual calls of the serving operators made natively: a CPython module (no GPU code) that reads torch's tensors, makes the results, and calls
+// Usual calls of the serving operators made natively: a CPython module (no GPU code) that reads torch's tensors, makes the results, and calls
 // the C ABI.  A small call costs as much as its checks, attribute by attribute in Python, as its launch (12 us a call; 5 to 6 with this module), and nothing
 // may be remembered between calls, since a tensor's storage, shape and strides can be changed at any time.
 //
 // It only ever ACCEPTS: calls without `out` and `stream` whose tensors are plain ones (torch.Tensor itself) of the types, shapes and strides that
-// drafts.py, pages.py and adapters.py take.  Anything else, whether it is wrong or merely unusual, gives None, and the Python
+// drafts.py, pages.py, adapters.py and cache.py's cache_write take.  Anything else, whether it is wrong or merely unusual, gives None, and the Python
 // functions decide and word the error.  An error of the C ABI comes back as its number.  No exception leaves this file.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -20,6 +20,7 @@
 namespace {
 
 constexpr int kDevices = 64;
+constexpr size_t kBeside = 1 << 16;  // bytes
 frisk_b200_ctx* contexts[kDevices] = {};
 
 // the C ABI, as the library that Python has loaded offers it
@@ -33,6 +34,7 @@ struct Abi {
   decltype(&frisk_b200_cache_keep) keep;
   decltype(&frisk_b200_adapter_gemm) adapters;
   decltype(&frisk_b200_adapter_workspace_bytes) adapters_workspace;
+  decltype(&frisk_b200_cache_write) write;
 } abi = {};
 
 struct Unusual {};  // left to Python
@@ -75,6 +77,23 @@ void rows_of(const at::Tensor& t, int dim, int dev) { require(t.dim() == dim && 
 at::Tensor made(at::IntArrayRef shape, at::ScalarType type, int dev) {
   return at::Tensor(at::detail::empty_cuda(shape, type, c10::Device(c10::kCUDA, (c10::DeviceIndex)dev), std::nullopt));
 }
+// Several results of a call in one allocation (each costs 0.8 us): tensors of their own on one storage, on 64 bytes
+struct Results {
+  at::Tensor held;
+  int64_t bytes = 0;
+  int64_t place(int64_t n) {  // of n more bytes
+    const int64_t at = bytes;
+    bytes += (n + 63) / 64 * 64;
+    return at;
+  }
+  void allocate(int dev) { held = made({bytes}, at::kByte, dev); }
+  at::Tensor at_place(int64_t place, at::IntArrayRef shape, at::ScalarType type) const {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(held.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(place / (int64_t)c10::elementSize(type));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+    return t;
+  }
+};
 void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
 
 int code_of(at::ScalarType t) {
@@ -183,7 +202,11 @@ PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int32_t* parents = a[1] == Py_None ? nullptr : static_cast<const int32_t*>(list(a[1], at::kInt, rows, dev));
     const int32_t* p_starts = static_cast<const int32_t*>(list(starts, at::kInt, batch + 1, dev));
     const float *accept = static_cast<const float*>(list(a[5], at::kFloat, rows, dev)), *sample = static_cast<const float*>(list(a[6], at::kFloat, batch, dev));
-    const at::Tensor kept = made({batch, max_new}, at::kInt, dev), counts = made({batch}, at::kInt, dev), next = made({batch}, tokens.scalar_type(), dev);
+    Results r;
+    const int64_t at_kept = r.place(batch * max_new * 4), at_counts = r.place(batch * 4), at_next = r.place(batch * 8);
+    r.allocate(dev);
+    const at::Tensor kept = r.at_place(at_kept, {batch, max_new}, at::kInt), counts = r.at_place(at_counts, {batch}, at::kInt),
+                     next = r.at_place(at_next, {batch}, tokens.scalar_type());
     void* stream = stream_of(dev);
     const int rc = call([&] {
       return abi.verify(contexts[dev], &d, p_tokens, parents, p_starts, address(target), draft, accept, sample, static_cast<int32_t*>(address(kept)),
@@ -213,14 +236,20 @@ PyObject* change(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (a[5] != Py_None) d.lengths = static_cast<const int32_t*>(list(a[5], at::kInt, batch, dev));
     const int32_t* parents = a[6] == Py_None ? nullptr : static_cast<const int32_t*>(list(a[6], at::kInt, batch, dev));
     const size_t bytes = abi.pages_workspace(&d, which);
+    const int64_t n_third = which == FRISK_B200_PAGES_COMPACT ? 1 : batch;
+    Results r;
+    const int64_t at_users = r.place(d.pages * 4), at_table = r.place(batch * width * 4), at_third = r.place(n_third * 4);
+    // (a small workspace beside the results; a larger one would be held with them)
+    const bool beside = bytes <= kBeside;
+    const int64_t at_workspace = beside ? r.place((int64_t)bytes) : 0;
+    r.allocate(dev);
     at::Tensor workspace;
-    if (bytes) workspace = made({(int64_t)bytes}, at::kByte, dev);
-    const at::Tensor users = made({d.pages}, at::kInt, dev), to = made({batch, width}, at::kInt, dev),
-                     third = made({which == FRISK_B200_PAGES_COMPACT ? 1 : batch}, at::kInt, dev);
+    if (!beside) workspace = made({(int64_t)bytes}, at::kByte, dev);
+    const at::Tensor users = r.at_place(at_users, {d.pages}, at::kInt), to = r.at_place(at_table, {batch, width}, at::kInt), third = r.at_place(at_third, {n_third}, at::kInt);
     t.users_out = static_cast<int32_t*>(address(users));
     t.table_out = static_cast<int32_t*>(address(to));
     t.lengths_out = static_cast<int32_t*>(address(third));
-    void *ws = bytes ? address(workspace) : nullptr, *stream = stream_of(dev);
+    void *ws = !bytes ? nullptr : beside ? static_cast<char*>(address(r.held)) + at_workspace : address(workspace), *stream = stream_of(dev);
     const int rc = call([&] {
       return which == FRISK_B200_PAGES_FORK   ? abi.fork(contexts[dev], &d, &t, parents, ws, bytes, stream)
              : which == FRISK_B200_PAGES_GROW ? abi.grow(contexts[dev], &d, &t, ws, bytes, stream)
@@ -230,21 +259,53 @@ PyObject* change(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// the tables of packed rows: of a cache's descriptor
+void tables_of(frisk_b200_cache_desc& d, PyObject* table, PyObject* starts, PyObject* lengths, int dev) {
+  const at::Tensor& t = table_of(table, dev);
+  const int64_t batch = t.size(0);
+  d.table = static_cast<const int32_t*>(address(t));
+  d.batch = (int32_t)batch;
+  d.table_width = (int32_t)t.size(1);
+  d.table_stride = t.stride(0);
+  d.starts = static_cast<const int32_t*>(list(starts, at::kInt, batch + 1, dev));
+  d.lengths = static_cast<const int32_t*>(list(lengths, at::kInt, batch, dev));
+}
+
+// write(cache, k, v, table, starts, lengths): True where it is done
+PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return usually([&]() -> PyObject* {
+    require(n == 6);
+    int dev;
+    frisk_b200_cache_desc d = cache_of(a[0], &dev);
+    const at::Tensor &k = tensor(a[1]), &v = tensor(a[2]);
+    const int code = code_of(k.scalar_type());
+    require((code == FRISK_B200_F16 || code == FRISK_B200_BF16) && (d.dtype == FRISK_B200_E4M3 || d.dtype == code));
+    require(v.scalar_type() == k.scalar_type() && k.dim() == 3 && v.sizes() == k.sizes() && k.size(1) == d.heads && k.size(2) == d.D);
+    frisk_b200_packed packed[2];
+    for (int i = 0; i < 2; ++i) {
+      const at::Tensor& t = i ? v : k;
+      require(t.stride(2) == 1 && t.get_device() == dev);
+      packed[i] = {address(t), t.stride(0), t.stride(1)};
+    }
+    d.rows = k.size(0);
+    tables_of(d, a[3], a[4], a[5], dev);
+    void* stream = stream_of(dev);
+    const int rc = call([&] { return abi.write(contexts[dev], &d, code, &packed[0], &packed[1], stream); });
+    if (rc) return PyLong_FromLong(rc);
+    Py_RETURN_TRUE;
+  });
+}
+
 // keep(cache, table, starts, lengths, kept, counts)
 PyObject* keep(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return usually([&]() -> PyObject* {
     require(n == 6);
     int dev;
     frisk_b200_cache_desc d = cache_of(a[0], &dev);
-    const at::Tensor &table = table_of(a[1], dev), &kept = table_of(a[4], dev);
-    const int64_t batch = table.size(0);
+    tables_of(d, a[1], a[2], a[3], dev);
+    const at::Tensor& kept = table_of(a[4], dev);
+    const int64_t batch = d.batch;
     require(kept.size(0) == batch);
-    d.table = static_cast<const int32_t*>(address(table));
-    d.batch = (int32_t)batch;
-    d.table_width = (int32_t)table.size(1);
-    d.table_stride = table.stride(0);
-    d.starts = static_cast<const int32_t*>(list(a[2], at::kInt, batch + 1, dev));
-    d.lengths = static_cast<const int32_t*>(list(a[3], at::kInt, batch, dev));
     const int32_t* counts = static_cast<const int32_t*>(list(a[5], at::kInt, batch, dev));
     const at::Tensor out = made({batch}, at::kInt, dev);
     void* stream = stream_of(dev);
@@ -318,13 +379,13 @@ PyObject* adapters(PyObject*, PyObject* const* o, Py_ssize_t n) {
   });
 }
 
-// library(nine addresses): the C ABI's functions, in the order of Abi
+// library(ten addresses): the C ABI's functions, in the order of Abi
 PyObject* library(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  void* at[9];
-  for (int i = 0; i < 9; ++i) {
-    at[i] = n == 9 ? PyLong_AsVoidPtr(a[i]) : nullptr;
+  void* at[10];
+  for (int i = 0; i < 10; ++i) {
+    at[i] = n == 10 ? PyLong_AsVoidPtr(a[i]) : nullptr;
     if (!at[i]) {
-      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "nine addresses");
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "ten addresses");
       return nullptr;
     }
   }
@@ -346,7 +407,7 @@ PyCFunction fast(F f) {
   return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
 }
 PyMethodDef methods[] = {{"verify", fast(verify), METH_FASTCALL, nullptr},     {"change", fast(change), METH_FASTCALL, nullptr},
-                         {"keep", fast(keep), METH_FASTCALL, nullptr},         {"copy", fast(copy), METH_FASTCALL, nullptr},
+                         {"write", fast(write), METH_FASTCALL, nullptr},       {"keep", fast(keep), METH_FASTCALL, nullptr},         {"copy", fast(copy), METH_FASTCALL, nullptr},
                          {"adapters", fast(adapters), METH_FASTCALL, nullptr}, {"library", fast(library), METH_FASTCALL, nullptr},
                          {"context", fast(context), METH_FASTCALL, nullptr},   {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -34,6 +34,8 @@ def arguments():
     users, table, lengths, starts = ints([1, 1, 2, 0, 0, 0, 0, 0, 0]), ints([[0, 2, -1], [1, 2, -1]], 5), ints([20, 25]), ints([0, 2, 4])
     other = tuple(t.cuda() for t in new_cache(9, 2, 16, 64, "float8_e4m3fn", 1))
     kept, counts = ints([[0, 1], [1, 1]]), ints([2, 1])
+    torch.manual_seed(6)
+    rows = torch.randn(4, 4, 64, device="cuda").bfloat16()
     fork, grow, compact = capi.PAGES_FORK, capi.PAGES_GROW, capi.PAGES_COMPACT
     return {
         "verify": (lambda *v: F.draft_verify(*v, max_new=6), verify, calls.verify, verify + [6]),
@@ -43,6 +45,7 @@ def arguments():
         "compact": (F.cache_compact, [cache, users, table], calls.change, [compact, cache, users, table, None, None, None]),
         "keep": (F.cache_keep, [cache, table, starts, lengths, kept, counts], calls.keep, [cache, table, starts, lengths, kept, counts]),
         "copy": (lambda a, b, c, d: F.cache_copy(a, b, c, into=d), [cache, ints([1, 0]), ints([4, 8]), other], calls.copy, [cache, ints([1, 0]), ints([4, 8]), other]),
+        "write": (F.cache_write, [cache, rows[:, :2], rows[:, 2:], table, starts, lengths], calls.write, [cache, rows[:, :2], rows[:, 2:], table, starts, lengths]),
     }
 
 
@@ -51,7 +54,7 @@ def flat(x):
     return [t.cpu().view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t.cpu() for t in ((x,) if isinstance(x, torch.Tensor) else x)]
 
 
-@pytest.mark.parametrize("name", ["verify", "adapters", "fork", "grow", "compact", "keep", "copy"])
+@pytest.mark.parametrize("name", ["verify", "adapters", "fork", "grow", "compact", "keep", "copy", "write"])
 def test_the_same_as_python(calls, name, monkeypatch):
     import torch
     import frisk_b200 as F
@@ -59,7 +62,7 @@ def test_the_same_as_python(calls, name, monkeypatch):
     given = native(*native_args)
     assert given is not None and type(given) is not int
     first = flat(function(*args))
-    for other in ("verify", "change", "keep", "copy", "adapters"):
+    for other in ("verify", "change", "keep", "copy", "adapters", "write"):
         monkeypatch.setattr(calls, other, lambda *_: None)
     function, args, _, _ = arguments()[name]  # (what a call changed in place is as it was)
     second = flat(function(*args))
@@ -69,7 +72,7 @@ def test_the_same_as_python(calls, name, monkeypatch):
         assert all(torch.equal(a, b) for a, b in zip(flat(given), first))
 
 
-@pytest.mark.parametrize("name", ["verify", "adapters", "fork", "grow", "compact", "keep", "copy"])
+@pytest.mark.parametrize("name", ["verify", "adapters", "fork", "grow", "compact", "keep", "copy", "write"])
 def test_what_is_unusual_is_left_to_python(calls, name):
     import torch
 
@@ -130,3 +133,27 @@ def test_on_the_current_stream(calls):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+def test_results_of_one_call_are_tensors_of_their_own(calls):
+    """They share an allocation: each is dense, on its own bytes, and may be changed, kept and passed on by itself."""
+    import torch
+    import frisk_b200 as F
+    made = arguments()
+    for name in ("verify", "fork", "grow", "compact"):
+        function, args, _, _ = made[name]
+        first, second = function(*args), function(*args)
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in first + second)
+        assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+        for i, (t, want) in enumerate(zip(first, second)):
+            assert t.is_contiguous() and t.device == args[1].device and not t.requires_grad and t.shape == want.shape and t.dtype == want.dtype
+            before = [u.clone() for u in first]
+            t.fill_(-7)
+            assert all(torch.equal(u, v) for j, (u, v) in enumerate(zip(first, before)) if j != i)
+            assert torch.equal(torch.clone(want), before[i])
+        kept = first[1]
+        del first
+        assert bool((kept == -7).all())
+    cache, users, table, lengths, _ = made["fork"][1]
+    empty = F.cache_fork(cache, users, table[:0], lengths[:0], lengths[:0])
+    assert torch.equal(empty[0], users) and empty[1].shape == (0, 3) and empty[2].shape == (0,)
