@@ -49,6 +49,75 @@ __device__ __forceinline__ uint4 load8(const uint16_t* at, int n) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// The tile of kRows rows that is number `tile`.  Up to kThreads sequences are brought together by adapter: the rows of those that share one lie behind one
+// another, in the order of the sequences, and the groups in that of their first ones.  (Rows that come together read the adapter once: 99 tokens over 21 adapters of
+// rank 64, K 4096, N 7744, 32-bit results 18 us, a tile for each 46.)  More sequences have tiles of their own.
+struct Rows {
+  int count, which;  // rows of the tile (0: there are fewer tiles), their adapter
+};
+template <int kRows>
+__device__ __forceinline__ Rows gather_tile(const AdapterParams& p, int tile, int (&row_of)[kRows]) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (!p.grouped) {
+    const Tile t = find_tile<kThreads>(p, tile, kRows, false);
+    if (tid < kRows) row_of[tid] = t.row + tid;
+    __syncthreads();
+    return Rows{t.seq < 0 ? 0 : t.rows, t.which};
+  }
+  __shared__ __align__(16) int keys[kThreads], many[kThreads];
+  __shared__ int sums[kWarps], found[3];
+  constexpr int kNone = -2;  // a sequence without rows
+  int lo = 0, n = 0, key = kNone;
+  if (tid < p.batch) {
+    lo = p.starts[tid];
+    key = p.adapters[tid];
+    const int64_t count = (int64_t)p.starts[tid + 1] - lo;
+    if (lo < 0 || count < 0 || lo + count > p.rows) atomicCAS(p.status, 0u, cache::ST_CACHE_ROWS);
+    else n = (int)count;
+    if (n > 0 && key >= p.count) atomicCAS(p.status, 0u, cache::ST_ADAPTER);
+    key = n == 0 ? kNone : key < p.count ? max(key, -1) : -1;
+  }
+  keys[tid] = key;
+  many[tid] = n;
+  if (tid < 3) found[tid] = 0;
+  __syncthreads();
+  int before = 0, all = 0;  // rows of this adapter in the sequences before, and in all
+  if (key != kNone) {
+#pragma unroll 4
+    for (int s = 0; s < p.batch; s += 4) {
+      const int4 k = *reinterpret_cast<const int4*>(keys + s), m = *reinterpret_cast<const int4*>(many + s);
+      const int a = k.x == key ? m.x : 0, b = k.y == key ? m.y : 0, c = k.z == key ? m.z : 0, d = k.w == key ? m.w : 0;
+      all += (a + b) + (c + d);
+      before += (s < tid ? a : 0) + (s + 1 < tid ? b : 0) + (s + 2 < tid ? c : 0) + (s + 3 < tid ? d : 0);
+    }
+  }
+  const int mine = key != kNone && before == 0 ? (all + kRows - 1) / kRows : 0;  // (tiles of the group, at its first sequence)
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int other = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += other;
+  }
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  int at = upto - mine;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i)
+    if (i < warp) at += sums[i];
+  if (tile >= at && tile < at + mine) {
+    found[0] = min(kRows, all - (tile - at) * kRows);
+    found[1] = key;
+    found[2] = (tile - at) * kRows;
+  }
+  __syncthreads();
+  const int rows = found[0], which = found[1], first = found[2];
+  if (key == which && rows > 0) {
+    for (int i = max(first, before); i < min(first + rows, before + n); ++i) row_of[i - first] = lo + i - before;
+  }
+  __syncthreads();
+  return Rows{rows, which};
+}
+
 // MW: groups of 16 rows a warp has; MWARPS: warps side by side over rows (the others share the inner index, then the columns)
 template <typename T, typename C, int RMAX, int MW, int MWARPS>
 struct Plan {
@@ -77,12 +146,12 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  const Tile found = find_tile<kThreads>(p, tile, P::kRows, false);
-  if (found.seq < 0) return;  // (the whole cluster: there are fewer tiles than clusters)
-  const int64_t row0 = found.row;
-  const int rows = found.rows, which = found.which;
-  const C* c = static_cast<const C*>(p.c) + row0 * p.ldc;
-  C* out = static_cast<C*>(p.out) + row0 * p.ldo;
+  __shared__ int row_of[P::kRows];
+  const Rows found = gather_tile<P::kRows>(p, tile, row_of);
+  if (found.count == 0) return;  // (the whole cluster: there are fewer tiles than clusters)
+  const int rows = found.count, which = found.which;
+  const C* c = static_cast<const C*>(p.c);
+  C* out = static_cast<C*>(p.out);
   const int blocks_n = (p.N + 31) / 32, n0 = (int)((int64_t)blocks_n * rank / C_), n1 = (int)((int64_t)blocks_n * (rank + 1) / C_);
   if (which < 0) {  // no adapter (the whole cluster)
     if (p.out != p.c) {
@@ -91,20 +160,28 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
         const int r = i / pieces, col = n0 * 32 + (i - r * pieces) * 8;
         if (col >= p.N) continue;
         Eight<C> old;
-        old.load(c + r * p.ldc + col, p.N - col, p.wide);
+        old.load(c + row_of[r] * p.ldc + col, p.N - col, p.wide);
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = old[j];
-        store_eight<C>(out + r * p.ldo + col, v, p.N - col, p.wide);
+        store_eight<C>(out + row_of[r] * p.ldo + col, v, p.N - col, p.wide);
       }
     }
     return;
   }
-  const uint16_t* x = static_cast<const uint16_t*>(p.x) + row0 * p.ldx;
+  const uint16_t* x = static_cast<const uint16_t*>(p.x);
   const uint16_t* a = static_cast<const uint16_t*>(p.a) + which * p.a_step;
   const uint16_t* bw = static_cast<const uint16_t*>(p.b) + which * p.b_step;
   const int mw = warp % MWARPS, share = warp / MWARPS;  // the warp's rows; its part of the inner index, then of the columns
   const int my_row = mw * 16 * MW;
+  int row[MW][2];  // of this lane, in memory
+#pragma unroll
+  for (int m = 0; m < MW; ++m)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = my_row + 16 * m + 8 * h + g;
+      row[m][h] = row_of[min(r, rows - 1)];
+    }
 
   // ---- x A^T over this CTA's part of K, shared by kShare warps in turns of 32
   // (The tensor cores cut what an addition leaves below 24 bits, always towards zero, some 2e-8 of the result each time.  Where the result has 32 bits an accumulator
@@ -131,7 +208,7 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = my_row + 16 * m + 8 * h + g;
-          xa[m][h] = load8(x + r * p.ldx + k, r < rows ? left : 0);
+          xa[m][h] = load8(x + row[m][h] * p.ldx + k, r < rows ? left : 0);
         }
 #pragma unroll
       for (int t = 0; t < P::kTiles; ++t) w[t] = load8(a + (8 * t + g) * p.lda + k, 8 * t < p.R ? left : 0);
@@ -236,7 +313,7 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r = my_row + 16 * m + 8 * h + g;
-        old[m][h].load(c + r * p.ldc + col, r < rows ? left : 0, p.wide);
+        old[m][h].load(c + row[m][h] * p.ldc + col, r < rows ? left : 0, p.wide);
       }
     // (the smaller terms apart, so that chains of cut additions are half as long)
     float d[MW][4][4], low[kExact ? MW : 1][4][4];
@@ -281,28 +358,44 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
           const float sum = d[m][j / 2][2 * h + j % 2] + (kExact ? low[m][j / 2][2 * h + j % 2] : 0.f);
           y[j] = fmaf(alpha, sum * up[m][h], old[m][h][j]);
         }
-        store_eight<C>(out + r * p.ldo + col, y, left, p.wide);
+        store_eight<C>(out + row[m][h] * p.ldo + col, y, left, p.wide);
       }
   }
 }
 
 template <typename T, typename C, int RMAX, int MW, int MWARPS>
-cudaError_t launch(frisk_b200_ctx* ctx, AdapterParams p, cudaStream_t s) {
+struct Launch {
   using P = Plan<T, C, RMAX, MW, MWARPS>;
+  static int capacity(int device, int cluster) {
+    static ClusterCapacity known;
+    return known(device, adapter_kernel<T, C, RMAX, MW, MWARPS>, kThreads, (int)P::kBytes, cluster);
+  }
+  // (at most: every sequence, or group of sequences that share an adapter or have none, may end with a tile that is not full)
+  static int64_t tiles(const AdapterParams& p) { return std::min<int64_t>(p.rows, p.rows / P::kRows + (p.grouped ? std::min<int64_t>(p.batch, (int64_t)p.count + 1) : p.batch)); }
+  static cudaError_t allow(int device) {
+    static PerDeviceOnce once;
+    cudaError_t e = cudaSuccess;
+    once(device, [&] {
+      e = cudaFuncSetAttribute(adapter_kernel<T, C, RMAX, MW, MWARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kBytes);
+      return e == cudaSuccess ? 0 : 1;
+    });
+    return e;
+  }
+  // whether all tiles run at once in the largest clusters
+  static bool fits(int device, const AdapterParams& p) { return allow(device) == cudaSuccess && capacity(device, kMaxCluster) >= tiles(p); }
+};
+
+template <typename T, typename C, int RMAX, int MW, int MWARPS>
+cudaError_t launch(frisk_b200_ctx* ctx, AdapterParams p, cudaStream_t s) {
+  using L = Launch<T, C, RMAX, MW, MWARPS>;
+  using P = typename L::P;
   auto kernel = adapter_kernel<T, C, RMAX, MW, MWARPS>;
-  static PerDeviceOnce once;
-  cudaError_t e = cudaSuccess;
-  once(ctx->device, [&] {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kBytes);
-    return e == cudaSuccess ? 0 : 1;
-  });
+  const cudaError_t e = L::allow(ctx->device);
   if (e != cudaSuccess) return e;
-  // (at most: every sequence may end with a tile that is not full)
-  const int64_t tiles = std::min<int64_t>(p.rows, p.rows / P::kRows + p.batch);
+  const int64_t tiles = L::tiles(p);
   // The most CTAs a tile with which all tiles run at once (64 requests of a token, rank 128: clusters of eight 57 us, of four 33).
-  static ClusterCapacity capacity;
   p.cluster = kMaxCluster;
-  while (p.cluster > 2 && capacity(ctx->device, kernel, kThreads, (int)P::kBytes, p.cluster) < tiles) p.cluster /= 2;
+  while (p.cluster > 2 && L::capacity(ctx->device, p.cluster) < tiles) p.cluster /= 2;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel waits (griddepcontrol.wait) itself
@@ -321,7 +414,13 @@ cudaError_t launch(frisk_b200_ctx* ctx, AdapterParams p, cudaStream_t s) {
 
 template <typename T, typename C, int RMAX>
 cudaError_t launch_rows(frisk_b200_ctx* ctx, const AdapterParams& p, cudaStream_t s) {
+  // Sequences that share an adapter come together where there are more tiles than run at once in the largest clusters, and fewer if they do (us, 72 tokens over 5 adapters of
+  // rank 16 24 -> 13; where they all run the more clusters the better: 37 tokens over 2 adapters 14.5, brought together 17.5, and 5 of 19 rows of one adapter 7.3 and 9.1).
   const int64_t mean = (p.rows + p.batch - 1) / p.batch;  // rows of a sequence
+  AdapterParams g = p;
+  g.grouped = p.batch <= kThreads && p.count + (int64_t)1 < p.batch && p.rows < (1 << 23);  // (rows are counted in 32 bits, even if sequences out of range name some again)
+  if (g.grouped && !(mean <= 16 ? Launch<T, C, RMAX, 1, 1>::fits(ctx->device, p) : Launch<T, C, RMAX, 2, 1>::fits(ctx->device, p)))
+    return p.rows <= 16 * ((int64_t)p.count + 1) ? launch<T, C, RMAX, 1, 1>(ctx, g, s) : launch<T, C, RMAX, 2, 1>(ctx, g, s);
   if (mean <= 16) return launch<T, C, RMAX, 1, 1>(ctx, p, s);
   return launch<T, C, RMAX, 2, 1>(ctx, p, s);
 }

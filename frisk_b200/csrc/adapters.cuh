@@ -17,7 +17,8 @@ struct AdapterParams {
   int64_t ldx, lda, a_step, ldb, b_step, ldc, ldo, rows;
   int K, N, R, count, batch;
   int cluster;
-  bool wide;  // c and out on 16 bytes, row by row
+  bool wide;     // c and out on 16 bytes, row by row
+  bool grouped;  // sequences are brought together by adapter
   unsigned* status;
 };
 

@@ -76,6 +76,75 @@ def test_adapters(counts, k, n, rank, dtype, wide):
     r.check(scales=False, in_place=True)
 
 
+SHARED = [[1] * 256, [1] * 257, [0, 1, 3, 2] * 50, [5] * 90 + [40], [47] * 50, [0] * 255 + [17], [1, 70, 30] * 30]
+
+
+@pytest.mark.parametrize("counts", SHARED, ids=range(len(SHARED)))
+@pytest.mark.parametrize("k,n,rank,count", [(250, 333, 8, 3), (64, 40, 16, 1), (520, 96, 64, 2), (72, 130, 104, 40)])
+@pytest.mark.parametrize("dtype,wide", [("bfloat16", False), ("float16", True)])
+def test_sequences_that_share_adapters(counts, k, n, rank, count, dtype, wide):
+    """Many sequences of few adapters, which come together by adapter, in every mixture."""
+    import torch
+    r = Requests(counts, k, n, rank, count, dtype, wide, seed=rank, gap=2, pitch=8, odd=n % 4)
+    r.check()
+    r.check(in_place=True)
+    r.which = [0] * len(counts)
+    r.check(scales=False)
+    r.which = [(7 * i) % (count + 1) - 1 for i in range(len(counts))]
+    plain = r.run().cpu()
+    # what is not finite stays in its row
+    last = r.starts[-1] - 1
+    r.whole[0][last, :k] = math.nan
+    got = r.run().cpu()
+    assert torch.equal(got[:last], plain[:last]) and torch.equal(got[last + 1:], plain[last + 1:])
+
+
+def test_many_requests_replayed():
+    """A captured call with other adapters and other numbers of rows, and tables out of range."""
+    import torch
+    import frisk_b200 as F
+    r = Requests([1] * 200, 200, 96, 16, 3, seed=2)
+    x, a, b, c = (t.cuda()[..., s] for t, s in zip(r.whole, r.cut))
+    starts, which, scales = torch.tensor(r.starts, dtype=torch.int32).cuda(), torch.tensor(r.which, dtype=torch.int32).cuda(), r.scales.cuda()
+    out = torch.full_like(c, 55.0)
+    graph = torch.cuda.CUDAGraph()
+    F.adapter_gemm(x, a, b, c, starts, which, scales=scales, out=out)
+    with torch.cuda.graph(graph):
+        F.adapter_gemm(x, a, b, c, starts, which, scales=scales, out=out)
+    for seed in range(4):
+        g = torch.Generator().manual_seed(seed)
+        cut = [0] + sorted(torch.randint(0, 201, (199,), generator=g).tolist()) + [200]
+        now = torch.randint(-1, 3, (200,), generator=g).tolist()
+        which.copy_(torch.tensor(now, dtype=torch.int32))
+        starts.copy_(torch.tensor(cut, dtype=torch.int32))
+        out.fill_(55.0)
+        graph.replay()
+        F.cache_check()
+        want, bound = so.adapters(*r.cpu, cut, now, r.scales)
+        assert float(((out.cpu().double() - want).abs() - bound).max()) <= 0
+    good = out.clone()
+    bad = list(cut)
+    bad[100] = -5  # sequences 99 and 100 have no rows
+    bad_which = list(now)
+    bad_which[0:3] = [3, 1 << 30, -9]
+    which.copy_(torch.tensor(bad_which, dtype=torch.int32))
+    starts.copy_(torch.tensor(bad, dtype=torch.int32))
+    out.fill_(55.0)
+    graph.replay()
+    with pytest.raises(RuntimeError, match="table"):
+        F.cache_check()
+    assert torch.equal(out[:cut[3]], c[:cut[3]]) and torch.equal(out[cut[3]:cut[99]], good[cut[3]:cut[99]]) and torch.equal(out[cut[101]:], good[cut[101]:])
+    assert bool((out[cut[99]:cut[101]] == 55.0).all())
+    # all rows again and again: more than there are tiles for
+    starts.copy_(torch.tensor([0, 200] * 100 + [0], dtype=torch.int32))
+    which.fill_(1)
+    graph.replay()
+    with pytest.raises(RuntimeError, match="table"):
+        F.cache_check()
+    want, bound = so.adapters(*r.cpu, [0, 200], [1], r.scales)
+    assert float(((out.cpu().double() - want).abs() - bound).max()) <= 0
+
+
 @pytest.mark.parametrize("counts", [[3, 0, 17], [300, 129, 200]])
 @pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("c_at,out_at,n", [(0, 1, 64), (1, 0, 64), (0, 8, 136), (3, 5, 37), (8, 0, 130), (0, 2, 2), (1, 1, 1)])
