@@ -26,6 +26,7 @@ namespace {
 using namespace adapter;
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kMostGrouped = 8 * kThreads;  // sequences that are brought together
 constexpr int kChain = 4;  // blocks of 32 of the inner index that an accumulator takes
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -49,9 +50,9 @@ __device__ __forceinline__ uint4 load8(const uint16_t* at, int n) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The tile of kRows rows that is number `tile`.  Up to kThreads sequences are brought together by adapter: the rows of those that share one lie behind one
-// another, in the order of the sequences, and the groups in that of their first ones.  (Rows that come together read the adapter once: 99 tokens over 21 adapters of
-// rank 64, K 4096, N 7744, 32-bit results 18 us, a tile for each 46.)  More sequences have tiles of their own.
+// The tile of kRows rows that is number `tile`.  Where it is asked for, sequences are brought together by adapter, kThreads of them at a time: the rows of those that share
+// one lie behind one another, in the order of the sequences, and the groups in that of their first ones.  (Rows that come together read the adapter once: 99 tokens over
+// 21 adapters of rank 64, K 4096, N 7744, 32-bit results 18 us, a tile for each 46.)  Else a sequence has tiles of its own.
 struct Rows {
   int count, which;  // rows of the tile (0: there are fewer tiles), their adapter
 };
@@ -67,55 +68,64 @@ __device__ __forceinline__ Rows gather_tile(const AdapterParams& p, int tile, in
   __shared__ __align__(16) int keys[kThreads], many[kThreads];
   __shared__ int sums[kWarps], found[3];
   constexpr int kNone = -2;  // a sequence without rows
-  int lo = 0, n = 0, key = kNone;
-  if (tid < p.batch) {
-    lo = p.starts[tid];
-    key = p.adapters[tid];
-    const int64_t count = (int64_t)p.starts[tid + 1] - lo;
-    if (lo < 0 || count < 0 || lo + count > p.rows) atomicCAS(p.status, 0u, cache::ST_CACHE_ROWS);
-    else n = (int)count;
-    if (n > 0 && key >= p.count) atomicCAS(p.status, 0u, cache::ST_ADAPTER);
-    key = n == 0 ? kNone : key < p.count ? max(key, -1) : -1;
-  }
-  keys[tid] = key;
-  many[tid] = n;
-  if (tid < 3) found[tid] = 0;
-  __syncthreads();
-  int before = 0, all = 0;  // rows of this adapter in the sequences before, and in all
-  if (key != kNone) {
-#pragma unroll 4
-    for (int s = 0; s < p.batch; s += 4) {
-      const int4 k = *reinterpret_cast<const int4*>(keys + s), m = *reinterpret_cast<const int4*>(many + s);
-      const int a = k.x == key ? m.x : 0, b = k.y == key ? m.y : 0, c = k.z == key ? m.z : 0, d = k.w == key ? m.w : 0;
-      all += (a + b) + (c + d);
-      before += (s < tid ? a : 0) + (s + 1 < tid ? b : 0) + (s + 2 < tid ? c : 0) + (s + 3 < tid ? d : 0);
+#pragma unroll 1
+  for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
+    const int b = b0 + tid;
+    int lo = 0, n = 0, key = kNone;
+    if (b < p.batch) {
+      lo = p.starts[b];
+      key = p.adapters[b];
+      const int64_t count = (int64_t)p.starts[b + 1] - lo;
+      if (lo < 0 || count < 0 || lo + count > p.rows) atomicCAS(p.status, 0u, cache::ST_CACHE_ROWS);
+      else n = (int)count;
+      if (n > 0 && key >= p.count) atomicCAS(p.status, 0u, cache::ST_ADAPTER);
+      key = n == 0 ? kNone : key < p.count ? max(key, -1) : -1;
     }
-  }
-  const int mine = key != kNone && before == 0 ? (all + kRows - 1) / kRows : 0;  // (tiles of the group, at its first sequence)
-  int upto = mine;
+    keys[tid] = key;
+    many[tid] = n;
+    if (tid < 3) found[tid] = 0;
+    __syncthreads();
+    int before = 0, all = 0;  // rows of this adapter in the sequences before, and in all
+    if (key != kNone) {
+      const int last = min(kThreads, p.batch - b0);
+#pragma unroll 4
+      for (int s = 0; s < last; s += 4) {
+        const int4 k = *reinterpret_cast<const int4*>(keys + s), m = *reinterpret_cast<const int4*>(many + s);
+        const int a = k.x == key ? m.x : 0, b = k.y == key ? m.y : 0, c = k.z == key ? m.z : 0, d = k.w == key ? m.w : 0;
+        all += (a + b) + (c + d);
+        before += (s < tid ? a : 0) + (s + 1 < tid ? b : 0) + (s + 2 < tid ? c : 0) + (s + 3 < tid ? d : 0);
+      }
+    }
+    const int mine = key != kNone && before == 0 ? (all + kRows - 1) / kRows : 0;  // (tiles of the group, at its first sequence)
+    int upto = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int other = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += other;
-  }
-  if (lane == 31) sums[warp] = upto;
-  __syncthreads();
-  int at = upto - mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += other;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    int at = upto - mine, total = 0;
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i)
-    if (i < warp) at += sums[i];
-  if (tile >= at && tile < at + mine) {
-    found[0] = min(kRows, all - (tile - at) * kRows);
-    found[1] = key;
-    found[2] = (tile - at) * kRows;
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) at += sums[i];
+      total += sums[i];
+    }
+    if (tile >= at && tile < at + mine) {
+      found[0] = min(kRows, all - (tile - at) * kRows);
+      found[1] = key;
+      found[2] = (tile - at) * kRows;
+    }
+    __syncthreads();
+    const int rows = found[0], which = found[1], first = found[2];
+    if (rows > 0 && key == which) {
+      for (int i = max(first, before); i < min(first + rows, before + n); ++i) row_of[i - first] = lo + i - before;
+    }
+    __syncthreads();
+    if (rows > 0) return Rows{rows, which};
+    tile -= total;
   }
-  __syncthreads();
-  const int rows = found[0], which = found[1], first = found[2];
-  if (key == which && rows > 0) {
-    for (int i = max(first, before); i < min(first + rows, before + n); ++i) row_of[i - first] = lo + i - before;
-  }
-  __syncthreads();
-  return Rows{rows, which};
+  return Rows{0, -1};
 }
 
 // MW: groups of 16 rows a warp has; MWARPS: warps side by side over rows (the others share the inner index, then the columns)
@@ -363,6 +373,9 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
   }
 }
 
+// at most: of sequences that share an adapter or have none, kThreads sequences at a time
+int64_t groups_of(const AdapterParams& p) { return (p.batch + kThreads - 1) / kThreads * ((int64_t)p.count + 1); }
+
 template <typename T, typename C, int RMAX, int MW, int MWARPS>
 struct Launch {
   using P = Plan<T, C, RMAX, MW, MWARPS>;
@@ -371,7 +384,7 @@ struct Launch {
     return known(device, adapter_kernel<T, C, RMAX, MW, MWARPS>, kThreads, (int)P::kBytes, cluster);
   }
   // (at most: every sequence, or group of sequences that share an adapter or have none, may end with a tile that is not full)
-  static int64_t tiles(const AdapterParams& p) { return std::min<int64_t>(p.rows, p.rows / P::kRows + (p.grouped ? std::min<int64_t>(p.batch, (int64_t)p.count + 1) : p.batch)); }
+  static int64_t tiles(const AdapterParams& p) { return std::min<int64_t>(p.rows, p.rows / P::kRows + (p.grouped ? groups_of(p) : p.batch)); }
   static cudaError_t allow(int device) {
     static PerDeviceOnce once;
     cudaError_t e = cudaSuccess;
@@ -418,9 +431,9 @@ cudaError_t launch_rows(frisk_b200_ctx* ctx, const AdapterParams& p, cudaStream_
   // rank 16 24 -> 13; where they all run the more clusters the better: 37 tokens over 2 adapters 14.5, brought together 17.5, and 5 of 19 rows of one adapter 7.3 and 9.1).
   const int64_t mean = (p.rows + p.batch - 1) / p.batch;  // rows of a sequence
   AdapterParams g = p;
-  g.grouped = p.batch <= kThreads && p.count + (int64_t)1 < p.batch && p.rows < (1 << 23);  // (rows are counted in 32 bits, even if sequences out of range name some again)
+  g.grouped = p.batch <= kMostGrouped && groups_of(p) < p.batch && p.rows < (1 << 23);  // (rows are counted in 32 bits, even if sequences out of range name some again)
   if (g.grouped && !(mean <= 16 ? Launch<T, C, RMAX, 1, 1>::fits(ctx->device, p) : Launch<T, C, RMAX, 2, 1>::fits(ctx->device, p)))
-    return p.rows <= 16 * ((int64_t)p.count + 1) ? launch<T, C, RMAX, 1, 1>(ctx, g, s) : launch<T, C, RMAX, 2, 1>(ctx, g, s);
+    return p.rows <= 16 * groups_of(p) ? launch<T, C, RMAX, 1, 1>(ctx, g, s) : launch<T, C, RMAX, 2, 1>(ctx, g, s);
   if (mean <= 16) return launch<T, C, RMAX, 1, 1>(ctx, p, s);
   return launch<T, C, RMAX, 2, 1>(ctx, p, s);
 }

@@ -613,10 +613,12 @@ int launch_both(frisk_b200_ctx* ctx, AdapterParams p, const Work& work, cudaStre
 
 }  // namespace
 
-// Long sequences, if adapters lie one behind the other (no tensor map has a step of 0).  K = N = 4096, here and in adapters.cu, us: rank 16, 64 sequences of 64 rows
-// 38 and 33, of 128 rows 50 and 62; rank 64, 16 of 32 rows 17.5 and 16.9, of 40 rows 18 and 31, 64 of 64 rows 42 and 66; 2 of 64 rows 12.8 and 11.7.
+// Long sequences, if adapters lie one behind the other (no tensor map has a step of 0).  How long is measured, K = N = 4096, 4 to 64 adapters, here and in adapters.cu, us:
+// rank 8 and 32, 16-bit results 100 sequences of 48 rows 51 and 58, 64 of 64 rows 40 and 34, 64 of 100 rows 49 and 61; 32-bit ones 128 of 32 rows 70 and 65, 64 of 64 rows 51 and 63;
+// rank 64, 64 of 24 rows 39 and 35, 128 of 32 rows 61 and 71; rank 128, 64 of 16 rows 52 and 47, of 24 rows 46 and 53, 24 of 24 rows 33 and 26 to 50.
 size_t adapter_tiles_workspace_bytes(const frisk_b200_adapter_desc& d) {
-  if (d.batch < 1 || d.rows < 512 || d.rows <= (d.rank <= 32 ? 64 : 32) * (int64_t)d.batch || d.count < 1) return 0;
+  const int64_t longest = d.rank > 64 ? 20 : d.rank > 32 ? 28 : d.dtype_c == FRISK_B200_F32 ? 40 : 64;  // mean rows that adapters.cu takes
+  if (d.batch < 1 || d.rows < 512 || d.rows <= longest * d.batch || d.count < 1) return 0;
   if (d.count > 1 && (d.a_step < d.lda || d.b_step < d.ldb)) return 0;
   if (most_tiles(d.rows, d.batch) * ((d.N + kColumns - 1) / kColumns) > INT32_MAX || d.rows * (int64_t)d.rank > INT32_MAX) return 0;
   const int terms = d.dtype_c == FRISK_B200_F32 && d.dtype == FRISK_B200_BF16 ? 3 : 2;

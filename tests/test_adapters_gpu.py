@@ -76,7 +76,7 @@ def test_adapters(counts, k, n, rank, dtype, wide):
     r.check(scales=False, in_place=True)
 
 
-SHARED = [[1] * 256, [1] * 257, [0, 1, 3, 2] * 50, [5] * 90 + [40], [47] * 50, [0] * 255 + [17], [1, 70, 30] * 30]
+SHARED = [[1] * 256, [1] * 257, [2, 0, 1] * 400, [1] * 2049, [0, 1, 3, 2] * 50, [5] * 90 + [40], [47] * 50, [0] * 255 + [17], [1, 70, 30] * 30]
 
 
 @pytest.mark.parametrize("counts", SHARED, ids=range(len(SHARED)))
