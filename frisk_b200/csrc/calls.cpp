@@ -1,5 +1,5 @@
 // Usual calls of the serving operators made natively: a CPython module (no GPU code) that reads torch's tensors, makes the results, and calls
-// the C ABI.  A small call costs as much as its checks, attribute by attribute in Python, as its launch (12 us a call; 5 to 6 with this module), and nothing
+// the C ABI.  A small call costs as much as its checks, attribute by attribute in Python, as its launch (12 us a call; 3 to 6 with this module), and nothing
 // may be remembered between calls, since a tensor's storage, shape and strides can be changed at any time.
 //
 // It only ever ACCEPTS: calls without `out` and `stream` whose tensors are plain ones (torch.Tensor itself) of the types, shapes and strides that

@@ -20,7 +20,7 @@
 //
 // Bound by HBM where there are many sequences (64 chains of 6 tokens over 128000 fp32 values: 21 us, 49 MB read), else by the chain starts -> tokens ->
 // values -> row -> sums -> row (one chain over 32000: 6 us with the launch) and, where much is rejected, by conversions to and products in 64 bits (16
-// trees of 24 over 50001 bf16 values: 22 us, some 3 a rejected child).
+// trees of 24 over 50001 bf16 values: 23 us, some 3 a rejected child).
 #include <cfloat>
 
 #include "cache_common.cuh"
