@@ -142,7 +142,7 @@ struct Plan {
   static constexpr size_t kBytes = kFirstBytes + kFullBytes + kRows * 4;
 };
 
-template <typename T, typename C, int RMAX, int MW, int MWARPS>
+template <typename T, typename C, int RMAX, int MW, int MWARPS, bool WIDE>
 __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p) {
   using P = Plan<T, C, RMAX, MW, MWARPS>;
   extern __shared__ __align__(16) uint8_t memory[];
@@ -169,12 +169,12 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
       for (int i = tid; i < rows * pieces; i += kThreads) {
         const int r = i / pieces, col = n0 * 32 + (i - r * pieces) * 8;
         if (col >= p.N) continue;
-        Eight<C> old;
-        old.load(c + row_of[r] * p.ldc + col, p.N - col, p.wide);
+        Eight<C, WIDE> old;
+        old.load(c + row_of[r] * p.ldc + col, p.N - col, p.begins);
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = old[j];
-        store_eight<C>(out + row_of[r] * p.ldo + col, v, p.N - col, p.wide);
+        store_eight<C, WIDE>(out + row_of[r] * p.ldo + col, v, p.N - col, p.begins);
       }
     }
     return;
@@ -317,13 +317,13 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
   const int first = 8 * (g >> 1) + (g & 1);  // of the rows of B that this lane's columns of the four tiles are: first + 2 j
   for (int nb = n0 + share; nb < n1; nb += P::kShare) {
     const int col = nb * 32 + 8 * q, left = p.N - col;
-    Eight<C> old[MW][2];
+    Eight<C, WIDE> old[MW][2];
 #pragma unroll
     for (int m = 0; m < MW; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r = my_row + 16 * m + 8 * h + g;
-        old[m][h].load(c + row[m][h] * p.ldc + col, r < rows ? left : 0, p.wide);
+        old[m][h].load(c + row[m][h] * p.ldc + col, r < rows ? left : 0, p.begins);
       }
     // (the smaller terms apart, so that chains of cut additions are half as long)
     float d[MW][4][4], low[kExact ? MW : 1][4][4];
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
           const float sum = d[m][j / 2][2 * h + j % 2] + (kExact ? low[m][j / 2][2 * h + j % 2] : 0.f);
           y[j] = fmaf(alpha, sum * up[m][h], old[m][h][j]);
         }
-        store_eight<C>(out + row[m][h] * p.ldo + col, y, left, p.wide);
+        store_eight<C, WIDE>(out + row[m][h] * p.ldo + col, y, left, p.begins);
       }
   }
 }
@@ -376,12 +376,12 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
 // at most: of sequences that share an adapter or have none, kThreads sequences at a time
 int64_t groups_of(const AdapterParams& p) { return (p.batch + kThreads - 1) / kThreads * ((int64_t)p.count + 1); }
 
-template <typename T, typename C, int RMAX, int MW, int MWARPS>
+template <typename T, typename C, int RMAX, int MW, int MWARPS, bool WIDE>
 struct Launch {
   using P = Plan<T, C, RMAX, MW, MWARPS>;
   static int capacity(int device, int cluster) {
     static ClusterCapacity known;
-    return known(device, adapter_kernel<T, C, RMAX, MW, MWARPS>, kThreads, (int)P::kBytes, cluster);
+    return known(device, adapter_kernel<T, C, RMAX, MW, MWARPS, WIDE>, kThreads, (int)P::kBytes, cluster);
   }
   // (at most: every sequence, or group of sequences that share an adapter or have none, may end with a tile that is not full)
   static int64_t tiles(const AdapterParams& p) { return std::min<int64_t>(p.rows, p.rows / P::kRows + (p.grouped ? groups_of(p) : p.batch)); }
@@ -389,7 +389,7 @@ struct Launch {
     static PerDeviceOnce once;
     cudaError_t e = cudaSuccess;
     once(device, [&] {
-      e = cudaFuncSetAttribute(adapter_kernel<T, C, RMAX, MW, MWARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kBytes);
+      e = cudaFuncSetAttribute(adapter_kernel<T, C, RMAX, MW, MWARPS, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kBytes);
       return e == cudaSuccess ? 0 : 1;
     });
     return e;
@@ -398,11 +398,11 @@ struct Launch {
   static bool fits(int device, const AdapterParams& p) { return allow(device) == cudaSuccess && capacity(device, kMaxCluster) >= tiles(p); }
 };
 
-template <typename T, typename C, int RMAX, int MW, int MWARPS>
+template <typename T, typename C, int RMAX, int MW, int MWARPS, bool WIDE>
 cudaError_t launch(frisk_b200_ctx* ctx, AdapterParams p, cudaStream_t s) {
-  using L = Launch<T, C, RMAX, MW, MWARPS>;
+  using L = Launch<T, C, RMAX, MW, MWARPS, WIDE>;
   using P = typename L::P;
-  auto kernel = adapter_kernel<T, C, RMAX, MW, MWARPS>;
+  auto kernel = adapter_kernel<T, C, RMAX, MW, MWARPS, WIDE>;
   const cudaError_t e = L::allow(ctx->device);
   if (e != cudaSuccess) return e;
   const int64_t tiles = L::tiles(p);
@@ -425,24 +425,30 @@ cudaError_t launch(frisk_b200_ctx* ctx, AdapterParams p, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-template <typename T, typename C, int RMAX>
+template <typename T, typename C, int RMAX, bool WIDE>
 cudaError_t launch_rows(frisk_b200_ctx* ctx, const AdapterParams& p, cudaStream_t s) {
   // Sequences that share an adapter come together where there are more tiles than run at once in the largest clusters, and fewer if they do (us, 72 tokens over 5 adapters of
   // rank 16 24 -> 13; where they all run the more clusters the better: 37 tokens over 2 adapters 14.5, brought together 17.5, and 5 of 19 rows of one adapter 7.3 and 9.1).
   const int64_t mean = (p.rows + p.batch - 1) / p.batch;  // rows of a sequence
   AdapterParams g = p;
   g.grouped = p.batch <= kMostGrouped && groups_of(p) < p.batch && p.rows < (1 << 23);  // (rows are counted in 32 bits, even if sequences out of range name some again)
-  if (g.grouped && !(mean <= 16 ? Launch<T, C, RMAX, 1, 1>::fits(ctx->device, p) : Launch<T, C, RMAX, 2, 1>::fits(ctx->device, p)))
-    return p.rows <= 16 * groups_of(p) ? launch<T, C, RMAX, 1, 1>(ctx, g, s) : launch<T, C, RMAX, 2, 1>(ctx, g, s);
-  if (mean <= 16) return launch<T, C, RMAX, 1, 1>(ctx, p, s);
-  return launch<T, C, RMAX, 2, 1>(ctx, p, s);
+  if (g.grouped && !(mean <= 16 ? Launch<T, C, RMAX, 1, 1, WIDE>::fits(ctx->device, p) : Launch<T, C, RMAX, 2, 1, WIDE>::fits(ctx->device, p)))
+    return p.rows <= 16 * groups_of(p) ? launch<T, C, RMAX, 1, 1, WIDE>(ctx, g, s) : launch<T, C, RMAX, 2, 1, WIDE>(ctx, g, s);
+  if (mean <= 16) return launch<T, C, RMAX, 1, 1, WIDE>(ctx, p, s);
+  return launch<T, C, RMAX, 2, 1, WIDE>(ctx, p, s);
 }
-template <typename T, typename C>
+template <typename T, typename C, bool WIDE>
 cudaError_t launch_rank(frisk_b200_ctx* ctx, const AdapterParams& p, cudaStream_t s) {
-  if (p.R <= 16) return launch_rows<T, C, 16>(ctx, p, s);
-  if (p.R <= 32) return launch_rows<T, C, 32>(ctx, p, s);
-  if (p.R <= 64) return launch_rows<T, C, 64>(ctx, p, s);
-  return launch_rows<T, C, 128>(ctx, p, s);
+  if (p.R <= 16) return launch_rows<T, C, 16, WIDE>(ctx, p, s);
+  if (p.R <= 32) return launch_rows<T, C, 32, WIDE>(ctx, p, s);
+  if (p.R <= 64) return launch_rows<T, C, 64, WIDE>(ctx, p, s);
+  return launch_rows<T, C, 128, WIDE>(ctx, p, s);
+}
+// (Rows that do not begin on 16 bytes have kernels of their own: the check in one took registers, 64 tokens of 40 adapters 12.2 -> 13.5 us; one by one their elements
+// took twice the time, 93 sequences of 42 rows, N 2420, 79 us for 38.)
+template <typename T, typename C>
+cudaError_t launch_types(frisk_b200_ctx* ctx, const AdapterParams& p, cudaStream_t s) {
+  return p.begins == 16 ? launch_rank<T, C, true>(ctx, p, s) : launch_rank<T, C, false>(ctx, p, s);
 }
 
 }  // namespace
@@ -539,13 +545,14 @@ extern "C" int frisk_b200_adapter_gemm(frisk_b200_ctx* ctx, const frisk_b200_ada
   p.R = d->rank;
   p.count = d->count;
   p.batch = d->batch;
-  p.wide = ((reinterpret_cast<uintptr_t>(c) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0 && (rows == 1 || (d->ldc | d->ldo) * (int64_t)cs % 16 == 0);
+  const uint64_t begins = reinterpret_cast<uintptr_t>(c) | reinterpret_cast<uintptr_t>(out) | (rows > 1 ? (uint64_t)((d->ldc | d->ldo) * (int64_t)cs) : 0);
+  p.begins = begins % 16 == 0 ? 16 : begins % 8 == 0 ? 8 : begins % 4 == 0 ? 4 : 0;
   p.status = ctx->d_status;
   FB_DEVICE(ctx);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (need) return launch_adapter_tiles(ctx, *d, p, workspace, s);
   const bool f32 = d->dtype_c == FRISK_B200_F32;
-  FB_CUDA(ctx, d->dtype == FRISK_B200_F16 ? (f32 ? launch_rank<__half, float>(ctx, p, s) : launch_rank<__half, __half>(ctx, p, s))
-                                          : (f32 ? launch_rank<__nv_bfloat16, float>(ctx, p, s) : launch_rank<__nv_bfloat16, __nv_bfloat16>(ctx, p, s)));
+  FB_CUDA(ctx, d->dtype == FRISK_B200_F16 ? (f32 ? launch_types<__half, float>(ctx, p, s) : launch_types<__half, __half>(ctx, p, s))
+                                          : (f32 ? launch_types<__nv_bfloat16, float>(ctx, p, s) : launch_types<__nv_bfloat16, __nv_bfloat16>(ctx, p, s)));
   return 0;
 }

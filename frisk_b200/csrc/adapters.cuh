@@ -17,7 +17,7 @@ struct AdapterParams {
   int64_t ldx, lda, a_step, ldb, b_step, ldc, ldo, rows;
   int K, N, R, count, batch;
   int cluster;
-  bool wide;     // c and out on 16 bytes, row by row
+  int begins;    // bytes that c's and out's rows begin on: 16, 8, 4, or 0 (an element)
   bool grouped;  // sequences are brought together by adapter
   unsigned* status;
 };
@@ -62,13 +62,23 @@ __device__ __forceinline__ void split(float a, float b, uint32_t (&words)[kTerms
 __device__ __forceinline__ uint32_t word(const uint4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
 
 // Eight neighbours of c, as they are in memory, of which the first n are there
-template <typename C>
+// WIDE: rows begin on 16 bytes; else on `begins`: 8, 4, or 0 (an element)
+template <typename C, bool WIDE>
 struct Eight {
   uint4 w[sizeof(C) / 2];
-  __device__ __forceinline__ void load(const C* at, int n, bool wide) {
-    if (wide && n >= 8) {
+  __device__ __forceinline__ void load(const C* at, int n, int begins) {
+    if (WIDE && n >= 8) {
 #pragma unroll
       for (int i = 0; i < (int)sizeof(C) / 2; ++i) w[i] = *(reinterpret_cast<const uint4*>(at) + i);
+    } else if (!WIDE && begins == 8 && n >= 8) {
+      uint2 v[sizeof(C)];
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(C); ++i) v[i] = *(reinterpret_cast<const uint2*>(at) + i);
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(C) / 2; ++i) w[i] = make_uint4(v[2 * i].x, v[2 * i].y, v[2 * i + 1].x, v[2 * i + 1].y);
+    } else if (!WIDE && sizeof(C) == 2 && begins == 4 && n >= 8) {
+      const uint32_t* v = reinterpret_cast<const uint32_t*>(at);
+      w[0] = make_uint4(v[0], v[1], v[2], v[3]);
     } else {
       C v[8];
 #pragma unroll
@@ -83,19 +93,27 @@ struct Eight {
     return Terms<T>::value((uint16_t)(word(w[0], i / 2) >> (16 * (i & 1))));
   }
 };
-template <typename C>
-__device__ __forceinline__ void store_eight(C* at, const float (&v)[8], int n, bool wide) {
-  if (wide && n >= 8) {
-    if (sizeof(C) == 4) {
-      reinterpret_cast<float4*>(at)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(at)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      using T = typename std::conditional<sizeof(C) == 2, C, __half>::type;
-      uint32_t w[4];
+template <typename C, bool WIDE>
+__device__ __forceinline__ void store_eight(C* at, const float (&v)[8], int n, int begins) {
+  constexpr int kWords = 2 * (int)sizeof(C);
+  uint32_t w[kWords];
+  if (sizeof(C) == 4) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = Terms<T>::round(v[2 * i]) | (uint32_t)Terms<T>::round(v[2 * i + 1]) << 16;
-      *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
+    for (int i = 0; i < kWords; ++i) w[i] = __float_as_uint(v[i % 8]);
+  } else {
+    using T = typename std::conditional<sizeof(C) == 2, C, __half>::type;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = Terms<T>::round(v[2 * i % 8]) | (uint32_t)Terms<T>::round(v[(2 * i + 1) % 8]) << 16;
+  }
+  if (WIDE && n >= 8) {
+#pragma unroll
+    for (int i = 0; i < kWords / 4; ++i) reinterpret_cast<uint4*>(at)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  } else if (!WIDE && begins == 8 && n >= 8) {
+#pragma unroll
+    for (int i = 0; i < kWords / 2; ++i) reinterpret_cast<uint2*>(at)[i] = make_uint2(w[2 * i], w[2 * i + 1]);
+  } else if (!WIDE && sizeof(C) == 2 && begins == 4 && n >= 8) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) reinterpret_cast<uint32_t*>(at)[i] = w[i];
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
