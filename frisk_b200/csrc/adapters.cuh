@@ -175,6 +175,9 @@ __device__ __forceinline__ Tile find_tile(const AdapterParams& p, int tile, int 
 
 }  // namespace adapter
 
+// few rows a sequence (adapters_rows.cuh), and whether c has 32 bits
+cudaError_t launch_adapter_rows_f16(frisk_b200_ctx* ctx, const adapter::AdapterParams& p, bool f32, cudaStream_t s);
+cudaError_t launch_adapter_rows_bf16(frisk_b200_ctx* ctx, const adapter::AdapterParams& p, bool f32, cudaStream_t s);
 // long sequences (adapters_tiles.cu)
 size_t adapter_tiles_workspace_bytes(const frisk_b200_adapter_desc& d);  // 0: adapters.cu takes it
 int launch_adapter_tiles(frisk_b200_ctx* ctx, const frisk_b200_adapter_desc& d, const adapter::AdapterParams& p, void* workspace, cudaStream_t s);
