@@ -22,7 +22,7 @@ def adapter_gemm(x, a, b, c, starts, adapters, *, scales=None, out=None, stream=
     128 (pad it with zeros).  ``c`` [rows, N], the result of the shared projection (``gemm``), has their type or float32 and any pitch, and the result
     its type; ``out`` may be ``c``.  ``starts`` int32 [batch + 1], ``adapters`` int32 [batch] and ``scales`` float32 [count] (1 if not given) are on the device, so that a
     captured step can be replayed for other requests; an adapter out of range counts as none, and ``cache_check`` raises.  Sums have 32
-    bits, and the result is rounded once."""
+    bits, those between the two products too, and the result is rounded once."""
     global _KINDS
     if out is None and stream is None:
         r = calls.adapters(x, a, b, c, starts, adapters, scales)

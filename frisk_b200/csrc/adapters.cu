@@ -9,14 +9,14 @@
 // Bound by memory for the ranks of adapters: an element of x, c or out takes R multiplications (R = 64 at 6.5 TB/s: 0.2 PFLOP/s).  So the products
 // are mma.sync's, operands go from memory to registers without a stop, and no tensor memory is set up.  For a few rows the adapters
 // themselves are what is read, each by a cluster of its own; then the time is a chain: tables, x and A, two meetings of the cluster, B and c (one token, rank 16,
-// K = N = 4096: 7.1 us with the launch; 64 tokens over 40 adapters of rank 32, N 5120: 12.3, 25 MB).  Long sequences have kernels of their own (adapters_tiles.cu).
+// K = N = 4096: 7.4 us with the launch; 64 tokens over 40 adapters of rank 32, N 5120: 12.7, 25 MB).  Long sequences have kernels of their own (adapters_tiles.cu).
 //
 // Order of a product's inner index is free if both sides have the same, so a lane takes 16 bytes of it at once: of 32 neighbouring elements lane q of
 // four has 8 q .. 8 q + 7, which serve two steps of 16.  Columns of a result are permuted the same way: a lane ends up with 8 neighbours.
 //
-// Sums are 32-bit.  Before the second product they become sums of 16-bit terms: two, or three for bf16 whose result is 32-bit, so that less is lost
-// than in the rounding of the result (16 and 24 bits in bf16, 22 in fp16; fp16 terms stand at a power of two that brings a row's
-// largest to 2^14, so that sums beyond fp16's range keep their value).
+// Sums are 32-bit.  Before the second product they become sums of three 16-bit terms, which hold all 24 bits (fp16 terms stand at a power of two that brings a row's
+// largest to 2^14, so that sums beyond fp16's range keep their value, and go down to 2^-39 of it).  With two terms, 16 bits in bf16 and 22 in fp16, times are 2 to 5 % less (one
+// token 7.2 for 7.45 us, 64 over 40 adapters 12.6 for 13.3, 7000 rows 68 for 70.6), but columns in which sums cancel lose what is left of them.
 #include <algorithm>
 
 #include "adapters.cuh"

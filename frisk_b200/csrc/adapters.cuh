@@ -32,9 +32,9 @@ template <> struct Terms<__nv_bfloat16> {
   static __device__ __forceinline__ uint16_t round(float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); }
 };
 
-// The 16-bit terms that a sum between the products becomes: two, or three for bf16 whose result is 32-bit
-template <typename T, typename C>
-constexpr int kTermsOf = sizeof(C) == 4 && std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
+// The 16-bit terms that a sum between the products becomes: all of its 24 bits, whatever the result's type.  (Two hold 16 bits of a bf16 sum and 22 of an fp16 one:
+// less than the result where columns cancel, or c the product.)
+constexpr int kTerms = 3;
 
 // fp16: the power of two that brings a row's largest sum, most = 1.m * 2^(e - 127), to 2^14.  (Infinities stay; a row of zeros or subnormals
 // stands at 2^126.)
@@ -43,7 +43,7 @@ __device__ __forceinline__ float row_power(float most) {
   return e == 255 ? 1.f : __uint_as_float((uint32_t)min(254, 268 - max(e, 15)) << 23);
 }
 // two neighbours as kTerms words of 16-bit terms: each term is what those before it leave (exact, but for the last)
-template <typename T, int kTerms>
+template <typename T>
 __device__ __forceinline__ void split(float a, float b, uint32_t (&words)[kTerms]) {
   float v[2] = {a, b};
 #pragma unroll

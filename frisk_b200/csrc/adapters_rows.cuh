@@ -116,7 +116,6 @@ template <typename T, typename C, int RMAX, int MW, int MWARPS>
 struct Plan {
   static constexpr int kRows = 16 * MW * MWARPS, kShare = kWarps / MWARPS;
   static constexpr int kTiles = RMAX / 8, kBlocks = (RMAX + 31) / 32;
-  static constexpr int kTerms = kTermsOf<T, C>;
   static constexpr int kPitch = RMAX + 8;  // of rows of sums, floats (lanes of a fragment meet no bank twice)
   static constexpr size_t kSumBytes = (size_t)kShare * kRows * kPitch * 4;
   static constexpr size_t kFullBytes = (size_t)kRows * kPitch * 4;
@@ -177,10 +176,9 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
     }
 
   // ---- x A^T over this CTA's part of K, shared by kShare warps in turns of 32
-  // (The tensor cores cut what an addition leaves below 24 bits, always towards zero, some 2e-8 of the result each time.  Where the result has 32 bits an accumulator
+  // (The tensor cores cut what an addition leaves below 24 bits, always towards zero, some 2e-8 of the result each time.  So an accumulator
   // takes kChain blocks, and the parts are summed up rounding to nearest, in shared memory.)
   const int blocks_k = (p.K + 31) / 32, k0 = (int)((int64_t)blocks_k * rank / C_), k1 = (int)((int64_t)blocks_k * (rank + 1) / C_);
-  constexpr bool kExact = sizeof(C) == 4;
   int kb = my_row < rows ? k0 + share : k1;
   bool begun = false;
   do {
@@ -191,7 +189,7 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
       for (int t = 0; t < P::kTiles; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[m][t][i] = 0.f;
-    const int end = kExact ? min(k1, kb + kChain * P::kShare) : k1;
+    const int end = min(k1, kb + kChain * P::kShare);
 #pragma unroll 2
     for (; kb < end; kb += P::kShare) {
       const int k = kb * 32 + q * 8, left = p.K - k;
@@ -221,11 +219,11 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float2* to = reinterpret_cast<float2*>(sums + (share * P::kRows + my_row + 16 * m + 8 * h + g) * P::kPitch + 8 * t + 2 * q);
-          const float2 old = kExact && begun ? *to : make_float2(0.f, 0.f);
+          const float2 old = begun ? *to : make_float2(0.f, 0.f);
           *to = make_float2(old.x + acc[m][t][2 * h], old.y + acc[m][t][2 * h + 1]);
         }
     begun = true;
-  } while (kExact && kb < k1);
+  } while (kb < k1);
   __syncthreads();
   // ---- parts added up: the CTA's warps, then the CTAs, each in their order
   const int quads = RMAX / 4, n_quads = rows * quads;
@@ -266,7 +264,7 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
   for (int i = warp; i < MW * MWARPS * P::kBlocks * 2; i += kWarps) {
     const int s = i & 1, kb = (i >> 1) % P::kBlocks, m = (i >> 1) / P::kBlocks;
     if (16 * m >= rows) continue;
-    uint32_t f[P::kTerms][4];
+    uint32_t f[kTerms][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int r = 16 * m + g + 8 * (j & 1), k = 32 * kb + 8 * q + 4 * s + 2 * (j >> 1);
@@ -277,13 +275,13 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
         v[0] = two.x * up;
         v[1] = two.y * up;
       }
-      uint32_t both[P::kTerms];
+      uint32_t both[kTerms];
       split<T>(v[0], v[1], both);
 #pragma unroll
-      for (int t = 0; t < P::kTerms; ++t) f[t][j] = both[t];
+      for (int t = 0; t < kTerms; ++t) f[t][j] = both[t];
     }
 #pragma unroll
-    for (int t = 0; t < P::kTerms; ++t) terms[(i * P::kTerms + t) * 32 + lane] = make_uint4(f[t][0], f[t][1], f[t][2], f[t][3]);
+    for (int t = 0; t < kTerms; ++t) terms[(i * kTerms + t) * 32 + lane] = make_uint4(f[t][0], f[t][1], f[t][2], f[t][3]);
   }
   __syncthreads();
   // ---- times B^T, 32 columns a step
@@ -309,15 +307,14 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
         old[m][h].load(c + row[m][h] * p.ldc + col, r < rows ? left : 0, p.begins);
       }
     // (the smaller terms apart, so that chains of cut additions are half as long)
-    float d[MW][4][4], low[kExact ? MW : 1][4][4];
+    float d[MW][4][4], low[MW][4][4];
 #pragma unroll
     for (int m = 0; m < MW; ++m)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          d[m][j][i] = 0.f;
-          if (kExact) low[m][j][i] = 0.f;
+          d[m][j][i] = low[m][j][i] = 0.f;
         }
 #pragma unroll
     for (int kb = 0; kb < P::kBlocks; ++kb) {
@@ -332,11 +329,11 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int t = 0; t < P::kTerms; ++t) {
-            const uint4 f = terms[((((my_row / 16 + m) * P::kBlocks + kb) * 2 + s) * P::kTerms + t) * 32 + lane];
+          for (int t = 0; t < kTerms; ++t) {
+            const uint4 f = terms[((((my_row / 16 + m) * P::kBlocks + kb) * 2 + s) * kTerms + t) * 32 + lane];
             const uint32_t fa[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mma<T>(kExact && t > 0 ? low[m][j] : d[m][j], fa, word(w[j], 2 * s), word(w[j], 2 * s + 1));
+            for (int j = 0; j < 4; ++j) mma<T>(t > 0 ? low[m][j] : d[m][j], fa, word(w[j], 2 * s), word(w[j], 2 * s + 1));
           }
     }
 #pragma unroll
@@ -348,7 +345,7 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
         float y[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float sum = d[m][j / 2][2 * h + j % 2] + (kExact ? low[m][j / 2][2 * h + j % 2] : 0.f);
+          const float sum = d[m][j / 2][2 * h + j % 2] + low[m][j / 2][2 * h + j % 2];
           y[j] = fmaf(alpha, sum * up[m][h], old[m][h][j]);
         }
         store_eight<C, WIDE>(out + row[m][h] * p.ldo + col, y, left, p.begins);

@@ -36,11 +36,11 @@ struct Work {
 };
 int64_t most_tiles(int64_t rows, int64_t batch) { return std::min<int64_t>(rows, rows / kRows + batch); }
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
-Work work_of(void* ws, int64_t rows, int R, int terms, int64_t batch) {
+Work work_of(void* ws, int64_t rows, int R, int64_t batch) {
   uint8_t* at = static_cast<uint8_t*>(ws);
   Work w;
   w.terms = reinterpret_cast<uint16_t*>(at);
-  at += up((size_t)rows * R * terms * 2);
+  at += up((size_t)rows * R * kTerms * 2);
   w.down = reinterpret_cast<float*>(at);
   at += up((size_t)rows * 4);
   w.tiles = reinterpret_cast<int4*>(at);
@@ -66,7 +66,7 @@ struct SumsLayout {  // of `width` columns, R rounded up to a multiple of 16
   static __host__ __device__ int bytes(int width) { return kSumStages * stage_bytes(width) + 1024; }
 };
 
-template <typename T, int kTerms, int kMost>  // kMost: the rank at most, 64 or 128
+template <typename T, int kMost>  // kMost: the rank at most, 64 or 128
 __global__ void __launch_bounds__(kSumThreads)
     adapter_sums_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ AdapterParams p,
                         const __grid_constant__ Work work) {
@@ -240,7 +240,7 @@ constexpr int kWriters = 16;    // warps that add c and store, eight an item in 
 constexpr int kColThreads = 64 + 32 * kWriters;
 constexpr int kBox = 32 * 128;   // bytes of a writer's box of c and results: 32 rows of 128 bytes
 
-template <int kTerms, int kHalves>  // halves: 64 of R each
+template <int kHalves>  // halves: 64 of R each
 struct ColumnsLayout {
   static constexpr int kTermBytes = kTerms * kHalves * kBoxBytes;
   static constexpr int kStages = 2;
@@ -309,8 +309,7 @@ __global__ void __launch_bounds__(kColThreads, 1)
     adapter_columns_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c,
                            const __grid_constant__ CUtensorMap map_out, const __grid_constant__ AdapterParams p, const __grid_constant__ Work work, const bool c_by_tma,
                            const bool out_by_tma) {
-  constexpr int kTerms = kTermsOf<T, C>;
-  using L = ColumnsLayout<kTerms, kHalves>;
+  using L = ColumnsLayout<kHalves>;
   constexpr int kStages = L::kStages;
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -582,8 +581,8 @@ cudaError_t allow(PerDeviceOnce& once, int device, K kernel, int smem) {
 
 template <typename T, typename C, int kHalves>
 int launch_both(frisk_b200_ctx* ctx, AdapterParams p, const Work& work, cudaStream_t s) {
-  constexpr int kTerms = kTermsOf<T, C>, dtype = std::is_same<T, __half>::value ? FRISK_B200_F16 : FRISK_B200_BF16;
-  using L = ColumnsLayout<kTerms, kHalves>;
+  constexpr int dtype = std::is_same<T, __half>::value ? FRISK_B200_F16 : FRISK_B200_BF16;
+  using L = ColumnsLayout<kHalves>;
   const int width = (p.R + 15) / 16 * 16;
   CUtensorMap map_x, map_a, map_t, map_b, map_c{}, map_out{};
   const int64_t a_step = p.count > 1 ? p.a_step : p.lda * p.R, b_step = p.count > 1 ? p.b_step : p.ldb * p.N;
@@ -599,7 +598,7 @@ int launch_both(frisk_b200_ctx* ctx, AdapterParams p, const Work& work, cudaStre
   if (out_by_tma) bad |= encode_tmap_2d(ctx, &map_out, dtype_c, p.out, p.N, p.rows, p.ldo * sizeof(C), U, 8, true);
   if (bad) return FRISK_B200_E_CUDA;
   static PerDeviceOnce once_sums, once_columns;
-  auto sums = adapter_sums_kernel<T, kTerms, 64 * kHalves>;
+  auto sums = adapter_sums_kernel<T, 64 * kHalves>;
   auto columns = adapter_columns_kernel<T, C, kHalves>;
   FB_CUDA(ctx, allow(once_sums, ctx->device, sums, SumsLayout::bytes(64 * kHalves)));
   FB_CUDA(ctx, allow(once_columns, ctx->device, columns, L::kBytes));
@@ -621,13 +620,12 @@ size_t adapter_tiles_workspace_bytes(const frisk_b200_adapter_desc& d) {
   if (d.batch < 1 || d.rows < 512 || d.rows <= longest * d.batch || d.count < 1) return 0;
   if (d.count > 1 && (d.a_step < d.lda || d.b_step < d.ldb)) return 0;
   if (most_tiles(d.rows, d.batch) * ((d.N + kColumns - 1) / kColumns) > INT32_MAX || d.rows * (int64_t)d.rank > INT32_MAX) return 0;
-  const int terms = d.dtype_c == FRISK_B200_F32 && d.dtype == FRISK_B200_BF16 ? 3 : 2;
-  return up((size_t)d.rows * d.rank * terms * 2) + up((size_t)d.rows * 4) + up((size_t)most_tiles(d.rows, d.batch) * 16) + 256;
+  return up((size_t)d.rows * d.rank * kTerms * 2) + up((size_t)d.rows * 4) + up((size_t)most_tiles(d.rows, d.batch) * 16) + 256;
 }
 
 int launch_adapter_tiles(frisk_b200_ctx* ctx, const frisk_b200_adapter_desc& d, const AdapterParams& p, void* workspace, cudaStream_t s) {
   const bool f32 = d.dtype_c == FRISK_B200_F32, half = d.dtype == FRISK_B200_F16;
-  const Work work = work_of(workspace, p.rows, p.R, f32 && !half ? 3 : 2, p.batch);
+  const Work work = work_of(workspace, p.rows, p.R, p.batch);
   if (p.R <= 64) {
     if (half) return f32 ? launch_both<__half, float, 1>(ctx, p, work, s) : launch_both<__half, __half, 1>(ctx, p, work, s);
     return f32 ? launch_both<__nv_bfloat16, float, 1>(ctx, p, work, s) : launch_both<__nv_bfloat16, __nv_bfloat16, 1>(ctx, p, work, s);

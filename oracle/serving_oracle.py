@@ -137,11 +137,11 @@ def verify(tokens, parents, starts, target, draft, accept, sample, max_new):
 def adapters(x, a, b, c, starts, which, scales=None):
     """(result, bound on what a kernel may be off by) of the rows that belong to sequences; the others are NaN.
 
-    The bound: 2^-23 for every addition of a sum in 32 bits (tensor cores truncate); the sums between the products as two 16-bit terms (three for
-    bf16 with a 32-bit result) of half a step each, fp16 terms no finer than 2^-25 where the row's largest is 2^14; the result's own rounding."""
+    The bound: 2^-23 for every addition of a sum in 32 bits (tensor cores truncate); the sums between the products as three 16-bit terms of
+    half a step each, fp16 terms no finer than 2^-25 where the row's largest is 2^14; the result's own rounding."""
     out = torch.full(c.shape, math.nan, dtype=torch.float64)
     bound = torch.zeros(c.shape, dtype=torch.float64)
-    terms = 3 if x.dtype == torch.bfloat16 and c.dtype == torch.float32 else 2
+    terms = 3
     k, r = x.shape[1], a.shape[1]
     for s, w in enumerate(which):
         rows = slice(starts[s], starts[s + 1])
