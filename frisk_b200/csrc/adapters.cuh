@@ -1,5 +1,6 @@
 // Pieces shared by the kernels of low-rank adapters: parameters, the 16-bit types, eight neighbours of c and the result.
 #pragma once
+#include <cfloat>
 #include <type_traits>
 
 #include "cache_common.cuh"
@@ -36,27 +37,46 @@ template <> struct Terms<__nv_bfloat16> {
 // less than the result where columns cancel, or c the product.)
 constexpr int kTerms = 3;
 
-// fp16: the power of two that brings a row's largest sum, most = 1.m * 2^(e - 127), to 2^14.  (Infinities stay; a row of zeros or subnormals
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= FLT_MAX; }
+// fp16: the power of two that brings a row's largest finite sum, most = 1.m * 2^(e - 127), to 2^14.  (Infinities stay; a row of zeros or subnormals
 // stands at 2^126.)
+__device__ __forceinline__ float finite_magnitude(float x) { return finite(x) ? fabsf(x) : 0.f; }
 __device__ __forceinline__ float row_power(float most) {
   const int e = (int)(__float_as_uint(most) >> 23);
-  return e == 255 ? 1.f : __uint_as_float((uint32_t)min(254, 268 - max(e, 15)) << 23);
+  return __uint_as_float((uint32_t)min(254, 268 - max(e, 15)) << 23);
 }
-// two neighbours as kTerms words of 16-bit terms: each term is what those before it leave (exact, but for the last)
+// A sum's terms: all of its sign, and none of them 0, so that the three products with an infinite weight add up to the infinity that the formula has.  (Terms rounded to
+// nearest may be 0, or of the other sign: NaN.)  With w the weight of the sum's last bit, each of the first two is what fits of the rest below 2 w and w: multiples of w, exact;
+// in bf16 the third has 1 to 256 w.  fp16 terms are multiples of 2^-24, and sums below 3 2^-24 (their row's largest is 2^14) become one term; so do bf16 sums below 2^-100.
+template <typename T>
+__device__ __forceinline__ void terms_of(float v, uint16_t (&terms)[kTerms]) {
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  const float a = fabsf(v);
+  const uint32_t last = (__float_as_uint(a) >> 23) << 23;  // 2^23 w
+  const float w = kHalf ? fmaxf(__uint_as_float(last) * 0x1p-23f, 0x1p-24f) : __uint_as_float(last) * 0x1p-23f;
+  const uint16_t sign = (uint16_t)(__float_as_uint(v) >> 16 & 0x8000u);
+  auto below = [](float x) -> uint16_t {
+    if (kHalf) return __half_as_ushort(__float2half_rz(x));
+    return (uint16_t)(__float_as_uint(x) >> 16);
+  };
+  // (by selection: with a branch for each, one after the other, a token took 7.9 us for 7.5)
+  const bool usual = finite(v) && a >= (kHalf ? 3 * 0x1p-24f : 0x1p-100f);
+  const uint16_t one = Terms<T>::round(a), others = finite(v) ? (uint16_t)0 : one;
+  const uint16_t first = below(a - 2.f * w);
+  const float rest = a - Terms<T>::value(first);
+  const uint16_t second = below(rest - w), third = Terms<T>::round(rest - Terms<T>::value(second));
+  terms[0] = (usual ? first : one) | sign;
+  terms[1] = (usual ? second : others) | sign;
+  terms[2] = (usual ? third : others) | sign;
+}
+// two neighbours as words of terms
 template <typename T>
 __device__ __forceinline__ void split(float a, float b, uint32_t (&words)[kTerms]) {
-  float v[2] = {a, b};
+  uint16_t lo[kTerms], hi[kTerms];
+  terms_of<T>(a, lo);
+  terms_of<T>(b, hi);
 #pragma unroll
-  for (int t = 0; t < kTerms; ++t) {
-    words[t] = 0;
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const uint16_t h = Terms<T>::round(v[n]);
-      const float back = Terms<T>::value(h);
-      words[t] |= (uint32_t)h << (16 * n);
-      v[n] = isfinite(back) ? v[n] - back : 0.f;
-    }
-  }
+  for (int t = 0; t < kTerms; ++t) words[t] = lo[t] | (uint32_t)hi[t] << 16;
 }
 
 __device__ __forceinline__ uint32_t word(const uint4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }

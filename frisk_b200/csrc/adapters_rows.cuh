@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterParams p
   if (std::is_same<T, __half>::value) {
     for (int r = warp; r < rows; r += kWarps) {
       float most = 0.f;
-      for (int i = lane; i < RMAX; i += 32) most = fmaxf(most, fabsf(full[r * P::kPitch + i]));
+      for (int i = lane; i < RMAX; i += 32) most = fmaxf(most, finite_magnitude(full[r * P::kPitch + i]));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
       if (lane == 0) row_scale[r] = row_power(most);

@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kSumThreads)
           for (int r = 0; r < kMostCtas; ++r) {
             v[j].x += part[r].x; v[j].y += part[r].y; v[j].z += part[r].z; v[j].w += part[r].w;
           }
-          most = fmaxf(fmaxf(fmaxf(most, fabsf(v[j].x)), fabsf(v[j].y)), fmaxf(fabsf(v[j].z), fabsf(v[j].w)));
+          most = fmaxf(fmaxf(fmaxf(most, finite_magnitude(v[j].x)), finite_magnitude(v[j].y)), fmaxf(finite_magnitude(v[j].z), finite_magnitude(v[j].w)));
         }
       }
       float up = 1.f;

@@ -70,3 +70,66 @@ def test_long_sums_that_cancel(dtype, rows, rank):
     want = c.double() + product
     off = (got.double() - want).norm()
     assert float(off) <= half * float(want.norm()) + 104 * u * float(product.norm())
+
+
+def by_definition(x, a, b, c, counts, which):
+    """Element by element in 64 bits, so that infinities and NaN go the way of the formula."""
+    import torch
+    of_row = torch.tensor(which).repeat_interleave(torch.tensor(counts))
+    out = c.double().clone()
+    for w in range(len(a)):
+        mine = of_row == w
+        t = torch.stack([(x[mine].double() * row.double()).sum(-1) for row in a[w]], -1)
+        out[mine] += torch.stack([(t * row.double()).sum(-1) for row in b[w]], -1)
+    return out
+
+
+@pytest.mark.parametrize("counts", [[6], [3, 0, 17, 40], [1] * 300, [128, 1, 130, 300]])
+@pytest.mark.parametrize("k,n,rank", [(64, 37, 8), (72, 65, 40), (200, 130, 128)])
+@pytest.mark.parametrize("dtype,wide", [("bfloat16", False), ("bfloat16", True), ("float16", False), ("float16", True)])
+def test_infinite_weights(counts, k, n, rank, dtype, wide):
+    """An infinite element of B makes its column infinite, by the sign of the sum that it weighs, and nothing else; one of A all that its sum reaches; 0 times it, and two of other signs, are NaN."""
+    import torch
+    import frisk_b200 as F
+    from oracle import serving_oracle as so
+    dt, rows, inf = getattr(torch, dtype), sum(counts), float("inf")
+    g = torch.Generator().manual_seed(rows + n)
+    # (sums beyond fp16's range, and what they weigh)
+    x, a, b = torch.randn(rows, k, generator=g) * 100, torch.randn(3, rank, k, generator=g) * 100, torch.randn(3, n, rank, generator=g) * 0.01
+    b[0, 3, 2], b[0, 5, 1], b[0, 5, 6], b[0, n - 1, rank - 1], b[1, 0, 0] = inf, inf, -inf, -inf, inf
+    a[1, 3, 7], a[2, 4, k - 1], a[2, 5, 0] = inf, -inf, inf
+    x[4::5] = 0
+    x, a, b = x.to(dt), a.to(dt), b.to(dt)
+    c = torch.randn(rows, n, generator=g).to(torch.float32 if wide else dt)
+    which = [(i + 1) % 3 if len(counts) > 1 else 0 for i in range(len(counts))]
+    starts, adapters = lists(counts, which)
+    got = F.adapter_gemm(x.cuda(), a.cuda(), b.cuda(), c.cuda(), starts, adapters).double().cpu()
+    F.cache_check()
+    want = by_definition(x, a, b, c, counts, which)
+    assert bool(want.isinf().any()) and bool(want.isnan().any()) and bool(want.isfinite().any())
+    _, bound = so.adapters(x, a, b, c, starts.tolist(), which)
+    most = torch.finfo(c.dtype).max
+    finite = want.isfinite() & (want.abs() < most)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got[want.isinf()], want[want.isinf()])
+    assert float(((got - want).abs() - bound)[finite].max()) <= 0
+
+
+@pytest.mark.parametrize("counts", [[2], [30, 3], [600]])
+@pytest.mark.parametrize("wide", [False, True])
+def test_sums_at_the_end_of_the_range(counts, wide):
+    """Sums between bf16's largest value, 1.9921875 2^127, and that of 32 bits keep their value."""
+    import torch
+    import frisk_b200 as F
+    rows = sum(counts)
+    x, a, b = torch.zeros(rows, 64), torch.zeros(1, 8, 64), torch.zeros(1, 24, 8)
+    x[:, :2] = torch.tensor([2.0 ** 63, 2.0 ** 60])
+    a[:, :, :2] = torch.tensor([1.9921875 * 2.0 ** 64, 3 * 2.0 ** 58])  # the largest value, and 3 2^-9 of the power: 1.998046875 2^127
+    a[:, 1::2] = -a[:, 1::2]
+    b[:] = torch.arange(1, 9) * 2.0 ** -120
+    x, a, b = (t.bfloat16().cuda() for t in (x, a, b))
+    starts, adapters = lists(counts, [0] * len(counts))
+    got = F.adapter_gemm(x, a, b, torch.zeros(rows, 24, dtype=torch.float32 if wide else torch.bfloat16, device="cuda"), starts, adapters)
+    F.cache_check()
+    want = 1.998046875 * -4 * 2.0 ** 7  # (the sum of 1 - 2 + 3 .. - 8 is -4)
+    assert torch.equal(got.cpu(), torch.full((rows, 24), want, dtype=got.dtype))
