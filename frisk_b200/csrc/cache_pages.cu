@@ -237,7 +237,7 @@ struct GrowWork {
 // it changes waits for the copies.)
 template <bool COPIES>
 __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
-  __shared__ int sums[32];
+  __shared__ int sums[32], any_refused;
   __shared__ int near[kSearched + 1];  // offsets, where they fit
   extern __shared__ int lists[];       // five of kSmall, and one place
   GrowWork w(t.ws, t.batch, t.width, t.pages);
@@ -257,6 +257,7 @@ __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
 #pragma unroll
   for (int j = 0; j < kEach; ++j) ahead[j] = own + 32 * j < t.pages ? t.users[own + 32 * j] : 1;
   // 1. the slots that each sequence's new tokens touch
+  if (tid == 0) any_refused = 0;
   int all = 0;
   for (int b0 = 0; b0 < t.batch; b0 += kPlan) {
     const int b = b0 + tid;
@@ -300,29 +301,45 @@ __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
     }
     return lo;
   };
-  // 2. what they name; those that others name too are listed
+  auto refused = [&](int b) { return *const_cast<volatile int*>(t.lengths_out + b) == 0; };
+  // 2. what they name; those that others name too are listed.  A sequence that names a page without users gets nothing: it is told, and all is listed again without its slots.
   int n_shared = 0;
-  for (int i0 = 0; i0 < all; i0 += kPlan) {
-    const int i = i0 + tid;
-    int entry = -1;
-    bool shared = false;
-    if (i < all) {
-      const int b = owner(i), slot = (t.lengths[b] >> t.page_log2) + i - offset[b];
-      entry = t.table[b * t.stride + slot];
-      if (entry >= t.pages) flag(t.status, ST_CACHE_PAGE);
-      const int users = entry >= 0 && entry < t.pages ? t.users[entry] : 0;
-      shared = users > 1;
-      w.kind[i] = entry < 0 ? TAKE : KEEP;
+  bool again = false;
+  while (true) {
+    for (int i0 = 0; i0 < all; i0 += kPlan) {
+      const int i = i0 + tid;
+      int entry = -1;
+      bool shared = false;
+      if (i < all) {
+        const int b = owner(i), slot = (t.lengths[b] >> t.page_log2) + i - offset[b];
+        entry = t.table[b * t.stride + slot];
+        const bool there = entry >= 0 && entry < t.pages, left = again && refused(b);
+        const int users = there ? t.users[entry] : 0;
+        if (entry >= t.pages) flag(t.status, ST_CACHE_PAGE);
+        if (there && users <= 0) {
+          flag(t.status, ST_CACHE_PAGE);
+          t.lengths_out[b] = 0;
+          any_refused = 1;
+        }
+        shared = users > 1 && !left;
+        const bool alone = users == 1 && !left;
+        w.kind[i] = entry < 0 && !left ? TAKE : KEEP;
+        w.free[i] = alone ? entry : -1;
+        if (alone) __stcg(w.last + entry, i);  // (any of those that name it)
+      }
+      int total;
+      const int at = n_shared + block_scan(shared, sums, &total);
+      if (shared) {
+        w.shared[at] = i;
+        w.page[at] = entry;
+      }
+      n_shared += total;
     }
-    int total;
-    const int at = n_shared + block_scan(shared, sums, &total);
-    if (shared) {
-      w.shared[at] = i;
-      w.page[at] = entry;
-    }
-    n_shared += total;
+    __syncthreads();
+    if (again || !any_refused) break;
+    again = true;
+    n_shared = 0;
   }
-  __syncthreads();
   // 3. of the sequences that are going to write into a page, all take one of their own but the last that has it, if no one else does
   auto decide = [&](int k, int page, int holders, bool last) {  // of the touched slots with that page: how many, and whether k is the last
     const int users = t.users[page];
@@ -362,21 +379,40 @@ __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
   // 4. how many pages are taken before each slot
   int taken = 0;
   for (int i0 = 0; i0 < all; i0 += kPlan) {
-    const int i = i0 + tid, kind = i < all ? w.kind[i] : KEEP;
+    const int i = i0 + tid, kind = i < all ? w.kind[i] : KEEP, alone = i < all ? w.free[i] : -1;
+    const int who = alone >= 0 ? __ldcg(w.last + alone) : i;  // (on its way meanwhile)
     int total;
     const int at = taken + block_scan(kind >= TAKE, sums, &total);
     if (i < all) w.before[i] = at;
+    if (who != i) flag(t.status, ST_CACHE_PAGE);  // two slots name a page of one user: left, as above
     if (kind == SWAP || kind == KEEP_AS_LAST) w.depends[owner(i)] = 1;  // (all that write it, write 1)
     taken += total;
   }
   if (tid == 0) w.before[all] = taken;
-  // 5. that many free pages, lowest first: a warp looks at 256 pages a round, 32 at a time
+  // 5. that many free pages, lowest first: a warp looks at 256 pages a round, 32 at a time.  (Not those that a refused sequence names: they are marked.)
+  if (again) {
+    for (int p = tid; p < t.pages; p += kPlan) w.last[p] = 0;
+    __syncthreads();
+    for (int i = tid; i < all; i += kPlan) {
+      const int b = owner(i), entry = t.table[b * t.stride + (t.lengths[b] >> t.page_log2) + i - offset[b]];
+      if (refused(b) && entry >= 0 && entry < t.pages) w.last[entry] = 1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (own + 32 * j < t.pages && __ldcg(w.last + own + 32 * j)) ahead[j] = 1;
+  }
   int found = 0;
   for (int p0 = 0; p0 < t.pages && found < taken; p0 += kPlan * kEach) {
     const int first = p0 + own;
     if (p0 > 0) {
 #pragma unroll
       for (int j = 0; j < kEach; ++j) ahead[j] = first + 32 * j < t.pages ? t.users[first + 32 * j] : 1;
+      if (again) {
+#pragma unroll
+        for (int j = 0; j < kEach; ++j)
+          if (first + 32 * j < t.pages && __ldcg(w.last + first + 32 * j)) ahead[j] = 1;
+      }
     }
     unsigned masks[kEach];
     int mine = 0;
@@ -399,7 +435,7 @@ __global__ void __launch_bounds__(kPlan) grow_plan_kernel(const PageTables t) {
   // 6. a sequence gets all it needs or, with those behind it, nothing
   for (int b = tid; b < t.batch; b += kPlan) {
     const int need = w.before[offset[b + 1]] - w.before[offset[b]];
-    const bool granted = w.before[offset[b + 1]] <= found || (need == 0 && !w.depends[b]);
+    const bool granted = !(again && refused(b)) && (w.before[offset[b + 1]] <= found || (need == 0 && !w.depends[b]));
     if (!granted) t.lengths_out[b] = 0;
     w.depends[b] = granted;
   }

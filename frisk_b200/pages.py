@@ -139,7 +139,9 @@ def cache_grow(cache, users, table, starts, lengths, *, out=None, stream=None):
     """The new (users, table) with pages for ``starts[b + 1] - starts[b]`` more keys of each sequence, and how many of these were granted, int32
     [batch].  Pages are taken lowest first, by sequences in their order.  A page that is going to be written and that other rows have too
     is replaced by a copy; where several of the call's sequences have it, the last keeps it if no one else does.  A sequence gets all that
-    it asks for or, from the first that lacks pages on, nothing (0; others than those that need no page)."""
+    it asks for or, from the first that lacks pages on, nothing (0; others than those that need no page).  Where ``users`` contradicts the pages that
+    would be written, ``cache_check`` raises: a sequence that names a page without users gets nothing, and a page that more of the call's rows
+    name than it has users is left to all of them."""
     return _change(capi.PAGES_GROW, cache, users, table, starts, lengths, None, out, stream)
 
 

@@ -374,7 +374,9 @@ int frisk_b200_cache_attention(frisk_b200_ctx* ctx, const frisk_b200_cache_desc*
  *   sequences in their order.  A page that would be written and that others have too is replaced by one of its own, into which the
  *   keys that are in it are copied; of several sequences of the call that have it, the last one keeps it if no one else does.
  *   A sequence gets all or nothing, and from the first that lacks pages on only those that need none get theirs.
- *   lengths_out: the new keys that have a place now, [batch] (0 where there was none).
+ *   lengths_out: the new keys that have a place now, [batch] (0 where there was none).  A sequence whose new keys touch a page without
+ *   users gets nothing, and nobody else that page; a page that more of the touched slots name than it has users is left as it is.
+ *   frisk_b200_check tells both.
  * compact: moves the used pages to the lowest indices: the k-th used page behind the first n, n their number, becomes the k-th
  *   free one among them.  lengths_out: n, [1].  starts and lengths are not used. */
 enum { FRISK_B200_PAGES_FORK = 0, FRISK_B200_PAGES_GROW = 1, FRISK_B200_PAGES_COMPACT = 2 };
