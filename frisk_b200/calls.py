@@ -2,7 +2,7 @@
 
 ``verify``, ``change``, ``keep``, ``copy``, ``adapters`` and ``write`` give an operator's results, an error number of the C ABI, or None where the Python functions
 have to look for themselves (and report what is wrong, if anything is): always where the extension is not built for this interpreter
-and this torch, which costs time and nothing else.
+and this torch, which costs time and nothing else, and where the device has no open context.  ``address`` gives the one that calls would take.
 """
 import ctypes
 import importlib.machinery
@@ -26,34 +26,30 @@ def _unknown(*_):
     return None
 
 
-verify = change = keep = copy = adapters = write = _unknown
-_register, _known = None, set()
+verify = change = keep = copy = adapters = write = address = _unknown
+_loaded = False
 
 
 def context_for(device):
-    """The device's context; once it has been made, calls there may be made natively."""
-    context = execute.context_for(device)
-    if device not in _known:
-        _known.add(device)
-        _know(device, context)
-    return context
+    """The device's context; once one has been made, calls may be made natively, each with the context that is there then."""
+    if not _loaded:
+        _load()
+    return execute.context_for(device)
 
 
-def _know(device, context):
-    global verify, change, keep, copy, adapters, write, _register
-    if _register is None:
-        import torch
-        file = path(torch.__version__)
-        if not file.exists():
-            _register = _unknown
-            return
-        loader = importlib.machinery.ExtensionFileLoader("_calls", os.fspath(file))
-        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_calls", loader))
-        loader.exec_module(module)
-        lib = capi.load()
-        module.library(*(ctypes.cast(getattr(lib, "frisk_b200_" + name), ctypes.c_void_p).value for name in _FUNCTIONS))
-        verify, change, keep, copy, adapters, write, _register = module.verify, module.change, module.keep, module.copy, module.adapters, module.write, module.context
-    _register(device, context.handle.value)
+def _load():
+    global verify, change, keep, copy, adapters, write, address, _loaded
+    import torch
+    _loaded = True
+    file = path(torch.__version__)
+    if not file.exists():
+        return
+    loader = importlib.machinery.ExtensionFileLoader("_calls", os.fspath(file))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_calls", loader))
+    loader.exec_module(module)
+    lib = capi.load()
+    module.library(execute._contexts, *(ctypes.cast(getattr(lib, "frisk_b200_" + name), ctypes.c_void_p).value for name in _FUNCTIONS))
+    verify, change, keep, copy, adapters, write, address = module.verify, module.change, module.keep, module.copy, module.adapters, module.write, module.context
 
 
 def result(r, device):

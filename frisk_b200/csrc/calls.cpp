@@ -19,9 +19,9 @@
 
 namespace {
 
-constexpr int kDevices = 64;
 constexpr size_t kBeside = 1 << 16;  // bytes
-frisk_b200_ctx* contexts[kDevices] = {};
+// execute's contexts by device, looked up anew by each call: one may have been closed, or given place to another; and the attributes that hold its address
+PyObject *contexts = nullptr, *name_h = nullptr, *name_value = nullptr;
 
 // the C ABI, as the library that Python has loaded offers it
 struct Abi {
@@ -62,9 +62,33 @@ void* address(const at::Tensor& t) { return t.data_ptr(); }
 
 int index_of(const at::Tensor& t) {
   const int dev = t.get_device();
-  require(dev >= 0 && dev < kDevices && contexts[dev]);
+  require(dev >= 0);
   return dev;
 }
+struct Owned {  // a reference, given back with the interpreter's lock held
+  PyObject* object;
+  explicit Owned(PyObject* o) : object(o) { require(o); }
+  Owned(const Owned&) = delete;
+  ~Owned() { Py_DECREF(object); }
+};
+PyObject* found(int dev) {  // the device's context, whose reference is new
+  const Owned key(PyLong_FromLong(dev));
+  PyObject* o = contexts ? PyDict_GetItemWithError(contexts, key.object) : nullptr;
+  Py_XINCREF(o);
+  return o;
+}
+// The library's context of a device, which stays while this does
+struct Context {
+  Owned owner;
+  frisk_b200_ctx* handle;
+  explicit Context(int dev) : owner(found(dev)) {
+    const Owned held(PyObject_GetAttr(owner.object, name_h));  // None if it is closed
+    require(held.object != Py_None);
+    const Owned value(PyObject_GetAttr(held.object, name_value));
+    handle = static_cast<frisk_b200_ctx*>(PyLong_AsVoidPtr(value.object));
+    require(handle && !PyErr_Occurred());
+  }
+};
 // a dense list of n elements
 void* list(const at::Tensor& t, at::ScalarType type, int64_t n, int dev) {
   require(t.scalar_type() == type && t.dim() == 1 && t.size(0) == n && t.get_device() == dev && t.is_contiguous());
@@ -208,8 +232,9 @@ PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor kept = r.at_place(at_kept, {batch, max_new}, at::kInt), counts = r.at_place(at_counts, {batch}, at::kInt),
                      next = r.at_place(at_next, {batch}, tokens.scalar_type());
     void* stream = stream_of(dev);
+    const Context context(dev);
     const int rc = call([&] {
-      return abi.verify(contexts[dev], &d, p_tokens, parents, p_starts, address(target), draft, accept, sample, static_cast<int32_t*>(address(kept)),
+      return abi.verify(context.handle, &d, p_tokens, parents, p_starts, address(target), draft, accept, sample, static_cast<int32_t*>(address(kept)),
                         static_cast<int32_t*>(address(counts)), address(next), stream);
     });
     return rc ? PyLong_FromLong(rc) : tuple_of({kept, counts, next});
@@ -250,10 +275,11 @@ PyObject* change(PyObject*, PyObject* const* a, Py_ssize_t n) {
     t.table_out = static_cast<int32_t*>(address(to));
     t.lengths_out = static_cast<int32_t*>(address(third));
     void *ws = !bytes ? nullptr : beside ? static_cast<char*>(address(r.held)) + at_workspace : address(workspace), *stream = stream_of(dev);
+    const Context context(dev);
     const int rc = call([&] {
-      return which == FRISK_B200_PAGES_FORK   ? abi.fork(contexts[dev], &d, &t, parents, ws, bytes, stream)
-             : which == FRISK_B200_PAGES_GROW ? abi.grow(contexts[dev], &d, &t, ws, bytes, stream)
-                                              : abi.compact(contexts[dev], &d, &t, ws, bytes, stream);
+      return which == FRISK_B200_PAGES_FORK   ? abi.fork(context.handle, &d, &t, parents, ws, bytes, stream)
+             : which == FRISK_B200_PAGES_GROW ? abi.grow(context.handle, &d, &t, ws, bytes, stream)
+                                              : abi.compact(context.handle, &d, &t, ws, bytes, stream);
     });
     return rc ? PyLong_FromLong(rc) : tuple_of({users, to, third});
   });
@@ -290,7 +316,8 @@ PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t n) {
     d.rows = k.size(0);
     tables_of(d, a[3], a[4], a[5], dev);
     void* stream = stream_of(dev);
-    const int rc = call([&] { return abi.write(contexts[dev], &d, code, &packed[0], &packed[1], stream); });
+    const Context context(dev);
+    const int rc = call([&] { return abi.write(context.handle, &d, code, &packed[0], &packed[1], stream); });
     if (rc) return PyLong_FromLong(rc);
     Py_RETURN_TRUE;
   });
@@ -309,8 +336,9 @@ PyObject* keep(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int32_t* counts = static_cast<const int32_t*>(list(a[5], at::kInt, batch, dev));
     const at::Tensor out = made({batch}, at::kInt, dev);
     void* stream = stream_of(dev);
+    const Context context(dev);
     const int rc = call([&] {
-      return abi.keep(contexts[dev], &d, static_cast<const int32_t*>(address(kept)), kept.stride(0), (int32_t)kept.size(1), counts,
+      return abi.keep(context.handle, &d, static_cast<const int32_t*>(address(kept)), kept.stride(0), (int32_t)kept.size(1), counts,
                       static_cast<int32_t*>(address(out)), stream);
     });
     return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
@@ -328,7 +356,8 @@ PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t count = source.size(0);
     const int32_t *s = static_cast<const int32_t*>(list(source, at::kInt, count, dev)), *t = static_cast<const int32_t*>(list(a[2], at::kInt, count, dev));
     void* stream = stream_of(dev);
-    const int rc = call([&] { return abi.copy(contexts[dev], &from, &into, s, t, count, stream); });
+    const Context context(dev);
+    const int rc = call([&] { return abi.copy(context.handle, &from, &into, s, t, count, stream); });
     if (rc) return PyLong_FromLong(rc);
     Py_RETURN_TRUE;
   });
@@ -372,34 +401,43 @@ PyObject* adapters(PyObject*, PyObject* const* o, Py_ssize_t n) {
     if (bytes) workspace = made({(int64_t)bytes}, at::kByte, dev);
     const at::Tensor out = made({d.rows, d.N}, c.scalar_type(), dev);
     void *ws = bytes ? address(workspace) : nullptr, *stream = stream_of(dev);
+    const Context context(dev);
     const int rc = call([&] {
-      return abi.adapters(contexts[dev], &d, address(x), address(a), address(b), address(c), scales, starts, p_which, address(out), ws, bytes, stream);
+      return abi.adapters(context.handle, &d, address(x), address(a), address(b), address(c), scales, starts, p_which, address(out), ws, bytes, stream);
     });
     return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
   });
 }
 
-// library(ten addresses): the C ABI's functions, in the order of Abi
+// library(contexts, ten addresses): where contexts are, and the C ABI's functions in the order of Abi
 PyObject* library(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* at[10];
+  if (n != 11 || !PyDict_Check(a[0])) {
+    PyErr_SetString(PyExc_ValueError, "a dictionary and ten addresses");
+    return nullptr;
+  }
   for (int i = 0; i < 10; ++i) {
-    at[i] = n == 10 ? PyLong_AsVoidPtr(a[i]) : nullptr;
+    at[i] = PyLong_AsVoidPtr(a[1 + i]);
     if (!at[i]) {
-      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "ten addresses");
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "an address of 0");
       return nullptr;
     }
   }
   static_assert(sizeof(Abi) == sizeof(at), "one address each");
   memcpy(&abi, at, sizeof(at));
+  if (!name_h) name_h = PyUnicode_InternFromString("_h");
+  if (!name_value) name_value = PyUnicode_InternFromString("value");
+  if (!name_h || !name_value) return nullptr;
+  Py_INCREF(a[0]);
+  Py_XSETREF(contexts, a[0]);
   Py_RETURN_NONE;
 }
-// context(device, address): where calls on that device go
+// context(device): the address that calls on that device would be given, or None
 PyObject* context(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  const long dev = n == 2 ? PyLong_AsLong(a[0]) : -1;
-  void* at = n == 2 ? PyLong_AsVoidPtr(a[1]) : nullptr;
-  if (PyErr_Occurred()) return nullptr;
-  if (dev >= 0 && dev < kDevices && abi.verify) contexts[dev] = static_cast<frisk_b200_ctx*>(at);
-  Py_RETURN_NONE;
+  return usually([&]() -> PyObject* {
+    require(n == 1);
+    return PyLong_FromVoidPtr(Context((int)whole(a[0])).handle);
+  });
 }
 
 template <typename F>

@@ -157,3 +157,33 @@ def test_results_of_one_call_are_tensors_of_their_own(calls):
     cache, users, table, lengths, _ = made["fork"][1]
     empty = F.cache_fork(cache, users, table[:0], lengths[:0], lengths[:0])
     assert torch.equal(empty[0], users) and empty[1].shape == (0, 3) and empty[2].shape == (0,)
+
+
+def test_closed_and_new_contexts(calls):
+    """A closed context is refused by every call, and one in its place takes them over, with what is told of them."""
+    import torch
+    import frisk_b200 as F
+    made = arguments()
+    want = {name: flat(made[name][0](*made[name][1])) for name in ("verify", "adapters", "fork", "grow", "compact", "keep")}
+    F.cache_check()
+    held = calls.execute._contexts
+    mine = held[0]
+    address = calls.address(0)
+    mine.close()
+    try:
+        assert address and calls.address(0) is None
+        for function, args, native, native_args in made.values():
+            assert native(*native_args) is None
+            with pytest.raises(RuntimeError, match="destroyed"):
+                function(*args)
+    finally:
+        del held[0]
+    again = arguments()
+    for name, results in want.items():
+        assert all(torch.equal(a, b) for a, b in zip(flat(again[name][0](*again[name][1])), results)), name
+    assert calls.address(0) == held[0].handle.value
+    F.cache_check()
+    _, args, native, native_args = again["keep"]
+    assert native(*native_args[:-1], ints([99, 99])) is not None
+    with pytest.raises(RuntimeError, match="table"):
+        F.cache_check()
