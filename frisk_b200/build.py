@@ -71,13 +71,14 @@ def build_calls(force=False):
     spec, gxx, headers = importlib.util.find_spec("torch"), shutil.which("g++"), sysconfig.get_paths()["include"]
     cuda = pathlib.Path(_nvcc()).resolve().parent.parent / "include"
     torch = None if spec is None else pathlib.Path(spec.submodule_search_locations[0])
-    source = CSRC / "calls.cpp"
+    source, target = CSRC / "calls.cpp", None if torch is None else path(importlib.metadata.version("torch"))
+    if target is not None and not force and not _stale(target, [source, INCLUDE / "frisk_b200.h"]):
+        return target
     if torch is None or gxx is None or not all(p.exists() for p in (torch / "include/ATen/cuda/EmptyTensor.h", pathlib.Path(headers, "Python.h"), cuda / "cuda_runtime_api.h")):
         sys.stderr.write("frisk_b200: no g++, or no headers of Python, torch or CUDA: built without native calls\n")
+        if target is not None:
+            target.unlink(missing_ok=True)  # (one of an older source, or of other structures)
         return None
-    target = path(importlib.metadata.version("torch"))
-    if not force and not _stale(target, [source, INCLUDE / "frisk_b200.h"]):
-        return target
     target.parent.mkdir(exist_ok=True)
     flags = ["-O2", "-std=c++17", "-shared", "-fPIC", "-I", headers, "-I", str(torch / "include"), "-I", str(torch / "include/torch/csrc/api/include"), "-I", str(cuda)]
     libs = ["-L", str(torch / "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]

@@ -2,13 +2,14 @@
 
 ``verify``, ``change``, ``keep``, ``copy``, ``adapters`` and ``write`` give an operator's results, an error number of the C ABI, or None where the Python functions
 have to look for themselves (and report what is wrong, if anything is): always where the extension is not built for this interpreter
-and this torch, which costs time and nothing else, and where the device has no open context.  ``address`` gives the one that calls would take.
+and this torch or cannot be loaded, which costs time and nothing else, and where the device has no open context.  ``address`` gives the one that calls would take.
 """
 import ctypes
 import importlib.machinery
 import importlib.util
 import os
 import pathlib
+import warnings
 
 from . import capi, execute
 
@@ -44,10 +45,14 @@ def _load():
     file = path(torch.__version__)
     if not file.exists():
         return
-    loader = importlib.machinery.ExtensionFileLoader("_calls", os.fspath(file))
-    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_calls", loader))
-    loader.exec_module(module)
     lib = capi.load()
+    loader = importlib.machinery.ExtensionFileLoader("_calls", os.fspath(file))
+    try:
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_calls", loader))
+        loader.exec_module(module)
+    except (ImportError, OSError) as e:  # (built against another torch of that version, or cut short)
+        warnings.warn(f"frisk_b200: {file.name} cannot be loaded, calls are made in Python: {e}", RuntimeWarning, stacklevel=3)
+        return
     module.library(execute._contexts, *(ctypes.cast(getattr(lib, "frisk_b200_" + name), ctypes.c_void_p).value for name in _FUNCTIONS))
     verify, change, keep, copy, adapters, write, address = module.verify, module.change, module.keep, module.copy, module.adapters, module.write, module.context
 
