@@ -100,7 +100,7 @@ struct Eight {
       const uint32_t* v = reinterpret_cast<const uint32_t*>(at);
       w[0] = make_uint4(v[0], v[1], v[2], v[3]);
     } else {
-      C v[8];
+      alignas(16) C v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = i < n ? at[i] : C(0.f);
 #pragma unroll

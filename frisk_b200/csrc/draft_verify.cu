@@ -67,7 +67,7 @@ struct Values {
   }
   // from index `at` of a row of n on: those before and behind the row are zero
   __device__ __forceinline__ void load_any(const T* row, int at, int n) {
-    T v[kLane];
+    alignas(16) T v[kLane];
 #pragma unroll
     for (int i = 0; i < kLane; ++i) v[i] = at + i >= 0 && at + i < n ? row[at + i] : T(0.f);
 #pragma unroll
@@ -125,7 +125,7 @@ __device__ __forceinline__ double warp_sum(double x) {
 
 template <typename T, bool DRAFT>
 __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams p) {
-  extern __shared__ int nodes[];  // of every node: token, parent, weight there, the draft's, random number; then masses or tokens taken off
+  extern __shared__ __align__(16) int nodes[];  // of every node: token, parent, weight there, the draft's, random number; then masses or tokens taken off
   __shared__ double part_sums[2][kMostParts], eighths[kWarps];
   __shared__ uint64_t arrived[2];  // all parts of a sum
   __shared__ uint32_t abort_word;
