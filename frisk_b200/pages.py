@@ -10,7 +10,8 @@ server is then
     lengths = cache_keep(cache, table, starts, lengths, kept, counts)                 # the accepted ones move together
 
 Tables live on the device and results follow from their contents alone, whatever the order of threads.  Results are new tensors; ``out``
-takes tensors for them, which may be the inputs (in place), so that a captured step can be replayed.  Contents are checked by the
+takes tensors for them, which may be the inputs (in place), so that a captured step can be replayed.  The three results of one call may share an
+allocation (with up to 64 KB of scratch), which lives as long as any of them: clone ``granted`` or ``lengths`` to keep it for longer than the table.  Contents are checked by the
 kernels: what is out of range is left out, and ``cache_check`` raises.
 """
 import contextlib

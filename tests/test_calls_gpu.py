@@ -187,3 +187,19 @@ def test_closed_and_new_contexts(calls):
     assert native(*native_args[:-1], ints([99, 99])) is not None
     with pytest.raises(RuntimeError, match="table"):
         F.cache_check()
+
+
+def test_what_results_keep(calls):
+    """Of a verification each its own memory; of new tables no more than the three and the scratch that the documentation names."""
+    made = arguments()
+    function, args, _, _ = made["verify"]
+    kept, counts, token = function(*args)
+    storages = [t.untyped_storage() for t in (kept, counts, token)]
+    assert len({s.data_ptr() for s in storages}) == 3
+    assert [s.nbytes() for s in storages] == [t.numel() * t.element_size() for t in (kept, counts, token)]
+    for name in ("fork", "grow", "compact"):
+        function, args, _, _ = made[name]
+        results = function(*args)
+        total = sum(-(-t.numel() * 4 // 64) * 64 for t in results)
+        assert all(t.untyped_storage().nbytes() <= total + (1 << 16) for t in results)
+        assert results[2].clone().untyped_storage().nbytes() == results[2].numel() * 4
