@@ -9,7 +9,7 @@
 // Bound by memory for the ranks of adapters: an element of x, c or out takes R multiplications (R = 64 at 6.5 TB/s: 0.2 PFLOP/s).  So the products
 // are mma.sync's, operands go from memory to registers without a stop, and no tensor memory is set up.  For a few rows the adapters
 // themselves are what is read, each by a cluster of its own; then the time is a chain: tables, x and A, two meetings of the cluster, B and c (one token, rank 16,
-// K = N = 4096: 7.4 us with the launch; 64 tokens over 40 adapters of rank 32, N 5120: 12.7, 25 MB).  Long sequences have kernels of their own (adapters_tiles.cu).
+// K = N = 4096: 7.5 us with the launch; 64 tokens over 40 adapters of rank 32, N 5120: 12.9, 25 MB).  Long sequences have kernels of their own (adapters_tiles.cu).
 //
 // Order of a product's inner index is free if both sides have the same, so a lane takes 16 bytes of it at once: of 32 neighbouring elements lane q of
 // four has 8 q .. 8 q + 7, which serve two steps of 16.  Columns of a result are permuted the same way: a lane ends up with 8 neighbours.

@@ -179,7 +179,7 @@ __device__ __forceinline__ Tile find_tile(const AdapterParams& p, int tile, int 
       if (i < warp) at += sums[i];
       before += sums[i];
     }
-    before = min(before, 1 << 30);  // (2^26 rows are at most 2^30 tiles of 16 for 256 sequences, and 2^28 of 128 for 512)
+    before = min(before, 1 << 30);  // (2^26 rows are at most 2^30 tiles of 16 for 256 sequences, and less than 2^28 of 128 for 320)
     if (tile >= at && tile < at + mine) {
       found[0] = b;
       found[1] = lo + (tile - at) * tile_rows;

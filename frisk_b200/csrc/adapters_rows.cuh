@@ -35,7 +35,7 @@ __device__ __forceinline__ uint4 load8(const uint16_t* at, int n) {
 
 // The tile of kRows rows that is number `tile`.  Where it is asked for, sequences are brought together by adapter, kThreads of them at a time: the rows of those that share
 // one lie behind one another, in the order of the sequences, and the groups in that of their first ones.  (Rows that come together read the adapter once: 99 tokens over
-// 21 adapters of rank 64, K 4096, N 7744, 32-bit results 18 us, a tile for each 46.)  Else a sequence has tiles of its own.
+// 21 adapters of rank 64, K 4096, N 7744, 32-bit results 19 us, a tile for each 46.)  Else a sequence has tiles of its own.
 struct Rows {
   int count, which;  // rows of the tile (0: there are fewer tiles), their adapter
 };
@@ -409,6 +409,8 @@ template <typename T, typename C, int RMAX, bool WIDE>
 cudaError_t launch_rows(frisk_b200_ctx* ctx, const AdapterParams& p, cudaStream_t s) {
   // Sequences that share an adapter come together where there are more tiles than run at once in the largest clusters, and fewer if they do (us, 72 tokens over 5 adapters of
   // rank 16 24 -> 13; where they all run the more clusters the better: 37 tokens over 2 adapters 14.5, brought together 17.5, and 5 of 19 rows of one adapter 7.3 and 9.1).
+  // Which adapters are named is known on the device only, so the bound on groups goes by all that are there: 256 tokens over 4 adapters of rank 64 are 17 us, of 64 adapters that are
+  // there 27, of 256, which leaves each its own tile, 53.
   const int64_t mean = (p.rows + p.batch - 1) / p.batch;  // rows of a sequence
   AdapterParams g = p;
   g.grouped = p.batch <= kMostGrouped && groups_of(p) < p.batch && p.rows < (1 << 23);  // (rows are counted in 32 bits, even if sequences out of range name some again)

@@ -9,8 +9,8 @@
 // Why not in one: the columns need all of K, and a CTA that made the sums for itself would read x as often as there are CTAs along the columns.  Why not mma.sync:
 // at R = 64 its rate is the whole time (7000 rows, K 4096, N 8192: 43 us, the floor at HBM's rate too; the kernel of adapters.cu took 330, with loads that nothing hid).
 //
-// Bound by HBM (x, c and the result once) and by a chain of barriers, MMAs and adding warps beside it: 67 us for these rows, 17 the sums (3.3 TB/s: 236 CTAs on 148 SMs, and 5
-// us of tables, meeting and terms), 45 the columns (5 TB/s; 30 without their loads and stores).
+// Bound by HBM (x, c and the result once) and by a chain of barriers, MMAs and adding warps beside it: 71 us for these rows, 17 the sums (3.3 TB/s: 236 CTAs on 148 SMs, and 5
+// us of tables, meeting and terms), 49 the columns (4.7 TB/s).
 #include <algorithm>
 
 #include "adapters.cuh"
@@ -613,8 +613,11 @@ int launch_both(frisk_b200_ctx* ctx, AdapterParams p, const Work& work, cudaStre
 }  // namespace
 
 // Long sequences, if adapters lie one behind the other (no tensor map has a step of 0).  How long is measured, K = N = 4096, 4 to 64 adapters, here and in adapters.cu, us:
-// rank 8 and 32, 16-bit results 100 sequences of 48 rows 51 and 58, 64 of 64 rows 40 and 34, 64 of 100 rows 49 and 61; 32-bit ones 128 of 32 rows 70 and 65, 64 of 64 rows 51 and 63;
-// rank 64, 64 of 24 rows 39 and 35, 128 of 32 rows 61 and 71; rank 128, 64 of 16 rows 52 and 47, of 24 rows 46 and 53, 24 of 24 rows 33 and 26 to 50.
+// rank 32, 16-bit results 100 sequences of 48 rows 56 and 67, 64 of 64 rows 44 and 38, 64 of 100 rows 53 and 67; 32-bit ones 128 of 32 rows 74 and 67, 64 of 64 rows 55 and 65;
+// rank 64, 64 of 24 rows 43 and 41, 128 of 32 rows 67 and 80; rank 128, 64 of 16 rows 58 and 49, of 24 rows 53 and 63, 24 of 24 rows 39 and 27 to 60.
+// No border of the mean is right everywhere (the first pair is on the wrong side of it), and one long sequence beside many short ones is taken whole by either kernel: lengths are
+// known on the device only.  2000 rows and 60 tokens, rank 32 and 64: 33 and 51, in two calls 20 + 11 and 22 + 12; 4096 rows and 255 tokens, rank 64 and 128: 82 and 119,
+// in two calls 33 + 19 and 56 + 24.
 size_t adapter_tiles_workspace_bytes(const frisk_b200_adapter_desc& d) {
   const int64_t longest = d.rank > 64 ? 20 : d.rank > 32 ? 28 : d.dtype_c == FRISK_B200_F32 ? 40 : 64;  // mean rows that adapters.cu takes
   if (d.batch < 1 || d.rows < 512 || d.rows <= longest * d.batch || d.count < 1) return 0;

@@ -13,7 +13,8 @@
 //          no store meets a row that is still to be read
 //
 // Bound by HBM where pages are copied (1400 pages of 256 KB: 128 us, 5.7 TB/s read and written; 2000 of 9000 pages of 33 KB moved together: 31 us, 22 of them
-// the copy at 6.1 TB/s, the rest the plan), else by launches and chains of dependent loads (fork of 16 rows 4.5 us, plan of grow for 16 sequences 8.7, for 192 10.9).
+// the copy at 6.1 TB/s, the rest the plan), else by launches and chains of dependent loads (fork of 16 rows 4.5 us; grow of 16 sequences 8.8 with its
+// copies, of 192 14.6).
 #include <algorithm>
 
 #include "cache_common.cuh"

@@ -427,7 +427,7 @@ int frisk_b200_draft_verify(frisk_b200_ctx* ctx, const frisk_b200_verify_desc* d
  * out[r] = c[r] + scales[w] * (x[r] . a[w]^T) . b[w]^T for the packed rows r of sequence s, w = adapters[s] (below 0: none, out[r] = c[r]).
  * x [rows, K], a [count, rank, K], b [count, N, rank] of dtype (F16 or BF16), rows on 16 bytes; rank a multiple of 8 up to 128, at most 2^26 rows and N 2^28.
  * c and out [rows, N] of dtype_c (dtype or F32), any row pitch and alignment; out may be c, else overlaps nothing (x, c and out
- * may be columns of one buffer of rows).  scales: [count] floats or NULL (1).  32-bit sums, one rounding.  starts, adapters and scales are on
+ * may be columns of one buffer of rows).  scales: [count] floats or NULL (1).  32-bit sums (those between the products too), one rounding.  starts, adapters and scales are on
  * the device.  Rows of no sequence are left as they are; an adapter out of range counts as none, and frisk_b200_check returns
  * FRISK_B200_E_DEVICE_TABLE.  The workspace (16-byte aligned, contents of no matter) must not be shared by calls that may overlap. */
 typedef struct frisk_b200_adapter_desc {
