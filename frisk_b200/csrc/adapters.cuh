@@ -47,7 +47,8 @@ __device__ __forceinline__ float row_power(float most) {
 }
 // A sum's terms: all of its sign, and none of them 0, so that the three products with an infinite weight add up to the infinity that the formula has.  (Terms rounded to
 // nearest may be 0, or of the other sign: NaN.)  With w the weight of the sum's last bit, each of the first two is what fits of the rest below 2 w and w: multiples of w, exact;
-// in bf16 the third has 1 to 256 w.  fp16 terms are multiples of 2^-24, and sums below 3 2^-24 (their row's largest is 2^14) become one term; so do bf16 sums below 2^-100.
+// in bf16 the third has 1 to 256 w.  fp16 terms are multiples of 2^-24.  Of fp16 sums below 3 2^-24 (their row's largest is 2^14), and bf16 ones
+// below 2^-100, the terms are rounded to nearest.
 template <typename T>
 __device__ __forceinline__ void terms_of(float v, uint16_t (&terms)[kTerms]) {
   constexpr bool kHalf = std::is_same<T, __half>::value;
@@ -61,13 +62,12 @@ __device__ __forceinline__ void terms_of(float v, uint16_t (&terms)[kTerms]) {
   };
   // (by selection: with a branch for each, one after the other, a token took 7.9 us for 7.5)
   const bool usual = finite(v) && a >= (kHalf ? 3 * 0x1p-24f : 0x1p-100f);
-  const uint16_t one = Terms<T>::round(a), others = finite(v) ? (uint16_t)0 : one;
-  const uint16_t first = below(a - 2.f * w);
+  const uint16_t first = usual ? below(a - 2.f * w) : Terms<T>::round(a);
   const float rest = a - Terms<T>::value(first);
-  const uint16_t second = below(rest - w), third = Terms<T>::round(rest - Terms<T>::value(second));
-  terms[0] = (usual ? first : one) | sign;
-  terms[1] = (usual ? second : others) | sign;
-  terms[2] = (usual ? third : others) | sign;
+  const uint16_t second = usual ? below(rest - w) : Terms<T>::round(rest), third = Terms<T>::round(rest - Terms<T>::value(second));
+  terms[0] = first ^ sign;
+  terms[1] = (finite(v) ? second : first) ^ sign;
+  terms[2] = (finite(v) ? third : first) ^ sign;
 }
 // two neighbours as words of terms
 template <typename T>

@@ -16,6 +16,17 @@ def lists(counts, which):
 @pytest.mark.parametrize("k,n,rank", [(64, 32, 8), (200, 100, 16), (72, 65, 40), (520, 130, 64), (1000, 200, 128)])
 @pytest.mark.parametrize("dtype,wide", [("bfloat16", False), ("bfloat16", True), ("float16", False), ("float16", True)])
 def test_sums_that_cancel(counts, k, n, rank, dtype, wide):
+    cancelling(counts, k, n, rank, dtype, wide)
+
+
+@pytest.mark.parametrize("counts", [[1], [3, 0, 17, 40], [700]])
+@pytest.mark.parametrize("wide", [False, True])
+def test_small_sums_that_cancel(counts, wide):
+    """The same near the lower end of the range: sums of 2^-101, and weights that bring them back."""
+    cancelling(counts, 200, 100, 16, "bfloat16", wide, 2.0 ** -116)
+
+
+def cancelling(counts, k, n, rank, dtype, wide, size=1.0):
     """Sums of 24 bits, p 2^8 + q + u 2^-8 with p, q, u of 8 bits, of which a column takes the difference of two that are less than 2^-1 apart: exact in sums of 32 bits,
     in whatever order (every partial sum is a multiple of 2^-8 below 2^16), and so is the result in any type."""
     import torch
@@ -24,7 +35,7 @@ def test_sums_that_cancel(counts, k, n, rank, dtype, wide):
     g = torch.Generator().manual_seed(rows + k)
     a, x = torch.zeros(3, rank, k), torch.zeros(rows, k)
     at = torch.randperm(k, generator=g)[:3]
-    x[:, at] = torch.tensor([256.0, 1.0, 2.0 ** -8])
+    x[:, at] = torch.tensor([256.0, 1.0, 2.0 ** -8]) * size
     a[:, ::2, at] = torch.randint(0, 256, (3, rank // 2, 3), generator=g).float()
     a[:, ::2, at[0]] = torch.randint(128, 256, (3, rank // 2), generator=g).float()
     a[:, ::2, at[2]] = torch.randint(64, 128, (3, rank // 2), generator=g).float()
@@ -34,6 +45,7 @@ def test_sums_that_cancel(counts, k, n, rank, dtype, wide):
     b = torch.zeros(3, n, rank)
     b.scatter_(2, (2 * pair)[..., None], sign[..., None]).scatter_(2, (2 * pair + 1)[..., None], -sign[..., None])
     x[::2] = -x[::2]
+    b /= size
     c = torch.randint(-1, 2, (rows, n), generator=g).float() / 256
     which = [i % 3 for i in range(len(counts))]
     starts, adapters = lists(counts, which)
