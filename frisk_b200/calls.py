@@ -50,11 +50,12 @@ def _load():
     try:
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_calls", loader))
         loader.exec_module(module)
-    except (ImportError, OSError) as e:  # (built against another torch of that version, or cut short)
+        made = module.verify, module.change, module.keep, module.copy, module.adapters, module.write, module.context
+        module.library(execute._contexts, *(ctypes.cast(getattr(lib, "frisk_b200_" + name), ctypes.c_void_p).value for name in _FUNCTIONS))
+    except (ImportError, OSError, AttributeError, TypeError, ValueError) as e:  # (built against another torch of that version, from another source, or cut short)
         warnings.warn(f"frisk_b200: {file.name} cannot be loaded, calls are made in Python: {e}", RuntimeWarning, stacklevel=3)
         return
-    module.library(execute._contexts, *(ctypes.cast(getattr(lib, "frisk_b200_" + name), ctypes.c_void_p).value for name in _FUNCTIONS))
-    verify, change, keep, copy, adapters, write, address = module.verify, module.change, module.keep, module.copy, module.adapters, module.write, module.context
+    verify, change, keep, copy, adapters, write, address = made
 
 
 def result(r, device):

@@ -88,3 +88,15 @@ def test_an_extension_of_another_source_does_not_stay(monkeypatch, tmp_path):
     os.utime(file, (later, later))
     assert build.build_calls() == file and file.exists()
     assert build.build_calls(force=True) is None and not file.exists()
+
+
+def test_an_extension_of_another_source(unloaded, monkeypatch):
+    """One that takes other functions than this package has."""
+    if not calls.path(torch.__version__).exists():
+        pytest.skip("built without native calls")
+    context = object()
+    monkeypatch.setattr(calls, "_FUNCTIONS", calls._FUNCTIONS[:-1])
+    monkeypatch.setitem(calls.execute._contexts, 5, context)
+    with pytest.warns(RuntimeWarning, match="cannot be loaded"):
+        assert calls.context_for(5) is context
+    assert all(getattr(calls, name) is calls._unknown for name in FUNCTIONS)
