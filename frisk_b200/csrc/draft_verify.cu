@@ -20,7 +20,7 @@
 //
 // Bound by HBM where there are many sequences (64 chains of 6 tokens over 128000 fp32 values: 21 us, 49 MB read), else by the chain starts -> tokens ->
 // values -> row -> sums -> row (one chain over 32000: 6 us with the launch) and, where much is rejected, by conversions to and products in 64 bits (16
-// trees of 24 over 50001 bf16 values: 21 to 29 us, some 3 a rejected child).  Weights are not kept: the j-th child of one node that is rejected takes j products and differences of every
+// trees of 24 over 50001 bf16 values: 19 to 29 us, some 3 a rejected child).  Weights are not kept: the j-th child of one node that is rejected takes j products and differences of every
 // entry of the row, so m of them take some m^2 / 2 (16 such nodes over 50001: 2 children 13 us, 8 58, 32 535, 128 7400; without a draft they take none).
 #include <cfloat>
 
